@@ -8,6 +8,7 @@ PoolLogicLayer).  All numerics run in libcompactlogic_hip.so, built in-tree by
 ``python -m compactlogic_amd.build``.
 """
 from . import checkpoint, circuit, convlogic_hip, difflogic_hip
+from .dropout_layer import Dropout, DropoutFunction, dropout
 from .layers import (ConvLayer, ConvLayerCudaFunction, ConvLayerSoftmaxFunction,
                      ConvLayerWindowFunction, GroupSum, GroupSumCrossEntropyFunction,
                      GroupSumFunction, LogicGroupSumCrossEntropyFunction, LogicLayer,
@@ -16,6 +17,8 @@ from .layers import (ConvLayer, ConvLayerCudaFunction, ConvLayerSoftmaxFunction,
 from .optim import FusedAdam
 from .packed_net import PackedNetwork
 from .plan import RunPlan, build_run_plan
+from .policy import (PolicyLossFunction, PreferenceLossFunction, SelectedLogProbsFunction,
+                     policy_loss, preference_loss, selected_log_probs)
 from .schedules import (EntropyRowResampler, FixedSequentialEntropyFreezer,
                         SequentialEntropyFreezer)
 from .treelogic import (ConvLogicFunction, ConvLogicLayer, FullConvLogicFunction,
@@ -29,5 +32,7 @@ __all__ = [
     "EntropyRowResampler", "PackedNetwork", "ConvLogicLayer", "TreeLogicLayer", "PoolLogicLayer",
     "ConvLogicFunction", "FullConvLogicFunction", "TreeLogicFunction", "FusedAdam",
     "LogicGroupSumCrossEntropyFunction", "logic_group_sum_cross_entropy",
-    "sequential_cross_entropy", "checkpoint", "circuit",
+    "sequential_cross_entropy", "checkpoint", "circuit", "Dropout", "DropoutFunction", "dropout",
+    "PolicyLossFunction", "PreferenceLossFunction", "SelectedLogProbsFunction", "policy_loss",
+    "preference_loss", "selected_log_probs",
 ]

@@ -19,6 +19,9 @@ CL_ERR_HIP = 3
 CL_DTYPE_F32 = 0
 CL_DTYPE_F64 = 1
 CL_DTYPE_F16 = 2
+CL_DTYPE_BF16 = 3
+
+CL_REDUCE = {"none": 0, "sum": 1, "mean": 2}
 
 ABI_VERSION = 1
 
@@ -128,6 +131,18 @@ SIGNATURES: dict[str, list] = {
     "cl_adam_clip_workspace": [_i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64)],
     "cl_adam_clip_step": [_int, _i64, _p, _p, _p, _p, ctypes.POINTER(_i64), _p, _f64, _f64,
                           _f64, _f64, _f64, _p, _i64, _p],
+    "cl_selected_log_prob_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
+    "cl_selected_log_prob_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
+    "cl_policy_loss_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _f64, _f64, _f64,
+                               _int, _p, _p, _p, _p, _p, _p],
+    "cl_policy_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _int, _p, _p, _p, _p],
+    "cl_preference_loss_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _f64, _f64,
+                                   _int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+    "cl_preference_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _int, _p, _p,
+                                    _p, _p],
+    "cl_dropout": [_int, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _int, _f64, _u64, _u64,
+                   _p, _p],
+    "cl_dropout_next": [_p, _p, _p],
     "cl_group_sum_cross_entropy_forward_noalloc": [_int, _p, _i64, _i64, _i64, _i64, _i64, _f64,
                                                    _p, _i64, _p, _p, _p, _p, _p],
     "cl_pack_bits": [_p, _i64, _i64, _i32, _p, ctypes.POINTER(_i64), _p],

@@ -32,6 +32,7 @@ import torch
 
 from . import _capi
 from . import difflogic_hip as _dl
+from .dropout_layer import Dropout
 from .layers import ConvLayer, GroupSum, LogicLayer, PackBitsTensor
 
 GATE_NAMES = ("CONST0", "AND", "A_AND_NOT_B", "A", "NOT_A_AND_B", "B", "XOR", "OR", "NOR",
@@ -87,15 +88,16 @@ class Circuit:
 
 
 def extract_circuit(model) -> Circuit:
-    """The circuit of `model` (LogicLayer / ConvLayer modules, Flatten, a final GroupSum) at
+    """The circuit of `model` (LogicLayer / ConvLayer modules, Flatten, Dropout, a final GroupSum) at
     its winner slots: `w` for a frozen layer, else the argmax of its logits (compiler/
     extract.py:47-197)."""
-    mods = [m for m in model if not isinstance(m, torch.nn.Flatten)]
+    mods = [m for m in model if not isinstance(m, (torch.nn.Flatten, Dropout))]
     if not mods or not isinstance(mods[-1], GroupSum):
         raise ValueError("the network must end with a GroupSum")
     layers = mods[:-1]
     if not layers or not all(isinstance(m, LogicLayer) for m in layers):
-        raise ValueError("the circuit takes LogicLayer / ConvLayer modules, Flatten and GroupSum")
+        raise ValueError("the circuit takes LogicLayer / ConvLayer modules, Flatten, Dropout "
+                         "and GroupSum")
     def features_in(m):
         # a ConvLayer's in_dim counts its padded plane; its inputs are the unpadded features
         return int(np.prod(m.in_shape)) if isinstance(m, ConvLayer) else int(m.in_dim)

@@ -53,6 +53,19 @@ def dense_dtype_code(t: torch.Tensor) -> int:
                            "float16, float32 and float64") from None
 
 
+_STORAGE_DTYPES = {**_DTYPES, torch.float16: _capi.CL_DTYPE_F16,
+                   torch.bfloat16: _capi.CL_DTYPE_BF16}
+
+
+def storage_dtype_code(t: torch.Tensor) -> int:
+    """dtype code for the operators that also take 16-bit tensors (sums in fp32)."""
+    try:
+        return _STORAGE_DTYPES[t.dtype]
+    except KeyError:
+        raise RuntimeError(f"unsupported floating dtype {t.dtype}; the kernels take float16, "
+                           "bfloat16, float32 and float64") from None
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

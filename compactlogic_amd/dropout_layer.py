@@ -1,0 +1,132 @@
+"""Dropout between logic layers on the HIP kernels (cl_dropout).  No counterpart in the reference.
+
+The mask is not stored: it is a function of a seed, an offset and the element's place, Philox
+4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC'11) with
+the seed as its key and (column / 8, row, offset) as its counter, sixteen bits an element.  The
+backward makes it again, a later evaluation of the same batch can ask for the same mask (a policy
+and the one it is compared with), and it does not depend on how the tensor lies in memory.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _capi
+from . import difflogic_hip as _dl
+from . import timing
+from .layers import PackBitsTensor
+
+
+def _apply(x, threshold, rescale, fill, seed, offset, rng):
+    """cl_dropout of a 2-D tensor, the result lying as the tensor does."""
+    rows, cols = x.shape
+    if (x.stride(1) == 1 or cols == 1) and x.stride(0) >= 0:
+        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    elif (x.stride(0) == 1 or rows == 1) and x.stride(1) >= 0:
+        y = torch.empty((cols, rows), dtype=x.dtype, device=x.device).t()
+    else:
+        x = x.contiguous()
+        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    with _dl.on_device_of(x):
+        timing.timed("cl_dropout", lambda: _capi.call(
+            "cl_dropout", _dl.storage_dtype_code(x), x.data_ptr(), x.stride(0), x.stride(1),
+            y.data_ptr(), y.stride(0), y.stride(1), rows, cols, threshold, int(rescale),
+            float(fill), seed, offset, _dl.ptr(rng), _dl.stream_of(x)))
+    return y
+
+
+class DropoutFunction(torch.autograd.Function):
+    """Dropout of a 2-D tensor; the gradient passes the same mask, made again from the seed (and is
+    itself a dropout, so it can be differentiated as often as one likes)."""
+
+    @staticmethod
+    def forward(ctx, x, threshold, fill, seed, offset, rng):
+        ctx.save_for_backward(rng)
+        ctx.args = threshold, fill is None, seed, offset
+        return _apply(x, threshold, fill is None, 0.0 if fill is None else fill, seed, offset, rng)
+
+    @staticmethod
+    def backward(ctx, grad):
+        threshold, rescale, seed, offset = ctx.args
+        (rng,) = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            grad = DropoutFunction.apply(grad, threshold, None if rescale else 0.0, seed, offset,
+                                         rng)
+        else:
+            grad = _apply(grad, threshold, rescale, 0.0, seed, offset, rng)
+        return (grad,) + (None,) * 5
+
+
+def _threshold(p) -> int:
+    if not 0 <= p <= 1:
+        raise ValueError(f"dropout probability must be in [0, 1], got {p}")
+    return int(round(65536 * float(p)))
+
+
+def dropout(x, p: float, seed, offset: int = 0, fill: float | None = None):
+    """Each element of x dropped with probability p, taken to the nearest multiple of 2^-16.
+
+    fill=None: dropped elements become 0 and the others are divided by the probability of
+    keeping them (the one that was taken), so that the mean stays; a number: dropped elements
+    become that number and the others stay as they are (0.5, a bit that is not known, keeps a
+    relaxed activation in [0, 1]).
+
+    seed, offset: integers, or seed an int64 tensor (seed, offset) on x's device, read when the
+    kernel runs (so a captured graph follows it).  Equal ones give equal masks; the last
+    dimension is the column, those before it together the row.  Where nothing can be dropped
+    (p below 2^-17) x itself is returned."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a tensor")
+    if x.device.type != "cuda":
+        raise RuntimeError("dropout needs a HIP device tensor")
+    _dl.storage_dtype_code(x)
+    threshold = _threshold(p)
+    rng = None
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.shape != (2,) or seed.device != x.device:
+            raise RuntimeError(f"seed must be an integer or an int64 tensor (seed, offset) on "
+                               f"{x.device}")
+        if offset != 0:
+            raise ValueError("offset is part of a seed tensor")
+        rng, seed = seed.contiguous(), 0
+    if threshold == 0 or x.numel() == 0:
+        return x
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1] if x.dim() else 1)
+    y = DropoutFunction.apply(flat, threshold, None if fill is None else float(fill),
+                              int(seed) & (2**64 - 1), int(offset) & (2**64 - 1), rng)
+    return y if x.dim() == 2 else y.reshape(x.shape)
+
+
+class Dropout(torch.nn.Module):
+    """`dropout` as a module, between the layers of a Sequential: in training every call draws the
+    next mask (its buffer `rng` holds the seed and the count of calls, on the device, so a
+    captured training step draws a new mask at every replay and a checkpoint resumes the
+    sequence); in eval mode, and for a PackBitsTensor, the identity.  seed=None takes one from
+    torch's generator."""
+
+    def __init__(self, p: float = 0.5, fill: float | None = None, seed: int | None = None):
+        super().__init__()
+        _threshold(p)
+        self.p = p
+        self.fill = fill
+        if seed is None:
+            seed = int(torch.randint(0, 2**63 - 1, (), device="cpu"))
+        if not -2**63 <= seed < 2**63:
+            raise ValueError("seed must fit in 64 bits")
+        self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
+
+    def next_rng(self) -> torch.Tensor:
+        """The (seed, offset) of the next mask, as `dropout` takes it; advances the module."""
+        _dl._check(self.rng, "rng")
+        used = torch.empty_like(self.rng)
+        with _dl.on_device_of(used):
+            _capi.call("cl_dropout_next", self.rng.data_ptr(), used.data_ptr(),
+                       _dl.stream_of(used))
+        return used
+
+    def forward(self, x):
+        if not self.training or isinstance(x, PackBitsTensor) or _threshold(self.p) == 0:
+            return x
+        return dropout(x, self.p, self.next_rng(), fill=self.fill)
+
+    def extra_repr(self):
+        return f"p={self.p}, fill={self.fill}"

@@ -18,6 +18,7 @@ import torch
 from . import _capi
 from . import convlogic_hip as _cl
 from . import difflogic_hip as _dl
+from . import policy as _policy
 from . import timing
 from .plan import PART_SLOTS, REORDER_FRACTION, RunPlan, build_run_plan, locality_order
 
@@ -1417,6 +1418,21 @@ class GroupSum(torch.nn.Module):
             loss, out = GroupSumCrossEntropyFunction.apply(x, labels, self.k, self.tau,
                                                            ignore_index)
         return (loss, out) if return_scores else loss
+
+    def log_probs(self, x, actions, ignore_index: int = -100):
+        """policy.selected_log_probs(self(x), actions): the log-probability of the chosen class of
+        every sample, differentiable by x."""
+        return _policy.selected_log_probs(self(x), actions, ignore_index)
+
+    def policy_loss(self, x, actions, old_log_probs, advantages, **options):
+        """policy.policy_loss(self(x), actions, old_log_probs, advantages, ...): the clipped policy
+        loss with a KL term of a network that chooses one of k classes."""
+        return _policy.policy_loss(self(x), actions, old_log_probs, advantages, **options)
+
+    def preference_loss(self, x, actions, offsets, **options):
+        """policy.preference_loss(self(x), actions, offsets, ...): the preference loss of paired
+        sequences of samples."""
+        return _policy.preference_loss(self(x), actions, offsets, **options)
 
     def extra_repr(self):
         return 'k={}, tau={}'.format(self.k, self.tau)

@@ -20,6 +20,7 @@ from . import timing
 from . import convlogic_hip as _cl
 from . import difflogic_hip as _dl
 from . import packed_circuit as _pc
+from .dropout_layer import Dropout
 from .layers import ConvLayer, GroupSum, LogicLayer, PackBitsTensor
 from .treelogic import ConvLogicLayer
 
@@ -295,7 +296,7 @@ class PackedNetwork:
     """
 
     def __init__(self, model, bank_aware: bool = True, prune: bool = True):
-        mods = list(model)
+        mods = [m for m in model if not isinstance(m, Dropout)]   # the identity in inference
         if not mods or not isinstance(mods[-1], GroupSum):
             raise ValueError("the network must end with a GroupSum")
         body = mods[:-1]

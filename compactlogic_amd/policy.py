@@ -1,0 +1,281 @@
+"""Training by preference and by reward on the HIP kernels: losses on the log-probability of one
+chosen class or token per row of logits, such as GroupSum's scores.
+
+The reference trains classifiers with torch's cross_entropy alone; these have no counterpart
+there.  `selected_log_probs` records what a policy (the acting one, or a frozen reference) gives
+to the chosen actions, `policy_loss` and `preference_loss` train on them; GroupSum has all three
+as methods, beside its cross_entropy.  Logits may be float32, float64, float16 or bfloat16; sums
+and softmax statistics are float32 or more, and log-probabilities, losses and what they are
+computed from are float32 (float64 for float64 logits).
+
+A row whose action is ``ignore_index`` (a prompt or padding) does not count: its log-probability
+and its gradient are 0 whatever its other inputs hold, NaN included.  Another action outside the
+logits' range gives NaN, as a label does in GroupSum.cross_entropy.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _capi
+from . import difflogic_hip as _dl
+from . import timing
+
+
+def _wide(logits: torch.Tensor) -> torch.dtype:
+    return torch.float64 if logits.dtype == torch.float64 else torch.float32
+
+
+def _flat(logits, actions):
+    """logits as [rows, cols] and actions as [rows], checked."""
+    if not isinstance(logits, torch.Tensor) or not isinstance(actions, torch.Tensor):
+        raise TypeError("logits and actions must be tensors")
+    if logits.device.type != "cuda" or actions.device != logits.device:
+        raise RuntimeError("logits and actions must be on the same HIP device")
+    _dl.storage_dtype_code(logits)
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError(f"logits must have a last dimension of at least one class, got shape "
+                           f"{tuple(logits.shape)}")
+    if actions.dtype != torch.int64 or actions.shape != logits.shape[:-1]:
+        raise RuntimeError(f"actions must be int64 of shape {tuple(logits.shape[:-1])}")
+    if logits.dim() != 2:
+        logits = logits.reshape(-1, logits.shape[-1])
+    return logits, actions.reshape(-1).contiguous()
+
+
+def _per_row(t, name, logits, actions):
+    """A constant per row as a contiguous [rows] tensor of the logits' wide type."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.device != logits.device or t.shape != actions.shape or not t.is_floating_point():
+        raise RuntimeError(f"{name} must be a floating-point tensor of shape "
+                           f"{tuple(actions.shape)} on {logits.device}")
+    if t.requires_grad:
+        raise RuntimeError(f"{name} is a constant of the loss: detach it")
+    return t.reshape(-1).to(_wide(logits)).contiguous()
+
+
+def _reduction(name):
+    if name not in _capi.CL_REDUCE:
+        raise ValueError(f"reduction must be one of {sorted(_capi.CL_REDUCE)}, got {name!r}")
+    return _capi.CL_REDUCE[name]
+
+
+def _rows_of(logits):
+    """logits as the kernels read them: contiguous rows, any distance apart."""
+    if logits.stride(1) != 1 and logits.shape[1] > 1:
+        logits = logits.contiguous()
+    return logits
+
+
+def _args(logits):
+    """The leading arguments of every entry point (an expanded row has stride 0)."""
+    return (_dl.storage_dtype_code(logits), logits.data_ptr(), logits.stride(0),
+            logits.shape[0], logits.shape[1])
+
+
+def _once():
+    """The backwards are kernels without a derivative of their own: under create_graph a second
+    derivative would silently lack its part."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the losses on chosen log-probabilities cannot be differentiated twice")
+
+
+def _state(logits):
+    return torch.empty((logits.shape[0], 4), dtype=_wide(logits), device=logits.device)
+
+
+class SelectedLogProbsFunction(torch.autograd.Function):
+    """lp[n] = log_softmax(logits[n])[actions[n]] in one pass over the logits; the backward makes
+    the probabilities again from the row's maximum and sum.  No counterpart in the reference."""
+
+    @staticmethod
+    def forward(ctx, logits, actions, ignore_index):
+        logits = _rows_of(logits)
+        state = _state(logits)
+        lp = torch.empty(logits.shape[0], dtype=state.dtype, device=logits.device)
+        with _dl.on_device_of(logits):
+            timing.timed("cl_selected_log_prob_forward", lambda: _capi.call(
+                "cl_selected_log_prob_forward", *_args(logits), actions.data_ptr(), ignore_index,
+                lp.data_ptr(), state.data_ptr(), _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, state)
+        return lp
+
+    @staticmethod
+    def backward(ctx, grad_lp):
+        _once()
+        logits, actions, state = ctx.saved_tensors
+        grad_lp = grad_lp.contiguous()
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        with _dl.on_device_of(logits):
+            timing.timed("cl_selected_log_prob_backward", lambda: _capi.call(
+                "cl_selected_log_prob_backward", *_args(logits), actions.data_ptr(),
+                state.data_ptr(), grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits)))
+        return grad, None, None
+
+
+class PolicyLossFunction(torch.autograd.Function):
+    """The clipped policy loss with a KL term (cl_policy_loss_forward / _backward).  Returns (loss,
+    log_probs); the log-probabilities are not differentiable through this function.  No
+    counterpart in the reference."""
+
+    @staticmethod
+    def forward(ctx, logits, actions, old, adv, ref, clip_low, clip_high, kl_coef, ignore_index,
+                reduction):
+        logits = _rows_of(logits)
+        state = _state(logits)
+        rows, dev, wide = logits.shape[0], logits.device, state.dtype
+        lp = torch.empty(rows, dtype=wide, device=dev)
+        terms = torch.empty(rows, dtype=wide, device=dev)
+        scalars = torch.empty(2, dtype=wide, device=dev) if reduction else None
+        loss, count = scalars.unbind() if reduction else (None, None)
+        with _dl.on_device_of(logits):
+            timing.timed("cl_policy_loss_forward", lambda: _capi.call(
+                "cl_policy_loss_forward", *_args(logits), actions.data_ptr(), ignore_index,
+                old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
+                reduction, lp.data_ptr(), state.data_ptr(), terms.data_ptr(), _dl.ptr(loss),
+                _dl.ptr(count), _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, state, count)
+        ctx.reduction = reduction
+        ctx.mark_non_differentiable(lp)
+        ctx.set_materialize_grads(False)
+        return (loss if reduction else terms), lp
+
+    @staticmethod
+    def backward(ctx, grad_loss, _grad_lp):
+        _once()
+        if grad_loss is None:
+            return (None,) * 10
+        logits, actions, state, count = ctx.saved_tensors
+        grad_loss = grad_loss.contiguous()
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        with _dl.on_device_of(logits):
+            timing.timed("cl_policy_loss_backward", lambda: _capi.call(
+                "cl_policy_loss_backward", *_args(logits), actions.data_ptr(), state.data_ptr(),
+                ctx.reduction, grad_loss.data_ptr(), _dl.ptr(count), grad.data_ptr(),
+                _dl.stream_of(logits)))
+        return (grad,) + (None,) * 9
+
+
+class PreferenceLossFunction(torch.autograd.Function):
+    """The preference loss of paired sequences (cl_preference_loss_forward / _backward).  Returns
+    (loss, margins); the margins are not differentiable through this function.  No counterpart in
+    the reference."""
+
+    @staticmethod
+    def forward(ctx, logits, actions, offsets, ref, beta, smoothing, ignore_index, reduction):
+        logits = _rows_of(logits)
+        state = _state(logits)
+        rows, dev, wide = logits.shape[0], logits.device, state.dtype
+        pairs = (offsets.numel() - 1) // 2
+        lp = torch.empty(rows, dtype=wide, device=dev)
+        gaps = torch.empty(rows, dtype=torch.float64, device=dev)
+        row_seq = torch.empty(rows, dtype=torch.int32, device=dev)
+        seq_slope = torch.empty(2 * pairs, dtype=wide, device=dev)
+        margins = torch.empty(pairs, dtype=wide, device=dev)
+        terms = torch.empty(pairs, dtype=wide, device=dev)
+        scalars = torch.empty(2, dtype=wide, device=dev) if reduction else None
+        loss, count = scalars.unbind() if reduction else (None, None)
+        with _dl.on_device_of(logits):
+            timing.timed("cl_preference_loss_forward", lambda: _capi.call(
+                "cl_preference_loss_forward", *_args(logits), actions.data_ptr(), ignore_index,
+                _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction,
+                lp.data_ptr(), state.data_ptr(), gaps.data_ptr(), row_seq.data_ptr(),
+                seq_slope.data_ptr(), margins.data_ptr(), terms.data_ptr(), _dl.ptr(loss),
+                _dl.ptr(count), _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, state, row_seq, seq_slope, count)
+        ctx.reduction, ctx.pairs = reduction, pairs
+        ctx.mark_non_differentiable(margins)
+        ctx.set_materialize_grads(False)
+        return (loss if reduction else terms), margins
+
+    @staticmethod
+    def backward(ctx, grad_loss, _grad_margins):
+        _once()
+        if grad_loss is None:
+            return (None,) * 8
+        logits, actions, state, row_seq, seq_slope, count = ctx.saved_tensors
+        grad_loss = grad_loss.contiguous()
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        with _dl.on_device_of(logits):
+            timing.timed("cl_preference_loss_backward", lambda: _capi.call(
+                "cl_preference_loss_backward", *_args(logits), actions.data_ptr(),
+                state.data_ptr(), row_seq.data_ptr(), seq_slope.data_ptr(), ctx.pairs,
+                ctx.reduction, grad_loss.data_ptr(), _dl.ptr(count), grad.data_ptr(),
+                _dl.stream_of(logits)))
+        return (grad,) + (None,) * 7
+
+
+def selected_log_probs(logits, actions, ignore_index: int = -100):
+    """The log-probability log_softmax(logits)[..., actions] of the chosen class or token:
+    logits [..., V], actions int64 [...] -> [...]; 0 where the action is ignore_index.
+    Differentiable by the logits."""
+    rows, acts = _flat(logits, actions)
+    return SelectedLogProbsFunction.apply(rows, acts, int(ignore_index)).reshape(actions.shape)
+
+
+def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
+                kl_coef: float = 0.0, ignore_index: int = -100, reduction: str = "mean",
+                return_log_probs: bool = False):
+    """The clipped policy loss with a KL term.  With lp the log-probability of the row's action,
+    r = exp(lp - old_log_probs) and g = ref_log_probs - lp, a row's term is::
+
+        -min(r A, clip(r, 1 - low, 1 + high) A) + kl_coef (exp(g) - g - 1)
+
+    logits [..., V]; actions, old_log_probs (the acting policy's), advantages A and ref_log_probs
+    (a frozen reference policy's, needed when kl_coef is not 0) [...].  clip: one number for both
+    sides or a pair (low, high).  reduction: 'mean' over the rows that count, 'sum', or 'none' (the
+    terms, [...]).  With return_log_probs, also the rows' log-probabilities (not differentiable
+    through this call)."""
+    rows, acts = _flat(logits, actions)
+    low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
+    low, high, kl_coef = float(low), float(high), float(kl_coef)
+    if not (low >= 0 and high >= 0):
+        raise ValueError(f"clip must not be negative, got {clip}")
+    if kl_coef != 0 and ref_log_probs is None:
+        raise ValueError("a KL term (kl_coef) needs ref_log_probs")
+    code = _reduction(reduction)
+    old = _per_row(old_log_probs, "old_log_probs", logits, actions)
+    adv = _per_row(advantages, "advantages", logits, actions)
+    ref = None
+    if ref_log_probs is not None:
+        ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
+    loss, lp = PolicyLossFunction.apply(rows, acts, old, adv, ref, low, high, kl_coef,
+                                        int(ignore_index), code)
+    if not code:
+        loss = loss.reshape(actions.shape)
+    return (loss, lp.reshape(actions.shape)) if return_log_probs else loss
+
+
+def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 0.1,
+                    label_smoothing: float = 0.0, ignore_index: int = -100,
+                    reduction: str = "mean", return_margins: bool = False):
+    """The preference loss of P pairs of sequences out of one ragged batch.  Sequence q holds the
+    rows offsets[q] .. offsets[q + 1] of logits [rows, V] and actions [rows] (offsets: int64
+    [2 P + 1], not decreasing); the first P are the chosen sequences, sequence P + i is the one
+    rejected against sequence i.  With D_q the sum of lp - ref_log_probs over a sequence's counted
+    rows (ref_log_probs: a frozen reference policy's, [rows]; None: 0) and the margin
+    h_i = beta (D_i - D_(P + i)), a pair's term is::
+
+        -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h)
+
+    reduction: 'mean' over the pairs, 'sum', or 'none' (the terms, [P]).  With return_margins, also
+    the margins [P] (not differentiable through this call).  Rows of no sequence do not count;
+    offsets that decrease or leave the rows make their pair's term NaN."""
+    rows, acts = _flat(logits, actions)
+    if logits.dim() != 2:
+        raise RuntimeError("preference_loss takes logits [rows, classes] of a ragged batch")
+    if not isinstance(offsets, torch.Tensor):
+        raise TypeError("offsets must be a tensor")
+    if offsets.device != logits.device or offsets.dtype != torch.int64 or offsets.dim() != 1 \
+            or offsets.numel() % 2 != 1:
+        raise RuntimeError(f"offsets must be int64 [2 pairs + 1] on {logits.device}")
+    if not 0 <= label_smoothing <= 1:
+        raise ValueError(f"label_smoothing must be in [0, 1], got {label_smoothing}")
+    code = _reduction(reduction)
+    ref = None
+    if ref_log_probs is not None:
+        ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
+    loss, margins = PreferenceLossFunction.apply(rows, acts, offsets.contiguous(), ref,
+                                                 float(beta), float(label_smoothing),
+                                                 int(ignore_index), code)
+    return (loss, margins) if return_margins else loss

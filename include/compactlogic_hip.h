@@ -43,6 +43,11 @@ extern "C" {
 #define CL_DTYPE_F32 0
 #define CL_DTYPE_F64 1
 #define CL_DTYPE_F16 2
+#define CL_DTYPE_BF16 3 /* the losses on chosen log-probabilities and cl_dropout */
+
+#define CL_REDUCE_NONE 0
+#define CL_REDUCE_SUM 1
+#define CL_REDUCE_MEAN 2
 
 /* ABI version of this header; bumped on any incompatible change. */
 int cl_abi_version(void);
@@ -547,6 +552,90 @@ int cl_adam_clip_step(int dtype, int64_t num_tensors, void* const* params, void*
                       void* step, double lr, double beta1, double beta2, double eps,
                       double max_norm, void* workspace, int64_t workspace_elements,
                       void* stream);
+
+/* -------------------------------------------------------------------------------------------
+ * Losses on the log-probability of one chosen class or token per row of logits (GroupSum's
+ * scores, or any other).  No counterpart in the reference.  logits: dtype F32, F64, F16 or
+ * BF16, [rows, cols] with row_stride elements between rows; actions: int64 [rows].  A row whose
+ * action is ignore_index does not count: its log-probability is 0, its gradient 0, and what its
+ * logits and other inputs hold has no effect.  Another action outside [0, cols) gives NaN.
+ * Every other float buffer has dtype wide: F64 for F64 logits, else F32.  row_state: 4 wide
+ * elements per row (16- resp. 32-byte aligned), written by a forward for its backward.
+ * grad_logits: dtype, contiguous [rows, cols].  Sums have a fixed order: bitwise repeatable.
+ * ----------------------------------------------------------------------------------------- */
+
+/* log_probs[n] = logits[n, a] - log sum_j exp(logits[n, j]), a = actions[n]. */
+int cl_selected_log_prob_forward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
+                                 int64_t cols, const int64_t* actions, int64_t ignore_index,
+                                 void* log_probs, void* row_state, void* stream);
+
+/* grad_logits[n, j] = grad_log_probs[n] * ([j == a] - softmax(logits[n])[j]). */
+int cl_selected_log_prob_backward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
+                                  int64_t cols, const int64_t* actions, const void* row_state,
+                                  const void* grad_log_probs, void* grad_logits, void* stream);
+
+/* The clipped policy loss with a KL term: with lp the row's chosen log-probability,
+ * r = exp(lp - old_log_probs[n]), A = advantages[n] and g = ref_log_probs[n] - lp,
+ *   terms[n] = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(g) - g - 1);
+ * loss: their sum (CL_REDUCE_SUM) or its mean over the counted rows (CL_REDUCE_MEAN; NaN when
+ * none counts); neither loss nor count is written for CL_REDUCE_NONE.  ref_log_probs may be
+ * NULL when kl_coef is 0. */
+int cl_policy_loss_forward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
+                           int64_t cols, const int64_t* actions, int64_t ignore_index,
+                           const void* old_log_probs, const void* advantages,
+                           const void* ref_log_probs, double clip_low, double clip_high,
+                           double kl_coef, int reduction, void* log_probs, void* row_state,
+                           void* terms, void* loss, void* count, void* stream);
+
+/* Its logits' gradient.  grad_loss: a device scalar, or [rows] for CL_REDUCE_NONE.  Where the
+ * clipped product is the smaller one and r lies outside the range, only the KL term has a
+ * gradient. */
+int cl_policy_loss_backward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
+                            int64_t cols, const int64_t* actions, const void* row_state,
+                            int reduction, const void* grad_loss, const void* count,
+                            void* grad_logits, void* stream);
+
+/* The preference loss of pairs of sequences: sequence q holds rows offsets[q] .. offsets[q + 1]
+ * (int64 [2 pairs + 1], not decreasing, within [0, rows]); q < pairs is the chosen sequence of
+ * pair q, pairs + q its rejected one.  With D_q the sum over a sequence's counted rows of
+ * lp - ref_log_probs (NULL: 0) and h = beta (D_i - D_(pairs + i)) = margins[i],
+ *   terms[i] = -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h);
+ * loss: their sum or mean over the pairs.  A pair whose offsets decrease or leave [0, rows] gets
+ * NaN.  Rows of no sequence do not count.  gaps: double [rows], row_seq: int32 [rows],
+ * seq_slope: wide [2 pairs]; written for the backward. */
+int cl_preference_loss_forward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
+                               int64_t cols, const int64_t* actions, int64_t ignore_index,
+                               const void* ref_log_probs, const int64_t* offsets, int64_t pairs,
+                               double beta, double label_smoothing, int reduction,
+                               void* log_probs, void* row_state, double* gaps, int32_t* row_seq,
+                               void* seq_slope, void* margins, void* terms, void* loss,
+                               void* count, void* stream);
+
+/* Its logits' gradient.  grad_loss: a device scalar, or [pairs] for CL_REDUCE_NONE. */
+int cl_preference_loss_backward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
+                                int64_t cols, const int64_t* actions, const void* row_state,
+                                const int32_t* row_seq, const void* seq_slope, int64_t pairs,
+                                int reduction, const void* grad_loss, const void* count,
+                                void* grad_logits, void* stream);
+
+/* -------------------------------------------------------------------------------------------
+ * Dropout whose mask is a function of (seed, offset, row, column) and is not stored (no
+ * counterpart in the reference).  Philox 4x32-10 (Salmon et al., SC'11) with key seed and
+ * counter (column / 8, row, offset): its words are eight 16-bit halves, low half first, and
+ * element (row, column) is dropped where half number column % 8 is below threshold (0..65536).
+ * y = fill where dropped, else x, times 65536 / (65536 - threshold) with rescale.  The gradient
+ * is the same call on the gradient with fill 0.  dtype: F32, F64, F16 or BF16.  x and y
+ * [rows, cols] (both below 2^32) are contiguous along the same dimension; they may be the same
+ * memory.  rng: int64 (seed, offset) on the device, or NULL for the two arguments before it.
+ * ----------------------------------------------------------------------------------------- */
+int cl_dropout(int dtype, const void* x, int64_t x_stride_row, int64_t x_stride_col, void* y,
+               int64_t y_stride_row, int64_t y_stride_col, int64_t rows, int64_t cols,
+               int64_t threshold, int rescale, double fill, uint64_t seed, uint64_t offset,
+               const int64_t* rng, void* stream);
+
+/* used = rng; rng's offset + 1: the state of one call, taken on the device so that a captured
+ * graph draws a new mask at every replay. */
+int cl_dropout_next(int64_t* rng, int64_t* used, void* stream);
 
 /* -------------------------------------------------------------------------------------------
  * Layout change: dst [cols, rows] = transpose of src [rows, cols] (both contiguous, not

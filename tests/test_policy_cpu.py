@@ -1,0 +1,89 @@
+"""What the losses on chosen log-probabilities refuse without a device, and their oracle against
+differences."""
+import numpy as np
+import pytest
+import torch
+
+import compactlogic_amd as cl
+from compactlogic_amd import _capi
+from oracle import policy_np as P
+
+
+def test_refusals_without_a_device():
+    z, a, f = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64), torch.zeros(3)
+    off = torch.tensor([0, 1, 2])
+    for call in (lambda: cl.selected_log_probs(z, a), lambda: cl.policy_loss(z, a, f, f),
+                 lambda: cl.preference_loss(z, a, off),
+                 lambda: cl.GroupSum(5).log_probs(z, a)):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call()
+    with pytest.raises(TypeError):
+        cl.selected_log_probs([1.0], a)
+
+
+def test_c_arguments_are_checked_before_the_device():
+    lib = _capi.load()
+    ok, bad = _capi.CL_OK, _capi.CL_ERR_INVALID_ARGUMENT
+
+    def lp(dtype=0, x=1, stride=8, rows=2, cols=8, act=1, out=1, state=1):
+        return lib.cl_selected_log_prob_forward(dtype, x, stride, rows, cols, act, -100, out, state,
+                                                None)
+
+    def policy(low=0.2, kl=0.0, ref=None, red=2, loss=1, old=1, rows=2):
+        return lib.cl_policy_loss_forward(0, 1, 8, rows, 8, 1, -100, old, 1, ref, low, 0.2, kl, red,
+                                          1, 1, 1, loss, loss, None)
+
+    def pref(pairs=1, smooth=0.0, off=1, red=2, gaps=1):
+        return lib.cl_preference_loss_forward(0, 1, 8, 2, 8, 1, -100, None, off, pairs, 0.1, smooth,
+                                              red, 1, 1, gaps, 1, 1, 1, 1, 1, 1, None)
+
+    assert lp(rows=0, x=None, act=None, out=None, state=None) == ok
+    assert lp(cols=0) == bad and lp(cols=2**31) == bad and lp(rows=-1) == bad
+    assert lp(rows=2**31) == bad and lp(stride=-1) == bad and lp(dtype=7) == bad
+    assert lp(x=None) == bad and lp(act=None) == bad and lp(out=None) == bad
+    assert lp(state=None) == bad
+    assert policy(low=-0.1) == bad and policy(low=float("nan")) == bad
+    assert policy(kl=0.1) == bad and b"KL" in lib.cl_last_error()
+    assert policy(red=3) == bad and policy(loss=None) == bad and policy(old=None) == bad
+    assert pref(pairs=-1) == bad and pref(smooth=1.5) == bad and pref(off=None) == bad
+    assert pref(red=-1) == bad and pref(gaps=None) == bad
+    assert lib.cl_selected_log_prob_backward(0, 1, 8, 2, 8, 1, 1, None, 1, None) == bad
+    assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 2, 1, None, 1, None) == bad
+    assert lib.cl_preference_loss_backward(0, 1, 8, 2, 8, 1, 1, None, 1, 1, 2, 1, 1, 1, None) == bad
+
+
+def _difference(f, z, eps=1e-6):
+    g = np.zeros(z.shape)
+    for i in np.ndindex(*z.shape):
+        hi, lo = z.copy(), z.copy()
+        hi[i] += eps
+        lo[i] -= eps
+        g[i] = (f(hi) - f(lo)) / (2 * eps)
+    return g
+
+
+def test_oracle_gradients_against_differences():
+    """Central differences at 1e-6: truncation about 1e-12, cancellation about 1e-16 / 1e-6."""
+    rng = np.random.default_rng(0)
+    z, actions = rng.standard_normal((6, 5)), np.array([0, 4, -100, 2, 1, 3])
+    lp, probs = P.log_probs(z, actions)
+    # ratios well inside and outside the clipped range
+    old = lp - np.log([0.5, 0.95, 1.0, 1.1, 1.6, 1.05])
+    adv, ref = rng.standard_normal(6), lp + 0.3 * rng.standard_normal(6)
+
+    def policy(zz):
+        return P.policy_terms(P.log_probs(zz, actions)[0], actions, old, adv, ref, 0.2, 0.28,
+                              0.05)[0].sum()
+
+    slope = P.policy_terms(lp, actions, old, adv, ref, 0.2, 0.28, 0.05)[1]
+    np.testing.assert_allclose(P.logit_gradient(probs, actions, slope), _difference(policy, z),
+                               atol=1e-8)
+    offsets = [0, 2, 4, 5, 6]
+
+    def preference(zz):
+        return P.preference_terms(P.log_probs(zz, actions)[0], actions, offsets, ref, 0.7,
+                                  0.1)[1].sum()
+
+    slope = P.preference_terms(lp, actions, offsets, ref, 0.7, 0.1)[2]
+    np.testing.assert_allclose(P.logit_gradient(probs, actions, slope), _difference(preference, z),
+                               atol=1e-8)

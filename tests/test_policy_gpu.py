@@ -1,0 +1,579 @@
+"""Losses on chosen log-probabilities against the float64 oracle: values and gradients over types,
+lengths, strides, masks, ragged sequences; graphs, streams, refusals."""
+import numpy as np
+import pytest
+import torch
+
+import compactlogic_amd as cl
+from oracle import policy_np as P
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float64, torch.float16, torch.bfloat16]
+IGNORE = -100
+
+
+def _unit(dtype):
+    return 2.0**-53 if dtype == torch.float64 else 2.0**-24
+
+
+def _sum_error(z, dtype):
+    """Relative error of a row's sum of exponentials, and so the absolute one of lp: no chain of
+    additions is longer than V / 256 + 32 (each rounds by a unit), an exponential is off by two
+    units in the last place and by its argument's rounding, which weighs |x - m| exp(x - m) <= 1
+    per term against a sum of at least 1, at most |x - m| <= spread of the finite logits."""
+    fin = np.where(np.isfinite(z) & (np.abs(z) < 1e30), z, np.nan)
+    spread = np.nanmax(fin) - np.nanmin(fin) if np.isfinite(fin).any() else 0.0
+    return (z.shape[1] / 256 + 40 + min(spread, 100.0)) * _unit(dtype)
+
+
+def _near(got, ref, err, dtype, half=None):
+    """|got - ref| <= err + the rounding to `dtype` (half a step, and a subnormal's)."""
+    got, ref = np.asarray(got, dtype=np.float64), np.asarray(ref, dtype=np.float64)
+    info = torch.finfo(dtype)
+    step = np.abs(ref) * (info.eps / 2) * 1.01 + info.smallest_normal * info.eps
+    same = (got == ref) | (np.isnan(got) & np.isnan(ref))
+    with np.errstate(invalid="ignore"):
+        bad = ~(same | (np.abs(got - ref) <= err + step))
+    assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], ref[bad][:5], np.max(err))
+
+
+def _np(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _wide(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+class Case:
+    """Rows of logits and what the losses need beside them; ratios away from the borders of the
+    clipped range (0.8, 1.28), so that rounding cannot change a row's side."""
+
+    def __init__(self, rows, vocab, dtype, device, seed=0, scale=2.5, ignored=0.2):
+        rng = np.random.default_rng(seed + 1000 * rows + vocab)
+        z = torch.as_tensor(rng.standard_normal((rows, vocab)) * scale).to(dtype)
+        self.dtype, self.wide = dtype, _wide(dtype)
+        self.logits = z.to(device)
+        self.z = _np(z)
+        self.actions = rng.integers(0, vocab, rows)
+        if rows > 2:
+            self.actions[rng.random(rows) < ignored] = IGNORE
+            self.actions[0] = vocab - 1
+        self.lp, self.probs = P.log_probs(self.z, self.actions)
+        ratio = rng.choice([0.4, 0.9, 1.0, 1.15, 1.7], rows)
+
+        def wide(v):
+            t = torch.as_tensor(v).to(self.wide)
+            return t.to(device), _np(t)
+
+        self.old_t, self.old = wide(self.lp - np.log(ratio))
+        self.ref_t, self.ref = wide(self.lp + 0.3 * rng.standard_normal(rows))
+        self.adv_t, self.adv = wide(rng.standard_normal(rows))
+        self.act_t = torch.as_tensor(self.actions).to(device)
+        self.err = _sum_error(self.z, dtype)
+
+    def check_gradient(self, grad, slope, slope_err=0.0):
+        """|[j = a] - p_j| <= 1: errors of the slope and of the probabilities pass as they are."""
+        ref = P.logit_gradient(self.probs, self.actions, slope)
+        err = (np.abs(slope) * 2 * self.err + slope_err)[:, None]
+        assert grad.dtype == self.dtype
+        _near(_np(grad), ref, np.where(np.isfinite(err), err, 0.0), self.dtype)
+
+
+SIZES = [(1, 1), (1, 2), (3, 5), (128, 10), (33, 64), (9, 129), (5, 513), (7, 1000), (3, 2049),
+         (4, 4099), (3, 8193), (2, 16385), (2, 33001), (3, 66000), (2, 131073), (1, 262147)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs(device, dtype):
+    for rows, vocab in SIZES:
+        c = Case(rows, vocab, dtype, device)
+        z = c.logits.requires_grad_()
+        lp = cl.selected_log_probs(z, c.act_t)
+        assert lp.dtype == c.wide and lp.shape == (rows,)
+        _near(_np(lp), c.lp, c.err, c.wide)
+        (g,) = torch.autograd.grad(lp, z, c.adv_t)
+        c.check_gradient(g, c.adv)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("kl", [0.0, 0.05])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_policy_loss(device, dtype, kl, reduction):
+    for rows, vocab in SIZES:
+        c = Case(rows, vocab, dtype, device)
+        z = c.logits.requires_grad_()
+        loss, lp = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, ref_log_probs=c.ref_t if kl else None,
+                                  clip=(0.2, 0.28), kl_coef=kl, reduction=reduction,
+                                  return_log_probs=True)
+        term, slope = P.policy_terms(c.lp, c.actions, c.old, c.adv, c.ref, 0.2, 0.28, kl)
+        counted = c.actions != IGNORE
+        n = counted.sum()
+        # |d term / d lp| <= 1.7 |A| + kl expm1(|g|); the terms are kept in the wide type
+        bound = 1.8 * np.abs(c.adv) + kl * 5
+        terr = bound * c.err + np.abs(term) * 2 * _unit(dtype)
+        serr = 2 * bound * c.err
+        _near(_np(lp), c.lp, c.err, c.wide)
+        assert loss.dtype == c.wide
+        if reduction == "none":
+            up = np.random.default_rng(1).standard_normal(rows)
+            ut = torch.as_tensor(up).to(c.wide).to(device)
+            up = _np(ut)
+            _near(_np(loss), term, terr, c.wide)
+            (g,) = torch.autograd.grad(loss, z, ut)
+            c.check_gradient(g, slope * up, serr * np.abs(up))
+        else:
+            div = n if reduction == "mean" else 1
+            _near(_np(loss), term[counted].sum() / div, terr[counted].sum() / div, c.wide)
+            for up in (1.0, 0.375):
+                (g,) = torch.autograd.grad(loss * up, z, retain_graph=True)
+                c.check_gradient(g, slope * up / div, serr * up / div)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("with_ref", [True, False])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_preference_loss(device, dtype, with_ref, reduction):
+    for lengths, vocab, tail in [([1, 1], 200, 0), ([3, 1, 2, 5], 33, 0), ([0, 4, 3, 0], 1000, 2),
+                                 ([300, 1, 2, 7, 31, 290], 129, 5), ([5, 2], 33001, 1),
+                                 ([1] * 128, 10, 0)]:
+        offsets = np.concatenate(([0], np.cumsum(lengths)))
+        rows, pairs = int(offsets[-1]) + tail, len(lengths) // 2
+        c = Case(rows, vocab, dtype, device, ignored=0.1)
+        z = c.logits.requires_grad_()
+        beta = 0.1 if with_ref else 0.02
+        loss, margins = cl.preference_loss(
+            z, c.act_t, torch.as_tensor(offsets).to(device),
+            ref_log_probs=c.ref_t if with_ref else None, beta=beta, label_smoothing=0.1,
+            reduction=reduction, return_margins=True)
+        h, term, slope = P.preference_terms(c.lp, c.actions, offsets, c.ref if with_ref else None,
+                                            beta, 0.1)
+        seq = np.diff(offsets)
+        herr = beta * (seq[:pairs] + seq[pairs:]) * c.err * 1.01
+        assert margins.shape == (pairs,) and margins.dtype == c.wide
+        _near(_np(margins), h, herr, c.wide)
+        # |d term / d h| <= 1, |d slope / d h| <= beta / 4; both kept in the wide type
+        serr = np.zeros(rows)
+        for i in range(pairs):
+            e = beta * herr[i] / 4 + 2 * beta * _unit(dtype)
+            serr[offsets[i]:offsets[i + 1]] = e
+            serr[offsets[pairs + i]:offsets[pairs + i + 1]] = e
+        terr = herr + np.abs(term) * 2 * _unit(dtype)
+        if reduction == "none":
+            up = np.linspace(-1, 2, pairs)
+            ut = torch.as_tensor(up).to(c.wide).to(device)
+            _near(_np(loss), term, terr, c.wide)
+            (g,) = torch.autograd.grad(loss, z, ut)
+            row_up = np.zeros(rows)
+            for i in range(pairs):
+                row_up[offsets[i]:offsets[i + 1]] = _np(ut)[i]
+                row_up[offsets[pairs + i]:offsets[pairs + i + 1]] = _np(ut)[i]
+            c.check_gradient(g, slope * row_up, serr * np.abs(row_up) + np.abs(slope * row_up) * 2 * _unit(dtype))
+        else:
+            div = pairs if reduction == "mean" else 1
+            _near(_np(loss), term.sum() / div, terr.sum() / div, c.wide)
+            for up in (1.0, 0.375):
+                (g,) = torch.autograd.grad(loss * up, z, retain_graph=True)
+                c.check_gradient(g, slope * up / div, serr * up / div)
+
+
+@pytest.mark.parametrize("layout", ["padded", "offset", "transposed", "expanded", "batched"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [10, 301, 5003, 40001])
+def test_layouts(device, vocab, dtype, layout):
+    """Strided logits give what contiguous ones give, bit by bit."""
+    rows = 6
+    c = Case(rows, vocab, dtype, device)
+    z = c.logits
+    if layout == "padded":
+        t = torch.zeros((rows, vocab + 7), dtype=dtype, device=device)
+        t[:, :vocab] = z
+        x = t[:, :vocab]
+    elif layout == "offset":
+        t = torch.zeros(rows * vocab + 3, dtype=dtype, device=device)
+        t[3:] = z.reshape(-1)
+        x = t[3:].view(rows, vocab)
+    elif layout == "transposed":
+        x = z.t().contiguous().t()
+    elif layout == "expanded":
+        z = z[:1].expand(rows, vocab)
+        x, z = z, z.contiguous()
+    else:
+        x = z.view(2, 3, vocab)
+    shape = x.shape[:-1]
+    x, z = x.detach().requires_grad_(), z.detach().requires_grad_()
+    a, o, v, r = (t.view(shape) for t in (c.act_t, c.old_t, c.adv_t, c.ref_t))
+    got = cl.policy_loss(x, a, o, v, r, kl_coef=0.1, return_log_probs=True)
+    ref = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, c.ref_t, kl_coef=0.1, return_log_probs=True)
+    assert got[1].shape == shape
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1].reshape(-1), ref[1])
+    gx = torch.autograd.grad(got[0], x)[0].reshape(rows, vocab)
+    gz = torch.autograd.grad(ref[0], z)[0]
+    assert torch.equal(gx, gz)
+    lx, lz = cl.selected_log_probs(x, a), cl.selected_log_probs(z, c.act_t)
+    assert torch.equal(lx.reshape(-1), lz)
+    assert torch.equal(torch.autograd.grad(lx, x, v)[0].reshape(rows, vocab),
+                       torch.autograd.grad(lz, z, c.adv_t)[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [7, 300, 5001, 70001])
+def test_masked_logits_and_rows(device, vocab, dtype):
+    """Masked classes (-inf, the type's lowest value), ignored rows full of NaN, rows with nothing
+    left, actions that do not exist."""
+    rows = 8
+    c = Case(rows, vocab, dtype, device, ignored=0.0)
+    z, a = c.logits.clone(), c.act_t.clone()
+    a[:] = torch.arange(rows, device=device) % vocab
+    low = torch.finfo(dtype).min
+    z[0, 1:] = float("-inf")                # one class left: lp = 0, gradient 0
+    z[1, 2:] = low                          # two classes left
+    z[2] = float("nan")
+    a[2] = IGNORE                           # does not count whatever it holds
+    z[3] = float("-inf")                    # nothing left: NaN
+    a[4] = vocab                            # no such class: NaN
+    a[5] = -1
+    z[6, 6 % vocab] = float("-inf")         # the chosen class is masked
+    c.z, c.actions = _np(z), a.cpu().numpy()
+    with np.errstate(invalid="ignore", divide="ignore"):
+        c.lp, c.probs = P.log_probs(c.z, c.actions)
+    c.err = _sum_error(c.z, dtype)
+    c.old_t[2] = c.adv_t[2] = c.ref_t[2] = float("nan")
+    z.requires_grad_()
+    lp = cl.selected_log_probs(z, a)
+    got = _np(lp)
+    assert np.isnan(got[[3, 4, 5]]).all() and got[6] == -np.inf and got[2] == 0 and got[0] == 0
+    _near(got, c.lp, c.err, c.wide)
+    up = torch.ones_like(lp)
+    (g,) = torch.autograd.grad(lp, z, up)
+    g = _np(g)
+    assert np.isnan(g[[3, 4, 5]]).all() and (g[2] == 0).all() and (g[0] == 0).all()
+    ok = [0, 1, 2, 6, 7]
+    ref = P.logit_gradient(c.probs, c.actions, np.ones(rows))
+    _near(g[ok], ref[ok], 2 * c.err, dtype)
+    # the losses: NaN rows make the loss NaN, not the gradient of the other rows
+    loss = cl.policy_loss(z, a, c.old_t, c.adv_t, reduction="none")
+    t = _np(loss)
+    assert np.isnan(t[[3, 4, 5]]).all() and np.isfinite(t[ok]).all() and t[2] == 0
+    total = cl.policy_loss(z, a, c.old_t, c.adv_t)
+    (g,) = torch.autograd.grad(total, z)
+    g = _np(g)
+    assert np.isnan(float(total)) and np.isnan(g[[3, 4, 5]]).all() and np.isfinite(g[ok]).all()
+    assert (g[2] == 0).all()
+
+
+def test_nothing_counts(device):
+    z = torch.randn(4, 9, device=device, requires_grad=True)
+    a = torch.full((4,), IGNORE, device=device)
+    f = torch.zeros(4, device=device)
+    loss = cl.policy_loss(z, a, f, f)
+    assert torch.isnan(loss)
+    assert (torch.autograd.grad(loss, z)[0] == 0).all()
+    assert float(cl.policy_loss(z, a, f, f, reduction="sum")) == 0
+    off = torch.tensor([0, 2, 4], device=device)
+    loss, h = cl.preference_loss(z, a, off, return_margins=True)
+    assert float(h) == 0 and abs(float(loss) - np.log(2)) < 1e-6
+    assert (torch.autograd.grad(loss, z)[0] == 0).all()
+    # no rows, no pairs
+    z0 = torch.empty(0, 9, device=device, requires_grad=True)
+    a0, f0 = a[:0], f[:0]
+    assert cl.selected_log_probs(z0, a0).shape == (0,)
+    loss = cl.policy_loss(z0, a0, f0, f0)
+    assert torch.isnan(loss) and torch.autograd.grad(loss, z0)[0].shape == (0, 9)
+    assert float(cl.policy_loss(z0, a0, f0, f0, reduction="sum")) == 0
+    assert cl.policy_loss(z0, a0, f0, f0, reduction="none").shape == (0,)
+    loss, h = cl.preference_loss(z, a, off[:1], return_margins=True)
+    assert torch.isnan(loss) and h.shape == (0,)
+    assert (torch.autograd.grad(loss, z)[0] == 0).all()
+    # a pair of empty sequences
+    loss, h = cl.preference_loss(z0, a0, off[:1].expand(3), return_margins=True)
+    assert float(h) == 0 and torch.autograd.grad(loss, z0)[0].shape == (0, 9)
+    # another ignore_index
+    b = torch.tensor([0, 3, 0, 5], device=device)
+    lp = cl.selected_log_probs(z, b, ignore_index=0)
+    ref = torch.log_softmax(z.detach().double(), 1)
+    assert lp[0] == 0 and lp[2] == 0 and abs(float(lp[3]) - float(ref[3, 5])) < 1e-5
+
+
+def test_bad_offsets_give_nan(device):
+    """Offsets that decrease or leave the rows are read within the rows, and their pair is NaN."""
+    c = Case(12, 20, torch.float32, device, ignored=0.0)
+    for off in ([0, 5, 3, 8, 12], [0, 3, 6, 9, 13], [-1, 3, 6, 9, 12], [2**62, 3, 6, 9, 12],
+                [0, 3, 6, 9, -2**62]):
+        terms, h = cl.preference_loss(c.logits, c.act_t, torch.tensor(off, device=device),
+                                      reduction="none", return_margins=True)
+        bad = [any(not 0 <= off[q] <= off[q + 1] <= 12 for q in (i, 2 + i)) for i in range(2)]
+        assert torch.isnan(terms).tolist() == bad and torch.isnan(h).tolist() == bad
+
+
+def test_near_certain_policy(device):
+    """1 - p of the chosen class, down to far below a unit of 1.  The row's sum 1 + 3 exp(-gap) is
+    held in fp32: three additions next to 1 round by 2^-24 each, and so does the gradient's last
+    product: 1 - p, which is known no better than the sum, is off by four of them."""
+    for gap in (5.0, 12.0, 20.0, 40.0):
+        z = torch.zeros(1, 4, device=device)
+        z[0, 1] = gap
+        z.requires_grad_()
+        a = torch.ones(1, dtype=torch.int64, device=device)
+        (g,) = torch.autograd.grad(cl.selected_log_probs(z, a).sum(), z)
+        rest = -np.expm1(-np.log1p(3 * np.exp(-gap)))
+        assert abs(float(g[0, 1]) - rest) <= 4 * 2.0**-24
+
+
+def test_gradients_against_differences(device):
+    """Central differences in float64 at 1e-6: cancellation leaves about 1e-10."""
+    c = Case(6, 11, torch.float64, device, ignored=0.2)
+    off = torch.tensor([0, 2, 3, 5, 6], device=device)
+    fs = [lambda z: cl.selected_log_probs(z, c.act_t).mul(c.adv_t).sum(),
+          lambda z: cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, c.ref_t, kl_coef=0.3),
+          lambda z: cl.preference_loss(z, c.act_t, off, c.ref_t, beta=0.7, label_smoothing=0.1)]
+    for f in fs:
+        z = c.logits.clone().requires_grad_()
+        (g,) = torch.autograd.grad(f(z), z)
+        d = torch.zeros_like(g)
+        with torch.no_grad():
+            for i in range(6):
+                for j in range(11):
+                    hi, lo = c.logits.clone(), c.logits.clone()
+                    hi[i, j] += 1e-6
+                    lo[i, j] -= 1e-6
+                    d[i, j] = (f(hi) - f(lo)) / 2e-6
+        assert float((g - d).abs().max()) < 1e-8
+
+
+def test_second_backward_and_other_upstream(device):
+    """A retained graph gives the same gradient again, whatever was done with the first."""
+    for dtype in (torch.float32, torch.bfloat16):
+        for vocab in (10, 3001):
+            c = Case(40, vocab, dtype, device)
+            z = c.logits.requires_grad_()
+            loss = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t)
+            (g1,) = torch.autograd.grad(loss, z, retain_graph=True)
+            keep = g1.clone()
+            (g2,) = torch.autograd.grad(loss * 0, z, retain_graph=True)
+            (g3,) = torch.autograd.grad(loss, z, retain_graph=True)
+            assert torch.equal(g1, keep) and torch.equal(g3, keep) and not g2.any()
+            g1.zero_()
+            (g4,) = torch.autograd.grad(loss, z)
+            assert torch.equal(g4, keep)
+
+
+def test_refusals(device):
+    z = torch.zeros(3, 5, device=device)
+    a = torch.zeros(3, dtype=torch.int64, device=device)
+    f = torch.zeros(3, device=device)
+    off = torch.tensor([0, 1, 2], device=device)
+    with pytest.raises(RuntimeError, match="actions must be int64"):
+        cl.selected_log_probs(z, a.int())
+    with pytest.raises(RuntimeError, match="actions must be int64"):
+        cl.selected_log_probs(z, a[:2])
+    with pytest.raises(RuntimeError, match="same HIP device"):
+        cl.selected_log_probs(z, a.cpu())
+    with pytest.raises(RuntimeError, match="dtype"):
+        cl.selected_log_probs(z.long(), a)
+    with pytest.raises(RuntimeError, match="at least one class"):
+        cl.selected_log_probs(z[:, :0], a)
+    with pytest.raises(RuntimeError, match="old_log_probs must be"):
+        cl.policy_loss(z, a, f[:2], f)
+    with pytest.raises(RuntimeError, match="advantages must be"):
+        cl.policy_loss(z, a, f, f.long())
+    with pytest.raises(RuntimeError, match="detach"):
+        cl.policy_loss(z, a, f.clone().requires_grad_(), f)
+    with pytest.raises(RuntimeError, match="ref_log_probs must be"):
+        cl.policy_loss(z, a, f, f, f.cpu())
+    with pytest.raises(ValueError, match="clip"):
+        cl.policy_loss(z, a, f, f, clip=-0.1)
+    with pytest.raises(ValueError, match="kl_coef"):
+        cl.policy_loss(z, a, f, f, kl_coef=0.1)
+    with pytest.raises(ValueError, match="reduction"):
+        cl.policy_loss(z, a, f, f, reduction="median")
+    for bad in (off[:2], off.int(), off.cpu(), off.view(1, 3)):
+        with pytest.raises(RuntimeError, match="offsets must be"):
+            cl.preference_loss(z, a, bad)
+    with pytest.raises(ValueError, match="label_smoothing"):
+        cl.preference_loss(z, a, off, label_smoothing=1.5)
+    with pytest.raises(RuntimeError, match="ragged batch"):
+        cl.preference_loss(z[None], a[None], off)
+    x = z.clone().requires_grad_()
+    for f2 in (lambda y: cl.policy_loss(y, a, f, f + 1), lambda y: cl.preference_loss(y, a, off),
+               lambda y: cl.selected_log_probs(y, a).sum()):
+        with pytest.raises(RuntimeError, match="twice"):
+            torch.autograd.grad(f2(x * x), x, create_graph=True)
+    y = x * 1
+    lp = cl.selected_log_probs(y, a)
+    y += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lp.sum().backward()
+
+
+def test_half_precision_constants_are_widened(device):
+    c = Case(20, 50, torch.bfloat16, device)
+    old, adv = c.old_t.half(), c.adv_t.bfloat16()
+    got = cl.policy_loss(c.logits, c.act_t, old, adv)
+    assert torch.equal(got, cl.policy_loss(c.logits, c.act_t, old.float(), adv.float()))
+
+
+def test_half_gradient_of_a_scaled_loss(device):
+    """A mean over many rows in half precision: the gradient is formed from the scaled loss, not
+    scaled after it was rounded to (or flushed below) half's smallest numbers."""
+    c = Case(4096, 40, torch.float16, device)
+    z = c.logits.requires_grad_()
+    loss = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t) * 65536.0
+    (g,) = torch.autograd.grad(loss, z)
+    term, slope = P.policy_terms(c.lp, c.actions, c.old, c.adv, c.ref, 0.2, 0.2, 0.0)
+    n = (c.actions != IGNORE).sum()
+    c.check_gradient(g, slope * 65536.0 / n, 2 * 1.8 * np.abs(c.adv) * c.err * 65536.0 / n)
+
+
+def test_group_sum_methods(device):
+    """The three losses of a network's class scores: GroupSum's scores through the functions, and
+    the gradient back through GroupSum, on a LogicLayer's layout."""
+    x = torch.rand(1200, 64, device=device).t().requires_grad_()
+    gs = cl.GroupSum(10, 4.0)
+    rng = np.random.default_rng(0)
+    a = torch.as_tensor(rng.integers(0, 10, 64)).to(device)
+    old = torch.as_tensor(rng.standard_normal(64) - 2.3).float().to(device)
+    adv = torch.as_tensor(rng.standard_normal(64)).float().to(device)
+    off = torch.arange(0, 65, 4, device=device)
+    scores = gs(x).detach().requires_grad_()
+    for via, direct in [
+            (gs.log_probs(x, a).sum(), cl.selected_log_probs(scores, a).sum()),
+            (gs.policy_loss(x, a, old, adv), cl.policy_loss(scores, a, old, adv)),
+            (gs.preference_loss(x, a, off[:-1] if off.numel() % 2 == 0 else off, beta=0.3),
+             cl.preference_loss(scores, a, off[:-1] if off.numel() % 2 == 0 else off, beta=0.3))]:
+        assert torch.equal(via, direct)
+        (gx,) = torch.autograd.grad(via, x)
+        (gsc,) = torch.autograd.grad(direct, scores)
+        assert torch.equal(gx, (gsc / 4.0).repeat_interleave(120, 1))
+        assert gx.t().is_contiguous()
+    h = gs.policy_loss(x.half(), a, old, adv)
+    assert h.dtype == torch.float32 and torch.isfinite(h)
+    with pytest.raises(RuntimeError, match="detach"):
+        gs.policy_loss(x, a, gs.log_probs(x, a), adv)
+
+
+def test_captured_policy_step(device):
+    """A policy step of a whole network (dropout, GroupSum, the clipped loss, Adam) captured once:
+    every replay equals the eager step with the same mask."""
+    torch.manual_seed(0)
+
+    def build():
+        torch.manual_seed(1)
+        net = torch.nn.Sequential(cl.LogicLayer(60, 300, connections="original"),
+                                  cl.Dropout(0.1, fill=0.5, seed=4), cl.LogicLayer(300, 300),
+                                  cl.GroupSum(10, 3.0)).to(device)
+        return net, cl.FusedAdam(net.parameters(), lr=0.01)
+
+    x = (torch.rand(128, 60, device=device) < 0.4).float()
+    a = torch.randint(0, 10, (128,), device=device)
+    adv = torch.randn(128, device=device)
+    net, opt = build()
+    with torch.no_grad():
+        old = net[3].log_probs(net[:3](x), a)
+        ref = old + 0.1 * torch.randn(128, device=device)
+
+    def step(net, opt):
+        opt.zero_grad(set_to_none=True)
+        loss, lp = net[3].policy_loss(net[:3](x), a, old, adv, ref_log_probs=ref, kl_coef=0.1,
+                                      return_log_probs=True)
+        loss.backward()
+        opt.step()
+        return loss.detach(), lp
+
+    net, opt = build()
+    eager = []
+    for _ in range(6):
+        loss, lp = step(net, opt)
+        eager.append((loss.clone(), lp.clone(), [p.detach().clone() for p in net.parameters()]))
+    net, opt = build()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(net, opt)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, lp = step(net, opt)
+    for k in range(2, 6):
+        junk = torch.randn(1000, device=device).sum()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = eager[k]
+        assert torch.equal(loss, want[0]) and torch.equal(lp, want[1]), f"replay {k}"
+        for p, w in zip(net.parameters(), want[2]):
+            assert torch.equal(p, w), f"replay {k}"
+        del junk
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [10, 3001, 70001])
+def test_captured_losses(device, dtype, vocab):
+    """Each loss with its gradient captured; replays on new inputs equal the eager calls."""
+    rows = 24
+    off = torch.tensor([0, 5, 9, 16, 22], device=device)
+    cases = [Case(rows, vocab, dtype, device, seed=s) for s in range(3)]
+    c0 = cases[0]
+    fs = [lambda z, c: cl.selected_log_probs(z, c.act_t).sum(),
+          lambda z, c: cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, c.ref_t, kl_coef=0.1),
+          lambda z, c: cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, reduction="sum") * 0.5,
+          lambda z, c: cl.preference_loss(z, c.act_t, off, c.ref_t)]
+    for f in fs:
+        want = []
+        for c in cases:
+            z = c.logits.clone().requires_grad_()
+            loss = f(z, c)
+            want.append((loss.detach().clone(), torch.autograd.grad(loss, z)[0]))
+            del loss, z
+        static = Case(rows, vocab, dtype, device, seed=0)
+        z = static.logits.clone().requires_grad_()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            loss = f(z, static)
+            torch.autograd.grad(loss, z)
+            del loss
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss = f(z, static)
+            (g,) = torch.autograd.grad(loss, z)
+        for c, (wl, wg) in zip(cases + cases[:1], want + want[:1]):
+            with torch.no_grad():
+                z.copy_(c.logits)
+            for name in ("act_t", "old_t", "adv_t", "ref_t"):
+                getattr(static, name).copy_(getattr(c, name))
+            torch.randn(100, device=device).sum()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(loss.detach(), wl) and torch.equal(g, wg)
+
+
+def test_streams(device):
+    c = Case(64, 5001, torch.bfloat16, device)
+    z = c.logits.requires_grad_()
+    ref = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t)
+    (gref,) = torch.autograd.grad(ref, z)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t)
+        (g,) = torch.autograd.grad(loss, z)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(loss, ref) and torch.equal(g, gref)
+
+
+def test_rows_beyond_32_bits(device):
+    """Logits whose last rows lie past 2^32 elements, reached through their stride."""
+    rows, vocab = 3, 1001
+    stride = (1 << 31) + 64
+    big = torch.empty(2 * stride + vocab, dtype=torch.float16, device=device)
+    x = big.as_strided((rows, vocab), (stride, 1))
+    c = Case(rows, vocab, torch.float16, device, ignored=0.0)
+    x.copy_(c.logits)
+    lp = cl.selected_log_probs(x, c.act_t)
+    assert torch.equal(lp, cl.selected_log_probs(c.logits, c.act_t))
+    _near(_np(lp), c.lp, c.err, c.wide)
