@@ -131,13 +131,14 @@ SIGNATURES: dict[str, list] = {
     "cl_adam_clip_workspace": [_i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64)],
     "cl_adam_clip_step": [_int, _i64, _p, _p, _p, _p, ctypes.POINTER(_i64), _p, _f64, _f64,
                           _f64, _f64, _f64, _p, _i64, _p],
-    "cl_selected_log_prob_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
+    "cl_token_loss_workspace": [_int, _i64, _i64, ctypes.POINTER(_i64)],
+    "cl_selected_log_prob_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p],
     "cl_selected_log_prob_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
     "cl_policy_loss_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _f64, _f64, _f64,
-                               _int, _p, _p, _p, _p, _p, _p],
+                               _int, _p, _p, _p, _p, _p, _p, _i64, _p],
     "cl_policy_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _int, _p, _p, _p, _p],
     "cl_preference_loss_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _f64, _f64,
-                                   _int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
+                                   _int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
     "cl_preference_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _int, _p, _p,
                                     _p, _p],
     "cl_dropout": [_int, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _int, _f64, _u64, _u64,

@@ -4,6 +4,8 @@
 
 #include "common.h"
 
+#include <type_traits>
+
 namespace cl {
 
 using half_t = _Float16;
@@ -42,23 +44,42 @@ using wide_t = typename WideType<T>::type;
         }                                                                                \
     } while (0)
 
-// N elements moved as one access, at any address that is a multiple of the element size: the
-// hardware takes 16-byte global accesses off 16 bytes, so rows need no alignment of their own.
+// N elements moved in 16-byte accesses, at any address that is a multiple of the element size:
+// the hardware takes them off 16 bytes, so rows need no alignment of their own.
 template <typename T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) Pack {
+struct Pack {
+    static_assert(N * sizeof(T) % 16 == 0, "whole 16-byte accesses");
     T v[N];
 };
 
+typedef uint32_t quad2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t quad4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t quad8 __attribute__((ext_vector_type(4), aligned(8)));
+
+template <typename T>
+using quad_of = std::conditional_t<sizeof(T) == 2, quad2,
+                                   std::conditional_t<sizeof(T) == 4, quad4, quad8>>;
+
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> pload(const T* p) {
-    Pack<T, N> r;
-    __builtin_memcpy(&r, p, sizeof(r));
-    return r;
+    using Q = quad_of<T>;
+    struct Words {
+        Q q[N * sizeof(T) / 16];
+    } w;
+#pragma unroll
+    for (int i = 0; i < int(N * sizeof(T) / 16); ++i) w.q[i] = reinterpret_cast<const Q*>(p)[i];
+    return __builtin_bit_cast(Pack<T, N>, w);
 }
 
 template <typename T, int N>
 __device__ __forceinline__ void pstore(T* p, const Pack<T, N>& r) {
-    __builtin_memcpy(p, &r, sizeof(r));
+    using Q = quad_of<T>;
+    struct Words {
+        Q q[N * sizeof(T) / 16];
+    };
+    const Words w = __builtin_bit_cast(Words, r);
+#pragma unroll
+    for (int i = 0; i < int(N * sizeof(T) / 16); ++i) reinterpret_cast<Q*>(p)[i] = w.q[i];
 }
 
 }  // namespace cl

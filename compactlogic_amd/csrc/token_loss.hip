@@ -17,8 +17,6 @@
 namespace cl {
 namespace {
 
-constexpr int kRowThreads = 256;
-
 // What the backward needs of a row.
 template <typename A>
 struct alignas(4 * sizeof(A)) RowState {
@@ -40,13 +38,27 @@ struct RowArgs {
     RowState<wide_t<T>>* state;
 };
 
-// ---- what each loss makes of a row's lp: writes its own outputs, returns the slope
+template <typename A>
+__device__ __forceinline__ A nan_value() {
+    return A(__builtin_nan(""));
+}
+
+// ---- what each loss makes of a row's lp.  `load` fetches the row's own inputs early; e[1] and
+// e[2] are the exponentials of arg(1) and arg(2), taken by neighbouring lanes at once; `counted`
+// writes the loss's outputs (one lane) and returns the slope.
+struct RowInputs {
+    double old_lp, adv, ref;
+};
+
 template <typename A>
 struct LogProbOp {
-    __device__ __forceinline__ A counted(int64_t, double lp) const {
-        return lp == lp ? A(1) : A(lp);
+    __device__ __forceinline__ RowInputs load(int64_t) const { return {}; }
+    __device__ __forceinline__ double arg(int, double lp, const RowInputs&) const { return lp; }
+    __device__ __forceinline__ double counted(int64_t, double lp, const RowInputs&, const double*,
+                                              bool) const {
+        return lp == lp ? 1.0 : lp;
     }
-    __device__ __forceinline__ void ignored(int64_t) const {}
+    __device__ __forceinline__ void ignored(int64_t, bool) const {}
 };
 
 // term = kl (exp(g) - g - 1) - clip(r) adv with r = exp(lp - old) clipped from above where adv
@@ -59,9 +71,15 @@ struct PolicyOp {
     const A* ref;
     double low, high, kl;
     A* terms;
-    __device__ __forceinline__ A counted(int64_t n, double lp) const {
-        const double a = double(adv[n]);
-        const double r = exp(lp - double(old_lp[n]));
+    __device__ __forceinline__ RowInputs load(int64_t n) const {
+        return {double(old_lp[n]), double(adv[n]), ref ? double(ref[n]) : 0.0};
+    }
+    __device__ __forceinline__ double arg(int i, double lp, const RowInputs& in) const {
+        return i == 1 ? lp - in.old_lp : in.ref - lp;
+    }
+    __device__ __forceinline__ double counted(int64_t n, double lp, const RowInputs& in,
+                                              const double* e, bool write) const {
+        const double a = in.adv, r = e[1];
         double term, slope;
         if (a >= 0) {
             term = -(r > high ? high : r) * a;
@@ -71,87 +89,355 @@ struct PolicyOp {
             slope = r < low ? 0.0 : -a * r;
         }
         if (ref) {
-            const double g = double(ref[n]) - lp;
-            const double e = expm1(g);
-            term += kl * (e - g);
-            slope -= kl * e;
+            term += kl * ((e[2] - 1.0) - (in.ref - lp));
+            slope -= kl * (e[2] - 1.0);
         }
-        terms[n] = A(term);
-        return A(slope);
+        if (write) terms[n] = A(term);
+        return slope;
     }
-    __device__ __forceinline__ void ignored(int64_t n) const { terms[n] = A(0); }
+    __device__ __forceinline__ void ignored(int64_t n, bool write) const {
+        if (write) terms[n] = A(0);
+    }
 };
 
-// gap = lp - ref, summed over sequences by k_pref_pairs.
+// gap = lp - ref, summed over sequences by pair_terms.
 template <typename A>
 struct PreferenceOp {
     const A* ref;
     double* gaps;
     int32_t* row_seq;
-    __device__ __forceinline__ A counted(int64_t n, double lp) const {
-        gaps[n] = lp - (ref ? double(ref[n]) : 0.0);
-        row_seq[n] = -1;
-        return A(1);
+    __device__ __forceinline__ RowInputs load(int64_t n) const {
+        return {0.0, 0.0, ref ? double(ref[n]) : 0.0};
     }
-    __device__ __forceinline__ void ignored(int64_t n) const {
-        gaps[n] = 0.0;
-        row_seq[n] = -1;
+    __device__ __forceinline__ double arg(int, double lp, const RowInputs&) const { return lp; }
+    __device__ __forceinline__ double counted(int64_t n, double lp, const RowInputs& in,
+                                              const double*, bool write) const {
+        if (write) {
+            gaps[n] = lp - in.ref;
+            row_seq[n] = -1;
+        }
+        return 1.0;
+    }
+    __device__ __forceinline__ void ignored(int64_t n, bool write) const {
+        if (write) {
+            gaps[n] = 0.0;
+            row_seq[n] = -1;
+        }
     }
 };
 
+// ---- exponentials and reductions
+// exp of a difference d = x - m <= 0.  fp32: the hardware's 2^t of t = d log2 e, log2 e in two
+// terms, so that t is rounded once and without a drift: over d in [-16, 0] the mean relative error
+// measures 3e-9 (1e-7 with log2 e as one fp32 number, which a sum over a vocabulary, and then over
+// a sequence, does not average out), the largest 7e-7, at the far end.
+__device__ __forceinline__ float exp_diff(float d) {
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.44269502162933349609f,
+                                                 d * 1.92596299112661746887e-8f));
+}
+__device__ __forceinline__ double exp_diff(double d) { return exp(d); }
+
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double max_of(double a, double b) { return __builtin_fmax(a, b); }
+
+// Where a part of a row saw nothing but -inf its maximum is -inf, and differences are taken from
+// 0 instead: its sum is 0, or NaN if a NaN came by.
 template <typename A>
-__device__ __forceinline__ A nan_value() {
-    return A(__builtin_nan(""));
+__device__ __forceinline__ A base_of(A m) {
+    return m == -A(__builtin_inf()) ? A(0) : m;
 }
 
-// Running maximum and sum of a softmax: two partial rows joined.  A part that saw nothing but
-// -inf has m = -inf; its sum is then kept as it is (0, or NaN if a NaN came by).
-template <typename A>
-__device__ __forceinline__ void join(A& m, A& s, A m2, A s2) {
-    const A mm = m2 > m ? m2 : m;
-    const A base = mm == -A(__builtin_inf()) ? A(0) : mm;
-    s = s * exp(m - base) + s2 * exp(m2 - base);
-    m = mm;
+// Over the TPR lanes of a row (16: a DPP row, 64: the wave), the same value in each of them.
+template <int TPR, typename A>
+__device__ __forceinline__ A lanes_max(A v) {
+    v = max_of(v, dpp_move<0xB1>(v));
+    v = max_of(v, dpp_move<0x4E>(v));
+    v = max_of(v, dpp_move<0x124>(v));
+    v = max_of(v, dpp_move<0x128>(v));
+    if constexpr (TPR == 64)
+        v = max_of(max_of(read_lane(v, 0), read_lane(v, 16)),
+                   max_of(read_lane(v, 32), read_lane(v, 48)));
+    return v;
 }
 
-// The row's scalars, by one thread.
-template <typename T, typename Op>
-__device__ __forceinline__ void finish_row(const RowArgs<T>& a, const Op& op, int64_t n,
-                                           wide_t<T> m, wide_t<T> s) {
+template <int TPR, typename A>
+__device__ __forceinline__ A lanes_sum(A v) {
+    if constexpr (TPR == 64) return wave_total(v);
+    v += dpp_move<0xB1>(v);
+    v += dpp_move<0x4E>(v);
+    v += dpp_move<0x124>(v);
+    v += dpp_move<0x128>(v);
+    return v;
+}
+
+// Running maximum m and sum s of exp(x - m) over the lanes of a row.
+template <int LANES, typename A>
+__device__ __forceinline__ void join_lanes(A& m, A& s) {
+    const A all = lanes_max<LANES>(m), base = base_of(all);
+    s = lanes_sum<LANES>(s * exp_diff(m - base));
+    m = all;
+}
+
+// The same over the waves of a workgroup that share a row; every wave ends with the row's m and s.
+template <int WAVES, typename A>
+__device__ __forceinline__ void join_waves(A& m, A& s, A (*part)[2]) {
+    join_lanes<64>(m, s);
+    if constexpr (WAVES > 1) {
+        if (lane_id() == 0) {
+            part[wave_id()][0] = m;
+            part[wave_id()][1] = s;
+        }
+        __syncthreads();
+        const int l = lane_id();
+        m = l < WAVES ? part[l][0] : -A(__builtin_inf());
+        s = l < WAVES ? part[l][1] : A(0);
+        join_lanes<64>(m, s);
+    }
+}
+
+// ---- the row's scalars from m and s, by all lanes of one wave (or of a 16-lane row); the lane
+// with write set stores them.
+template <int LANES, typename T, typename Op>
+__device__ __forceinline__ RowState<wide_t<T>> finish_row(const RowArgs<T>& a, const Op& op,
+                                                          int64_t n, int64_t act, wide_t<T> xa,
+                                                          const RowInputs& in, wide_t<T> m,
+                                                          wide_t<T> s, bool write) {
     using A = wide_t<T>;
-    const int64_t act = a.actions[n];
     RowState<A> st{m, A(1) / s, A(0), A(0)};
     if (act == a.ignore) {
-        op.ignored(n);
-        a.lp[n] = A(0);
+        op.ignored(n, write);
+        if (write) a.lp[n] = A(0);
     } else {
-        double lp = nan_value<double>();
-        if (act >= 0 && act < a.cols)
-            lp = (double(a.x[n * a.stride + act]) - double(m)) - log(double(s));
-        a.lp[n] = A(lp);
-        st.rest = A(-expm1(lp));
-        st.slope = op.counted(n, lp);
+        double lp = (double(xa) - double(m)) - log(double(s));
+        if (act < 0 || act >= a.cols) lp = nan_value<double>();
+        const int l = lane_id() & (LANES - 1);
+        const double mine = exp(l == 1 || l == 2 ? op.arg(l, lp, in) : lp);
+        const double e[3] = {__shfl(mine, 0, LANES), __shfl(mine, 1, LANES),
+                             __shfl(mine, 2, LANES)};
+        if (write) a.lp[n] = A(lp);
+        st.rest = A(1.0 - e[0]);
+        st.slope = A(op.counted(n, lp, in, e, write));
     }
-    a.state[n] = st;
+    if (write) a.state[n] = st;
+    return st;
+}
+
+// The action as a place in the row, far before it where there is none.
+template <typename T>
+__device__ __forceinline__ int action_place(const RowArgs<T>& a, int64_t act) {
+    return act >= 0 && act < a.cols ? int(act) : INT32_MIN / 2;
+}
+
+template <typename T>
+__device__ __forceinline__ wide_t<T> action_logit(const RowArgs<T>& a, const T* x, int64_t act) {
+    return act >= 0 && act < a.cols ? wide_t<T>(x[act]) : wide_t<T>(0);
+}
+
+// ---- gradient of one logit: c ([j = a] - p_j) as exp(x - m) * k, k = -c / s, or c (1 - p_a).
+template <typename A>
+struct RowGrad {
+    A m, k, own;
+    __device__ __forceinline__ RowGrad(const RowState<A>& st, A c)
+        : m(st.m), k(-c * st.inv_s), own(c * st.rest) {}
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> grad_of(const Pack<T, VEC>& x, const RowGrad<wide_t<T>>& g,
+                                                int from_act) {
+    using A = wide_t<T>;
+    Pack<T, VEC> r;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+        r.v[e] = T(e == from_act ? g.own : exp_diff(A(x.v[e]) - g.m) * g.k);
+    return r;
+}
+
+// ---- maximum and sum of a row held in registers: NV vectors of 16 bytes and one element of the
+// rest per thread.  Two sweeps over registers instead of a running maximum: one exponential per
+// element.
+template <typename T, int NV>
+struct Held {
+    static constexpr int VEC = wide_vec<T>();
+    Pack<T, VEC> v[NV];
+    T tail;
+    int nvec, ntail;  // vectors of the row, elements after them
+
+    template <int TPR>
+    __device__ __forceinline__ void load(const T* x, int cols, int t) {
+        nvec = cols / VEC;
+        ntail = cols - nvec * VEC;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i * TPR + t < nvec) v[i] = pload<T, VEC>(x + int64_t(i * TPR + t) * VEC);
+        if (t < ntail) tail = x[nvec * VEC + t];
+    }
+
+    template <int TPR>
+    __device__ __forceinline__ void reduce(int t, wide_t<T>& m, wide_t<T>& s) const {
+        using A = wide_t<T>;
+        m = -A(__builtin_inf());
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i * TPR + t < nvec) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) m = max_of(m, A(v[i].v[e]));
+            }
+        if (t < ntail) m = max_of(m, A(tail));
+        const A base = base_of(m);
+        s = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i * TPR + t < nvec) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s += exp_diff(A(v[i].v[e]) - base);
+            }
+        if (t < ntail) s += exp_diff(A(tail) - base);
+    }
+
+    template <int TPR>
+    __device__ __forceinline__ void store_grad(T* g, int t, int act,
+                                               const RowGrad<wide_t<T>>& rg) const {
+        using A = wide_t<T>;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = (i * TPR + t) * VEC;
+            if (i * TPR + t < nvec) pstore<T, VEC>(g + j, grad_of<T, VEC>(v[i], rg, act - j));
+        }
+        if (t < ntail) {
+            const int j = nvec * VEC + t;
+            g[j] = T(j == act ? rg.own : exp_diff(A(tail) - rg.m) * rg.k);
+        }
+    }
+
+    template <int TPR>
+    __device__ __forceinline__ void store_zero(T* g, int cols, int t) const {
+        const int n = cols / VEC;
+        const Pack<T, VEC> z{};
+        for (int i = t; i < n; i += TPR) pstore<T, VEC>(g + int64_t(i) * VEC, z);
+        if (t < cols - n * VEC) g[int64_t(n) * VEC + t] = T(0);
+    }
+};
+
+constexpr int kRowBlock = 256;
+
+// ---- short rows: TPR lanes (16 or 64) of a wave per row, several rows per workgroup, no LDS.
+template <typename T, int TPR, int NV, typename Op>
+__global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op) {
+    using A = wide_t<T>;
+    const int64_t n = int64_t(blockIdx.x) * (kRowBlock / TPR) + threadIdx.x / TPR;
+    if (n >= a.rows) return;
+    const int t = threadIdx.x % TPR;
+    const int64_t act = a.actions[n];
+    const T* x = a.x + n * a.stride;
+    const RowInputs in = op.load(n);
+    const A xa = action_logit(a, x, act);
+    Held<T, NV> row;
+    row.template load<TPR>(x, int(a.cols), t);
+    A m, s;
+    row.template reduce<TPR>(t, m, s);
+    join_lanes<TPR>(m, s);
+    finish_row<TPR>(a, op, n, act, xa, in, m, s, t == 0);
+}
+
+// ---- a row per workgroup, read once with a running maximum and sum; ignored rows are not read.
+constexpr int kStreamUnroll = 4;  // vectors in flight per thread
+
+// Vectors lo..hi-1 of a row, and the elements after its last whole vector with `tail`.
+template <typename T>
+__device__ __forceinline__ void stream_part(const T* x, int cols, int lo, int hi, bool tail,
+                                            wide_t<T>& m, wide_t<T>& s) {
+    using A = wide_t<T>;
+    constexpr int VEC = wide_vec<T>(), U = kStreamUnroll;
+    m = -A(__builtin_inf());
+    s = 0;
+    for (int i = lo + int(threadIdx.x); i < hi; i += U * kRowBlock) {
+        Pack<T, VEC> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * kRowBlock < hi) v[u] = pload<T, VEC>(x + int64_t(i + u * kRowBlock) * VEC);
+        A top = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * kRowBlock < hi) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) top = max_of(top, A(v[u].v[e]));
+            }
+        const A base = base_of(top);
+        A add = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i + u * kRowBlock < hi) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) add += exp_diff(A(v[u].v[e]) - base);
+            }
+        s = s * exp_diff(m - base) + add;
+        m = top;
+    }
+    const int whole = cols / VEC * VEC;
+    if (tail && int(threadIdx.x) < cols - whole) {
+        const A v = A(x[whole + threadIdx.x]), top = max_of(m, v), base = base_of(top);
+        s = s * exp_diff(m - base) + exp_diff(v - base);
+        m = top;
+    }
 }
 
 template <typename T, typename Op>
-__global__ __launch_bounds__(kRowThreads) void k_rows(RowArgs<T> a, Op op) {
+__global__ __launch_bounds__(kRowBlock) void k_rows_stream(RowArgs<T> a, Op op) {
     using A = wide_t<T>;
-    __shared__ A sm[kRowThreads], ss[kRowThreads];
+    __shared__ A part[kRowBlock / 64][2];
     const int64_t n = blockIdx.x;
-    const T* x = a.x + n * a.stride;
-    A m = -A(__builtin_inf()), s = 0;
-    for (int64_t j = threadIdx.x; j < a.cols; j += kRowThreads) join(m, s, A(x[j]), A(1));
-    sm[threadIdx.x] = m;
-    ss[threadIdx.x] = s;
-    __syncthreads();
-    for (int h = kRowThreads / 2; h > 0; h >>= 1) {
-        if (int(threadIdx.x) < h)
-            join(sm[threadIdx.x], ss[threadIdx.x], sm[threadIdx.x + h], ss[threadIdx.x + h]);
-        __syncthreads();
+    const int64_t act = a.actions[n];
+    A m = 0, s = 1, xa = 0;
+    RowInputs in{};
+    if (act != a.ignore) {
+        const T* x = a.x + n * a.stride;
+        in = op.load(n);
+        xa = action_logit(a, x, act);
+        stream_part<T>(x, int(a.cols), 0, int(a.cols) / wide_vec<T>(), true, m, s);
+        join_waves<kRowBlock / 64>(m, s, part);
     }
-    if (threadIdx.x == 0) finish_row(a, op, n, sm[0], ss[0]);
+    if (wave_id() == 0) finish_row<64>(a, op, n, act, xa, in, m, s, lane_id() == 0);
+}
+
+// ---- few long rows: (row, part) workgroups, the parts joined by one wave per row.
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_rows_split(RowArgs<T> a, int parts, int per,
+                                                          wide_t<T>* __restrict__ ws) {
+    using A = wide_t<T>;
+    __shared__ A part[kRowBlock / 64][2];
+    const int64_t n = blockIdx.y;
+    const int p = blockIdx.x;
+    if (a.actions[n] == a.ignore) return;
+    const int nvec = int(a.cols) / wide_vec<T>();
+    A m, s;
+    stream_part<T>(a.x + n * a.stride, int(a.cols), p * per, std::min(nvec, (p + 1) * per),
+                   p == parts - 1, m, s);
+    join_waves<kRowBlock / 64>(m, s, part);
+    if (threadIdx.x == 0) {
+        ws[(n * parts + p) * 2] = m;
+        ws[(n * parts + p) * 2 + 1] = s;
+    }
+}
+
+template <typename T, typename Op>
+__global__ __launch_bounds__(kRowBlock) void k_rows_joined(RowArgs<T> a, Op op, int parts,
+                                                           const wide_t<T>* __restrict__ ws) {
+    using A = wide_t<T>;
+    const int64_t n = int64_t(blockIdx.x) * (kRowBlock / 64) + wave_id();
+    if (n >= a.rows) return;
+    const int64_t act = a.actions[n];
+    A m = -A(__builtin_inf()), s = 0, xa = 0;
+    RowInputs in{};
+    if (act != a.ignore) {
+        in = op.load(n);
+        xa = action_logit(a, a.x + n * a.stride, act);
+        if (lane_id() < parts) {
+            m = ws[(n * parts + lane_id()) * 2];
+            s = ws[(n * parts + lane_id()) * 2 + 1];
+        }
+        join_lanes<64>(m, s);
+    }
+    finish_row<64>(a, op, n, act, xa, in, m, s, lane_id() == 0);
 }
 
 // ---- the upstream gradient of a row's slope
@@ -179,36 +465,62 @@ struct Upstream {
     }
 };
 
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void k_logit_grad(RowArgs<T> a, Upstream<wide_t<T>> up,
-                                                            T* __restrict__ grad) {
+// Rows whose slope is 0 are written without being read: ignored, clipped, or of no sequence.
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(kRowBlock) void k_grad_short(RowArgs<T> a, Upstream<wide_t<T>> up,
+                                                          T* __restrict__ grad) {
     using A = wide_t<T>;
-    const int64_t n = blockIdx.x;
+    const int64_t n = int64_t(blockIdx.x) * (kRowBlock / TPR) + threadIdx.x / TPR;
+    if (n >= a.rows) return;
+    const int t = threadIdx.x % TPR;
     const RowState<A> st = a.state[n];
-    const A c = up(n, st.slope);
     const int64_t act = a.actions[n];
-    const T* x = a.x + n * a.stride;
+    const A c = up(n, st.slope);
     T* g = grad + n * a.cols;
-    for (int64_t j = threadIdx.x; j < a.cols; j += kRowThreads) {
-        A v = 0;
-        if (c != A(0)) v = j == act ? c * st.rest : -c * (exp(A(x[j]) - st.m) * st.inv_s);
-        g[j] = T(v);
+    Held<T, NV> row;
+    if (c == A(0)) {
+        row.template store_zero<TPR>(g, int(a.cols), t);
+        return;
     }
+    row.template load<TPR>(a.x + n * a.stride, int(a.cols), t);
+    row.template store_grad<TPR>(g, t, action_place(a, act), RowGrad<A>(st, c));
+}
+
+constexpr int kGradVecs = 4;  // vectors per thread
+
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_grad_long(RowArgs<T> a, Upstream<wide_t<T>> up,
+                                                         T* __restrict__ grad, uint32_t chunks) {
+    using A = wide_t<T>;
+    constexpr int VEC = wide_vec<T>();
+    constexpr int CHUNK = kRowBlock * kGradVecs * VEC;
+    const int64_t n = blockIdx.x / chunks;
+    const int64_t j0 = int64_t(blockIdx.x % chunks) * CHUNK;
+    const int cols = int(std::min<int64_t>(CHUNK, a.cols - j0));
+    const RowState<A> st = a.state[n];
+    const int64_t act = a.actions[n];
+    const A c = up(n, st.slope);
+    T* g = grad + n * a.cols + j0;
+    Held<T, kGradVecs> row;
+    if (c == A(0)) {
+        row.template store_zero<kRowBlock>(g, cols, threadIdx.x);
+        return;
+    }
+    row.template load<kRowBlock>(a.x + n * a.stride + j0, cols, threadIdx.x);
+    row.template store_grad<kRowBlock>(g, threadIdx.x, action_place(a, act) - int(j0),
+                                       RowGrad<A>(st, c));
 }
 
 // ---- sums in a fixed order by one workgroup, in fp64
 constexpr int kSumThreads = 1024;
 
+// Over the workgroup, by lanes and then waves; the result in every thread of wave 0.
 __device__ __forceinline__ double group_sum(double v, double* red) {
-    red[threadIdx.x] = v;
+    v = wave_total(v);
+    if (lane_id() == 0) red[wave_id()] = v;
     __syncthreads();
-    for (int h = int(blockDim.x) / 2; h > 0; h >>= 1) {
-        if (int(threadIdx.x) < h) red[threadIdx.x] += red[threadIdx.x + h];
-        __syncthreads();
-    }
-    const double r = red[0];
-    __syncthreads();
-    return r;
+    const int waves = int(blockDim.x) >> 6;
+    return wave_total(lane_id() < waves ? red[lane_id()] : 0.0);
 }
 
 // loss = sum of the rows' terms, divided by the number of counted rows for a mean.
@@ -218,60 +530,75 @@ __global__ __launch_bounds__(kSumThreads) void k_policy_sum(const A* __restrict_
                                                             int64_t rows, int64_t ignore, int mean,
                                                             A* __restrict__ loss,
                                                             A* __restrict__ count) {
-    __shared__ double red[kSumThreads];
+    __shared__ double red[2][kSumThreads / 64];
     double t = 0, c = 0;
     for (int64_t n = threadIdx.x; n < rows; n += kSumThreads) {
         t += double(terms[n]);
         c += actions[n] != ignore ? 1.0 : 0.0;
     }
-    t = group_sum(t, red);
-    c = group_sum(c, red);
+    t = group_sum(t, red[0]);
+    c = group_sum(c, red[1]);
     if (threadIdx.x == 0) {
         loss[0] = A(mean ? t / c : t);  // no counted row: 0 / 0 = NaN, the mean of nothing
         count[0] = A(c);
     }
 }
 
-// One workgroup per pair: the sums over both sequences, the margin h, the loss term
+template <typename A>
+struct PairArgs {
+    const double* gaps;
+    const int64_t* offsets;
+    int64_t rows, pairs;
+    double beta, smooth;
+    int32_t* row_seq;
+    A* seq_slope;
+    A* margins;
+    A* terms;
+};
+
+// Pair i by one wave: the sums over both sequences, the margin h, the loss term
 //   -(1 - e) log sigma(h) - e log sigma(-h)
 // and its slope by the chosen sequence's sum; the rejected one's is the negative.
 template <typename A>
-__global__ __launch_bounds__(kRowThreads) void k_pref_pairs(const double* __restrict__ gaps,
-                                                            const int64_t* __restrict__ offsets,
-                                                            int64_t rows, int64_t pairs,
-                                                            double beta, double smooth,
-                                                            int32_t* __restrict__ row_seq,
-                                                            A* __restrict__ seq_slope,
-                                                            A* __restrict__ margins,
-                                                            A* __restrict__ terms) {
-    __shared__ double red[kRowThreads];
-    const int64_t i = blockIdx.x;
+__device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i) {
     double d[2];
     bool bad = false;
+#pragma unroll
     for (int side = 0; side < 2; ++side) {
-        const int64_t q = i + side * pairs;
-        int64_t b = offsets[q], e = offsets[q + 1];
-        bad |= b < 0 || e < b || e > rows;
-        b = std::min(std::max<int64_t>(b, 0), rows);
-        e = std::min(std::max(e, b), rows);
+        const int64_t q = i + side * a.pairs;
+        int64_t b = a.offsets[q], e = a.offsets[q + 1];
+        bad |= b < 0 || e < b || e > a.rows;
+        b = std::min(std::max<int64_t>(b, 0), a.rows);
+        e = std::min(std::max(e, b), a.rows);
         double t = 0;
-        for (int64_t n = b + threadIdx.x; n < e; n += kRowThreads) {
-            t += gaps[n];
-            row_seq[n] = int32_t(q);
+        for (int64_t n = b + lane_id(); n < e; n += 64) {
+            t += a.gaps[n];
+            a.row_seq[n] = int32_t(q);
         }
-        d[side] = group_sum(t, red);
+        d[side] = wave_total(t);
     }
-    if (threadIdx.x != 0) return;
-    double h = beta * (d[0] - d[1]);
+    double h = a.beta * (d[0] - d[1]);
     if (bad) h = nan_value<double>();
-    const double tail = log1p(exp(-fabs(h)));
-    const double away = tail - (h < 0 ? h : 0.0);  // -log sigma(h)
-    const double near = tail + (h > 0 ? h : 0.0);  // -log sigma(-h)
-    const double slope = beta * (smooth / (1 + exp(-h)) - (1 - smooth) / (1 + exp(h)));
-    margins[i] = A(h);
-    terms[i] = A((1 - smooth) * away + smooth * near);
-    seq_slope[i] = A(slope);
-    seq_slope[i + pairs] = A(-slope);
+    // with u = exp(-|h|): log sigma(h) = min(h, 0) - log(1 + u), sigma(h) = 1 / (1 + u) or
+    // u / (1 + u)
+    const double u = exp(-fabs(h)), tail = log1p(u), inv = 1.0 / (1.0 + u);
+    const double away = tail - (h < 0 ? h : 0.0), near = tail + (h > 0 ? h : 0.0);
+    const double yes = h >= 0 ? inv : u * inv, no = h >= 0 ? u * inv : inv;  // sigma(h), sigma(-h)
+    const double slope = a.beta * (a.smooth * yes - (1 - a.smooth) * no);
+    const double term = (1 - a.smooth) * away + a.smooth * near;
+    if (lane_id() == 0) {
+        a.margins[i] = A(h);
+        a.terms[i] = A(term);
+        a.seq_slope[i] = A(slope);
+        a.seq_slope[i + a.pairs] = A(-slope);
+    }
+    return double(A(term));
+}
+
+template <typename A>
+__global__ __launch_bounds__(kRowBlock) void k_pref_pairs(PairArgs<A> a) {
+    const int64_t i = int64_t(blockIdx.x) * (kRowBlock / 64) + wave_id();
+    if (i < a.pairs) pair_term(a, i);
 }
 
 template <typename A>
@@ -279,13 +606,32 @@ __global__ __launch_bounds__(kSumThreads) void k_pref_sum(const A* __restrict__ 
                                                           int64_t pairs, int mean,
                                                           A* __restrict__ loss,
                                                           A* __restrict__ count) {
-    __shared__ double red[kSumThreads];
+    __shared__ double red[kSumThreads / 64];
     double t = 0;
     for (int64_t i = threadIdx.x; i < pairs; i += kSumThreads) t += double(terms[i]);
     t = group_sum(t, red);
     if (threadIdx.x == 0) {
         loss[0] = A(mean ? t / double(pairs) : t);
         count[0] = A(pairs);
+    }
+}
+
+// Both in one launch, for batches of few rows: 16 waves take the pairs in turn.
+template <typename A>
+__global__ __launch_bounds__(kSumThreads) void k_pref_small(PairArgs<A> a, int mean,
+                                                            A* __restrict__ loss,
+                                                            A* __restrict__ count) {
+    __shared__ double red[kSumThreads / 64];
+    double t = 0;
+    for (int64_t i = wave_id(); i < a.pairs; i += kSumThreads / 64) {
+        const double term = pair_term(a, i);
+        t += lane_id() == 0 ? term : 0.0;
+    }
+    if (!loss) return;
+    t = group_sum(t, red);
+    if (threadIdx.x == 0) {
+        loss[0] = A(mean ? t / double(a.pairs) : t);
+        count[0] = A(a.pairs);
     }
 }
 
@@ -314,16 +660,84 @@ RowArgs<T> row_args(const void* logits, int64_t row_stride, int64_t rows, int64_
     return a;
 }
 
-template <typename T, typename Op>
-void launch_rows(const RowArgs<T>& a, const Op& op, hipStream_t s) {
-    if (a.rows > 0) k_rows<T, Op><<<unsigned(a.rows), kRowThreads, 0, s>>>(a, op);
+// Rows up to 4 KB stay in registers of a wave or a quarter of one; longer ones take a workgroup,
+// or several where the rows alone would not fill the card.
+constexpr int64_t kPrefSmallRows = 16384, kPrefSmallPairs = 256;
+constexpr int64_t kSplitBlocks = 1024;  // workgroups wanted
+constexpr int kMaxParts = 64;           // joined by the lanes of one wave
+
+template <typename T>
+int row_parts(int64_t rows, int64_t cols) {
+    const int64_t per_block = int64_t(kRowBlock) * kStreamUnroll;  // vectors of one sweep
+    const int64_t nvec = cols / wide_vec<T>();
+    if (rows <= 0 || rows > kSplitBlocks / 2 || nvec < 2 * per_block) return 1;
+    return int(std::min<int64_t>(std::min<int64_t>(nvec / per_block, kMaxParts),
+                                 ceil_div(kSplitBlocks, rows)));
 }
 
 template <typename T>
-void launch_logit_grad(const RowArgs<T>& a, const Upstream<wide_t<T>>& up, void* grad,
-                       hipStream_t s) {
-    if (a.rows > 0)
-        k_logit_grad<T><<<unsigned(a.rows), kRowThreads, 0, s>>>(a, up, static_cast<T*>(grad));
+int64_t rows_workspace(int64_t rows, int64_t cols) {
+    const int parts = row_parts<T>(rows, cols);
+    return parts > 1 ? rows * parts * 2 * int64_t(sizeof(wide_t<T>)) : 0;
+}
+
+template <typename T, int TPR, int NV, typename Op>
+void launch_rows_short(const RowArgs<T>& a, const Op& op, hipStream_t s) {
+    k_rows_short<T, TPR, NV, Op>
+        <<<unsigned(ceil_div(a.rows, kRowBlock / TPR)), kRowBlock, 0, s>>>(a, op);
+}
+
+template <typename T, typename Op>
+int launch_rows(const RowArgs<T>& a, const Op& op, void* workspace, int64_t workspace_bytes,
+                hipStream_t s) {
+    if (a.rows == 0) return CL_OK;
+    const int64_t bytes = a.cols * int64_t(sizeof(T));
+    const int parts = row_parts<T>(a.rows, a.cols);
+    if (bytes <= 256) {
+        launch_rows_short<T, 16, 1>(a, op, s);
+    } else if (bytes <= 1024) {
+        launch_rows_short<T, 64, 1>(a, op, s);
+    } else if (bytes <= 4096) {
+        launch_rows_short<T, 64, 4>(a, op, s);
+    } else if (parts > 1) {
+        CL_ARG(workspace && workspace_bytes >= rows_workspace<T>(a.rows, a.cols),
+               "workspace of %lld bytes needed (cl_token_loss_workspace)",
+               (long long)rows_workspace<T>(a.rows, a.cols));
+        auto* ws = static_cast<wide_t<T>*>(workspace);
+        const int per = int(ceil_div(a.cols / wide_vec<T>(), parts));
+        k_rows_split<T><<<dim3(unsigned(parts), unsigned(a.rows)), kRowBlock, 0, s>>>(a, parts,
+                                                                                    per, ws);
+        if (int rc = check_launch("row parts")) return rc;
+        k_rows_joined<T, Op><<<unsigned(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
+            a, op, parts, ws);
+    } else {
+        k_rows_stream<T, Op><<<unsigned(a.rows), kRowBlock, 0, s>>>(a, op);
+    }
+    return check_launch("rows");
+}
+
+template <typename T>
+int launch_logit_grad(const RowArgs<T>& a, const Upstream<wide_t<T>>& up, void* grad,
+                      hipStream_t s) {
+    if (a.rows == 0) return CL_OK;
+    const int64_t bytes = a.cols * int64_t(sizeof(T));
+    T* g = static_cast<T*>(grad);
+    if (bytes <= 256) {
+        k_grad_short<T, 16, 1><<<unsigned(ceil_div(a.rows, kRowBlock / 16)), kRowBlock, 0, s>>>(
+            a, up, g);
+    } else if (bytes <= 1024) {
+        k_grad_short<T, 64, 1><<<unsigned(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
+            a, up, g);
+    } else if (bytes <= 4096) {
+        k_grad_short<T, 64, 4><<<unsigned(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
+            a, up, g);
+    } else {
+        const int64_t chunks = ceil_div(a.cols, kRowBlock * kGradVecs * wide_vec<T>());
+        CL_ARG(a.rows * chunks < (int64_t(1) << 31), "too many logits for one call");
+        k_grad_long<T><<<unsigned(a.rows * chunks), kRowBlock, 0, s>>>(a, up, g,
+                                                                      uint32_t(chunks));
+    }
+    return check_launch("logit gradient");
 }
 
 }  // namespace
@@ -331,9 +745,19 @@ void launch_logit_grad(const RowArgs<T>& a, const Upstream<wide_t<T>>& up, void*
 
 using namespace cl;
 
+extern "C" int cl_token_loss_workspace(int dtype, int64_t rows, int64_t cols, int64_t* bytes) {
+    clear_error();
+    CL_ARG(bytes, "null pointer argument");
+    CL_ARG(rows >= 0 && rows < (int64_t(1) << 31) && cols >= 1 && cols < (int64_t(1) << 31),
+           "bad shape");
+    CL_STORAGE_SWITCH(dtype, { *bytes = rows_workspace<scalar_t>(rows, cols); });
+    return CL_OK;
+}
+
 extern "C" int cl_selected_log_prob_forward(int dtype, const void* logits, int64_t row_stride,
                                             int64_t rows, int64_t cols, const int64_t* actions,
                                             int64_t ignore_index, void* log_probs, void* row_state,
+                                            void* workspace, int64_t workspace_bytes,
                                             void* stream) {
     clear_error();
     if (int rc = check_logits(logits, row_stride, rows, cols, actions, row_state)) return rc;
@@ -341,11 +765,10 @@ extern "C" int cl_selected_log_prob_forward(int dtype, const void* logits, int64
     if (rows == 0) return CL_OK;
     CL_STORAGE_SWITCH(dtype, {
         using T = scalar_t;
-        launch_rows(row_args<T>(logits, row_stride, rows, cols, actions, ignore_index, log_probs,
-                                row_state),
-                    LogProbOp<wide_t<T>>{}, as_stream(stream));
+        return launch_rows(row_args<T>(logits, row_stride, rows, cols, actions, ignore_index,
+                                       log_probs, row_state),
+                           LogProbOp<wide_t<T>>{}, workspace, workspace_bytes, as_stream(stream));
     });
-    return check_launch("cl_selected_log_prob_forward");
 }
 
 extern "C" int cl_selected_log_prob_backward(int dtype, const void* logits, int64_t row_stride,
@@ -361,11 +784,10 @@ extern "C" int cl_selected_log_prob_backward(int dtype, const void* logits, int6
         using A = wide_t<T>;
         Upstream<A> up{};
         up.rows = static_cast<const A*>(grad_log_probs);
-        launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
+        return launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
                                       row_state),
                           up, grad_logits, as_stream(stream));
     });
-    return check_launch("cl_selected_log_prob_backward");
 }
 
 extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row_stride,
@@ -374,7 +796,8 @@ extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row
                                       const void* advantages, const void* ref_log_probs,
                                       double clip_low, double clip_high, double kl_coef,
                                       int reduction, void* log_probs, void* row_state,
-                                      void* terms, void* loss, void* count, void* stream) {
+                                      void* terms, void* loss, void* count, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
     clear_error();
     if (int rc = check_logits(logits, row_stride, rows, cols, actions, row_state)) return rc;
     CL_ARG(rows == 0 || (old_log_probs && advantages && log_probs && terms),
@@ -396,10 +819,10 @@ extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row
         op.high = 1.0 + clip_high;
         op.kl = kl_coef;
         op.terms = static_cast<A*>(terms);
-        launch_rows(row_args<T>(logits, row_stride, rows, cols, actions, ignore_index, log_probs,
-                                row_state),
-                    op, s);
-        if (int rc = check_launch("cl_policy_loss_forward(rows)")) return rc;
+        if (int rc = launch_rows(row_args<T>(logits, row_stride, rows, cols, actions,
+                                             ignore_index, log_probs, row_state),
+                                 op, workspace, workspace_bytes, s))
+            return rc;
         if (reduction != CL_REDUCE_NONE)
             k_policy_sum<A><<<1, kSumThreads, 0, s>>>(op.terms, actions, rows, ignore_index,
                                                       reduction == CL_REDUCE_MEAN,
@@ -429,11 +852,10 @@ extern "C" int cl_policy_loss_backward(int dtype, const void* logits, int64_t ro
         else
             up.scalar = static_cast<const A*>(grad_loss);
         if (reduction == CL_REDUCE_MEAN) up.count = static_cast<const A*>(count);
-        launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
+        return launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
                                       row_state),
                           up, grad_logits, as_stream(stream));
     });
-    return check_launch("cl_policy_loss_backward");
 }
 
 extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t row_stride,
@@ -443,7 +865,8 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
                                           double label_smoothing, int reduction, void* log_probs,
                                           void* row_state, double* gaps, int32_t* row_seq,
                                           void* seq_slope, void* margins, void* terms, void* loss,
-                                          void* count, void* stream) {
+                                          void* count, void* workspace, int64_t workspace_bytes,
+                                          void* stream) {
     clear_error();
     if (int rc = check_logits(logits, row_stride, rows, cols, actions, row_state)) return rc;
     CL_ARG(rows == 0 || (log_probs && gaps && row_seq), "null pointer argument");
@@ -458,19 +881,26 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
         using T = scalar_t;
         using A = wide_t<T>;
         PreferenceOp<A> op{static_cast<const A*>(ref_log_probs), gaps, row_seq};
-        launch_rows(row_args<T>(logits, row_stride, rows, cols, actions, ignore_index, log_probs,
-                                row_state),
-                    op, s);
-        if (int rc = check_launch("cl_preference_loss_forward(rows)")) return rc;
+        if (int rc = launch_rows(row_args<T>(logits, row_stride, rows, cols, actions,
+                                             ignore_index, log_probs, row_state),
+                                 op, workspace, workspace_bytes, s))
+            return rc;
+        const PairArgs<A> pa{gaps, offsets, rows, pairs, beta, label_smoothing, row_seq,
+                             static_cast<A*>(seq_slope), static_cast<A*>(margins),
+                             static_cast<A*>(terms)};
+        const int mean = reduction == CL_REDUCE_MEAN;
+        A* out = reduction != CL_REDUCE_NONE ? static_cast<A*>(loss) : nullptr;
+        if (rows <= kPrefSmallRows && pairs <= kPrefSmallPairs) {
+            if (pairs > 0 || out)
+                k_pref_small<A><<<1, kSumThreads, 0, s>>>(pa, mean, out, static_cast<A*>(count));
+            return check_launch("cl_preference_loss_forward(pairs)");
+        }
         if (pairs > 0)
-            k_pref_pairs<A><<<unsigned(pairs), kRowThreads, 0, s>>>(
-                gaps, offsets, rows, pairs, beta, label_smoothing, row_seq,
-                static_cast<A*>(seq_slope), static_cast<A*>(margins), static_cast<A*>(terms));
+            k_pref_pairs<A><<<unsigned(ceil_div(pairs, kRowBlock / 64)), kRowBlock, 0, s>>>(pa);
         if (int rc = check_launch("cl_preference_loss_forward(pairs)")) return rc;
-        if (reduction != CL_REDUCE_NONE)
-            k_pref_sum<A><<<1, kSumThreads, 0, s>>>(static_cast<const A*>(terms), pairs,
-                                                    reduction == CL_REDUCE_MEAN,
-                                                    static_cast<A*>(loss), static_cast<A*>(count));
+        if (out)
+            k_pref_sum<A><<<1, kSumThreads, 0, s>>>(static_cast<const A*>(terms), pairs, mean, out,
+                                                    static_cast<A*>(count));
     });
     return check_launch("cl_preference_loss_forward(sum)");
 }
@@ -502,9 +932,8 @@ extern "C" int cl_preference_loss_backward(int dtype, const void* logits, int64_
         else
             up.scalar = static_cast<const A*>(grad_loss);
         if (reduction == CL_REDUCE_MEAN) up.count = static_cast<const A*>(count);
-        launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
+        return launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
                                       row_state),
                           up, grad_logits, as_stream(stream));
     });
-    return check_launch("cl_preference_loss_backward");
 }

@@ -14,6 +14,8 @@ logits' range gives NaN, as a label does in GroupSum.cross_entropy.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _capi
@@ -39,7 +41,8 @@ def _flat(logits, actions):
         raise RuntimeError(f"actions must be int64 of shape {tuple(logits.shape[:-1])}")
     if logits.dim() != 2:
         logits = logits.reshape(-1, logits.shape[-1])
-    return logits, actions.reshape(-1).contiguous()
+        actions = actions.reshape(-1)
+    return logits, actions.contiguous()
 
 
 def _per_row(t, name, logits, actions):
@@ -51,7 +54,9 @@ def _per_row(t, name, logits, actions):
                            f"{tuple(actions.shape)} on {logits.device}")
     if t.requires_grad:
         raise RuntimeError(f"{name} is a constant of the loss: detach it")
-    return t.reshape(-1).to(_wide(logits)).contiguous()
+    if t.dim() != 1:
+        t = t.reshape(-1)
+    return t.to(_wide(logits)).contiguous()
 
 
 def _reduction(name):
@@ -67,10 +72,19 @@ def _rows_of(logits):
     return logits
 
 
-def _args(logits):
-    """The leading arguments of every entry point (an expanded row has stride 0)."""
-    return (_dl.storage_dtype_code(logits), logits.data_ptr(), logits.stride(0),
-            logits.shape[0], logits.shape[1])
+class _Shape:
+    """One call's logits as the entry points take them, and the bytes of its buffers."""
+
+    def __init__(self, logits):
+        self.code = _dl.storage_dtype_code(logits)
+        self.rows, self.cols = logits.shape
+        # (an expanded row has stride 0)
+        self.args = (self.code, logits.data_ptr(), logits.stride(0), self.rows, self.cols)
+        self.size = 8 if logits.dtype == torch.float64 else 4
+        self.state_bytes = 4 * self.size * self.rows
+        need = ctypes.c_int64()
+        _capi.call("cl_token_loss_workspace", self.code, self.rows, self.cols, ctypes.byref(need))
+        self.workspace_bytes = need.value
 
 
 def _once():
@@ -80,8 +94,16 @@ def _once():
         raise RuntimeError("the losses on chosen log-probabilities cannot be differentiated twice")
 
 
-def _state(logits):
-    return torch.empty((logits.shape[0], 4), dtype=_wide(logits), device=logits.device)
+def _aux(logits, *sizes):
+    """One buffer for everything a call keeps to itself, and the addresses of its parts, 16 bytes
+    or a multiple apart: allocations cost a small call more than its kernels."""
+    total, starts = 0, []
+    for n in sizes:
+        starts.append(total)
+        total += (n + 31) & ~31
+    buf = torch.empty(max(total, 32), dtype=torch.uint8, device=logits.device)
+    base = buf.data_ptr()
+    return buf, [base + s for s in starts]
 
 
 class SelectedLogProbsFunction(torch.autograd.Function):
@@ -91,25 +113,27 @@ class SelectedLogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, ignore_index):
         logits = _rows_of(logits)
-        state = _state(logits)
-        lp = torch.empty(logits.shape[0], dtype=state.dtype, device=logits.device)
+        sh = _Shape(logits)
+        aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+        lp = torch.empty(sh.rows, dtype=_wide(logits), device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_selected_log_prob_forward", lambda: _capi.call(
-                "cl_selected_log_prob_forward", *_args(logits), actions.data_ptr(), ignore_index,
-                lp.data_ptr(), state.data_ptr(), _dl.stream_of(logits)))
-        ctx.save_for_backward(logits, actions, state)
+                "cl_selected_log_prob_forward", *sh.args, actions.data_ptr(), ignore_index,
+                lp.data_ptr(), state, ws, sh.workspace_bytes, _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, aux)
+        ctx.args, ctx.state = sh.args, state
         return lp
 
     @staticmethod
     def backward(ctx, grad_lp):
         _once()
-        logits, actions, state = ctx.saved_tensors
+        logits, actions, aux = ctx.saved_tensors
         grad_lp = grad_lp.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_selected_log_prob_backward", lambda: _capi.call(
-                "cl_selected_log_prob_backward", *_args(logits), actions.data_ptr(),
-                state.data_ptr(), grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits)))
+                "cl_selected_log_prob_backward", *ctx.args, actions.data_ptr(), ctx.state,
+                grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits)))
         return grad, None, None
 
 
@@ -122,36 +146,42 @@ class PolicyLossFunction(torch.autograd.Function):
     def forward(ctx, logits, actions, old, adv, ref, clip_low, clip_high, kl_coef, ignore_index,
                 reduction):
         logits = _rows_of(logits)
-        state = _state(logits)
-        rows, dev, wide = logits.shape[0], logits.device, state.dtype
-        lp = torch.empty(rows, dtype=wide, device=dev)
-        terms = torch.empty(rows, dtype=wide, device=dev)
-        scalars = torch.empty(2, dtype=wide, device=dev) if reduction else None
-        loss, count = scalars.unbind() if reduction else (None, None)
+        sh = _Shape(logits)
+        wide = old.dtype
+        lp = torch.empty(sh.rows, dtype=wide, device=logits.device)
+        if reduction:
+            loss = torch.empty((), dtype=wide, device=logits.device)
+            aux, (state, count, terms, ws) = _aux(logits, sh.state_bytes, sh.size,
+                                                  sh.rows * sh.size, sh.workspace_bytes)
+            loss_at = loss.data_ptr()
+        else:
+            loss = torch.empty(sh.rows, dtype=wide, device=logits.device)
+            aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+            terms, loss_at, count = loss.data_ptr(), None, None
         with _dl.on_device_of(logits):
             timing.timed("cl_policy_loss_forward", lambda: _capi.call(
-                "cl_policy_loss_forward", *_args(logits), actions.data_ptr(), ignore_index,
+                "cl_policy_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
                 old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
-                reduction, lp.data_ptr(), state.data_ptr(), terms.data_ptr(), _dl.ptr(loss),
-                _dl.ptr(count), _dl.stream_of(logits)))
-        ctx.save_for_backward(logits, actions, state, count)
-        ctx.reduction = reduction
+                reduction, lp.data_ptr(), state, terms, loss_at, count, ws, sh.workspace_bytes,
+                _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, aux)
+        ctx.args, ctx.state, ctx.count, ctx.reduction = sh.args, state, count, reduction
         ctx.mark_non_differentiable(lp)
         ctx.set_materialize_grads(False)
-        return (loss if reduction else terms), lp
+        return loss, lp
 
     @staticmethod
     def backward(ctx, grad_loss, _grad_lp):
         _once()
         if grad_loss is None:
             return (None,) * 10
-        logits, actions, state, count = ctx.saved_tensors
+        logits, actions, aux = ctx.saved_tensors
         grad_loss = grad_loss.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_policy_loss_backward", lambda: _capi.call(
-                "cl_policy_loss_backward", *_args(logits), actions.data_ptr(), state.data_ptr(),
-                ctx.reduction, grad_loss.data_ptr(), _dl.ptr(count), grad.data_ptr(),
+                "cl_policy_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
+                ctx.reduction, grad_loss.data_ptr(), ctx.count, grad.data_ptr(),
                 _dl.stream_of(logits)))
         return (grad,) + (None,) * 9
 
@@ -164,44 +194,42 @@ class PreferenceLossFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, offsets, ref, beta, smoothing, ignore_index, reduction):
         logits = _rows_of(logits)
-        state = _state(logits)
-        rows, dev, wide = logits.shape[0], logits.device, state.dtype
-        pairs = (offsets.numel() - 1) // 2
-        lp = torch.empty(rows, dtype=wide, device=dev)
-        gaps = torch.empty(rows, dtype=torch.float64, device=dev)
-        row_seq = torch.empty(rows, dtype=torch.int32, device=dev)
-        seq_slope = torch.empty(2 * pairs, dtype=wide, device=dev)
-        margins = torch.empty(pairs, dtype=wide, device=dev)
-        terms = torch.empty(pairs, dtype=wide, device=dev)
-        scalars = torch.empty(2, dtype=wide, device=dev) if reduction else None
-        loss, count = scalars.unbind() if reduction else (None, None)
+        sh = _Shape(logits)
+        wide, pairs = _wide(logits), (offsets.numel() - 1) // 2
+        margins = torch.empty(pairs, dtype=wide, device=logits.device)
+        loss = torch.empty(() if reduction else (pairs,), dtype=wide, device=logits.device)
+        aux, (state, count, row_seq, seq_slope, gaps, lp, terms, ws) = _aux(
+            logits, sh.state_bytes, sh.size, 4 * sh.rows, 2 * pairs * sh.size, 8 * sh.rows,
+            sh.rows * sh.size, pairs * sh.size if reduction else 0, sh.workspace_bytes)
+        loss_at = loss.data_ptr() if reduction else None
+        if not reduction:
+            terms = loss.data_ptr()
         with _dl.on_device_of(logits):
             timing.timed("cl_preference_loss_forward", lambda: _capi.call(
-                "cl_preference_loss_forward", *_args(logits), actions.data_ptr(), ignore_index,
-                _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction,
-                lp.data_ptr(), state.data_ptr(), gaps.data_ptr(), row_seq.data_ptr(),
-                seq_slope.data_ptr(), margins.data_ptr(), terms.data_ptr(), _dl.ptr(loss),
-                _dl.ptr(count), _dl.stream_of(logits)))
-        ctx.save_for_backward(logits, actions, state, row_seq, seq_slope, count)
-        ctx.reduction, ctx.pairs = reduction, pairs
+                "cl_preference_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
+                _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction, lp, state,
+                gaps, row_seq, seq_slope, margins.data_ptr(), terms, loss_at, count, ws,
+                sh.workspace_bytes, _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, aux)
+        ctx.args, ctx.reduction, ctx.pairs = sh.args, reduction, pairs
+        ctx.state, ctx.row_seq, ctx.seq_slope, ctx.count = state, row_seq, seq_slope, count
         ctx.mark_non_differentiable(margins)
         ctx.set_materialize_grads(False)
-        return (loss if reduction else terms), margins
+        return loss, margins
 
     @staticmethod
     def backward(ctx, grad_loss, _grad_margins):
         _once()
         if grad_loss is None:
             return (None,) * 8
-        logits, actions, state, row_seq, seq_slope, count = ctx.saved_tensors
+        logits, actions, aux = ctx.saved_tensors
         grad_loss = grad_loss.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_preference_loss_backward", lambda: _capi.call(
-                "cl_preference_loss_backward", *_args(logits), actions.data_ptr(),
-                state.data_ptr(), row_seq.data_ptr(), seq_slope.data_ptr(), ctx.pairs,
-                ctx.reduction, grad_loss.data_ptr(), _dl.ptr(count), grad.data_ptr(),
-                _dl.stream_of(logits)))
+                "cl_preference_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
+                ctx.row_seq, ctx.seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(),
+                ctx.count, grad.data_ptr(), _dl.stream_of(logits)))
         return (grad,) + (None,) * 7
 
 

@@ -564,10 +564,14 @@ int cl_adam_clip_step(int dtype, int64_t num_tensors, void* const* params, void*
  * grad_logits: dtype, contiguous [rows, cols].  Sums have a fixed order: bitwise repeatable.
  * ----------------------------------------------------------------------------------------- */
 
+/* Bytes of workspace that the three forwards need for this shape (0: none). */
+int cl_token_loss_workspace(int dtype, int64_t rows, int64_t cols, int64_t* bytes);
+
 /* log_probs[n] = logits[n, a] - log sum_j exp(logits[n, j]), a = actions[n]. */
 int cl_selected_log_prob_forward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
                                  int64_t cols, const int64_t* actions, int64_t ignore_index,
-                                 void* log_probs, void* row_state, void* stream);
+                                 void* log_probs, void* row_state, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
 
 /* grad_logits[n, j] = grad_log_probs[n] * ([j == a] - softmax(logits[n])[j]). */
 int cl_selected_log_prob_backward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
@@ -585,7 +589,8 @@ int cl_policy_loss_forward(int dtype, const void* logits, int64_t row_stride, in
                            const void* old_log_probs, const void* advantages,
                            const void* ref_log_probs, double clip_low, double clip_high,
                            double kl_coef, int reduction, void* log_probs, void* row_state,
-                           void* terms, void* loss, void* count, void* stream);
+                           void* terms, void* loss, void* count, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /* Its logits' gradient.  grad_loss: a device scalar, or [rows] for CL_REDUCE_NONE.  Where the
  * clipped product is the smaller one and r lies outside the range, only the KL term has a
@@ -609,7 +614,8 @@ int cl_preference_loss_forward(int dtype, const void* logits, int64_t row_stride
                                double beta, double label_smoothing, int reduction,
                                void* log_probs, void* row_state, double* gaps, int32_t* row_seq,
                                void* seq_slope, void* margins, void* terms, void* loss,
-                               void* count, void* stream);
+                               void* count, void* workspace, int64_t workspace_bytes,
+                               void* stream);
 
 /* Its logits' gradient.  grad_loss: a device scalar, or [pairs] for CL_REDUCE_NONE. */
 int cl_preference_loss_backward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
@@ -622,7 +628,7 @@ int cl_preference_loss_backward(int dtype, const void* logits, int64_t row_strid
  * Dropout whose mask is a function of (seed, offset, row, column) and is not stored (no
  * counterpart in the reference).  Philox 4x32-10 (Salmon et al., SC'11) with key seed and
  * counter (column / 8, row, offset): its words are eight 16-bit halves, low half first, and
- * element (row, column) is dropped where half number column % 8 is below threshold (0..65536).
+ * element (row, column) is dropped where half number column % 8 is below threshold (1..65536).
  * y = fill where dropped, else x, times 65536 / (65536 - threshold) with rescale.  The gradient
  * is the same call on the gradient with fill 0.  dtype: F32, F64, F16 or BF16.  x and y
  * [rows, cols] (both below 2^32) are contiguous along the same dimension; they may be the same

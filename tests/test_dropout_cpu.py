@@ -59,7 +59,7 @@ def test_c_arguments_are_checked_before_the_device():
 
     bad = _capi.CL_ERR_INVALID_ARGUMENT
     assert rc(rows=0) == _capi.CL_OK
-    assert rc(t=65537) == bad and rc(t=-1) == bad
+    assert rc(t=65537) == bad and rc(t=0) == bad and rc(t=-1) == bad
     assert rc(rows=-1) == bad and rc(rows=2**32) == bad and rc(cols=2**32) == bad
     assert rc(x=None) == bad and rc(y=None) == bad
     assert rc(dtype=9) == bad and b"dtype" in lib.cl_last_error()
@@ -69,3 +69,4 @@ def test_c_arguments_are_checked_before_the_device():
     assert rc(ys=(7, 1)) == bad and b"overlap" in lib.cl_last_error()
     assert rc(rows=2**31, cols=2**31, xs=(2**31, 1), ys=(2**31, 1)) == bad
     assert lib.cl_dropout_next(None, None, None) == bad
+    assert rc(rows=0) == _capi.CL_OK and lib.cl_last_error() == b""

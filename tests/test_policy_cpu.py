@@ -1,5 +1,7 @@
 """What the losses on chosen log-probabilities refuse without a device, and their oracle against
 differences."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -27,21 +29,27 @@ def test_c_arguments_are_checked_before_the_device():
 
     def lp(dtype=0, x=1, stride=8, rows=2, cols=8, act=1, out=1, state=1):
         return lib.cl_selected_log_prob_forward(dtype, x, stride, rows, cols, act, -100, out, state,
-                                                None)
+                                                None, 0, None)
 
     def policy(low=0.2, kl=0.0, ref=None, red=2, loss=1, old=1, rows=2):
         return lib.cl_policy_loss_forward(0, 1, 8, rows, 8, 1, -100, old, 1, ref, low, 0.2, kl, red,
-                                          1, 1, 1, loss, loss, None)
+                                          1, 1, 1, loss, loss, None, 0, None)
 
     def pref(pairs=1, smooth=0.0, off=1, red=2, gaps=1):
         return lib.cl_preference_loss_forward(0, 1, 8, 2, 8, 1, -100, None, off, pairs, 0.1, smooth,
-                                              red, 1, 1, gaps, 1, 1, 1, 1, 1, 1, None)
+                                              red, 1, 1, gaps, 1, 1, 1, 1, 1, 1, None, 0, None)
 
     assert lp(rows=0, x=None, act=None, out=None, state=None) == ok
     assert lp(cols=0) == bad and lp(cols=2**31) == bad and lp(rows=-1) == bad
     assert lp(rows=2**31) == bad and lp(stride=-1) == bad and lp(dtype=7) == bad
     assert lp(x=None) == bad and lp(act=None) == bad and lp(out=None) == bad
     assert lp(state=None) == bad
+    # few long rows are split over workgroups that meet in a workspace
+    need = ctypes.c_int64()
+    assert lib.cl_token_loss_workspace(0, 4, 1 << 17, ctypes.byref(need)) == ok and need.value > 0
+    assert lp(rows=4, cols=1 << 17, stride=1 << 17) == bad and b"workspace" in lib.cl_last_error()
+    assert lib.cl_token_loss_workspace(0, 4, 10, ctypes.byref(need)) == ok and need.value == 0
+    assert lib.cl_token_loss_workspace(0, 4, 0, ctypes.byref(need)) == bad
     assert policy(low=-0.1) == bad and policy(low=float("nan")) == bad
     assert policy(kl=0.1) == bad and b"KL" in lib.cl_last_error()
     assert policy(red=3) == bad and policy(loss=None) == bad and policy(old=None) == bad
@@ -50,6 +58,7 @@ def test_c_arguments_are_checked_before_the_device():
     assert lib.cl_selected_log_prob_backward(0, 1, 8, 2, 8, 1, 1, None, 1, None) == bad
     assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 2, 1, None, 1, None) == bad
     assert lib.cl_preference_loss_backward(0, 1, 8, 2, 8, 1, 1, None, 1, 1, 2, 1, 1, 1, None) == bad
+    assert lp(rows=0) == ok and lib.cl_last_error() == b""
 
 
 def _difference(f, z, eps=1e-6):
