@@ -135,8 +135,10 @@ SIGNATURES: dict[str, list] = {
     "cl_selected_log_prob_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p],
     "cl_selected_log_prob_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
     "cl_policy_loss_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _f64, _f64, _f64,
-                               _int, _p, _p, _p, _p, _p, _p, _i64, _p],
-    "cl_policy_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _int, _p, _p, _p, _p],
+                               _int, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
+    "cl_policy_loss_prefills": [_int, _i64, _i64, ctypes.POINTER(_int)],
+    "cl_policy_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _int, _p, _p, _int, _p, _p],
+    "cl_stream_capture_id": [_p, ctypes.POINTER(_u64)],
     "cl_preference_loss_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _f64, _f64,
                                    _int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
     "cl_preference_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _int, _p, _p,

@@ -31,3 +31,17 @@ int check_launch(const char* what) {
 extern "C" int cl_abi_version(void) { return 1; }
 
 extern "C" const char* cl_last_error(void) { return cl::g_error; }
+
+extern "C" int cl_stream_capture_id(void* stream, uint64_t* id) {
+    using namespace cl;
+    clear_error();
+    CL_ARG(id, "null pointer argument");
+    *id = 0;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long got = 0;
+    const hipError_t e = hipStreamGetCaptureInfo(as_stream(stream), &status, &got);
+    CL_REQUIRE(e == hipSuccess, CL_ERR_HIP, "hipStreamGetCaptureInfo: HIP error %d (%s)", int(e),
+               hipGetErrorString(e));
+    if (status == hipStreamCaptureStatusActive) *id = got;
+    return CL_OK;
+}

@@ -60,18 +60,24 @@ template <typename T>
 using quad_of = std::conditional_t<sizeof(T) == 2, quad2,
                                    std::conditional_t<sizeof(T) == 4, quad4, quad8>>;
 
-template <typename T, int N>
+// THROUGH: past the caches (non-temporal), for what is read or written once and does not fit them.
+template <typename T, int N, bool THROUGH = false>
 __device__ __forceinline__ Pack<T, N> pload(const T* p) {
     using Q = quad_of<T>;
     struct Words {
         Q q[N * sizeof(T) / 16];
     } w;
 #pragma unroll
-    for (int i = 0; i < int(N * sizeof(T) / 16); ++i) w.q[i] = reinterpret_cast<const Q*>(p)[i];
+    for (int i = 0; i < int(N * sizeof(T) / 16); ++i) {
+        if constexpr (THROUGH)
+            w.q[i] = __builtin_nontemporal_load(reinterpret_cast<const Q*>(p) + i);
+        else
+            w.q[i] = reinterpret_cast<const Q*>(p)[i];
+    }
     return __builtin_bit_cast(Pack<T, N>, w);
 }
 
-template <typename T, int N>
+template <typename T, int N, bool THROUGH = false>
 __device__ __forceinline__ void pstore(T* p, const Pack<T, N>& r) {
     using Q = quad_of<T>;
     struct Words {
@@ -79,7 +85,12 @@ __device__ __forceinline__ void pstore(T* p, const Pack<T, N>& r) {
     };
     const Words w = __builtin_bit_cast(Words, r);
 #pragma unroll
-    for (int i = 0; i < int(N * sizeof(T) / 16); ++i) reinterpret_cast<Q*>(p)[i] = w.q[i];
+    for (int i = 0; i < int(N * sizeof(T) / 16); ++i) {
+        if constexpr (THROUGH)
+            __builtin_nontemporal_store(w.q[i], reinterpret_cast<Q*>(p) + i);
+        else
+            reinterpret_cast<Q*>(p)[i] = w.q[i];
+    }
 }
 
 }  // namespace cl

@@ -36,6 +36,13 @@ struct RowArgs {
     int64_t ignore;
     wide_t<T>* lp;
     RowState<wide_t<T>>* state;
+    // Logits and gradient past the 256 MiB cache, by their size.  A gradient from 96 MiB on would
+    // push out the logits that the cache still holds (131 MB of bf16, policy loss and gradient 60
+    // -> 55 us with the stores past it, 192 MB 96 -> 71, 262 MB of fp32 121 -> 100; at 38 MB
+    // nothing changes, and what comes next finds it).  Logits larger than the cache are not found
+    // again in it (328 MB 151 -> 126 us with the loads past it as well, 537 MB 237 -> 203; at 262
+    // MB they cost 17 us).
+    bool through_load, through_store;
 };
 
 template <typename A>
@@ -147,13 +154,14 @@ __device__ __forceinline__ A base_of(A m) {
     return m == -A(__builtin_inf()) ? A(0) : m;
 }
 
-// Over the TPR lanes of a row (16: a DPP row, 64: the wave), the same value in each of them.
+// Over the TPR lanes of a row (16: a DPP row, 64: the wave), the same bits in each of them: every
+// step exchanges with a mirror image, whose partial sum is the same two numbers the other way round.
 template <int TPR, typename A>
 __device__ __forceinline__ A lanes_max(A v) {
-    v = max_of(v, dpp_move<0xB1>(v));
-    v = max_of(v, dpp_move<0x4E>(v));
-    v = max_of(v, dpp_move<0x124>(v));
-    v = max_of(v, dpp_move<0x128>(v));
+    v = max_of(v, dpp_move<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = max_of(v, dpp_move<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = max_of(v, dpp_move<0x141>(v));  // row_half_mirror
+    v = max_of(v, dpp_move<0x140>(v));  // row_mirror
     if constexpr (TPR == 64)
         v = max_of(max_of(read_lane(v, 0), read_lane(v, 16)),
                    max_of(read_lane(v, 32), read_lane(v, 48)));
@@ -165,14 +173,16 @@ __device__ __forceinline__ A lanes_sum(A v) {
     if constexpr (TPR == 64) return wave_total(v);
     v += dpp_move<0xB1>(v);
     v += dpp_move<0x4E>(v);
-    v += dpp_move<0x124>(v);
-    v += dpp_move<0x128>(v);
+    v += dpp_move<0x141>(v);
+    v += dpp_move<0x140>(v);
     return v;
 }
 
 // Running maximum m and sum s of exp(x - m) over the lanes of a row.
 template <int LANES, typename A>
 __device__ __forceinline__ void join_lanes(A& m, A& s) {
+    // no product fused into the first addition: one lane would add it unrounded, its partner not
+#pragma clang fp contract(off)
     const A all = lanes_max<LANES>(m), base = base_of(all);
     s = lanes_sum<LANES>(s * exp_diff(m - base));
     m = all;
@@ -233,24 +243,23 @@ __device__ __forceinline__ wide_t<T> action_logit(const RowArgs<T>& a, const T* 
     return act >= 0 && act < a.cols ? wide_t<T>(x[act]) : wide_t<T>(0);
 }
 
-// ---- gradient of one logit: c ([j = a] - p_j) as exp(x - m) * k, k = -c / s, or c (1 - p_a).
-template <typename A>
+// ---- gradient of one logit: c ([j = a] - p_j) as exp(x - m) * k, k = -c / s; the action's own,
+// c (1 - p_a), is written over it by the thread that wrote it.  A result of 16 bits takes the
+// exponent as one product and sum, off by some 2^-20 of it; fp32 takes it as the loss does.
+template <typename T>
 struct RowGrad {
-    A m, k, own;
-    __device__ __forceinline__ RowGrad(const RowState<A>& st, A c)
-        : m(st.m), k(-c * st.inv_s), own(c * st.rest) {}
-};
-
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> grad_of(const Pack<T, VEC>& x, const RowGrad<wide_t<T>>& g,
-                                                int from_act) {
     using A = wide_t<T>;
-    Pack<T, VEC> r;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e)
-        r.v[e] = T(e == from_act ? g.own : exp_diff(A(x.v[e]) - g.m) * g.k);
-    return r;
-}
+    A m, k, own, shift;
+    __device__ __forceinline__ RowGrad(const RowState<A>& st, A c)
+        : m(st.m), k(-c * st.inv_s), own(c * st.rest), shift(st.m * A(-1.44269504088896340736)) {}
+    __device__ __forceinline__ T operator()(T x) const {
+        if constexpr (sizeof(T) == 2)
+            return T(__builtin_amdgcn_exp2f(__builtin_fmaf(A(x), 1.44269504088896340736f, shift)) *
+                     k);
+        else
+            return T(exp_diff(A(x) - m) * k);
+    }
+};
 
 // ---- maximum and sum of a row held in registers: NV vectors of 16 bytes and one element of the
 // rest per thread.  Two sweeps over registers instead of a running maximum: one exponential per
@@ -262,18 +271,43 @@ struct Held {
     T tail;
     int nvec, ntail;  // vectors of the row, elements after them
 
-    template <int TPR>
-    __device__ __forceinline__ void load(const T* x, int cols, int t) {
-        nvec = cols / VEC;
-        ntail = cols - nvec * VEC;
+    template <int TPR, bool THROUGH>
+    __device__ __forceinline__ void load_vecs(const T* x, int t) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (i * TPR + t < nvec) v[i] = pload<T, VEC>(x + int64_t(i * TPR + t) * VEC);
-        if (t < ntail) tail = x[nvec * VEC + t];
+            if (i * TPR + t < nvec)
+                v[i] = pload<T, VEC, THROUGH>(x + int64_t(i * TPR + t) * VEC);
     }
 
     template <int TPR>
-    __device__ __forceinline__ void reduce(int t, wide_t<T>& m, wide_t<T>& s) const {
+    __device__ __forceinline__ void load(const T* x, int cols, int t, bool through) {
+        nvec = cols / VEC;
+        ntail = cols - nvec * VEC;
+        if (t < ntail) tail = x[nvec * VEC + t];
+        if (through)
+            load_vecs<TPR, true>(x, t);
+        else
+            load_vecs<TPR, false>(x, t);
+    }
+
+    // Between two sweeps: the row stays as it was loaded.  Without this the compiler keeps 16-bit
+    // elements widened from one sweep to the next, in twice the registers (64 KB of bf16 by 512
+    // threads: 103 registers and half the waves).
+    __device__ __forceinline__ void keep_packed() {
+        if constexpr (sizeof(T) == 2) {
+            typedef uint32_t words __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                words w = __builtin_bit_cast(words, v[i]);
+                asm volatile("" : "+v"(w));
+                using Vector = Pack<T, VEC>;
+                v[i] = __builtin_bit_cast(Vector, w);
+            }
+        }
+    }
+
+    template <int TPR>
+    __device__ __forceinline__ void reduce(int t, wide_t<T>& m, wide_t<T>& s) {
         using A = wide_t<T>;
         m = -A(__builtin_inf());
 #pragma unroll
@@ -284,6 +318,7 @@ struct Held {
             }
         if (t < ntail) m = max_of(m, A(tail));
         const A base = base_of(m);
+        keep_packed();
         s = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -294,35 +329,77 @@ struct Held {
         if (t < ntail) s += exp_diff(A(tail) - base);
     }
 
-    template <int TPR>
-    __device__ __forceinline__ void store_grad(T* g, int t, int act,
-                                               const RowGrad<wide_t<T>>& rg) const {
-        using A = wide_t<T>;
+    template <int TPR, bool THROUGH>
+    __device__ __forceinline__ void store_vecs(T* g, int t, const RowGrad<T>& rg) const {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = (i * TPR + t) * VEC;
-            if (i * TPR + t < nvec) pstore<T, VEC>(g + j, grad_of<T, VEC>(v[i], rg, act - j));
-        }
-        if (t < ntail) {
-            const int j = nvec * VEC + t;
-            g[j] = T(j == act ? rg.own : exp_diff(A(tail) - rg.m) * rg.k);
-        }
+        for (int i = 0; i < NV; ++i)
+            if (i * TPR + t < nvec) {
+                Pack<T, VEC> r;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) r.v[e] = rg(v[i].v[e]);
+                pstore<T, VEC, THROUGH>(g + (i * TPR + t) * VEC, r);
+            }
     }
 
     template <int TPR>
-    __device__ __forceinline__ void store_zero(T* g, int cols, int t) const {
+    __device__ __forceinline__ void store_grad(T* g, int t, int act, const RowGrad<T>& rg,
+                                               bool through) const {
+        if (through)
+            store_vecs<TPR, true>(g, t, rg);
+        else
+            store_vecs<TPR, false>(g, t, rg);
+        if (t < ntail) g[nvec * VEC + t] = rg(tail);
+        // the action's vector is thread (act / VEC) % TPR's, its place in the tail thread
+        // act - nvec * VEC's; a thread's own stores stay in order
+        const bool in_vecs = act >= 0 && act < nvec * VEC;
+        const bool in_tail = act >= nvec * VEC && act < nvec * VEC + ntail;
+        if ((in_vecs && t == (act / VEC) % TPR) || (in_tail && t == act - nvec * VEC))
+            g[act] = T(rg.own);
+    }
+
+    template <int TPR>
+    __device__ __forceinline__ void store_zero(T* g, int cols, int t, bool through) const {
         const int n = cols / VEC;
         const Pack<T, VEC> z{};
-        for (int i = t; i < n; i += TPR) pstore<T, VEC>(g + int64_t(i) * VEC, z);
+        if (through) {
+            for (int i = t; i < n; i += TPR) pstore<T, VEC, true>(g + int64_t(i) * VEC, z);
+        } else {
+            for (int i = t; i < n; i += TPR) pstore<T, VEC>(g + int64_t(i) * VEC, z);
+        }
         if (t < cols - n * VEC) g[int64_t(n) * VEC + t] = T(0);
     }
 };
 
 constexpr int kRowBlock = 256;
 
+// ---- the gradient out of the forward, for an upstream gradient of 1: the row is still in
+// registers.  grad: null where the forward only takes the loss.
+template <typename T>
+struct GradOut {
+    T* grad;
+    const wide_t<T>* count;  // what a mean divides by, or null
+    __device__ __forceinline__ wide_t<T> slope(wide_t<T> s) const {
+        if (s == wide_t<T>(0)) return wide_t<T>(0);
+        return count ? s * (wide_t<T>(1) / count[0]) : s;
+    }
+};
+
+template <typename T, int TPR, int NV>
+__device__ __forceinline__ void emit_grad(const RowArgs<T>& a, const GradOut<T>& out, int64_t n,
+                                          int64_t act, int t, const Held<T, NV>& row,
+                                          const RowState<wide_t<T>>& st) {
+    const wide_t<T> c = out.slope(st.slope);
+    T* g = out.grad + n * a.cols;
+    if (c == wide_t<T>(0))
+        row.template store_zero<TPR>(g, int(a.cols), t, a.through_store);
+    else
+        row.template store_grad<TPR>(g, t, action_place(a, act), RowGrad<T>(st, c),
+                                     a.through_store);
+}
+
 // ---- short rows: TPR lanes (16 or 64) of a wave per row, several rows per workgroup, no LDS.
-template <typename T, int TPR, int NV, typename Op>
-__global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op) {
+template <typename T, int TPR, int NV, typename Op, bool GRAD>
+__global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op, GradOut<T> out) {
     using A = wide_t<T>;
     const int64_t n = int64_t(blockIdx.x) * (kRowBlock / TPR) + threadIdx.x / TPR;
     if (n >= a.rows) return;
@@ -332,18 +409,51 @@ __global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op) {
     const RowInputs in = op.load(n);
     const A xa = action_logit(a, x, act);
     Held<T, NV> row;
-    row.template load<TPR>(x, int(a.cols), t);
+    row.template load<TPR>(x, int(a.cols), t, a.through_load);
     A m, s;
     row.template reduce<TPR>(t, m, s);
     join_lanes<TPR>(m, s);
-    finish_row<TPR>(a, op, n, act, xa, in, m, s, t == 0);
+    const RowState<A> st = finish_row<TPR>(a, op, n, act, xa, in, m, s, t == 0);
+    if constexpr (GRAD) emit_grad<T, TPR, NV>(a, out, n, act, t, row, st);
+}
+
+// ---- a row per workgroup, held in its registers between the loss and the gradient.
+template <typename T, int TPR, int NV, typename Op>
+__global__ __launch_bounds__(TPR, 8) void k_rows_held(RowArgs<T> a, Op op, GradOut<T> out) {
+    using A = wide_t<T>;
+    __shared__ A part[TPR / 64][2];
+    __shared__ RowState<A> shared;
+    const int64_t n = blockIdx.x;
+    const int t = threadIdx.x;
+    const int64_t act = a.actions[n];
+    Held<T, NV> row;
+    RowState<A> st{A(0), A(1), A(0), A(0)};
+    if (act == a.ignore) {
+        if (wave_id() == 0) finish_row<64>(a, op, n, act, A(0), RowInputs{}, A(0), A(1), t == 0);
+    } else {
+        const T* x = a.x + n * a.stride;
+        const RowInputs in = op.load(n);
+        const A xa = action_logit(a, x, act);
+        row.template load<TPR>(x, int(a.cols), t, a.through_load);
+        A m, s;
+        row.template reduce<TPR>(t, m, s);
+        row.keep_packed();
+        join_waves<TPR / 64>(m, s, part);
+        if (wave_id() == 0) {
+            st = finish_row<64>(a, op, n, act, xa, in, m, s, t == 0);
+            if (t == 0) shared = st;
+        }
+        __syncthreads();
+        st = shared;
+    }
+    emit_grad<T, TPR, NV>(a, out, n, act, t, row, st);
 }
 
 // ---- a row per workgroup, read once with a running maximum and sum; ignored rows are not read.
 constexpr int kStreamUnroll = 4;  // vectors in flight per thread
 
 // Vectors lo..hi-1 of a row, and the elements after its last whole vector with `tail`.
-template <typename T>
+template <typename T, bool THROUGH = false>
 __device__ __forceinline__ void stream_part(const T* x, int cols, int lo, int hi, bool tail,
                                             wide_t<T>& m, wide_t<T>& s) {
     using A = wide_t<T>;
@@ -354,7 +464,8 @@ __device__ __forceinline__ void stream_part(const T* x, int cols, int lo, int hi
         Pack<T, VEC> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i + u * kRowBlock < hi) v[u] = pload<T, VEC>(x + int64_t(i + u * kRowBlock) * VEC);
+            if (i + u * kRowBlock < hi)
+                v[u] = pload<T, VEC, THROUGH>(x + int64_t(i + u * kRowBlock) * VEC);
         A top = m;
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -393,7 +504,11 @@ __global__ __launch_bounds__(kRowBlock) void k_rows_stream(RowArgs<T> a, Op op) 
         const T* x = a.x + n * a.stride;
         in = op.load(n);
         xa = action_logit(a, x, act);
-        stream_part<T>(x, int(a.cols), 0, int(a.cols) / wide_vec<T>(), true, m, s);
+        const int nvec = int(a.cols) / wide_vec<T>();
+        if (a.through_load)
+            stream_part<T, true>(x, int(a.cols), 0, nvec, true, m, s);
+        else
+            stream_part<T>(x, int(a.cols), 0, nvec, true, m, s);
         join_waves<kRowBlock / 64>(m, s, part);
     }
     if (wave_id() == 0) finish_row<64>(a, op, n, act, xa, in, m, s, lane_id() == 0);
@@ -460,7 +575,7 @@ struct Upstream {
             if (pair_grad) g *= pair_grad[q < pairs ? q : q - pairs];
         }
         if (rows) g *= rows[n];
-        if (scalar) g *= count ? scalar[0] / count[0] : scalar[0];
+        if (scalar) g *= count ? scalar[0] / count[0] : scalar[0];  // (1: as GradOut has it)
         return g;
     }
 };
@@ -479,23 +594,21 @@ __global__ __launch_bounds__(kRowBlock) void k_grad_short(RowArgs<T> a, Upstream
     T* g = grad + n * a.cols;
     Held<T, NV> row;
     if (c == A(0)) {
-        row.template store_zero<TPR>(g, int(a.cols), t);
+        row.template store_zero<TPR>(g, int(a.cols), t, a.through_store);
         return;
     }
-    row.template load<TPR>(a.x + n * a.stride, int(a.cols), t);
-    row.template store_grad<TPR>(g, t, action_place(a, act), RowGrad<A>(st, c));
+    row.template load<TPR>(a.x + n * a.stride, int(a.cols), t, a.through_load);
+    row.template store_grad<TPR>(g, t, action_place(a, act), RowGrad<T>(st, c), a.through_store);
 }
 
 constexpr int kGradVecs = 4;  // vectors per thread
 
 template <typename T>
-__global__ __launch_bounds__(kRowBlock) void k_grad_long(RowArgs<T> a, Upstream<wide_t<T>> up,
-                                                         T* __restrict__ grad, uint32_t chunks) {
+__device__ __forceinline__ void grad_chunk(const RowArgs<T>& a, const Upstream<wide_t<T>>& up,
+                                           T* grad, int64_t n, int64_t chunk) {
     using A = wide_t<T>;
-    constexpr int VEC = wide_vec<T>();
-    constexpr int CHUNK = kRowBlock * kGradVecs * VEC;
-    const int64_t n = blockIdx.x / chunks;
-    const int64_t j0 = int64_t(blockIdx.x % chunks) * CHUNK;
+    constexpr int CHUNK = kRowBlock * kGradVecs * wide_vec<T>();
+    const int64_t j0 = chunk * CHUNK;
     const int cols = int(std::min<int64_t>(CHUNK, a.cols - j0));
     const RowState<A> st = a.state[n];
     const int64_t act = a.actions[n];
@@ -503,12 +616,28 @@ __global__ __launch_bounds__(kRowBlock) void k_grad_long(RowArgs<T> a, Upstream<
     T* g = grad + n * a.cols + j0;
     Held<T, kGradVecs> row;
     if (c == A(0)) {
-        row.template store_zero<kRowBlock>(g, cols, threadIdx.x);
+        row.template store_zero<kRowBlock>(g, cols, threadIdx.x, a.through_store);
         return;
     }
-    row.template load<kRowBlock>(a.x + n * a.stride + j0, cols, threadIdx.x);
+    row.template load<kRowBlock>(a.x + n * a.stride + j0, cols, threadIdx.x, a.through_load);
     row.template store_grad<kRowBlock>(g, threadIdx.x, action_place(a, act) - int(j0),
-                                       RowGrad<A>(st, c));
+                                       RowGrad<T>(st, c), a.through_store);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_grad_long(RowArgs<T> a, Upstream<wide_t<T>> up,
+                                                         T* __restrict__ grad, uint32_t chunks) {
+    grad_chunk<T>(a, up, grad, blockIdx.x / chunks, blockIdx.x % chunks);
+}
+
+// A gradient that the forward left for an upstream gradient of 1: nothing to do where it is 1,
+// else formed again.  Few workgroups, which walk the chunks.
+template <typename T>
+__global__ __launch_bounds__(kRowBlock) void k_grad_again(RowArgs<T> a, Upstream<wide_t<T>> up,
+                                                          T* __restrict__ grad, uint32_t chunks) {
+    if (up.scalar[0] == wide_t<T>(1)) return;
+    for (int64_t i = blockIdx.x; i < a.rows * chunks; i += gridDim.x)
+        grad_chunk<T>(a, up, grad, i / chunks, i % chunks);
 }
 
 // ---- sums in a fixed order by one workgroup, in fp64
@@ -523,6 +652,19 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
     return wave_total(lane_id() < waves ? red[lane_id()] : 0.0);
 }
 
+// Rows that count, before the rows themselves where the forward divides by their number.
+template <typename A>
+__global__ __launch_bounds__(kSumThreads) void k_count(const int64_t* __restrict__ actions,
+                                                       int64_t rows, int64_t ignore,
+                                                       A* __restrict__ count) {
+    __shared__ double red[kSumThreads / 64];
+    int c = 0;
+#pragma unroll 8
+    for (int64_t n = threadIdx.x; n < rows; n += kSumThreads) c += actions[n] != ignore;
+    const double t = group_sum(double(c), red);
+    if (threadIdx.x == 0) count[0] = A(t);
+}
+
 // loss = sum of the rows' terms, divided by the number of counted rows for a mean.
 template <typename A>
 __global__ __launch_bounds__(kSumThreads) void k_policy_sum(const A* __restrict__ terms,
@@ -532,6 +674,7 @@ __global__ __launch_bounds__(kSumThreads) void k_policy_sum(const A* __restrict_
                                                             A* __restrict__ count) {
     __shared__ double red[2][kSumThreads / 64];
     double t = 0, c = 0;
+#pragma unroll 8
     for (int64_t n = threadIdx.x; n < rows; n += kSumThreads) {
         t += double(terms[n]);
         c += actions[n] != ignore ? 1.0 : 0.0;
@@ -657,6 +800,9 @@ RowArgs<T> row_args(const void* logits, int64_t row_stride, int64_t rows, int64_
     a.ignore = ignore;
     a.lp = static_cast<wide_t<T>*>(lp);
     a.state = const_cast<RowState<wide_t<T>>*>(static_cast<const RowState<wide_t<T>>*>(state));
+    const int64_t bytes = rows * cols * int64_t(sizeof(T));
+    a.through_store = bytes >= (int64_t(96) << 20);
+    a.through_load = bytes >= (int64_t(256) << 20);
     return a;
 }
 
@@ -681,24 +827,67 @@ int64_t rows_workspace(int64_t rows, int64_t cols) {
     return parts > 1 ? rows * parts * 2 * int64_t(sizeof(wide_t<T>)) : 0;
 }
 
-template <typename T, int TPR, int NV, typename Op>
-void launch_rows_short(const RowArgs<T>& a, const Op& op, hipStream_t s) {
-    k_rows_short<T, TPR, NV, Op>
-        <<<unsigned(ceil_div(a.rows, kRowBlock / TPR)), kRowBlock, 0, s>>>(a, op);
+template <typename T, int TPR, int NV, bool GRAD, typename Op>
+void launch_rows_short(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipStream_t s) {
+    k_rows_short<T, TPR, NV, Op, GRAD>
+        <<<unsigned(ceil_div(a.rows, kRowBlock / TPR)), kRowBlock, 0, s>>>(a, op, out);
+}
+
+template <bool GRAD, typename T, typename Op>
+bool launch_short(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipStream_t s) {
+    const int64_t bytes = a.cols * int64_t(sizeof(T));
+    if (bytes <= 256)
+        launch_rows_short<T, 16, 1, GRAD>(a, op, out, s);
+    else if (bytes <= 1024)
+        launch_rows_short<T, 64, 1, GRAD>(a, op, out, s);
+    else if (bytes <= 4096)
+        launch_rows_short<T, 64, 4, GRAD>(a, op, out, s);
+    else
+        return false;
+    return true;
+}
+
+// The largest row, in bytes, that one workgroup holds, and the fewest logits, in bytes, for which
+// the loss and its gradient are taken in one pass.
+constexpr int64_t kHeldRow = 131072;
+constexpr int64_t kHeldLogits = int64_t(48) << 20;
+
+template <typename T>
+bool policy_prefills(int64_t rows, int64_t cols) {
+    return (std::is_same_v<T, float> || std::is_same_v<T, bf16_t>) &&
+           cols * int64_t(sizeof(T)) <= kHeldRow && rows * cols * int64_t(sizeof(T)) >= kHeldLogits;
+}
+
+// The rows' terms and, for an upstream gradient of 1, the logits' gradient.
+template <typename T, typename Op>
+int launch_rows_grad(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipStream_t s) {
+    if constexpr (std::is_same_v<T, float> || std::is_same_v<T, bf16_t>) {
+        const int64_t bytes = a.cols * int64_t(sizeof(T));
+        const unsigned grid = unsigned(a.rows);
+        if (a.rows == 0) return CL_OK;
+        if (launch_short<true>(a, op, out, s)) {
+        } else if (bytes <= 16384) {
+            k_rows_held<T, 256, 4, Op><<<grid, 256, 0, s>>>(a, op, out);
+        } else if (bytes <= 32768) {
+            k_rows_held<T, 512, 4, Op><<<grid, 512, 0, s>>>(a, op, out);
+        } else if (bytes <= 65536) {
+            k_rows_held<T, 512, 8, Op><<<grid, 512, 0, s>>>(a, op, out);
+        } else {
+            CL_ARG(bytes <= kHeldRow, "rows of %lld bytes are not held", (long long)bytes);
+            k_rows_held<T, 1024, 8, Op><<<grid, 1024, 0, s>>>(a, op, out);
+        }
+        return check_launch("rows and gradient");
+    } else {
+        CL_ARG(false, "the gradient of this type is not taken by the forward");
+    }
 }
 
 template <typename T, typename Op>
 int launch_rows(const RowArgs<T>& a, const Op& op, void* workspace, int64_t workspace_bytes,
                 hipStream_t s) {
     if (a.rows == 0) return CL_OK;
-    const int64_t bytes = a.cols * int64_t(sizeof(T));
     const int parts = row_parts<T>(a.rows, a.cols);
-    if (bytes <= 256) {
-        launch_rows_short<T, 16, 1>(a, op, s);
-    } else if (bytes <= 1024) {
-        launch_rows_short<T, 64, 1>(a, op, s);
-    } else if (bytes <= 4096) {
-        launch_rows_short<T, 64, 4>(a, op, s);
+    if (launch_short<false>(a, op, GradOut<T>{}, s)) {
     } else if (parts > 1) {
         CL_ARG(workspace && workspace_bytes >= rows_workspace<T>(a.rows, a.cols),
                "workspace of %lld bytes needed (cl_token_loss_workspace)",
@@ -718,11 +907,15 @@ int launch_rows(const RowArgs<T>& a, const Op& op, void* workspace, int64_t work
 
 template <typename T>
 int launch_logit_grad(const RowArgs<T>& a, const Upstream<wide_t<T>>& up, void* grad,
-                      hipStream_t s) {
+                      hipStream_t s, bool prefilled = false) {
     if (a.rows == 0) return CL_OK;
     const int64_t bytes = a.cols * int64_t(sizeof(T));
     T* g = static_cast<T*>(grad);
-    if (bytes <= 256) {
+    if (prefilled) {
+        const int64_t chunks = ceil_div(a.cols, kRowBlock * kGradVecs * wide_vec<T>());
+        k_grad_again<T><<<unsigned(std::min<int64_t>(a.rows * chunks, 1024)), kRowBlock, 0, s>>>(
+            a, up, g, uint32_t(chunks));
+    } else if (bytes <= 256) {
         k_grad_short<T, 16, 1><<<unsigned(ceil_div(a.rows, kRowBlock / 16)), kRowBlock, 0, s>>>(
             a, up, g);
     } else if (bytes <= 1024) {
@@ -790,18 +983,28 @@ extern "C" int cl_selected_log_prob_backward(int dtype, const void* logits, int6
     });
 }
 
+extern "C" int cl_policy_loss_prefills(int dtype, int64_t rows, int64_t cols, int* yes) {
+    clear_error();
+    CL_ARG(yes, "null pointer argument");
+    CL_ARG(rows >= 0 && cols >= 1, "bad shape");
+    CL_STORAGE_SWITCH(dtype, { *yes = policy_prefills<scalar_t>(rows, cols) ? 1 : 0; });
+    return CL_OK;
+}
+
 extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row_stride,
                                       int64_t rows, int64_t cols, const int64_t* actions,
                                       int64_t ignore_index, const void* old_log_probs,
                                       const void* advantages, const void* ref_log_probs,
                                       double clip_low, double clip_high, double kl_coef,
                                       int reduction, void* log_probs, void* row_state,
-                                      void* terms, void* loss, void* count, void* workspace,
-                                      int64_t workspace_bytes, void* stream) {
+                                      void* terms, void* loss, void* count, void* grad_logits,
+                                      void* workspace, int64_t workspace_bytes, void* stream) {
     clear_error();
     if (int rc = check_logits(logits, row_stride, rows, cols, actions, row_state)) return rc;
     CL_ARG(rows == 0 || (old_log_probs && advantages && log_probs && terms),
            "null pointer argument");
+    CL_ARG(!grad_logits || reduction == CL_REDUCE_SUM || reduction == CL_REDUCE_MEAN,
+           "the forward takes the gradient of a scalar loss only");
     CL_ARG(clip_low >= 0 && clip_high >= 0, "the clipped range must contain 1");
     CL_ARG(kl_coef == 0 || ref_log_probs, "a KL term needs the reference's log-probabilities");
     CL_ARG(reduction >= CL_REDUCE_NONE && reduction <= CL_REDUCE_MEAN, "unknown reduction %d",
@@ -819,10 +1022,19 @@ extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row
         op.high = 1.0 + clip_high;
         op.kl = kl_coef;
         op.terms = static_cast<A*>(terms);
-        if (int rc = launch_rows(row_args<T>(logits, row_stride, rows, cols, actions,
-                                             ignore_index, log_probs, row_state),
-                                 op, workspace, workspace_bytes, s))
+        const RowArgs<T> a = row_args<T>(logits, row_stride, rows, cols, actions, ignore_index,
+                                         log_probs, row_state);
+        if (grad_logits) {
+            const bool mean = reduction == CL_REDUCE_MEAN;
+            if (mean)
+                k_count<A><<<1, kSumThreads, 0, s>>>(actions, rows, ignore_index,
+                                                     static_cast<A*>(count));
+            const GradOut<T> out{static_cast<T*>(grad_logits),
+                                 mean ? static_cast<const A*>(count) : nullptr};
+            if (int rc = launch_rows_grad(a, op, out, s)) return rc;
+        } else if (int rc = launch_rows(a, op, workspace, workspace_bytes, s)) {
             return rc;
+        }
         if (reduction != CL_REDUCE_NONE)
             k_policy_sum<A><<<1, kSumThreads, 0, s>>>(op.terms, actions, rows, ignore_index,
                                                       reduction == CL_REDUCE_MEAN,
@@ -835,13 +1047,15 @@ extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row
 extern "C" int cl_policy_loss_backward(int dtype, const void* logits, int64_t row_stride,
                                        int64_t rows, int64_t cols, const int64_t* actions,
                                        const void* row_state, int reduction, const void* grad_loss,
-                                       const void* count, void* grad_logits, void* stream) {
+                                       const void* count, int prefilled, void* grad_logits,
+                                       void* stream) {
     clear_error();
     if (int rc = check_logits(logits, row_stride, rows, cols, actions, row_state)) return rc;
     CL_ARG(rows == 0 || (grad_loss && grad_logits), "null pointer argument");
     CL_ARG(reduction >= CL_REDUCE_NONE && reduction <= CL_REDUCE_MEAN, "unknown reduction %d",
            reduction);
     CL_ARG(reduction != CL_REDUCE_MEAN || count, "null pointer argument");
+    CL_ARG(!prefilled || reduction != CL_REDUCE_NONE, "only a scalar loss's gradient is prefilled");
     if (rows == 0) return CL_OK;
     CL_STORAGE_SWITCH(dtype, {
         using T = scalar_t;
@@ -854,7 +1068,7 @@ extern "C" int cl_policy_loss_backward(int dtype, const void* logits, int64_t ro
         if (reduction == CL_REDUCE_MEAN) up.count = static_cast<const A*>(count);
         return launch_logit_grad(row_args<T>(logits, row_stride, rows, cols, actions, 0, nullptr,
                                       row_state),
-                          up, grad_logits, as_stream(stream));
+                          up, grad_logits, as_stream(stream), prefilled != 0);
     });
 }
 

@@ -106,6 +106,19 @@ def _aux(logits, *sizes):
     return buf, [base + s for s in starts]
 
 
+def _prefills(sh):
+    yes = ctypes.c_int()
+    _capi.call("cl_policy_loss_prefills", sh.code, sh.rows, sh.cols, ctypes.byref(yes))
+    return bool(yes.value)
+
+
+def _capture_id(t) -> int:
+    """Which graph capture t's current stream records, 0 outside of one."""
+    got = ctypes.c_uint64()
+    _capi.call("cl_stream_capture_id", _dl.stream_of(t), ctypes.byref(got))
+    return got.value
+
+
 class SelectedLogProbsFunction(torch.autograd.Function):
     """lp[n] = log_softmax(logits[n])[actions[n]] in one pass over the logits; the backward makes
     the probabilities again from the row's maximum and sum.  No counterpart in the reference."""
@@ -158,12 +171,17 @@ class PolicyLossFunction(torch.autograd.Function):
             loss = torch.empty(sh.rows, dtype=wide, device=logits.device)
             aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
             terms, loss_at, count = loss.data_ptr(), None, None
+        grad = None
+        if reduction and ctx.needs_input_grad[0] and _prefills(sh):
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            ctx.capture = _capture_id(logits)
         with _dl.on_device_of(logits):
             timing.timed("cl_policy_loss_forward", lambda: _capi.call(
                 "cl_policy_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
                 old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
-                reduction, lp.data_ptr(), state, terms, loss_at, count, ws, sh.workspace_bytes,
-                _dl.stream_of(logits)))
+                reduction, lp.data_ptr(), state, terms, loss_at, count, _dl.ptr(grad), ws,
+                sh.workspace_bytes, _dl.stream_of(logits)))
+        ctx.grad = grad
         ctx.save_for_backward(logits, actions, aux)
         ctx.args, ctx.state, ctx.count, ctx.reduction = sh.args, state, count, reduction
         ctx.mark_non_differentiable(lp)
@@ -177,11 +195,16 @@ class PolicyLossFunction(torch.autograd.Function):
             return (None,) * 10
         logits, actions, aux = ctx.saved_tensors
         grad_loss = grad_loss.contiguous()
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        # the forward's gradient is handed out once, and only in the capture (or outside of any)
+        # that it was written in: a replay of the backward alone would find it used
+        grad, ctx.grad = ctx.grad, None
+        prefilled = grad is not None and ctx.capture == _capture_id(logits)
+        if not prefilled:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_policy_loss_backward", lambda: _capi.call(
                 "cl_policy_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
-                ctx.reduction, grad_loss.data_ptr(), ctx.count, grad.data_ptr(),
+                ctx.reduction, grad_loss.data_ptr(), ctx.count, int(prefilled), grad.data_ptr(),
                 _dl.stream_of(logits)))
         return (grad,) + (None,) * 9
 

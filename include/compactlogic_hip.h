@@ -52,6 +52,9 @@ extern "C" {
 /* ABI version of this header; bumped on any incompatible change. */
 int cl_abi_version(void);
 
+/* Identity of the capture that `stream` is recording, 0 when it records none. */
+int cl_stream_capture_id(void* stream, uint64_t* id);
+
 /* Message describing the last failed call on the calling thread ("" if none). */
 const char* cl_last_error(void);
 
@@ -583,22 +586,26 @@ int cl_selected_log_prob_backward(int dtype, const void* logits, int64_t row_str
  *   terms[n] = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(g) - g - 1);
  * loss: their sum (CL_REDUCE_SUM) or its mean over the counted rows (CL_REDUCE_MEAN; NaN when
  * none counts); neither loss nor count is written for CL_REDUCE_NONE.  ref_log_probs may be
- * NULL when kl_coef is 0. */
+ * NULL when kl_coef is 0.  grad_logits: NULL, or (for a scalar loss, where
+ * cl_policy_loss_prefills says so) written with the logits' gradient for grad_loss 1, the row
+ * still in registers: the logits are then read once for both. */
+int cl_policy_loss_prefills(int dtype, int64_t rows, int64_t cols, int* yes);
 int cl_policy_loss_forward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
                            int64_t cols, const int64_t* actions, int64_t ignore_index,
                            const void* old_log_probs, const void* advantages,
                            const void* ref_log_probs, double clip_low, double clip_high,
                            double kl_coef, int reduction, void* log_probs, void* row_state,
-                           void* terms, void* loss, void* count, void* workspace,
-                           int64_t workspace_bytes, void* stream);
+                           void* terms, void* loss, void* count, void* grad_logits,
+                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Its logits' gradient.  grad_loss: a device scalar, or [rows] for CL_REDUCE_NONE.  Where the
  * clipped product is the smaller one and r lies outside the range, only the KL term has a
- * gradient. */
+ * gradient.  prefilled: grad_logits holds what the forward wrote; it is formed again unless
+ * grad_loss is 1 (decided on the device). */
 int cl_policy_loss_backward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
                             int64_t cols, const int64_t* actions, const void* row_state,
                             int reduction, const void* grad_loss, const void* count,
-                            void* grad_logits, void* stream);
+                            int prefilled, void* grad_logits, void* stream);
 
 /* The preference loss of pairs of sequences: sequence q holds rows offsets[q] .. offsets[q + 1]
  * (int64 [2 pairs + 1], not decreasing, within [0, rows]); q < pairs is the chosen sequence of

@@ -31,9 +31,9 @@ def test_c_arguments_are_checked_before_the_device():
         return lib.cl_selected_log_prob_forward(dtype, x, stride, rows, cols, act, -100, out, state,
                                                 None, 0, None)
 
-    def policy(low=0.2, kl=0.0, ref=None, red=2, loss=1, old=1, rows=2):
+    def policy(low=0.2, kl=0.0, ref=None, red=2, loss=1, old=1, rows=2, grad=None):
         return lib.cl_policy_loss_forward(0, 1, 8, rows, 8, 1, -100, old, 1, ref, low, 0.2, kl, red,
-                                          1, 1, 1, loss, loss, None, 0, None)
+                                          1, 1, 1, loss, loss, grad, None, 0, None)
 
     def pref(pairs=1, smooth=0.0, off=1, red=2, gaps=1):
         return lib.cl_preference_loss_forward(0, 1, 8, 2, 8, 1, -100, None, off, pairs, 0.1, smooth,
@@ -53,10 +53,12 @@ def test_c_arguments_are_checked_before_the_device():
     assert policy(low=-0.1) == bad and policy(low=float("nan")) == bad
     assert policy(kl=0.1) == bad and b"KL" in lib.cl_last_error()
     assert policy(red=3) == bad and policy(loss=None) == bad and policy(old=None) == bad
+    assert policy(red=0, loss=None, grad=1) == bad and b"scalar" in lib.cl_last_error()
     assert pref(pairs=-1) == bad and pref(smooth=1.5) == bad and pref(off=None) == bad
     assert pref(red=-1) == bad and pref(gaps=None) == bad
     assert lib.cl_selected_log_prob_backward(0, 1, 8, 2, 8, 1, 1, None, 1, None) == bad
-    assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 2, 1, None, 1, None) == bad
+    assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 2, 1, None, 0, 1, None) == bad
+    assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 0, 1, None, 1, 1, None) == bad
     assert lib.cl_preference_loss_backward(0, 1, 8, 2, 8, 1, 1, None, 1, 1, 2, 1, 1, 1, None) == bad
     assert lp(rows=0) == ok and lib.cl_last_error() == b""
 

@@ -345,9 +345,15 @@ def test_gradients_against_differences(device):
 def test_second_backward_and_other_upstream(device):
     """A retained graph gives the same gradient again, whatever was done with the first."""
     for dtype in (torch.float32, torch.bfloat16):
-        for vocab in (10, 3001):
+        for vocab in (10, 300, 3001, 8001, 20011, 33001):
             c = Case(40, vocab, dtype, device)
             z = c.logits.requires_grad_()
+            loss = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t)
+            (g0,) = torch.autograd.grad(loss * 0, z, retain_graph=True)
+            (g1,) = torch.autograd.grad(loss, z)
+            assert not g0.any() and g1.any()
+            (g2,) = torch.autograd.grad(cl.policy_loss(z, c.act_t, c.old_t, c.adv_t) * -2, z)
+            assert torch.equal(g2, g1 * -2)          # a power of two: every rounding moves with it
             loss = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t)
             (g1,) = torch.autograd.grad(loss, z, retain_graph=True)
             keep = g1.clone()
