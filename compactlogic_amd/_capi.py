@@ -97,6 +97,9 @@ SIGNATURES: dict[str, list] = {
     "cl_conv_window_moments": [_int, _p, _p, _p, _p, _p, _i64, _i64] + [_i64] * 11 + [_p],
     "cl_conv_window_finalize": [_int, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p],
     "cl_group_sum_forward": [_int, _p, _i64, _i64, _i64, _i64, _i64, _f64, _p, _p, _i64, _p],
+    "cl_group_sum_centered_workspace_size": [_int, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "cl_group_sum_centered_forward": [_int, _p, _i64, _i64, _i64, _i64, _i64, _f64, _p, _p, _i64,
+                                      _p],
     "cl_group_sum_workspace_size": [_int, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "cl_group_sum_backward": [_int, _p, _i64, _i64, _i64, _f64, _p, _i64, _i64, _p],
     "cl_group_sum_cross_entropy_forward": [_int, _p, _i64, _i64, _i64, _i64, _i64, _f64, _p,

@@ -220,6 +220,83 @@ struct CrossEntropyGrad {
     }
 };
 
+// ---- scores less the sample's largest one, out[n, c] = z[n, c] - max z[n], for losses that only
+// depend on such differences.  A class sum of 1200 activations is near 600, where fp32 steps are
+// 6e-5 wide: rounded there, as k_gsum_finish rounds it, a softmax is off by some 1e-5.  The slices
+// are therefore added, divided and subtracted in fp64 and rounded once, at the size of the
+// difference.  k_gsum_center: workgroup of kCenterSamples samples, their scores in LDS; it is bound
+// by the loads of the slices, as the finish (1024 samples, 26 slices of 10 classes: 1.1 MB).
+constexpr int kCenterSamples = 16;
+
+template <typename T>
+__device__ __forceinline__ void center_row(const double* z, int64_t k, T* __restrict__ out) {
+    double mx = -__builtin_inf();
+    bool nan = false;
+    for (int64_t c = lane_id(); c < k; c += kWave) {
+        mx = fmax(mx, z[c]);
+        nan |= z[c] != z[c];
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor(mx, off, kWave));
+    // all of a row's differences are NaN where a score is, as its softmax would be
+    if (__any(nan)) mx = __builtin_nan("");
+    for (int64_t c = lane_id(); c < k; c += kWave) out[c] = T(z[c] - mx);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_gsum_center(const T* __restrict__ part, int64_t B,
+                                                     int64_t k, int64_t nslices, double tau,
+                                                     T* __restrict__ out) {
+    extern __shared__ __align__(16) unsigned char center_lds[];
+    double* z = reinterpret_cast<double*>(center_lds);  // [kCenterSamples][k]
+    const int64_t n0 = int64_t(blockIdx.x) * kCenterSamples;
+    const int64_t ns = std::min<int64_t>(kCenterSamples, B - n0);
+    const int64_t step = k * B;
+    for (int64_t e = threadIdx.x; e < ns * k; e += 256) {
+        // samples side by side: a slice's elements of one class are contiguous over the batch
+        const int64_t c = e / ns, i = e - c * ns;
+        const T* src = part + c * B + n0 + i;
+        double t = 0;
+        int64_t sl = 0;
+        for (; sl + 16 <= nslices; sl += 16) {
+            T v[16];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v[u] = src[(sl + u) * step];
+#pragma unroll
+            for (int u = 0; u < 16; ++u) t += double(v[u]);
+        }
+        T v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) v[u] = sl + u < nslices ? src[(sl + u) * step] : T(0);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) t += sl + u < nslices ? double(v[u]) : 0.0;
+        z[i * k + c] = t / tau;
+    }
+    __syncthreads();
+    for (int64_t i = wave_id(); i < ns; i += 4) center_row(z + i * k, k, out + (n0 + i) * k);
+}
+
+// Any layout: a workgroup per sample, its waves taking the classes in turn.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gsum_center_any(const T* __restrict__ x, int64_t F,
+                                                         int64_t sb, int64_t sf, int64_t gsz,
+                                                         int64_t k, double tau,
+                                                         T* __restrict__ out) {
+    extern __shared__ __align__(16) unsigned char center_lds[];
+    double* z = reinterpret_cast<double*>(center_lds);  // [k]
+    const int64_t n = blockIdx.x;
+    for (int64_t c = wave_id(); c < k; c += 4) {
+        const int64_t j1 = std::min<int64_t>((c + 1) * gsz, F);
+        double t = 0;
+        for (int64_t j = c * gsz + lane_id(); j < j1; j += kWave)
+            t += double(x[n * sb + j * sf]);
+        t = wave_sum(t);
+        if (lane_id() == 0) z[c] = t / tau;
+    }
+    __syncthreads();
+    if (wave_id() == 0) center_row(z, k, out + n * k);
+}
+
 // ---- backward: grad_x[n, j] = src(n, j / gsz).  Elements are visited in memory order
 // of grad_x: `inner` is the unit-stride dimension (batch or feature).
 template <typename T, int VEC, bool BATCH_INNER, typename Src>
@@ -508,6 +585,77 @@ extern "C" int cl_group_sum_forward(int dtype, const void* x, int64_t batch, int
         }
     });
     return check_launch("cl_group_sum_forward");
+}
+
+namespace {
+constexpr int64_t kCenterMaxClasses = 65536 / (8 * kCenterSamples);  // of one workgroup's LDS
+
+int64_t center_workspace(int64_t batch, int64_t features, int64_t stride_batch, int64_t k,
+                         int64_t size) {
+    if (!gsum_split_applies(batch, features, stride_batch)) return 0;
+    return gsum_slices(batch, features, k, 1) * k * batch * size;
+}
+}  // namespace
+
+extern "C" int cl_group_sum_centered_workspace_size(int dtype, int64_t batch, int64_t features,
+                                                    int64_t stride_batch, int64_t k,
+                                                    int64_t* bytes) {
+    clear_error();
+    CL_ARG(bytes, "null pointer argument");
+    CL_ARG(batch >= 0 && features >= 0 && k >= 1, "bad shape");
+    *bytes = -1;
+    if (k > kCenterMaxClasses) return CL_OK;
+    CL_DTYPE_SWITCH(dtype, {
+        *bytes = center_workspace(batch, features, stride_batch, k, int64_t(sizeof(scalar_t)));
+    });
+    return CL_OK;
+}
+
+extern "C" int cl_group_sum_centered_forward(int dtype, const void* x, int64_t batch,
+                                             int64_t features, int64_t stride_batch,
+                                             int64_t stride_feature, int64_t k, double tau,
+                                             void* out, void* workspace, int64_t workspace_bytes,
+                                             void* stream) {
+    clear_error();
+    CL_ARG(batch >= 0 && features >= 0, "negative shape");
+    CL_ARG(batch < (int64_t(1) << 31), "batch must be below 2^31");
+    CL_ARG(k >= 1 && k <= kCenterMaxClasses, "k must be in [1, %lld], got %lld",
+           (long long)kCenterMaxClasses, (long long)k);
+    CL_ARG(stride_batch >= 0 && stride_feature >= 0, "negative strides are not supported");
+    if (batch == 0) return CL_OK;
+    CL_ARG(out, "null pointer argument");
+    CL_ARG(features == 0 || x, "null pointer argument");
+    const int64_t gsz = features == 0 ? 1 : ceil_div(features, k);
+    hipStream_t s = as_stream(stream);
+    CL_DTYPE_SWITCH(dtype, {
+        using T = scalar_t;
+        const T* xs = static_cast<const T*>(x);
+        T* os = static_cast<T*>(out);
+        if (gsum_split_applies(batch, features, stride_batch)) {
+            constexpr int W = wide_vec<T>();
+            const bool wide = batch % W == 0 && stride_feature % W == 0 && aligned(x, 16);
+            const int64_t slices = gsum_slices(batch, features, k, wide ? W : 1);
+            CL_ARG(workspace && workspace_bytes >= slices * k * batch * int64_t(sizeof(T)),
+                   "workspace needed (cl_group_sum_centered_workspace_size)");
+            T* part = static_cast<T*>(workspace);
+            const int64_t slice = ceil_div(gsz, slices);
+            const dim3 grid(unsigned(ceil_div(batch, 64 * (wide ? W : 1))), unsigned(k),
+                            unsigned(slices));
+            if (wide)
+                k_gsum_partial<T, W><<<grid, kPartWaves * 64, 0, s>>>(
+                    xs, batch, features, stride_feature, gsz, k, slice, part);
+            else
+                k_gsum_partial<T, 1><<<grid, kPartWaves * 64, 0, s>>>(
+                    xs, batch, features, stride_feature, gsz, k, slice, part);
+            if (int rc = check_launch("cl_group_sum_centered_forward(partial)")) return rc;
+            k_gsum_center<T><<<unsigned(ceil_div(batch, kCenterSamples)), 256,
+                               size_t(kCenterSamples * k * 8), s>>>(part, batch, k, slices, tau, os);
+        } else {
+            k_gsum_center_any<T><<<unsigned(batch), 256, size_t(k * 8), s>>>(
+                xs, features, stride_batch, stride_feature, gsz, k, tau, os);
+        }
+    });
+    return check_launch("cl_group_sum_centered_forward");
 }
 
 namespace {

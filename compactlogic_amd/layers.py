@@ -1419,20 +1419,40 @@ class GroupSum(torch.nn.Module):
                                                            ignore_index)
         return (loss, out) if return_scores else loss
 
+    def _head(self, x):
+        """x and the (k, tau) by which the losses of policy.py take its scores themselves, summed in
+        more bits; or the scores, for more classes than they take."""
+        if not isinstance(x, torch.Tensor):
+            raise TypeError("GroupSum's losses need a tensor of activations")
+        if x.dtype == torch.float16:
+            x = x.float()
+        if not _policy.takes_group(self.k):
+            return self(x), None
+        return x, (self.k, float(self.tau))
+
     def log_probs(self, x, actions, ignore_index: int = -100):
-        """policy.selected_log_probs(self(x), actions): the log-probability of the chosen class of
-        every sample, differentiable by x."""
-        return _policy.selected_log_probs(self(x), actions, ignore_index)
+        """policy.selected_log_probs(self(x), actions) in one op: the log-probability of the chosen
+        class of every sample, differentiable by x."""
+        x, group = self._head(x)
+        return _policy._selected_log_probs(x, actions, ignore_index, group)
 
-    def policy_loss(self, x, actions, old_log_probs, advantages, **options):
-        """policy.policy_loss(self(x), actions, old_log_probs, advantages, ...): the clipped policy
-        loss with a KL term of a network that chooses one of k classes."""
-        return _policy.policy_loss(self(x), actions, old_log_probs, advantages, **options)
+    def policy_loss(self, x, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
+                    kl_coef: float = 0.0, ignore_index: int = -100, reduction: str = "mean",
+                    return_log_probs: bool = False):
+        """policy.policy_loss(self(x), actions, ...) in one op: the clipped policy loss with a KL
+        term of a network that chooses one of k classes, differentiable by x."""
+        x, group = self._head(x)
+        return _policy._policy_loss(x, actions, old_log_probs, advantages, ref_log_probs, clip,
+                                    kl_coef, ignore_index, reduction, return_log_probs, group)
 
-    def preference_loss(self, x, actions, offsets, **options):
-        """policy.preference_loss(self(x), actions, offsets, ...): the preference loss of paired
-        sequences of samples."""
-        return _policy.preference_loss(self(x), actions, offsets, **options)
+    def preference_loss(self, x, actions, offsets, ref_log_probs=None, beta: float = 0.1,
+                        label_smoothing: float = 0.0, ignore_index: int = -100,
+                        reduction: str = "mean", return_margins: bool = False):
+        """policy.preference_loss(self(x), actions, offsets, ...) in one op: the preference loss of
+        paired sequences of samples, differentiable by x."""
+        x, group = self._head(x)
+        return _policy._preference_loss(x, actions, offsets, ref_log_probs, beta, label_smoothing,
+                                        ignore_index, reduction, return_margins, group)
 
     def extra_repr(self):
         return 'k={}, tau={}'.format(self.k, self.tau)

@@ -15,6 +15,7 @@ logits' range gives NaN, as a label does in GroupSum.cross_entropy.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -28,7 +29,8 @@ def _wide(logits: torch.Tensor) -> torch.dtype:
 
 
 def _flat(logits, actions):
-    """logits as [rows, cols] and actions as [rows], checked."""
+    """logits (or the activations that GroupSum makes them of) as [rows, cols] and actions as
+    [rows], checked."""
     if not isinstance(logits, torch.Tensor) or not isinstance(actions, torch.Tensor):
         raise TypeError("logits and actions must be tensors")
     if logits.device.type != "cuda" or actions.device != logits.device:
@@ -54,9 +56,12 @@ def _per_row(t, name, logits, actions):
                            f"{tuple(actions.shape)} on {logits.device}")
     if t.requires_grad:
         raise RuntimeError(f"{name} is a constant of the loss: detach it")
+    wide = _wide(logits)
     if t.dim() != 1:
         t = t.reshape(-1)
-    return t.to(_wide(logits)).contiguous()
+    if t.dtype != wide:
+        t = t.to(wide)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _reduction(name):
@@ -72,19 +77,86 @@ def _rows_of(logits):
     return logits
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(code, rows, cols) -> int:
+    need = ctypes.c_int64()
+    _capi.call("cl_token_loss_workspace", code, rows, cols, ctypes.byref(need))
+    return need.value
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefills(code, rows, cols) -> bool:
+    yes = ctypes.c_int()
+    _capi.call("cl_policy_loss_prefills", code, rows, cols, ctypes.byref(yes))
+    return bool(yes.value)
+
+
+@functools.lru_cache(maxsize=1024)
+def _centered_bytes(code, batch, feats, stride_batch, k) -> int:
+    need = ctypes.c_int64()
+    _capi.call("cl_group_sum_centered_workspace_size", code, batch, feats, stride_batch, k,
+               ctypes.byref(need))
+    return need.value
+
+
+def takes_group(k: int) -> bool:
+    """Whether the losses take GroupSum's scores of k classes from its input."""
+    return _centered_bytes(_capi.CL_DTYPE_F32, 1, 1, 1, int(k)) >= 0
+
+
+def _logits_of(ctx, x, group):
+    """The rows of logits to work on: x itself, or, with group (k, tau), GroupSum's scores of the
+    activations x [batch, features], less each sample's largest one (which no loss here depends
+    on), so that they are not rounded at the size of a class sum."""
+    ctx.group = None
+    if group is None:
+        return _rows_of(x)
+    k, tau = group
+    code = _dl.dtype_code(x)
+    batch, feats = x.shape
+    sb, sf = x.stride()
+    if batch > 1 and feats > 1 and (sb == 0 or sf == 0):
+        x = x.contiguous()
+        sb, sf = x.stride()
+    scores = torch.empty((batch, k), dtype=x.dtype, device=x.device)
+    need = _centered_bytes(code, batch, feats, sb, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    with _dl.on_device_of(x):
+        timing.timed("cl_group_sum_centered_forward", lambda: _capi.call(
+            "cl_group_sum_centered_forward", code, x.data_ptr(), batch, feats, sb, sf, k, tau,
+            scores.data_ptr(), _dl.ptr(ws), need, _dl.stream_of(x)))
+    ctx.group = k, tau, batch, feats, sb == 1 and sf != 1
+    return scores
+
+
+def _input_grad(ctx, grad):
+    """The input's gradient from the logits': through GroupSum, in its input's layout."""
+    if ctx.group is None:
+        return grad
+    k, tau, batch, feats, batch_major = ctx.group
+    if batch_major:
+        grad_x = torch.empty((feats, batch), dtype=grad.dtype, device=grad.device).t()
+    else:
+        grad_x = torch.empty((batch, feats), dtype=grad.dtype, device=grad.device)
+    sb, sf = grad_x.stride()
+    with _dl.on_device_of(grad):
+        timing.timed("cl_group_sum_backward", lambda: _capi.call(
+            "cl_group_sum_backward", _dl.dtype_code(grad), grad.data_ptr(), batch, feats, k, tau,
+            grad_x.data_ptr(), sb, sf, _dl.stream_of(grad)))
+    return grad_x
+
+
 class _Shape:
     """One call's logits as the entry points take them, and the bytes of its buffers."""
 
     def __init__(self, logits):
-        self.code = _dl.storage_dtype_code(logits)
-        self.rows, self.cols = logits.shape
+        self.code = code = _dl.storage_dtype_code(logits)
+        self.rows, self.cols = rows, cols = logits.shape
         # (an expanded row has stride 0)
-        self.args = (self.code, logits.data_ptr(), logits.stride(0), self.rows, self.cols)
+        self.args = (code, logits.data_ptr(), logits.stride(0), rows, cols)
         self.size = 8 if logits.dtype == torch.float64 else 4
-        self.state_bytes = 4 * self.size * self.rows
-        need = ctypes.c_int64()
-        _capi.call("cl_token_loss_workspace", self.code, self.rows, self.cols, ctypes.byref(need))
-        self.workspace_bytes = need.value
+        self.state_bytes = 4 * self.size * rows
+        self.workspace_bytes = _workspace_bytes(code, rows, cols)
 
 
 def _once():
@@ -106,12 +178,6 @@ def _aux(logits, *sizes):
     return buf, [base + s for s in starts]
 
 
-def _prefills(sh):
-    yes = ctypes.c_int()
-    _capi.call("cl_policy_loss_prefills", sh.code, sh.rows, sh.cols, ctypes.byref(yes))
-    return bool(yes.value)
-
-
 def _capture_id(t) -> int:
     """Which graph capture t's current stream records, 0 outside of one."""
     got = ctypes.c_uint64()
@@ -124,8 +190,8 @@ class SelectedLogProbsFunction(torch.autograd.Function):
     the probabilities again from the row's maximum and sum.  No counterpart in the reference."""
 
     @staticmethod
-    def forward(ctx, logits, actions, ignore_index):
-        logits = _rows_of(logits)
+    def forward(ctx, x, actions, ignore_index, group=None):
+        logits = _logits_of(ctx, x, group)
         sh = _Shape(logits)
         aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
         lp = torch.empty(sh.rows, dtype=_wide(logits), device=logits.device)
@@ -147,7 +213,7 @@ class SelectedLogProbsFunction(torch.autograd.Function):
             timing.timed("cl_selected_log_prob_backward", lambda: _capi.call(
                 "cl_selected_log_prob_backward", *ctx.args, actions.data_ptr(), ctx.state,
                 grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits)))
-        return grad, None, None
+        return _input_grad(ctx, grad), None, None, None
 
 
 class PolicyLossFunction(torch.autograd.Function):
@@ -156,9 +222,9 @@ class PolicyLossFunction(torch.autograd.Function):
     counterpart in the reference."""
 
     @staticmethod
-    def forward(ctx, logits, actions, old, adv, ref, clip_low, clip_high, kl_coef, ignore_index,
-                reduction):
-        logits = _rows_of(logits)
+    def forward(ctx, x, actions, old, adv, ref, clip_low, clip_high, kl_coef, ignore_index,
+                reduction, group=None):
+        logits = _logits_of(ctx, x, group)
         sh = _Shape(logits)
         wide = old.dtype
         lp = torch.empty(sh.rows, dtype=wide, device=logits.device)
@@ -172,7 +238,7 @@ class PolicyLossFunction(torch.autograd.Function):
             aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
             terms, loss_at, count = loss.data_ptr(), None, None
         grad = None
-        if reduction and ctx.needs_input_grad[0] and _prefills(sh):
+        if reduction and ctx.needs_input_grad[0] and _prefills(sh.code, sh.rows, sh.cols):
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             ctx.capture = _capture_id(logits)
         with _dl.on_device_of(logits):
@@ -192,7 +258,7 @@ class PolicyLossFunction(torch.autograd.Function):
     def backward(ctx, grad_loss, _grad_lp):
         _once()
         if grad_loss is None:
-            return (None,) * 10
+            return (None,) * 11
         logits, actions, aux = ctx.saved_tensors
         grad_loss = grad_loss.contiguous()
         # the forward's gradient is handed out once, and only in the capture (or outside of any)
@@ -206,7 +272,7 @@ class PolicyLossFunction(torch.autograd.Function):
                 "cl_policy_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
                 ctx.reduction, grad_loss.data_ptr(), ctx.count, int(prefilled), grad.data_ptr(),
                 _dl.stream_of(logits)))
-        return (grad,) + (None,) * 9
+        return (_input_grad(ctx, grad),) + (None,) * 10
 
 
 class PreferenceLossFunction(torch.autograd.Function):
@@ -215,8 +281,9 @@ class PreferenceLossFunction(torch.autograd.Function):
     the reference."""
 
     @staticmethod
-    def forward(ctx, logits, actions, offsets, ref, beta, smoothing, ignore_index, reduction):
-        logits = _rows_of(logits)
+    def forward(ctx, x, actions, offsets, ref, beta, smoothing, ignore_index, reduction,
+                group=None):
+        logits = _logits_of(ctx, x, group)
         sh = _Shape(logits)
         wide, pairs = _wide(logits), (offsets.numel() - 1) // 2
         margins = torch.empty(pairs, dtype=wide, device=logits.device)
@@ -244,7 +311,7 @@ class PreferenceLossFunction(torch.autograd.Function):
     def backward(ctx, grad_loss, _grad_margins):
         _once()
         if grad_loss is None:
-            return (None,) * 8
+            return (None,) * 9
         logits, actions, aux = ctx.saved_tensors
         grad_loss = grad_loss.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -253,15 +320,20 @@ class PreferenceLossFunction(torch.autograd.Function):
                 "cl_preference_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
                 ctx.row_seq, ctx.seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(),
                 ctx.count, grad.data_ptr(), _dl.stream_of(logits)))
-        return (grad,) + (None,) * 7
+        return (_input_grad(ctx, grad),) + (None,) * 8
 
 
 def selected_log_probs(logits, actions, ignore_index: int = -100):
     """The log-probability log_softmax(logits)[..., actions] of the chosen class or token:
     logits [..., V], actions int64 [...] -> [...]; 0 where the action is ignore_index.
     Differentiable by the logits."""
+    return _selected_log_probs(logits, actions, ignore_index)
+
+
+def _selected_log_probs(logits, actions, ignore_index=-100, group=None):
     rows, acts = _flat(logits, actions)
-    return SelectedLogProbsFunction.apply(rows, acts, int(ignore_index)).reshape(actions.shape)
+    lp = SelectedLogProbsFunction.apply(rows, acts, int(ignore_index), group)
+    return lp if actions.dim() == 1 else lp.reshape(actions.shape)
 
 
 def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
@@ -277,6 +349,13 @@ def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, 
     sides or a pair (low, high).  reduction: 'mean' over the rows that count, 'sum', or 'none' (the
     terms, [...]).  With return_log_probs, also the rows' log-probabilities (not differentiable
     through this call)."""
+    return _policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs, clip, kl_coef,
+                        ignore_index, reduction, return_log_probs)
+
+
+def _policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
+                 kl_coef=0.0, ignore_index=-100, reduction="mean", return_log_probs=False,
+                 group=None):
     rows, acts = _flat(logits, actions)
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl_coef = float(low), float(high), float(kl_coef)
@@ -291,10 +370,12 @@ def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, 
     if ref_log_probs is not None:
         ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
     loss, lp = PolicyLossFunction.apply(rows, acts, old, adv, ref, low, high, kl_coef,
-                                        int(ignore_index), code)
-    if not code:
-        loss = loss.reshape(actions.shape)
-    return (loss, lp.reshape(actions.shape)) if return_log_probs else loss
+                                        int(ignore_index), code, group)
+    if actions.dim() != 1:
+        lp = lp.reshape(actions.shape)
+        if not code:
+            loss = loss.reshape(actions.shape)
+    return (loss, lp) if return_log_probs else loss
 
 
 def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 0.1,
@@ -312,6 +393,12 @@ def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 
     reduction: 'mean' over the pairs, 'sum', or 'none' (the terms, [P]).  With return_margins, also
     the margins [P] (not differentiable through this call).  Rows of no sequence do not count;
     offsets that decrease or leave the rows make their pair's term NaN."""
+    return _preference_loss(logits, actions, offsets, ref_log_probs, beta, label_smoothing,
+                            ignore_index, reduction, return_margins)
+
+
+def _preference_loss(logits, actions, offsets, ref_log_probs=None, beta=0.1, label_smoothing=0.0,
+                     ignore_index=-100, reduction="mean", return_margins=False, group=None):
     rows, acts = _flat(logits, actions)
     if logits.dim() != 2:
         raise RuntimeError("preference_loss takes logits [rows, classes] of a ragged batch")
@@ -328,5 +415,5 @@ def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 
         ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
     loss, margins = PreferenceLossFunction.apply(rows, acts, offsets.contiguous(), ref,
                                                  float(beta), float(label_smoothing),
-                                                 int(ignore_index), code)
+                                                 int(ignore_index), code, group)
     return (loss, margins) if return_margins else loss

@@ -447,6 +447,17 @@ int cl_group_sum_forward(int dtype, const void* x, int64_t batch, int64_t featur
 int cl_group_sum_workspace_size(int dtype, int64_t batch, int64_t features, int64_t stride_batch,
                                 int64_t stride_feature, int64_t k, int64_t* bytes);
 
+/* The scores less each sample's largest one, summed and subtracted in fp64 and rounded once: what
+ * a softmax or a loss on differences of scores needs, without the rounding of the scores
+ * themselves.  k <= 512; *bytes = -1 above.  workspace: cl_group_sum_centered_workspace_size
+ * bytes.  The gradient of such a loss is cl_group_sum_backward's. */
+int cl_group_sum_centered_workspace_size(int dtype, int64_t batch, int64_t features,
+                                         int64_t stride_batch, int64_t k, int64_t* bytes);
+int cl_group_sum_centered_forward(int dtype, const void* x, int64_t batch, int64_t features,
+                                  int64_t stride_batch, int64_t stride_feature, int64_t k,
+                                  double tau, void* out, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 /* grad_x[n, j] = grad_out[n, group(j)] / tau, written through (stride_batch, stride_feature). */
 int cl_group_sum_backward(int dtype, const void* grad_out, int64_t batch, int64_t features,
                           int64_t k, double tau, void* grad_x, int64_t stride_batch,

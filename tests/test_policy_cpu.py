@@ -50,6 +50,13 @@ def test_c_arguments_are_checked_before_the_device():
     assert lp(rows=4, cols=1 << 17, stride=1 << 17) == bad and b"workspace" in lib.cl_last_error()
     assert lib.cl_token_loss_workspace(0, 4, 10, ctypes.byref(need)) == ok and need.value == 0
     assert lib.cl_token_loss_workspace(0, 4, 0, ctypes.byref(need)) == bad
+    # more classes than one workgroup holds are not summed for a loss
+    assert lib.cl_group_sum_centered_workspace_size(0, 64, 900, 1, 512, ctypes.byref(need)) == ok
+    assert need.value >= 512 * 64 * 4
+    assert lib.cl_group_sum_centered_workspace_size(0, 64, 900, 1, 513, ctypes.byref(need)) == ok
+    assert need.value == -1
+    assert lib.cl_group_sum_centered_forward(0, 1, 64, 900, 1, 64, 513, 1.0, 1, 1, 1, None) == bad
+    assert lib.cl_group_sum_centered_forward(0, 1, 64, 900, 1, 64, 10, 1.0, 1, None, 0, None) == bad
     assert policy(low=-0.1) == bad and policy(low=float("nan")) == bad
     assert policy(kl=0.1) == bad and b"KL" in lib.cl_last_error()
     assert policy(red=3) == bad and policy(loss=None) == bad and policy(old=None) == bad

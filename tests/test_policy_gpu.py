@@ -432,31 +432,100 @@ def test_half_gradient_of_a_scaled_loss(device):
     c.check_gradient(g, slope * 65536.0 / n, 2 * 1.8 * np.abs(c.adv) * c.err * 65536.0 / n)
 
 
-def test_group_sum_methods(device):
-    """The three losses of a network's class scores: GroupSum's scores through the functions, and
-    the gradient back through GroupSum, on a LogicLayer's layout."""
-    x = torch.rand(1200, 64, device=device).t().requires_grad_()
-    gs = cl.GroupSum(10, 4.0)
-    rng = np.random.default_rng(0)
-    a = torch.as_tensor(rng.integers(0, 10, 64)).to(device)
-    old = torch.as_tensor(rng.standard_normal(64) - 2.3).float().to(device)
-    adv = torch.as_tensor(rng.standard_normal(64)).float().to(device)
-    off = torch.arange(0, 65, 4, device=device)
-    scores = gs(x).detach().requires_grad_()
-    for via, direct in [
-            (gs.log_probs(x, a).sum(), cl.selected_log_probs(scores, a).sum()),
-            (gs.policy_loss(x, a, old, adv), cl.policy_loss(scores, a, old, adv)),
-            (gs.preference_loss(x, a, off[:-1] if off.numel() % 2 == 0 else off, beta=0.3),
-             cl.preference_loss(scores, a, off[:-1] if off.numel() % 2 == 0 else off, beta=0.3))]:
-        assert torch.equal(via, direct)
-        (gx,) = torch.autograd.grad(via, x)
-        (gsc,) = torch.autograd.grad(direct, scores)
-        assert torch.equal(gx, (gsc / 4.0).repeat_interleave(120, 1))
-        assert gx.t().is_contiguous()
-    h = gs.policy_loss(x.half(), a, old, adv)
-    assert h.dtype == torch.float32 and torch.isfinite(h)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.float16])
+@pytest.mark.parametrize("batch,feats,k,layout", [
+    (1, 30, 10, "rows"), (63, 1200, 10, "columns"), (64, 12000, 10, "columns"),
+    (130, 2001, 200, "columns"), (7, 25, 10, "rows"), (1024, 12000, 10, "rows"),
+    (96, 777, 5, "strided"), (70, 1030, 513, "columns"), (5, 3, 7, "rows")])
+def test_group_sum_methods(device, batch, feats, k, layout, dtype):
+    """The three losses from a network's last activations against the oracle on scores summed in 64
+    bits.  An fp32 partial sum adds at most feats / k + 8 numbers of up to 1, each addition off by a
+    unit of the sum so far; the rest is fp64 until one rounding at the size of a difference.  (More
+    than 512 classes take GroupSum's own fp32 scores, rounded at the size of the score.)"""
+    rng = np.random.default_rng(batch + feats + k)
+    tau = 2.0
+    x = torch.as_tensor(rng.random((batch, feats))).to(dtype).to(device)
+    xn = _np(x)
+    if layout == "columns":
+        x = x.t().contiguous().t()
+    elif layout == "strided":
+        x = torch.zeros((batch, 2 * feats), dtype=dtype, device=device)[:, ::2].copy_(x)
+    x.requires_grad_()
+    wide = _wide(dtype)
+    gsz = -(-feats // k)
+    padded = np.zeros((batch, gsz * k))
+    padded[:, :feats] = xn
+    z = padded.reshape(batch, k, gsz).sum(2) / tau
+    actions = rng.integers(0, k, batch)
+    actions[rng.random(batch) < 0.1] = IGNORE
+    lp, probs = P.log_probs(z, actions)
+    a = torch.as_tensor(actions).to(device)
+    old = torch.as_tensor(lp - np.log(rng.choice([0.4, 0.9, 1.1, 1.7], batch))).to(wide).to(device)
+    ref = torch.as_tensor(lp + 0.3 * rng.standard_normal(batch)).to(wide).to(device)
+    adv = torch.as_tensor(rng.standard_normal(batch)).to(wide).to(device)
+    spread = z.max() - z.min()
+    unit = _unit(wide)
+    score_err = (gsz + 8) * gsz * unit / tau + spread * unit + (np.abs(z).max() * unit if k > 512 else 0)
+    err = 2 * score_err + _sum_error(z - z.max(1, keepdims=True), wide)
+    gs = cl.GroupSum(k, tau)
+    scale = np.repeat(np.eye(k), gsz, axis=1)[:, :feats] / tau      # d score / d x
+
+    def check(grad, slope, serr):
+        full = P.logit_gradient(probs, actions, slope)
+        bound = ((np.abs(slope) * 2 * err + serr)[:, None] + np.abs(full) * 3 * unit) @ scale
+        assert grad.dtype == dtype and grad.shape == (batch, feats)
+        if layout == "columns" and batch > 1:
+            assert grad.t().is_contiguous()
+        _near(_np(grad), full @ scale, bound, dtype)
+
+    got = gs.log_probs(x, a)
+    assert got.dtype == wide
+    _near(_np(got), lp, err, wide)
+    check(torch.autograd.grad(got, x, adv)[0], _np(adv), 0.0)
+
+    loss, lps = gs.policy_loss(x, a, old, adv, ref, clip=(0.2, 0.28), kl_coef=0.05,
+                               return_log_probs=True, reduction="sum")
+    term, slope = P.policy_terms(lp, actions, _np(old), _np(adv), _np(ref), 0.2, 0.28, 0.05)
+    bound = 1.8 * np.abs(_np(adv)) + 0.25
+    _near(_np(lps), lp, err, wide)
+    _near(float(loss.detach()), term.sum(), (bound * err + np.abs(term) * 2 * unit).sum(), wide)
+    check(torch.autograd.grad(loss, x)[0], slope, 2 * bound * err)
+
+    pairs = batch // 2
+    off = np.arange(2 * pairs + 1)
+    loss, h = gs.preference_loss(x, a, torch.as_tensor(off).to(device), ref, beta=0.3,
+                                 return_margins=True, reduction="sum")
+    want, term, slope = P.preference_terms(lp, actions, off, _np(ref), 0.3, 0.0)
+    _near(_np(h), want, 0.6 * err + 4 * unit, wide)
+    _near(float(loss.detach()), term.sum(), (0.6 * err + 4 * unit) * max(pairs, 1)
+          + np.abs(term).sum() * 2 * unit, wide)
+    check(torch.autograd.grad(loss, x)[0], slope, 0.3 * 0.6 * err + 0.3 * 4 * unit)
+
+
+def test_group_sum_methods_shapes(device):
+    """Leading dimensions, non-finite activations, refusals."""
+    gs = cl.GroupSum(5, 2.0)
+    x = torch.rand(4, 3, 50, device=device)
+    a = torch.randint(0, 5, (4, 3), device=device)
+    lp = gs.log_probs(x, a)
+    assert lp.shape == (4, 3)
+    assert torch.equal(lp.view(-1), gs.log_probs(x.view(12, 50), a.view(-1)))
+    y = x.view(12, 50).clone()
+    y[3, 7], y[5, 8], y[6, 9] = float("nan"), float("inf"), float("-inf")
+    bad = gs.log_probs(y, a.view(-1))
+    assert torch.isnan(bad[3]) and torch.isnan(bad[5])
+    ok = torch.ones(12, dtype=torch.bool)
+    ok[[3, 5, 6]] = False
+    assert torch.equal(bad.cpu()[ok], lp.view(-1).cpu()[ok])
+    f = torch.zeros(12, device=device)
     with pytest.raises(RuntimeError, match="detach"):
-        gs.policy_loss(x, a, gs.log_probs(x, a), adv)
+        gs.policy_loss(y, a.view(-1), f.requires_grad_(), f)
+    with pytest.raises(RuntimeError, match="dtype"):
+        gs.log_probs(y.bfloat16(), a.view(-1))
+    with pytest.raises(TypeError):
+        gs.log_probs(cl.PackBitsTensor(y > 0.5, 64), a)
+    with pytest.raises(RuntimeError, match="actions must be int64"):
+        gs.log_probs(y, a)
 
 
 def test_captured_policy_step(device):
