@@ -182,9 +182,10 @@ def test_preference_loss(device, dtype, with_ref, reduction):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("vocab", [10, 301, 5003, 40001])
 def test_layouts(device, vocab, dtype, layout):
-    """Strided logits give what contiguous ones give, bit by bit."""
+    """Strided, shifted and expanded logits against the oracle (a row is cut where its memory is
+    aligned, so sums may be added in another order than for a contiguous copy)."""
     rows = 6
-    c = Case(rows, vocab, dtype, device)
+    c = Case(rows, vocab, dtype, device, ignored=0.0)
     z = c.logits
     if layout == "padded":
         t = torch.zeros((rows, vocab + 7), dtype=dtype, device=device)
@@ -197,24 +198,27 @@ def test_layouts(device, vocab, dtype, layout):
     elif layout == "transposed":
         x = z.t().contiguous().t()
     elif layout == "expanded":
-        z = z[:1].expand(rows, vocab)
-        x, z = z, z.contiguous()
+        x = z[:1].expand(rows, vocab)
+        c.z = np.repeat(c.z[:1], rows, 0)
+        c.lp, c.probs = P.log_probs(c.z, c.actions)
+        c.old_t, c.ref_t = [torch.as_tensor(c.lp + d).to(c.wide).to(device) for d in (0.05, -0.3)]
+        c.old, c.ref = _np(c.old_t), _np(c.ref_t)
     else:
         x = z.view(2, 3, vocab)
     shape = x.shape[:-1]
-    x, z = x.detach().requires_grad_(), z.detach().requires_grad_()
+    x = x.detach().requires_grad_()
     a, o, v, r = (t.view(shape) for t in (c.act_t, c.old_t, c.adv_t, c.ref_t))
-    got = cl.policy_loss(x, a, o, v, r, kl_coef=0.1, return_log_probs=True)
-    ref = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, c.ref_t, kl_coef=0.1, return_log_probs=True)
-    assert got[1].shape == shape
-    assert torch.equal(got[0], ref[0]) and torch.equal(got[1].reshape(-1), ref[1])
-    gx = torch.autograd.grad(got[0], x)[0].reshape(rows, vocab)
-    gz = torch.autograd.grad(ref[0], z)[0]
-    assert torch.equal(gx, gz)
-    lx, lz = cl.selected_log_probs(x, a), cl.selected_log_probs(z, c.act_t)
-    assert torch.equal(lx.reshape(-1), lz)
-    assert torch.equal(torch.autograd.grad(lx, x, v)[0].reshape(rows, vocab),
-                       torch.autograd.grad(lz, z, c.adv_t)[0])
+    loss, lp = cl.policy_loss(x, a, o, v, r, kl_coef=0.1, reduction="sum", return_log_probs=True)
+    assert lp.shape == shape
+    _near(_np(lp).reshape(-1), c.lp, c.err, c.wide)
+    term, slope = P.policy_terms(c.lp, c.actions, c.old, c.adv, c.ref, 0.2, 0.2, 0.1)
+    bound = 1.8 * np.abs(c.adv) + 0.5
+    _near(float(loss.detach()), term.sum(), (bound * c.err + np.abs(term) * 2 * _unit(dtype)).sum(),
+          c.wide)
+    c.check_gradient(torch.autograd.grad(loss, x)[0].reshape(rows, vocab), slope, 2 * bound * c.err)
+    lp = cl.selected_log_probs(x, a)
+    _near(_np(lp).reshape(-1), c.lp, c.err, c.wide)
+    c.check_gradient(torch.autograd.grad(lp, x, v)[0].reshape(rows, vocab), c.adv)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
