@@ -679,39 +679,69 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
     return wave_total(lane_id() < waves ? red[lane_id()] : 0.0);
 }
 
-// Rows that count, before the rows themselves where the forward divides by their number.
+// Where there are more rows than one workgroup adds in a few microseconds, workgroups first add
+// kSumRows each into partial sums, which the last one adds in order: a policy step on 10^6 rows of
+// 10 classes takes 213 us instead of 346, on 10^5 rows 39 instead of 47.
+constexpr int64_t kSumRows = 16384;
+
+struct RowSums {
+    double term, count;
+};
+
 template <typename A>
-__global__ __launch_bounds__(kSumThreads) void k_count(const int64_t* __restrict__ actions,
-                                                       int64_t rows, int64_t ignore,
-                                                       A* __restrict__ count) {
-    __shared__ double red[kSumThreads / 64];
+__device__ __forceinline__ RowSums sum_rows(const A* terms, const int64_t* actions, int64_t from,
+                                            int64_t to, int64_t ignore, double (*red)[kSumThreads / 64]) {
+    double t = 0;
     int c = 0;
 #pragma unroll 8
-    for (int64_t n = threadIdx.x; n < rows; n += kSumThreads) c += actions[n] != ignore;
-    const double t = group_sum(double(c), red);
-    if (threadIdx.x == 0) count[0] = A(t);
+    for (int64_t n = from + threadIdx.x; n < to; n += kSumThreads) {
+        if (terms) t += double(terms[n]);
+        c += actions[n] != ignore;
+    }
+    RowSums r{0.0, group_sum(double(c), red[0])};
+    if (terms) r.term = group_sum(t, red[1]);
+    return r;
 }
 
-// loss = sum of the rows' terms, divided by the number of counted rows for a mean.
-template <typename A>
-__global__ __launch_bounds__(kSumThreads) void k_policy_sum(const A* __restrict__ terms,
-                                                            const int64_t* __restrict__ actions,
-                                                            int64_t rows, int64_t ignore, int mean,
-                                                            A* __restrict__ loss,
-                                                            A* __restrict__ count) {
-    __shared__ double red[2][kSumThreads / 64];
+__device__ __forceinline__ RowSums sum_parts(const RowSums* parts, int64_t n,
+                                             double (*red)[kSumThreads / 64]) {
     double t = 0, c = 0;
-#pragma unroll 8
-    for (int64_t n = threadIdx.x; n < rows; n += kSumThreads) {
-        t += double(terms[n]);
-        c += actions[n] != ignore ? 1.0 : 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kSumThreads) {
+        t += parts[i].term;
+        c += parts[i].count;
     }
-    t = group_sum(t, red[0]);
-    c = group_sum(c, red[1]);
-    if (threadIdx.x == 0) {
-        loss[0] = A(mean ? t / c : t);  // no counted row: 0 / 0 = NaN, the mean of nothing
-        count[0] = A(c);
-    }
+    c = group_sum(c, red[0]);
+    t = group_sum(t, red[1]);
+    return {t, c};
+}
+
+template <typename A>
+__global__ __launch_bounds__(kSumThreads) void k_sum_parts(const A* __restrict__ terms,
+                                                           const int64_t* __restrict__ actions,
+                                                           int64_t rows, int64_t ignore,
+                                                           RowSums* __restrict__ parts) {
+    __shared__ double red[2][kSumThreads / 64];
+    const int64_t from = int64_t(blockIdx.x) * kSumRows;
+    const RowSums r = sum_rows(terms, actions, from, std::min(rows, from + kSumRows), ignore, red);
+    if (threadIdx.x == 0) parts[blockIdx.x] = r;
+}
+
+// The number of rows that count, and, with terms, their sum or mean as the loss; from the rows or
+// from nparts partial sums.
+template <typename A>
+__global__ __launch_bounds__(kSumThreads) void k_sum(const A* __restrict__ terms,
+                                                     const int64_t* __restrict__ actions,
+                                                     int64_t rows, int64_t ignore,
+                                                     const RowSums* __restrict__ parts,
+                                                     int64_t nparts, int mean, A* __restrict__ loss,
+                                                     A* __restrict__ count) {
+    __shared__ double red[2][kSumThreads / 64];
+    const RowSums r = nparts ? sum_parts(parts, nparts, red)
+                             : sum_rows(terms, actions, 0, rows, ignore, red);
+    if (threadIdx.x != 0) return;
+    // no counted row: 0 / 0 = NaN, the mean of nothing
+    if (terms) loss[0] = A(mean ? r.term / r.count : r.term);
+    count[0] = A(r.count);
 }
 
 template <typename A>
@@ -726,11 +756,14 @@ struct PairArgs {
     A* terms;
 };
 
-// Pair i by one wave: the sums over both sequences, the margin h, the loss term
+// Pair i by one wave, or by a workgroup of WAVES (then all of its threads come here): the sums
+// over both sequences, the margin h, the loss term
 //   -(1 - e) log sigma(h) - e log sigma(-h)
 // and its slope by the chosen sequence's sum; the rejected one's is the negative.
-template <typename A>
-__device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i) {
+template <int WAVES, typename A>
+__device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i, double* red) {
+    constexpr int STEP = WAVES * 64;
+    const int t0 = WAVES > 1 ? int(threadIdx.x) : lane_id();
     double d[2];
     bool bad = false;
 #pragma unroll
@@ -742,17 +775,20 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i) {
         e = std::min(std::max(e, b), a.rows);
         double t = 0;
         // eight loads at a time, in row order
-        for (int64_t n = b + lane_id(); n < e; n += 8 * 64) {
+        for (int64_t n = b + t0; n < e; n += 8 * STEP) {
             double v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = n + u * 64 < e ? a.gaps[n + u * 64] : 0.0;
+            for (int u = 0; u < 8; ++u) v[u] = n + u * STEP < e ? a.gaps[n + u * STEP] : 0.0;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 t += v[u];
-                if (n + u * 64 < e) a.row_seq[n + u * 64] = int32_t(q);
+                if (n + u * STEP < e) a.row_seq[n + u * STEP] = int32_t(q);
             }
         }
-        d[side] = wave_total(t);
+        if constexpr (WAVES > 1)
+            d[side] = group_sum(t, red + side * WAVES);
+        else
+            d[side] = wave_total(t);
     }
     double h = a.beta * (d[0] - d[1]);
     if (bad) h = nan_value<double>();
@@ -763,7 +799,7 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i) {
     const double yes = h >= 0 ? inv : u * inv, no = h >= 0 ? u * inv : inv;  // sigma(h), sigma(-h)
     const double slope = a.beta * (a.smooth * yes - (1 - a.smooth) * no);
     const double term = (1 - a.smooth) * away + a.smooth * near;
-    if (lane_id() == 0) {
+    if (t0 == 0) {
         a.margins[i] = A(h);
         a.terms[i] = A(term);
         a.seq_slope[i] = A(slope);
@@ -775,7 +811,13 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i) {
 template <typename A>
 __global__ __launch_bounds__(kRowBlock) void k_pref_pairs(PairArgs<A> a) {
     const int64_t i = int64_t(blockIdx.x) * (kRowBlock / 64) + wave_id();
-    if (i < a.pairs) pair_term(a, i);
+    if (i < a.pairs) pair_term<1>(a, i, nullptr);
+}
+
+template <typename A>
+__global__ __launch_bounds__(kSumThreads) void k_pref_long(PairArgs<A> a) {
+    __shared__ double red[2 * kSumThreads / 64];
+    pair_term<kSumThreads / 64>(a, blockIdx.x, red);
 }
 
 template <typename A>
@@ -801,7 +843,7 @@ __global__ __launch_bounds__(kSumThreads) void k_pref_small(PairArgs<A> a, int m
     __shared__ double red[kSumThreads / 64];
     double t = 0;
     for (int64_t i = wave_id(); i < a.pairs; i += kSumThreads / 64) {
-        const double term = pair_term(a, i);
+        const double term = pair_term<1>(a, i, nullptr);
         t += lane_id() == 0 ? term : 0.0;
     }
     if (!loss) return;
@@ -842,7 +884,7 @@ RowArgs<T> row_args(const void* logits, int64_t row_stride, int64_t rows, int64_
 
 // Rows up to 4 KB stay in registers of a wave or a quarter of one; longer ones take a workgroup,
 // or several where the rows alone would not fill the card.
-constexpr int64_t kPrefSmallRows = 16384, kPrefSmallPairs = 256;
+constexpr int64_t kPrefSmallRows = 16384, kPrefSmallPairs = 256, kPrefLongRows = 2048;
 constexpr int64_t kSplitBlocks = 1024;  // workgroups wanted
 constexpr int kMaxParts = 64;           // joined by the lanes of one wave
 
@@ -855,10 +897,31 @@ int row_parts(int64_t rows, int64_t cols) {
                                  ceil_div(kSplitBlocks, rows)));
 }
 
+// (few rows are split, many are summed in parts: never both)
 template <typename T>
 int64_t rows_workspace(int64_t rows, int64_t cols) {
     const int parts = row_parts<T>(rows, cols);
-    return parts > 1 ? rows * parts * 2 * int64_t(sizeof(wide_t<T>)) : 0;
+    if (parts > 1) return rows * parts * 2 * int64_t(sizeof(wide_t<T>));
+    return rows > kSumRows ? ceil_div(rows, kSumRows) * int64_t(sizeof(RowSums)) : 0;
+}
+
+// The loss and the number of counted rows; without terms that number alone.
+template <typename A>
+int launch_sum(const A* terms, const int64_t* actions, int64_t rows, int64_t ignore, bool mean,
+               A* loss, A* count, void* workspace, int64_t workspace_bytes, hipStream_t s) {
+    const int64_t nparts = rows > kSumRows ? ceil_div(rows, kSumRows) : 0;
+    auto* parts = static_cast<RowSums*>(workspace);
+    if (nparts) {
+        CL_ARG(workspace && workspace_bytes >= nparts * int64_t(sizeof(RowSums)),
+               "workspace of %lld bytes needed (cl_token_loss_workspace)",
+               (long long)(nparts * int64_t(sizeof(RowSums))));
+        k_sum_parts<A><<<unsigned(nparts), kSumThreads, 0, s>>>(terms, actions, rows, ignore,
+                                                               parts);
+        if (int rc = check_launch("sums in parts")) return rc;
+    }
+    k_sum<A><<<1, kSumThreads, 0, s>>>(terms, actions, rows, ignore, parts, nparts, mean, loss,
+                                       count);
+    return check_launch("sum");
 }
 
 template <typename T, int TPR, int NV, bool GRAD, typename Op>
@@ -1061,21 +1124,20 @@ extern "C" int cl_policy_loss_forward(int dtype, const void* logits, int64_t row
         if (grad_logits) {
             const bool mean = reduction == CL_REDUCE_MEAN;
             if (mean)
-                k_count<A><<<1, kSumThreads, 0, s>>>(actions, rows, ignore_index,
-                                                     static_cast<A*>(count));
+                if (int rc = launch_sum<A>(nullptr, actions, rows, ignore_index, true, nullptr,
+                                           static_cast<A*>(count), workspace, workspace_bytes, s))
+                    return rc;
             const GradOut<T> out{static_cast<T*>(grad_logits),
                                  mean ? static_cast<const A*>(count) : nullptr};
             if (int rc = launch_rows_grad(a, op, out, s)) return rc;
         } else if (int rc = launch_rows(a, op, workspace, workspace_bytes, s)) {
             return rc;
         }
-        if (reduction != CL_REDUCE_NONE)
-            k_policy_sum<A><<<1, kSumThreads, 0, s>>>(op.terms, actions, rows, ignore_index,
-                                                      reduction == CL_REDUCE_MEAN,
-                                                      static_cast<A*>(loss),
-                                                      static_cast<A*>(count));
+        if (reduction == CL_REDUCE_NONE) return CL_OK;
+        return launch_sum<A>(op.terms, actions, rows, ignore_index, reduction == CL_REDUCE_MEAN,
+                             static_cast<A*>(loss), static_cast<A*>(count), workspace,
+                             workspace_bytes, s);
     });
-    return check_launch("cl_policy_loss_forward(sum)");
 }
 
 extern "C" int cl_policy_loss_backward(int dtype, const void* logits, int64_t row_stride,
@@ -1138,12 +1200,17 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
                              static_cast<A*>(terms)};
         const int mean = reduction == CL_REDUCE_MEAN;
         A* out = reduction != CL_REDUCE_NONE ? static_cast<A*>(loss) : nullptr;
-        if (rows <= kPrefSmallRows && pairs <= kPrefSmallPairs) {
+        // a wave takes 512 rows of a pair at a time, a workgroup 8192: a step on one pair of 32768
+        // rows each of 64 classes 43 us instead of 86
+        const bool longs = pairs > 0 && rows / pairs > kPrefLongRows;
+        if (!longs && rows <= kPrefSmallRows && pairs <= kPrefSmallPairs) {
             if (pairs > 0 || out)
                 k_pref_small<A><<<1, kSumThreads, 0, s>>>(pa, mean, out, static_cast<A*>(count));
             return check_launch("cl_preference_loss_forward(pairs)");
         }
-        if (pairs > 0)
+        if (longs)
+            k_pref_long<A><<<unsigned(pairs), kSumThreads, 0, s>>>(pa);
+        else if (pairs > 0)
             k_pref_pairs<A><<<unsigned(ceil_div(pairs, kRowBlock / 64)), kRowBlock, 0, s>>>(pa);
         if (int rc = check_launch("cl_preference_loss_forward(pairs)")) return rc;
         if (out)

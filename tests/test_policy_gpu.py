@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import compactlogic_amd as cl
+from compactlogic_amd import policy
 from oracle import policy_np as P
 
 pytestmark = pytest.mark.gpu
@@ -44,6 +45,15 @@ def _np(t):
 
 def _wide(dtype):
     return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+@pytest.fixture(params=[False, True], ids=["two passes", "one pass"])
+def one_pass(request, monkeypatch):
+    """The gradient out of the forward for every size that a workgroup holds, or for none."""
+    def prefills(code, rows, cols):
+        return request.param and code in (0, 3) and cols * (4 if code == 0 else 2) <= 131072
+    monkeypatch.setattr(policy, "_prefills", prefills)
+    return request.param
 
 
 class Case:
@@ -100,7 +110,7 @@ def test_log_probs(device, dtype):
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("kl", [0.0, 0.05])
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_policy_loss(device, dtype, kl, reduction):
+def test_policy_loss(device, one_pass, dtype, kl, reduction):
     for rows, vocab in SIZES:
         c = Case(rows, vocab, dtype, device)
         z = c.logits.requires_grad_()
@@ -181,7 +191,7 @@ def test_preference_loss(device, dtype, with_ref, reduction):
 @pytest.mark.parametrize("layout", ["padded", "offset", "transposed", "expanded", "batched"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("vocab", [10, 301, 5003, 40001])
-def test_layouts(device, vocab, dtype, layout):
+def test_layouts(device, one_pass, vocab, dtype, layout):
     """Strided, shifted and expanded logits against the oracle (a row is cut where its memory is
     aligned, so sums may be added in another order than for a contiguous copy)."""
     rows = 6
@@ -223,7 +233,7 @@ def test_layouts(device, vocab, dtype, layout):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [7, 300, 5001, 70001])
-def test_masked_logits_and_rows(device, vocab, dtype):
+def test_masked_logits_and_rows(device, one_pass, vocab, dtype):
     """Masked classes (-inf, the type's lowest value), ignored rows full of NaN, rows with nothing
     left, actions that do not exist."""
     rows = 8
@@ -267,7 +277,7 @@ def test_masked_logits_and_rows(device, vocab, dtype):
     assert (g[2] == 0).all()
 
 
-def test_nothing_counts(device):
+def test_nothing_counts(device, one_pass):
     z = torch.randn(4, 9, device=device, requires_grad=True)
     a = torch.full((4,), IGNORE, device=device)
     f = torch.zeros(4, device=device)
@@ -346,7 +356,7 @@ def test_gradients_against_differences(device):
         assert float((g - d).abs().max()) < 1e-8
 
 
-def test_second_backward_and_other_upstream(device):
+def test_second_backward_and_other_upstream(device, one_pass):
     """A retained graph gives the same gradient again, whatever was done with the first."""
     for dtype in (torch.float32, torch.bfloat16):
         for vocab in (10, 300, 3001, 8001, 20011, 33001):
@@ -532,7 +542,7 @@ def test_group_sum_methods_shapes(device):
         gs.log_probs(y, a)
 
 
-def test_captured_policy_step(device):
+def test_captured_policy_step(device, one_pass):
     """A policy step of a whole network (dropout, GroupSum, the clipped loss, Adam) captured once:
     every replay equals the eager step with the same mask."""
     torch.manual_seed(0)
@@ -589,7 +599,7 @@ def test_captured_policy_step(device):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("vocab", [10, 3001, 70001])
-def test_captured_losses(device, dtype, vocab):
+def test_captured_losses(device, one_pass, dtype, vocab):
     """Each loss with its gradient captured; replays on new inputs equal the eager calls."""
     rows = 24
     off = torch.tensor([0, 5, 9, 16, 22], device=device)
@@ -643,6 +653,70 @@ def test_streams(device):
         (g,) = torch.autograd.grad(loss, z)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(loss, ref) and torch.equal(g, gref)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [
+    (20001, 3, torch.float32), (100003, 17, torch.bfloat16), (240000, 60, torch.float32),
+    (60000, 220, torch.float32), (60001, 450, torch.bfloat16), (50000, 300, torch.float32),
+    (20000, 1300, torch.bfloat16), (4000, 3500, torch.float32), (1700, 8191, torch.float32),
+    (900, 16383, torch.float32), (700, 50021, torch.bfloat16), (450, 32767, torch.float32)])
+def test_many_rows(device, rows, vocab, dtype):
+    """Sizes that take the gradient out of the forward by themselves, and sums over more rows than
+    one workgroup adds, against float64 formulas on the device."""
+    g = torch.Generator(device=device).manual_seed(rows)
+    z = (torch.randn((rows, vocab), generator=g, device=device) * 2.5).to(dtype).requires_grad_()
+    a = torch.randint(0, vocab, (rows,), generator=g, device=device)
+    a[::7] = IGNORE
+    z64 = z.detach().double()
+    counted = a != IGNORE
+    act = a.clamp(min=0)
+    probs = torch.softmax(z64, 1)
+    lp = torch.log_softmax(z64, 1).gather(1, act[:, None])[:, 0] * counted
+    pick = torch.randint(0, 5, (rows,), generator=g, device=device)
+    old = (lp - torch.tensor([0.4, 0.9, 1.0, 1.15, 1.7], device=device).double().log()[pick]).float()
+    adv = torch.randn(rows, generator=g, device=device)
+    loss, got = cl.policy_loss(z, a, old, adv, return_log_probs=True)
+    (grad,) = torch.autograd.grad(loss, z)
+    r = torch.exp(lp - old.double())
+    A = adv.double()
+    term = -torch.minimum(r * A, r.clamp(0.8, 1.2) * A) * counted
+    slope = torch.where(r * A <= r.clamp(0.8, 1.2) * A, -r * A, 0.0) * counted / counted.sum()
+    err = (vocab / 256 + 40 + float(z64.max() - z64.min())) * 2.0**-24
+    assert float((got.double() - lp).abs().max()) <= err + 2.0**-23 * float(lp.abs().max())
+    bound = float(A.abs().max()) * 1.8
+    assert abs(float(loss.detach()) - float(term.sum() / counted.sum())) <= bound * (err + 2.0**-23)
+    ref = -probs * slope[:, None]
+    ref.scatter_add_(1, act[:, None], slope[:, None])
+    # as Case.check_gradient: errors of the slope and of the probabilities, then one rounding
+    far = (2 * err * slope.abs() + 2 * bound * err / float(counted.sum()))[:, None] \
+        + ref.abs() * (torch.finfo(dtype).eps / 2 * 1.01) + 1e-37
+    assert bool(((grad.double() - ref).abs() <= far).all())
+    assert not grad[::7].any()
+
+
+@pytest.mark.parametrize("pairs,rows", [(1, 9000), (2, 30001), (300, 4000), (5000, 20001)])
+def test_preference_of_many_rows(device, pairs, rows):
+    """Few long sequences (a workgroup for each pair) and many short ones (a wave for each)."""
+    vocab = 6
+    c = Case(rows, vocab, torch.float32, device, ignored=0.1)
+    rng = np.random.default_rng(pairs)
+    cuts = np.sort(rng.integers(0, rows + 1, 2 * pairs - 1))
+    offsets = np.concatenate(([0], cuts, [rows - 1]))
+    offsets = np.minimum(offsets, rows - 1)
+    z = c.logits.requires_grad_()
+    loss, h = cl.preference_loss(z, c.act_t, torch.as_tensor(offsets).to(device), c.ref_t, beta=0.05,
+                                 return_margins=True)
+    want, term, slope = P.preference_terms(c.lp, c.actions, offsets, c.ref, 0.05, 0.0)
+    seq = np.diff(offsets)
+    herr = 0.05 * (seq[:pairs] + seq[pairs:]) * c.err * 1.01
+    _near(_np(h), want, herr, c.wide)
+    _near(float(loss.detach()), term.mean(), herr.mean() + np.abs(term).mean() * 2.0**-23, c.wide)
+    serr = np.zeros(rows)
+    for i in range(pairs):
+        e = 0.05 * herr[i] / 4 + 0.1 * 2.0**-24
+        serr[offsets[i]:offsets[i + 1]] = e
+        serr[offsets[pairs + i]:offsets[pairs + i + 1]] = e
+    c.check_gradient(torch.autograd.grad(loss, z)[0], slope / pairs, serr / pairs)
 
 
 def test_rows_beyond_32_bits(device):
