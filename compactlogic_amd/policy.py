@@ -146,14 +146,18 @@ def _input_grad(ctx, grad):
     return grad_x
 
 
+def _args(logits):
+    """logits as the entry points take them (an expanded row has stride 0)."""
+    rows, cols = logits.shape
+    return _dl.storage_dtype_code(logits), logits.data_ptr(), logits.stride(0), rows, cols
+
+
 class _Shape:
     """One call's logits as the entry points take them, and the bytes of its buffers."""
 
     def __init__(self, logits):
-        self.code = code = _dl.storage_dtype_code(logits)
-        self.rows, self.cols = rows, cols = logits.shape
-        # (an expanded row has stride 0)
-        self.args = (code, logits.data_ptr(), logits.stride(0), rows, cols)
+        self.args = code, _, _, rows, cols = _args(logits)
+        self.code, self.rows, self.cols = code, rows, cols
         self.size = 8 if logits.dtype == torch.float64 else 4
         self.state_bytes = 4 * self.size * rows
         self.workspace_bytes = _workspace_bytes(code, rows, cols)
@@ -167,15 +171,21 @@ def _once():
 
 
 def _aux(logits, *sizes):
-    """One buffer for everything a call keeps to itself, and the addresses of its parts, 16 bytes
-    or a multiple apart: allocations cost a small call more than its kernels."""
+    """One buffer for everything a call keeps to itself, and where its parts start, a multiple of
+    32 bytes each: allocations cost a small call more than its kernels."""
     total, starts = 0, []
     for n in sizes:
         starts.append(total)
         total += (n + 31) & ~31
-    buf = torch.empty(max(total, 32), dtype=torch.uint8, device=logits.device)
-    base = buf.data_ptr()
-    return buf, [base + s for s in starts]
+    return torch.empty(max(total, 32), dtype=torch.uint8, device=logits.device), starts
+
+
+def _saved(ctx):
+    """The logits, actions and buffer that a forward saved, wherever they lie now (hooks on saved
+    tensors may have moved them), and the logits as the entry points take them."""
+    logits, actions, aux = ctx.saved_tensors
+    logits = _rows_of(logits)
+    return logits, actions, aux.data_ptr(), _args(logits), aux
 
 
 def _capture_id(t) -> int:
@@ -193,25 +203,25 @@ class SelectedLogProbsFunction(torch.autograd.Function):
     def forward(ctx, x, actions, ignore_index, group=None):
         logits = _logits_of(ctx, x, group)
         sh = _Shape(logits)
-        aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+        aux, (_, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+        at = aux.data_ptr()
         lp = torch.empty(sh.rows, dtype=_wide(logits), device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_selected_log_prob_forward", lambda: _capi.call(
                 "cl_selected_log_prob_forward", *sh.args, actions.data_ptr(), ignore_index,
-                lp.data_ptr(), state, ws, sh.workspace_bytes, _dl.stream_of(logits)))
-        ctx.save_for_backward(logits, actions, aux)
-        ctx.args, ctx.state = sh.args, state
+                lp.data_ptr(), at, at + ws, sh.workspace_bytes, _dl.stream_of(logits)))
+        ctx.save_for_backward(logits, actions, aux)   # (the rows' state comes first in aux)
         return lp
 
     @staticmethod
     def backward(ctx, grad_lp):
         _once()
-        logits, actions, aux = ctx.saved_tensors
+        logits, actions, at, args, _kept = _saved(ctx)
         grad_lp = grad_lp.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_selected_log_prob_backward", lambda: _capi.call(
-                "cl_selected_log_prob_backward", *ctx.args, actions.data_ptr(), ctx.state,
+                "cl_selected_log_prob_backward", *args, actions.data_ptr(), at,
                 grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits)))
         return _input_grad(ctx, grad), None, None, None
 
@@ -230,12 +240,14 @@ class PolicyLossFunction(torch.autograd.Function):
         lp = torch.empty(sh.rows, dtype=wide, device=logits.device)
         if reduction:
             loss = torch.empty((), dtype=wide, device=logits.device)
-            aux, (state, count, terms, ws) = _aux(logits, sh.state_bytes, sh.size,
+            aux, (_, ctx.count, terms, ws) = _aux(logits, sh.state_bytes, sh.size,
                                                   sh.rows * sh.size, sh.workspace_bytes)
-            loss_at = loss.data_ptr()
+            at = aux.data_ptr()
+            terms, loss_at, count = at + terms, loss.data_ptr(), at + ctx.count
         else:
             loss = torch.empty(sh.rows, dtype=wide, device=logits.device)
-            aux, (state, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+            aux, (_, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+            at = aux.data_ptr()
             terms, loss_at, count = loss.data_ptr(), None, None
         grad = None
         if reduction and ctx.needs_input_grad[0] and _prefills(sh.code, sh.rows, sh.cols):
@@ -245,11 +257,10 @@ class PolicyLossFunction(torch.autograd.Function):
             timing.timed("cl_policy_loss_forward", lambda: _capi.call(
                 "cl_policy_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
                 old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
-                reduction, lp.data_ptr(), state, terms, loss_at, count, _dl.ptr(grad), ws,
+                reduction, lp.data_ptr(), at, terms, loss_at, count, _dl.ptr(grad), at + ws,
                 sh.workspace_bytes, _dl.stream_of(logits)))
-        ctx.grad = grad
         ctx.save_for_backward(logits, actions, aux)
-        ctx.args, ctx.state, ctx.count, ctx.reduction = sh.args, state, count, reduction
+        ctx.grad, ctx.reduction = grad, reduction
         ctx.mark_non_differentiable(lp)
         ctx.set_materialize_grads(False)
         return loss, lp
@@ -259,7 +270,7 @@ class PolicyLossFunction(torch.autograd.Function):
         _once()
         if grad_loss is None:
             return (None,) * 11
-        logits, actions, aux = ctx.saved_tensors
+        logits, actions, at, args, _kept = _saved(ctx)
         grad_loss = grad_loss.contiguous()
         # the forward's gradient is handed out once, and only in the capture (or outside of any)
         # that it was written in: a replay of the backward alone would find it used
@@ -269,9 +280,9 @@ class PolicyLossFunction(torch.autograd.Function):
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_policy_loss_backward", lambda: _capi.call(
-                "cl_policy_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
-                ctx.reduction, grad_loss.data_ptr(), ctx.count, int(prefilled), grad.data_ptr(),
-                _dl.stream_of(logits)))
+                "cl_policy_loss_backward", *args, actions.data_ptr(), at, ctx.reduction,
+                grad_loss.data_ptr(), at + ctx.count if ctx.reduction else None, int(prefilled),
+                grad.data_ptr(), _dl.stream_of(logits)))
         return (_input_grad(ctx, grad),) + (None,) * 10
 
 
@@ -288,21 +299,20 @@ class PreferenceLossFunction(torch.autograd.Function):
         wide, pairs = _wide(logits), (offsets.numel() - 1) // 2
         margins = torch.empty(pairs, dtype=wide, device=logits.device)
         loss = torch.empty(() if reduction else (pairs,), dtype=wide, device=logits.device)
-        aux, (state, count, row_seq, seq_slope, gaps, lp, terms, ws) = _aux(
+        aux, (_, count, row_seq, seq_slope, gaps, lp, terms, ws) = _aux(
             logits, sh.state_bytes, sh.size, 4 * sh.rows, 2 * pairs * sh.size, 8 * sh.rows,
             sh.rows * sh.size, pairs * sh.size if reduction else 0, sh.workspace_bytes)
+        at = aux.data_ptr()
         loss_at = loss.data_ptr() if reduction else None
-        if not reduction:
-            terms = loss.data_ptr()
+        terms_at = at + terms if reduction else loss.data_ptr()
         with _dl.on_device_of(logits):
             timing.timed("cl_preference_loss_forward", lambda: _capi.call(
                 "cl_preference_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
-                _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction, lp, state,
-                gaps, row_seq, seq_slope, margins.data_ptr(), terms, loss_at, count, ws,
-                sh.workspace_bytes, _dl.stream_of(logits)))
+                _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction, at + lp, at,
+                at + gaps, at + row_seq, at + seq_slope, margins.data_ptr(), terms_at, loss_at,
+                at + count, at + ws, sh.workspace_bytes, _dl.stream_of(logits)))
         ctx.save_for_backward(logits, actions, aux)
-        ctx.args, ctx.reduction, ctx.pairs = sh.args, reduction, pairs
-        ctx.state, ctx.row_seq, ctx.seq_slope, ctx.count = state, row_seq, seq_slope, count
+        ctx.reduction, ctx.pairs, ctx.parts = reduction, pairs, (row_seq, seq_slope, count)
         ctx.mark_non_differentiable(margins)
         ctx.set_materialize_grads(False)
         return loss, margins
@@ -312,14 +322,15 @@ class PreferenceLossFunction(torch.autograd.Function):
         _once()
         if grad_loss is None:
             return (None,) * 9
-        logits, actions, aux = ctx.saved_tensors
+        logits, actions, at, args, _kept = _saved(ctx)
+        row_seq, seq_slope, count = ctx.parts
         grad_loss = grad_loss.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
             timing.timed("cl_preference_loss_backward", lambda: _capi.call(
-                "cl_preference_loss_backward", *ctx.args, actions.data_ptr(), ctx.state,
-                ctx.row_seq, ctx.seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(),
-                ctx.count, grad.data_ptr(), _dl.stream_of(logits)))
+                "cl_preference_loss_backward", *args, actions.data_ptr(), at, at + row_seq,
+                at + seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(), at + count,
+                grad.data_ptr(), _dl.stream_of(logits)))
         return (_input_grad(ctx, grad),) + (None,) * 8
 
 

@@ -641,6 +641,33 @@ def test_captured_losses(device, one_pass, dtype, vocab):
             assert torch.equal(loss.detach(), wl) and torch.equal(g, wg)
 
 
+def test_moved_saved_tensors(device, one_pass):
+    """Hooks that move what a forward saved (here to the host and back): the backward reads it where
+    it is then."""
+    off = torch.tensor([0, 5, 9, 16, 22], device=device)
+    for vocab in (10, 301, 9001):
+        c = Case(24, vocab, torch.bfloat16, device)
+        wide = torch.zeros((24, vocab + 5), dtype=torch.bfloat16, device=device)
+        wide[:, :vocab] = c.logits
+        z = wide[:, :vocab].requires_grad_()
+        for f in (lambda: cl.selected_log_probs(z, c.act_t).sum(),
+                  lambda: cl.policy_loss(z, c.act_t, c.old_t, c.adv_t) * 0.5,
+                  lambda: cl.preference_loss(z, c.act_t, off, c.ref_t)):
+            (want,) = torch.autograd.grad(f(), z)
+            with torch.autograd.graph.save_on_cpu():
+                loss = f()
+            junk = [torch.full((1 << 16,), 255, dtype=torch.uint8, device=device) for _ in range(8)]
+            (got,) = torch.autograd.grad(loss, z)
+            assert torch.equal(got, want)
+            del junk
+    x = torch.rand(40, 30, device=device, requires_grad=True)
+    rng = torch.tensor([3, 4], device=device)
+    (want,) = torch.autograd.grad(cl.dropout(x, 0.5, rng).sum(), x)
+    with torch.autograd.graph.save_on_cpu():
+        y = cl.dropout(x, 0.5, rng).sum()
+    assert torch.equal(torch.autograd.grad(y, x)[0], want)
+
+
 def test_streams(device):
     c = Case(64, 5001, torch.bfloat16, device)
     z = c.logits.requires_grad_()
