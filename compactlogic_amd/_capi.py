@@ -206,7 +206,7 @@ def load() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Invoke entry point `name`; translate a failure status into a Python exception."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != CL_OK:
         msg = lib.cl_last_error().decode(errors="replace")

@@ -244,7 +244,8 @@ extern "C" int cl_dropout(int dtype, const void* x, int64_t x_stride_row, int64_
         a.rows = rows;
         a.cols = cols;
         a.last = uint32_t((uint64_t(threshold) << 16) - 1);
-        a.scale = wide_t<T>(rescale && threshold < 65536 ? 65536.0 / double(65536 - threshold) : 1.0);
+        const double keep = double(65536 - threshold);
+        a.scale = wide_t<T>(rescale && keep > 0 ? 65536.0 / keep : 1.0);
         a.fill = wide_t<T>(T(wide_t<T>(fill)));
         a.seed = seed;
         a.offset = offset;

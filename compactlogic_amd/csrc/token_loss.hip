@@ -6,7 +6,7 @@
 //   lp = (x_a - m) - log s,   p_j = exp(x_j - m) / s,   d lp / d x_j = [j = a] - p_j.
 // Every loss is a function of the rows' lp, so its gradient is a number per row, the slope,
 // times [j = a] - p_j.  The forward leaves per row (m, 1 / s, 1 - p_a, slope) and the backward
-// forms the gradient from them (1 - p_a is -expm1(lp), rounded once).
+// forms the gradient from them (1 - p_a from the fp64 lp, rounded once).
 //
 // The row's scalars (lp and what the losses make of it) are taken in fp64: rows lie next to the
 // borders of the clipped range, and the preference loss subtracts sums over whole sequences.
@@ -155,7 +155,8 @@ __device__ __forceinline__ A base_of(A m) {
 }
 
 // Over the TPR lanes of a row (16: a DPP row, 64: the wave), the same bits in each of them: every
-// step exchanges with a mirror image, whose partial sum is the same two numbers the other way round.
+// step exchanges with a mirror image, whose partial sum is the same two numbers the other way
+// round.
 template <int TPR, typename A>
 __device__ __forceinline__ A lanes_max(A v) {
     v = max_of(v, dpp_move<0xB1>(v));   // quad_perm [1,0,3,2]
@@ -690,7 +691,8 @@ struct RowSums {
 
 template <typename A>
 __device__ __forceinline__ RowSums sum_rows(const A* terms, const int64_t* actions, int64_t from,
-                                            int64_t to, int64_t ignore, double (*red)[kSumThreads / 64]) {
+                                            int64_t to, int64_t ignore,
+                                            double (*red)[kSumThreads / 64]) {
     double t = 0;
     int c = 0;
 #pragma unroll 8

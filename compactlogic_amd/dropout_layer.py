@@ -16,21 +16,23 @@ from . import timing
 from .layers import PackBitsTensor
 
 
-def _apply(x, threshold, rescale, fill, seed, offset, rng):
+def _apply(x, code, threshold, rescale, fill, seed, offset, rng):
     """cl_dropout of a 2-D tensor, the result lying as the tensor does."""
     rows, cols = x.shape
-    if (x.stride(1) == 1 or cols == 1) and x.stride(0) >= 0:
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    elif (x.stride(0) == 1 or rows == 1) and x.stride(1) >= 0:
-        y = torch.empty((cols, rows), dtype=x.dtype, device=x.device).t()
-    else:
+    sr, sc = x.stride()
+    if not (sc == 1 or cols == 1 or sr == 1 or rows == 1):
         x = x.contiguous()
+        sr, sc = x.stride()
+    if sc == 1 or cols == 1:
         y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        yr, yc = cols, 1
+    else:
+        y = torch.empty_strided((rows, cols), (1, rows), dtype=x.dtype, device=x.device)
+        yr, yc = 1, rows
     with _dl.on_device_of(x):
-        timing.timed("cl_dropout", lambda: _capi.call(
-            "cl_dropout", _dl.storage_dtype_code(x), x.data_ptr(), x.stride(0), x.stride(1),
-            y.data_ptr(), y.stride(0), y.stride(1), rows, cols, threshold, int(rescale),
-            float(fill), seed, offset, _dl.ptr(rng), _dl.stream_of(x)))
+        timing.call("cl_dropout", code, x.data_ptr(), sr, sc, y.data_ptr(), yr, yc, rows, cols,
+                    threshold, rescale, fill, seed, offset,
+                    None if rng is None else rng.data_ptr(), _dl.stream_of(x))
     return y
 
 
@@ -40,20 +42,22 @@ class DropoutFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, threshold, fill, seed, offset, rng):
+        code = _dl.storage_dtype_code(x)
         ctx.save_for_backward(rng)
-        ctx.args = threshold, fill is None, seed, offset
-        return _apply(x, threshold, fill is None, 0.0 if fill is None else fill, seed, offset, rng)
+        ctx.args = code, threshold, int(fill is None), 0.0, seed, offset
+        return _apply(x, code, threshold, int(fill is None), 0.0 if fill is None else fill, seed,
+                      offset, rng)
 
     @staticmethod
     def backward(ctx, grad):
-        threshold, rescale, seed, offset = ctx.args
         (rng,) = ctx.saved_tensors
         if torch.is_grad_enabled():
+            _, threshold, rescale, _, seed, offset = ctx.args
             grad = DropoutFunction.apply(grad, threshold, None if rescale else 0.0, seed, offset,
                                          rng)
         else:
-            grad = _apply(grad, threshold, rescale, 0.0, seed, offset, rng)
-        return (grad,) + (None,) * 5
+            grad = _apply(grad, *ctx.args, rng)
+        return grad, None, None, None, None, None
 
 
 def _threshold(p) -> int:

@@ -122,9 +122,8 @@ def _logits_of(ctx, x, group):
     need = _centered_bytes(code, batch, feats, sb, k)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     with _dl.on_device_of(x):
-        timing.timed("cl_group_sum_centered_forward", lambda: _capi.call(
-            "cl_group_sum_centered_forward", code, x.data_ptr(), batch, feats, sb, sf, k, tau,
-            scores.data_ptr(), _dl.ptr(ws), need, _dl.stream_of(x)))
+        timing.call("cl_group_sum_centered_forward", code, x.data_ptr(), batch, feats, sb, sf, k,
+                    tau, scores.data_ptr(), _dl.ptr(ws), need, _dl.stream_of(x))
     ctx.group = k, tau, batch, feats, sb == 1 and sf != 1
     return scores
 
@@ -140,9 +139,8 @@ def _input_grad(ctx, grad):
         grad_x = torch.empty((batch, feats), dtype=grad.dtype, device=grad.device)
     sb, sf = grad_x.stride()
     with _dl.on_device_of(grad):
-        timing.timed("cl_group_sum_backward", lambda: _capi.call(
-            "cl_group_sum_backward", _dl.dtype_code(grad), grad.data_ptr(), batch, feats, k, tau,
-            grad_x.data_ptr(), sb, sf, _dl.stream_of(grad)))
+        timing.call("cl_group_sum_backward", _dl.dtype_code(grad), grad.data_ptr(), batch, feats,
+                    k, tau, grad_x.data_ptr(), sb, sf, _dl.stream_of(grad))
     return grad_x
 
 
@@ -207,9 +205,8 @@ class SelectedLogProbsFunction(torch.autograd.Function):
         at = aux.data_ptr()
         lp = torch.empty(sh.rows, dtype=_wide(logits), device=logits.device)
         with _dl.on_device_of(logits):
-            timing.timed("cl_selected_log_prob_forward", lambda: _capi.call(
-                "cl_selected_log_prob_forward", *sh.args, actions.data_ptr(), ignore_index,
-                lp.data_ptr(), at, at + ws, sh.workspace_bytes, _dl.stream_of(logits)))
+            timing.call("cl_selected_log_prob_forward", *sh.args, actions.data_ptr(), ignore_index,
+                        lp.data_ptr(), at, at + ws, sh.workspace_bytes, _dl.stream_of(logits))
         ctx.save_for_backward(logits, actions, aux)   # (the rows' state comes first in aux)
         return lp
 
@@ -220,9 +217,8 @@ class SelectedLogProbsFunction(torch.autograd.Function):
         grad_lp = grad_lp.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
-            timing.timed("cl_selected_log_prob_backward", lambda: _capi.call(
-                "cl_selected_log_prob_backward", *args, actions.data_ptr(), at,
-                grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits)))
+            timing.call("cl_selected_log_prob_backward", *args, actions.data_ptr(), at,
+                        grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits))
         return _input_grad(ctx, grad), None, None, None
 
 
@@ -254,11 +250,10 @@ class PolicyLossFunction(torch.autograd.Function):
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             ctx.capture = _capture_id(logits)
         with _dl.on_device_of(logits):
-            timing.timed("cl_policy_loss_forward", lambda: _capi.call(
-                "cl_policy_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
-                old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
-                reduction, lp.data_ptr(), at, terms, loss_at, count, _dl.ptr(grad), at + ws,
-                sh.workspace_bytes, _dl.stream_of(logits)))
+            timing.call("cl_policy_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
+                        old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
+                        reduction, lp.data_ptr(), at, terms, loss_at, count, _dl.ptr(grad), at + ws,
+                        sh.workspace_bytes, _dl.stream_of(logits))
         ctx.save_for_backward(logits, actions, aux)
         ctx.grad, ctx.reduction = grad, reduction
         ctx.mark_non_differentiable(lp)
@@ -279,10 +274,9 @@ class PolicyLossFunction(torch.autograd.Function):
         if not prefilled:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
-            timing.timed("cl_policy_loss_backward", lambda: _capi.call(
-                "cl_policy_loss_backward", *args, actions.data_ptr(), at, ctx.reduction,
-                grad_loss.data_ptr(), at + ctx.count if ctx.reduction else None, int(prefilled),
-                grad.data_ptr(), _dl.stream_of(logits)))
+            timing.call("cl_policy_loss_backward", *args, actions.data_ptr(), at, ctx.reduction,
+                        grad_loss.data_ptr(), at + ctx.count if ctx.reduction else None,
+                        int(prefilled), grad.data_ptr(), _dl.stream_of(logits))
         return (_input_grad(ctx, grad),) + (None,) * 10
 
 
@@ -306,11 +300,11 @@ class PreferenceLossFunction(torch.autograd.Function):
         loss_at = loss.data_ptr() if reduction else None
         terms_at = at + terms if reduction else loss.data_ptr()
         with _dl.on_device_of(logits):
-            timing.timed("cl_preference_loss_forward", lambda: _capi.call(
-                "cl_preference_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
-                _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction, at + lp, at,
-                at + gaps, at + row_seq, at + seq_slope, margins.data_ptr(), terms_at, loss_at,
-                at + count, at + ws, sh.workspace_bytes, _dl.stream_of(logits)))
+            timing.call("cl_preference_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
+                        _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction,
+                        at + lp, at, at + gaps, at + row_seq, at + seq_slope, margins.data_ptr(),
+                        terms_at, loss_at, at + count, at + ws, sh.workspace_bytes,
+                        _dl.stream_of(logits))
         ctx.save_for_backward(logits, actions, aux)
         ctx.reduction, ctx.pairs, ctx.parts = reduction, pairs, (row_seq, seq_slope, count)
         ctx.mark_non_differentiable(margins)
@@ -327,10 +321,9 @@ class PreferenceLossFunction(torch.autograd.Function):
         grad_loss = grad_loss.contiguous()
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         with _dl.on_device_of(logits):
-            timing.timed("cl_preference_loss_backward", lambda: _capi.call(
-                "cl_preference_loss_backward", *args, actions.data_ptr(), at, at + row_seq,
-                at + seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(), at + count,
-                grad.data_ptr(), _dl.stream_of(logits)))
+            timing.call("cl_preference_loss_backward", *args, actions.data_ptr(), at, at + row_seq,
+                        at + seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(), at + count,
+                        grad.data_ptr(), _dl.stream_of(logits))
         return (_input_grad(ctx, grad),) + (None,) * 8
 
 

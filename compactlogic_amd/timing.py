@@ -20,6 +20,8 @@ from collections import defaultdict
 
 import torch
 
+from . import _capi
+
 _active = None
 
 # Spin of the settle kernel in microseconds (converted to clock cycles on first use).
@@ -71,6 +73,15 @@ def record(settle: bool = True, repeat: dict | None = None):
         yield _active
     finally:
         _active = prev
+
+
+def call(name: str, *args) -> None:
+    """_capi.call(name, *args), bracketed when a recorder is active: `timed` for the calls whose
+    kernels are shorter than a closure and its frame."""
+    if _active is None:
+        _capi.call(name, *args)
+    else:
+        timed(name, lambda: _capi.call(name, *args))
 
 
 def timed(name: str, fn, stream=None):

@@ -114,9 +114,9 @@ def test_policy_loss(device, one_pass, dtype, kl, reduction):
     for rows, vocab in SIZES:
         c = Case(rows, vocab, dtype, device)
         z = c.logits.requires_grad_()
-        loss, lp = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, ref_log_probs=c.ref_t if kl else None,
-                                  clip=(0.2, 0.28), kl_coef=kl, reduction=reduction,
-                                  return_log_probs=True)
+        loss, lp = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t,
+                                  ref_log_probs=c.ref_t if kl else None, clip=(0.2, 0.28),
+                                  kl_coef=kl, reduction=reduction, return_log_probs=True)
         term, slope = P.policy_terms(c.lp, c.actions, c.old, c.adv, c.ref, 0.2, 0.28, kl)
         counted = c.actions != IGNORE
         n = counted.sum()
@@ -179,7 +179,8 @@ def test_preference_loss(device, dtype, with_ref, reduction):
             for i in range(pairs):
                 row_up[offsets[i]:offsets[i + 1]] = _np(ut)[i]
                 row_up[offsets[pairs + i]:offsets[pairs + i + 1]] = _np(ut)[i]
-            c.check_gradient(g, slope * row_up, serr * np.abs(row_up) + np.abs(slope * row_up) * 2 * _unit(dtype))
+            c.check_gradient(g, slope * row_up, serr * np.abs(row_up)
+                             + np.abs(slope * row_up) * 2 * _unit(dtype))
         else:
             div = pairs if reduction == "mean" else 1
             _near(_np(loss), term.sum() / div, terr.sum() / div, c.wide)
@@ -479,7 +480,9 @@ def test_group_sum_methods(device, batch, feats, k, layout, dtype):
     adv = torch.as_tensor(rng.standard_normal(batch)).to(wide).to(device)
     spread = z.max() - z.min()
     unit = _unit(wide)
-    score_err = (gsz + 8) * gsz * unit / tau + spread * unit + (np.abs(z).max() * unit if k > 512 else 0)
+    score_err = (gsz + 8) * gsz * unit / tau + spread * unit
+    if k > 512:
+        score_err += np.abs(z).max() * unit
     err = 2 * score_err + _sum_error(z - z.max(1, keepdims=True), wide)
     gs = cl.GroupSum(k, tau)
     scale = np.repeat(np.eye(k), gsz, axis=1)[:, :feats] / tau      # d score / d x
@@ -700,7 +703,8 @@ def test_many_rows(device, rows, vocab, dtype):
     probs = torch.softmax(z64, 1)
     lp = torch.log_softmax(z64, 1).gather(1, act[:, None])[:, 0] * counted
     pick = torch.randint(0, 5, (rows,), generator=g, device=device)
-    old = (lp - torch.tensor([0.4, 0.9, 1.0, 1.15, 1.7], device=device).double().log()[pick]).float()
+    ratio = torch.tensor([0.4, 0.9, 1.0, 1.15, 1.7], dtype=torch.float64, device=device)
+    old = (lp - ratio.log()[pick]).float()
     adv = torch.randn(rows, generator=g, device=device)
     loss, got = cl.policy_loss(z, a, old, adv, return_log_probs=True)
     (grad,) = torch.autograd.grad(loss, z)
@@ -731,8 +735,8 @@ def test_preference_of_many_rows(device, pairs, rows):
     offsets = np.concatenate(([0], cuts, [rows - 1]))
     offsets = np.minimum(offsets, rows - 1)
     z = c.logits.requires_grad_()
-    loss, h = cl.preference_loss(z, c.act_t, torch.as_tensor(offsets).to(device), c.ref_t, beta=0.05,
-                                 return_margins=True)
+    loss, h = cl.preference_loss(z, c.act_t, torch.as_tensor(offsets).to(device), c.ref_t,
+                                 beta=0.05, return_margins=True)
     want, term, slope = P.preference_terms(c.lp, c.actions, offsets, c.ref, 0.05, 0.0)
     seq = np.diff(offsets)
     herr = 0.05 * (seq[:pairs] + seq[pairs:]) * c.err * 1.01
