@@ -228,52 +228,57 @@ struct CrossEntropyGrad {
 // by the loads of the slices, as the finish (1024 samples, 26 slices of 10 classes: 1.1 MB).
 constexpr int kCenterSamples = 16;
 
+// One sample by the 16 lanes of a DPP row.
 template <typename T>
-__device__ __forceinline__ void center_row(const double* z, int64_t k, T* __restrict__ out) {
+__device__ __forceinline__ void center_row(const double* z, int k, T* __restrict__ out) {
+    const int l = lane_id() & 15;
     double mx = -__builtin_inf();
-    bool nan = false;
-    for (int64_t c = lane_id(); c < k; c += kWave) {
+    int nan = 0;
+    for (int c = l; c < k; c += 16) {
         mx = fmax(mx, z[c]);
         nan |= z[c] != z[c];
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) mx = fmax(mx, __shfl_xor(mx, off, kWave));
-    // all of a row's differences are NaN where a score is, as its softmax would be
-    if (__any(nan)) mx = __builtin_nan("");
-    for (int64_t c = lane_id(); c < k; c += kWave) out[c] = T(z[c] - mx);
+    mx = fmax(mx, dpp_move<0xB1>(mx));   // quad_perm [1,0,3,2]
+    mx = fmax(mx, dpp_move<0x4E>(mx));   // quad_perm [2,3,0,1]
+    mx = fmax(mx, dpp_move<0x141>(mx));  // row_half_mirror
+    mx = fmax(mx, dpp_move<0x140>(mx));  // row_mirror
+    nan |= dpp_move<0xB1>(nan);
+    nan |= dpp_move<0x4E>(nan);
+    nan |= dpp_move<0x141>(nan);
+    nan |= dpp_move<0x140>(nan);
+    // all of a sample's differences are NaN where a score is, as its softmax would be
+    if (nan) mx = __builtin_nan("");
+    for (int c = l; c < k; c += 16) out[c] = T(z[c] - mx);
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_gsum_center(const T* __restrict__ part, int64_t B,
-                                                     int64_t k, int64_t nslices, double tau,
+__global__ __launch_bounds__(256) void k_gsum_center(const T* __restrict__ part, int64_t B, int k,
+                                                     int64_t nslices, double tau,
                                                      T* __restrict__ out) {
     extern __shared__ __align__(16) unsigned char center_lds[];
     double* z = reinterpret_cast<double*>(center_lds);  // [kCenterSamples][k]
     const int64_t n0 = int64_t(blockIdx.x) * kCenterSamples;
-    const int64_t ns = std::min<int64_t>(kCenterSamples, B - n0);
+    const int ns = int(std::min<int64_t>(kCenterSamples, B - n0));
     const int64_t step = k * B;
-    for (int64_t e = threadIdx.x; e < ns * k; e += 256) {
-        // samples side by side: a slice's elements of one class are contiguous over the batch
-        const int64_t c = e / ns, i = e - c * ns;
+    // samples side by side: a slice's elements of one class are contiguous over the batch
+    for (int e = threadIdx.x; e < kCenterSamples * k; e += 256) {
+        const int c = e / kCenterSamples, i = e % kCenterSamples;
+        if (i >= ns) continue;
         const T* src = part + c * B + n0 + i;
         double t = 0;
-        int64_t sl = 0;
-        for (; sl + 16 <= nslices; sl += 16) {
+        // sixteen loads at a time, past the end the last slice again (no branch between loads)
+        for (int64_t sl = 0; sl < nslices; sl += 16) {
             T v[16];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) v[u] = src[(sl + u) * step];
+            for (int u = 0; u < 16; ++u) v[u] = src[std::min(sl + u, nslices - 1) * step];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) t += double(v[u]);
+            for (int u = 0; u < 16; ++u) t += sl + u < nslices ? double(v[u]) : 0.0;
         }
-        T v[16];
-#pragma unroll
-        for (int u = 0; u < 16; ++u) v[u] = sl + u < nslices ? src[(sl + u) * step] : T(0);
-#pragma unroll
-        for (int u = 0; u < 16; ++u) t += sl + u < nslices ? double(v[u]) : 0.0;
         z[i * k + c] = t / tau;
     }
     __syncthreads();
-    for (int64_t i = wave_id(); i < ns; i += 4) center_row(z + i * k, k, out + (n0 + i) * k);
+    const int i = threadIdx.x / 16;
+    if (i < ns) center_row(z + i * k, k, out + (n0 + i) * k);
 }
 
 // Any layout: a workgroup per sample, its waves taking the classes in turn.
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(256) void k_gsum_center_any(const T* __restrict__ x
         if (lane_id() == 0) z[c] = t / tau;
     }
     __syncthreads();
-    if (wave_id() == 0) center_row(z, k, out + n * k);
+    if (threadIdx.x < 16) center_row(z, int(k), out + n * k);
 }
 
 // ---- backward: grad_x[n, j] = src(n, j / gsz).  Elements are visited in memory order
@@ -649,7 +654,8 @@ extern "C" int cl_group_sum_centered_forward(int dtype, const void* x, int64_t b
                     xs, batch, features, stride_feature, gsz, k, slice, part);
             if (int rc = check_launch("cl_group_sum_centered_forward(partial)")) return rc;
             k_gsum_center<T><<<unsigned(ceil_div(batch, kCenterSamples)), 256,
-                               size_t(kCenterSamples * k * 8), s>>>(part, batch, k, slices, tau, os);
+                               size_t(kCenterSamples * k * 8), s>>>(part, batch, int(k), slices, tau,
+                                                                  os);
         } else {
             k_gsum_center_any<T><<<unsigned(batch), 256, size_t(k * 8), s>>>(
                 xs, features, stride_batch, stride_feature, gsz, k, tau, os);

@@ -758,14 +758,13 @@ struct PairArgs {
     A* terms;
 };
 
-// Pair i by one wave, or by a workgroup of WAVES (then all of its threads come here): the sums
-// over both sequences, the margin h, the loss term
+// Pair i by LANES threads: a DPP row (16), a wave (64) or a workgroup (then all of its threads come
+// here): the sums over both sequences, the margin h, the loss term
 //   -(1 - e) log sigma(h) - e log sigma(-h)
 // and its slope by the chosen sequence's sum; the rejected one's is the negative.
-template <int WAVES, typename A>
+template <int LANES, typename A>
 __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i, double* red) {
-    constexpr int STEP = WAVES * 64;
-    const int t0 = WAVES > 1 ? int(threadIdx.x) : lane_id();
+    const int t0 = int(threadIdx.x) % LANES;
     double d[2];
     bool bad = false;
 #pragma unroll
@@ -777,20 +776,20 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i, dou
         e = std::min(std::max(e, b), a.rows);
         double t = 0;
         // eight loads at a time, in row order
-        for (int64_t n = b + t0; n < e; n += 8 * STEP) {
+        for (int64_t n = b + t0; n < e; n += 8 * LANES) {
             double v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = n + u * STEP < e ? a.gaps[n + u * STEP] : 0.0;
+            for (int u = 0; u < 8; ++u) v[u] = n + u * LANES < e ? a.gaps[n + u * LANES] : 0.0;
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 t += v[u];
-                if (n + u * STEP < e) a.row_seq[n + u * STEP] = int32_t(q);
+                if (n + u * LANES < e) a.row_seq[n + u * LANES] = int32_t(q);
             }
         }
-        if constexpr (WAVES > 1)
-            d[side] = group_sum(t, red + side * WAVES);
+        if constexpr (LANES > 64)
+            d[side] = group_sum(t, red + side * (LANES / 64));
         else
-            d[side] = wave_total(t);
+            d[side] = lanes_sum<LANES>(t);
     }
     double h = a.beta * (d[0] - d[1]);
     if (bad) h = nan_value<double>();
@@ -813,13 +812,13 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i, dou
 template <typename A>
 __global__ __launch_bounds__(kRowBlock) void k_pref_pairs(PairArgs<A> a) {
     const int64_t i = int64_t(blockIdx.x) * (kRowBlock / 64) + wave_id();
-    if (i < a.pairs) pair_term<1>(a, i, nullptr);
+    if (i < a.pairs) pair_term<64>(a, i, nullptr);
 }
 
 template <typename A>
 __global__ __launch_bounds__(kSumThreads) void k_pref_long(PairArgs<A> a) {
     __shared__ double red[2 * kSumThreads / 64];
-    pair_term<kSumThreads / 64>(a, blockIdx.x, red);
+    pair_term<kSumThreads>(a, blockIdx.x, red);
 }
 
 template <typename A>
@@ -837,16 +836,17 @@ __global__ __launch_bounds__(kSumThreads) void k_pref_sum(const A* __restrict__ 
     }
 }
 
-// Both in one launch, for batches of few rows: 16 waves take the pairs in turn.
-template <typename A>
+// Both in one launch, for batches of few rows: 64 rows of lanes, or 16 waves, take the pairs in
+// turn.
+template <int LANES, typename A>
 __global__ __launch_bounds__(kSumThreads) void k_pref_small(PairArgs<A> a, int mean,
                                                             A* __restrict__ loss,
                                                             A* __restrict__ count) {
     __shared__ double red[kSumThreads / 64];
     double t = 0;
-    for (int64_t i = wave_id(); i < a.pairs; i += kSumThreads / 64) {
-        const double term = pair_term<1>(a, i, nullptr);
-        t += lane_id() == 0 ? term : 0.0;
+    for (int64_t i = threadIdx.x / LANES; i < a.pairs; i += kSumThreads / LANES) {
+        const double term = pair_term<LANES>(a, i, nullptr);
+        t += threadIdx.x % LANES == 0 ? term : 0.0;
     }
     if (!loss) return;
     t = group_sum(t, red);
@@ -1206,8 +1206,13 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
         // rows each of 64 classes 43 us instead of 86
         const bool longs = pairs > 0 && rows / pairs > kPrefLongRows;
         if (!longs && rows <= kPrefSmallRows && pairs <= kPrefSmallPairs) {
-            if (pairs > 0 || out)
-                k_pref_small<A><<<1, kSumThreads, 0, s>>>(pa, mean, out, static_cast<A*>(count));
+            // up to 16 loads of a row of lanes per pair, else a wave's
+            if (pairs > 0 && rows / pairs <= 256)
+                k_pref_small<16, A><<<1, kSumThreads, 0, s>>>(pa, mean, out,
+                                                             static_cast<A*>(count));
+            else if (pairs > 0 || out)
+                k_pref_small<64, A><<<1, kSumThreads, 0, s>>>(pa, mean, out,
+                                                             static_cast<A*>(count));
             return check_launch("cl_preference_loss_forward(pairs)");
         }
         if (longs)
