@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import torch
 
-from . import _capi
 from . import difflogic_hip as _dl
 from . import timing
 from .layers import PackBitsTensor
@@ -29,10 +28,8 @@ def _apply(x, code, threshold, rescale, fill, seed, offset, rng):
     else:
         y = torch.empty_strided((rows, cols), (1, rows), dtype=x.dtype, device=x.device)
         yr, yc = 1, rows
-    with _dl.on_device_of(x):
-        timing.call("cl_dropout", code, x.data_ptr(), sr, sc, y.data_ptr(), yr, yc, rows, cols,
-                    threshold, rescale, fill, seed, offset,
-                    None if rng is None else rng.data_ptr(), _dl.stream_of(x))
+    timing.launch(x, "cl_dropout", code, x.data_ptr(), sr, sc, y.data_ptr(), yr, yc, rows, cols,
+                  threshold, rescale, fill, seed, offset, None if rng is None else rng.data_ptr())
     return y
 
 
@@ -122,9 +119,7 @@ class Dropout(torch.nn.Module):
         """The (seed, offset) of the next mask, as `dropout` takes it; advances the module."""
         _dl._check(self.rng, "rng")
         used = torch.empty_like(self.rng)
-        with _dl.on_device_of(used):
-            _capi.call("cl_dropout_next", self.rng.data_ptr(), used.data_ptr(),
-                       _dl.stream_of(used))
+        timing.launch(used, "cl_dropout_next", self.rng.data_ptr(), used.data_ptr())
         return used
 
     def forward(self, x):

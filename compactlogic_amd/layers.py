@@ -1434,7 +1434,7 @@ class GroupSum(torch.nn.Module):
         """policy.selected_log_probs(self(x), actions) in one op: the log-probability of the chosen
         class of every sample, differentiable by x."""
         x, group = self._head(x)
-        return _policy._selected_log_probs(x, actions, ignore_index, group)
+        return _policy.selected_log_probs(x, actions, ignore_index, _group=group)
 
     def policy_loss(self, x, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
                     kl_coef: float = 0.0, ignore_index: int = -100, reduction: str = "mean",
@@ -1442,8 +1442,9 @@ class GroupSum(torch.nn.Module):
         """policy.policy_loss(self(x), actions, ...) in one op: the clipped policy loss with a KL
         term of a network that chooses one of k classes, differentiable by x."""
         x, group = self._head(x)
-        return _policy._policy_loss(x, actions, old_log_probs, advantages, ref_log_probs, clip,
-                                    kl_coef, ignore_index, reduction, return_log_probs, group)
+        return _policy.policy_loss(x, actions, old_log_probs, advantages, ref_log_probs, clip,
+                                   kl_coef, ignore_index, reduction, return_log_probs,
+                                   _group=group)
 
     def preference_loss(self, x, actions, offsets, ref_log_probs=None, beta: float = 0.1,
                         label_smoothing: float = 0.0, ignore_index: int = -100,
@@ -1451,8 +1452,8 @@ class GroupSum(torch.nn.Module):
         """policy.preference_loss(self(x), actions, offsets, ...) in one op: the preference loss of
         paired sequences of samples, differentiable by x."""
         x, group = self._head(x)
-        return _policy._preference_loss(x, actions, offsets, ref_log_probs, beta, label_smoothing,
-                                        ignore_index, reduction, return_margins, group)
+        return _policy.preference_loss(x, actions, offsets, ref_log_probs, beta, label_smoothing,
+                                       ignore_index, reduction, return_margins, _group=group)
 
     def extra_repr(self):
         return 'k={}, tau={}'.format(self.k, self.tau)

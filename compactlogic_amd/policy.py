@@ -11,6 +11,9 @@ computed from are float32 (float64 for float64 logits).
 A row whose action is ``ignore_index`` (a prompt or padding) does not count: its log-probability
 and its gradient are 0 whatever its other inputs hold, NaN included.  Another action outside the
 logits' range gives NaN, as a label does in GroupSum.cross_entropy.
+
+A small call spends most of its time in Python, on both sides of autograd: sizes are looked up
+once per shape, what a call keeps to itself is one allocation, and there are few frames.
 """
 from __future__ import annotations
 
@@ -23,9 +26,8 @@ from . import _capi
 from . import difflogic_hip as _dl
 from . import timing
 
-
-def _wide(logits: torch.Tensor) -> torch.dtype:
-    return torch.float64 if logits.dtype == torch.float64 else torch.float32
+_CODES = _dl._STORAGE_DTYPES
+_F32, _F64 = torch.float32, torch.float64
 
 
 def _flat(logits, actions):
@@ -33,30 +35,32 @@ def _flat(logits, actions):
     [rows], checked."""
     if not isinstance(logits, torch.Tensor) or not isinstance(actions, torch.Tensor):
         raise TypeError("logits and actions must be tensors")
-    if logits.device.type != "cuda" or actions.device != logits.device:
+    if not logits.is_cuda or actions.device != logits.device:
         raise RuntimeError("logits and actions must be on the same HIP device")
-    _dl.storage_dtype_code(logits)
-    if logits.dim() < 1 or logits.shape[-1] < 1:
+    if logits.dtype not in _CODES:
+        _dl.storage_dtype_code(logits)
+    shape = logits.shape
+    if not shape or shape[-1] < 1:
         raise RuntimeError(f"logits must have a last dimension of at least one class, got shape "
-                           f"{tuple(logits.shape)}")
-    if actions.dtype != torch.int64 or actions.shape != logits.shape[:-1]:
-        raise RuntimeError(f"actions must be int64 of shape {tuple(logits.shape[:-1])}")
-    if logits.dim() != 2:
-        logits = logits.reshape(-1, logits.shape[-1])
+                           f"{tuple(shape)}")
+    if actions.dtype != torch.int64 or actions.shape != shape[:-1]:
+        raise RuntimeError(f"actions must be int64 of shape {tuple(shape[:-1])}")
+    if len(shape) != 2:
+        logits = logits.reshape(-1, shape[-1])
         actions = actions.reshape(-1)
-    return logits, actions.contiguous()
+    return logits, actions if actions.is_contiguous() else actions.contiguous()
 
 
-def _per_row(t, name, logits, actions):
-    """A constant per row as a contiguous [rows] tensor of the logits' wide type."""
+def _per_row(t, name, like, actions):
+    """A constant per row as a contiguous [rows] tensor of the type that goes with `like`."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.device != logits.device or t.shape != actions.shape or not t.is_floating_point():
+    if t.device != like.device or t.shape != actions.shape or not t.is_floating_point():
         raise RuntimeError(f"{name} must be a floating-point tensor of shape "
-                           f"{tuple(actions.shape)} on {logits.device}")
+                           f"{tuple(actions.shape)} on {like.device}")
     if t.requires_grad:
         raise RuntimeError(f"{name} is a constant of the loss: detach it")
-    wide = _wide(logits)
+    wide = _F64 if like.dtype == _F64 else _F32
     if t.dim() != 1:
         t = t.reshape(-1)
     if t.dtype != wide:
@@ -65,9 +69,10 @@ def _per_row(t, name, logits, actions):
 
 
 def _reduction(name):
-    if name not in _capi.CL_REDUCE:
+    code = _capi.CL_REDUCE.get(name)
+    if code is None:
         raise ValueError(f"reduction must be one of {sorted(_capi.CL_REDUCE)}, got {name!r}")
-    return _capi.CL_REDUCE[name]
+    return code
 
 
 def _rows_of(logits):
@@ -77,21 +82,16 @@ def _rows_of(logits):
     return logits
 
 
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(code, rows, cols) -> int:
-    need = ctypes.c_int64()
-    _capi.call("cl_token_loss_workspace", code, rows, cols, ctypes.byref(need))
-    return need.value
+# ---- sizes, once per shape
 
-
-@functools.lru_cache(maxsize=1024)
+@functools.lru_cache(maxsize=4096)
 def _prefills(code, rows, cols) -> bool:
     yes = ctypes.c_int()
     _capi.call("cl_policy_loss_prefills", code, rows, cols, ctypes.byref(yes))
     return bool(yes.value)
 
 
-@functools.lru_cache(maxsize=1024)
+@functools.lru_cache(maxsize=4096)
 def _centered_bytes(code, batch, feats, stride_batch, k) -> int:
     need = ctypes.c_int64()
     _capi.call("cl_group_sum_centered_workspace_size", code, batch, feats, stride_batch, k,
@@ -103,6 +103,21 @@ def takes_group(k: int) -> bool:
     """Whether the losses take GroupSum's scores of k classes from its input."""
     return _centered_bytes(_capi.CL_DTYPE_F32, 1, 1, 1, int(k)) >= 0
 
+
+@functools.lru_cache(maxsize=4096)
+def _buffer(code, rows, cols, *sizes):
+    """The one buffer of a call: its bytes, the workspace's, and where the parts behind the rows'
+    state start: those of `sizes` bytes, then the workspace; a multiple of 32 bytes each."""
+    need = ctypes.c_int64()
+    _capi.call("cl_token_loss_workspace", code, rows, cols, ctypes.byref(need))
+    total, starts = 0, []
+    for n in (4 * (8 if code == _capi.CL_DTYPE_F64 else 4) * rows, *sizes, need.value):
+        starts.append(total)
+        total += (n + 31) & ~31
+    return max(total, 32), need.value, *starts[1:]
+
+
+# ---- GroupSum's scores
 
 def _logits_of(ctx, x, group):
     """The rows of logits to work on: x itself, or, with group (k, tau), GroupSum's scores of the
@@ -121,9 +136,8 @@ def _logits_of(ctx, x, group):
     scores = torch.empty((batch, k), dtype=x.dtype, device=x.device)
     need = _centered_bytes(code, batch, feats, sb, k)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    with _dl.on_device_of(x):
-        timing.call("cl_group_sum_centered_forward", code, x.data_ptr(), batch, feats, sb, sf, k,
-                    tau, scores.data_ptr(), _dl.ptr(ws), need, _dl.stream_of(x))
+    timing.launch(x, "cl_group_sum_centered_forward", code, x.data_ptr(), batch, feats, sb, sf, k,
+                  tau, scores.data_ptr(), _dl.ptr(ws), need)
     ctx.group = k, tau, batch, feats, sb == 1 and sf != 1
     return scores
 
@@ -134,56 +148,27 @@ def _input_grad(ctx, grad):
         return grad
     k, tau, batch, feats, batch_major = ctx.group
     if batch_major:
-        grad_x = torch.empty((feats, batch), dtype=grad.dtype, device=grad.device).t()
+        sb, sf = 1, batch
+        grad_x = torch.empty_strided((batch, feats), (1, batch), dtype=grad.dtype,
+                                     device=grad.device)
     else:
+        sb, sf = feats, 1
         grad_x = torch.empty((batch, feats), dtype=grad.dtype, device=grad.device)
-    sb, sf = grad_x.stride()
-    with _dl.on_device_of(grad):
-        timing.call("cl_group_sum_backward", _dl.dtype_code(grad), grad.data_ptr(), batch, feats,
-                    k, tau, grad_x.data_ptr(), sb, sf, _dl.stream_of(grad))
+    timing.launch(grad, "cl_group_sum_backward", _CODES[grad.dtype], grad.data_ptr(), batch, feats,
+                  k, tau, grad_x.data_ptr(), sb, sf)
     return grad_x
 
 
-def _args(logits):
-    """logits as the entry points take them (an expanded row has stride 0)."""
-    rows, cols = logits.shape
-    return _dl.storage_dtype_code(logits), logits.data_ptr(), logits.stride(0), rows, cols
-
-
-class _Shape:
-    """One call's logits as the entry points take them, and the bytes of its buffers."""
-
-    def __init__(self, logits):
-        self.args = code, _, _, rows, cols = _args(logits)
-        self.code, self.rows, self.cols = code, rows, cols
-        self.size = 8 if logits.dtype == torch.float64 else 4
-        self.state_bytes = 4 * self.size * rows
-        self.workspace_bytes = _workspace_bytes(code, rows, cols)
-
-
-def _once():
-    """The backwards are kernels without a derivative of their own: under create_graph a second
-    derivative would silently lack its part."""
-    if torch.is_grad_enabled():
-        raise RuntimeError("the losses on chosen log-probabilities cannot be differentiated twice")
-
-
-def _aux(logits, *sizes):
-    """One buffer for everything a call keeps to itself, and where its parts start, a multiple of
-    32 bytes each: allocations cost a small call more than its kernels."""
-    total, starts = 0, []
-    for n in sizes:
-        starts.append(total)
-        total += (n + 31) & ~31
-    return torch.empty(max(total, 32), dtype=torch.uint8, device=logits.device), starts
-
+# ---- autograd
 
 def _saved(ctx):
     """The logits, actions and buffer that a forward saved, wherever they lie now (hooks on saved
-    tensors may have moved them), and the logits as the entry points take them."""
+    tensors may have moved them).  The backwards are kernels without a derivative of their own:
+    under create_graph a second derivative would silently lack its part."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the losses on chosen log-probabilities cannot be differentiated twice")
     logits, actions, aux = ctx.saved_tensors
-    logits = _rows_of(logits)
-    return logits, actions, aux.data_ptr(), _args(logits), aux
+    return _rows_of(logits), actions, aux
 
 
 def _capture_id(t) -> int:
@@ -200,25 +185,29 @@ class SelectedLogProbsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, actions, ignore_index, group=None):
         logits = _logits_of(ctx, x, group)
-        sh = _Shape(logits)
-        aux, (_, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
+        dtype, dev = logits.dtype, logits.device
+        code = _CODES[dtype]
+        rows, cols = logits.shape
+        total, ws_bytes, ws = _buffer(code, rows, cols)
+        aux = torch.empty(total, dtype=torch.uint8, device=dev)
+        lp = torch.empty(rows, dtype=_F64 if dtype == _F64 else _F32, device=dev)
         at = aux.data_ptr()
-        lp = torch.empty(sh.rows, dtype=_wide(logits), device=logits.device)
-        with _dl.on_device_of(logits):
-            timing.call("cl_selected_log_prob_forward", *sh.args, actions.data_ptr(), ignore_index,
-                        lp.data_ptr(), at, at + ws, sh.workspace_bytes, _dl.stream_of(logits))
+        timing.launch(logits, "cl_selected_log_prob_forward", code, logits.data_ptr(),
+                      logits.stride(0), rows, cols, actions.data_ptr(), ignore_index,
+                      lp.data_ptr(), at, at + ws, ws_bytes)
         ctx.save_for_backward(logits, actions, aux)   # (the rows' state comes first in aux)
         return lp
 
     @staticmethod
     def backward(ctx, grad_lp):
-        _once()
-        logits, actions, at, args, _kept = _saved(ctx)
-        grad_lp = grad_lp.contiguous()
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        with _dl.on_device_of(logits):
-            timing.call("cl_selected_log_prob_backward", *args, actions.data_ptr(), at,
-                        grad_lp.data_ptr(), grad.data_ptr(), _dl.stream_of(logits))
+        logits, actions, aux = _saved(ctx)
+        if not grad_lp.is_contiguous():
+            grad_lp = grad_lp.contiguous()
+        rows, cols = logits.shape
+        grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
+        timing.launch(logits, "cl_selected_log_prob_backward", _CODES[logits.dtype],
+                      logits.data_ptr(), logits.stride(0), rows, cols, actions.data_ptr(),
+                      aux.data_ptr(), grad_lp.data_ptr(), grad.data_ptr())
         return _input_grad(ctx, grad), None, None, None
 
 
@@ -231,53 +220,53 @@ class PolicyLossFunction(torch.autograd.Function):
     def forward(ctx, x, actions, old, adv, ref, clip_low, clip_high, kl_coef, ignore_index,
                 reduction, group=None):
         logits = _logits_of(ctx, x, group)
-        sh = _Shape(logits)
-        wide = old.dtype
-        lp = torch.empty(sh.rows, dtype=wide, device=logits.device)
-        if reduction:
-            loss = torch.empty((), dtype=wide, device=logits.device)
-            aux, (_, ctx.count, terms, ws) = _aux(logits, sh.state_bytes, sh.size,
-                                                  sh.rows * sh.size, sh.workspace_bytes)
-            at = aux.data_ptr()
-            terms, loss_at, count = at + terms, loss.data_ptr(), at + ctx.count
-        else:
-            loss = torch.empty(sh.rows, dtype=wide, device=logits.device)
-            aux, (_, ws) = _aux(logits, sh.state_bytes, sh.workspace_bytes)
-            at = aux.data_ptr()
-            terms, loss_at, count = loss.data_ptr(), None, None
+        dtype, dev, wide = logits.dtype, logits.device, old.dtype
+        code = _CODES[dtype]
+        rows, cols = logits.shape
+        size = 8 if dtype == _F64 else 4
+        total, ws_bytes, count, terms, ws = _buffer(code, rows, cols, size,
+                                                    size * rows if reduction else 0)
+        aux = torch.empty(total, dtype=torch.uint8, device=dev)
+        at = aux.data_ptr()
+        lp = torch.empty(rows, dtype=wide, device=dev)
+        loss = torch.empty(() if reduction else rows, dtype=wide, device=dev)
+        loss_at = loss.data_ptr()
         grad = None
-        if reduction and ctx.needs_input_grad[0] and _prefills(sh.code, sh.rows, sh.cols):
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if reduction and ctx.needs_input_grad[0] and _prefills(code, rows, cols):
+            grad = torch.empty((rows, cols), dtype=dtype, device=dev)
             ctx.capture = _capture_id(logits)
-        with _dl.on_device_of(logits):
-            timing.call("cl_policy_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
-                        old.data_ptr(), adv.data_ptr(), _dl.ptr(ref), clip_low, clip_high, kl_coef,
-                        reduction, lp.data_ptr(), at, terms, loss_at, count, _dl.ptr(grad), at + ws,
-                        sh.workspace_bytes, _dl.stream_of(logits))
+        timing.launch(logits, "cl_policy_loss_forward", code, logits.data_ptr(), logits.stride(0),
+                      rows, cols, actions.data_ptr(), ignore_index, old.data_ptr(),
+                      adv.data_ptr(), None if ref is None else ref.data_ptr(), clip_low, clip_high,
+                      kl_coef, reduction, lp.data_ptr(), at, at + terms if reduction else loss_at,
+                      loss_at, at + count, None if grad is None else grad.data_ptr(), at + ws,
+                      ws_bytes)
         ctx.save_for_backward(logits, actions, aux)
-        ctx.grad, ctx.reduction = grad, reduction
+        ctx.grad, ctx.reduction, ctx.count = grad, reduction, count
         ctx.mark_non_differentiable(lp)
         ctx.set_materialize_grads(False)
         return loss, lp
 
     @staticmethod
     def backward(ctx, grad_loss, _grad_lp):
-        _once()
         if grad_loss is None:
             return (None,) * 11
-        logits, actions, at, args, _kept = _saved(ctx)
-        grad_loss = grad_loss.contiguous()
+        logits, actions, aux = _saved(ctx)
+        if not grad_loss.is_contiguous():
+            grad_loss = grad_loss.contiguous()
+        rows, cols = logits.shape
         # the forward's gradient is handed out once, and only in the capture (or outside of any)
         # that it was written in: a replay of the backward alone would find it used
         grad, ctx.grad = ctx.grad, None
         prefilled = grad is not None and ctx.capture == _capture_id(logits)
         if not prefilled:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        with _dl.on_device_of(logits):
-            timing.call("cl_policy_loss_backward", *args, actions.data_ptr(), at, ctx.reduction,
-                        grad_loss.data_ptr(), at + ctx.count if ctx.reduction else None,
-                        int(prefilled), grad.data_ptr(), _dl.stream_of(logits))
-        return (_input_grad(ctx, grad),) + (None,) * 10
+            grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
+        at = aux.data_ptr()
+        timing.launch(logits, "cl_policy_loss_backward", _CODES[logits.dtype], logits.data_ptr(),
+                      logits.stride(0), rows, cols, actions.data_ptr(), at, ctx.reduction,
+                      grad_loss.data_ptr(), at + ctx.count, int(prefilled), grad.data_ptr())
+        return (_input_grad(ctx, grad), None, None, None, None, None, None, None, None, None,
+                None)
 
 
 class PreferenceLossFunction(torch.autograd.Function):
@@ -289,22 +278,25 @@ class PreferenceLossFunction(torch.autograd.Function):
     def forward(ctx, x, actions, offsets, ref, beta, smoothing, ignore_index, reduction,
                 group=None):
         logits = _logits_of(ctx, x, group)
-        sh = _Shape(logits)
-        wide, pairs = _wide(logits), (offsets.numel() - 1) // 2
-        margins = torch.empty(pairs, dtype=wide, device=logits.device)
-        loss = torch.empty(() if reduction else (pairs,), dtype=wide, device=logits.device)
-        aux, (_, count, row_seq, seq_slope, gaps, lp, terms, ws) = _aux(
-            logits, sh.state_bytes, sh.size, 4 * sh.rows, 2 * pairs * sh.size, 8 * sh.rows,
-            sh.rows * sh.size, pairs * sh.size if reduction else 0, sh.workspace_bytes)
+        dtype, dev = logits.dtype, logits.device
+        code = _CODES[dtype]
+        rows, cols = logits.shape
+        wide, size = (_F64, 8) if dtype == _F64 else (_F32, 4)
+        pairs = (offsets.numel() - 1) // 2
+        total, ws_bytes, count, row_seq, seq_slope, gaps, lp, terms, ws = _buffer(
+            code, rows, cols, size, 4 * rows, 2 * pairs * size, 8 * rows, size * rows,
+            size * pairs if reduction else 0)
+        aux = torch.empty(total, dtype=torch.uint8, device=dev)
         at = aux.data_ptr()
-        loss_at = loss.data_ptr() if reduction else None
-        terms_at = at + terms if reduction else loss.data_ptr()
-        with _dl.on_device_of(logits):
-            timing.call("cl_preference_loss_forward", *sh.args, actions.data_ptr(), ignore_index,
-                        _dl.ptr(ref), offsets.data_ptr(), pairs, beta, smoothing, reduction,
-                        at + lp, at, at + gaps, at + row_seq, at + seq_slope, margins.data_ptr(),
-                        terms_at, loss_at, at + count, at + ws, sh.workspace_bytes,
-                        _dl.stream_of(logits))
+        margins = torch.empty(pairs, dtype=wide, device=dev)
+        loss = torch.empty(() if reduction else pairs, dtype=wide, device=dev)
+        loss_at = loss.data_ptr()
+        timing.launch(logits, "cl_preference_loss_forward", code, logits.data_ptr(),
+                      logits.stride(0), rows, cols, actions.data_ptr(), ignore_index,
+                      None if ref is None else ref.data_ptr(), offsets.data_ptr(), pairs, beta,
+                      smoothing, reduction, at + lp, at, at + gaps, at + row_seq, at + seq_slope,
+                      margins.data_ptr(), at + terms if reduction else loss_at, loss_at,
+                      at + count, at + ws, ws_bytes)
         ctx.save_for_backward(logits, actions, aux)
         ctx.reduction, ctx.pairs, ctx.parts = reduction, pairs, (row_seq, seq_slope, count)
         ctx.mark_non_differentiable(margins)
@@ -313,36 +305,36 @@ class PreferenceLossFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_loss, _grad_margins):
-        _once()
         if grad_loss is None:
             return (None,) * 9
-        logits, actions, at, args, _kept = _saved(ctx)
+        logits, actions, aux = _saved(ctx)
+        if not grad_loss.is_contiguous():
+            grad_loss = grad_loss.contiguous()
+        rows, cols = logits.shape
         row_seq, seq_slope, count = ctx.parts
-        grad_loss = grad_loss.contiguous()
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        with _dl.on_device_of(logits):
-            timing.call("cl_preference_loss_backward", *args, actions.data_ptr(), at, at + row_seq,
-                        at + seq_slope, ctx.pairs, ctx.reduction, grad_loss.data_ptr(), at + count,
-                        grad.data_ptr(), _dl.stream_of(logits))
-        return (_input_grad(ctx, grad),) + (None,) * 8
+        grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
+        at = aux.data_ptr()
+        timing.launch(logits, "cl_preference_loss_backward", _CODES[logits.dtype],
+                      logits.data_ptr(), logits.stride(0), rows, cols, actions.data_ptr(), at,
+                      at + row_seq, at + seq_slope, ctx.pairs, ctx.reduction,
+                      grad_loss.data_ptr(), at + count, grad.data_ptr())
+        return _input_grad(ctx, grad), None, None, None, None, None, None, None, None
 
 
-def selected_log_probs(logits, actions, ignore_index: int = -100):
+# ---- public functions (_group: GroupSum's (k, tau), the logits then being its input)
+
+def selected_log_probs(logits, actions, ignore_index: int = -100, *, _group=None):
     """The log-probability log_softmax(logits)[..., actions] of the chosen class or token:
     logits [..., V], actions int64 [...] -> [...]; 0 where the action is ignore_index.
     Differentiable by the logits."""
-    return _selected_log_probs(logits, actions, ignore_index)
-
-
-def _selected_log_probs(logits, actions, ignore_index=-100, group=None):
     rows, acts = _flat(logits, actions)
-    lp = SelectedLogProbsFunction.apply(rows, acts, int(ignore_index), group)
+    lp = SelectedLogProbsFunction.apply(rows, acts, int(ignore_index), _group)
     return lp if actions.dim() == 1 else lp.reshape(actions.shape)
 
 
 def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
                 kl_coef: float = 0.0, ignore_index: int = -100, reduction: str = "mean",
-                return_log_probs: bool = False):
+                return_log_probs: bool = False, *, _group=None):
     """The clipped policy loss with a KL term.  With lp the log-probability of the row's action,
     r = exp(lp - old_log_probs) and g = ref_log_probs - lp, a row's term is::
 
@@ -353,13 +345,6 @@ def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, 
     sides or a pair (low, high).  reduction: 'mean' over the rows that count, 'sum', or 'none' (the
     terms, [...]).  With return_log_probs, also the rows' log-probabilities (not differentiable
     through this call)."""
-    return _policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs, clip, kl_coef,
-                        ignore_index, reduction, return_log_probs)
-
-
-def _policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, clip=0.2,
-                 kl_coef=0.0, ignore_index=-100, reduction="mean", return_log_probs=False,
-                 group=None):
     rows, acts = _flat(logits, actions)
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl_coef = float(low), float(high), float(kl_coef)
@@ -374,7 +359,7 @@ def _policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None,
     if ref_log_probs is not None:
         ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
     loss, lp = PolicyLossFunction.apply(rows, acts, old, adv, ref, low, high, kl_coef,
-                                        int(ignore_index), code, group)
+                                        int(ignore_index), code, _group)
     if actions.dim() != 1:
         lp = lp.reshape(actions.shape)
         if not code:
@@ -384,7 +369,7 @@ def _policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None,
 
 def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 0.1,
                     label_smoothing: float = 0.0, ignore_index: int = -100,
-                    reduction: str = "mean", return_margins: bool = False):
+                    reduction: str = "mean", return_margins: bool = False, *, _group=None):
     """The preference loss of P pairs of sequences out of one ragged batch.  Sequence q holds the
     rows offsets[q] .. offsets[q + 1] of logits [rows, V] and actions [rows] (offsets: int64
     [2 P + 1], not decreasing); the first P are the chosen sequences, sequence P + i is the one
@@ -397,12 +382,6 @@ def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 
     reduction: 'mean' over the pairs, 'sum', or 'none' (the terms, [P]).  With return_margins, also
     the margins [P] (not differentiable through this call).  Rows of no sequence do not count;
     offsets that decrease or leave the rows make their pair's term NaN."""
-    return _preference_loss(logits, actions, offsets, ref_log_probs, beta, label_smoothing,
-                            ignore_index, reduction, return_margins)
-
-
-def _preference_loss(logits, actions, offsets, ref_log_probs=None, beta=0.1, label_smoothing=0.0,
-                     ignore_index=-100, reduction="mean", return_margins=False, group=None):
     rows, acts = _flat(logits, actions)
     if logits.dim() != 2:
         raise RuntimeError("preference_loss takes logits [rows, classes] of a ragged batch")
@@ -419,5 +398,5 @@ def _preference_loss(logits, actions, offsets, ref_log_probs=None, beta=0.1, lab
         ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
     loss, margins = PreferenceLossFunction.apply(rows, acts, offsets.contiguous(), ref,
                                                  float(beta), float(label_smoothing),
-                                                 int(ignore_index), code, group)
+                                                 int(ignore_index), code, _group)
     return (loss, margins) if return_margins else loss

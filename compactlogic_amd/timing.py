@@ -75,13 +75,19 @@ def record(settle: bool = True, repeat: dict | None = None):
         _active = prev
 
 
-def call(name: str, *args) -> None:
-    """_capi.call(name, *args), bracketed when a recorder is active: `timed` for the calls whose
-    kernels are shorter than a closure and its frame."""
-    if _active is None:
-        _capi.call(name, *args)
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """Entry point `name` with `args` and the current stream of t's device, on that device: what
+    _capi.call inside of torch.cuda.device and `timed` does, for calls whose kernels are shorter
+    than a closure and two context managers."""
+    index = t.get_device()
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            timed(name, lambda: _capi.call(name, *args, stream))
+    elif _active is not None:
+        timed(name, lambda: _capi.call(name, *args, stream))
     else:
-        timed(name, lambda: _capi.call(name, *args))
+        _capi.call(name, *args, stream)
 
 
 def timed(name: str, fn, stream=None):
