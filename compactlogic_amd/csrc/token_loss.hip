@@ -425,7 +425,9 @@ __device__ __forceinline__ void emit_grad(const RowArgs<T>& a, const GradOut<T>&
                                      a.through_store);
 }
 
-// ---- short rows: TPR lanes (16 or 64) of a wave per row, several rows per workgroup, no LDS.
+// ---- short rows: TPR lanes (16 or 64) of a wave per row, several rows per workgroup, no LDS.  A
+// launch and the chain action -> logits -> fp64 scalars bound it: 128 x 10 or 1024 x 200 fp32 take
+// 3.4 us.
 template <typename T, int TPR, int NV, typename Op, bool GRAD>
 __global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op, GradOut<T> out) {
     using A = wide_t<T>;
@@ -445,7 +447,12 @@ __global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op, G
     if constexpr (GRAD) emit_grad<T, TPR, NV>(a, out, n, act, t, row, st);
 }
 
-// ---- a row per workgroup, held in its registers between the loss and the gradient.
+// ---- a row per workgroup, held in its registers between the loss and the gradient.  Bound by
+// memory: 8192 x 32768 bf16, a quarter of the rows ignored (403 MB read, 537 written), 155 us = 6.0
+// TB/s; 2047 x 32003 fp32, a tenth ignored (236 MB read, 262 written), 83 us.  Eight waves per SIMD
+// (64 registers, four of them spilled round the fp64 scalars) let two workgroups or more of a CU
+// take turns at loading and storing: the step on 8192 x 32768 took 247 us at four waves, 236 at
+// eight, before the choices of cut and cache below and above.
 template <typename T, int TPR, int NV, typename Op>
 __global__ __launch_bounds__(TPR, 8) void k_rows_held(RowArgs<T> a, Op op, GradOut<T> out) {
     using A = wide_t<T>;
@@ -478,6 +485,8 @@ __global__ __launch_bounds__(TPR, 8) void k_rows_held(RowArgs<T> a, Op op, GradO
 }
 
 // ---- a row per workgroup, read once with a running maximum and sum; ignored rows are not read.
+// One exponential per element and one per 32 for the running maximum.  Bound by memory: 8192 x
+// 32000 bf16 81 us = 6.4 TB/s.
 constexpr int kStreamUnroll = 4;  // vectors in flight per thread
 
 // Vectors lo..hi-1 of a row, and its loose elements with `loose`.
@@ -542,7 +551,8 @@ __global__ __launch_bounds__(kRowBlock) void k_rows_stream(RowArgs<T> a, Op op) 
     if (wave_id() == 0) finish_row<64>(a, op, n, act, xa, in, m, s, lane_id() == 0);
 }
 
-// ---- few long rows: (row, part) workgroups, the parts joined by one wave per row.
+// ---- few long rows: (row, part) workgroups, the parts joined by one wave per row.  16 rows of
+// 131072 fp16: 3.6 + 3.0 us, where one workgroup per row took 108 us.
 template <typename T>
 __global__ __launch_bounds__(kRowBlock) void k_rows_split(RowArgs<T> a, int parts, int per,
                                                           wide_t<T>* __restrict__ ws) {
@@ -608,7 +618,8 @@ struct Upstream {
     }
 };
 
-// Rows whose slope is 0 are written without being read: ignored, clipped, or of no sequence.
+// ---- the gradient in a pass of its own.  Rows whose slope is 0 are written without being read:
+// ignored, clipped, or of no sequence.  Bound by memory: 8192 x 32000 bf16 165 us = 6.3 TB/s.
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(kRowBlock) void k_grad_short(RowArgs<T> a, Upstream<wide_t<T>> up,
                                                           T* __restrict__ grad) {
@@ -828,7 +839,7 @@ __global__ __launch_bounds__(kSumThreads) void k_pref_sum(const A* __restrict__ 
                                                           A* __restrict__ count) {
     __shared__ double red[kSumThreads / 64];
     double t = 0;
-    for (int64_t i = threadIdx.x; i < pairs; i += kSumThreads) t += double(terms[i]);
+    for (int64_t i = threadIdx.x; i < pairs; i += blockDim.x) t += double(terms[i]);
     t = group_sum(t, red);
     if (threadIdx.x == 0) {
         loss[0] = A(mean ? t / double(pairs) : t);
@@ -836,17 +847,17 @@ __global__ __launch_bounds__(kSumThreads) void k_pref_sum(const A* __restrict__ 
     }
 }
 
-// Both in one launch, for batches of few rows: 64 rows of lanes, or 16 waves, take the pairs in
-// turn.
-template <int LANES, typename A>
+// Both in one launch, 16 lanes per pair: for batches of at most 64 pairs of about 128 rows, each
+// pair's loads then in flight together.
+template <typename A>
 __global__ __launch_bounds__(kSumThreads) void k_pref_small(PairArgs<A> a, int mean,
                                                             A* __restrict__ loss,
                                                             A* __restrict__ count) {
     __shared__ double red[kSumThreads / 64];
     double t = 0;
-    for (int64_t i = threadIdx.x / LANES; i < a.pairs; i += kSumThreads / LANES) {
-        const double term = pair_term<LANES>(a, i, nullptr);
-        t += threadIdx.x % LANES == 0 ? term : 0.0;
+    for (int64_t i = threadIdx.x / 16; i < a.pairs; i += kSumThreads / 16) {
+        const double term = pair_term<16>(a, i, nullptr);
+        t += threadIdx.x % 16 == 0 ? term : 0.0;
     }
     if (!loss) return;
     t = group_sum(t, red);
@@ -884,9 +895,12 @@ RowArgs<T> row_args(const void* logits, int64_t row_stride, int64_t rows, int64_
     return a;
 }
 
-// Rows up to 4 KB stay in registers of a wave or a quarter of one; longer ones take a workgroup,
-// or several where the rows alone would not fill the card.
-constexpr int64_t kPrefSmallRows = 16384, kPrefSmallPairs = 256, kPrefLongRows = 2048;
+// Rows up to 256 bytes stay in registers of 16 lanes, up to 4 KB of a wave; longer ones take a
+// workgroup, or several where the rows alone would not fill the card.  Chosen log-probabilities and
+// gradient: 20000 x 64 fp32 16 us on 16 lanes, 22 on 64; 12000 x 1000 fp32 32 us on a wave, 42 on a
+// workgroup; 16 x 131072 see k_rows_split.
+constexpr int64_t kPrefSmallPairs = 64;
+constexpr int64_t kPrefSmallRows = 128, kPrefLongRows = 2048;  // of a pair, on average
 constexpr int64_t kSplitBlocks = 1024;  // workgroups wanted
 constexpr int kMaxParts = 64;           // joined by the lanes of one wave
 
@@ -947,7 +961,10 @@ bool launch_short(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipS
 }
 
 // The largest row, in bytes, that one workgroup holds, and the fewest logits, in bytes, for which
-// the loss and its gradient are taken in one pass.
+// the loss and its gradient are taken in one pass (67 MB of fp32 36 us, 43 in two; 34 MB of bf16 31
+// and 30, the one pass having two launches more).  fp16 keeps two: a gradient formed before the
+// upstream one is known may vanish in half's range, which a scaled loss is meant to prevent.  fp64
+// rows are not worth their registers.
 constexpr int64_t kHeldRow = 131072;
 constexpr int64_t kHeldLogits = int64_t(48) << 20;
 
@@ -1202,27 +1219,26 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
                              static_cast<A*>(terms)};
         const int mean = reduction == CL_REDUCE_MEAN;
         A* out = reduction != CL_REDUCE_NONE ? static_cast<A*>(loss) : nullptr;
-        // a wave takes 512 rows of a pair at a time, a workgroup 8192: a step on one pair of 32768
-        // rows each of 64 classes 43 us instead of 86
-        const bool longs = pairs > 0 && rows / pairs > kPrefLongRows;
-        if (!longs && rows <= kPrefSmallRows && pairs <= kPrefSmallPairs) {
-            // up to 16 loads of a row of lanes per pair, else a wave's
-            if (pairs > 0 && rows / pairs <= 256)
-                k_pref_small<16, A><<<1, kSumThreads, 0, s>>>(pa, mean, out,
-                                                             static_cast<A*>(count));
-            else if (pairs > 0 || out)
-                k_pref_small<64, A><<<1, kSumThreads, 0, s>>>(pa, mean, out,
-                                                             static_cast<A*>(count));
+        // Steps on 64 classes: 64 pairs of 1 + 1 rows take 19.6 us in one launch and 20.1 in two,
+        // of 128 + 128 21.7 and 20.6; one pair of 32768 rows each 43 us by a workgroup (8192 rows
+        // at a time), 86 by a wave (512).
+        const int64_t each = pairs > 0 ? rows / pairs : 0;
+        if (pairs <= kPrefSmallPairs && each <= kPrefSmallRows) {
+            if (pairs > 0 || out)
+                k_pref_small<A><<<1, kSumThreads, 0, s>>>(pa, mean, out, static_cast<A*>(count));
             return check_launch("cl_preference_loss_forward(pairs)");
         }
+        const bool longs = each > kPrefLongRows;
         if (longs)
             k_pref_long<A><<<unsigned(pairs), kSumThreads, 0, s>>>(pa);
         else if (pairs > 0)
             k_pref_pairs<A><<<unsigned(ceil_div(pairs, kRowBlock / 64)), kRowBlock, 0, s>>>(pa);
         if (int rc = check_launch("cl_preference_loss_forward(pairs)")) return rc;
-        if (out)
-            k_pref_sum<A><<<1, kSumThreads, 0, s>>>(static_cast<const A*>(terms), pairs, mean, out,
-                                                    static_cast<A*>(count));
+        if (out) {
+            const int64_t threads = std::min<int64_t>(kSumThreads, ceil_div(pairs, 64) * 64);
+            k_pref_sum<A><<<1, unsigned(threads), 0, s>>>(static_cast<const A*>(terms), pairs,
+                                                          mean, out, static_cast<A*>(count));
+        }
     });
     return check_launch("cl_preference_loss_forward(sum)");
 }
