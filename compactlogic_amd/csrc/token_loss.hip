@@ -245,18 +245,17 @@ __device__ __forceinline__ wide_t<T> action_logit(const RowArgs<T>& a, const T* 
 }
 
 // ---- gradient of one logit: c ([j = a] - p_j) as exp(x - m) * k, k = -c / s; the action's own,
-// c (1 - p_a), is written over it by the thread that wrote it.  A result of 16 bits takes the
-// exponent as one product and sum, off by some 2^-20 of it; fp32 takes it as the loss does.
+// c (1 - p_a), is written over it by the thread that wrote it.  A result of 16 bits takes log2 e as
+// one number, off by some 2^-20 of the result; fp32 takes it as the loss does.
 template <typename T>
 struct RowGrad {
     using A = wide_t<T>;
-    A m, k, own, shift;
+    A m, k, own;
     __device__ __forceinline__ RowGrad(const RowState<A>& st, A c)
-        : m(st.m), k(-c * st.inv_s), own(c * st.rest), shift(st.m * A(-1.44269504088896340736)) {}
+        : m(st.m), k(-c * st.inv_s), own(c * st.rest) {}
     __device__ __forceinline__ T operator()(T x) const {
         if constexpr (sizeof(T) == 2)
-            return T(__builtin_amdgcn_exp2f(__builtin_fmaf(A(x), 1.44269504088896340736f, shift)) *
-                     k);
+            return T(__builtin_amdgcn_exp2f((A(x) - m) * 1.44269504088896340736f) * k);
         else
             return T(exp_diff(A(x) - m) * k);
     }

@@ -278,6 +278,37 @@ def test_masked_logits_and_rows(device, one_pass, vocab, dtype):
     assert (g[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [7, 300, 5001, 20001, 70001])
+def test_rows_of_the_lowest_value(device, one_pass, vocab, dtype):
+    """A mask of the type's lowest value that leaves nothing, or one class of an ordinary or of the
+    highest value: equal probabilities, or all of it for that class."""
+    info = torch.finfo(dtype)
+    z = torch.full((6, vocab), info.min, dtype=dtype, device=device)
+    a = torch.tensor([0, vocab - 1, 2, 2, 2, 3], device=device)
+    z[2, 2], z[3, 3], z[4, 2] = 1.5, -2.0, info.max
+    z[5, :] = info.max
+    z.requires_grad_()
+    lp = cl.selected_log_probs(z, a)
+    low = _np(z)[0, 0]
+    zn = _np(z)
+    zn = zn - zn.max(1, keepdims=True)       # in 64 bits these differences are finite
+    lpn, probs = P.log_probs(zn, a.cpu().numpy())
+    err = (vocab / 256 + 40) * _unit(dtype)
+    want = _np(lp)
+    ok = [0, 1, 2, 4, 5]
+    _near(want[ok], lpn[ok], err, _wide(dtype))
+    assert want[3] == -np.inf or want[3] <= low / 2      # beyond the wide type, or far down
+    up = torch.ones(6, dtype=_wide(dtype), device=device)
+    (g,) = torch.autograd.grad(lp, z, up)
+    _near(_np(g), P.logit_gradient(probs, a.cpu().numpy(), np.ones(6)), 2 * err, dtype)
+    old = torch.where(lp.detach().isinf(), 0, lp.detach())
+    loss = cl.policy_loss(z, a, old, up, reduction="sum")
+    (g,) = torch.autograd.grad(loss, z)
+    slope = -np.exp(np.minimum(want - _np(old), 0.0))
+    _near(_np(g), P.logit_gradient(probs, a.cpu().numpy(), slope), 4 * err, dtype)
+
+
 def test_nothing_counts(device, one_pass):
     z = torch.randn(4, 9, device=device, requires_grad=True)
     a = torch.full((4,), IGNORE, device=device)
