@@ -4,7 +4,9 @@ Same public modules as the reference package `compactlogic` (compactlogic/__init
 LogicLayer, ConvLayer, GroupSum and the autograd bridges LogicLayerCudaFunction and
 ConvLayerCudaFunction, plus the packed-bit inference API (PackBitsTensor), and the logic-tree
 conv blocks of the third-party ConvLogic package (ConvLogicLayer, TreeLogicLayer,
-PoolLogicLayer).  All numerics run in libcompactlogic_hip.so, built in-tree by
+PoolLogicLayer).  Beside the reference's modules: losses for training by reward or preference
+(policy.py), dropout between logic layers (dropout_layer.py), a fused optimizer step (optim.py).
+All numerics run in libcompactlogic_hip.so, built in-tree by
 ``python -m compactlogic_amd.build``.
 """
 from . import checkpoint, circuit, convlogic_hip, difflogic_hip

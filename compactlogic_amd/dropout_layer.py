@@ -72,9 +72,9 @@ def dropout(x, p: float, seed, offset: int = 0, fill: float | None = None):
     relaxed activation in [0, 1]).
 
     seed, offset: integers, or seed an int64 tensor (seed, offset) on x's device, read when the
-    kernel runs (so a captured graph follows it).  Equal ones give equal masks; the last
-    dimension is the column, those before it together the row.  Where nothing can be dropped
-    (p below 2^-17) x itself is returned."""
+    kernel runs (so a captured graph follows it).  Equal ones give equal masks: the first
+    dimension is the row, the others together the column (so that Flatten may come before or
+    after).  Where nothing can be dropped (p below 2^-17) x itself is returned."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be a tensor")
     if x.device.type != "cuda":
@@ -91,7 +91,7 @@ def dropout(x, p: float, seed, offset: int = 0, fill: float | None = None):
         rng, seed = seed.contiguous(), 0
     if threshold == 0 or x.numel() == 0:
         return x
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1] if x.dim() else 1)
+    flat = x if x.dim() == 2 else x.reshape(x.shape[0] if x.dim() > 2 else 1, -1)
     y = DropoutFunction.apply(flat, threshold, None if fill is None else float(fill),
                               int(seed) & (2**64 - 1), int(offset) & (2**64 - 1), rng)
     return y if x.dim() == 2 else y.reshape(x.shape)

@@ -631,6 +631,42 @@ def test_captured_policy_step(device, one_pass):
         del junk
 
 
+def test_policy_and_reference_under_one_mask(device):
+    """As they are used together: a network with dropout records its log-probabilities under the
+    masks of a step, and a later evaluation under the same masks has ratios of 1: the loss is minus
+    the mean advantage, the margins against itself are 0, to rounding; other masks give others."""
+    torch.manual_seed(2)
+    layers = [cl.LogicLayer(60, 400, connections="original"), cl.LogicLayer(400, 400)]
+    net = torch.nn.Sequential(*layers).to(device)
+    head = cl.GroupSum(10, 3.0)
+    x = (torch.rand(128, 60, device=device) < 0.4).float()
+    a = torch.randint(0, 10, (128,), device=device)
+    adv = torch.randn(128, device=device)
+
+    def body(offset):
+        return net[1](cl.dropout(net[0](x), 0.2, 77, offset, fill=0.5))
+
+    with torch.no_grad():
+        old = head.log_probs(body(3), a)
+        other = head.log_probs(body(4), a)
+    assert not torch.equal(old, other)
+    loss, lp = head.policy_loss(body(3), a, old, adv, ref_log_probs=old, kl_coef=0.1,
+                                return_log_probs=True)
+    assert torch.equal(lp, old)
+    # the recorded log-probabilities are rounded once, what the losses compare them with is not
+    step = 2.0**-24 * float(old.abs().max())
+    assert abs(float(loss.detach()) + float(adv.double().mean())) \
+        <= float(adv.abs().mean()) * (step + 2.0**-22)
+    loss.backward()
+    assert all(p.grad.abs().sum() > 0 for p in net.parameters())
+    off = torch.arange(0, 129, 2, device=device)[:65]
+    loss, h = head.preference_loss(body(3), a, off, ref_log_probs=old, return_margins=True)
+    assert float(h.abs().max()) <= 0.1 * 2 * 2 * step      # two sequences of two rows
+    assert abs(float(loss.detach()) - np.log(2)) <= 0.1 * 2 * step + 2.0**-24
+    _, h = head.preference_loss(body(3), a, off, ref_log_probs=other, return_margins=True)
+    assert float(h.abs().max()) > 0.01
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("vocab", [10, 3001, 70001])
 def test_captured_losses(device, one_pass, dtype, vocab):
