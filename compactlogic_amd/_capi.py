@@ -100,6 +100,8 @@ SIGNATURES: dict[str, list] = {
     "cl_group_sum_centered_workspace_size": [_int, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "cl_group_sum_centered_forward": [_int, _p, _i64, _i64, _i64, _i64, _i64, _f64, _p, _p, _i64,
                                       _p],
+    "cl_group_sum_chosen_backward": [_int, _p, _i64, _i64, _i64, _f64, _p, _p, _p, _p, _p, _p, _p,
+                                     _p, _i64, _p, _i64, _i64, _p],
     "cl_group_sum_workspace_size": [_int, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64)],
     "cl_group_sum_backward": [_int, _p, _i64, _i64, _i64, _f64, _p, _i64, _i64, _p],
     "cl_group_sum_cross_entropy_forward": [_int, _p, _i64, _i64, _i64, _i64, _i64, _f64, _p,

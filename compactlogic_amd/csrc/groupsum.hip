@@ -10,6 +10,7 @@
 //   feature-contiguous (stride_feature == 1): one wave reduces one contiguous group
 // and a plain strided variant for anything else.
 #include "common.h"
+#include "row_loss.h"
 
 #include <algorithm>
 
@@ -301,6 +302,26 @@ __global__ __launch_bounds__(256) void k_gsum_center_any(const T* __restrict__ x
     __syncthreads();
     if (threadIdx.x < 16) center_row(z, int(k), out + n * k);
 }
+
+// A loss on the log-probability of the chosen class (row_loss.h): the gradient of the scores is
+// formed where it is spread over the features, in the same operations as in a pass of its own.
+template <typename T>
+struct ChosenGrad {
+    const T* scores;
+    const RowState<T>* state;
+    const int64_t* actions;
+    Upstream<T> up;
+    int64_t k;
+    T tau;
+    __device__ __forceinline__ T operator()(int64_t n, int64_t c) const {
+        const RowState<T> st = state[n];
+        const int64_t act = actions[n];
+        const T z = scores[n * k + c];
+        const T g = up(n, st.slope);
+        if (g == T(0)) return T(0);
+        return (c == act ? g * st.rest : exp_diff(z - st.m) * (-g * st.inv_s)) / tau;
+    }
+};
 
 // ---- backward: grad_x[n, j] = src(n, j / gsz).  Elements are visited in memory order
 // of grad_x: `inner` is the unit-stride dimension (batch or feature).
@@ -719,6 +740,39 @@ extern "C" int cl_group_sum_backward(int dtype, const void* grad_out, int64_t ba
                                 stride_feature, s);
     });
     return check_launch("cl_group_sum_backward");
+}
+
+extern "C" int cl_group_sum_chosen_backward(int dtype, const void* scores, int64_t batch,
+                                            int64_t features, int64_t k, double tau,
+                                            const int64_t* actions, const void* row_state,
+                                            const void* row_grad, const void* loss_grad,
+                                            const void* count, const int32_t* row_seq,
+                                            const void* seq_slope, const void* pair_grad,
+                                            int64_t pairs, void* grad_x, int64_t stride_batch,
+                                            int64_t stride_feature, void* stream) {
+    clear_error();
+    CL_ARG(batch >= 0 && features >= 0, "negative shape");
+    CL_ARG(k >= 1, "k must be >= 1, got %lld", (long long)k);
+    CL_ARG(stride_batch >= 0 && stride_feature >= 0, "negative strides are not supported");
+    CL_ARG(pairs >= 0 && (!row_seq || pairs == 0 || seq_slope), "null pointer argument");
+    if (batch == 0 || features == 0) return CL_OK;
+    CL_ARG(scores && actions && row_state && grad_x, "null pointer argument");
+    CL_ARG(row_grad || loss_grad || pair_grad || (row_seq && pairs == 0),
+           "an upstream gradient is needed");
+    hipStream_t s = as_stream(stream);
+    CL_DTYPE_SWITCH(dtype, {
+        using T = scalar_t;
+        const Upstream<T> up{static_cast<const T*>(row_grad), static_cast<const T*>(loss_grad),
+                             static_cast<const T*>(count), row_seq,
+                             static_cast<const T*>(seq_slope), static_cast<const T*>(pair_grad),
+                             pairs};
+        const ChosenGrad<T> src{static_cast<const T*>(scores),
+                                static_cast<const RowState<T>*>(row_state), actions, up, k,
+                                T(tau)};
+        launch_gsum_backward<T>(src, batch, features, k, static_cast<T*>(grad_x), stride_batch,
+                                stride_feature, s);
+    });
+    return check_launch("cl_group_sum_chosen_backward");
 }
 
 extern "C" int cl_group_sum_cross_entropy_workspace_size(int dtype, int64_t batch,

@@ -28,6 +28,7 @@ from . import timing
 
 _CODES = _dl._STORAGE_DTYPES
 _F32, _F64 = torch.float32, torch.float64
+_MEAN = _capi.CL_REDUCE["mean"]
 
 
 def _flat(logits, actions):
@@ -142,20 +143,21 @@ def _logits_of(ctx, x, group):
     return scores
 
 
-def _input_grad(ctx, grad):
-    """The input's gradient from the logits': through GroupSum, in its input's layout."""
-    if ctx.group is None:
-        return grad
+def _group_grad(ctx, scores, actions, at, row_grad=None, loss_grad=None, count=None, row_seq=None,
+                seq_slope=None, pair_grad=None, pairs=0):
+    """The gradient of GroupSum's input in its layout, formed from the scores where it is spread
+    over the features."""
     k, tau, batch, feats, batch_major = ctx.group
+    dtype, dev = scores.dtype, scores.device
     if batch_major:
         sb, sf = 1, batch
-        grad_x = torch.empty_strided((batch, feats), (1, batch), dtype=grad.dtype,
-                                     device=grad.device)
+        grad_x = torch.empty_strided((batch, feats), (1, batch), dtype=dtype, device=dev)
     else:
         sb, sf = feats, 1
-        grad_x = torch.empty((batch, feats), dtype=grad.dtype, device=grad.device)
-    timing.launch(grad, "cl_group_sum_backward", _CODES[grad.dtype], grad.data_ptr(), batch, feats,
-                  k, tau, grad_x.data_ptr(), sb, sf)
+        grad_x = torch.empty((batch, feats), dtype=dtype, device=dev)
+    timing.launch(scores, "cl_group_sum_chosen_backward", _CODES[dtype], scores.data_ptr(), batch,
+                  feats, k, tau, actions.data_ptr(), at, row_grad, loss_grad, count, row_seq,
+                  seq_slope, pair_grad, pairs, grad_x.data_ptr(), sb, sf)
     return grad_x
 
 
@@ -203,12 +205,15 @@ class SelectedLogProbsFunction(torch.autograd.Function):
         logits, actions, aux = _saved(ctx)
         if not grad_lp.is_contiguous():
             grad_lp = grad_lp.contiguous()
+        if ctx.group is not None:
+            return _group_grad(ctx, logits, actions, aux.data_ptr(),
+                               row_grad=grad_lp.data_ptr()), None, None, None
         rows, cols = logits.shape
         grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
         timing.launch(logits, "cl_selected_log_prob_backward", _CODES[logits.dtype],
                       logits.data_ptr(), logits.stride(0), rows, cols, actions.data_ptr(),
                       aux.data_ptr(), grad_lp.data_ptr(), grad.data_ptr())
-        return _input_grad(ctx, grad), None, None, None
+        return grad, None, None, None
 
 
 class PolicyLossFunction(torch.autograd.Function):
@@ -232,7 +237,7 @@ class PolicyLossFunction(torch.autograd.Function):
         loss = torch.empty(() if reduction else rows, dtype=wide, device=dev)
         loss_at = loss.data_ptr()
         grad = None
-        if reduction and ctx.needs_input_grad[0] and _prefills(code, rows, cols):
+        if reduction and group is None and ctx.needs_input_grad[0] and _prefills(code, rows, cols):
             grad = torch.empty((rows, cols), dtype=dtype, device=dev)
             ctx.capture = _capture_id(logits)
         timing.launch(logits, "cl_policy_loss_forward", code, logits.data_ptr(), logits.stride(0),
@@ -254,6 +259,13 @@ class PolicyLossFunction(torch.autograd.Function):
         logits, actions, aux = _saved(ctx)
         if not grad_loss.is_contiguous():
             grad_loss = grad_loss.contiguous()
+        reduction, at = ctx.reduction, aux.data_ptr()
+        if ctx.group is not None:
+            up = grad_loss.data_ptr()
+            gx = _group_grad(ctx, logits, actions, at, loss_grad=up,
+                             count=at + ctx.count if reduction == _MEAN else None) if reduction \
+                else _group_grad(ctx, logits, actions, at, row_grad=up)
+            return gx, None, None, None, None, None, None, None, None, None, None
         rows, cols = logits.shape
         # the forward's gradient is handed out once, and only in the capture (or outside of any)
         # that it was written in: a replay of the backward alone would find it used
@@ -261,12 +273,10 @@ class PolicyLossFunction(torch.autograd.Function):
         prefilled = grad is not None and ctx.capture == _capture_id(logits)
         if not prefilled:
             grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
-        at = aux.data_ptr()
         timing.launch(logits, "cl_policy_loss_backward", _CODES[logits.dtype], logits.data_ptr(),
-                      logits.stride(0), rows, cols, actions.data_ptr(), at, ctx.reduction,
+                      logits.stride(0), rows, cols, actions.data_ptr(), at, reduction,
                       grad_loss.data_ptr(), at + ctx.count, int(prefilled), grad.data_ptr())
-        return (_input_grad(ctx, grad), None, None, None, None, None, None, None, None, None,
-                None)
+        return grad, None, None, None, None, None, None, None, None, None, None
 
 
 class PreferenceLossFunction(torch.autograd.Function):
@@ -310,15 +320,22 @@ class PreferenceLossFunction(torch.autograd.Function):
         logits, actions, aux = _saved(ctx)
         if not grad_loss.is_contiguous():
             grad_loss = grad_loss.contiguous()
-        rows, cols = logits.shape
         row_seq, seq_slope, count = ctx.parts
-        grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
         at = aux.data_ptr()
+        if ctx.group is not None:
+            up, mean = grad_loss.data_ptr(), ctx.reduction == _MEAN
+            gx = _group_grad(ctx, logits, actions, at, loss_grad=up if ctx.reduction else None,
+                             count=at + count if mean else None, row_seq=at + row_seq,
+                             seq_slope=at + seq_slope, pair_grad=None if ctx.reduction else up,
+                             pairs=ctx.pairs)
+            return gx, None, None, None, None, None, None, None, None
+        rows, cols = logits.shape
+        grad = torch.empty((rows, cols), dtype=logits.dtype, device=logits.device)
         timing.launch(logits, "cl_preference_loss_backward", _CODES[logits.dtype],
                       logits.data_ptr(), logits.stride(0), rows, cols, actions.data_ptr(), at,
                       at + row_seq, at + seq_slope, ctx.pairs, ctx.reduction,
                       grad_loss.data_ptr(), at + count, grad.data_ptr())
-        return _input_grad(ctx, grad), None, None, None, None, None, None, None, None
+        return grad, None, None, None, None, None, None, None, None
 
 
 # ---- public functions (_group: GroupSum's (k, tau), the logits then being its input)

@@ -642,6 +642,20 @@ int cl_preference_loss_backward(int dtype, const void* logits, int64_t row_strid
                                 int reduction, const void* grad_loss, const void* count,
                                 void* grad_logits, void* stream);
 
+/* The input gradient of any of the three losses where the logits were GroupSum's scores (F32 or
+ * F64, [batch, k], as cl_group_sum_centered_forward gives them): what cl_group_sum_backward makes
+ * of the loss's own backward, bit by bit, without storing the scores' gradient.  Upstream: row_grad
+ * [batch] (the log-probabilities, or a policy loss without reduction), else loss_grad, a device
+ * scalar, divided by count[0] where count is given, or pair_grad [pairs] (a preference loss without
+ * reduction); row_seq, seq_slope and pairs as the preference loss left them, else NULL and 0. */
+int cl_group_sum_chosen_backward(int dtype, const void* scores, int64_t batch, int64_t features,
+                                 int64_t k, double tau, const int64_t* actions,
+                                 const void* row_state, const void* row_grad,
+                                 const void* loss_grad, const void* count,
+                                 const int32_t* row_seq, const void* seq_slope,
+                                 const void* pair_grad, int64_t pairs, void* grad_x,
+                                 int64_t stride_batch, int64_t stride_feature, void* stream);
+
 /* -------------------------------------------------------------------------------------------
  * Dropout whose mask is a function of (seed, offset, row, column) and is not stored (no
  * counterpart in the reference).  Philox 4x32-10 (Salmon et al., SC'11) with key seed and

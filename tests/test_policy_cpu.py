@@ -57,6 +57,14 @@ def test_c_arguments_are_checked_before_the_device():
     assert need.value == -1
     assert lib.cl_group_sum_centered_forward(0, 1, 64, 900, 1, 64, 513, 1.0, 1, 1, 1, None) == bad
     assert lib.cl_group_sum_centered_forward(0, 1, 64, 900, 1, 64, 10, 1.0, 1, None, 0, None) == bad
+    def chosen(batch=4, k=10, scores=1, up=1, sb=1, pairs=0, seq=None, slope=None):
+        return lib.cl_group_sum_chosen_backward(0, scores, batch, 100, k, 1.0, 1, 1, up, None, None,
+                                                seq, slope, None, pairs, 1, sb, 4, None)
+
+    assert chosen(batch=0) == ok
+    assert chosen(batch=-1) == bad and chosen(k=0) == bad and chosen(scores=None) == bad
+    assert chosen(up=None) == bad and b"upstream" in lib.cl_last_error()
+    assert chosen(sb=-1) == bad and chosen(pairs=-1) == bad and chosen(pairs=2, seq=1) == bad
     assert policy(low=-0.1) == bad and policy(low=float("nan")) == bad
     assert policy(kl=0.1) == bad and b"KL" in lib.cl_last_error()
     assert policy(red=3) == bad and policy(loss=None) == bad and policy(old=None) == bad

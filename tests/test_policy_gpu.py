@@ -550,6 +550,43 @@ def test_group_sum_methods(device, batch, feats, k, layout, dtype):
     check(torch.autograd.grad(loss, x)[0], slope, 0.3 * 0.6 * err + 0.3 * 4 * unit)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_group_sum_gradient_is_that_of_the_scores(device, dtype, reduction):
+    """The fused backward gives what the losses' own gradient of the (centred) scores gives through
+    GroupSum, bit by bit, in every layout and reduction."""
+    batch, feats, k, tau = 96, 1201, 10, 3.0
+    g = torch.Generator().manual_seed(5)
+    base = torch.rand((batch, feats), generator=g, dtype=torch.float64).to(dtype).to(device)
+    a = torch.randint(0, k, (batch,), generator=g).to(device)
+    a[::9] = IGNORE
+    old = (torch.randn(batch, generator=g) * 0.2 - 2.3).to(dtype).to(device)
+    adv, ref = torch.randn(batch, generator=g).to(dtype).to(device), old + 0.1
+    off = torch.tensor([0, 20, 40, 41, 60, 60, 90], device=device)
+    gs = cl.GroupSum(k, tau)
+    for x in (base.clone(), base.t().contiguous().t(), base[:, :1200:1].clone()):
+        x.requires_grad_()
+        seen = []
+
+        class Spy:
+            group = None
+        scores = policy._logits_of(Spy(), x.detach(), (k, tau)).requires_grad_()
+        up = torch.randn(batch if reduction == "none" else (), generator=g,
+                         dtype=torch.float64).to(dtype).to(device)
+        seen.append((gs.policy_loss(x, a, old, adv, ref, kl_coef=0.1, reduction=reduction),
+                     cl.policy_loss(scores, a, old, adv, ref, kl_coef=0.1, reduction=reduction),
+                     up))
+        up = up[:3].contiguous() if reduction == "none" else up
+        seen.append((gs.preference_loss(x, a, off, ref, beta=0.5, reduction=reduction),
+                     cl.preference_loss(scores, a, off, ref, beta=0.5, reduction=reduction), up))
+        seen.append((gs.log_probs(x, a), cl.selected_log_probs(scores, a), adv))
+        for fused, apart, u in seen:
+            assert torch.equal(fused, apart)
+            (gx,) = torch.autograd.grad(fused, x, u)
+            (gz,) = torch.autograd.grad(apart, scores, u)
+            assert torch.equal(gx, torch.autograd.grad(gs(x), x, gz)[0])
+
+
 def test_group_sum_methods_shapes(device):
     """Leading dimensions, non-finite activations, refusals."""
     gs = cl.GroupSum(5, 2.0)
