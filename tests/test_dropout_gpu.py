@@ -226,3 +226,23 @@ def test_network_with_dropout_matches_its_layers(device):
     assert torch.equal(cl.PackedNetwork(net)(cl.PackBitsTensor(bits, 64)), want)
     c = cl.circuit.extract_circuit(net)
     assert c.k == 10 and len(c.gates) == 2
+
+
+@pytest.mark.parametrize("layout", ["rows", "columns"])
+def test_large_tensors(device, layout):
+    """First, middle and last rows of tensors past 32 bits, against the oracle's counters."""
+    if layout == "rows":                  # 2^31 blocks and some, one each for a thread
+        rows, cols = 262145, 65536
+        x = torch.ones((rows, cols), dtype=torch.bfloat16, device=device)
+    else:                                 # 2^32 elements and some
+        rows, cols = 70000, 65537
+        x = torch.ones((cols, rows), dtype=torch.bfloat16, device=device).t()
+    y = cl.dropout(x, 0.5, SEED, OFFSET, fill=0.0)
+    for r in (0, rows // 2, rows - 1):
+        blocks = -(-cols // 8)
+        counter = np.zeros((blocks, 4), dtype=np.uint64)
+        counter[:, 0], counter[:, 1] = np.arange(blocks), r
+        counter[:, 2], counter[:, 3] = OFFSET & 0xFFFFFFFF, OFFSET >> 32
+        words = D.philox(counter, np.array([SEED & 0xFFFFFFFF, SEED >> 32], dtype=np.uint64))
+        halves = np.stack((words & 0xFFFF, words >> 16), -1).reshape(-1)[:cols]
+        np.testing.assert_array_equal(y[r].float().cpu().numpy(), (halves >= 32768) * 1.0)

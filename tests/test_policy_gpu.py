@@ -865,3 +865,30 @@ def test_rows_beyond_32_bits(device):
     lp = cl.selected_log_probs(x, c.act_t)
     assert torch.equal(lp, cl.selected_log_probs(c.logits, c.act_t))
     _near(_np(lp), c.lp, c.err, c.wide)
+
+
+def test_more_than_2_to_32_logits(device):
+    """The last rows of 66000 x 65536 logits (8.7 GB), in one pass and in two."""
+    rows, vocab = 66000, 65536
+    z = torch.empty((rows, vocab), dtype=torch.bfloat16, device=device)
+    z.copy_((torch.randn(vocab, device=device) * 2.5).expand(rows, vocab))
+    c = Case(4, vocab, torch.bfloat16, device, ignored=0.0)
+    z[-4:] = c.logits
+    a = torch.full((rows,), IGNORE, device=device)
+    a[-4:] = c.act_t
+    f = torch.zeros(rows, device=device)
+    old, adv = f.clone(), f.clone()
+    old[-4:], adv[-4:] = c.old_t, c.adv_t
+    z.requires_grad_()
+    loss, lp = cl.policy_loss(z, a, old, adv, reduction="sum", return_log_probs=True)
+    _near(_np(lp[-4:]), c.lp, c.err, c.wide)
+    (g,) = torch.autograd.grad(loss, z)
+    term, slope = P.policy_terms(c.lp, c.actions, c.old, c.adv, c.ref, 0.2, 0.2, 0.0)
+    c.check_gradient(g[-4:], slope, 4 * np.abs(c.adv) * c.err)
+    assert not g[:-4].any()
+    del g, loss
+    lp = cl.selected_log_probs(z, a)
+    (g,) = torch.autograd.grad(lp, z, adv)
+    _near(_np(lp[-4:]), c.lp, c.err, c.wide)
+    c.check_gradient(g[-4:], c.adv)
+    assert not g[:-4].any()
