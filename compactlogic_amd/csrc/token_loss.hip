@@ -925,15 +925,18 @@ constexpr int64_t kHeldRow = 131072;
 constexpr int64_t kHeldLogits = int64_t(48) << 20;
 
 template <typename T>
+constexpr bool kPrefillType = std::is_same_v<T, float> || std::is_same_v<T, bf16_t>;
+
+template <typename T>
 bool policy_prefills(int64_t rows, int64_t cols) {
-    return (std::is_same_v<T, float> || std::is_same_v<T, bf16_t>) &&
-           cols * int64_t(sizeof(T)) <= kHeldRow && rows * cols * int64_t(sizeof(T)) >= kHeldLogits;
+    const int64_t bytes = cols * int64_t(sizeof(T));
+    return kPrefillType<T> && bytes <= kHeldRow && rows * bytes >= kHeldLogits;
 }
 
 // The rows' terms and, for an upstream gradient of 1, the logits' gradient.
 template <typename T, typename Op>
 int launch_rows_grad(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipStream_t s) {
-    if constexpr (std::is_same_v<T, float> || std::is_same_v<T, bf16_t>) {
+    if constexpr (kPrefillType<T>) {
         const int64_t bytes = a.cols * int64_t(sizeof(T));
         const unsigned grid = unsigned(a.rows);
         if (a.rows == 0) return CL_OK;
@@ -984,9 +987,13 @@ int launch_logit_grad(const RowArgs<T>& a, const Upstream<wide_t<T>>& up, void* 
     const int64_t bytes = a.cols * int64_t(sizeof(T));
     T* g = static_cast<T*>(grad);
     if (prefilled) {
-        const int64_t chunks = ceil_div(a.cols, kRowBlock * kGradVecs * wide_vec<T>());
-        k_grad_again<T><<<unsigned(std::min<int64_t>(a.rows * chunks, 1024)), kRowBlock, 0, s>>>(
-            a, up, g, uint32_t(chunks));
+        if constexpr (kPrefillType<T>) {
+            const int64_t chunks = ceil_div(a.cols, kRowBlock * kGradVecs * wide_vec<T>());
+            const int64_t grid = std::min<int64_t>(a.rows * chunks, 1024);
+            k_grad_again<T><<<unsigned(grid), kRowBlock, 0, s>>>(a, up, g, uint32_t(chunks));
+        } else {
+            CL_ARG(false, "the gradient of this type is not taken by the forward");
+        }
     } else if (bytes <= 256) {
         k_grad_short<T, 16, 1><<<unsigned(ceil_div(a.rows, kRowBlock / 16)), kRowBlock, 0, s>>>(
             a, up, g);

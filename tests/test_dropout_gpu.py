@@ -75,7 +75,7 @@ def test_mask_is_a_function_of_the_place(device):
     assert torch.equal(y, cl.dropout(ones.t().contiguous().t(), 0.5, SEED, 3, fill=0.0))
     assert torch.equal(y, cl.dropout(ones.bfloat16(), 0.5, SEED, 3, fill=0.0).float())
     assert torch.equal(y, cl.dropout(ones.view(60, 7, 1, 11), 0.5, SEED, 3, fill=0.0).view(60, 77))
-    last = ones.view(60, 7, 11).permute(1, 2, 0).contiguous().permute(2, 0, 1)   # feature-major
+    last = ones.view(60, 7, 11).permute(1, 2, 0).contiguous().permute(2, 0, 1)  # feature-major
     assert torch.equal(y, cl.dropout(last, 0.5, SEED, 3, fill=0.0).reshape(60, 77))
     odd = ones.view(60, 7, 11).transpose(1, 2)                                   # copied
     assert torch.equal(cl.dropout(odd, 0.5, SEED, 3, fill=0.0).reshape(60, 77), y)

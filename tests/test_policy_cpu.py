@@ -74,6 +74,14 @@ def test_c_arguments_are_checked_before_the_device():
     assert lib.cl_selected_log_prob_backward(0, 1, 8, 2, 8, 1, 1, None, 1, None) == bad
     assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 2, 1, None, 0, 1, None) == bad
     assert lib.cl_policy_loss_backward(0, 1, 8, 2, 8, 1, 1, 0, 1, None, 1, 1, None) == bad
+    assert lib.cl_policy_loss_backward(2, 1, 8, 2, 8, 1, 1, 2, 1, 1, 1, 1, None) == bad
+    assert b"type" in lib.cl_last_error()
+    yes = ctypes.c_int()
+    for dtype, rows, cols, want in [(0, 8192, 4096, 1), (3, 8192, 4096, 1), (2, 8192, 4096, 0),
+                                    (1, 8192, 4096, 0), (0, 128, 10, 0), (3, 4096, 65536, 1),
+                                    (3, 4096, 65537, 0), (0, 4096, 32768, 1), (0, 4096, 32769, 0)]:
+        assert lib.cl_policy_loss_prefills(dtype, rows, cols, ctypes.byref(yes)) == ok
+        assert yes.value == want, (dtype, rows, cols)
     assert lib.cl_preference_loss_backward(0, 1, 8, 2, 8, 1, 1, None, 1, 1, 2, 1, 1, 1, None) == bad
     assert lp(rows=0) == ok and lib.cl_last_error() == b""
 
