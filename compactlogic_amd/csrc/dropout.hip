@@ -109,7 +109,7 @@ struct Split<true> {
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kDropThreads) void k_dropout_rows(DropArgs<T> a, int64_t items,
                                                                Split<WIDE> split) {
-    const int64_t item = int64_t(blockIdx.x) * kDropThreads + threadIdx.x;
+    const int64_t item = group_index() * kDropThreads + threadIdx.x;
     if (item >= items) return;
     int64_t row, blk;
     split(item, row, blk);
@@ -139,7 +139,7 @@ template <typename T, bool WIDE>
 __global__ __launch_bounds__(kDropThreads) void k_dropout_cols(DropArgs<T> a, int64_t items,
                                                                Split<WIDE> split) {
     constexpr int R = wide_vec<T>();
-    const int64_t item = int64_t(blockIdx.x) * kDropThreads + threadIdx.x;
+    const int64_t item = group_index() * kDropThreads + threadIdx.x;
     if (item >= items) return;
     int64_t blk, rb;
     split(item, blk, rb);
@@ -191,15 +191,15 @@ int launch_dropout(const DropArgs<T>& a, bool by_rows, hipStream_t s) {
     if (items < (int64_t(1) << 31)) {
         const Split<false> split{make_fastdiv(uint32_t(d))};
         if (by_rows)
-            k_dropout_rows<T, false><<<unsigned(grid), kDropThreads, 0, s>>>(a, items, split);
+            k_dropout_rows<T, false><<<wide_grid(grid), kDropThreads, 0, s>>>(a, items, split);
         else
-            k_dropout_cols<T, false><<<unsigned(grid), kDropThreads, 0, s>>>(a, items, split);
+            k_dropout_cols<T, false><<<wide_grid(grid), kDropThreads, 0, s>>>(a, items, split);
     } else {
         const Split<true> split{d};
         if (by_rows)
-            k_dropout_rows<T, true><<<unsigned(grid), kDropThreads, 0, s>>>(a, items, split);
+            k_dropout_rows<T, true><<<wide_grid(grid), kDropThreads, 0, s>>>(a, items, split);
         else
-            k_dropout_cols<T, true><<<unsigned(grid), kDropThreads, 0, s>>>(a, items, split);
+            k_dropout_cols<T, true><<<wide_grid(grid), kDropThreads, 0, s>>>(a, items, split);
     }
     return check_launch("cl_dropout");
 }

@@ -11,6 +11,7 @@
 // and a plain strided variant for anything else.
 #include "common.h"
 #include "row_loss.h"
+#include "storage.h"
 
 #include <algorithm>
 
@@ -284,13 +285,14 @@ __global__ __launch_bounds__(256) void k_gsum_center(const T* __restrict__ part,
 
 // Any layout: a workgroup per sample, its waves taking the classes in turn.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gsum_center_any(const T* __restrict__ x, int64_t F,
-                                                         int64_t sb, int64_t sf, int64_t gsz,
-                                                         int64_t k, double tau,
+__global__ __launch_bounds__(256) void k_gsum_center_any(const T* __restrict__ x, int64_t B,
+                                                         int64_t F, int64_t sb, int64_t sf,
+                                                         int64_t gsz, int64_t k, double tau,
                                                          T* __restrict__ out) {
     extern __shared__ __align__(16) unsigned char center_lds[];
     double* z = reinterpret_cast<double*>(center_lds);  // [k]
-    const int64_t n = blockIdx.x;
+    const int64_t n = group_index();
+    if (n >= B) return;
     for (int64_t c = wave_id(); c < k; c += 4) {
         const int64_t j1 = std::min<int64_t>((c + 1) * gsz, F);
         double t = 0;
@@ -678,8 +680,8 @@ extern "C" int cl_group_sum_centered_forward(int dtype, const void* x, int64_t b
                                size_t(kCenterSamples * k * 8), s>>>(part, batch, int(k), slices, tau,
                                                                   os);
         } else {
-            k_gsum_center_any<T><<<unsigned(batch), 256, size_t(k * 8), s>>>(
-                xs, features, stride_batch, stride_feature, gsz, k, tau, os);
+            k_gsum_center_any<T><<<wide_grid(batch), 256, size_t(k * 8), s>>>(
+                xs, batch, features, stride_batch, stride_feature, gsz, k, tau, os);
         }
     });
     return check_launch("cl_group_sum_centered_forward");

@@ -44,6 +44,17 @@ using wide_t = typename WideType<T>::type;
         }                                                                                \
     } while (0)
 
+// Any number of workgroups below 2^31: a launch counts the threads of a grid dimension in 32 bits,
+// so what lies past 2^21 workgroups goes to the second one.  The last row of a grid may be partly
+// past the end.
+constexpr int64_t kGridRow = int64_t(1) << 21;
+
+inline dim3 wide_grid(int64_t groups) {
+    return dim3(unsigned(groups < kGridRow ? groups : kGridRow),
+                unsigned((groups + kGridRow - 1) / kGridRow));
+}
+__device__ __forceinline__ int64_t group_index() { return blockIdx.y * kGridRow + blockIdx.x; }
+
 // N elements moved in 16-byte accesses, at any address that is a multiple of the element size:
 // the hardware takes them off 16 bytes, so rows need no alignment of their own.
 template <typename T, int N>

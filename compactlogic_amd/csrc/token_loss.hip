@@ -215,10 +215,10 @@ __device__ __forceinline__ RowState<wide_t<T>> finish_row(const RowArgs<T>& a, c
     return st;
 }
 
-// The action as a place in the row, far before it where there is none.
-template <typename T>
-__device__ __forceinline__ int action_place(const RowArgs<T>& a, int64_t act) {
-    return act >= 0 && act < a.cols ? int(act) : INT32_MIN / 2;
+// The action as a place among the cols elements from j0 on, -1 where it is none of them.
+__device__ __forceinline__ int action_place(int64_t act, int64_t j0, int cols) {
+    const uint64_t place = uint64_t(act) - uint64_t(j0);
+    return place < uint64_t(cols) ? int(place) : -1;
 }
 
 template <typename T>
@@ -363,7 +363,7 @@ struct Held {
         const int owner = in >= 0 && in < body ? (in / VEC) % TPR
                           : in < 0             ? act
                                                : act - body;
-        if (act >= 0 && act < body + cut.loose && t == owner) g[act] = T(rg.own);
+        if (act >= 0 && t == owner) g[act] = T(rg.own);
     }
 
     static __device__ __forceinline__ void store_zero(T* g, int cols, int t, bool through) {
@@ -402,8 +402,7 @@ __device__ __forceinline__ void emit_grad(const RowArgs<T>& a, const GradOut<T>&
     if (c == wide_t<T>(0))
         row.store_zero(g, int(a.cols), t, a.through_store);
     else
-        row.store_grad(g, t, action_place(a, act), RowGrad<T>(st, c),
-                                     a.through_store);
+        row.store_grad(g, t, action_place(act, 0, int(a.cols)), RowGrad<T>(st, c), a.through_store);
 }
 
 // ---- short rows: TPR lanes (16 or 64) of a wave per row, several rows per workgroup, no LDS.  A
@@ -412,7 +411,7 @@ __device__ __forceinline__ void emit_grad(const RowArgs<T>& a, const GradOut<T>&
 template <typename T, int TPR, int NV, typename Op, bool GRAD>
 __global__ __launch_bounds__(kRowBlock) void k_rows_short(RowArgs<T> a, Op op, GradOut<T> out) {
     using A = wide_t<T>;
-    const int64_t n = int64_t(blockIdx.x) * (kRowBlock / TPR) + threadIdx.x / TPR;
+    const int64_t n = group_index() * (kRowBlock / TPR) + threadIdx.x / TPR;
     if (n >= a.rows) return;
     const int t = threadIdx.x % TPR;
     const int64_t act = a.actions[n];
@@ -439,7 +438,8 @@ __global__ __launch_bounds__(TPR, 8) void k_rows_held(RowArgs<T> a, Op op, GradO
     using A = wide_t<T>;
     __shared__ A part[TPR / 64][2];
     __shared__ RowState<A> shared;
-    const int64_t n = blockIdx.x;
+    const int64_t n = group_index();
+    if (n >= a.rows) return;
     const int t = threadIdx.x;
     const int64_t act = a.actions[n];
     Held<T, TPR, NV> row;
@@ -514,7 +514,8 @@ template <typename T, typename Op>
 __global__ __launch_bounds__(kRowBlock) void k_rows_stream(RowArgs<T> a, Op op) {
     using A = wide_t<T>;
     __shared__ A part[kRowBlock / 64][2];
-    const int64_t n = blockIdx.x;
+    const int64_t n = group_index();
+    if (n >= a.rows) return;
     const int64_t act = a.actions[n];
     A m = 0, s = 1, xa = 0;
     RowInputs in{};
@@ -580,7 +581,7 @@ template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(kRowBlock) void k_grad_short(RowArgs<T> a, Upstream<wide_t<T>> up,
                                                           T* __restrict__ grad) {
     using A = wide_t<T>;
-    const int64_t n = int64_t(blockIdx.x) * (kRowBlock / TPR) + threadIdx.x / TPR;
+    const int64_t n = group_index() * (kRowBlock / TPR) + threadIdx.x / TPR;
     if (n >= a.rows) return;
     const int t = threadIdx.x % TPR;
     const RowState<A> st = a.state[n];
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(kRowBlock) void k_grad_short(RowArgs<T> a, Upstream
         return;
     }
     row.load(a.x + n * a.stride, g, int(a.cols), t, a.through_load);
-    row.store_grad(g, t, action_place(a, act), RowGrad<T>(st, c), a.through_store);
+    row.store_grad(g, t, action_place(act, 0, int(a.cols)), RowGrad<T>(st, c), a.through_store);
 }
 
 constexpr int kGradVecs = 4;  // vectors per thread
@@ -615,14 +616,14 @@ __device__ __forceinline__ void grad_chunk(const RowArgs<T>& a, const Upstream<w
         return;
     }
     row.load(a.x + n * a.stride + j0, g, cols, threadIdx.x, a.through_load);
-    row.store_grad(g, threadIdx.x, action_place(a, act) - int(j0),
-                                       RowGrad<T>(st, c), a.through_store);
+    row.store_grad(g, threadIdx.x, action_place(act, j0, cols), RowGrad<T>(st, c), a.through_store);
 }
 
 template <typename T>
 __global__ __launch_bounds__(kRowBlock) void k_grad_long(RowArgs<T> a, Upstream<wide_t<T>> up,
                                                          T* __restrict__ grad, uint32_t chunks) {
-    grad_chunk<T>(a, up, grad, blockIdx.x / chunks, blockIdx.x % chunks);
+    const uint32_t i = uint32_t(group_index()), n = i / chunks;
+    if (n < a.rows) grad_chunk<T>(a, up, grad, n, i % chunks);
 }
 
 // A gradient that the forward left for an upstream gradient of 1: nothing to do where it is 1,
@@ -778,7 +779,7 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i, dou
 
 template <typename A>
 __global__ __launch_bounds__(kRowBlock) void k_pref_pairs(PairArgs<A> a) {
-    const int64_t i = int64_t(blockIdx.x) * (kRowBlock / 64) + wave_id();
+    const int64_t i = group_index() * (kRowBlock / 64) + wave_id();
     if (i < a.pairs) pair_term<64>(a, i, nullptr);
 }
 
@@ -899,7 +900,7 @@ int launch_sum(const A* terms, const int64_t* actions, int64_t rows, int64_t ign
 template <typename T, int TPR, int NV, bool GRAD, typename Op>
 void launch_rows_short(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipStream_t s) {
     k_rows_short<T, TPR, NV, Op, GRAD>
-        <<<unsigned(ceil_div(a.rows, kRowBlock / TPR)), kRowBlock, 0, s>>>(a, op, out);
+        <<<wide_grid(ceil_div(a.rows, kRowBlock / TPR)), kRowBlock, 0, s>>>(a, op, out);
 }
 
 template <bool GRAD, typename T, typename Op>
@@ -938,7 +939,7 @@ template <typename T, typename Op>
 int launch_rows_grad(const RowArgs<T>& a, const Op& op, const GradOut<T>& out, hipStream_t s) {
     if constexpr (kPrefillType<T>) {
         const int64_t bytes = a.cols * int64_t(sizeof(T));
-        const unsigned grid = unsigned(a.rows);
+        const dim3 grid = wide_grid(a.rows);
         if (a.rows == 0) return CL_OK;
         if (launch_short<true>(a, op, out, s)) {
         } else if (bytes <= 16384) {
@@ -975,7 +976,7 @@ int launch_rows(const RowArgs<T>& a, const Op& op, void* workspace, int64_t work
         k_rows_joined<T, Op><<<unsigned(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
             a, op, parts, ws);
     } else {
-        k_rows_stream<T, Op><<<unsigned(a.rows), kRowBlock, 0, s>>>(a, op);
+        k_rows_stream<T, Op><<<wide_grid(a.rows), kRowBlock, 0, s>>>(a, op);
     }
     return check_launch("rows");
 }
@@ -995,18 +996,18 @@ int launch_logit_grad(const RowArgs<T>& a, const Upstream<wide_t<T>>& up, void* 
             CL_ARG(false, "the gradient of this type is not taken by the forward");
         }
     } else if (bytes <= 256) {
-        k_grad_short<T, 16, 1><<<unsigned(ceil_div(a.rows, kRowBlock / 16)), kRowBlock, 0, s>>>(
+        k_grad_short<T, 16, 1><<<wide_grid(ceil_div(a.rows, kRowBlock / 16)), kRowBlock, 0, s>>>(
             a, up, g);
     } else if (bytes <= 1024) {
-        k_grad_short<T, 64, 1><<<unsigned(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
+        k_grad_short<T, 64, 1><<<wide_grid(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
             a, up, g);
     } else if (bytes <= 4096) {
-        k_grad_short<T, 64, 4><<<unsigned(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
+        k_grad_short<T, 64, 4><<<wide_grid(ceil_div(a.rows, kRowBlock / 64)), kRowBlock, 0, s>>>(
             a, up, g);
     } else {
         const int64_t chunks = ceil_div(a.cols, kRowBlock * kGradVecs * wide_vec<T>());
         CL_ARG(a.rows * chunks < (int64_t(1) << 31), "too many logits for one call");
-        k_grad_long<T><<<unsigned(a.rows * chunks), kRowBlock, 0, s>>>(a, up, g,
+        k_grad_long<T><<<wide_grid(a.rows * chunks), kRowBlock, 0, s>>>(a, up, g,
                                                                       uint32_t(chunks));
     }
     return check_launch("logit gradient");
@@ -1195,7 +1196,7 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
         if (longs)
             k_pref_long<A><<<unsigned(pairs), kSumThreads, 0, s>>>(pa);
         else if (pairs > 0)
-            k_pref_pairs<A><<<unsigned(ceil_div(pairs, kRowBlock / 64)), kRowBlock, 0, s>>>(pa);
+            k_pref_pairs<A><<<wide_grid(ceil_div(pairs, kRowBlock / 64)), kRowBlock, 0, s>>>(pa);
         if (int rc = check_launch("cl_preference_loss_forward(pairs)")) return rc;
         if (out) {
             const int64_t threads = std::min<int64_t>(kSumThreads, ceil_div(pairs, 64) * 64);

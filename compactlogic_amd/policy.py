@@ -223,7 +223,7 @@ class PolicyLossFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, actions, old, adv, ref, clip_low, clip_high, kl_coef, ignore_index,
-                reduction, group=None):
+                reduction, trains, group=None):
         logits = _logits_of(ctx, x, group)
         dtype, dev, wide = logits.dtype, logits.device, old.dtype
         code = _CODES[dtype]
@@ -237,7 +237,7 @@ class PolicyLossFunction(torch.autograd.Function):
         loss = torch.empty(() if reduction else rows, dtype=wide, device=dev)
         loss_at = loss.data_ptr()
         grad = None
-        if reduction and group is None and ctx.needs_input_grad[0] and _prefills(code, rows, cols):
+        if trains and reduction and group is None and _prefills(code, rows, cols):
             grad = torch.empty((rows, cols), dtype=dtype, device=dev)
             ctx.capture = _capture_id(logits)
         timing.launch(logits, "cl_policy_loss_forward", code, logits.data_ptr(), logits.stride(0),
@@ -255,7 +255,7 @@ class PolicyLossFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_loss, _grad_lp):
         if grad_loss is None:
-            return (None,) * 11
+            return (None,) * 12
         logits, actions, aux = _saved(ctx)
         if not grad_loss.is_contiguous():
             grad_loss = grad_loss.contiguous()
@@ -265,7 +265,7 @@ class PolicyLossFunction(torch.autograd.Function):
             gx = _group_grad(ctx, logits, actions, at, loss_grad=up,
                              count=at + ctx.count if reduction == _MEAN else None) if reduction \
                 else _group_grad(ctx, logits, actions, at, row_grad=up)
-            return gx, None, None, None, None, None, None, None, None, None, None
+            return gx, None, None, None, None, None, None, None, None, None, None, None
         rows, cols = logits.shape
         # the forward's gradient is handed out once, and only in the capture (or outside of any)
         # that it was written in: a replay of the backward alone would find it used
@@ -276,7 +276,7 @@ class PolicyLossFunction(torch.autograd.Function):
         timing.launch(logits, "cl_policy_loss_backward", _CODES[logits.dtype], logits.data_ptr(),
                       logits.stride(0), rows, cols, actions.data_ptr(), at, reduction,
                       grad_loss.data_ptr(), at + ctx.count, int(prefilled), grad.data_ptr())
-        return grad, None, None, None, None, None, None, None, None, None, None
+        return grad, None, None, None, None, None, None, None, None, None, None, None
 
 
 class PreferenceLossFunction(torch.autograd.Function):
@@ -375,8 +375,10 @@ def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, 
     ref = None
     if ref_log_probs is not None:
         ref = _per_row(ref_log_probs, "ref_log_probs", logits, actions)
+    # (needs_input_grad is true under no_grad as well)
+    trains = logits.requires_grad and torch.is_grad_enabled()
     loss, lp = PolicyLossFunction.apply(rows, acts, old, adv, ref, low, high, kl_coef,
-                                        int(ignore_index), code, _group)
+                                        int(ignore_index), code, trains, _group)
     if actions.dim() != 1:
         lp = lp.reshape(actions.shape)
         if not code:

@@ -246,3 +246,21 @@ def test_large_tensors(device, layout):
         words = D.philox(counter, np.array([SEED & 0xFFFFFFFF, SEED >> 32], dtype=np.uint64))
         halves = np.stack((words & 0xFFFF, words >> 16), -1).reshape(-1)[:cols]
         np.testing.assert_array_equal(y[r].float().cpu().numpy(), (halves >= 32768) * 1.0)
+
+
+def test_threads_past_32_bits(device):
+    """2^32 generator blocks and some (69 GB), a thread each: the first and last rows against the
+    oracle's counters."""
+    rows, cols = (1 << 20) + 1, 32768
+    x = torch.ones((1, cols), dtype=torch.bfloat16, device=device).expand(rows, cols)
+    y = cl.dropout(x, 0.5, SEED, OFFSET, fill=0.0)
+    counter = np.zeros((cols // 8, 4), dtype=np.uint64)
+    counter[:, 0] = np.arange(cols // 8)
+    counter[:, 2], counter[:, 3] = OFFSET & 0xFFFFFFFF, OFFSET >> 32
+    for r in (0, rows // 2, rows - 2, rows - 1):
+        counter[:, 1] = r
+        words = D.philox(counter, np.array([SEED & 0xFFFFFFFF, SEED >> 32], dtype=np.uint64))
+        halves = np.stack((words & 0xFFFF, words >> 16), -1).reshape(-1)
+        np.testing.assert_array_equal(y[r].float().cpu().numpy(), (halves >= 32768) * 1.0)
+    del y
+    torch.cuda.empty_cache()

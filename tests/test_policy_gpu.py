@@ -892,3 +892,101 @@ def test_more_than_2_to_32_logits(device):
     _near(_np(lp[-4:]), c.lp, c.err, c.wide)
     c.check_gradient(g[-4:], c.adv)
     assert not g[:-4].any()
+
+
+def test_threads_past_32_bits_short_rows(device):
+    """2^28 rows and some of two classes, 16 threads each, and half as many pairs."""
+    pairs, beta = (1 << 27) + 1, 0.5
+    rows = 2 * pairs
+    torch.manual_seed(0)
+    z = torch.randint(-8, 9, (rows, 2), device=device, dtype=torch.int8).to(torch.bfloat16)
+    a = torch.arange(rows, device=device) % 2
+    z.requires_grad_()
+    loss, h = cl.preference_loss(z, a, torch.arange(rows + 1, device=device), beta=beta,
+                                 reduction="sum", return_margins=True)
+    (g,) = torch.autograd.grad(loss, z)
+    with torch.no_grad():
+        d = (z[:, 0].double() - z[:, 1].double()) * (1 - 2 * a)   # chosen less other: -16 .. 16
+        lp = torch.nn.functional.logsigmoid(d)
+        want = beta * (lp[:pairs] - lp[pairs:])
+        err = (2 / 256 + 40 + 16) * 2.0**-24      # of lp (_sum_error)
+        assert ((h - want).abs() <= 2 * beta * err + want.abs() * 2.0**-24).all()
+        total = float(torch.nn.functional.softplus(-want).sum())
+        # per pair beta's two errors and a rounding of the term, 16 at most; the sum's rounding
+        assert abs(float(loss) - total) <= pairs * (2 * beta * err + 16 * 2.0**-24) \
+            + total * 2.0**-24
+        slope = -beta * torch.sigmoid(-want)
+        slope = torch.cat((slope, -slope))
+        own = slope * torch.sigmoid(-d)
+        # 1 - p_a is off by lp's error, the slope by a quarter of the margin's
+        off = beta * (err + 2 * beta * err / 4 + 4 * 2.0**-24)
+        mine = g.gather(1, a[:, None])[:, 0].double()
+        other = g.gather(1, 1 - a[:, None])[:, 0].double()
+        assert ((mine - own).abs() <= off + own.abs() * 2.0**-8).all()
+        assert ((other + own).abs() <= off + own.abs() * 2.0**-8).all()
+
+
+def test_threads_past_32_bits_long_rows(device):
+    """2^24 rows and some, a workgroup each: the same row of 2050 classes over and over, counted
+    at both ends; the gradient (69 GB) in a pass of its own and out of the forward."""
+    rows, vocab = (1 << 24) + 3, 2050
+    c = Case(6, vocab, torch.bfloat16, device, ignored=0.0, seed=3)
+    row = c.logits[0].clone()
+    one = np.repeat(_np(row)[None], 6, axis=0)
+    lp, probs = P.log_probs(one, c.actions)
+    at = torch.tensor([0, 1, 2, rows - 3, rows - 2, rows - 1], device=device)
+    a = torch.full((rows,), IGNORE, device=device)
+    a[at] = c.act_t
+    up = torch.zeros(rows, device=device)
+    up[at] = torch.tensor([1.0, -0.5, 2.0, 0.25, -1.0, 3.0], device=device)
+    z = row.expand(rows, vocab).requires_grad_()
+    err = _sum_error(one, torch.float32)
+
+    def check(got, g):
+        _near(_np(got[at]), lp, err, torch.float32)
+        slope = _np(up[at])
+        own = P.logit_gradient(probs, c.actions, slope)
+        # the probabilities' error, both lps' in the ratio, and the exponential's 2^-20
+        _near(_np(g[at]), own, np.abs(slope)[:, None] * (3 * err + 2.0**-18), torch.bfloat16)
+        assert not got[3:-3].any() and not g[3:-3].any()
+
+    got = cl.selected_log_probs(z, a)
+    (g,) = torch.autograd.grad(got, z, up)
+    check(got.detach(), g)
+    del g
+    # ratios of exactly 1 in fp64 are not to be had: inside the range the slope is -A r
+    old = torch.zeros(rows, device=device)
+    old[at] = got.detach()[at]
+    assert policy._prefills(3, rows, vocab)
+    loss, got = cl.policy_loss(z, a, old, -up, reduction="sum", return_log_probs=True)
+    (g,) = torch.autograd.grad(loss, z)
+    check(got, g)
+    del g
+    torch.cuda.empty_cache()
+
+
+def test_group_sum_threads_past_32_bits(device):
+    """2^24 samples and some, a workgroup each."""
+    rows, k = (1 << 24) + 3, 4
+    torch.manual_seed(1)
+    x = torch.rand((rows, 8), device=device)
+    a = torch.arange(rows, device=device) % k
+    lp = cl.GroupSum(k, tau=0.25).log_probs(x, a)
+    z = x.double().view(rows, k, 2).sum(-1) / 0.25
+    want = torch.log_softmax(z, -1).gather(1, a[:, None])[:, 0]
+    assert ((lp - want).abs() <= (k / 256 + 40 + 8) * 2.0**-24 + want.abs() * 2.0**-24).all()
+
+
+def test_no_gradient_is_formed_where_none_is_recorded(device):
+    z = torch.randn((8192, 4096), device=device, dtype=torch.bfloat16).requires_grad_()
+    a = torch.zeros(8192, dtype=torch.int64, device=device)
+    f = torch.zeros(8192, device=device)
+    assert policy._prefills(3, 8192, 4096)
+    with torch.no_grad():
+        want = cl.policy_loss(z, a, f, f + 1)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        got = cl.policy_loss(z, a, f, f + 1)
+    assert torch.cuda.max_memory_allocated() - before < z.nbytes // 8
+    assert torch.equal(got, want)
