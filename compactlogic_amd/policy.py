@@ -361,7 +361,11 @@ def policy_loss(logits, actions, old_log_probs, advantages, ref_log_probs=None, 
     (a frozen reference policy's, needed when kl_coef is not 0) [...].  clip: one number for both
     sides or a pair (low, high).  reduction: 'mean' over the rows that count, 'sum', or 'none' (the
     terms, [...]).  With return_log_probs, also the rows' log-probabilities (not differentiable
-    through this call)."""
+    through this call).
+
+    Large float32 and bfloat16 logits get their gradient along with a scalar loss, as it is for
+    loss.backward().  A scaled loss (divided by a number of accumulated batches) forms it again;
+    scaling advantages and kl_coef instead, in which the loss is linear, saves that."""
     rows, acts = _flat(logits, actions)
     low, high = (clip, clip) if isinstance(clip, (int, float)) else clip
     low, high, kl_coef = float(low), float(high), float(kl_coef)
