@@ -6,11 +6,11 @@ ConvLayerCudaFunction, plus the packed-bit inference API (PackBitsTensor), and t
 conv blocks of the third-party ConvLogic package (ConvLogicLayer, TreeLogicLayer,
 PoolLogicLayer).  Beside the reference's modules: losses for training by reward or preference
 (policy.py), dropout between logic layers (dropout_layer.py), a fused optimizer step (optim.py).
-All numerics run in libcompactlogic_hip.so, built in-tree by
-``python -m compactlogic_amd.build``.
+All numerics run in libcompactlogic_hip.so, built in-tree (with the C++ autograd Functions of the
+losses and of dropout, csrc/autograd.cpp) by ``python -m compactlogic_amd.build``.
 """
 from . import checkpoint, circuit, convlogic_hip, difflogic_hip
-from .dropout_layer import Dropout, DropoutFunction, dropout
+from .dropout_layer import Dropout, dropout
 from .layers import (ConvLayer, ConvLayerCudaFunction, ConvLayerSoftmaxFunction,
                      ConvLayerWindowFunction, GroupSum, GroupSumCrossEntropyFunction,
                      GroupSumFunction, LogicGroupSumCrossEntropyFunction, LogicLayer,
@@ -19,8 +19,7 @@ from .layers import (ConvLayer, ConvLayerCudaFunction, ConvLayerSoftmaxFunction,
 from .optim import FusedAdam
 from .packed_net import PackedNetwork
 from .plan import RunPlan, build_run_plan
-from .policy import (PolicyLossFunction, PreferenceLossFunction, SelectedLogProbsFunction,
-                     policy_loss, preference_loss, selected_log_probs)
+from .policy import policy_loss, preference_loss, selected_log_probs
 from .schedules import (EntropyRowResampler, FixedSequentialEntropyFreezer,
                         SequentialEntropyFreezer)
 from .treelogic import (ConvLogicFunction, ConvLogicLayer, FullConvLogicFunction,
@@ -34,7 +33,6 @@ __all__ = [
     "EntropyRowResampler", "PackedNetwork", "ConvLogicLayer", "TreeLogicLayer", "PoolLogicLayer",
     "ConvLogicFunction", "FullConvLogicFunction", "TreeLogicFunction", "FusedAdam",
     "LogicGroupSumCrossEntropyFunction", "logic_group_sum_cross_entropy",
-    "sequential_cross_entropy", "checkpoint", "circuit", "Dropout", "DropoutFunction", "dropout",
-    "PolicyLossFunction", "PreferenceLossFunction", "SelectedLogProbsFunction", "policy_loss",
-    "preference_loss", "selected_log_probs",
+    "sequential_cross_entropy", "checkpoint", "circuit", "Dropout", "dropout",
+    "policy_loss", "preference_loss", "selected_log_probs",
 ]

@@ -10,51 +10,9 @@ from __future__ import annotations
 
 import torch
 
+from . import _native
 from . import difflogic_hip as _dl
-from . import timing
 from .layers import PackBitsTensor
-
-
-def _apply(x, code, threshold, rescale, fill, seed, offset, rng):
-    """cl_dropout of a 2-D tensor, the result lying as the tensor does."""
-    rows, cols = x.shape
-    sr, sc = x.stride()
-    if not (sc == 1 or cols == 1 or sr == 1 or rows == 1):
-        x = x.contiguous()
-        sr, sc = x.stride()
-    if sc == 1 or cols == 1:
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        yr, yc = cols, 1
-    else:
-        y = torch.empty_strided((rows, cols), (1, rows), dtype=x.dtype, device=x.device)
-        yr, yc = 1, rows
-    timing.launch(x, "cl_dropout", code, x.data_ptr(), sr, sc, y.data_ptr(), yr, yc, rows, cols,
-                  threshold, rescale, fill, seed, offset, None if rng is None else rng.data_ptr())
-    return y
-
-
-class DropoutFunction(torch.autograd.Function):
-    """Dropout of a 2-D tensor; the gradient passes the same mask, made again from the seed (and is
-    itself a dropout, so it can be differentiated as often as one likes)."""
-
-    @staticmethod
-    def forward(ctx, x, threshold, fill, seed, offset, rng):
-        code = _dl.storage_dtype_code(x)
-        ctx.save_for_backward(rng)
-        ctx.args = code, threshold, int(fill is None), 0.0, seed, offset
-        return _apply(x, code, threshold, int(fill is None), 0.0 if fill is None else fill, seed,
-                      offset, rng)
-
-    @staticmethod
-    def backward(ctx, grad):
-        (rng,) = ctx.saved_tensors
-        if torch.is_grad_enabled():
-            _, threshold, rescale, _, seed, offset = ctx.args
-            grad = DropoutFunction.apply(grad, threshold, None if rescale else 0.0, seed, offset,
-                                         rng)
-        else:
-            grad = _apply(grad, *ctx.args, rng)
-        return grad, None, None, None, None, None
 
 
 def _threshold(p) -> int:
@@ -92,8 +50,8 @@ def dropout(x, p: float, seed, offset: int = 0, fill: float | None = None):
     if threshold == 0 or x.numel() == 0:
         return x
     flat = x if x.dim() == 2 else x.reshape(x.shape[0] if x.dim() > 2 else 1, -1)
-    y = DropoutFunction.apply(flat, threshold, None if fill is None else float(fill),
-                              int(seed) & (2**64 - 1), int(offset) & (2**64 - 1), rng)
+    y = _native.load().dropout(flat, threshold, None if fill is None else float(fill),
+                               int(seed) & (2**64 - 1), int(offset) & (2**64 - 1), rng)
     return y if x.dim() == 2 else y.reshape(x.shape)
 
 
@@ -118,9 +76,7 @@ class Dropout(torch.nn.Module):
     def next_rng(self) -> torch.Tensor:
         """The (seed, offset) of the next mask, as `dropout` takes it; advances the module."""
         _dl._check(self.rng, "rng")
-        used = torch.empty_like(self.rng)
-        timing.launch(used, "cl_dropout_next", self.rng.data_ptr(), used.data_ptr())
-        return used
+        return _native.load().dropout_next(self.rng)
 
     def forward(self, x):
         if not self.training or isinstance(x, PackBitsTensor) or _threshold(self.p) == 0:

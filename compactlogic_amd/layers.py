@@ -1427,8 +1427,9 @@ class GroupSum(torch.nn.Module):
         if x.dtype == torch.float16:
             x = x.float()
         if not _policy.takes_group(self.k):
-            return self(x), None
-        return x, (self.k, float(self.tau))
+            return self(x), _policy._NO_GROUP
+        _dl.dtype_code(x)
+        return x, (int(self.k), float(self.tau))
 
     def log_probs(self, x, actions, ignore_index: int = -100):
         """policy.selected_log_probs(self(x), actions) in one op: the log-probability of the chosen

@@ -23,6 +23,7 @@ import torch
 from . import _capi
 
 _active = None
+_native = None   # the autograd extension, which calls `timed` itself while a recorder is active
 
 # Spin of the settle kernel in microseconds (converted to clock cycles on first use).
 SETTLE_US = 60.0
@@ -69,25 +70,24 @@ def record(settle: bool = True, repeat: dict | None = None):
     before the call, so that a repeat overwrites the same outputs with the same values)."""
     global _active
     prev, _active = _active, Recorder(settle, repeat)
+    _tell()
     try:
         yield _active
     finally:
         _active = prev
+        _tell()
 
 
-def launch(t: torch.Tensor, name: str, *args) -> None:
-    """Entry point `name` with `args` and the current stream of t's device, on that device: what
-    _capi.call inside of torch.cuda.device and `timed` does, for calls whose kernels are shorter
-    than a closure and two context managers."""
-    index = t.get_device()
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if index != torch._C._cuda_getDevice():
-        with torch.cuda.device(index):
-            timed(name, lambda: _capi.call(name, *args, stream))
-    elif _active is not None:
-        timed(name, lambda: _capi.call(name, *args, stream))
-    else:
-        _capi.call(name, *args, stream)
+def attach(native) -> None:
+    """Let the autograd extension's calls be timed too."""
+    global _native
+    _native = native
+    _tell()
+
+
+def _tell() -> None:
+    if _native is not None:
+        _native.set_timed(timed if _active is not None else None)
 
 
 def timed(name: str, fn, stream=None):

@@ -1,11 +1,14 @@
 """Losses on chosen log-probabilities against the float64 oracle: values and gradients over types,
 lengths, strides, masks, ragged sequences; graphs, streams, refusals."""
+import concurrent.futures
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import compactlogic_amd as cl
-from compactlogic_amd import policy
+from compactlogic_amd import _capi, policy, timing
 from oracle import policy_np as P
 
 pytestmark = pytest.mark.gpu
@@ -550,6 +553,19 @@ def test_group_sum_methods(device, batch, feats, k, layout, dtype):
     check(torch.autograd.grad(loss, x)[0], slope, 0.3 * 0.6 * err + 0.3 * 4 * unit)
 
 
+def _centred_scores(x, k, tau):
+    code = 0 if x.dtype == torch.float32 else 1
+    need = ctypes.c_int64()
+    _capi.call("cl_group_sum_centered_workspace_size", code, *x.shape, x.stride(0), k,
+               ctypes.byref(need))
+    ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device=x.device)
+    out = torch.empty((x.shape[0], k), dtype=x.dtype, device=x.device)
+    _capi.call("cl_group_sum_centered_forward", code, x.data_ptr(), *x.shape, *x.stride(), k, tau,
+               out.data_ptr(), ws.data_ptr(), need.value,
+               torch.cuda.current_stream(x.device).cuda_stream)
+    return out
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
 def test_group_sum_gradient_is_that_of_the_scores(device, dtype, reduction):
@@ -567,10 +583,7 @@ def test_group_sum_gradient_is_that_of_the_scores(device, dtype, reduction):
     for x in (base.clone(), base.t().contiguous().t(), base[:, :1200:1].clone()):
         x.requires_grad_()
         seen = []
-
-        class Spy:
-            group = None
-        scores = policy._logits_of(Spy(), x.detach(), (k, tau)).requires_grad_()
+        scores = _centred_scores(x, k, tau).requires_grad_()
         up = torch.randn(batch if reduction == "none" else (), generator=g,
                          dtype=torch.float64).to(dtype).to(device)
         seen.append((gs.policy_loss(x, a, old, adv, ref, kl_coef=0.1, reduction=reduction),
@@ -990,3 +1003,56 @@ def test_no_gradient_is_formed_where_none_is_recorded(device):
         got = cl.policy_loss(z, a, f, f + 1)
     assert torch.cuda.max_memory_allocated() - before < z.nbytes // 8
     assert torch.equal(got, want)
+
+
+def test_calls_are_timed(device):
+    """A recorder sees the forward's calls and those of the backward's thread, and their results
+    are the untimed ones."""
+    z = torch.randn((64, 10), device=device, requires_grad=True)
+    a = torch.zeros(64, dtype=torch.int64, device=device)
+    x = torch.rand((64, 100), device=device, requires_grad=True)
+    off = torch.tensor([0, 30, 64], device=device)
+    drop = cl.Dropout(0.5, seed=1).to(device)
+
+    def step():
+        lp = cl.selected_log_probs(z, a)
+        g = torch.autograd.grad(lp.sum() + cl.policy_loss(z, a, lp.detach(), lp.detach()), z)[0]
+        loss = cl.GroupSum(10).preference_loss(x, a, off, reduction="sum")
+        return g, torch.autograd.grad(loss, x)[0]
+
+    want = step()
+    with timing.record() as rec:
+        got = step()
+        drop(x)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    names = {"cl_selected_log_prob_forward", "cl_selected_log_prob_backward",
+             "cl_policy_loss_forward", "cl_policy_loss_backward", "cl_group_sum_centered_forward",
+             "cl_preference_loss_forward", "cl_group_sum_chosen_backward", "cl_dropout_next",
+             "cl_dropout"}
+    calls = rec.summary()
+    assert set(calls) == names and all(v["calls"] == 1 for v in calls.values())
+    step()
+    assert rec.summary() == calls
+
+
+def test_threads(device):
+    """Two threads, a stream each, call at once."""
+    cases = [Case(64, 1000, torch.float32, device, seed=s) for s in (0, 1)]
+    torch.cuda.synchronize()
+
+    def step(c):
+        z = c.logits.detach().requires_grad_()
+        loss = cl.policy_loss(z, c.act_t, c.old_t, c.adv_t, c.ref_t, kl_coef=0.1)
+        return torch.cat((loss.detach()[None], torch.autograd.grad(loss, z)[0].flatten()))
+
+    want = [step(c) for c in cases]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [step(cases[i]) for _ in range(50)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(g, want[i]) for g in got)
+
+    with concurrent.futures.ThreadPoolExecutor(2) as ex:
+        assert all(ex.map(work, (0, 1)))
