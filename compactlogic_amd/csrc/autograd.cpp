@@ -2,10 +2,10 @@
 // allocate, launch and save, and their backwards, over the entry points of
 // libcompactlogic_hip.so.
 //
-// A small call's kernels take 5 to 15 us.  As Functions in Python these calls took 75 to 95 us:
-// autograd runs a backward on a thread of its own, and two interpreters' turns on two cores cost
-// 30 us beside the hand-over itself (about 40 us for any operator of torch's own).  Arguments are
-// checked in policy.py and dropout_layer.py; nothing here is a public interface.
+// A small call's kernels take 6 to 15 us.  As Functions in Python such calls took 76 to 97 us, here
+// 45 to 62: autograd runs a backward on a thread of its own, and an interpreter on either side of
+// that hand-over costs 30 us more (torch's own negation, forward and backward, takes 45).
+// Arguments are checked in policy.py and dropout_layer.py; nothing here is a public interface.
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
