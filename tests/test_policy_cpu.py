@@ -1,13 +1,15 @@
 """What the losses on chosen log-probabilities refuse without a device, and their oracle against
 differences."""
 import ctypes
+import sys
+import types
 
 import numpy as np
 import pytest
 import torch
 
 import compactlogic_amd as cl
-from compactlogic_amd import _capi
+from compactlogic_amd import _capi, _native
 from oracle import policy_np as P
 
 
@@ -121,3 +123,21 @@ def test_oracle_gradients_against_differences():
     slope = P.preference_terms(lp, actions, offsets, ref, 0.7, 0.1)[2]
     np.testing.assert_allclose(P.logit_gradient(probs, actions, slope), _difference(preference, z),
                                atol=1e-8)
+
+
+def test_autograd_extension(monkeypatch):
+    """Built, and refused where it is missing or of another torch."""
+    built = _native.load()
+    assert {"selected_log_probs", "policy_loss", "preference_loss", "dropout",
+            "dropout_next"} <= set(dir(built))
+    assert _native.load() is built
+    monkeypatch.setattr(_native, "_module", None)
+    monkeypatch.delattr(cl, "_autograd")
+    monkeypatch.setitem(sys.modules, "compactlogic_amd._autograd", None)
+    with pytest.raises(_capi.CompactLogicError, match="compactlogic_amd.build"):
+        _native.load()
+    other = types.SimpleNamespace(torch_version="0.0.1")
+    monkeypatch.setattr(cl, "_autograd", other, raising=False)
+    monkeypatch.setitem(sys.modules, "compactlogic_amd._autograd", other)
+    with pytest.raises(_capi.CompactLogicError, match="torch 0.0.1"):
+        _native.load()

@@ -6,6 +6,7 @@ import ctypes
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import compactlogic_amd as cl
 from compactlogic_amd import _capi, policy, timing
@@ -1056,3 +1057,35 @@ def test_threads(device):
 
     with concurrent.futures.ThreadPoolExecutor(2) as ex:
         assert all(ex.map(work, (0, 1)))
+
+
+def test_checkpointed_and_inference(device):
+    """The losses inside of a recomputed segment, and where nothing is recorded."""
+    c = Case(48, 1000, torch.float32, device)
+    z = c.logits.requires_grad_()
+    off = torch.tensor([0, 20, 48], device=device)
+
+    def both(x):
+        x = x * 1.0
+        return cl.policy_loss(x, c.act_t, c.old_t, c.adv_t, c.ref_t, kl_coef=0.1) \
+            + cl.preference_loss(x, c.act_t, off, c.ref_t) \
+            + cl.selected_log_probs(x, c.act_t).sum() \
+            + cl.dropout(x, 0.5, 7).sum()
+
+    want = both(z)
+    (g,) = torch.autograd.grad(want, z)
+    for reentrant in (False, True):
+        got = torch.utils.checkpoint.checkpoint(both, z, use_reentrant=reentrant)
+        assert torch.equal(got, want)
+        if reentrant:
+            z.grad = None
+            got.backward()
+            assert torch.equal(z.grad, g)
+        else:
+            assert torch.equal(torch.autograd.grad(got, z)[0], g)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            got = both(z)
+        assert torch.equal(got, want) and not got.requires_grad
+    with pytest.raises(RuntimeError):
+        torch.func.grad(both)(z.detach())
