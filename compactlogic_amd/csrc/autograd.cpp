@@ -15,6 +15,7 @@
 #include <utility>
 
 #include "../../include/compactlogic_hip.h"
+#include "timed_hook.h"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -33,19 +34,15 @@ struct Failure : std::runtime_error {
           status(rc) {}
 };
 
-// timing.timed while a recorder is active, else null.
-PyObject* g_timed = nullptr;
+cl::TimedHook g_timed;
 
 // One entry point on the current stream of the current device.
 template <typename F>
 void launch(const char* name, int device, F&& f) {
     void* stream = c10::hip::getCurrentHIPStream(c10::DeviceIndex(device)).stream();
-    auto call = [&] {
+    g_timed.run(name, [&] {
         if (const int rc = f(stream)) throw Failure(name, rc);
-    };
-    if (!g_timed) return call();
-    py::gil_scoped_acquire gil;
-    py::reinterpret_borrow<py::object>(g_timed)(name, py::cpp_function(call));
+    });
 }
 
 int code_of(const Tensor& t) {
@@ -511,10 +508,7 @@ Tensor dropout_next(const Tensor& rng) {
     return used;
 }
 
-void set_timed(py::object timed) {
-    Py_XDECREF(g_timed);
-    g_timed = timed.is_none() ? nullptr : timed.release().ptr();
-}
+void set_timed(py::object timed) { g_timed.set(std::move(timed)); }
 
 }  // namespace
 
