@@ -60,7 +60,11 @@ class Dropout(torch.nn.Module):
     next mask (its buffer `rng` holds the seed and the count of calls, on the device, so a
     captured training step draws a new mask at every replay and a checkpoint resumes the
     sequence); in eval mode, and for a PackBitsTensor, the identity.  seed=None takes one from
-    torch's generator."""
+    torch's generator.
+
+    A segment that torch.utils.checkpoint runs again in the backward would draw another mask
+    there, which is refused: take the mask before the segment and call the function in it,
+    ``rng = drop.next_rng()`` and ``dropout(h, drop.p, rng, fill=drop.fill)``."""
 
     def __init__(self, p: float = 0.5, fill: float | None = None, seed: int | None = None):
         super().__init__()
@@ -75,6 +79,11 @@ class Dropout(torch.nn.Module):
 
     def next_rng(self) -> torch.Tensor:
         """The (seed, offset) of the next mask, as `dropout` takes it; advances the module."""
+        if torch._C._current_graph_task_id() != -1:    # inside of a backward pass
+            raise RuntimeError(
+                "a Dropout module cannot draw its mask again in a backward pass, where "
+                "torch.utils.checkpoint recomputes a segment: take rng = next_rng() before the "
+                "segment and call dropout(x, p, rng, fill) in it")
         _dl._check(self.rng, "rng")
         return _native.load().dropout_next(self.rng)
 

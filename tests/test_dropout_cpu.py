@@ -2,9 +2,10 @@
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import compactlogic_amd as cl
-from compactlogic_amd import _capi
+from compactlogic_amd import _capi, dropout_layer
 from oracle import dropout_np as D
 
 
@@ -70,3 +71,47 @@ def test_c_arguments_are_checked_before_the_device():
     assert rc(rows=2**31, cols=2**31, xs=(2**31, 1), ys=(2**31, 1)) == bad
     assert lib.cl_dropout_next(None, None, None) == bad
     assert rc(rows=0) == _capi.CL_OK and lib.cl_last_error() == b""
+
+
+@pytest.fixture
+def plain_dropout(monkeypatch):
+    """The module on CPU tensors: the oracle's masks, and the count of calls kept on the CPU."""
+    def next_mask(rng):
+        used = rng.clone()
+        rng[1] += 1
+        return used
+
+    def dropout(x, p, rng, fill=None):
+        keep = torch.as_tensor(D.keep_mask(*x.shape, p, *(int(v) for v in rng)))
+        return torch.where(keep, x, 0.0)
+
+    native = type("Native", (), {"dropout_next": staticmethod(next_mask)})
+    monkeypatch.setattr(dropout_layer._native, "load", lambda: native)
+    monkeypatch.setattr(dropout_layer._dl, "_check", lambda t, name: None)
+    monkeypatch.setattr(dropout_layer, "dropout", dropout)
+    return dropout
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_module_refuses_to_draw_again_in_a_backward(plain_dropout, reentrant):
+    """A recomputed segment would drop other elements than the loss saw.  With the mask taken
+    before the segment the gradient is that of the mask."""
+    x = torch.rand(20, 30, generator=torch.Generator().manual_seed(0)).requires_grad_()
+    drop = cl.Dropout(0.5, seed=3)
+    y = torch.utils.checkpoint.checkpoint(lambda h: drop(h * h).sum(), x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="next_rng"):
+        y.backward()
+    assert int(drop.rng[1]) == 1
+
+    rng = drop.next_rng()
+    y = torch.utils.checkpoint.checkpoint(lambda h: plain_dropout(h * h, drop.p, rng).sum(), x,
+                                          use_reentrant=reentrant)
+    y.backward()
+    keep = torch.as_tensor(D.keep_mask(20, 30, 0.5, 3, 1))
+    assert torch.equal(x.grad, torch.where(keep, 2 * x.detach(), 0.0))
+    assert int(drop.rng[1]) == 2
+    drop.eval()                                      # the identity may be run again
+    x.grad = None
+    torch.utils.checkpoint.checkpoint(lambda h: drop(h * h).sum(), x,
+                                      use_reentrant=reentrant).backward()
+    assert torch.equal(x.grad, 2 * x.detach())

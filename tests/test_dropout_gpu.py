@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import compactlogic_amd as cl
 from oracle import dropout_np as D
@@ -264,3 +265,31 @@ def test_threads_past_32_bits(device):
         np.testing.assert_array_equal(y[r].float().cpu().numpy(), (halves >= 32768) * 1.0)
     del y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_module_in_a_recomputed_segment(device, reentrant):
+    """The module would draw another mask there and is refused; a mask taken before the segment
+    gives what the segment gives without recomputation."""
+    x = torch.rand(33, 70, device=device, requires_grad=True)
+    drop = cl.Dropout(0.5, seed=3).to(device)
+
+    def segment(h):
+        return drop(h * h).sum()
+
+    y = torch.utils.checkpoint.checkpoint(segment, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="next_rng"):
+        y.backward()
+    assert drop.rng.tolist() == [3, 1]
+
+    rng = drop.next_rng()
+
+    def masked(h):
+        return cl.dropout(h * h, drop.p, rng, fill=drop.fill).sum()
+
+    (want,) = torch.autograd.grad(masked(x), x)
+    x.grad = None
+    torch.utils.checkpoint.checkpoint(masked, x, use_reentrant=reentrant).backward()
+    assert torch.equal(x.grad, want) and drop.rng.tolist() == [3, 2]
+    keep = D.keep_mask(33, 70, 0.5, 3, 1)
+    assert np.array_equal(want.cpu().numpy() != 0, keep & (x.detach().cpu().numpy() != 0))
