@@ -62,15 +62,16 @@ __global__ __launch_bounds__(kSplitWaves * 64) void k_gsum_fwd_bc(const T* __res
 // ---- forward, batch-contiguous, split: block = (batch tile, class c, slice s of the
 // group).  Each block writes the partial sum of its slice; k_gsum_finish adds the slices in
 // slice order.  Used when a workspace is given, so that enough blocks fill the GPU.
+// P: the type of the additions and the partial sums (fp64 for the centred scores below).
 constexpr int kPartWaves = 4;
 
-template <typename T, int VEC>
+template <typename T, int VEC, typename P = T>
 __global__ __launch_bounds__(kPartWaves * 64) void k_gsum_partial(const T* __restrict__ x,
                                                                  int64_t B, int64_t F,
                                                                  int64_t sf, int64_t gsz,
                                                                  int64_t k, int64_t slice,
-                                                                 T* __restrict__ part) {
-    __shared__ T red[kPartWaves][64 * VEC];
+                                                                 P* __restrict__ part) {
+    __shared__ P red[kPartWaves][64 * VEC];
     const int wv = threadIdx.x >> 6;
     const int lane = threadIdx.x & 63;
     const int64_t c = blockIdx.y, sidx = blockIdx.z;
@@ -78,9 +79,9 @@ __global__ __launch_bounds__(kPartWaves * 64) void k_gsum_partial(const T* __res
     const int64_t g_end = std::min<int64_t>((c + 1) * gsz, F);
     const int64_t j0 = c * gsz + sidx * slice;
     const int64_t j1 = std::min<int64_t>(j0 + slice, g_end);
-    Vec<T, VEC> acc;
+    P acc[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) acc.v[i] = T(0);
+    for (int i = 0; i < VEC; ++i) acc[i] = P(0);
     if (n0 < B) {
         // the wave's rows eight at a time: the loads are issued together, the additions stay
         // in row order
@@ -92,22 +93,22 @@ __global__ __launch_bounds__(kPartWaves * 64) void k_gsum_partial(const T* __res
 #pragma unroll
             for (int r = 0; r < 8; ++r)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc.v[i] += v[r].v[i];
+                for (int i = 0; i < VEC; ++i) acc[i] += P(v[r].v[i]);
         }
         for (; j < j1; j += kPartWaves) {
             const Vec<T, VEC> v = vload<T, VEC>(x + j * sf + n0);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) acc.v[i] += v.v[i];
+            for (int i = 0; i < VEC; ++i) acc[i] += P(v.v[i]);
         }
     }
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) red[wv][lane * VEC + i] = acc.v[i];
+    for (int i = 0; i < VEC; ++i) red[wv][lane * VEC + i] = acc[i];
     __syncthreads();
-    T* dst = part + (sidx * k + c) * B;
+    P* dst = part + (sidx * k + c) * B;
     for (int e = threadIdx.x; e < 64 * VEC; e += kPartWaves * 64) {
         const int64_t n = int64_t(blockIdx.x) * 64 * VEC + e;
         if (n < B) {
-            T t = red[0][e];
+            P t = red[0][e];
 #pragma unroll
             for (int w = 1; w < kPartWaves; ++w) t += red[w][e];
             dst[n] = t;
@@ -224,10 +225,13 @@ struct CrossEntropyGrad {
 
 // ---- scores less the sample's largest one, out[n, c] = z[n, c] - max z[n], for losses that only
 // depend on such differences.  A class sum of 1200 activations is near 600, where fp32 steps are
-// 6e-5 wide: rounded there, as k_gsum_finish rounds it, a softmax is off by some 1e-5.  The slices
-// are therefore added, divided and subtracted in fp64 and rounded once, at the size of the
-// difference.  k_gsum_center: workgroup of kCenterSamples samples, their scores in LDS; it is bound
-// by the loads of the slices, as the finish (1024 samples, 26 slices of 10 classes: 1.1 MB).
+// 6e-5 wide: rounded there, as k_gsum_finish rounds it, a softmax is off by some 1e-5 or more.
+// Activations are therefore added, divided and subtracted in fp64 and rounded once, at the size of
+// the difference: log-probabilities over 10 classes are off by at most 4e-6 at 12000 activations and
+// 6e-6 at 200000, in either layout (with the slices added in fp32 2.7e-5 and 7.2e-4), and
+// k_gsum_partial, bound by its loads, takes 9.7 us for 1024 x 12000 either way.
+// k_gsum_center: workgroup of kCenterSamples samples, their scores in LDS; it is bound by the loads
+// of the slices, as the finish (1024 samples, 26 slices of 10 classes: 2.1 MB).
 constexpr int kCenterSamples = 16;
 
 // One sample by the 16 lanes of a DPP row.
@@ -254,8 +258,8 @@ __device__ __forceinline__ void center_row(const double* z, int k, T* __restrict
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void k_gsum_center(const T* __restrict__ part, int64_t B, int k,
-                                                     int64_t nslices, double tau,
+__global__ __launch_bounds__(256) void k_gsum_center(const double* __restrict__ part, int64_t B,
+                                                     int k, int64_t nslices, double tau,
                                                      T* __restrict__ out) {
     extern __shared__ __align__(16) unsigned char center_lds[];
     double* z = reinterpret_cast<double*>(center_lds);  // [kCenterSamples][k]
@@ -266,15 +270,15 @@ __global__ __launch_bounds__(256) void k_gsum_center(const T* __restrict__ part,
     for (int e = threadIdx.x; e < kCenterSamples * k; e += 256) {
         const int c = e / kCenterSamples, i = e % kCenterSamples;
         if (i >= ns) continue;
-        const T* src = part + c * B + n0 + i;
+        const double* src = part + c * B + n0 + i;
         double t = 0;
         // sixteen loads at a time, past the end the last slice again (no branch between loads)
         for (int64_t sl = 0; sl < nslices; sl += 16) {
-            T v[16];
+            double v[16];
 #pragma unroll
             for (int u = 0; u < 16; ++u) v[u] = src[std::min(sl + u, nslices - 1) * step];
 #pragma unroll
-            for (int u = 0; u < 16; ++u) t += sl + u < nslices ? double(v[u]) : 0.0;
+            for (int u = 0; u < 16; ++u) t += sl + u < nslices ? v[u] : 0.0;
         }
         z[i * k + c] = t / tau;
     }
@@ -618,10 +622,9 @@ extern "C" int cl_group_sum_forward(int dtype, const void* x, int64_t batch, int
 namespace {
 constexpr int64_t kCenterMaxClasses = 65536 / (8 * kCenterSamples);  // of one workgroup's LDS
 
-int64_t center_workspace(int64_t batch, int64_t features, int64_t stride_batch, int64_t k,
-                         int64_t size) {
+int64_t center_workspace(int64_t batch, int64_t features, int64_t stride_batch, int64_t k) {
     if (!gsum_split_applies(batch, features, stride_batch)) return 0;
-    return gsum_slices(batch, features, k, 1) * k * batch * size;
+    return gsum_slices(batch, features, k, 1) * k * batch * int64_t(sizeof(double));
 }
 }  // namespace
 
@@ -633,9 +636,9 @@ extern "C" int cl_group_sum_centered_workspace_size(int dtype, int64_t batch, in
     CL_ARG(batch >= 0 && features >= 0 && k >= 1, "bad shape");
     *bytes = -1;
     if (k > kCenterMaxClasses) return CL_OK;
-    CL_DTYPE_SWITCH(dtype, {
-        *bytes = center_workspace(batch, features, stride_batch, k, int64_t(sizeof(scalar_t)));
-    });
+    CL_ARG(dtype == CL_DTYPE_F32 || dtype == CL_DTYPE_F64,
+           "unsupported dtype code %d (expected CL_DTYPE_F32 or F64)", dtype);
+    *bytes = center_workspace(batch, features, stride_batch, k);
     return CL_OK;
 }
 
@@ -663,17 +666,18 @@ extern "C" int cl_group_sum_centered_forward(int dtype, const void* x, int64_t b
             constexpr int W = wide_vec<T>();
             const bool wide = batch % W == 0 && stride_feature % W == 0 && aligned(x, 16);
             const int64_t slices = gsum_slices(batch, features, k, wide ? W : 1);
-            CL_ARG(workspace && workspace_bytes >= slices * k * batch * int64_t(sizeof(T)),
+            CL_ARG(workspace && workspace_bytes >= slices * k * batch * int64_t(sizeof(double)),
                    "workspace needed (cl_group_sum_centered_workspace_size)");
-            T* part = static_cast<T*>(workspace);
+            CL_ARG(aligned(workspace, 8), "the workspace must be aligned to 8 bytes");
+            auto* part = static_cast<double*>(workspace);
             const int64_t slice = ceil_div(gsz, slices);
             const dim3 grid(unsigned(ceil_div(batch, 64 * (wide ? W : 1))), unsigned(k),
                             unsigned(slices));
             if (wide)
-                k_gsum_partial<T, W><<<grid, kPartWaves * 64, 0, s>>>(
+                k_gsum_partial<T, W, double><<<grid, kPartWaves * 64, 0, s>>>(
                     xs, batch, features, stride_feature, gsz, k, slice, part);
             else
-                k_gsum_partial<T, 1><<<grid, kPartWaves * 64, 0, s>>>(
+                k_gsum_partial<T, 1, double><<<grid, kPartWaves * 64, 0, s>>>(
                     xs, batch, features, stride_feature, gsz, k, slice, part);
             if (int rc = check_launch("cl_group_sum_centered_forward(partial)")) return rc;
             k_gsum_center<T><<<unsigned(ceil_div(batch, kCenterSamples)), 256,

@@ -450,7 +450,7 @@ int cl_group_sum_workspace_size(int dtype, int64_t batch, int64_t features, int6
 /* The scores less each sample's largest one, summed and subtracted in fp64 and rounded once: what
  * a softmax or a loss on differences of scores needs, without the rounding of the scores
  * themselves.  k <= 512; *bytes = -1 above.  workspace: cl_group_sum_centered_workspace_size
- * bytes.  The gradient of such a loss is cl_group_sum_backward's. */
+ * bytes, aligned to 8.  The gradient of such a loss is cl_group_sum_backward's. */
 int cl_group_sum_centered_workspace_size(int dtype, int64_t batch, int64_t features,
                                          int64_t stride_batch, int64_t k, int64_t* bytes);
 int cl_group_sum_centered_forward(int dtype, const void* x, int64_t batch, int64_t features,

@@ -1089,3 +1089,39 @@ def test_checkpointed_and_inference(device):
         assert torch.equal(got, want) and not got.requires_grad
     with pytest.raises(RuntimeError):
         torch.func.grad(both)(z.detach())
+
+
+@pytest.mark.parametrize("layout", ["columns", "rows", "strided"])
+@pytest.mark.parametrize("batch,feats,k", [(64, 12000, 10), (1024, 12000, 10), (65, 200001, 10),
+                                           (64, 200000, 2), (128, 30000, 300)])
+def test_group_sum_methods_sum_in_64_bits(device, batch, feats, k, layout):
+    """In every layout a score's error is that of one rounding at the size of its difference from
+    the largest one (spread 2^-24), whatever the class sums' size: twice that in lp, which is a
+    difference of two such numbers, and the fp64 additions' own, at most gsz + 8 of numbers up to
+    gsz.  Class sums in fp32 would be off by some sqrt(gsz) gsz 2^-24 / tau, ten times as much and
+    more."""
+    rng = np.random.default_rng(feats + k)
+    tau, unit, gsz = 2.0, 2.0**-24, -(-feats // k)
+    x = torch.as_tensor(rng.random((batch, feats))).float()
+    xn = _np(x)
+    if layout == "columns":
+        x = x.t().contiguous().to(device).t()
+    elif layout == "strided":
+        x = torch.zeros((batch, 2 * feats), device=device)[:, ::2].copy_(x)
+    x = x.to(device).requires_grad_()
+    padded = np.zeros((batch, gsz * k))
+    padded[:, :feats] = xn
+    z = padded.reshape(batch, k, gsz).sum(2) / tau
+    # the most likely class, whose log-probability is the smallest number, and any other
+    actions = np.where(rng.random(batch) < 0.5, z.argmax(1), rng.integers(0, k, batch))
+    lp, probs = P.log_probs(z, actions)
+    d = z - z.max(1, keepdims=True)
+    err = 2 * -d.min() * unit + 2 * (gsz + 8) * gsz * 2.0**-53 / tau + _sum_error(d, torch.float32)
+    got = cl.GroupSum(k, tau).log_probs(x, torch.as_tensor(actions).to(device))
+    _near(_np(got), lp, err, torch.float32)
+    up = torch.as_tensor(rng.standard_normal(batch)).float().to(device)
+    (grad,) = torch.autograd.grad(got, x, up)
+    want = P.logit_gradient(probs, actions, _np(up))
+    bound = np.abs(_np(up))[:, None] * 2 * err + np.abs(want) * 3 * unit
+    spread = np.repeat(np.eye(k), gsz, axis=1)[:, :feats] / tau
+    _near(_np(grad), want @ spread, bound @ spread, torch.float32)
