@@ -87,8 +87,9 @@ def _link_autograd(obj: Path) -> None:
 
 
 def build(verbose: bool = True) -> Path:
-    """Compile every csrc/*.hip for gfx950 and link the shared library, and the autograd extension
-    over it. Returns the library's path."""
+    """Compile every csrc/*.hip for gfx950 and link the shared library, then the autograd extension
+    over it. Returns the library's path.  Where only the extension fails, this raises with the
+    library in place."""
     hipcc = _hipcc()
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.hip"))
@@ -98,12 +99,17 @@ def build(verbose: bool = True) -> Path:
     with cf.ThreadPoolExecutor(max_workers=workers) as ex:
         autograd = ex.submit(_compile_autograd)
         objs = list(ex.map(lambda s: _compile(s, hipcc), sources))
-        autograd = autograd.result()
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
-    _run(cmd, "link")
-    os.replace(tmp, LIB)
-    _link_autograd(autograd)
+        tmp = LIB.with_suffix(".so.tmp")
+        cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
+        _run(cmd, "link")
+        os.replace(tmp, LIB)
+        try:
+            _link_autograd(autograd.result())
+        except Exception as e:
+            # one of an earlier build goes with an earlier library
+            AUTOGRAD.unlink(missing_ok=True)
+            raise RuntimeError(f"built {LIB}, but not the autograd extension (the losses of "
+                               f"policy.py and dropout need it): {e}") from e
     if verbose:
         print(f"built {LIB} from {len(sources)} sources", file=sys.stderr)
     return LIB
