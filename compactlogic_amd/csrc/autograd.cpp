@@ -25,14 +25,19 @@ using torch::autograd::variable_list;
 
 namespace {
 
-// A failure status of the library; becomes the Python package's exception.
-struct Failure : std::runtime_error {
-    int status;
-    Failure(const char* name, int rc)
-        : std::runtime_error(std::string(name) + " failed (status " + std::to_string(rc) +
-                             "): " + cl_last_error()),
-          status(rc) {}
-};
+// A failure status of the library as the Python package's exception.  It is raised as one here, on
+// any thread: of a C++ exception that leaves a backward, autograd hands on the text alone.
+[[noreturn]] void fail(const char* name, int status) {
+    const std::string text = std::string(name) + " failed (status " + std::to_string(status) +
+                             "): " + cl_last_error();
+    py::gil_scoped_acquire gil;
+    const py::object type =
+        status == CL_ERR_VALUE
+            ? py::reinterpret_borrow<py::object>(PyExc_ValueError)
+            : py::module_::import("compactlogic_amd._capi").attr("CompactLogicError");
+    PyErr_SetString(type.ptr(), text.c_str());
+    throw py::error_already_set();
+}
 
 cl::TimedHook g_timed;
 
@@ -41,7 +46,7 @@ template <typename F>
 void launch(const char* name, int device, F&& f) {
     void* stream = c10::hip::getCurrentHIPStream(c10::DeviceIndex(device)).stream();
     g_timed.run(name, [&] {
-        if (const int rc = f(stream)) throw Failure(name, rc);
+        if (const int rc = f(stream)) fail(name, rc);
     });
 }
 
@@ -60,7 +65,7 @@ at::TensorOptions wide_of(const Tensor& t) {
 }
 
 void sized(const char* name, int rc) {
-    if (rc) throw Failure(name, rc);
+    if (rc) fail(name, rc);
 }
 
 const int64_t* ints(const Tensor& t) { return static_cast<const int64_t*>(t.data_ptr()); }
@@ -513,17 +518,6 @@ void set_timed(py::object timed) { g_timed.set(std::move(timed)); }
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
-    py::register_exception_translator([](std::exception_ptr p) {
-        try {
-            if (p) std::rethrow_exception(p);
-        } catch (const Failure& f) {
-            const py::object capi = py::module_::import("compactlogic_amd._capi");
-            const py::object type = f.status == CL_ERR_VALUE
-                                        ? py::reinterpret_borrow<py::object>(PyExc_ValueError)
-                                        : capi.attr("CompactLogicError");
-            PyErr_SetString(type.ptr(), f.what());
-        }
-    });
     using unlocked = py::call_guard<py::gil_scoped_release>;
     m.def("selected_log_probs", &selected_log_probs, unlocked());
     m.def("policy_loss", &policy_loss, unlocked());

@@ -141,3 +141,10 @@ def test_autograd_extension(monkeypatch):
     monkeypatch.setitem(sys.modules, "compactlogic_amd._autograd", other)
     with pytest.raises(_capi.CompactLogicError, match="torch 0.0.1"):
         _native.load()
+
+
+def test_a_failing_call_raises_the_package_error():
+    """Sizes are refused before anything is allocated or launched."""
+    with pytest.raises(_capi.CompactLogicError, match="cl_token_loss_workspace failed.*bad shape"):
+        _native.load().selected_log_probs(torch.zeros(3, 0), torch.zeros(3, dtype=torch.int64),
+                                          -100, 0, 1.0)

@@ -1,6 +1,7 @@
 """Losses on chosen log-probabilities against the float64 oracle: values and gradients over types,
 lengths, strides, masks, ragged sequences; graphs, streams, refusals."""
 import concurrent.futures
+import contextlib
 import ctypes
 
 import numpy as np
@@ -1125,3 +1126,32 @@ def test_group_sum_methods_sum_in_64_bits(device, batch, feats, k, layout):
     bound = np.abs(_np(up))[:, None] * 2 * err + np.abs(want) * 3 * unit
     spread = np.repeat(np.eye(k), gsz, axis=1)[:, :feats] / tau
     _near(_np(grad), want @ spread, bound @ spread, torch.float32)
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_failing_backward_raises_the_package_error(device, recorded):
+    """The library refuses a backward whose saved buffer has gone (it checks before any launch);
+    its error keeps its type on the way from autograd's thread."""
+    c = Case(8, 20, torch.float32, device)
+    x = torch.rand((8, 100), device=device, requires_grad=True)
+    z = c.logits.requires_grad_()
+    off = torch.tensor([0, 3, 8], device=device)
+    gs = cl.GroupSum(20)
+    calls = [lambda: cl.selected_log_probs(z, c.act_t).sum(),
+             lambda: cl.policy_loss(z, c.act_t, c.old_t, c.adv_t),
+             lambda: cl.preference_loss(z, c.act_t, off),
+             lambda: gs.policy_loss(x, c.act_t, c.old_t, c.adv_t)]
+
+    def lost(t):
+        return t[:0].clone() if t.dtype == torch.uint8 else t
+
+    for call in calls:
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lost):
+            loss = call()
+        with timing.record() if recorded else contextlib.nullcontext():
+            with pytest.raises(_capi.CompactLogicError, match=r"cl_.*backward failed.*null"):
+                loss.backward()
+    assert z.grad is None and x.grad is None
+    for call in calls:
+        call().backward()
+    assert torch.isfinite(z.grad).all() and torch.isfinite(x.grad).all()
