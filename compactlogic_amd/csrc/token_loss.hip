@@ -727,6 +727,7 @@ struct PairArgs {
     const int64_t* offsets;
     int64_t rows, pairs;
     double beta, smooth;
+    RowState<A>* state;
     int32_t* row_seq;
     A* seq_slope;
     A* margins;
@@ -747,6 +748,10 @@ __device__ __forceinline__ double pair_term(const PairArgs<A>& a, int64_t i, dou
         const int64_t q = i + side * a.pairs;
         int64_t b = a.offsets[q], e = a.offsets[q + 1];
         bad |= b < 0 || e < b || e > a.rows;
+        // Rows inside of a decrease may lie in several sequences, whose stores of row_seq then race:
+        // their gradient is NaN whichever comes last.
+        for (int64_t n = std::max<int64_t>(e, 0) + t0; n < std::min(b, a.rows); n += LANES)
+            if (a.state[n].slope != A(0)) a.state[n].slope = nan_value<A>();
         b = std::min(std::max<int64_t>(b, 0), a.rows);
         e = std::min(std::max(e, b), a.rows);
         double t = 0;
@@ -1186,7 +1191,8 @@ extern "C" int cl_preference_loss_forward(int dtype, const void* logits, int64_t
                                              ignore_index, log_probs, row_state),
                                  op, workspace, workspace_bytes, s))
             return rc;
-        const PairArgs<A> pa{gaps, offsets, rows, pairs, beta, label_smoothing, row_seq,
+        const PairArgs<A> pa{gaps, offsets, rows, pairs, beta, label_smoothing,
+                             static_cast<RowState<A>*>(row_state), row_seq,
                              static_cast<A*>(seq_slope), static_cast<A*>(margins),
                              static_cast<A*>(terms)};
         const int mean = reduction == CL_REDUCE_MEAN;

@@ -158,7 +158,8 @@ def preference_loss(logits, actions, offsets, ref_log_probs=None, beta: float = 
 
     reduction: 'mean' over the pairs, 'sum', or 'none' (the terms, [P]).  With return_margins, also
     the margins [P] (not differentiable through this call).  Rows of no sequence do not count;
-    offsets that decrease or leave the rows make their pair's term NaN."""
+    offsets that decrease or leave the rows make their pair's term NaN, and a decrease the gradient
+    of the rows inside of it, which may lie in several sequences."""
     rows, acts = _flat(logits, actions)
     if logits.dim() != 2:
         raise RuntimeError("preference_loss takes logits [rows, classes] of a ragged batch")

@@ -624,8 +624,9 @@ int cl_policy_loss_backward(int dtype, const void* logits, int64_t row_stride, i
  * lp - ref_log_probs (NULL: 0) and h = beta (D_i - D_(pairs + i)) = margins[i],
  *   terms[i] = -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h);
  * loss: their sum or mean over the pairs.  A pair whose offsets decrease or leave [0, rows] gets
- * NaN.  Rows of no sequence do not count.  gaps: double [rows], row_seq: int32 [rows],
- * seq_slope: wide [2 pairs]; written for the backward. */
+ * NaN, and so does the gradient of rows inside of a decrease (offsets[q + 1] <= row < offsets[q]),
+ * which may lie in several sequences.  Rows of no sequence do not count.  gaps: double [rows],
+ * row_seq: int32 [rows], seq_slope: wide [2 pairs]; written for the backward. */
 int cl_preference_loss_forward(int dtype, const void* logits, int64_t row_stride, int64_t rows,
                                int64_t cols, const int64_t* actions, int64_t ignore_index,
                                const void* ref_log_probs, const int64_t* offsets, int64_t pairs,

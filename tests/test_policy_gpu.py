@@ -1155,3 +1155,45 @@ def test_a_failing_backward_raises_the_package_error(device, recorded):
     for call in calls:
         call().backward()
     assert torch.isfinite(z.grad).all() and torch.isfinite(x.grad).all()
+
+
+@pytest.mark.parametrize("pairs,rows", [(2, 12), (2, 9000), (70, 9000)])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_rows_inside_a_decrease_of_the_offsets(device, pairs, rows, grouped):
+    """Where sequence 1 runs backwards, from row 5 to 3, rows 3 and 4 lie in sequences 0 and 2: no
+    order of their kernels' stores decides, the gradient is NaN (0 where the row does not count).
+    The other rows of the pairs without a decrease have theirs.  One kernel for few short pairs,
+    for long ones, for many."""
+    rng = np.random.default_rng(rows + pairs)
+    k = 20
+    z = rng.standard_normal((rows, k))
+    z = torch.as_tensor(z - z.max(1, keepdims=True)).float()      # as GroupSum's scores are centred
+    actions = rng.integers(0, k, rows)
+    actions[[4, 7]] = IGNORE
+    off = np.concatenate(([0, 5, 3], np.linspace(8, rows, 2 * pairs - 2).astype(int)))
+    lp, probs = P.log_probs(_np(z), actions)
+    h = P.preference_terms(lp, actions, off, None, 0.1, 0.0)[0]
+    slope = np.zeros(rows)
+    for i in range(pairs):
+        d = np.nan if i == 1 else -0.1 / (1 + np.exp(h[i]))
+        slope[off[i]:off[i + 1]] = d
+        slope[off[pairs + i]:off[pairs + i + 1]] = -d
+    slope[3:5] = np.nan
+    slope[actions == IGNORE] = 0.0
+    x = z.to(device).requires_grad_()               # a class per feature: the scores are x
+    act, offsets = torch.as_tensor(actions).to(device), torch.as_tensor(off).to(device)
+    loss = cl.GroupSum(k).preference_loss if grouped else cl.preference_loss
+    terms = loss(x, act, offsets, reduction="none")
+    assert torch.isnan(terms).tolist() == [i == 1 for i in range(pairs)]
+    (grad,) = torch.autograd.grad(terms, x, torch.ones_like(terms))
+    grad = _np(grad)
+    bad = np.isnan(slope)
+    assert np.isnan(grad[bad]).all() and (grad[actions == IGNORE] == 0).all()
+    # a margin adds gaps of rows of two sequences, each off by the error of its lp
+    err = _sum_error(_np(z), torch.float32)
+    longest = np.diff(off).max()
+    known = np.where(bad, 0.0, slope)
+    want = P.logit_gradient(probs, actions, known)
+    bound = np.abs(known)[:, None] * 2 * err + 0.1 * (0.1 * 2 * longest * err) \
+        + np.abs(want) * 3 * 2.0**-24
+    _near(grad[~bad], want[~bad], bound[~bad], torch.float32)
