@@ -16,7 +16,7 @@ from .layers import (ConvLayer, ConvLayerCudaFunction, ConvLayerSoftmaxFunction,
                      GroupSumFunction, LogicGroupSumCrossEntropyFunction, LogicLayer,
                      LogicLayerCudaFunction, LogicLayerRunsFunction, PackBitsTensor,
                      logic_group_sum_cross_entropy, sequential_cross_entropy)
-from .optim import FusedAdam
+from .optim import FusedAdam, FusedAdamW
 from .packed_net import PackedNetwork
 from .plan import RunPlan, build_run_plan
 from .policy import policy_loss, preference_loss, selected_log_probs
@@ -31,7 +31,7 @@ __all__ = [
     "ConvLayer", "ConvLayerCudaFunction", "ConvLayerSoftmaxFunction", "ConvLayerWindowFunction",
     "convlogic_hip", "SequentialEntropyFreezer", "FixedSequentialEntropyFreezer",
     "EntropyRowResampler", "PackedNetwork", "ConvLogicLayer", "TreeLogicLayer", "PoolLogicLayer",
-    "ConvLogicFunction", "FullConvLogicFunction", "TreeLogicFunction", "FusedAdam",
+    "ConvLogicFunction", "FullConvLogicFunction", "TreeLogicFunction", "FusedAdam", "FusedAdamW",
     "LogicGroupSumCrossEntropyFunction", "logic_group_sum_cross_entropy",
     "sequential_cross_entropy", "checkpoint", "circuit", "Dropout", "dropout",
     "policy_loss", "preference_loss", "selected_log_probs",

@@ -136,6 +136,10 @@ SIGNATURES: dict[str, list] = {
     "cl_adam_clip_workspace": [_i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64)],
     "cl_adam_clip_step": [_int, _i64, _p, _p, _p, _p, ctypes.POINTER(_i64), _p, _f64, _f64,
                           _f64, _f64, _f64, _p, _i64, _p],
+    "cl_adamw_workspace": [_i64, ctypes.POINTER(_i64)],
+    "cl_adamw_step": [_i64, _p, _i64, _p, _f64, _p, _p, _i64, _p],
+    "cl_adamw_moments_read": [_i64, _p, _p],
+    "cl_adamw_moments_write": [_i64, _p, _p],
     "cl_token_loss_workspace": [_int, _i64, _i64, ctypes.POINTER(_i64)],
     "cl_selected_log_prob_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p],
     "cl_selected_log_prob_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],
@@ -175,6 +179,20 @@ SIGNATURES: dict[str, list] = {
     "cl_packed_network_columns": [_p, _i64, _i64, _i64, _p, ctypes.POINTER(_i64), _i64, _i64,
                                   _p, _p],
 }
+
+
+
+class AdamWTensor(ctypes.Structure):
+    """cl_adamw_tensor"""
+    _fields_ = [("param", _p), ("grad", _p), ("exp_avg", _p), ("exp_avg_sq", _p), ("powers", _p),
+                ("numel", _i64), ("dtype", _i32), ("bits", _i32), ("group", _i32),
+                ("reserved", _i32)]
+
+
+class AdamWGroup(ctypes.Structure):
+    """cl_adamw_group"""
+    _fields_ = [(name, _f64) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
 
 _lib = None
 

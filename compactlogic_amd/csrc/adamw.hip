@@ -1,0 +1,708 @@
+// One AdamW step over many tensors, with moments in 32 bits (64 for fp64 parameters) or in 8.
+//
+//   c = min(1, M / (|g| + 1e-6)),  g' = c g                     (|g| over all tensors, in fp64)
+//   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+//   k_adamw_begin   the step count, each group's coefficients (fp64, once) and the sums of g^2 of
+//                   the workgroups, at most kNormParts of them
+//   k_adamw         adds the sums in a fixed order (the norm), then one pass over p, g, m, v
+//
+// Tensors are cut into tiles, so that a small one costs one workgroup; a launch takes kTensors
+// tensors of one type, their addresses in the kernel's arguments (a captured graph keeps them, and
+// nothing is copied to the device).  A lane holds one tensor's first tile, and the tile's tensor is
+// the number of lanes whose first tile is not behind it.
+//
+// Moments in 8 bits go by blocks of 256 consecutive elements, each with a power of two for m and one
+// for v: codes that have exponents of their own lose nothing by a power of two where a free scale
+// would keep their mantissas, and scaling is exact.  m is e4m3, the block's largest in [128, 256).
+// v >= 0 has five bits of exponent and three of mantissa, the block's largest in [1, 2): code c in
+// 1..254 is the fp32 number whose bits are (c + 770) << 20, 2^-31 * 1.375 to 2; 255 is NaN.  Only 0
+// is held as 0: the root of v divides, and an element whose v were lost under its neighbours' would
+// make a step of m / eps.
+#include "storage.h"
+
+namespace cl {
+namespace {
+
+constexpr int kOptThreads = 256;
+constexpr int kTile = 2048;        // elements; whole blocks
+constexpr int kTensors = 64;       // of a launch: a lane each
+constexpr int kGroups = 32;
+constexpr int kHeld = 256;         // elements of a block
+constexpr int kNormParts = 512;
+constexpr int kCoefs = 8;
+
+// A group's coefficients as the first kernel leaves them (fp64).
+enum { kDecay, kSize, kInvRoot, kB1, kRest1, kB2, kRest2, kEps };
+
+struct Tensors {
+    int n;
+    uint32_t tiles;
+    uint32_t first[kTensors];  // first tile; those of no tensor: UINT32_MAX
+    int64_t numel[kTensors];
+    void* param[kTensors];
+    void* grad[kTensors];
+    void* m[kTensors];
+    void* v[kTensors];
+    uint8_t* power[kTensors];  // 8 bits: exponents + 127 of the blocks, m's and then v's
+    uint8_t group[kTensors];
+};
+
+struct Grads {
+    int n;
+    uint32_t tiles;
+    uint32_t first[kTensors];
+    int64_t numel[kTensors];
+    const void* grad[kTensors];
+};
+
+struct Groups {
+    int n;
+    double lr[kGroups], b1[kGroups], b2[kGroups], eps[kGroups], decay[kGroups];
+};
+
+// The tensor that a tile lies in, the same in all lanes.
+__device__ __forceinline__ int tensor_of(const uint32_t* first, uint32_t tile) {
+    return int(__builtin_popcountll(__ballot(first[lane_id()] <= tile))) - 1;
+}
+
+// Sum over the workgroup, the same bits in every thread.
+__device__ __forceinline__ double group_total(double v, double* red) {
+    v = wave_total(v);
+    if (lane_id() == 0) red[wave_id()] = v;
+    __syncthreads();
+    double s = red[0];
+#pragma unroll
+    for (int i = 1; i < kOptThreads / 64; ++i) s += red[i];
+    return s;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads ts, double* __restrict__ parts,
+                                                             Groups groups,
+                                                             double* __restrict__ step,
+                                                             double* __restrict__ coefs) {
+    constexpr int VEC = wide_vec<T>(), NV = kTile / kOptThreads / VEC;
+    __shared__ double red[kOptThreads / 64];
+    if (groups.n > 0 && blockIdx.x == 0 && wave_id() == 0) {
+        const double t = step[0] + 1.0;
+        const int i = threadIdx.x;
+        if (i < groups.n) {
+            double* c = coefs + i * kCoefs;
+            const double b1 = groups.b1[i], b2 = groups.b2[i], lr = groups.lr[i];
+            c[kDecay] = 1.0 - lr * groups.decay[i];
+            c[kSize] = lr / (1.0 - pow(b1, t));
+            c[kInvRoot] = 1.0 / sqrt(1.0 - pow(b2, t));
+            c[kB1] = b1;
+            c[kRest1] = 1.0 - b1;
+            c[kB2] = b2;
+            c[kRest2] = 1.0 - b2;
+            c[kEps] = groups.eps[i];
+        }
+        if (i == 0) step[0] = t;
+    }
+    if (ts.n == 0) return;
+    double s = 0.0;
+    for (uint32_t tile = blockIdx.x; tile < ts.tiles; tile += gridDim.x) {
+        const int k = tensor_of(ts.first, tile);
+        const int64_t i0 = int64_t(tile - ts.first[k]) * kTile, n = ts.numel[k] - i0;
+        const T* g = static_cast<const T*>(ts.grad[k]) + i0;
+        if (n >= kTile) {
+            Pack<T, VEC> v[NV];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) v[j] = pload<T, VEC>(g + (j * kOptThreads + threadIdx.x) * VEC);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s = fma(double(v[j].v[e]), double(v[j].v[e]), s);
+        } else {
+            for (int j = threadIdx.x; j < int(n); j += kOptThreads) s = fma(double(g[j]), double(g[j]), s);
+        }
+    }
+    s = group_total(s, red);
+    if (threadIdx.x == 0) parts[blockIdx.x] = s;
+}
+
+// ---- the update of one element.  m and v are rounded product by product, so that an 8-bit code does
+// not depend on what a compiler fuses; the quotient, which only p takes, by the hardware's square
+// root and reciprocal, each within a unit in the last place (fp32; a v below 2^-126 counts as 0
+// there).  The IEEE forms take some 20 instructions more of about 60.
+template <typename A>
+struct Coefs {
+    A scale;  // of the gradient
+    A decay, size, inv_root, b1, rest1, b2, rest2, eps;
+};
+
+__device__ __forceinline__ float quotient(float m, float v, const Coefs<float>& c) {
+    const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v), c.inv_root, c.eps);
+    return m * __builtin_amdgcn_rcpf(d);
+}
+__device__ __forceinline__ double quotient(double m, double v, const Coefs<double>& c) {
+    return m / (sqrt(v) * c.inv_root + c.eps);
+}
+
+template <typename A>
+__device__ __forceinline__ void moments_step(A g, A& m, A& v, const Coefs<A>& c) {
+#pragma clang fp contract(off)
+    g = g * c.scale;
+    const A q = g * g;
+    m = m * c.b1 + g * c.rest1;
+    v = v * c.b2 + q * c.rest2;
+}
+
+template <typename A>
+__device__ __forceinline__ A param_step(A p, A m, A v, const Coefs<A>& c) {
+    return fma(p, c.decay, -(c.size * quotient(m, v, c)));
+}
+
+// Every workgroup adds the same sums in the same order.
+template <typename A>
+__device__ __forceinline__ Coefs<A> load_coefs(const double* __restrict__ parts, int nparts,
+                                               double max_norm, const double* __restrict__ coefs,
+                                               int group, double* red) {
+    const double* c = coefs + group * kCoefs;
+    Coefs<A> r;
+    r.decay = A(c[kDecay]);
+    r.size = A(c[kSize]);
+    r.inv_root = A(c[kInvRoot]);
+    r.b1 = A(c[kB1]);
+    r.rest1 = A(c[kRest1]);
+    r.b2 = A(c[kB2]);
+    r.rest2 = A(c[kRest2]);
+    r.eps = A(c[kEps]);
+    r.scale = A(1);
+    if (nparts > 0) {
+        double s = 0.0;
+        for (int i = threadIdx.x; i < nparts; i += kOptThreads) s += parts[i];
+        const double k = max_norm / (sqrt(group_total(s, red)) + 1e-6);
+        r.scale = A(k < 1.0 ? k : 1.0);
+    }
+    return r;
+}
+
+// ---- 8 bits.  A block of 256 lies in 32 lanes of 8 elements.
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+    v = max(v, dpp_move<0xB1>(v));   // quad_perm [1,0,3,2]
+    v = max(v, dpp_move<0x4E>(v));   // quad_perm [2,3,0,1]
+    v = max(v, dpp_move<0x141>(v));  // row_half_mirror
+    v = max(v, dpp_move<0x140>(v));  // row_mirror
+    return max(v, xor_lane<16>(v));
+}
+
+constexpr uint32_t kInfBits = 0x7F800000u, kMagnitude = 0x7FFFFFFFu;
+constexpr uint32_t kFirstCode = 770;
+
+__device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ float float_of(uint32_t x) { return __builtin_bit_cast(float, x); }
+
+struct Codes {
+    uint2 m, v;
+};
+
+// Exponents of the block, from its largest finite magnitude, and the codes of this lane's elements.
+// A code of what is not finite is NaN, whatever the block's other elements are.
+struct Powers {
+    int m, v;
+};
+
+// Leaves no m and v that are not finite.
+__device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& power) {
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        top_m = max(top_m, bits_of(m[e]) & kMagnitude);
+        top_v = max(top_v, bits_of(v[e]) & kMagnitude);
+    }
+    top_m = block_max(top_m);
+    top_v = block_max(top_v);
+    const bool odd = max(top_m, top_v) >= kInfBits;
+    uint32_t no_m = 0, no_v = 0;
+    if (odd) {  // the same in the 32 lanes of a block
+        top_m = top_v = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t a = bits_of(m[e]) & kMagnitude, b = bits_of(v[e]) & kMagnitude;
+            if (a >= kInfBits) {
+                no_m |= 1u << e;
+                m[e] = 0.0f;
+            } else {
+                top_m = max(top_m, a);
+            }
+            if (b >= kInfBits) {
+                no_v |= 1u << e;
+                v[e] = 0.0f;
+            } else {
+                top_v = max(top_v, b);
+            }
+        }
+        top_m = block_max(top_m);
+        top_v = block_max(top_v);
+    }
+    power.m = max(int(top_m >> 23) - 134, -126);
+    power.v = max(int(top_v >> 23) - 127, -126);
+    Codes c;
+    uint32_t pm[2], pv[2] = {0, 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = __builtin_amdgcn_ldexpf(m[4 * h + e], -power.m);
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], 0, false);
+        pm[h] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], w, true));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t b = bits_of(__builtin_amdgcn_ldexpf(v[4 * h + e], -power.v));
+            const int r = int((b + 0x7FFFFu + ((b >> 20) & 1)) >> 20) - int(kFirstCode);
+            // the middle one of r, 1 and a number that is 0 for v = 0 (r is then below 0) and else not
+            // below r, nor 0 where scaling lost v
+            const int some = int(b | bits_of(v[4 * h + e]));
+            const int code = max(min(r, 1), min(max(r, 1), some));
+            pv[h] |= uint32_t(code) << (8 * e);
+        }
+    }
+    if (odd) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int s = 8 * (e & 3);
+            if (no_m >> e & 1) pm[e >> 2] |= 0x7Fu << s;
+            if (no_v >> e & 1) pv[e >> 2] |= 0xFFu << s;
+        }
+    }
+    c.m = make_uint2(pm[0], pm[1]);
+    c.v = make_uint2(pv[0], pv[1]);
+    return c;
+}
+
+__device__ __forceinline__ void decode(const Codes& c, const Powers& power, float (&m)[8],
+                                       float (&v)[8]) {
+    const uint32_t wm[2] = {c.m.x, c.m.y}, wv[2] = {c.v.x, c.v.y};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        typedef float pair __attribute__((ext_vector_type(2)));
+        const pair lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(wm[h]), false);
+        const pair hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(wm[h]), true);
+        const float u[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            m[4 * h + e] = __builtin_amdgcn_ldexpf(u[e], power.m);
+            const uint32_t code = (wv[h] >> (8 * e)) & 0xFFu;
+            // 255 has the bits of 2 * 1.125
+            uint32_t b = code == 0 ? 0u : (code + kFirstCode) << 20;
+            if (code == 0xFFu) b = 0x7FC00000u;
+            v[4 * h + e] = __builtin_amdgcn_ldexpf(float_of(b), power.v);
+        }
+    }
+}
+
+// Codes of eight elements, the last ones of a tensor one by one.
+__device__ __forceinline__ uint2 load_codes(const uint8_t* p, int count) {
+    if (count >= 8) {
+        typedef uint32_t words __attribute__((ext_vector_type(2), aligned(1)));
+        const words w = *reinterpret_cast<const words*>(p);
+        return make_uint2(w.x, w.y);
+    }
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (e < count) w[e >> 2] |= uint32_t(p[e]) << (8 * (e & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int count) {
+    if (count >= 8) {
+        typedef uint32_t words __attribute__((ext_vector_type(2), aligned(1)));
+        *reinterpret_cast<words*>(p) = words{c.x, c.y};
+        return;
+    }
+    const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (e < count) p[e] = uint8_t(w[e >> 2] >> (8 * (e & 3)));
+}
+
+template <typename T>
+struct Eight {
+    T v[8];
+};
+
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int count) {
+    Eight<T> r;
+    if (count >= 8) return __builtin_bit_cast(Eight<T>, pload<T, 8>(p));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = e < count ? p[e] : T(0);
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, const Eight<T>& r, int count) {
+    if (count >= 8) {
+        pstore<T, 8>(p, __builtin_bit_cast(Pack<T, 8>, r));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+        if (e < count) p[e] = r.v[e];
+}
+
+// Eight elements of a tile per thread, kHeld in 32 lanes; every lane takes part, those past the
+// tensor's end with count <= 0 (and zeros).
+struct Place {
+    int64_t at;   // of the tensor
+    int64_t block, blocks;
+    int count;
+    __device__ __forceinline__ Place(uint32_t tile, int64_t numel) {
+        at = int64_t(tile) * kTile + threadIdx.x * 8;
+        block = at / kHeld;
+        blocks = (numel + kHeld - 1) / kHeld;
+        const int64_t left = numel - at;
+        count = left >= 8 ? 8 : left > 0 ? int(left) : 0;
+    }
+};
+
+__device__ __forceinline__ Powers load_powers(const uint8_t* power, const Place& at) {
+    if (at.count == 0) return {0, 0};
+    return {int(power[at.block]) - 127, int(power[at.blocks + at.block]) - 127};
+}
+
+__device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, const Powers& p) {
+    if (at.count > 0 && (threadIdx.x & 31) == 0) {
+        power[at.block] = uint8_t(p.m + 127);
+        power[at.blocks + at.block] = uint8_t(p.v + 127);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors ts, const double* __restrict__ parts,
+                                                        int nparts, double max_norm,
+                                                        const double* __restrict__ coefs) {
+    __shared__ double red[kOptThreads / 64];
+    const uint32_t tile = uint32_t(group_index());
+    if (tile >= ts.tiles) return;
+    const int k = tensor_of(ts.first, tile);
+    const Place at(tile - ts.first[k], ts.numel[k]);
+    T* p = static_cast<T*>(ts.param[k]) + at.at;
+    uint8_t* pm = static_cast<uint8_t*>(ts.m[k]) + at.at;
+    uint8_t* pv = static_cast<uint8_t*>(ts.v[k]) + at.at;
+    Eight<T> w = load_eight(p, at.count);
+    const Eight<T> g = load_eight(static_cast<const T*>(ts.grad[k]) + at.at, at.count);
+    const Codes held{load_codes(pm, at.count), load_codes(pv, at.count)};
+    Powers power = load_powers(ts.power[k], at);
+    const Coefs<float> c = load_coefs<float>(parts, nparts, max_norm, coefs, ts.group[k], red);
+    float m[8], v[8];
+    decode(held, power, m, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        moments_step(float(g.v[e]), m[e], v[e], c);
+        w.v[e] = T(param_step(float(w.v[e]), m[e], v[e], c));
+    }
+    const Codes next = encode(m, v, power);
+    store_eight(p, w, at.count);
+    store_codes(pm, next.m, at.count);
+    store_codes(pv, next.v, at.count);
+    store_powers(ts.power[k], at, power);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors ts, const double* __restrict__ parts,
+                                                       int nparts, double max_norm,
+                                                       const double* __restrict__ coefs) {
+    using A = wide_t<T>;
+    constexpr int VEC = wide_vec<T>(), NV = kTile / kOptThreads / VEC;
+    __shared__ double red[kOptThreads / 64];
+    const uint32_t tile = uint32_t(group_index());
+    if (tile >= ts.tiles) return;
+    const int k = tensor_of(ts.first, tile);
+    const int64_t i0 = int64_t(tile - ts.first[k]) * kTile, n = ts.numel[k] - i0;
+    T* p = static_cast<T*>(ts.param[k]) + i0;
+    const T* g = static_cast<const T*>(ts.grad[k]) + i0;
+    A* pm = static_cast<A*>(ts.m[k]) + i0;
+    A* pv = static_cast<A*>(ts.v[k]) + i0;
+    if (n >= kTile) {
+        Pack<T, VEC> w[NV], d[NV];
+        Pack<A, VEC> m[NV], v[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = (j * kOptThreads + threadIdx.x) * VEC;
+            w[j] = pload<T, VEC>(p + i);
+            d[j] = pload<T, VEC>(g + i);
+            m[j] = pload<A, VEC>(pm + i);
+            v[j] = pload<A, VEC>(pv + i);
+        }
+        const Coefs<A> c = load_coefs<A>(parts, nparts, max_norm, coefs, ts.group[k], red);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int i = (j * kOptThreads + threadIdx.x) * VEC;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                moments_step(A(d[j].v[e]), m[j].v[e], v[j].v[e], c);
+                w[j].v[e] = T(param_step(A(w[j].v[e]), m[j].v[e], v[j].v[e], c));
+            }
+            pstore<T, VEC>(p + i, w[j]);
+            pstore<A, VEC>(pm + i, m[j]);
+            pstore<A, VEC>(pv + i, v[j]);
+        }
+    } else {
+        const Coefs<A> c = load_coefs<A>(parts, nparts, max_norm, coefs, ts.group[k], red);
+        for (int i = threadIdx.x; i < int(n); i += kOptThreads) {
+            A m = pm[i], v = pv[i];
+            moments_step(A(g[i]), m, v, c);
+            p[i] = T(param_step(A(p[i]), m, v, c));
+            pm[i] = m;
+            pv[i] = v;
+        }
+    }
+}
+
+// What 8 bits hold, in bf16 (which holds it all), and 8 bits from fp32.  param: exp_avg, grad:
+// exp_avg_sq as they are outside.
+__global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors ts) {
+    const uint32_t tile = uint32_t(group_index());
+    if (tile >= ts.tiles) return;
+    const int k = tensor_of(ts.first, tile);
+    const Place at(tile - ts.first[k], ts.numel[k]);
+    const Codes held{load_codes(static_cast<uint8_t*>(ts.m[k]) + at.at, at.count),
+                     load_codes(static_cast<uint8_t*>(ts.v[k]) + at.at, at.count)};
+    float m[8], v[8];
+    decode(held, load_powers(ts.power[k], at), m, v);
+    Eight<bf16_t> a, b;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        a.v[e] = bf16_t(m[e]);
+        b.v[e] = bf16_t(v[e]);
+    }
+    store_eight(static_cast<bf16_t*>(ts.param[k]) + at.at, a, at.count);
+    store_eight(static_cast<bf16_t*>(ts.grad[k]) + at.at, b, at.count);
+}
+
+__global__ __launch_bounds__(kOptThreads) void k_adamw8_write(Tensors ts) {
+    const uint32_t tile = uint32_t(group_index());
+    if (tile >= ts.tiles) return;
+    const int k = tensor_of(ts.first, tile);
+    const Place at(tile - ts.first[k], ts.numel[k]);
+    const Eight<float> a = load_eight(static_cast<const float*>(ts.param[k]) + at.at, at.count);
+    const Eight<float> b = load_eight(static_cast<const float*>(ts.grad[k]) + at.at, at.count);
+    float m[8], v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        m[e] = a.v[e];
+        v[e] = b.v[e] < 0.0f ? __builtin_nanf("") : b.v[e] + 0.0f;  // no -0
+    }
+    Powers power;
+    const Codes c = encode(m, v, power);
+    store_codes(static_cast<uint8_t*>(ts.m[k]) + at.at, c.m, at.count);
+    store_codes(static_cast<uint8_t*>(ts.v[k]) + at.at, c.v, at.count);
+    store_powers(ts.power[k], at, power);
+}
+
+// ---- tensors into launches
+struct Batch {
+    Tensors ts{};
+    int64_t tiles = 0;
+
+    Batch() { clear(); }
+    void clear() {
+        ts.n = 0;
+        tiles = 0;
+        for (int i = 0; i < kTensors; ++i) ts.first[i] = UINT32_MAX;
+    }
+    // Whether the tensor has a place in this launch.
+    bool fits(int64_t numel) const {
+        return ts.n < kTensors && tiles + ceil_div(numel, kTile) < (int64_t(1) << 31);
+    }
+    dim3 grid() const { return wide_grid(tiles); }
+    void add(const cl_adamw_tensor& t) {
+        const int i = ts.n++;
+        ts.first[i] = uint32_t(tiles);
+        ts.numel[i] = t.numel;
+        ts.param[i] = t.param;
+        ts.grad[i] = t.grad;
+        ts.m[i] = t.exp_avg;
+        ts.v[i] = t.exp_avg_sq;
+        ts.power[i] = t.powers;
+        ts.group[i] = uint8_t(t.group);
+        tiles += ceil_div(t.numel, kTile);
+        ts.tiles = uint32_t(tiles);
+    }
+    Grads grads() const {
+        Grads g;
+        g.n = ts.n;
+        g.tiles = uint32_t(tiles);
+        for (int i = 0; i < kTensors; ++i) {
+            g.first[i] = ts.first[i];
+            g.numel[i] = ts.numel[i];
+            g.grad[i] = ts.grad[i];
+        }
+        return g;
+    }
+};
+
+// What must be the same within a launch: the type of the gradients; that and the bits of the moments
+// (kinds from 4 on: 8 bits); nothing.
+enum class Alike { kDtype, kDtypeAndBits, kAll };
+constexpr int kKinds = 8;
+
+int kind_of(const cl_adamw_tensor& t, Alike alike) {
+    if (alike == Alike::kAll) return 0;
+    return t.dtype + (alike == Alike::kDtypeAndBits && t.bits == 8 ? 4 : 0);
+}
+
+// Calls f(kind, batch) for the launches that the tensors make, kind by kind.
+template <typename F>
+int each_batch(const cl_adamw_tensor* t, int64_t n, Alike alike, F&& f) {
+    Batch b;
+    for (int kind = 0; kind < kKinds; ++kind) {
+        b.clear();
+        for (int64_t i = 0; i < n; ++i) {
+            if (t[i].numel == 0 || kind_of(t[i], alike) != kind) continue;
+            if (!b.fits(t[i].numel)) {
+                if (int rc = f(kind, b)) return rc;
+                b.clear();
+            }
+            b.add(t[i]);
+        }
+        if (b.ts.n)
+            if (int rc = f(kind, b)) return rc;
+    }
+    return CL_OK;
+}
+
+int check_tensor(const cl_adamw_tensor& t, int64_t i, int64_t num_groups, bool values) {
+    CL_ARG(t.numel >= 0, "negative tensor size at index %lld", (long long)i);
+    CL_ARG(ceil_div(t.numel, kTile) < (int64_t(1) << 31) - 1, "tensor %lld is too long",
+           (long long)i);
+    CL_ARG(t.bits == 8 || (!values && t.bits == 32), "moments are held in 32 or 8 bits");
+    CL_ARG(t.numel == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq &&
+                            (t.bits == 32 || t.powers)),
+           "null tensor pointer at index %lld", (long long)i);
+    if (values) return CL_OK;
+    CL_ARG(t.dtype >= CL_DTYPE_F32 && t.dtype <= CL_DTYPE_BF16,
+           "unsupported dtype code %d (expected F32, F64, F16 or BF16)", int(t.dtype));
+    CL_ARG(t.bits == 32 || t.dtype != CL_DTYPE_F64, "fp64 parameters have no moments in 8 bits");
+    CL_ARG(t.group >= 0 && t.group < num_groups, "no group %d", int(t.group));
+    return CL_OK;
+}
+
+// Sums that a launch of the norm may leave: its share of kNormParts by its tiles, at least one.
+int64_t norm_parts(int64_t tiles, int64_t all) {
+    const int64_t share = tiles * kNormParts / all;
+    return share < 1 ? 1 : share < tiles ? share : tiles;
+}
+
+}  // namespace
+}  // namespace cl
+
+using namespace cl;
+
+extern "C" int cl_adamw_workspace(int64_t num_tensors, int64_t* bytes) {
+    clear_error();
+    CL_ARG(bytes, "null pointer argument");
+    CL_ARG(num_tensors >= 0, "negative number of tensors");
+    // coefficients, and the norm's sums: kNormParts, and at most one more for each launch
+    *bytes = 8 * (kGroups * kCoefs + kNormParts + num_tensors);
+    return CL_OK;
+}
+
+extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors,
+                             int64_t num_groups, const cl_adamw_group* groups, double max_norm,
+                             double* step, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+    clear_error();
+    CL_ARG(num_tensors >= 0 && num_groups >= 0, "negative count");
+    CL_ARG(num_groups <= kGroups, "at most %d parameter groups", kGroups);
+    CL_ARG((num_tensors == 0 || tensors) && (num_groups == 0 || groups), "null pointer argument");
+    CL_ARG(step, "null step pointer");
+    Groups gs{};
+    gs.n = int(num_groups);
+    for (int i = 0; i < gs.n; ++i) {
+        const cl_adamw_group& g = groups[i];
+        CL_ARG(g.lr >= 0 && g.beta1 >= 0 && g.beta1 < 1 && g.beta2 >= 0 && g.beta2 < 1 &&
+                   g.eps >= 0 && g.weight_decay >= 0,
+               "invalid AdamW hyper-parameters");
+        gs.lr[i] = g.lr;
+        gs.b1[i] = g.beta1;
+        gs.b2[i] = g.beta2;
+        gs.eps[i] = g.eps;
+        gs.decay[i] = g.weight_decay;
+    }
+    int64_t all = 0;
+    for (int64_t i = 0; i < num_tensors; ++i) {
+        if (int rc = check_tensor(tensors[i], i, num_groups, false)) return rc;
+        all += ceil_div(tensors[i].numel, kTile);
+    }
+    int64_t need = 0;
+    if (int rc = cl_adamw_workspace(num_tensors, &need)) return rc;
+    CL_ARG(workspace && workspace_bytes >= need, "workspace of %lld bytes needed (cl_adamw_workspace)",
+           (long long)need);
+    CL_ARG(aligned(workspace, 8), "workspace must be aligned to 8 bytes");
+    hipStream_t s = as_stream(stream);
+    double* coefs = static_cast<double*>(workspace);
+    double* parts = coefs + kGroups * kCoefs;
+    int64_t nparts = 0;
+    bool begun = false;
+    auto begin = [&](int kind, const Grads& g, unsigned grid) -> int {
+        Groups now = gs;
+        if (begun) now.n = 0;
+        begun = true;
+        CL_STORAGE_SWITCH(kind, {
+            k_adamw_begin<scalar_t><<<grid, kOptThreads, 0, s>>>(g, parts + nparts, now, step, coefs);
+        });
+        return check_launch("cl_adamw_step(begin)");
+    };
+    if (gs.n == 0) gs.n = 1;  // the kernel counts the step along with the first group
+    if (max_norm > 0 && all > 0) {
+        const int rc = each_batch(tensors, num_tensors, Alike::kDtype, [&](int kind, const Batch& b) -> int {
+            const int64_t grid = norm_parts(b.tiles, all);
+            if (int r = begin(kind, b.grads(), unsigned(grid))) return r;
+            nparts += grid;
+            return CL_OK;
+        });
+        if (rc) return rc;
+    } else {
+        Grads none{};
+        if (int rc = begin(CL_DTYPE_F32, none, 1)) return rc;
+    }
+    return each_batch(tensors, num_tensors, Alike::kDtypeAndBits, [&](int kind, const Batch& b) -> int {
+        const dim3 grid = b.grid();
+        CL_STORAGE_SWITCH(kind & 3, {
+            if (kind < 4) {
+                k_adamw<scalar_t><<<grid, kOptThreads, 0, s>>>(b.ts, parts, int(nparts), max_norm, coefs);
+            } else if constexpr (!std::is_same_v<scalar_t, double>) {
+                k_adamw8<scalar_t><<<grid, kOptThreads, 0, s>>>(b.ts, parts, int(nparts), max_norm, coefs);
+            }
+        });
+        return check_launch("cl_adamw_step");
+    });
+}
+
+namespace {
+
+int moments(const char* what, bool read, int64_t num_tensors, const cl_adamw_tensor* tensors,
+            void* stream) {
+    clear_error();
+    CL_ARG(num_tensors >= 0, "negative count");
+    CL_ARG(num_tensors == 0 || tensors, "null pointer argument");
+    for (int64_t i = 0; i < num_tensors; ++i)
+        if (int rc = check_tensor(tensors[i], i, 0, true)) return rc;
+    hipStream_t s = as_stream(stream);
+    return each_batch(tensors, num_tensors, Alike::kAll, [&](int, const Batch& b) -> int {
+        if (read)
+            k_adamw8_read<<<b.grid(), kOptThreads, 0, s>>>(b.ts);
+        else
+            k_adamw8_write<<<b.grid(), kOptThreads, 0, s>>>(b.ts);
+        return check_launch(what);
+    });
+}
+
+}  // namespace
+
+extern "C" int cl_adamw_moments_read(int64_t num_tensors, const cl_adamw_tensor* tensors,
+                                     void* stream) {
+    return moments("cl_adamw_moments_read", true, num_tensors, tensors, stream);
+}
+
+extern "C" int cl_adamw_moments_write(int64_t num_tensors, const cl_adamw_tensor* tensors,
+                                      void* stream) {
+    return moments("cl_adamw_moments_write", false, num_tensors, tensors, stream);
+}

@@ -1,6 +1,6 @@
 // The autograd side of the losses on chosen log-probabilities and of dropout: what their calls
 // allocate, launch and save, and their backwards, over the entry points of
-// libcompactlogic_hip.so.
+// libcompactlogic_hip.so; and the walk over an optimizer's tensors.
 //
 // A small call's kernels take 6 to 15 us.  As Functions in Python such calls took 76 to 97 us, here
 // 45 to 62: autograd runs a backward on a thread of its own, and an interpreter on either side of
@@ -13,6 +13,7 @@
 #include <stdexcept>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "../../include/compactlogic_hip.h"
 #include "timed_hook.h"
@@ -513,6 +514,125 @@ Tensor dropout_next(const Tensor& rng) {
     return used;
 }
 
+// ---- one AdamW step over the parameters of an optimizer.  The walk over its groups and states is here
+// because a Python loop costs some 2 us a tensor, a small tensor's share of the kernels 0.1.
+
+[[noreturn]] void refuse(const std::string& text) { throw std::runtime_error("FusedAdamW " + text); }
+
+py::handle item_of(PyObject* dict, const char* name) {
+    PyObject* v = PyDict_GetItemString(dict, name);
+    return v ? v : Py_None;
+}
+
+// The state's tensor of that name as a kernel can take it (contiguous on the device, of the type and
+// shape), else null.
+const Tensor* held(PyObject* state, const char* name, const Tensor& p, at::ScalarType type,
+                   bool shaped) {
+    PyObject* v = PyDict_GetItemString(state, name);
+    if (!v || !THPVariable_Check(v)) return nullptr;
+    const Tensor& t = THPVariable_Unpack(v);
+    if (t.scalar_type() != type || t.device() != p.device() || !t.is_contiguous() ||
+        (shaped ? t.sizes() != p.sizes() : t.numel() != 2 * ((p.numel() + 255) / 256)))
+        return nullptr;
+    return &t;
+}
+
+// The parameter's moments in `out`; false where the state has none that fit.
+bool moments_of(const Tensor& p, PyObject* state, int bits, cl_adamw_tensor& out) {
+    const bool small = bits == 8;
+    const at::ScalarType wide = p.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
+    const Tensor* m = held(state, "exp_avg", p, small ? at::kFloat8_e4m3fn : wide, true);
+    const Tensor* v = held(state, "exp_avg_sq", p, small ? at::kByte : wide, true);
+    const Tensor* e = small ? held(state, "exponents", p, at::kByte, false) : nullptr;
+    if (!m || !v || (small && !e)) return false;
+    out.exp_avg = m->data_ptr();
+    out.exp_avg_sq = v->data_ptr();
+    out.powers = small ? static_cast<uint8_t*>(e->data_ptr()) : nullptr;
+    out.numel = p.numel();
+    out.bits = bits;
+    return true;
+}
+
+// False, with nothing done, where a parameter with a gradient has no moments yet.
+bool adamw_step(const py::list& param_groups, const py::dict& states, const Tensor& step,
+                double max_norm) {
+    const at::NoGradGuard no_grad;
+    const c10::Device device = step.device();
+    std::vector<cl_adamw_tensor> tensors;
+    std::vector<cl_adamw_group> groups;
+    std::vector<Tensor> copies;  // of gradients that are not contiguous
+    std::vector<at::TensorImpl*> stepped;
+    for (const py::handle group : param_groups) {
+        const auto betas = py::cast<py::sequence>(item_of(group.ptr(), "betas"));
+        const int bits = py::cast<int>(item_of(group.ptr(), "state_bits"));
+        const int64_t first = int64_t(tensors.size());
+        for (const py::handle item : py::cast<py::list>(item_of(group.ptr(), "params"))) {
+            const Tensor& p = THPVariable_Unpack(item.ptr());
+            const Tensor& grad = p.grad();
+            if (!grad.defined()) continue;
+            if (grad.layout() != at::kStrided) refuse("does not support sparse gradients");
+            if (p.device() != device) refuse("needs all parameters on one HIP device");
+            if (!p.is_contiguous()) refuse("needs contiguous parameters");
+            if (grad.scalar_type() != p.scalar_type() || grad.device() != device ||
+                grad.sizes() != p.sizes())
+                refuse("needs gradients of the parameters' dtype, shape and device");
+            PyObject* state = PyDict_GetItem(states.ptr(), item.ptr());
+            cl_adamw_tensor t{};
+            if (!state || !moments_of(p, state, bits, t)) return false;
+            t.param = p.data_ptr();
+            if (grad.is_contiguous()) {
+                t.grad = grad.data_ptr();
+            } else {
+                copies.push_back(grad.contiguous());
+                t.grad = copies.back().data_ptr();
+            }
+            t.dtype = code_of(p);
+            t.group = int(groups.size());
+            tensors.push_back(t);
+            stepped.push_back(p.unsafeGetTensorImpl());
+        }
+        if (int64_t(tensors.size()) == first) continue;
+        groups.push_back({py::cast<double>(item_of(group.ptr(), "lr")), py::cast<double>(betas[0]),
+                          py::cast<double>(betas[1]), py::cast<double>(item_of(group.ptr(), "eps")),
+                          py::cast<double>(item_of(group.ptr(), "weight_decay"))});
+    }
+    if (tensors.empty()) return true;
+    const c10::DeviceGuard guard(device);
+    int64_t need = 0;
+    sized("cl_adamw_workspace", cl_adamw_workspace(int64_t(tensors.size()), &need));
+    const Tensor ws = at::empty({need}, step.options().dtype(at::kByte));
+    launch("cl_adamw_step", device.index(), [&](void* stream) {
+        return cl_adamw_step(int64_t(tensors.size()), tensors.data(), int64_t(groups.size()),
+                             groups.data(), max_norm, static_cast<double*>(step.data_ptr()),
+                             ws.data_ptr(), need, stream);
+    });
+    for (at::TensorImpl* p : stepped)
+        if (!p->is_inference()) p->bump_version();  // autograd: what it saved of them is another now
+    return true;
+}
+
+// 8-bit moments of each parameter from (write) or to the tensors of `first` and `second`.
+void adamw_moments(const std::vector<Tensor>& params, const py::list& states,
+                   const std::vector<Tensor>& first, const std::vector<Tensor>& second, bool write) {
+    if (params.empty()) return;
+    const c10::DeviceGuard guard(params[0].device());
+    std::vector<cl_adamw_tensor> tensors;
+    for (size_t i = 0; i < params.size(); ++i) {
+        cl_adamw_tensor t{};
+        if (params[i].device() != params[0].device() ||
+            !moments_of(params[i], states[i].ptr(), 8, t))
+            refuse("has no moments in 8 bits for a parameter");
+        t.param = first[i].data_ptr();
+        t.grad = second[i].data_ptr();
+        tensors.push_back(t);
+    }
+    launch(write ? "cl_adamw_moments_write" : "cl_adamw_moments_read", params[0].get_device(),
+           [&](void* stream) {
+               return (write ? cl_adamw_moments_write : cl_adamw_moments_read)(
+                   int64_t(tensors.size()), tensors.data(), stream);
+           });
+}
+
 void set_timed(py::object timed) { g_timed.set(std::move(timed)); }
 
 }  // namespace
@@ -524,6 +644,8 @@ PYBIND11_MODULE(_autograd, m) {
     m.def("preference_loss", &preference_loss, unlocked());
     m.def("dropout", &dropout, unlocked());
     m.def("dropout_next", &dropout_next, unlocked());
+    m.def("adamw_step", &adamw_step);
+    m.def("adamw_moments", &adamw_moments);
     m.def("set_timed", &set_timed);
     m.attr("torch_version") = TORCH_VERSION;
 }

@@ -14,7 +14,7 @@ update is bitwise reproducible.
 
 Differences from torch.optim.Adam: every parameter of the optimizer shares one step count,
 which advances on every call (torch advances a parameter's count only when it has a
-gradient); weight decay, amsgrad and maximize are not supported.  State dicts interchange
+gradient); amsgrad and maximize are not supported, weight decay by `FusedAdamW` alone.  State dicts interchange
 with torch.optim.Adam's: ``state_dict()`` gives each parameter its step as a float32 host
 scalar, as Adam keeps it, and after ``load_state_dict`` the shared count resumes from the
 loaded steps (which must agree), so the bias corrections continue where they stopped.
@@ -25,12 +25,60 @@ import ctypes
 
 import torch
 
-from . import _capi
+from . import _capi, _native
 from . import difflogic_hip as _dl
 from . import timing
 
 
-class FusedAdam(torch.optim.Optimizer):
+class _OneCount(torch.optim.Optimizer):
+    """An optimizer whose parameters share one step count, a device tensor."""
+
+    _step_t = None
+
+    def _loaded_step(self) -> float:
+        """The step count held in the state (after load_state_dict, one of torch's Adam
+        optimizers or of these): equal for every parameter that has one, else an error; 0 when
+        no parameter has one yet."""
+        steps = set()
+        for p, _ in self._params():
+            st = self.state.get(p, {})
+            if "step" in st:
+                v = st["step"]
+                steps.add(float(v.item() if torch.is_tensor(v) else v))
+        if len(steps) > 1:
+            raise RuntimeError(f"{type(self).__name__} shares one step count, but the loaded state holds "
+                               f"several: {sorted(steps)}")
+        return steps.pop() if steps else 0.0
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the shared count is taken from the loaded per-parameter steps at the next step()
+        self._step_t = None
+
+    def state_dict(self):
+        """torch.optim.Adam's layout: per-parameter step as a float32 host scalar."""
+        sd = super().state_dict()
+        state, counts = {}, {}
+        for k, st in sd["state"].items():
+            st = dict(st)
+            t = st.get("step")
+            if torch.is_tensor(t):
+                if id(t) not in counts:      # the parameters share one
+                    counts[id(t)] = float(t.item())
+                st["step"] = torch.tensor(counts[id(t)], dtype=torch.float32)
+            state[k] = st
+        sd["state"] = state
+        return sd
+
+    def _params(self):
+        out = []
+        for group in self.param_groups:
+            for p in group["params"]:
+                out.append((p, group))
+        return out
+
+
+class FusedAdam(_OneCount):
     """clip_grad_norm_(params, max_norm) followed by Adam(lr, betas, eps), fused.
 
     ``max_norm=None`` (or <= 0) skips the clipping.  All parameters must be HIP tensors of one
@@ -45,45 +93,6 @@ class FusedAdam(torch.optim.Optimizer):
         self.max_norm = max_norm
         self._step_t = None     # shared device step count
         self._workspace = None
-
-    def _loaded_step(self) -> float:
-        """The step count held in the state (after load_state_dict, a torch.optim.Adam or a
-        FusedAdam state dict): equal for every parameter that has one, else an error; 0 when
-        no parameter has one yet."""
-        steps = set()
-        for p, _ in self._params():
-            st = self.state.get(p, {})
-            if "step" in st:
-                v = st["step"]
-                steps.add(float(v.item() if torch.is_tensor(v) else v))
-        if len(steps) > 1:
-            raise RuntimeError(f"FusedAdam shares one step count, but the loaded state holds "
-                               f"several: {sorted(steps)}")
-        return steps.pop() if steps else 0.0
-
-    def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
-        # the shared count is taken from the loaded per-parameter steps at the next step()
-        self._step_t = None
-
-    def state_dict(self):
-        """torch.optim.Adam's layout: per-parameter step as a float32 host scalar."""
-        sd = super().state_dict()
-        state = {}
-        for k, st in sd["state"].items():
-            st = dict(st)
-            if "step" in st and torch.is_tensor(st["step"]):
-                st["step"] = torch.tensor(float(st["step"].item()), dtype=torch.float32)
-            state[k] = st
-        sd["state"] = state
-        return sd
-
-    def _params(self):
-        out = []
-        for group in self.param_groups:
-            for p in group["params"]:
-                out.append((p, group))
-        return out
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -151,3 +160,170 @@ class FusedAdam(torch.optim.Optimizer):
                 float(lr), float(beta1), float(beta2), float(eps), max_norm,
                 self._workspace.data_ptr(), self._workspace.numel(), _dl.stream_of(p0)))
         return loss
+
+
+class FusedAdamW(_OneCount):
+    """clip_grad_norm_(params, max_norm) followed by AdamW(lr, betas, eps, weight_decay) over any
+    number of tensors of any of float32, float64, float16 and bfloat16, fused (cl_adamw_step).
+
+    Arithmetic is float32 (float64 for float64 parameters), a parameter of 16 bits is rounded once.
+    state_bits=32 holds the moments in that wide type.  state_bits=8 holds them in a byte each, with
+    two more for 256 elements (float64 parameters have none): ``exp_avg`` float8_e4m3fn,
+    ``exp_avg_sq`` uint8 codes and the blocks' ``exponents``; `moments` gives their values.  The
+    update itself takes the new moments before they are rounded to 8 bits.
+
+    lr, betas, eps, weight_decay and state_bits may differ between parameter groups (at most 32);
+    ``max_norm`` is one for all, on the norm over all of them (float64 sums in a fixed order: steps
+    are bitwise reproducible); None or <= 0 skips the clipping.  The gradients are left as they are:
+    unlike clip_grad_norm_ and FusedAdam, ``p.grad`` is not scaled.  Where it holds infinities or NaN
+    the step follows the formulas (an infinite norm scales finite gradients to 0).
+
+    State dicts interchange with torch.optim.AdamW's (of float32 moments for parameters of any type)
+    and between 32 and 8 bits.  Tensors that are of the type and on the device already are taken as
+    they are, without a copy."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, max_norm: float | None = 10.0, state_bits: int = 32):
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
+                                      weight_decay=weight_decay, state_bits=state_bits))
+        self.max_norm = max_norm
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm}
+
+    def add_param_group(self, param_group):
+        params = param_group["params"]
+        if not isinstance(params, torch.Tensor):
+            params = param_group["params"] = list(params)
+            if len({id(p) for p in params}) != len(params):
+                raise ValueError("a parameter group holds a parameter twice")
+        g = {**self.defaults, **param_group}
+        b1, b2 = g["betas"]
+        if not (g["lr"] >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0 and 0 <= b1 < 1
+                and 0 <= b2 < 1):
+            raise ValueError(f"invalid AdamW hyper-parameters lr={g['lr']} betas={g['betas']} "
+                             f"eps={g['eps']} weight_decay={g['weight_decay']}")
+        if g["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {g['state_bits']}")
+        super().add_param_group(param_group)
+
+    def load_state_dict(self, state_dict):
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise RuntimeError("FusedAdamW has no amsgrad and no maximize")
+        bits = [g["state_bits"] for g in self.param_groups]
+        super().load_state_dict(state_dict)
+        for group, n in zip(self.param_groups, bits):   # how moments are held stays as it was
+            group["state_bits"] = n
+        # torch has cast the moments to the parameters' types: take them as they were given
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        with torch.no_grad():
+            for i, (p, group) in zip(ids, self._params()):
+                given = state_dict["state"].get(i)
+                if given is not None and "exp_avg" in given:
+                    self._hold(p, group, {k: given[k] for k in
+                                          ("exp_avg", "exp_avg_sq", "exponents") if k in given})
+
+    def _hold(self, p, group, given):
+        """The parameter's moments in the form of its group, from given ones in either."""
+        small = group["state_bits"] == 8
+        st = self.state[p]
+        for name in ("exp_avg", "exp_avg_sq"):
+            if given[name].shape != p.shape:
+                raise RuntimeError(f"FusedAdamW state {name} has shape "
+                                   f"{tuple(given[name].shape)}, the parameter {tuple(p.shape)}")
+        given = {k: t.to(p.device).contiguous() for k, t in given.items()}
+        if small and p.dtype == torch.float64:
+            raise RuntimeError("FusedAdamW holds no moments of float64 parameters in 8 bits")
+        if ("exponents" in given) == small:
+            wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+            if small:
+                st.update(given)
+            else:
+                st.pop("exponents", None)
+                st.update({k: t.to(wide) for k, t in given.items()})
+        elif small:
+            _dl._check(p, "parameter")
+            self._empty_small(p, st)
+            _native.load().adamw_moments([p], [st], [given["exp_avg"].float()],
+                                         [given["exp_avg_sq"].float()], True)
+        else:
+            held = self._read_small([p], [given])
+            st.pop("exponents", None)
+            st["exp_avg"], st["exp_avg_sq"] = (t[0].float() for t in held)
+
+    @staticmethod
+    def _empty_small(p, st):
+        st["exp_avg"] = torch.zeros(p.shape, dtype=torch.uint8,
+                                    device=p.device).view(torch.float8_e4m3fn)
+        st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+        st["exponents"] = torch.ones(2 * (-(-p.numel() // 256)), dtype=torch.uint8, device=p.device)
+
+    @staticmethod
+    def _read_small(params, states):
+        first = [torch.empty(p.shape, dtype=torch.bfloat16, device=p.device) for p in params]
+        second = [torch.empty_like(t) for t in first]
+        _native.load().adamw_moments(params, states, first, second, False)
+        return first, second
+
+    def _prepare_states(self):
+        """Moments for the parameters that have a gradient and none yet, checked for the others."""
+        for p, group in self._params():
+            if p.grad is None:
+                continue
+            _dl._check(p, "parameter")
+            _dl.storage_dtype_code(p)
+            st = self.state[p]
+            if "exp_avg" in st:
+                self._hold(p, group, {k: st[k] for k in ("exp_avg", "exp_avg_sq", "exponents")
+                                      if k in st})
+            elif group["state_bits"] == 8:
+                if p.dtype == torch.float64:
+                    raise RuntimeError("FusedAdamW holds no moments of float64 parameters in 8 bits")
+                self._empty_small(p, st)
+            else:
+                wide = torch.float64 if p.dtype == torch.float64 else torch.float32
+                for name in ("exp_avg", "exp_avg_sq"):
+                    st[name] = torch.zeros(p.shape, dtype=wide, device=p.device)
+            st["step"] = self._step_t
+
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        native = _native.load()
+        max_norm = float(self.max_norm) if self.max_norm is not None else 0.0
+        if self._step_t is None:
+            first = next((p for p, _ in self._params() if p.grad is not None), None)
+            if first is None:
+                return loss
+            _dl._check(first, "parameter")
+            self._step_t = torch.full((), self._loaded_step(), dtype=torch.float64,
+                                      device=first.device)
+            for st in self.state.values():
+                st["step"] = self._step_t
+        if not native.adamw_step(self.param_groups, self.state, self._step_t, max_norm):
+            with torch.no_grad():
+                self._prepare_states()
+            if not native.adamw_step(self.param_groups, self.state, self._step_t, max_norm):
+                raise RuntimeError("FusedAdamW's state does not fit its parameters")
+        return loss
+
+    @torch.no_grad()
+    def moments(self, params=None):
+        """(first, second): lists of the exponential averages of the gradient and of its square of
+        `params` (default: every parameter that has them), in float32 (float64) where they are held
+        in 32 bits and in bfloat16, which holds all of their values, where in 8."""
+        params = [p for p, _ in self._params() if "exp_avg" in self.state.get(p, {})] \
+            if params is None else list(params)
+        states = [self.state.get(p, {}) for p in params]
+        for st in states:
+            if "exp_avg" not in st:
+                raise RuntimeError("a parameter has no moments before its first step")
+        first, second = [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
+        small = [i for i, st in enumerate(states) if "exponents" in st]
+        if small:
+            held = self._read_small([params[i] for i in small], [states[i] for i in small])
+            for i, m, v in zip(small, *held):
+                first[i], second[i] = m, v
+        return first, second

@@ -43,7 +43,7 @@ extern "C" {
 #define CL_DTYPE_F32 0
 #define CL_DTYPE_F64 1
 #define CL_DTYPE_F16 2
-#define CL_DTYPE_BF16 3 /* the losses on chosen log-probabilities and cl_dropout */
+#define CL_DTYPE_BF16 3 /* the losses on chosen log-probabilities, cl_dropout, cl_adamw_* */
 
 #define CL_REDUCE_NONE 0
 #define CL_REDUCE_SUM 1
@@ -566,6 +566,53 @@ int cl_adam_clip_step(int dtype, int64_t num_tensors, void* const* params, void*
                       void* step, double lr, double beta1, double beta2, double eps,
                       double max_norm, void* workspace, int64_t workspace_elements,
                       void* stream);
+
+/* -------------------------------------------------------------------------------------------
+ * One AdamW step over any number of tensors (no reference counterpart).  With t = step[0] + 1,
+ * written back to step (a device fp64 scalar), and c = min(1, max_norm / (|g| + 1e-6)), |g| the norm
+ * over all tensors in fp64 (c = 1 where max_norm <= 0), per element
+ *   m = beta1 m + (1 - beta1) c g,  v = beta2 v + (1 - beta2) (c g)^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
+ * Gradients are not written.  The tensors' addresses travel in the kernels' arguments.
+ *
+ * param, grad: numel contiguous elements of dtype (F32, F64, F16, BF16), at any address that is a
+ * multiple of the element size.  bits 32: exp_avg, exp_avg_sq hold numel fp32 elements (fp64 for
+ * F64).  bits 8 (not for F64): they hold numel bytes, and powers 2 * ceil(numel / 256) bytes, the
+ * biased exponents (+127) of the blocks of 256 elements, exp_avg's and then exp_avg_sq's: exp_avg
+ * in e4m3 (OCP), the block's largest in [128, 256) times its power of two; exp_avg_sq as code c = 0
+ * for 0, 255 for NaN, else the fp32 number of bits (c + 770) << 20, the block's largest in [1, 2)
+ * times its power of two; exponents are at least -126, what is above 0 is at least code 1, what is
+ * not finite is NaN and does not count for its block.  Codes are rounded to nearest, ties to even.
+ * group: its hyper-parameters; at most 32 groups a call.  workspace: cl_adamw_workspace bytes, on
+ * 8 bytes.  Sums have a fixed order: bitwise reproducible.
+ *
+ * cl_adamw_moments_read gives back what 8 bits hold, in bf16 (exactly), exp_avg to param and
+ * exp_avg_sq to grad; cl_adamw_moments_write takes fp32 elements from param and grad into 8 bits
+ * (an exp_avg_sq below 0 becomes NaN).  Both go by the tensors' other fields, dtype and group unread.
+ * ----------------------------------------------------------------------------------------- */
+typedef struct {
+    void* param;
+    void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    uint8_t* powers;
+    int64_t numel;
+    int32_t dtype;
+    int32_t bits;
+    int32_t group;
+    int32_t reserved;
+} cl_adamw_tensor;
+
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay;
+} cl_adamw_group;
+
+int cl_adamw_workspace(int64_t num_tensors, int64_t* bytes);
+int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors, int64_t num_groups,
+                  const cl_adamw_group* groups, double max_norm, double* step, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int cl_adamw_moments_read(int64_t num_tensors, const cl_adamw_tensor* tensors, void* stream);
+int cl_adamw_moments_write(int64_t num_tensors, const cl_adamw_tensor* tensors, void* stream);
 
 /* -------------------------------------------------------------------------------------------
  * Losses on the log-probability of one chosen class or token per row of logits (GroupSum's
