@@ -20,6 +20,7 @@ from .optim import FusedAdam, FusedAdamW
 from .packed_net import PackedNetwork
 from .plan import RunPlan, build_run_plan
 from .policy import policy_loss, preference_loss, selected_log_probs
+from .recurrence import LogicRecurrence, gated_recurrence
 from .schedules import (EntropyRowResampler, FixedSequentialEntropyFreezer,
                         SequentialEntropyFreezer)
 from .treelogic import (ConvLogicFunction, ConvLogicLayer, FullConvLogicFunction,
@@ -35,4 +36,5 @@ __all__ = [
     "LogicGroupSumCrossEntropyFunction", "logic_group_sum_cross_entropy",
     "sequential_cross_entropy", "checkpoint", "circuit", "Dropout", "dropout",
     "policy_loss", "preference_loss", "selected_log_probs",
+    "LogicRecurrence", "gated_recurrence",
 ]

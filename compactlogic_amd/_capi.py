@@ -140,6 +140,10 @@ SIGNATURES: dict[str, list] = {
     "cl_adamw_step": [_i64, _p, _i64, _p, _f64, _p, _p, _i64, _p],
     "cl_adamw_moments_read": [_i64, _p, _p],
     "cl_adamw_moments_write": [_i64, _p, _p],
+    "cl_recurrence_sizes": [_int, _int, _i64, _i64, _i64, ctypes.POINTER(_i64),
+                            ctypes.POINTER(_i64)],
+    "cl_recurrence_forward": [_int, _int, _int] + [_p] * 6 + [_i64] * 3 + [_p] * 6 + [_i64, _p],
+    "cl_recurrence_backward": [_int, _int, _int] + [_p] * 11 + [_i64] * 3 + [_p] * 7 + [_i64, _p],
     "cl_token_loss_workspace": [_int, _i64, _i64, ctypes.POINTER(_i64)],
     "cl_selected_log_prob_forward": [_int, _p, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _i64, _p],
     "cl_selected_log_prob_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p],

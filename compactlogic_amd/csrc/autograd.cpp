@@ -1,11 +1,11 @@
-// The autograd side of the losses on chosen log-probabilities and of dropout: what their calls
-// allocate, launch and save, and their backwards, over the entry points of
+// The autograd side of the losses on chosen log-probabilities, of dropout and of the recurrence: what
+// their calls allocate, launch and save, and their backwards, over the entry points of
 // libcompactlogic_hip.so; and the walk over an optimizer's tensors.
 //
 // A small call's kernels take 6 to 15 us.  As Functions in Python such calls took 76 to 97 us, here
 // 45 to 62: autograd runs a backward on a thread of its own, and an interpreter on either side of
 // that hand-over costs 30 us more (torch's own negation, forward and backward, takes 45).
-// Arguments are checked in policy.py and dropout_layer.py; nothing here is a public interface.
+// Arguments are checked in policy.py, dropout_layer.py and recurrence.py; nothing here is a public interface.
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
@@ -468,7 +468,149 @@ struct Drop : Function<Drop> {
     }
 };
 
+// ---- the gated linear recurrence of [batch, time, features]: (y, last state).
+
+// What is contiguous in x, and the order of the rest (CL_RECURRENCE_*); -1: nothing that a kernel takes.
+int order_of(const Tensor& x) {
+    const int64_t batch = x.size(0), time = x.size(1), features = x.size(2);
+    if (features > 1 && x.stride(2) == 1) return CL_RECURRENCE_FEATURES;
+    if (time > 1)
+        return x.stride(1) != 1 ? -1
+               : x.stride(0) >= x.stride(2) ? CL_RECURRENCE_TIME_BATCH
+                                            : CL_RECURRENCE_TIME_FEATURES;
+    if (batch > 1) return x.stride(0) == 1 ? CL_RECURRENCE_BATCH : -1;
+    return features > 1 ? -1 : CL_RECURRENCE_FEATURES;
+}
+
+bool ordered(const Tensor& t, int order) {
+    const int d = order == CL_RECURRENCE_FEATURES ? 2 : order == CL_RECURRENCE_BATCH ? 0 : 1;
+    return t.size(d) <= 1 || t.stride(d) == 1;
+}
+
+bool features_outermost(int order) {
+    return order == CL_RECURRENCE_TIME_FEATURES || order == CL_RECURRENCE_BATCH;
+}
+
+Tensor sequence_like(const Tensor& x, int order) {
+    const int64_t batch = x.size(0), time = x.size(1), features = x.size(2);
+    if (order == CL_RECURRENCE_FEATURES) return at::empty({batch, time, features}, x.options());
+    if (order == CL_RECURRENCE_TIME_BATCH)
+        return at::empty_strided({batch, time, features}, {features * time, 1, time}, x.options());
+    return at::empty_strided({batch, time, features}, {time, 1, batch * time}, x.options());
+}
+
+Tensor state_like(const Tensor& x, int order) {
+    const int64_t batch = x.size(0), features = x.size(2);
+    if (!features_outermost(order)) return at::empty({batch, features}, wide_of(x));
+    return at::empty_strided({batch, features}, {1, batch}, wide_of(x));
+}
+
+Tensor in_order(const Tensor& t, int order) {
+    if (ordered(t, order)) return t;
+    return sequence_like(t, order).copy_(t);
+}
+
+const int64_t* strides_of(const Tensor& t) { return t.defined() ? t.strides().data() : nullptr; }
+void* data_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+struct Sizes {
+    int64_t starts = 0, workspace = 0;
+    Sizes(const Tensor& x, int order) {
+        sized("cl_recurrence_sizes", cl_recurrence_sizes(code_of(x), order, x.size(0), x.size(1),
+                                                         x.size(2), &starts, &workspace));
+    }
+    Tensor allocate(const Tensor& x) const {
+        return workspace ? at::empty({workspace}, x.options().dtype(at::kByte)) : Tensor();
+    }
+};
+
+struct Swept {
+    Tensor x, gate, y, last, starts;
+    int order;
+};
+
+Swept swept(const Tensor& input, const Tensor& gates, const Tensor& state, int form, bool keep) {
+    Swept r;
+    r.order = order_of(input);
+    r.x = input;
+    if (r.order < 0) {
+        r.x = input.contiguous();
+        r.order = order_of(r.x);
+    }
+    r.gate = in_order(gates, r.order);
+    r.y = sequence_like(r.x, r.order);
+    r.last = state_like(r.x, r.order);
+    const Sizes sizes(r.x, r.order);
+    if (keep && sizes.starts) r.starts = at::empty({sizes.starts}, r.last.options());
+    const Tensor ws = sizes.allocate(r.x);
+    launch("cl_recurrence_forward", r.x.get_device(), [&](void* stream) {
+        return cl_recurrence_forward(
+            code_of(r.x), r.order, form, r.x.data_ptr(), strides_of(r.x), r.gate.data_ptr(),
+            strides_of(r.gate), data_of(state), strides_of(state), r.x.size(0), r.x.size(1),
+            r.x.size(2), r.y.data_ptr(), strides_of(r.y), r.last.data_ptr(), strides_of(r.last),
+            data_of(r.starts), data_of(ws), sizes.workspace, stream);
+    });
+    return r;
+}
+
+struct Recurrence : Function<Recurrence> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate,
+                                 const c10::optional<Tensor>& given, int64_t form) {
+        const Tensor state = given.value_or(Tensor());
+        Swept r = swept(x, gate, state, int(form), true);
+        ctx->save_for_backward({r.x, r.gate, state, r.starts});
+        ctx->saved_data["form"] = form;
+        ctx->saved_data["order"] = int64_t(r.order);
+        ctx->set_materialize_grads(false);
+        return {r.y, r.last};
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        if (at::GradMode::is_enabled())
+            throw std::runtime_error("the gated recurrence cannot be differentiated twice");
+        if (!grads[0].defined() && !grads[1].defined())
+            return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const int form = int(ctx->saved_data["form"].toInt());
+        const int order = int(ctx->saved_data["order"].toInt());
+        const variable_list v = ctx->get_saved_variables();
+        const c10::DeviceGuard guard(v[0].device());
+        // (hooks on saved tensors may have moved them)
+        const Tensor x = in_order(v[0], order), gate = in_order(v[1], order), state = v[2];
+        const Tensor starts = v[3].defined() ? v[3].contiguous() : v[3];
+        const Tensor gy = grads[0].defined() ? in_order(grads[0], order) : grads[0];
+        const Tensor gl = grads[1];
+        Tensor gx, gg, gs;
+        if (ctx->needs_input_grad(0)) gx = sequence_like(x, order);
+        if (ctx->needs_input_grad(1)) gg = sequence_like(x, order);
+        if (state.defined() && ctx->needs_input_grad(2)) gs = state_like(x, order);
+        const Sizes sizes(x, order);
+        const Tensor ws = sizes.allocate(x);
+        launch("cl_recurrence_backward", x.get_device(), [&](void* stream) {
+            return cl_recurrence_backward(
+                code_of(x), order, form, x.data_ptr(), strides_of(x), gate.data_ptr(),
+                strides_of(gate), data_of(state), strides_of(state), data_of(starts), data_of(gy),
+                strides_of(gy), data_of(gl), strides_of(gl), x.size(0), x.size(1), x.size(2),
+                data_of(gx), strides_of(gx), data_of(gg), strides_of(gg), data_of(gs),
+                strides_of(gs), data_of(ws), sizes.workspace, stream);
+        });
+        return {gx, gg, gs, Tensor()};
+    }
+};
+
 // ---- what Python calls, with the arguments checked
+
+std::pair<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& gate,
+                                           const c10::optional<Tensor>& state, int64_t form) {
+    const c10::DeviceGuard guard(x.device());
+    const Tensor h0 = state.value_or(Tensor());
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || gate.requires_grad() || (h0.defined() && h0.requires_grad()))) {
+        variable_list r = Recurrence::apply(x, gate, state, form);
+        return {r[0], r[1]};
+    }
+    Swept r = swept(x, gate, h0, int(form), false);
+    return {r.y, r.last};
+}
 
 Tensor selected_log_probs(const Tensor& x, const Tensor& actions, int64_t ignore, int64_t k,
                           double tau) {
@@ -642,6 +784,7 @@ PYBIND11_MODULE(_autograd, m) {
     m.def("selected_log_probs", &selected_log_probs, unlocked());
     m.def("policy_loss", &policy_loss, unlocked());
     m.def("preference_loss", &preference_loss, unlocked());
+    m.def("gated_recurrence", &gated_recurrence, unlocked());
     m.def("dropout", &dropout, unlocked());
     m.def("dropout_next", &dropout_next, unlocked());
     m.def("adamw_step", &adamw_step);

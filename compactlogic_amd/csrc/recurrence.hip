@@ -1,0 +1,1133 @@
+// A gated linear recurrence over sequences, per batch entry and feature,
+//   h_t = g_t h_(t-1) + b_t,   b_t = (1 - g_t) x_t ("mix") or x_t ("add"),
+// and its gradients: with G_t = dy_t + c_t, c_(t-1) = g_t G_t (c of the last step: its state's gradient),
+//   dx_t = (1 - g_t) G_t or G_t,   dg_t = G_t (h_(t-1) - x_t) or G_t h_(t-1),   dh_(-1) = c_(-1).
+//
+// A run of steps is a map h -> a h + b, and two maps in a row are one: (a2 a1, a2 b1 + b2).  So a
+// workgroup takes a stretch of time at once: every thread the map of a few steps of its own, a scan
+// over the threads' maps, then each thread's steps again from the state it starts with.  Both sweeps
+// read the registers; memory is read once.  The backward goes through the stretches from the last one,
+// makes their states again from the state each one began with (which the forward leaves, one per
+// stretch) and scans the gradients' maps, c -> a c + q with the same a, the other way.
+//
+// A gate of exactly 0 drops what came before and one of exactly 1 leaves x unread, NaN and infinities
+// too: a * h is not formed where a is 0, and a product of gates that are not 0 is kept from becoming 0.
+//
+// Where there are too few sequences for the chip, time is cut into segments: a first pass finds the
+// map of each (reading everything once more), and every segment starts from the maps before it.
+//
+// Two layouts: features (or, for one step, the batch) contiguous, lanes beside each other; or time
+// contiguous, as a LogicLayer gives batch * time samples, lanes one after the other in time.
+// Arithmetic and states in fp32 (fp64 for fp64), each result rounded once.
+#include "storage.h"
+
+#include <algorithm>
+
+namespace cl {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxSegments = 64;
+
+__device__ __forceinline__ float least(float) { return 1.401298464324817e-45f; }
+__device__ __forceinline__ double least(double) { return 4.9406564584124654e-324; }
+
+// a h + b, h dropped by an a of 0
+template <typename A>
+__device__ __forceinline__ A apply(A a, A h, A b) {
+    return a == A(0) ? b : fma(a, h, b);
+}
+
+// A product of factors other than 0 that is not 0 either.
+template <typename A>
+__device__ __forceinline__ A kept_product(A a, A b) {
+    const A r = a * b;
+    return r == A(0) && a != A(0) && b != A(0) ? least(r) : r;
+}
+
+template <bool MIX, typename A>
+__device__ __forceinline__ A input_of(A g, A x) {
+    if constexpr (MIX)
+        return g == A(1) ? A(0) : (A(1) - g) * x;
+    else
+        return x;
+}
+
+// The map of consecutive steps.
+template <typename A>
+struct Map {
+    A a = A(1), b = A(0);
+    bool dropped = false;
+    __device__ __forceinline__ void then(A g, A in) {
+        b = apply(g, b, in);
+        a *= g;
+        dropped |= g == A(0);
+    }
+    __device__ __forceinline__ A factor() const {
+        return dropped ? A(0) : a == A(0) ? least(a) : a;
+    }
+};
+
+// The same of the gradients, from the last step to the first.
+template <typename A>
+__device__ __forceinline__ A back_of(A g, A whole) {
+    return g == A(0) ? A(0) : g * whole;
+}
+
+template <bool MIX, typename A>
+__device__ __forceinline__ void gradients(A g, A x, A before, A whole, A& gx, A& gg) {
+    if constexpr (MIX) {
+        gx = g == A(1) ? A(0) : (A(1) - g) * whole;
+        gg = whole * (before - x);
+    } else {
+        gx = whole;
+        gg = whole * before;
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_part(const T* p, int count, T fill) {
+    if (count >= N) return pload<T, N>(p);
+    Pack<T, N> r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r.v[e] = e < count ? p[e] : fill;
+    return r;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_part(T* p, const Pack<T, N>& r, int count) {
+    if (count >= N) {
+        pstore<T, N>(p, r);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N - 1; ++e)
+        if (e < count) p[e] = r.v[e];
+}
+
+// A tensor [outer, time, inner] by its strides, and states [outer, inner] by theirs.
+template <typename T>
+struct Seq {
+    T* p;
+    int64_t so, st, si;
+};
+
+template <typename A>
+struct States {
+    A* p;  // may be null
+    int64_t so, si;
+    __device__ __forceinline__ A& at(int64_t o, int64_t i) const { return p[o * so + i * si]; }
+};
+
+template <typename T>
+struct Args {
+    using A = wide_t<T>;
+    Seq<const T> x, g;
+    Seq<T> y;                // forward
+    Seq<const T> gy;         // backward; p may be null
+    Seq<T> gx, gg;           // p may be null
+    States<A> h0, last;      // last: the last state, or its gradient; h0: p may be null (0)
+    States<A> gh0;
+    A* starts;               // states at the stretches' starts [stretch, outer, inner]; may be null
+    A* maps;                 // [segment][a, b][outer, inner]; null: one segment
+    int64_t outer, time, inner;
+    int segments;
+    int64_t per_segment;     // stretches
+    FastDiv tiles, outers;   // rows: workgroups of an outer place, outer places
+    int64_t groups;
+};
+
+// ---------------------------------------------------------------- inner contiguous
+//
+// FL lanes of 16 bytes side by side, TG groups of C steps each one after the other: a stretch is
+// TG * C steps.  The groups' maps go through LDS; one thread per inner place scans them, 32 groups of
+// 8 steps taking some 600 cycles of the 11000 that their bytes take.
+template <typename T, int FL, int TG, int C>
+struct Tile {
+    using A = wide_t<T>;
+    static constexpr int VEC = wide_vec<T>();
+    static constexpr int NT = FL * TG;
+    static constexpr int PLACES = FL * VEC;
+    static constexpr int STRETCH = TG * C;
+    static constexpr int PER = (PLACES + NT - 1) / NT;  // places of a scanning thread
+
+    int fl, tg, count;
+    int64_t segment, o, i0, i;
+    bool live;
+
+    __device__ __forceinline__ Tile(const Args<T>& a) {
+        const int64_t group = group_index();
+        live = group < a.groups;
+        const uint32_t rest = fast_div(uint32_t(group), a.tiles);
+        segment = fast_div(rest, a.outers);
+        o = rest - uint32_t(segment) * a.outers.d;
+        i0 = int64_t(uint32_t(group) - rest * a.tiles.d) * PLACES;
+        fl = threadIdx.x % FL;
+        tg = threadIdx.x / FL;
+        i = i0 + fl * VEC;
+        const int64_t left = a.inner - i;
+        count = left >= VEC ? VEC : left > 0 ? int(left) : 0;
+    }
+    __device__ __forceinline__ bool scans(int p, int64_t inner) const {
+        return p < PLACES && i0 + p < inner;
+    }
+};
+
+// State that segment `segment` starts with, or the gradient that it ends with (from the other side).
+template <bool BACK, typename T>
+__device__ __forceinline__ wide_t<T> segment_start(const Args<T>& a, int64_t segment, int64_t o,
+                                                   int64_t i) {
+    using A = wide_t<T>;
+    const States<A>& from = BACK ? a.last : a.h0;
+    A h = from.p ? from.at(o, i) : A(0);
+    if (!a.maps) return h;
+    const int64_t n = a.outer * a.inner;
+    const A* m = a.maps + o * a.inner + i;
+    if constexpr (BACK) {
+        for (int64_t s = a.segments - 1; s > segment; --s) h = apply(m[2 * s * n], h, m[(2 * s + 1) * n]);
+    } else {
+        for (int64_t s = 0; s < segment; ++s) h = apply(m[2 * s * n], h, m[(2 * s + 1) * n]);
+    }
+    return h;
+}
+
+template <typename T, bool MIX, int FL, int TG, int C>
+__global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
+    using A = wide_t<T>;
+    using W = Tile<T, FL, TG, C>;
+    constexpr int VEC = W::VEC;
+    __shared__ A fac[2][TG][W::PLACES], sum[2][TG][W::PLACES];
+    const W w(a);
+    if (!w.live) return;
+    A carry[W::PER];
+#pragma unroll
+    for (int k = 0; k < W::PER; ++k) {
+        const int p = threadIdx.x + k * W::NT;
+        carry[k] = w.scans(p, a.inner) ? segment_start<false>(a, w.segment, w.o, w.i0 + p) : A(0);
+    }
+    const int64_t s0 = w.segment * a.per_segment;
+    const int64_t s1 = std::min((w.segment + 1) * a.per_segment,
+                                (a.time + W::STRETCH - 1) / W::STRETCH);
+    const T* x = a.x.p + w.o * a.x.so + w.i;
+    const T* g = a.g.p + w.o * a.g.so + w.i;
+    T* y = a.y.p + w.o * a.y.so + w.i;
+    Pack<T, VEC> xs[C], gs[C];
+    auto load = [&](int64_t s) {
+        const int64_t t = s * W::STRETCH + w.tg * C;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int count = t + c < a.time ? w.count : 0;
+            xs[c] = load_part<T, VEC>(x + (t + c) * a.x.st, count, T(0));
+            gs[c] = load_part<T, VEC>(g + (t + c) * a.g.st, count, T(1));
+        }
+    };
+    int buf = 0;
+    for (int64_t s = s0; s < s1; ++s, buf ^= 1) {
+        load(s);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            Map<A> m;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const A gate = A(gs[c].v[e]);
+                m.then(gate, input_of<MIX>(gate, A(xs[c].v[e])));
+            }
+            fac[buf][w.tg][w.fl * VEC + e] = m.factor();
+            sum[buf][w.tg][w.fl * VEC + e] = m.b;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < W::PER; ++k) {
+            const int p = threadIdx.x + k * W::NT;
+            if (p >= W::PLACES) continue;
+            if (a.starts && w.scans(p, a.inner))
+                a.starts[(s * a.outer + w.o) * a.inner + w.i0 + p] = carry[k];
+            A h = carry[k];
+#pragma unroll
+            for (int q = 0; q < TG; ++q) {
+                const A f = fac[buf][q][p], b = sum[buf][q][p];
+                sum[buf][q][p] = h;
+                h = apply(f, h, b);
+            }
+            carry[k] = h;
+        }
+        __syncthreads();
+        A h[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[e] = sum[buf][w.tg][w.fl * VEC + e];
+        const int64_t t = s * W::STRETCH + w.tg * C;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            Pack<T, VEC> out;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs[c].v[e]);
+                h[e] = apply(gate, h[e], input_of<MIX>(gate, A(xs[c].v[e])));
+                out.v[e] = T(h[e]);
+            }
+            if (t + c < a.time) store_part<T, VEC>(y + (t + c) * a.y.st, out, w.count);
+        }
+    }
+    if (w.segment == a.segments - 1) {
+#pragma unroll
+        for (int k = 0; k < W::PER; ++k) {
+            const int p = threadIdx.x + k * W::NT;
+            if (w.scans(p, a.inner)) a.last.at(w.o, w.i0 + p) = carry[k];
+        }
+    }
+}
+
+template <typename T, bool MIX, int FL, int TG, int C>
+__global__ __launch_bounds__(FL * TG) void k_rows_backward(Args<T> a) {
+    using A = wide_t<T>;
+    using W = Tile<T, FL, TG, C>;
+    constexpr int VEC = W::VEC;
+    __shared__ A fac[2][TG][W::PLACES], sum[2][TG][W::PLACES], back[2][TG][W::PLACES];
+    const W w(a);
+    if (!w.live) return;
+    // the states by the first threads, the gradients by the last ones
+    const int rev = W::NT - 1 - int(threadIdx.x);
+    A carry[W::PER];
+#pragma unroll
+    for (int k = 0; k < W::PER; ++k) {
+        const int p = rev + k * W::NT;
+        carry[k] = w.scans(p, a.inner) ? segment_start<true>(a, w.segment, w.o, w.i0 + p) : A(0);
+    }
+    const int64_t s0 = w.segment * a.per_segment;
+    const int64_t s1 = std::min((w.segment + 1) * a.per_segment,
+                                (a.time + W::STRETCH - 1) / W::STRETCH);
+    const T* x = a.x.p + w.o * a.x.so + w.i;
+    const T* g = a.g.p + w.o * a.g.so + w.i;
+    const T* gy = a.gy.p + w.o * a.gy.so + w.i;
+    T* gx = a.gx.p + w.o * a.gx.so + w.i;
+    T* gg = a.gg.p + w.o * a.gg.so + w.i;
+    int buf = 0;
+    for (int64_t s = s1 - 1; s >= s0; --s, buf ^= 1) {
+        const int64_t t = s * W::STRETCH + w.tg * C;
+        Pack<T, VEC> xs[C], gs[C], ds[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int count = t + c < a.time ? w.count : 0;
+            xs[c] = load_part<T, VEC>(x + (t + c) * a.x.st, count, T(0));
+            gs[c] = load_part<T, VEC>(g + (t + c) * a.g.st, count, T(1));
+            ds[c] = load_part<T, VEC>(gy + (t + c) * a.gy.st, a.gy.p ? count : 0, T(0));
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            Map<A> m;
+            A q = A(0);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const A gate = A(gs[c].v[e]);
+                m.then(gate, input_of<MIX>(gate, A(xs[c].v[e])));
+            }
+#pragma unroll
+            for (int c = C - 1; c >= 0; --c) q = back_of(A(gs[c].v[e]), A(ds[c].v[e]) + q);
+            fac[buf][w.tg][w.fl * VEC + e] = m.factor();
+            sum[buf][w.tg][w.fl * VEC + e] = m.b;
+            back[buf][w.tg][w.fl * VEC + e] = q;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < W::PER; ++k) {
+            const int p = threadIdx.x + k * W::NT;
+            if (p < W::PLACES) {
+                A h = A(0);
+                if (w.scans(p, a.inner)) {
+                    if (a.starts)
+                        h = a.starts[(s * a.outer + w.o) * a.inner + w.i0 + p];
+                    else if (a.h0.p)
+                        h = a.h0.at(w.o, w.i0 + p);
+                }
+#pragma unroll
+                for (int q = 0; q < TG; ++q) {
+                    const A f = fac[buf][q][p], b = sum[buf][q][p];
+                    sum[buf][q][p] = h;
+                    h = apply(f, h, b);
+                }
+            }
+            const int r = rev + k * W::NT;
+            if (r < W::PLACES) {
+                A c = carry[k];
+#pragma unroll
+                for (int q = TG - 1; q >= 0; --q) {
+                    const A f = fac[buf][q][r], b = back[buf][q][r];
+                    back[buf][q][r] = c;
+                    c = apply(f, c, b);
+                }
+                carry[k] = c;
+            }
+        }
+        __syncthreads();
+        A before[C][VEC], c_in[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            A h = sum[buf][w.tg][w.fl * VEC + e];
+            c_in[e] = back[buf][w.tg][w.fl * VEC + e];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                before[c][e] = h;
+                const A gate = A(gs[c].v[e]);
+                h = apply(gate, h, input_of<MIX>(gate, A(xs[c].v[e])));
+            }
+        }
+#pragma unroll
+        for (int c = C - 1; c >= 0; --c) {
+            Pack<T, VEC> ox, og;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs[c].v[e]), whole = A(ds[c].v[e]) + c_in[e];
+                A dx, dg;
+                gradients<MIX>(gate, A(xs[c].v[e]), before[c][e], whole, dx, dg);
+                ox.v[e] = T(dx);
+                og.v[e] = T(dg);
+                c_in[e] = back_of(gate, whole);
+            }
+            if (t + c < a.time) {
+                if (a.gx.p) store_part<T, VEC>(gx + (t + c) * a.gx.st, ox, w.count);
+                if (a.gg.p) store_part<T, VEC>(gg + (t + c) * a.gg.st, og, w.count);
+            }
+        }
+    }
+    if (w.segment == 0 && a.gh0.p) {
+#pragma unroll
+        for (int k = 0; k < W::PER; ++k) {
+            const int p = rev + k * W::NT;
+            if (w.scans(p, a.inner)) a.gh0.at(w.o, w.i0 + p) = carry[k];
+        }
+    }
+}
+
+// The map of each segment: a group's steps lie one behind the other here.
+template <typename T, bool MIX, bool BACK, int FL, int TG>
+__global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
+    using A = wide_t<T>;
+    using W = Tile<T, FL, TG, 1>;
+    constexpr int VEC = W::VEC, U = 8;
+    __shared__ A fac[TG][W::PLACES], sum[TG][W::PLACES];
+    const W w(a);
+    if (!w.live) return;
+    const int64_t t0 = w.segment * a.per_segment * stretch;
+    const int64_t t1 = std::min(a.time, t0 + a.per_segment * stretch);
+    const int64_t each = (t1 - t0 + TG - 1) / TG;
+    const int64_t b0 = std::min(t1, t0 + w.tg * each), b1 = std::min(t1, b0 + each);
+    const T* g = a.g.p + w.o * a.g.so + w.i;
+    const Seq<const T>& in = BACK ? a.gy : a.x;
+    const T* d = in.p + w.o * in.so + w.i;
+    const bool some = !BACK || in.p;
+    Map<A> m[VEC];
+    for (int64_t n = 0; n < b1 - b0; n += U) {
+        Pack<T, VEC> gs[U], ds[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t t = BACK ? b1 - 1 - n - u : b0 + n + u;
+            const int count = n + u < b1 - b0 ? w.count : 0;
+            gs[u] = load_part<T, VEC>(g + t * a.g.st, count, T(1));
+            ds[u] = load_part<T, VEC>(d + t * in.st, some ? count : 0, T(0));
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs[u].v[e]), v = A(ds[u].v[e]);
+                if constexpr (BACK) {
+                    m[e].b = back_of(gate, v + m[e].b);
+                    m[e].a *= gate;
+                    m[e].dropped |= gate == A(0);
+                } else {
+                    m[e].then(gate, input_of<MIX>(gate, v));
+                }
+            }
+        // a product of many gates: kept from 0 now and then
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (m[e].a == A(0) && !m[e].dropped) m[e].a = least(m[e].a);
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        fac[w.tg][w.fl * VEC + e] = m[e].factor();
+        sum[w.tg][w.fl * VEC + e] = m[e].b;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W::PER; ++k) {
+        const int p = threadIdx.x + k * W::NT;
+        if (!w.scans(p, a.inner)) continue;
+        A f = A(1), b = A(0);
+        for (int q = 0; q < TG; ++q) {
+            const int r = BACK ? TG - 1 - q : q;
+            b = apply(fac[r][p], b, sum[r][p]);
+            f = kept_product(f, fac[r][p]);
+        }
+        const int64_t n = a.outer * a.inner;
+        A* to = a.maps + 2 * w.segment * n + w.o * a.inner + w.i0 + p;
+        to[0] = f;
+        to[n] = b;
+    }
+}
+
+// A few steps: a thread walks through them, VEC places side by side.
+template <typename T, bool MIX, bool BACK>
+__global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
+    using A = wide_t<T>;
+    using W = Tile<T, kThreads, 1, 1>;
+    constexpr int VEC = W::VEC;
+    // the threads of a workgroup go on to the next outer place where a row has fewer lanes
+    const int64_t lanes = (a.inner + VEC - 1) / VEC;
+    const int64_t item = group_index() * kThreads + threadIdx.x;
+    if (item >= a.outer * lanes) return;
+    int64_t o, lane;
+    if (a.outer * lanes < (int64_t(1) << 31)) {
+        o = fast_div(uint32_t(item), a.tiles);
+        lane = uint32_t(item) - uint32_t(o) * a.tiles.d;
+    } else {
+        o = item / lanes;
+        lane = item - o * lanes;
+    }
+    const int64_t i = lane * VEC;
+    const int count = int(std::min<int64_t>(VEC, a.inner - i));
+    auto states = [&](const States<A>& s, A (&h)[VEC]) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) h[e] = s.p && e < count ? s.at(o, i + e) : A(0);
+    };
+    auto put = [&](const States<A>& s, const A (&h)[VEC]) {
+        if (!s.p) return;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e < count) s.at(o, i + e) = h[e];
+    };
+    auto from = [&](const Seq<const T>& s, int64_t t, T fill) {
+        return load_part<T, VEC>(s.p + o * s.so + t * s.st + i, s.p ? count : 0, fill);
+    };
+    if constexpr (!BACK) {
+        A h[VEC];
+        Pack<T, VEC> xs = from(a.x, 0, T(0)), gs = from(a.g, 0, T(0));
+        states(a.h0, h);
+        for (int64_t t = 0; t < a.time; ++t) {
+            Pack<T, VEC> out;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs.v[e]);
+                h[e] = apply(gate, h[e], input_of<MIX>(gate, A(xs.v[e])));
+                out.v[e] = T(h[e]);
+            }
+            store_part<T, VEC>(a.y.p + o * a.y.so + t * a.y.st + i, out, count);
+            if (t + 1 < a.time) {
+                xs = from(a.x, t + 1, T(0));
+                gs = from(a.g, t + 1, T(0));
+            }
+        }
+        put(a.last, h);
+    } else {
+        constexpr int MOST = 2;  // kFew
+        A before[MOST][VEC], c[VEC];
+        Pack<T, VEC> xs[MOST], gs[MOST], ds[MOST];
+#pragma unroll
+        for (int t = 0; t < MOST; ++t)
+            if (t < a.time) {
+                xs[t] = from(a.x, t, T(0));
+                gs[t] = from(a.g, t, T(0));
+                ds[t] = from(a.gy, t, T(0));
+            }
+        states(a.h0, before[0]);
+        states(a.last, c);
+        if (a.time > 1) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs[0].v[e]);
+                before[1][e] = apply(gate, before[0][e], input_of<MIX>(gate, A(xs[0].v[e])));
+            }
+        }
+#pragma unroll
+        for (int t = MOST - 1; t >= 0; --t) {
+            if (t >= a.time) continue;
+            Pack<T, VEC> ox, og;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs[t].v[e]), whole = A(ds[t].v[e]) + c[e];
+                A dx, dg;
+                gradients<MIX>(gate, A(xs[t].v[e]), before[t][e], whole, dx, dg);
+                ox.v[e] = T(dx);
+                og.v[e] = T(dg);
+                c[e] = back_of(gate, whole);
+            }
+            if (a.gx.p) store_part<T, VEC>(a.gx.p + o * a.gx.so + t * a.gx.st + i, ox, count);
+            if (a.gg.p) store_part<T, VEC>(a.gg.p + o * a.gg.so + t * a.gg.st + i, og, count);
+        }
+        put(a.gh0, c);
+    }
+}
+constexpr int64_t kFew = 2;
+
+// ---------------------------------------------------------------- time contiguous
+//
+// L lanes of 16 bytes of one sequence one after the other: a stretch is L * VEC steps, scanned across
+// the lanes; 64 lanes for long sequences, which go through their stretches one by one, 16 or 4 where
+// one stretch of those is enough.
+
+// The value k lanes before (after: BACK) in the 16 lanes of a DPP row, `none` where there is none.
+template <bool BACK, int K, typename A>
+__device__ __forceinline__ A beside(A v, A none) {
+    constexpr int ctrl = (BACK ? 0x100 : 0x110) | K;  // row_shl / row_shr
+    if constexpr (sizeof(A) == 4) {
+        return __builtin_bit_cast(
+            A, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                           ctrl, 0xF, 0xF, false));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v), n = __builtin_bit_cast(uint64_t, none);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(int(uint32_t(n)), int(uint32_t(u)), ctrl, 0xF,
+                                                        0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(int(uint32_t(n >> 32)), int(uint32_t(u >> 32)),
+                                                        ctrl, 0xF, 0xF, false);
+        return __builtin_bit_cast(A, (uint64_t(hi) << 32) | lo);
+    }
+}
+
+template <int L, bool BACK, int K, typename A>
+__device__ __forceinline__ void scan_step(A& a, A& b, int l) {
+    A pa = beside<BACK, K>(a, A(1)), pb = beside<BACK, K>(b, A(0));
+    if constexpr (L < 16) {
+        const bool none = BACK ? l + K >= L : l < K;
+        if (none) {
+            pa = A(1);
+            pb = A(0);
+        }
+    }
+    b = apply(a, pb, b);
+    a = kept_product(pa, a);
+}
+
+// From the lanes' maps and the state `carry` that the stretch starts with (BACK: from its end), the
+// state that each lane starts with; carry becomes the one after the stretch where L is 64.
+template <int L, bool BACK, typename A>
+__device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
+    const int l = lane_id() & (L - 1);
+    scan_step<L, BACK, 1>(a, b, l);
+    scan_step<L, BACK, 2>(a, b, l);
+    if constexpr (L >= 16) {
+        scan_step<L, BACK, 4>(a, b, l);
+        scan_step<L, BACK, 8>(a, b, l);
+    }
+    A pa = beside<BACK, 1>(a, A(1)), pb = beside<BACK, 1>(b, A(0));
+    if constexpr (L < 16) {
+        if (BACK ? l + 1 >= L : l < 1) {
+            pa = A(1);
+            pb = A(0);
+        }
+    }
+    A from = carry;
+    if constexpr (L == 64) {
+        constexpr int ends[4] = {BACK ? 48 : 15, BACK ? 32 : 31, BACK ? 16 : 47, BACK ? 0 : 63};
+        const int row = BACK ? 3 - (l >> 4) : l >> 4;
+        A h = carry;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (r > 0 && row == r) from = h;
+            h = apply(read_lane(a, ends[r]), h, read_lane(b, ends[r]));
+        }
+        carry = h;
+    }
+    return apply(pa, from, pb);
+}
+
+template <typename T, int L>
+struct Line {
+    static constexpr int VEC = wide_vec<T>();
+    static constexpr int STRETCH = L * VEC;
+    static constexpr int ROWS = kThreads / L;
+    int64_t row, o, i, segment;
+    int l;
+    bool live;
+
+    __device__ __forceinline__ Line(const Args<T>& a) {
+        const int64_t rows = a.outer * a.inner;
+        int64_t group = group_index();
+        segment = 0;
+        if (a.segments > 1) {  // then groups < 2^31
+            segment = fast_div(uint32_t(group), a.tiles);
+            group -= segment * a.tiles.d;
+        }
+        row = group * ROWS + threadIdx.x / L;
+        l = threadIdx.x % L;
+        live = group_index() < a.groups && row < rows;
+        if (rows < (int64_t(1) << 31)) {
+            o = fast_div(uint32_t(row), a.outers);
+        } else {
+            o = row / a.inner;
+        }
+        i = row - o * a.inner;
+    }
+    __device__ __forceinline__ int count(int64_t t, int64_t time) const {
+        const int64_t left = time - t;
+        return !live || left <= 0 ? 0 : left >= VEC ? VEC : int(left);
+    }
+};
+
+template <typename T, bool MIX, int L>
+__global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
+    using A = wide_t<T>;
+    using W = Line<T, L>;
+    constexpr int VEC = W::VEC;
+    const W w(a);
+    const T* x = a.x.p + w.o * a.x.so + w.i * a.x.si;
+    const T* g = a.g.p + w.o * a.g.so + w.i * a.g.si;
+    T* y = a.y.p + w.o * a.y.so + w.i * a.y.si;
+    const int64_t t0 = w.segment * a.per_segment * W::STRETCH;
+    const int64_t t1 = std::min(a.time, t0 + a.per_segment * W::STRETCH);
+    int64_t t = t0 + w.l * VEC;
+    int count = w.count(t, a.time);
+    Pack<T, VEC> xs = load_part<T, VEC>(x + t, count, T(0)), gs = load_part<T, VEC>(g + t, count, T(1));
+    A carry = w.live ? segment_start<false>(a, w.segment, w.o, w.i) : A(0);
+    A h = carry;
+    for (int64_t s = t0; s < t1; s += W::STRETCH) {
+        const Pack<T, VEC> xn = xs, gn = gs;
+        const int now = count;
+        const int64_t at = t;
+        if constexpr (L == 64) {  // the next stretch's loads are under way during this one's scan
+            if (s + W::STRETCH < t1) {
+                t += W::STRETCH;
+                count = w.count(t, a.time);
+                xs = load_part<T, VEC>(x + t, count, T(0));
+                gs = load_part<T, VEC>(g + t, count, T(1));
+            }
+            if (a.starts && w.l == 0 && w.live)
+                a.starts[s / W::STRETCH * (a.outer * a.inner) + w.row] = carry;
+        }
+        Map<A> m;
+        A in[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const A gate = A(gn.v[e]);
+            in[e] = input_of<MIX>(gate, A(xn.v[e]));
+            m.then(gate, in[e]);
+        }
+        h = scan_lanes<L, false>(m.factor(), m.b, carry);
+        Pack<T, VEC> out;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            h = apply(A(gn.v[e]), h, in[e]);
+            out.v[e] = T(h);
+        }
+        store_part<T, VEC>(y + at, out, now);
+    }
+    if (w.live && w.segment == a.segments - 1 && w.l == L - 1) a.last.at(w.o, w.i) = h;
+}
+
+template <typename T, bool MIX, int L>
+__global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
+    using A = wide_t<T>;
+    using W = Line<T, L>;
+    constexpr int VEC = W::VEC;
+    const W w(a);
+    const T* x = a.x.p + w.o * a.x.so + w.i * a.x.si;
+    const T* g = a.g.p + w.o * a.g.so + w.i * a.g.si;
+    const T* gy = a.gy.p + w.o * a.gy.so + w.i * a.gy.si;
+    T* gx = a.gx.p + w.o * a.gx.so + w.i * a.gx.si;
+    T* gg = a.gg.p + w.o * a.gg.so + w.i * a.gg.si;
+    const int64_t s0 = w.segment * a.per_segment;
+    const int64_t s1 = std::min(s0 + a.per_segment, (a.time + W::STRETCH - 1) / W::STRETCH);
+    int64_t t = (s1 - 1) * W::STRETCH + w.l * VEC;
+    int count = 0;
+    Pack<T, VEC> xs, gs, ds;
+    A start = A(0);
+    auto load = [&](int64_t s) {
+        count = w.count(t, a.time);
+        xs = load_part<T, VEC>(x + t, count, T(0));
+        gs = load_part<T, VEC>(g + t, count, T(1));
+        ds = load_part<T, VEC>(gy + t, a.gy.p ? count : 0, T(0));
+        if (w.live) {
+            if (L == 64 && a.starts)
+                start = a.starts[s * (a.outer * a.inner) + w.row];
+            else if (a.h0.p)
+                start = a.h0.at(w.o, w.i);
+        }
+    };
+    load(s1 - 1);
+    A carry = w.live ? segment_start<true>(a, w.segment, w.o, w.i) : A(0);
+    A c = carry;
+    for (int64_t s = s1 - 1; s >= s0; --s) {
+        const Pack<T, VEC> xn = xs, gn = gs, dn = ds;
+        const int now = count;
+        const int64_t at = t;
+        A begin = start;
+        if constexpr (L == 64) {
+            if (s > s0) {
+                t -= W::STRETCH;
+                load(s - 1);
+            }
+        }
+        Map<A> m;
+        A q = A(0), before[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const A gate = A(gn.v[e]);
+            before[e] = input_of<MIX>(gate, A(xn.v[e]));
+            m.then(gate, before[e]);
+        }
+#pragma unroll
+        for (int e = VEC - 1; e >= 0; --e) q = back_of(A(gn.v[e]), A(dn.v[e]) + q);
+        const A f = m.factor();
+        A h = scan_lanes<L, false>(f, m.b, begin);
+        c = scan_lanes<L, true>(f, q, carry);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const A in = before[e];
+            before[e] = h;
+            h = apply(A(gn.v[e]), h, in);
+        }
+        Pack<T, VEC> ox, og;
+#pragma unroll
+        for (int e = VEC - 1; e >= 0; --e) {
+            const A gate = A(gn.v[e]), whole = A(dn.v[e]) + c;
+            A dx, dg;
+            gradients<MIX>(gate, A(xn.v[e]), before[e], whole, dx, dg);
+            ox.v[e] = T(dx);
+            og.v[e] = T(dg);
+            c = back_of(gate, whole);
+        }
+        if (a.gx.p) store_part<T, VEC>(gx + at, ox, now);
+        if (a.gg.p) store_part<T, VEC>(gg + at, og, now);
+    }
+    if (w.live && w.segment == 0 && w.l == 0 && a.gh0.p) a.gh0.at(w.o, w.i) = c;
+}
+
+template <typename T, bool MIX, bool BACK>
+__global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
+    using A = wide_t<T>;
+    using W = Line<T, 64>;
+    constexpr int VEC = W::VEC;
+    const W w(a);
+    const T* g = a.g.p + w.o * a.g.so + w.i * a.g.si;
+    const Seq<const T>& src = BACK ? a.gy : a.x;
+    const T* d = src.p + w.o * src.so + w.i * src.si;
+    const bool some = !BACK || src.p;
+    const int64_t t0 = w.segment * a.per_segment * W::STRETCH;
+    const int64_t t1 = std::min(a.time, t0 + a.per_segment * W::STRETCH);
+    const int64_t each = (t1 - t0 + 63) / 64;  // a lane's steps, rounded up to whole accesses
+    const int64_t mine = (each + VEC - 1) / VEC * VEC;
+    const int64_t b0 = std::min(t1, t0 + w.l * mine), b1 = w.live ? std::min(t1, b0 + mine) : b0;
+    Map<A> m;
+    for (int64_t n = 0; n < b1 - b0; n += VEC) {
+        // (BACK: the last, shorter access first)
+        const int64_t t = BACK ? b0 + (b1 - b0 - 1 - n) / VEC * VEC : b0 + n;
+        const int count = int(std::min<int64_t>(VEC, b1 - t));
+        const Pack<T, VEC> gs = load_part<T, VEC>(g + t, count, T(1));
+        const Pack<T, VEC> ds = load_part<T, VEC>(d + t, some ? count : 0, T(0));
+        if constexpr (BACK) {
+#pragma unroll
+            for (int e = VEC - 1; e >= 0; --e) {
+                const A gate = A(gs.v[e]);
+                m.b = back_of(gate, A(ds.v[e]) + m.b);
+                m.a *= gate;
+                m.dropped |= gate == A(0);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const A gate = A(gs.v[e]);
+                m.then(gate, input_of<MIX>(gate, A(ds.v[e])));
+            }
+        }
+        if (m.a == A(0) && !m.dropped) m.a = least(m.a);
+    }
+    // the lanes' maps in a row: what the last lane (BACK: the first) makes of the state 0, and of a
+    // factor
+    A a1 = m.factor(), b1v = m.b;
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+        const A pa = BACK ? __shfl_down(a1, k, 64) : __shfl_up(a1, k, 64);
+        const A pb = BACK ? __shfl_down(b1v, k, 64) : __shfl_up(b1v, k, 64);
+        const bool none = BACK ? w.l + k >= 64 : w.l < k;
+        if (!none) {
+            b1v = apply(a1, pb, b1v);
+            a1 = kept_product(pa, a1);
+        }
+    }
+    if (w.live && w.l == (BACK ? 0 : 63)) {
+        const int64_t n = a.outer * a.inner;
+        A* to = a.maps + 2 * w.segment * n + w.row;
+        to[0] = a1;
+        to[n] = b1v;
+    }
+}
+
+// ---------------------------------------------------------------- launches
+
+// How a call goes: which kernels, and into how many segments of how many stretches.
+enum Way { kRowsFew, kRowsShort, kRowsLong, kLines4, kLines16, kLines64 };
+
+struct Route {
+    Way way;
+    int64_t stretch;      // steps
+    int64_t stretches;
+    int segments;
+    int64_t per_segment;  // stretches
+    int64_t units;        // workgroups of one segment
+};
+
+// Segments where there are fewer workgroups than would fill the chip's 256 CUs: as many as bring
+// them to 1024 (two to four a CU), the first pass costing two thirds of another forward.
+void cut(Route& r) {
+    int64_t n = 1;
+    if (r.units < 256) n = std::min<int64_t>({1024 / r.units, r.stretches / 2, kMaxSegments});
+    if (n < 1) n = 1;
+    r.per_segment = ceil_div(r.stretches, n);
+    r.segments = int(ceil_div(r.stretches, r.per_segment));
+}
+
+// time contiguous: outer * inner lines; else inner contiguous
+Route route_of(int64_t vec, bool lines, int64_t outer, int64_t time, int64_t inner) {
+    Route r{};
+    if (lines) {
+        const int l = time <= 4 * vec ? 4 : time <= 16 * vec ? 16 : 64;
+        r.way = l == 4 ? kLines4 : l == 16 ? kLines16 : kLines64;
+        r.stretch = l * vec;
+        r.units = ceil_div(outer * inner, kThreads / l);
+    } else if (time <= kFew) {
+        r.way = kRowsFew;
+        r.stretch = kFew;
+        r.units = ceil_div(outer * ceil_div(inner, vec), kThreads);
+    } else {
+        // 64 lanes side by side and 4 groups of 8 steps, or 8 and 32
+        const bool few = time <= 32;
+        r.way = few ? kRowsShort : kRowsLong;
+        r.stretch = few ? 32 : 256;
+        r.units = outer * ceil_div(inner, (few ? 64 : 8) * vec);
+    }
+    r.stretches = ceil_div(time, r.stretch);
+    cut(r);
+    return r;
+}
+
+template <typename T>
+int route_args(Args<T>& a, const Route& r, bool lines, void* workspace) {
+    a.segments = r.segments;
+    a.per_segment = r.per_segment;
+    a.maps = r.segments > 1 ? static_cast<wide_t<T>*>(workspace) : nullptr;
+    if (r.stretches <= 1) a.starts = nullptr;
+    a.groups = r.units * r.segments;
+    CL_ARG(a.groups < (int64_t(1) << 31), "too many sequences for one call");
+    if (lines) {
+        a.tiles = make_fastdiv(uint32_t(r.units));
+        a.outers = make_fastdiv(uint32_t(std::min<int64_t>(a.inner, INT32_MAX)));
+    } else {
+        const int64_t lanes = ceil_div(a.inner, wide_vec<T>());
+        const int64_t tiles = r.way == kRowsFew ? lanes : ceil_div(lanes, r.way == kRowsShort ? 64 : 8);
+        a.tiles = make_fastdiv(uint32_t(std::min<int64_t>(tiles, INT32_MAX)));
+        a.outers = make_fastdiv(uint32_t(std::min<int64_t>(a.outer, INT32_MAX)));
+    }
+    return CL_OK;
+}
+
+template <typename T, bool MIX, bool BACK>
+int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
+    const dim3 grid = wide_grid(a.groups);
+    if (r.segments > 1) {
+        if (r.way == kLines64)
+            k_lines_maps<T, MIX, BACK><<<grid, kThreads, 0, s>>>(a);
+        else
+            k_rows_maps<T, MIX, BACK, 8, 32><<<grid, kThreads, 0, s>>>(a, int(r.stretch));
+        if (int rc = check_launch("cl_recurrence(maps)")) return rc;
+    }
+    switch (r.way) {
+        case kRowsFew:
+            k_rows_few<T, MIX, BACK><<<grid, kThreads, 0, s>>>(a);
+            break;
+        case kRowsShort:
+            if constexpr (BACK)
+                k_rows_backward<T, MIX, 64, 4, 8><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_rows_forward<T, MIX, 64, 4, 8><<<grid, kThreads, 0, s>>>(a);
+            break;
+        case kRowsLong:
+            if constexpr (BACK)
+                k_rows_backward<T, MIX, 8, 32, 8><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_rows_forward<T, MIX, 8, 32, 8><<<grid, kThreads, 0, s>>>(a);
+            break;
+        case kLines4:
+            if constexpr (BACK)
+                k_lines_backward<T, MIX, 4><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_lines_forward<T, MIX, 4><<<grid, kThreads, 0, s>>>(a);
+            break;
+        case kLines16:
+            if constexpr (BACK)
+                k_lines_backward<T, MIX, 16><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_lines_forward<T, MIX, 16><<<grid, kThreads, 0, s>>>(a);
+            break;
+        case kLines64:
+            if constexpr (BACK)
+                k_lines_backward<T, MIX, 64><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_lines_forward<T, MIX, 64><<<grid, kThreads, 0, s>>>(a);
+            break;
+    }
+    return check_launch("cl_recurrence");
+}
+
+// The dimensions as the kernels name them: which of batch and features is the outer one.
+struct Dims {
+    int64_t outer, time, inner;
+    bool lines;
+    int o, i;  // the strides' places of outer and inner in (batch, time, features)
+};
+
+int dims_of(int order, int64_t batch, int64_t time, int64_t features, Dims& d) {
+    CL_ARG(batch >= 0 && time >= 0 && features >= 0, "negative shape");
+    switch (order) {
+        case CL_RECURRENCE_FEATURES:
+            d = {batch, time, features, false, 0, 2};
+            return CL_OK;
+        case CL_RECURRENCE_TIME_BATCH:
+            d = {batch, time, features, true, 0, 2};
+            return CL_OK;
+        case CL_RECURRENCE_TIME_FEATURES:
+            d = {features, time, batch, true, 2, 0};
+            return CL_OK;
+        case CL_RECURRENCE_BATCH:
+            CL_ARG(time <= 1, "the batch is contiguous for one step only");
+            d = {features, time, batch, false, 2, 0};
+            return CL_OK;
+        default:
+            set_error("unknown order %d", order);
+            return CL_ERR_INVALID_ARGUMENT;
+    }
+}
+
+template <typename T>
+int sequence(Seq<T>& s, const char* name, const void* p, const int64_t* strides, const Dims& d,
+             bool optional) {
+    s = {static_cast<T*>(const_cast<void*>(p)), 0, 0, 0};
+    if (!p && optional) return CL_OK;
+    CL_ARG(p && strides, "null pointer argument");
+    s.so = strides[d.o];
+    s.st = strides[1];
+    s.si = strides[d.i];
+    CL_ARG(s.so >= 0 && s.st >= 0 && s.si >= 0, "negative strides are not supported");
+    if (d.lines)
+        CL_ARG(s.st == 1 || d.time <= 1, "%s is not contiguous along its time", name);
+    else
+        CL_ARG(s.si == 1 || d.inner <= 1, "%s is not contiguous along its inner dimension", name);
+    return CL_OK;
+}
+
+template <typename A>
+int states(States<A>& s, const void* p, const int64_t* strides, const Dims& d, bool optional) {
+    s = {static_cast<A*>(const_cast<void*>(p)), 0, 0};
+    if (!p && optional) return CL_OK;
+    CL_ARG(p && strides, "null pointer argument");
+    s.so = strides[d.o == 0 ? 0 : 1];
+    s.si = strides[d.i == 0 ? 0 : 1];
+    CL_ARG(s.so >= 0 && s.si >= 0, "negative strides are not supported");
+    return CL_OK;
+}
+
+int vec_of(int dtype) { return dtype == CL_DTYPE_F64 ? 2 : dtype == CL_DTYPE_F32 ? 4 : 8; }
+
+int sizes(int dtype, int order, int64_t batch, int64_t time, int64_t features, Dims& d, Route& r,
+          int64_t& starts, int64_t& bytes) {
+    CL_ARG(dtype >= CL_DTYPE_F32 && dtype <= CL_DTYPE_BF16,
+           "unsupported dtype code %d (expected F32, F64, F16 or BF16)", dtype);
+    if (int rc = dims_of(order, batch, time, features, d)) return rc;
+    starts = bytes = 0;
+    if (batch == 0 || time == 0 || features == 0) return CL_OK;
+    r = route_of(vec_of(dtype), d.lines, d.outer, d.time, d.inner);
+    const int64_t n = batch * features;
+    starts = r.stretches > 1 ? r.stretches * n : 0;
+    bytes = r.segments > 1 ? 2 * r.segments * n * (dtype == CL_DTYPE_F64 ? 8 : 4) : 0;
+    return CL_OK;
+}
+
+}  // namespace
+}  // namespace cl
+
+using namespace cl;
+
+extern "C" int cl_recurrence_sizes(int dtype, int order, int64_t batch, int64_t time, int64_t features,
+                                   int64_t* starts, int64_t* workspace_bytes) {
+    clear_error();
+    CL_ARG(starts && workspace_bytes, "null pointer argument");
+    Dims d;
+    Route r;
+    return sizes(dtype, order, batch, time, features, d, r, *starts, *workspace_bytes);
+}
+
+extern "C" int cl_recurrence_forward(int dtype, int order, int form, const void* x,
+                                     const int64_t* x_strides, const void* gate,
+                                     const int64_t* gate_strides, const void* state,
+                                     const int64_t* state_strides, int64_t batch, int64_t time,
+                                     int64_t features, void* y, const int64_t* y_strides, void* last,
+                                     const int64_t* last_strides, void* starts, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+    clear_error();
+    CL_ARG(form == CL_RECURRENCE_MIX || form == CL_RECURRENCE_ADD, "unknown form %d", form);
+    Dims d;
+    Route r;
+    int64_t n = 0, need = 0;
+    if (int rc = sizes(dtype, order, batch, time, features, d, r, n, need)) return rc;
+    CL_ARG(time > 0, "a recurrence of no steps");
+    if (batch == 0 || features == 0) return CL_OK;
+    CL_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 8)),
+           "workspace of %lld bytes needed (cl_recurrence_sizes)", (long long)need);
+    hipStream_t s = as_stream(stream);
+    CL_STORAGE_SWITCH(dtype, {
+        Args<scalar_t> a{};
+        a.outer = d.outer;
+        a.time = time;
+        a.inner = d.inner;
+        a.starts = static_cast<wide_t<scalar_t>*>(starts);
+        if (int rc = sequence(a.x, "x", x, x_strides, d, false)) return rc;
+        if (int rc = sequence(a.g, "gate", gate, gate_strides, d, false)) return rc;
+        if (int rc = sequence(a.y, "y", y, y_strides, d, false)) return rc;
+        if (int rc = states(a.h0, state, state_strides, d, true)) return rc;
+        if (int rc = states(a.last, last, last_strides, d, false)) return rc;
+        if (int rc = route_args(a, r, d.lines, workspace)) return rc;
+        return form == CL_RECURRENCE_MIX ? launch_recurrence<scalar_t, true, false>(a, r, s)
+                                         : launch_recurrence<scalar_t, false, false>(a, r, s);
+    });
+}
+
+extern "C" int cl_recurrence_backward(int dtype, int order, int form, const void* x,
+                                      const int64_t* x_strides, const void* gate,
+                                      const int64_t* gate_strides, const void* state,
+                                      const int64_t* state_strides, const void* starts,
+                                      const void* grad_y, const int64_t* grad_y_strides,
+                                      const void* grad_last, const int64_t* grad_last_strides,
+                                      int64_t batch, int64_t time, int64_t features, void* grad_x,
+                                      const int64_t* grad_x_strides, void* grad_gate,
+                                      const int64_t* grad_gate_strides, void* grad_state,
+                                      const int64_t* grad_state_strides, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+    clear_error();
+    CL_ARG(form == CL_RECURRENCE_MIX || form == CL_RECURRENCE_ADD, "unknown form %d", form);
+    Dims d;
+    Route r;
+    int64_t n = 0, need = 0;
+    if (int rc = sizes(dtype, order, batch, time, features, d, r, n, need)) return rc;
+    CL_ARG(time > 0, "a recurrence of no steps");
+    if (batch == 0 || features == 0) return CL_OK;
+    CL_ARG(n == 0 || starts, "the forward's starts are needed (cl_recurrence_sizes)");
+    CL_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 8)),
+           "workspace of %lld bytes needed (cl_recurrence_sizes)", (long long)need);
+    hipStream_t s = as_stream(stream);
+    CL_STORAGE_SWITCH(dtype, {
+        Args<scalar_t> a{};
+        a.outer = d.outer;
+        a.time = time;
+        a.inner = d.inner;
+        a.starts = static_cast<wide_t<scalar_t>*>(const_cast<void*>(starts));
+        if (int rc = sequence(a.x, "x", x, x_strides, d, false)) return rc;
+        if (int rc = sequence(a.g, "gate", gate, gate_strides, d, false)) return rc;
+        if (int rc = sequence(a.gy, "grad_y", grad_y, grad_y_strides, d, true)) return rc;
+        if (int rc = sequence(a.gx, "grad_x", grad_x, grad_x_strides, d, true)) return rc;
+        if (int rc = sequence(a.gg, "grad_gate", grad_gate, grad_gate_strides, d, true)) return rc;
+        if (int rc = states(a.h0, state, state_strides, d, true)) return rc;
+        if (int rc = states(a.last, grad_last, grad_last_strides, d, true)) return rc;
+        if (int rc = states(a.gh0, grad_state, grad_state_strides, d, true)) return rc;
+        if (int rc = route_args(a, r, d.lines, workspace)) return rc;
+        return form == CL_RECURRENCE_MIX ? launch_recurrence<scalar_t, true, true>(a, r, s)
+                                         : launch_recurrence<scalar_t, false, true>(a, r, s);
+    });
+}

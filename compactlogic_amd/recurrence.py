@@ -1,0 +1,97 @@
+"""Recurrences over sequences of logic activations on the HIP kernels.  No counterpart in the
+reference.
+
+A relaxed multiplexer whose output is fed back, ``h = g h + (1 - g) x``, is the relaxation of a
+latch: on binary gates and inputs it holds (1) or takes its input (0) exactly.  As the recurrence is
+linear in h, a long sequence need not be walked step by step: the steps of a stretch of time are one
+linear map, and maps are joined in any grouping (csrc/recurrence.hip).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native
+from . import difflogic_hip as _dl
+from .layers import LogicLayer, PackBitsTensor, to_rows
+
+_FORMS = {"mix": 0, "add": 1}
+
+
+def gated_recurrence(x, gate, state=None, form: str = "mix", return_state: bool = False):
+    """``h_t = g_t h_(t-1) + (1 - g_t) x_t`` (form "mix") or ``h_t = g_t h_(t-1) + x_t`` ("add")
+    over the time of x and gate [batch, time, features] from state [batch, features] (None: 0).
+    Returns h [batch, time, features] in x's type, and with return_state also the last state
+    [batch, features] in float32 (float64), from which a later call goes on: one step at a time
+    gives what the whole sequence gives, up to rounding, while the state is handed on as it is.
+
+    x and gate: float32, float64, float16 or bfloat16.  Features or times may lie contiguous (a
+    LogicLayer's output for batch * time samples has its times so, and the result lies alike); other
+    layouts are copied.  States and arithmetic are float32 (float64), each result is rounded once.
+    Differentiable once by x, gate and state, through the outputs and the last state.
+
+    A gate of exactly 0 drops what came before, and one of exactly 1 leaves x unread in "mix": a
+    sequence may begin anew inside of a row, or end before it, whatever the other steps hold, NaN
+    included (the gate's own gradient is the formula's there)."""
+    if not isinstance(x, torch.Tensor) or not isinstance(gate, torch.Tensor):
+        raise TypeError("x and gate must be tensors")
+    if not x.is_cuda or gate.device != x.device:
+        raise RuntimeError("x and gate must be on the same HIP device")
+    _dl.storage_dtype_code(x)
+    if x.dim() != 3 or gate.shape != x.shape or gate.dtype != x.dtype:
+        raise RuntimeError(f"x and gate must be [batch, time, features] of one shape and dtype, got "
+                           f"{tuple(x.shape)} {x.dtype} and {tuple(gate.shape)} {gate.dtype}")
+    code = _FORMS.get(form)
+    if code is None:
+        raise ValueError(f"form must be one of {sorted(_FORMS)}, got {form!r}")
+    if state is not None:
+        if not isinstance(state, torch.Tensor):
+            raise TypeError("state must be a tensor")
+        if state.device != x.device or state.shape != (x.shape[0], x.shape[2]) \
+                or not state.is_floating_point():
+            raise RuntimeError(f"state must be a floating-point tensor of shape "
+                               f"{(x.shape[0], x.shape[2])} on {x.device}")
+        wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+        if state.dtype != wide:
+            state = state.to(wide)
+    if x.shape[1] == 0:
+        wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+        last = x.new_zeros((x.shape[0], x.shape[2]), dtype=wide) if state is None else state.clone()
+        return (x.clone(), last) if return_state else x.clone()
+    y, last = _native.load().gated_recurrence(x, gate, state, code)
+    return (y, last) if return_state else y
+
+
+class LogicRecurrence(torch.nn.Module):
+    """A layer of latches: one LogicLayer computes each latch's gate from the step's input, one its
+    data, and a latch holds where its gate is 1 and takes its data where it is 0.
+
+    x [batch, time, in_dim] -> [batch, time, out_dim], from a state [batch, out_dim] (None: zeros);
+    with return_state also the state behind the last step, for the next call.  In eval mode, or
+    frozen, gates and data are the discrete ones of `LogicLayer`, and so is the result for binary
+    inputs.  Packed inputs are not supported.  The other arguments are LogicLayer's."""
+
+    def __init__(self, in_dim: int, out_dim: int, connections: str = 'random', num_gates=16,
+                 residual_init: bool = False):
+        super().__init__()
+        self.in_dim = in_dim
+        self.out_dim = out_dim
+        self.gate = LogicLayer(in_dim, out_dim, connections, num_gates, residual_init)
+        self.data = LogicLayer(in_dim, out_dim, connections, num_gates, residual_init)
+
+    def forward(self, x, state=None, return_state: bool = False):
+        if isinstance(x, PackBitsTensor):
+            raise RuntimeError("LogicRecurrence takes sequences of activations, not packed bits")
+        if x.dim() != 3 or x.shape[2] != self.in_dim:
+            raise RuntimeError(f"x must be [batch, time, {self.in_dim}], got {tuple(x.shape)}")
+        steps = x.shape[:2]
+        rows = to_rows(x.reshape(-1, self.in_dim)).transpose(0, 1)
+        gate, data = self.gate(rows), self.data(rows)
+        return gated_recurrence(data.unflatten(0, steps), gate.unflatten(0, steps), state,
+                                return_state=return_state)
+
+    def freeze(self):
+        self.gate.freeze()
+        self.data.freeze()
+
+    def extra_repr(self):
+        return f"{self.in_dim}, {self.out_dim}"

@@ -568,6 +568,53 @@ int cl_adam_clip_step(int dtype, int64_t num_tensors, void* const* params, void*
                       void* stream);
 
 /* -------------------------------------------------------------------------------------------
+ * Gated linear recurrence over sequences (no reference counterpart), per batch entry and feature
+ *   h_t = g_t h_(t-1) + b_t,  b_t = (1 - g_t) x_t (CL_RECURRENCE_MIX) or x_t (CL_RECURRENCE_ADD),
+ * y_t = h_t, and its gradients: with G_t = grad_y_t + c_t, c_(t-1) = g_t G_t, c of the last step
+ * grad_last,  grad_x_t = (1 - g_t) G_t or G_t,  grad_gate_t = G_t (h_(t-1) - x_t) or G_t h_(t-1),
+ * grad_state = c before the first step.  A gate of exactly 0 drops what came before (and what comes
+ * back from behind), one of exactly 1 leaves x unread in the outputs of MIX, NaN and infinities too.
+ *
+ * x, gate, y and their gradients: dtype (F32, F64, F16, BF16), [batch, time, features] by strides
+ * (elements: batch, time, features); state, last and theirs: fp32 (fp64 for F64), [batch, features]
+ * by two strides.  order says what is contiguous in all of the former, and which of the others lies
+ * farther apart:
+ *   CL_RECURRENCE_FEATURES       features contiguous
+ *   CL_RECURRENCE_TIME_BATCH     time contiguous, batch outermost
+ *   CL_RECURRENCE_TIME_FEATURES  time contiguous, features outermost
+ *   CL_RECURRENCE_BATCH          batch contiguous, one step only
+ * The stride of a dimension of size one is not read.  state may be NULL (0).  time must not be 0.
+ * starts: the states that stretches of time begin with, cl_recurrence_sizes elements of the wide
+ * type; the forward writes them (NULL: it does not), the backward needs them where there are any.
+ * workspace: cl_recurrence_sizes bytes, on 8 bytes, for either call.  grad_y and grad_last may be
+ * NULL (0), each output of the backward too.  Arithmetic and states in the wide type, each result
+ * rounded once; results are bitwise reproducible for equal sizes and orders. */
+#define CL_RECURRENCE_MIX 0
+#define CL_RECURRENCE_ADD 1
+#define CL_RECURRENCE_FEATURES 0
+#define CL_RECURRENCE_TIME_BATCH 1
+#define CL_RECURRENCE_TIME_FEATURES 2
+#define CL_RECURRENCE_BATCH 3
+
+int cl_recurrence_sizes(int dtype, int order, int64_t batch, int64_t time, int64_t features,
+                        int64_t* starts, int64_t* workspace_bytes);
+int cl_recurrence_forward(int dtype, int order, int form, const void* x, const int64_t* x_strides,
+                          const void* gate, const int64_t* gate_strides, const void* state,
+                          const int64_t* state_strides, int64_t batch, int64_t time,
+                          int64_t features, void* y, const int64_t* y_strides, void* last,
+                          const int64_t* last_strides, void* starts, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+int cl_recurrence_backward(int dtype, int order, int form, const void* x, const int64_t* x_strides,
+                           const void* gate, const int64_t* gate_strides, const void* state,
+                           const int64_t* state_strides, const void* starts, const void* grad_y,
+                           const int64_t* grad_y_strides, const void* grad_last,
+                           const int64_t* grad_last_strides, int64_t batch, int64_t time,
+                           int64_t features, void* grad_x, const int64_t* grad_x_strides,
+                           void* grad_gate, const int64_t* grad_gate_strides, void* grad_state,
+                           const int64_t* grad_state_strides, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* -------------------------------------------------------------------------------------------
  * One AdamW step over any number of tensors (no reference counterpart).  With t = step[0] + 1,
  * written back to step (a device fp64 scalar), and c = min(1, max_norm / (|g| + 1e-6)), |g| the norm
  * over all tensors in fp64 (c = 1 where max_norm <= 0), per element
