@@ -11,6 +11,7 @@ losses and of dropout, csrc/autograd.cpp) by ``python -m compactlogic_amd.build`
 """
 from . import checkpoint, circuit, convlogic_hip, difflogic_hip
 from .dropout_layer import Dropout, dropout
+from .drafts import verify_drafts
 from .layers import (ConvLayer, ConvLayerCudaFunction, ConvLayerSoftmaxFunction,
                      ConvLayerWindowFunction, GroupSum, GroupSumCrossEntropyFunction,
                      GroupSumFunction, LogicGroupSumCrossEntropyFunction, LogicLayer,
@@ -36,5 +37,5 @@ __all__ = [
     "LogicGroupSumCrossEntropyFunction", "logic_group_sum_cross_entropy",
     "sequential_cross_entropy", "checkpoint", "circuit", "Dropout", "dropout",
     "policy_loss", "preference_loss", "selected_log_probs",
-    "LogicRecurrence", "gated_recurrence",
+    "LogicRecurrence", "gated_recurrence", "verify_drafts",
 ]

@@ -156,6 +156,9 @@ SIGNATURES: dict[str, list] = {
                                    _int, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p],
     "cl_preference_loss_backward": [_int, _p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _int, _p, _p,
                                     _p, _p],
+    "cl_verify_drafts_workspace": [_int, _i64, _i64, _i64, ctypes.POINTER(_i64)],
+    "cl_verify_drafts": [_int, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _int, _i64, _i64, _i64,
+                         _p, _p, _p, _p, _i64, _p],
     "cl_dropout": [_int, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _int, _f64, _u64, _u64,
                    _p, _p],
     "cl_dropout_next": [_p, _p, _p],

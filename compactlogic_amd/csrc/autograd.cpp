@@ -5,13 +5,15 @@
 // A small call's kernels take 6 to 15 us.  As Functions in Python such calls took 76 to 97 us, here
 // 45 to 62: autograd runs a backward on a thread of its own, and an interpreter on either side of
 // that hand-over costs 30 us more (torch's own negation, forward and backward, takes 45).
-// Arguments are checked in policy.py, dropout_layer.py and recurrence.py; nothing here is a public interface.
+// Arguments are checked in policy.py, dropout_layer.py, recurrence.py and
+// drafts.py; nothing here is a public interface.
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
 
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -656,6 +658,35 @@ Tensor dropout_next(const Tensor& rng) {
     return used;
 }
 
+// (tokens, accepted, log_probs) of logits [sequences, drafts + 1, cols]
+std::tuple<Tensor, Tensor, Tensor> verify_drafts(const Tensor& logits, const Tensor& drafted,
+                                                 const c10::optional<Tensor>& draft,
+                                                 const Tensor& uniforms, int64_t ignore) {
+    const c10::DeviceGuard guard(logits.device());
+    const at::NoGradGuard no_grad;
+    const int code = code_of(logits);
+    const int64_t seqs = logits.size(0), drafts = drafted.size(1), cols = logits.size(2);
+    auto rows = [&](const Tensor& t) {
+        return cols > 1 && t.stride(2) != 1 ? t.contiguous() : t;
+    };
+    const Tensor p = rows(logits), q = draft ? rows(*draft) : Tensor();
+    Tensor tokens = at::empty({seqs, drafts + 1}, drafted.options());
+    Tensor accepted = at::empty({seqs}, drafted.options());
+    Tensor lp = at::empty({seqs, drafts + 1}, wide_of(logits));
+    int64_t need = 0;
+    sized("cl_verify_drafts_workspace",
+          cl_verify_drafts_workspace(code, seqs, drafts, cols, &need));
+    const Tensor ws = need ? at::empty({need}, logits.options().dtype(at::kByte)) : Tensor();
+    launch("cl_verify_drafts", logits.get_device(), [&](void* stream) {
+        return cl_verify_drafts(
+            code, p.data_ptr(), p.stride(0), p.stride(1), data_of(q), q.defined() ? q.stride(0) : 0,
+            q.defined() ? q.stride(1) : 0, ints(drafted), ignore, uniforms.data_ptr(),
+            code_of(uniforms), seqs, drafts, cols, static_cast<int64_t*>(tokens.data_ptr()),
+            static_cast<int64_t*>(accepted.data_ptr()), lp.data_ptr(), data_of(ws), need, stream);
+    });
+    return {tokens, accepted, lp};
+}
+
 // ---- one AdamW step over the parameters of an optimizer.  The walk over its groups and states is here
 // because a Python loop costs some 2 us a tensor, a small tensor's share of the kernels 0.1.
 
@@ -785,6 +816,7 @@ PYBIND11_MODULE(_autograd, m) {
     m.def("policy_loss", &policy_loss, unlocked());
     m.def("preference_loss", &preference_loss, unlocked());
     m.def("gated_recurrence", &gated_recurrence, unlocked());
+    m.def("verify_drafts", &verify_drafts, unlocked());
     m.def("dropout", &dropout, unlocked());
     m.def("dropout_next", &dropout_next, unlocked());
     m.def("adamw_step", &adamw_step);

@@ -1,0 +1,680 @@
+// Verification of drafted tokens against the target's probabilities.  Sequence s has K drafted tokens
+// x_i, drawn from the draft's probabilities q_i, and the target's p_0 .. p_K, all as logits, and K + 1
+// uniform numbers.  Token i is accepted while
+//   u_i q_i(x_i) < p_i(x_i);
+// at the first one that is not, a token is drawn from max(p_i - q_i, 0), and behind the last one from
+// p_i, by the last number r: the first j whose sum of weights up to j is above r times their sum.  What
+// comes out is distributed as the target's own tokens are, whatever the draft was.
+//
+// The tests take a maximum and a sum in fp32 over each row, as the losses do.  The draw takes a sum in
+// fp64 of exponentials in fp64, of one row of each: next to some 10^5 borders between tokens, fp32 sums
+// would draw a neighbour once in 10^3 draws, as their order goes.
+//
+//   k_small    one workgroup a sequence does it all, where a row is one chunk
+// else, each row cut into chunks of kChunk elements,
+//   k_stats    (m, s) of every chunk of the rows
+//   k_sums     joins them, takes the tests (every workgroup of a sequence the same ones), and the
+//              fp64 sums of its chunk of the two rows
+//   k_weights  the sum of max(p - q, 0) of its chunk
+//   k_pick     the chunk that the number falls into, and the place in it
+#include "row_loss.h"
+#include "storage.h"
+
+namespace cl {
+namespace {
+
+constexpr int kChunk = 8192;
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kRun = kChunk / kThreads;  // elements of a thread, one behind the other
+constexpr int kStatThreads = 256;
+
+template <typename A>
+struct Stat {
+    A m, s;
+};
+
+// What the tests leave for the draw.
+struct Draw {
+    double mp, mq;   // largest logits of the two rows
+    int64_t n;       // accepted tokens
+    int64_t refused; // one was drafted there: the draft's row counts
+};
+
+template <typename T>
+struct Args {
+    using A = wide_t<T>;
+    const T *p, *q;                  // q may be null: the draft was sure of its tokens
+    int64_t p_seq, p_row, q_seq, q_row;
+    const int64_t* tokens;
+    const void* uniforms;
+    bool uniforms64;
+    int64_t ignore;
+    int64_t seqs, drafts, cols;
+    int64_t* out;
+    int64_t* accepted;
+    A* lp;
+    // workspace, where a row has several chunks
+    int chunks;
+    Stat<A>* stats;                  // [seq][2 drafts + 1][chunk], the target's rows first
+    Draw* draws;
+    double* sums;                    // [seq][chunk][p, q]
+    double* weights;                 // [seq][chunk]
+
+    __device__ __forceinline__ double uniform(int64_t seq, int64_t i) const {
+        const int64_t at = seq * (drafts + 1) + i;
+        return uniforms64 ? static_cast<const double*>(uniforms)[at]
+                          : double(static_cast<const float*>(uniforms)[at]);
+    }
+    __device__ __forceinline__ const T* row(int64_t seq, int64_t i, bool draft) const {
+        return draft ? q + seq * q_seq + i * q_row : p + seq * p_seq + i * p_row;
+    }
+    __device__ __forceinline__ Stat<A>* stat(int64_t seq, int64_t i, bool draft) const {
+        return stats + (seq * (2 * drafts + 1) + i + (draft ? drafts + 1 : 0)) * chunks;
+    }
+    __device__ __forceinline__ bool holds(int64_t token) const { return token >= 0 && token < cols; }
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_part(const T* p, int64_t count) {
+    if (count >= N) return pload<T, N>(p);
+    Pack<T, N> r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r.v[e] = e < count ? p[e] : T(-__builtin_inff());
+    return r;
+}
+
+// ---- maximum and sum of exp(x - m).  Where there was nothing but -inf, differences are taken from 0.
+template <typename A>
+__device__ __forceinline__ A base_of(A m) {
+    return m == -A(__builtin_inf()) ? A(0) : m;
+}
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double max_of(double a, double b) { return __builtin_fmax(a, b); }
+
+template <int LANES, typename A>
+__device__ __forceinline__ Stat<A> join(Stat<A> st) {
+    A m = st.m;
+    m = max_of(m, dpp_move<0xB1>(m));   // quad_perm [1,0,3,2]
+    m = max_of(m, dpp_move<0x4E>(m));   // quad_perm [2,3,0,1]
+    m = max_of(m, dpp_move<0x141>(m));  // row_half_mirror
+    m = max_of(m, dpp_move<0x140>(m));  // row_mirror
+    if constexpr (LANES == 64)
+        m = max_of(max_of(read_lane(m, 0), read_lane(m, 16)),
+                   max_of(read_lane(m, 32), read_lane(m, 48)));
+    A s = st.s * exp_diff(st.m - base_of(m));
+    if constexpr (LANES == 64) {
+        s = wave_total(s);
+    } else {
+        s += dpp_move<0xB1>(s);
+        s += dpp_move<0x4E>(s);
+        s += dpp_move<0x141>(s);
+        s += dpp_move<0x140>(s);
+    }
+    return {m, s};
+}
+
+template <typename A>
+__device__ __forceinline__ void add(Stat<A>& st, const Stat<A>& more) {
+    const A m = max_of(st.m, more.m), base = base_of(m);
+    st.s = st.s * exp_diff(st.m - base) + more.s * exp_diff(more.m - base);
+    st.m = m;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kStatThreads) void k_stats(Args<T> a) {
+    using A = wide_t<T>;
+    constexpr int VEC = wide_vec<T>(), NV = kChunk / kStatThreads / VEC;
+    __shared__ Stat<A> part[kStatThreads / 64];
+    const int64_t rows = 2 * a.drafts + 1;
+    int64_t group = group_index();
+    if (group >= a.seqs * rows * a.chunks) return;
+    const int chunk = int(group % a.chunks);
+    group /= a.chunks;
+    const int64_t seq = group / rows, r = group - seq * rows;
+    const bool draft = r > a.drafts;
+    const int64_t i = draft ? r - a.drafts - 1 : r;
+    if (draft && !a.q) return;
+    // a row behind the end of the drafts is not read
+    bool ended = false;
+    for (int64_t j = 0; j < (draft ? i + 1 : i); ++j) ended |= a.tokens[seq * a.drafts + j] == a.ignore;
+    if (ended) return;
+    const int64_t j0 = int64_t(chunk) * kChunk;
+    const T* x = a.row(seq, i, draft) + j0;
+    const int64_t n = a.cols - j0;
+    Pack<T, VEC> v[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int64_t at = (k * kStatThreads + threadIdx.x) * VEC;
+        v[k] = load_part<T, VEC>(x + at, n - at);
+    }
+    Stat<A> st{-A(__builtin_inf()), A(0)};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) st.m = max_of(st.m, A(v[k].v[e]));
+    const A base = base_of(st.m);
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) st.s += exp_diff(A(v[k].v[e]) - base);
+    st = join<64>(st);
+    if (lane_id() == 0) part[wave_id()] = st;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kStatThreads / 64; ++w) add(st, part[w]);
+        a.stat(seq, i, draft)[chunk] = st;
+    }
+}
+
+// ---- the tests, kThreads / LANES rows at a time: position i's target and draft beside each other.
+// Every thread returns with the outcome.  rows(seq, i, draft) gives a row's (m, s) to its lanes.
+template <int LANES>
+struct Round {
+    static constexpr int N = kThreads / LANES / 2;  // positions
+    double prob[N][2], m[N][2], lp[N];
+    int first;
+};
+
+template <int LANES, typename T, typename F>
+__device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANES>& sh, bool write,
+                                       F&& rows) {
+    using A = wide_t<T>;
+    constexpr int N = Round<LANES>::N;
+    const int g = threadIdx.x / LANES;
+    for (int64_t i0 = 0;; i0 += N) {
+        const bool draft = g & 1;
+        const int64_t i = i0 + g / 2;
+        const int64_t token = i < a.drafts ? a.tokens[seq * a.drafts + i] : a.ignore;
+        const bool given = i < a.drafts && token != a.ignore;
+        if (draft ? given && a.q : i <= a.drafts) {
+            const Stat<A> st = rows(seq, i, draft);
+            double pr = 0.0, lp = -__builtin_inf();
+            if (given && a.holds(token)) {
+                const double d = double(a.row(seq, i, draft)[token]) - double(st.m);
+                pr = exp(d) / double(st.s);
+                lp = d - log(double(st.s));
+            }
+            if (threadIdx.x % LANES == 0) {
+                sh.prob[g / 2][draft] = pr;
+                sh.m[g / 2][draft] = double(st.m);
+                if (!draft) sh.lp[g / 2] = lp;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int l = threadIdx.x;
+            const int64_t at = i0 + l;
+            bool stop = false;
+            if (l < N && at <= a.drafts) {
+                const int64_t mine = at < a.drafts ? a.tokens[seq * a.drafts + at] : a.ignore;
+                stop = true;
+                if (at < a.drafts && mine != a.ignore) {
+                    const double q = !a.q ? 1.0 : sh.prob[l][1];
+                    stop = !(a.uniform(seq, at) * q < sh.prob[l][0]);
+                }
+            }
+            const uint64_t stops = __ballot(stop);
+            const int first = stops ? __builtin_ctzll(stops) : N;
+            if (write && l < first && l < N) {
+                a.out[seq * (a.drafts + 1) + at] = a.tokens[seq * a.drafts + at];
+                a.lp[seq * (a.drafts + 1) + at] = A(sh.lp[l]);
+            }
+            if (l == 0) sh.first = first;
+        }
+        __syncthreads();
+        const int first = sh.first;
+        if (first < N) {
+            const int64_t n = i0 + first;
+            const bool refused = n < a.drafts && a.tokens[seq * a.drafts + n] != a.ignore;
+            if (write) {
+                for (int64_t k = n + 1 + threadIdx.x; k <= a.drafts; k += kThreads) {
+                    a.out[seq * (a.drafts + 1) + k] = a.ignore;
+                    a.lp[seq * (a.drafts + 1) + k] = A(0);
+                }
+                if (threadIdx.x == 0) a.accepted[seq] = n;
+            }
+            return {sh.m[first][0], refused && a.q ? sh.m[first][1] : 0.0, n, refused};
+        }
+        __syncthreads();
+    }
+}
+
+// ---- fp64 sums over a workgroup
+__device__ __forceinline__ double group_total(double v, double* red) {
+    v = wave_total(v);
+    if (lane_id() == 0) red[wave_id()] = v;
+    __syncthreads();
+    double s = red[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) s += red[w];
+    __syncthreads();
+    return s;
+}
+
+// Sum up to and with each thread's v; `total`: of all.
+__device__ __forceinline__ double group_scan(double v, double* red, double& total) {
+    const int l = lane_id();
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+        const double before = __shfl_up(v, k, 64);
+        if (l >= k) v += before;
+    }
+    if (l == 63) red[wave_id()] = v;
+    __syncthreads();
+    double before = 0.0;
+    total = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        if (w == wave_id()) before = total;
+        total += red[w];
+    }
+    __syncthreads();
+    return before + v;
+}
+
+// ---- the draw.  A thread's elements of a chunk: `run` of them from `at` on.
+template <typename T>
+struct Place {
+    int64_t at;
+    int count;
+    __device__ __forceinline__ Place(int64_t j0, int64_t cols) {
+        constexpr int VEC = wide_vec<T>();
+        const int64_t n = cols - j0 < kChunk ? cols - j0 : kChunk;
+        const int run = int((n + kThreads * VEC - 1) / (kThreads * VEC)) * VEC;
+        at = j0 + int64_t(threadIdx.x) * run;
+        const int64_t left = j0 + n - at;
+        count = left >= run ? run : left > 0 ? int(left) : 0;
+    }
+};
+
+// exp(x - m) of the thread's elements in fp64, 0 behind them.
+template <typename T>
+__device__ __forceinline__ void exponentials(const T* row, const Place<T>& w, double m,
+                                             double (&e)[kRun]) {
+    constexpr int VEC = wide_vec<T>();
+    Pack<T, VEC> v[kRun / VEC];
+#pragma unroll
+    for (int k = 0; k < kRun / VEC; ++k)
+        v[k] = load_part<T, VEC>(row + w.at + k * VEC, w.count - k * VEC);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k)
+        e[k] = k < w.count ? exp(double(v[k / VEC].v[k % VEC]) - m) : 0.0;
+}
+
+template <typename T>
+struct Rows {
+    const T *p, *q;   // q null: no draft counts, or it was sure of `token`
+    int64_t token;
+    bool sure;
+    __device__ __forceinline__ Rows(const Args<T>& a, int64_t seq, const Draw& d) {
+        p = a.row(seq, d.n, false);
+        q = d.refused && a.q ? a.row(seq, d.n, true) : nullptr;
+        sure = d.refused && !a.q;
+        token = sure ? a.tokens[seq * a.drafts + d.n] : 0;
+    }
+};
+
+// Weights of the thread's elements where a draft was refused: max(p - q, 0).
+template <typename T>
+__device__ __forceinline__ void over(const Rows<T>& r, const Place<T>& w, const Draw& d, double sp,
+                                     double sq, double (&e)[kRun]) {
+    exponentials(r.p, w, d.mp, e);
+    if (r.q) {
+        double f[kRun];
+        exponentials(r.q, w, d.mq, f);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            const double v = e[k] / sp - f[k] / sq;
+            e[k] = v > 0.0 || v != v ? v : 0.0;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) e[k] = w.at + k == r.token ? 0.0 : e[k] / sp;
+    }
+}
+
+// The place of the first weight up to and with which the sum is above `goal`, `before` counted in; the
+// last weight above 0 if rounding leaves none.  sh: first and last thread; the owner writes `*place`.
+template <typename T>
+__device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T>& w, double upto,
+                                         double before, double goal, int* sh, int64_t* place) {
+    double mine = 0.0;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) mine += e[k];
+    if (threadIdx.x == 0) {
+        sh[0] = kThreads;
+        sh[1] = -1;
+        *place = -1;
+    }
+    __syncthreads();
+    if (mine > 0.0) {
+        if (before + upto > goal) atomicMin(&sh[0], int(threadIdx.x));
+        atomicMax(&sh[1], int(threadIdx.x));
+    }
+    __syncthreads();
+    const int owner = sh[0] < kThreads ? sh[0] : sh[1];
+    if (int(threadIdx.x) == owner) {
+        double c = before + (upto - mine);
+        int at = -1;
+        bool found = false;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+            c += e[k];
+            if (e[k] > 0.0 && !found) {
+                at = k;
+                found = sh[0] < kThreads && c > goal;
+            }
+        }
+        *place = w.at + at;
+    }
+    __syncthreads();
+}
+
+template <typename T>
+__device__ __forceinline__ void put(const Args<T>& a, int64_t seq, const Draw& d, const T* p, double sp,
+                                    int64_t place) {
+    using A = wide_t<T>;
+    const int64_t to = seq * (a.drafts + 1) + d.n;
+    a.out[to] = place >= 0 ? place : a.ignore;
+    a.lp[to] = place >= 0 ? A((double(p[place]) - d.mp) - log(sp)) : A(__builtin_nan(""));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_small(Args<T> a) {
+    using A = wide_t<T>;
+    constexpr int VEC = wide_vec<T>();
+    __shared__ Round<64> round;
+    __shared__ double red[kWaves];
+    __shared__ int ends[2];
+    __shared__ int64_t place;
+    const int64_t seq = group_index();
+    if (seq >= a.seqs) return;
+    const Draw d = decide<64>(a, seq, round, true, [&](int64_t s, int64_t i, bool draft) {
+        const T* x = a.row(s, i, draft);
+        Stat<A> st{-A(__builtin_inf()), A(0)};
+        for (int64_t j = lane_id() * VEC; j < a.cols; j += 64 * VEC) {
+            const Pack<T, VEC> v = load_part<T, VEC>(x + j, a.cols - j);
+            A m = st.m;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = max_of(m, A(v.v[e]));
+            const A base = base_of(m);
+            st.s *= exp_diff(st.m - base);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) st.s += exp_diff(A(v.v[e]) - base);
+            st.m = m;
+        }
+        return join<64>(st);
+    });
+    const Rows<T> r(a, seq, d);
+    const Place<T> w(0, a.cols);
+    const double u = a.uniform(seq, a.drafts);
+    double e[kRun], mine = 0.0, total;
+    exponentials(r.p, w, d.mp, e);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) mine += e[k];
+    const double upto_p = group_scan(mine, red, total);
+    const double sp = total;
+    double upto = upto_p;
+    if (d.refused) {
+        double sq = 1.0;
+        if (r.q) {
+            double f[kRun];
+            exponentials(r.q, w, d.mq, f);
+            mine = 0.0;
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) mine += f[k];
+            sq = group_total(mine, red);
+        }
+        over(r, w, d, sp, sq, e);
+        mine = 0.0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) mine += e[k];
+        upto = group_scan(mine, red, total);
+        if (!(total > 0.0)) {  // nothing above the draft: the target's own
+            exponentials(r.p, w, d.mp, e);
+            total = sp;
+            upto = upto_p;
+        }
+    }
+    place_of(e, w, upto, 0.0, u * total, ends, &place);
+    if (threadIdx.x == 0) put(a, seq, d, r.p, sp, sp > 0.0 ? place : -1);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_sums(Args<T> a) {
+    using A = wide_t<T>;
+    __shared__ Round<16> round;
+    __shared__ double red[kWaves];
+    const int64_t group = group_index();
+    if (group >= a.seqs * a.chunks) return;
+    const int64_t seq = group / a.chunks;
+    const int chunk = int(group - seq * a.chunks);
+    const Draw d = decide<16>(a, seq, round, chunk == 0, [&](int64_t s, int64_t i, bool draft) {
+        const Stat<A>* part = a.stat(s, i, draft);
+        Stat<A> st{-A(__builtin_inf()), A(0)};
+        for (int c = threadIdx.x & 15; c < a.chunks; c += 16) add(st, part[c]);
+        return join<16>(st);
+    });
+    if (chunk == 0 && threadIdx.x == 0) a.draws[seq] = d;
+    const Rows<T> r(a, seq, d);
+    const Place<T> w(int64_t(chunk) * kChunk, a.cols);
+    double e[kRun], mine = 0.0, total;
+    exponentials(r.p, w, d.mp, e);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) mine += e[k];
+    group_scan(mine, red, total);   // as k_pick will have it
+    if (threadIdx.x == 0) a.sums[2 * group] = total;
+    if (r.q) {
+        exponentials(r.q, w, d.mq, e);
+        mine = 0.0;
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) mine += e[k];
+        total = group_total(mine, red);
+        if (threadIdx.x == 0) a.sums[2 * group + 1] = total;
+    }
+}
+
+// The sum of the chunks' sums, the same in every thread; stride: of them.
+__device__ __forceinline__ double chunks_total(const double* sums, int stride, int chunks) {
+    double s = 0.0;
+    for (int c = lane_id(); c < chunks; c += 64) s += sums[int64_t(c) * stride];
+    return wave_total(s);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_weights(Args<T> a) {
+    __shared__ double red[kWaves];
+    const int64_t group = group_index();
+    if (group >= a.seqs * a.chunks) return;
+    const int64_t seq = group / a.chunks;
+    const Draw d = a.draws[seq];
+    if (!d.refused) return;
+    const int chunk = int(group - seq * a.chunks);
+    const Rows<T> r(a, seq, d);
+    const Place<T> w(int64_t(chunk) * kChunk, a.cols);
+    const double* sums = a.sums + 2 * seq * a.chunks;
+    const double sp = chunks_total(sums, 2, a.chunks);
+    const double sq = r.q ? chunks_total(sums + 1, 2, a.chunks) : 1.0;
+    double e[kRun], mine = 0.0, total;
+    over(r, w, d, sp, sq, e);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) mine += e[k];
+    group_scan(mine, red, total);
+    if (threadIdx.x == 0) a.weights[group] = total;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_pick(Args<T> a) {
+    __shared__ double red[kWaves];
+    __shared__ int ends[2];
+    __shared__ int64_t place;
+    const int64_t seq = group_index();
+    if (seq >= a.seqs) return;
+    const Draw d = a.draws[seq];
+    const Rows<T> r(a, seq, d);
+    const double* sums = a.sums + 2 * seq * a.chunks;
+    const double sp = chunks_total(sums, 2, a.chunks);
+    const double sq = r.q ? chunks_total(sums + 1, 2, a.chunks) : 1.0;
+    const double* parts = a.weights + seq * a.chunks;
+    int stride = 1;
+    double total = d.refused ? chunks_total(parts, 1, a.chunks) : 0.0;
+    const bool own = !(total > 0.0);  // the target's own: no draft was refused, or nothing is above it
+    if (own) {
+        parts = sums;
+        stride = 2;
+        total = sp;
+    }
+    // the chunk, as place_of finds a place in it; every wave alike
+    const double goal = a.uniform(seq, a.drafts) * total;
+    int chosen = -1, last = -1;
+    double before = 0.0, at_last = 0.0, carry = 0.0;
+    for (int c0 = 0; c0 < a.chunks && chosen < 0; c0 += 64) {
+        const int c = c0 + lane_id();
+        const double mine = c < a.chunks ? parts[int64_t(c) * stride] : 0.0;
+        double v = mine;
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) {
+            const double prior = __shfl_up(v, k, 64);
+            if (lane_id() >= k) v += prior;
+        }
+        const uint64_t some = __ballot(mine > 0.0);
+        const uint64_t hit = __ballot(mine > 0.0 && carry + v > goal);
+        const double start = __shfl_up(v, 1, 64);
+        const double prior = carry + (lane_id() == 0 ? 0.0 : start);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            chosen = c0 + l;
+            before = read_lane(prior, l);
+        } else if (some) {
+            const int l = 63 - __builtin_clzll(some);
+            last = c0 + l;
+            at_last = read_lane(prior, l);
+        }
+        carry += read_lane(v, 63);
+    }
+    if (chosen < 0) {
+        chosen = last;
+        before = at_last;
+    }
+    if (chosen < 0) {  // no weight anywhere, or NaN
+        if (threadIdx.x == 0) put(a, seq, d, r.p, sp, -1);
+        return;
+    }
+    const Place<T> w(int64_t(chosen) * kChunk, a.cols);
+    double e[kRun], mine = 0.0;
+    if (own)
+        exponentials(r.p, w, d.mp, e);
+    else
+        over(r, w, d, sp, sq, e);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) mine += e[k];
+    double sum;
+    const double upto = group_scan(mine, red, sum);
+    place_of(e, w, upto, before, goal, ends, &place);
+    if (threadIdx.x == 0) put(a, seq, d, r.p, sp, sp > 0.0 ? place : -1);
+}
+
+// Chunks of a row, and the parts of the workspace behind each other on 16 bytes.
+struct Layout {
+    int64_t chunks, stats, draws, sums, weights, total;
+};
+
+int layout_of(int dtype, int64_t seqs, int64_t drafts, int64_t cols, Layout& l) {
+    CL_ARG(dtype >= CL_DTYPE_F32 && dtype <= CL_DTYPE_BF16,
+           "unsupported dtype code %d (expected F32, F64, F16 or BF16)", dtype);
+    CL_ARG(seqs >= 0 && drafts >= 0 && cols >= 1, "bad shape: %lld sequences, %lld drafts, %lld classes",
+           (long long)seqs, (long long)drafts, (long long)cols);
+    l.chunks = ceil_div(cols, kChunk);
+    CL_ARG(l.chunks < (int64_t(1) << 24) && drafts < (int64_t(1) << 24) &&
+               seqs < (int64_t(1) << 31) &&
+               double(seqs) * (2.0 * drafts + 1) * l.chunks < double(int64_t(1) << 31),
+           "too many logits for one call");
+    l.stats = 0;
+    if (l.chunks == 1) {
+        l.draws = l.sums = l.weights = l.total = 0;
+        return CL_OK;
+    }
+    const int64_t wide = dtype == CL_DTYPE_F64 ? 8 : 4;
+    l.draws = ceil_div(2 * wide * seqs * (2 * drafts + 1) * l.chunks, 16) * 16;
+    l.sums = l.draws + int64_t(sizeof(Draw)) * seqs;
+    l.weights = l.sums + 16 * seqs * l.chunks;
+    l.total = l.weights + 8 * seqs * l.chunks;
+    return CL_OK;
+}
+
+}  // namespace
+}  // namespace cl
+
+using namespace cl;
+
+extern "C" int cl_verify_drafts_workspace(int dtype, int64_t sequences, int64_t drafts, int64_t cols,
+                                          int64_t* bytes) {
+    clear_error();
+    CL_ARG(bytes, "null pointer argument");
+    Layout l;
+    if (int rc = layout_of(dtype, sequences, drafts, cols, l)) return rc;
+    *bytes = l.total;
+    return CL_OK;
+}
+
+extern "C" int cl_verify_drafts(int dtype, const void* logits, int64_t seq_stride, int64_t row_stride,
+                                const void* draft_logits, int64_t draft_seq_stride,
+                                int64_t draft_row_stride, const int64_t* draft_tokens,
+                                int64_t ignore_index, const void* uniforms, int uniforms_dtype,
+                                int64_t sequences, int64_t drafts, int64_t cols, int64_t* tokens,
+                                int64_t* accepted, void* log_probs, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+    clear_error();
+    Layout l;
+    if (int rc = layout_of(dtype, sequences, drafts, cols, l)) return rc;
+    CL_ARG(uniforms_dtype == CL_DTYPE_F32 || uniforms_dtype == CL_DTYPE_F64,
+           "the uniform numbers must be F32 or F64");
+    CL_ARG(seq_stride >= 0 && row_stride >= 0 && draft_seq_stride >= 0 && draft_row_stride >= 0,
+           "negative strides are not supported");
+    if (sequences == 0) return CL_OK;
+    CL_ARG(logits && uniforms && tokens && accepted && log_probs && (drafts == 0 || draft_tokens),
+           "null pointer argument");
+    CL_ARG(l.total == 0 || (workspace && workspace_bytes >= l.total && aligned(workspace, 16)),
+           "workspace of %lld bytes needed (cl_verify_drafts_workspace)", (long long)l.total);
+    hipStream_t s = as_stream(stream);
+    CL_STORAGE_SWITCH(dtype, {
+        using T = scalar_t;
+        Args<T> a{};
+        a.p = static_cast<const T*>(logits);
+        a.q = static_cast<const T*>(draft_logits);
+        a.p_seq = seq_stride;
+        a.p_row = row_stride;
+        a.q_seq = draft_seq_stride;
+        a.q_row = draft_row_stride;
+        a.tokens = draft_tokens;
+        a.uniforms = uniforms;
+        a.uniforms64 = uniforms_dtype == CL_DTYPE_F64;
+        a.ignore = ignore_index;
+        a.seqs = sequences;
+        a.drafts = drafts;
+        a.cols = cols;
+        a.out = tokens;
+        a.accepted = accepted;
+        a.lp = static_cast<wide_t<T>*>(log_probs);
+        a.chunks = int(l.chunks);
+        if (l.chunks == 1) {
+            k_small<T><<<wide_grid(sequences), kThreads, 0, s>>>(a);
+            return check_launch("cl_verify_drafts");
+        }
+        char* ws = static_cast<char*>(workspace);
+        a.stats = reinterpret_cast<Stat<wide_t<T>>*>(ws + l.stats);
+        a.draws = reinterpret_cast<Draw*>(ws + l.draws);
+        a.sums = reinterpret_cast<double*>(ws + l.sums);
+        a.weights = reinterpret_cast<double*>(ws + l.weights);
+        const dim3 grid = wide_grid(sequences * l.chunks);
+        k_stats<T><<<wide_grid(sequences * (2 * drafts + 1) * l.chunks), kStatThreads, 0, s>>>(a);
+        if (int rc = check_launch("cl_verify_drafts(stats)")) return rc;
+        k_sums<T><<<grid, kThreads, 0, s>>>(a);
+        if (int rc = check_launch("cl_verify_drafts(sums)")) return rc;
+        k_weights<T><<<grid, kThreads, 0, s>>>(a);
+        if (int rc = check_launch("cl_verify_drafts(weights)")) return rc;
+        k_pick<T><<<wide_grid(sequences), kThreads, 0, s>>>(a);
+        return check_launch("cl_verify_drafts");
+    });
+}

@@ -751,6 +751,28 @@ int cl_group_sum_chosen_backward(int dtype, const void* scores, int64_t batch, i
                                  const void* pair_grad, int64_t pairs, void* grad_x,
                                  int64_t stride_batch, int64_t stride_feature, void* stream);
 
+/* Verification of drafted tokens (no reference counterpart).  logits: the target's, dtype (F32, F64,
+ * F16, BF16), [sequences, drafts + 1, cols] by two strides (elements), cols contiguous; draft_logits:
+ * the draft's, [sequences, drafts, cols] likewise, NULL for a draft that was sure of its tokens
+ * (probability 1); draft_tokens [sequences, drafts]; uniforms [sequences, drafts + 1], F32 or F64, in
+ * [0, 1).  With p and q the softmax of a position's logits, token x of position i is accepted while
+ * uniforms[i] q(x) < p(x).  The first draft_token that is ignore_index ends a sequence's drafts; a
+ * token outside of the classes has probability 0.  Behind the accepted tokens one is drawn by
+ * uniforms[drafts], the first j with sum_(k <= j) w_k > uniforms[drafts] sum_k w_k: w = max(p - q, 0)
+ * where a token was refused, p where none was left, or where max(p - q, 0) is 0 everywhere or NaN.
+ * tokens [sequences, drafts + 1]: these, then ignore_index; accepted [sequences]: how many were;
+ * log_probs [sequences, drafts + 1] (fp32, fp64 for F64): the target's, then 0.  Where p is no
+ * probability (NaN, infinite logits, none above -infinity) no token is drawn: ignore_index and NaN.
+ * The draw's sums are in fp64.  workspace: cl_verify_drafts_workspace bytes, on 16 bytes. */
+int cl_verify_drafts_workspace(int dtype, int64_t sequences, int64_t drafts, int64_t cols,
+                               int64_t* bytes);
+int cl_verify_drafts(int dtype, const void* logits, int64_t seq_stride, int64_t row_stride,
+                     const void* draft_logits, int64_t draft_seq_stride, int64_t draft_row_stride,
+                     const int64_t* draft_tokens, int64_t ignore_index, const void* uniforms,
+                     int uniforms_dtype, int64_t sequences, int64_t drafts, int64_t cols,
+                     int64_t* tokens, int64_t* accepted, void* log_probs, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 /* -------------------------------------------------------------------------------------------
  * Dropout whose mask is a function of (seed, offset, row, column) and is not stored (no
  * counterpart in the reference).  Philox 4x32-10 (Salmon et al., SC'11) with key seed and
