@@ -45,39 +45,35 @@ __device__ __forceinline__ A kept_product(A a, A b) {
     return r == A(0) && a != A(0) && b != A(0) ? least(r) : r;
 }
 
-template <bool MIX, typename A>
-__device__ __forceinline__ A input_of(A g, A x) {
-    if constexpr (MIX)
-        return g == A(1) ? A(0) : (A(1) - g) * x;
-    else
-        return x;
+__device__ __forceinline__ float least_magnitude(float a, float b) {
+    return __builtin_fminf(a, __builtin_fabsf(b));
+}
+__device__ __forceinline__ double least_magnitude(double a, double b) {
+    return __builtin_fmin(a, __builtin_fabs(b));
 }
 
-// The map of consecutive steps.
-template <typename A>
-struct Map {
-    A a = A(1), b = A(0);
-    bool dropped = false;
-    __device__ __forceinline__ void then(A g, A in) {
-        b = apply(g, b, in);
-        a *= g;
-        dropped |= g == A(0);
-    }
-    __device__ __forceinline__ A factor() const {
-        return dropped ? A(0) : a == A(0) ? least(a) : a;
-    }
-};
+// One step.  The rules of the ends of the gate differ from plain arithmetic only where something is
+// not finite, and what is not finite stays so (0 * inf and 0 * NaN are NaN): a walk is taken in plain
+// arithmetic, and again by the rules (EXACT) if its last value is not finite.  That saves three of some
+// ten instructions an element, and the scalar registers of a mask for each.
+template <bool EXACT, bool MIX, typename A>
+__device__ __forceinline__ A step(A g, A x, A h) {
+    A in = x;
+    if constexpr (MIX) in = EXACT && g == A(1) ? A(0) : (A(1) - g) * x;
+    if constexpr (EXACT) return apply(g, h, in);
+    return fma(g, h, in);
+}
 
-// The same of the gradients, from the last step to the first.
-template <typename A>
+// The gradient that goes on to the step before.
+template <bool EXACT, typename A>
 __device__ __forceinline__ A back_of(A g, A whole) {
-    return g == A(0) ? A(0) : g * whole;
+    return EXACT && g == A(0) ? A(0) : g * whole;
 }
 
-template <bool MIX, typename A>
+template <bool EXACT, bool MIX, typename A>
 __device__ __forceinline__ void gradients(A g, A x, A before, A whole, A& gx, A& gg) {
     if constexpr (MIX) {
-        gx = g == A(1) ? A(0) : (A(1) - g) * whole;
+        gx = EXACT && g == A(1) ? A(0) : (A(1) - g) * whole;
         gg = whole * (before - x);
     } else {
         gx = whole;
@@ -85,19 +81,90 @@ __device__ __forceinline__ void gradients(A g, A x, A before, A whole, A& gx, A&
     }
 }
 
+template <typename A>
+__device__ __forceinline__ bool finite(A v) {
+    return __builtin_isfinite(v);
+}
+
+// The map of consecutive steps.
+template <typename A>
+struct Map {
+    A a = A(1), b = A(0), lowest = A(1);  // lowest: of the gates' magnitudes
+    template <bool EXACT, bool MIX>
+    __device__ __forceinline__ void then(A g, A x) {
+        b = step<EXACT, MIX>(g, x, b);
+        factor_by(g);
+    }
+    __device__ __forceinline__ void factor_by(A g) {
+        a *= g;
+        lowest = least_magnitude(lowest, g);
+    }
+    // 0 only by a gate of 0
+    __device__ __forceinline__ A factor() const {
+        return lowest == A(0) ? A(0) : a == A(0) ? least(a) : a;
+    }
+};
+
+// N elements of an access of 8 or 16 bytes at any address that is a multiple of the element size.  They
+// stay as they were loaded until they are used: unpacked where the loads of a partial access and of a
+// whole one meet, each load of 16-bit elements would be waited for by itself (a stretch of 16 loads
+// took 11 us).
+typedef uint32_t pair2 __attribute__((ext_vector_type(2), aligned(2)));
+
 template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> load_part(const T* p, int count, T fill) {
-    if (count >= N) return pload<T, N>(p);
-    Pack<T, N> r;
+struct Few {
+    using Access = std::conditional_t<
+        N == 1, std::conditional_t<sizeof(T) == 2, uint16_t,
+                                   std::conditional_t<sizeof(T) == 4, uint32_t, uint64_t>>,
+        std::conditional_t<N * sizeof(T) == 8, pair2, quad_of<T>>>;
+    struct Elements {
+        T v[N];
+    };
+    Access w;
+
+    __device__ __forceinline__ T operator[](int e) const {
+        return __builtin_bit_cast(Elements, w).v[e];
+    }
+    __device__ __forceinline__ static Few of(const Elements& e) {
+        return {__builtin_bit_cast(Access, e)};
+    }
+    __device__ __forceinline__ static Few all(T v) {
+        Elements e;
 #pragma unroll
-    for (int e = 0; e < N; ++e) r.v[e] = e < count ? p[e] : fill;
-    return r;
+        for (int k = 0; k < N; ++k) e.v[k] = v;
+        return of(e);
+    }
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Few<T, N> load_whole(const T* p) {
+    return {*reinterpret_cast<const typename Few<T, N>::Access*>(p)};
 }
 
 template <typename T, int N>
-__device__ __forceinline__ void store_part(T* p, const Pack<T, N>& r, int count) {
+__device__ __forceinline__ Few<T, N> load_part(const T* p, int count, T fill) {
+    if (count >= N) return load_whole<T, N>(p);
+    typename Few<T, N>::Elements r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r.v[e] = e < count ? p[e] : fill;
+    return Few<T, N>::of(r);
+}
+
+// through: past the caches (non-temporal)
+template <typename T, int N>
+__device__ __forceinline__ void store_whole(T* p, const typename Few<T, N>::Elements& r,
+                                            bool through = false) {
+    auto* const to = reinterpret_cast<typename Few<T, N>::Access*>(p);
+    if (through)
+        __builtin_nontemporal_store(Few<T, N>::of(r).w, to);
+    else
+        *to = Few<T, N>::of(r).w;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_part(T* p, const typename Few<T, N>::Elements& r, int count) {
     if (count >= N) {
-        pstore<T, N>(p, r);
+        store_whole<T, N>(p, r);
         return;
     }
 #pragma unroll
@@ -135,28 +202,45 @@ struct Args {
     int64_t per_segment;     // stretches
     FastDiv tiles, outers;   // rows: workgroups of an outer place, outer places
     int64_t groups;
+    // Rows: outputs past the 256 MiB cache from 96 MiB on, where what comes next would not find them
+    // in it (134 MB each: forward 94 -> 86 us, backward 135 -> 128; 66 MB: 62 -> 66).
+    bool through;
 };
+
+// The place of this workgroup's work: consecutive workgroups go to the 8 XCDs in turn, each with an L2 of
+// its own, so each XCD gets a run of neighbours.  Two tiles that share lines of memory (64 bytes of a
+// row each) otherwise fetch every line twice.
+__device__ __forceinline__ int64_t neighbour_index(int64_t groups) {
+    const uint32_t b = uint32_t(group_index()), n = uint32_t(groups);
+    if (b >= n) return b;
+    const uint32_t x = b & 7, rest = n & 7;
+    return x * (n >> 3) + (x < rest ? x : rest) + (b >> 3);
+}
 
 // ---------------------------------------------------------------- inner contiguous
 //
-// FL lanes of 16 bytes side by side, TG groups of C steps each one after the other: a stretch is
-// TG * C steps.  The groups' maps go through LDS; one thread per inner place scans them, 32 groups of
-// 8 steps taking some 600 cycles of the 11000 that their bytes take.
-template <typename T, int FL, int TG, int C>
+// FL lanes side by side, of VEC places, TG groups of C steps each one after the other: a stretch is
+// TG * C steps.  The groups' maps go through LDS; one thread per inner place scans them.  While a
+// stretch is worked on, the loads of the next one are under way.
+//
+// Every access is a whole one: the last lane of a row starts VEC places before its end, beside (and
+// doing again) what its neighbour does, steps behind the last one are read from it and then replaced
+// by ones that change nothing.  Rows of fewer than four places take one place a lane.
+template <typename T, int FL, int TG, int C, int VEC>
 struct Tile {
     using A = wide_t<T>;
-    static constexpr int VEC = wide_vec<T>();
+    using V = Few<T, VEC>;
     static constexpr int NT = FL * TG;
     static constexpr int PLACES = FL * VEC;
     static constexpr int STRETCH = TG * C;
     static constexpr int PER = (PLACES + NT - 1) / NT;  // places of a scanning thread
 
-    int fl, tg, count;
+    int fl, tg;
     int64_t segment, o, i0, i;
-    bool live;
+    bool live, writes;
 
     __device__ __forceinline__ Tile(const Args<T>& a) {
-        const int64_t group = group_index();
+        const int64_t group = neighbour_index(a.groups);
         live = group < a.groups;
         const uint32_t rest = fast_div(uint32_t(group), a.tiles);
         segment = fast_div(rest, a.outers);
@@ -164,14 +248,56 @@ struct Tile {
         i0 = int64_t(uint32_t(group) - rest * a.tiles.d) * PLACES;
         fl = threadIdx.x % FL;
         tg = threadIdx.x / FL;
-        i = i0 + fl * VEC;
-        const int64_t left = a.inner - i;
-        count = left >= VEC ? VEC : left > 0 ? int(left) : 0;
+        i = at(fl, a.inner);
+        writes = i0 + fl * VEC < a.inner;
+    }
+    __device__ __forceinline__ int64_t at(int lane, int64_t inner) const {
+        const int64_t first = i0 + lane * VEC;
+        return first < inner - VEC ? first : inner - VEC;
+    }
+    // The inner place that place p of the tile stands for, and whether it is one of the tensor's.
+    __device__ __forceinline__ int64_t place(int p, int64_t inner) const {
+        return at(p / VEC, inner) + p % VEC;
     }
     __device__ __forceinline__ bool scans(int p, int64_t inner) const {
-        return p < PLACES && i0 + p < inner;
+        return p < PLACES && i0 + p / VEC * VEC < inner;
+    }
+    // A thread's steps of stretch s; those behind the last one as `fill`.
+    __device__ __forceinline__ void load(V (&v)[C], const Seq<const T>& from, int64_t s, int64_t time,
+                                         T fill) const {
+        const T* p = from.p + o * from.so + i;
+        const int64_t t = s * STRETCH + tg * C;
+        if ((s + 1) * STRETCH <= time) {
+            p += t * from.st;
+#pragma unroll
+            for (int c = 0; c < C; ++c, p += from.st) v[c] = load_whole<T, VEC>(p);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int64_t row = t + c < time ? t + c : time - 1;
+                v[c] = load_whole<T, VEC>(p + row * from.st);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (t + c >= time) v[c] = V::all(fill);
+        }
     }
 };
+
+// Between two sweeps: 16-bit elements stay packed as they were loaded.  Without this the compiler keeps
+// them widened, in twice the registers.
+template <typename V, int C>
+__device__ __forceinline__ void keep_packed(V (&v)[C]) {
+    if constexpr (sizeof(v[0][0]) == 2 && sizeof(V) == 8) {
+        typedef uint32_t words __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            words w = __builtin_bit_cast(words, v[c]);
+            asm volatile("" : "+v"(w));
+            v[c] = __builtin_bit_cast(V, w);
+        }
+    }
+}
 
 // State that segment `segment` starts with, or the gradient that it ends with (from the other side).
 template <bool BACK, typename T>
@@ -183,227 +309,319 @@ __device__ __forceinline__ wide_t<T> segment_start(const Args<T>& a, int64_t seg
     if (!a.maps) return h;
     const int64_t n = a.outer * a.inner;
     const A* m = a.maps + o * a.inner + i;
-    if constexpr (BACK) {
-        for (int64_t s = a.segments - 1; s > segment; --s) h = apply(m[2 * s * n], h, m[(2 * s + 1) * n]);
-    } else {
-        for (int64_t s = 0; s < segment; ++s) h = apply(m[2 * s * n], h, m[(2 * s + 1) * n]);
+    constexpr int U = 16;  // loads under way at once: one by one, 63 maps took 40 us
+    const int count = int(BACK ? a.segments - 1 - segment : segment);
+    for (int k0 = 0; k0 < count; k0 += U) {
+        A f[U], b[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int j = k0 + k < count ? k0 + k : count - 1;
+            const int64_t s = BACK ? a.segments - 1 - j : j;
+            f[k] = m[2 * s * n];
+            b[k] = m[(2 * s + 1) * n];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (k0 + k < count) h = apply(f[k], h, b[k]);
     }
     return h;
 }
 
-template <typename T, bool MIX, int FL, int TG, int C>
+// The maps of a thread's C steps, place by place.
+template <bool EXACT, bool MIX, typename A, typename V, int C, int VEC>
+__device__ __forceinline__ void walk_maps(const V (&gs)[C], const V (&xs)[C], Map<A> (&m)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        m[e] = Map<A>();
+#pragma unroll
+        for (int c = 0; c < C; ++c) m[e].template then<EXACT, MIX>(A(gs[c][e]), A(xs[c][e]));
+    }
+}
+
+template <bool MIX, typename A, typename V, int C, int VEC>
+__device__ __forceinline__ void maps_of(const V (&gs)[C], const V (&xs)[C], Map<A> (&m)[VEC]) {
+    walk_maps<false, MIX>(gs, xs, m);
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) fine = fine && finite(m[e].b);
+    if (!fine) walk_maps<true, MIX>(gs, xs, m);
+}
+
+// What the gradients of a thread's steps make of 0 behind them.
+template <typename A, typename V, int C, int VEC>
+__device__ __forceinline__ void backs_of(const V (&gs)[C], const V (&ds)[C], A (&q)[VEC]) {
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        q[e] = A(0);
+#pragma unroll
+        for (int c = C - 1; c >= 0; --c) q[e] = back_of<false>(A(gs[c][e]), A(ds[c][e]) + q[e]);
+        fine = fine && finite(q[e]);
+    }
+    if (!fine) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            q[e] = A(0);
+#pragma unroll
+            for (int c = C - 1; c >= 0; --c) q[e] = back_of<true>(A(gs[c][e]), A(ds[c][e]) + q[e]);
+        }
+    }
+}
+
+// Joins the groups' maps of place p in turn (BACK: from the last one): from `h` on, `to` gets what each
+// group starts with.
+template <bool BACK, int TG, int PLACES, typename A>
+__device__ __forceinline__ A join_groups(const A (&fac)[TG][PLACES], A (&to)[TG][PLACES], int p, A h) {
+    constexpr int U = TG < 16 ? TG : 16;
+#pragma unroll
+    for (int q0 = 0; q0 < TG; q0 += U) {
+        A f[U], b[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int q = BACK ? TG - 1 - q0 - k : q0 + k;
+            f[k] = fac[q][p];
+            b[k] = to[q][p];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int q = BACK ? TG - 1 - q0 - k : q0 + k;
+            to[q][p] = h;
+            h = apply(f[k], h, b[k]);
+        }
+    }
+    return h;
+}
+
+// A forward's stretch may be STARTS of the backward's, and leaves a start for each.
+template <typename T, bool MIX, int FL, int TG, int C, int VEC, int STARTS>
 __global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
     using A = wide_t<T>;
-    using W = Tile<T, FL, TG, C>;
-    constexpr int VEC = W::VEC;
+    using W = Tile<T, FL, TG, C, VEC>;
     __shared__ A fac[2][TG][W::PLACES], sum[2][TG][W::PLACES];
     const W w(a);
     if (!w.live) return;
+    const int64_t s0 = w.segment * a.per_segment / STARTS;
+    const int64_t s1 = std::min((w.segment + 1) * a.per_segment / STARTS,
+                                (a.time + W::STRETCH - 1) / W::STRETCH);
+    T* const y = a.y.p + w.o * a.y.so + w.i;
+    Few<T, VEC> xn[C], gn[C];
+    w.load(xn, a.x, s0, a.time, T(0));
+    w.load(gn, a.g, s0, a.time, T(1));
     A carry[W::PER];
 #pragma unroll
     for (int k = 0; k < W::PER; ++k) {
         const int p = threadIdx.x + k * W::NT;
-        carry[k] = w.scans(p, a.inner) ? segment_start<false>(a, w.segment, w.o, w.i0 + p) : A(0);
+        carry[k] = w.scans(p, a.inner)
+                       ? segment_start<false>(a, w.segment, w.o, w.place(p, a.inner)) : A(0);
     }
-    const int64_t s0 = w.segment * a.per_segment;
-    const int64_t s1 = std::min((w.segment + 1) * a.per_segment,
-                                (a.time + W::STRETCH - 1) / W::STRETCH);
-    const T* x = a.x.p + w.o * a.x.so + w.i;
-    const T* g = a.g.p + w.o * a.g.so + w.i;
-    T* y = a.y.p + w.o * a.y.so + w.i;
-    Pack<T, VEC> xs[C], gs[C];
-    auto load = [&](int64_t s) {
-        const int64_t t = s * W::STRETCH + w.tg * C;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int count = t + c < a.time ? w.count : 0;
-            xs[c] = load_part<T, VEC>(x + (t + c) * a.x.st, count, T(0));
-            gs[c] = load_part<T, VEC>(g + (t + c) * a.g.st, count, T(1));
-        }
-    };
     int buf = 0;
     for (int64_t s = s0; s < s1; ++s, buf ^= 1) {
-        load(s);
+        Few<T, VEC> xs[C], gs[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            xs[c] = xn[c];
+            gs[c] = gn[c];
+        }
+        if (s + 1 < s1) {
+            w.load(xn, a.x, s + 1, a.time, T(0));
+            w.load(gn, a.g, s + 1, a.time, T(1));
+        }
+        Map<A> m[VEC];
+        maps_of<MIX>(gs, xs, m);
+        keep_packed(gs);
+        keep_packed(xs);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            Map<A> m;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const A gate = A(gs[c].v[e]);
-                m.then(gate, input_of<MIX>(gate, A(xs[c].v[e])));
-            }
-            fac[buf][w.tg][w.fl * VEC + e] = m.factor();
-            sum[buf][w.tg][w.fl * VEC + e] = m.b;
+            fac[buf][w.tg][w.fl * VEC + e] = m[e].factor();
+            sum[buf][w.tg][w.fl * VEC + e] = m[e].b;
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
             const int p = threadIdx.x + k * W::NT;
             if (p >= W::PLACES) continue;
-            if (a.starts && w.scans(p, a.inner))
-                a.starts[(s * a.outer + w.o) * a.inner + w.i0 + p] = carry[k];
-            A h = carry[k];
+            carry[k] = join_groups<false>(fac[buf], sum[buf], p, carry[k]);
+            if (a.starts && w.scans(p, a.inner)) {
+                const int64_t i = w.place(p, a.inner);
 #pragma unroll
-            for (int q = 0; q < TG; ++q) {
-                const A f = fac[buf][q][p], b = sum[buf][q][p];
-                sum[buf][q][p] = h;
-                h = apply(f, h, b);
+                for (int j = 0; j < STARTS; ++j)
+                    if (j == 0 || (s * STARTS + j) * (W::STRETCH / STARTS) < a.time)
+                        a.starts[((s * STARTS + j) * a.outer + w.o) * a.inner + i] =
+                            sum[buf][TG / STARTS * j][p];
             }
-            carry[k] = h;
         }
         __syncthreads();
-        A h[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) h[e] = sum[buf][w.tg][w.fl * VEC + e];
         const int64_t t = s * W::STRETCH + w.tg * C;
+        const int steps = w.writes ? int(std::min<int64_t>(C, a.time - t)) : 0;
+        auto sweep = [&](auto exact) {
+            bool fine = true;
+            A h[VEC];
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            Pack<T, VEC> out;
+            for (int e = 0; e < VEC; ++e) h[e] = sum[buf][w.tg][w.fl * VEC + e];
+            T* to = y + t * a.y.st;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs[c].v[e]);
-                h[e] = apply(gate, h[e], input_of<MIX>(gate, A(xs[c].v[e])));
-                out.v[e] = T(h[e]);
+            for (int c = 0; c < C; ++c, to += a.y.st) {
+                typename Few<T, VEC>::Elements out;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    h[e] = step<decltype(exact)::value, MIX>(A(gs[c][e]), A(xs[c][e]), h[e]);
+                    out.v[e] = T(h[e]);
+                }
+                if (c < steps) store_whole<T, VEC>(to, out, a.through);
             }
-            if (t + c < a.time) store_part<T, VEC>(y + (t + c) * a.y.st, out, w.count);
-        }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) fine = fine && finite(h[e]);
+            return fine;
+        };
+        if (!sweep(std::false_type{})) sweep(std::true_type{});
     }
     if (w.segment == a.segments - 1) {
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
             const int p = threadIdx.x + k * W::NT;
-            if (w.scans(p, a.inner)) a.last.at(w.o, w.i0 + p) = carry[k];
+            if (w.scans(p, a.inner)) a.last.at(w.o, w.place(p, a.inner)) = carry[k];
         }
     }
 }
 
-template <typename T, bool MIX, int FL, int TG, int C>
+template <typename T, bool MIX, int FL, int TG, int C, int VEC>
 __global__ __launch_bounds__(FL * TG) void k_rows_backward(Args<T> a) {
     using A = wide_t<T>;
-    using W = Tile<T, FL, TG, C>;
-    constexpr int VEC = W::VEC;
+    using W = Tile<T, FL, TG, C, VEC>;
     __shared__ A fac[2][TG][W::PLACES], sum[2][TG][W::PLACES], back[2][TG][W::PLACES];
     const W w(a);
     if (!w.live) return;
+    const int64_t s0 = w.segment * a.per_segment;
+    const int64_t s1 = std::min((w.segment + 1) * a.per_segment,
+                                (a.time + W::STRETCH - 1) / W::STRETCH);
+    T* const gx = a.gx.p + w.o * a.gx.so + w.i;
+    T* const gg = a.gg.p + w.o * a.gg.so + w.i;
+    Few<T, VEC> xn[C], gn[C], dn[C];
+    A start[W::PER];  // states that the stretch begins with
+    auto load = [&](int64_t s) {
+        w.load(xn, a.x, s, a.time, T(0));
+        w.load(gn, a.g, s, a.time, T(1));
+        if (a.gy.p) w.load(dn, a.gy, s, a.time, T(0));
+#pragma unroll
+        for (int k = 0; k < W::PER; ++k) {
+            const int p = threadIdx.x + k * W::NT;
+            start[k] = A(0);
+            if (w.scans(p, a.inner)) {
+                const int64_t i = w.place(p, a.inner);
+                if (a.starts)
+                    start[k] = a.starts[(s * a.outer + w.o) * a.inner + i];
+                else if (a.h0.p)
+                    start[k] = a.h0.at(w.o, i);
+            }
+        }
+    };
+    if (!a.gy.p) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) dn[c] = Few<T, VEC>::all(T(0));
+    }
+    load(s1 - 1);
     // the states by the first threads, the gradients by the last ones
     const int rev = W::NT - 1 - int(threadIdx.x);
     A carry[W::PER];
 #pragma unroll
     for (int k = 0; k < W::PER; ++k) {
         const int p = rev + k * W::NT;
-        carry[k] = w.scans(p, a.inner) ? segment_start<true>(a, w.segment, w.o, w.i0 + p) : A(0);
+        carry[k] = w.scans(p, a.inner)
+                       ? segment_start<true>(a, w.segment, w.o, w.place(p, a.inner)) : A(0);
     }
-    const int64_t s0 = w.segment * a.per_segment;
-    const int64_t s1 = std::min((w.segment + 1) * a.per_segment,
-                                (a.time + W::STRETCH - 1) / W::STRETCH);
-    const T* x = a.x.p + w.o * a.x.so + w.i;
-    const T* g = a.g.p + w.o * a.g.so + w.i;
-    const T* gy = a.gy.p + w.o * a.gy.so + w.i;
-    T* gx = a.gx.p + w.o * a.gx.so + w.i;
-    T* gg = a.gg.p + w.o * a.gg.so + w.i;
     int buf = 0;
     for (int64_t s = s1 - 1; s >= s0; --s, buf ^= 1) {
-        const int64_t t = s * W::STRETCH + w.tg * C;
-        Pack<T, VEC> xs[C], gs[C], ds[C];
+        Few<T, VEC> xs[C], gs[C], ds[C];
+        A begin[W::PER];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int count = t + c < a.time ? w.count : 0;
-            xs[c] = load_part<T, VEC>(x + (t + c) * a.x.st, count, T(0));
-            gs[c] = load_part<T, VEC>(g + (t + c) * a.g.st, count, T(1));
-            ds[c] = load_part<T, VEC>(gy + (t + c) * a.gy.st, a.gy.p ? count : 0, T(0));
+            xs[c] = xn[c];
+            gs[c] = gn[c];
+            ds[c] = dn[c];
         }
 #pragma unroll
+        for (int k = 0; k < W::PER; ++k) begin[k] = start[k];
+        if (s > s0) load(s - 1);
+        Map<A> m[VEC];
+        A q[VEC];
+        maps_of<MIX>(gs, xs, m);
+        keep_packed(gs);
+        keep_packed(xs);
+        backs_of(gs, ds, q);
+        keep_packed(gs);
+        keep_packed(ds);
+#pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            Map<A> m;
-            A q = A(0);
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const A gate = A(gs[c].v[e]);
-                m.then(gate, input_of<MIX>(gate, A(xs[c].v[e])));
-            }
-#pragma unroll
-            for (int c = C - 1; c >= 0; --c) q = back_of(A(gs[c].v[e]), A(ds[c].v[e]) + q);
-            fac[buf][w.tg][w.fl * VEC + e] = m.factor();
-            sum[buf][w.tg][w.fl * VEC + e] = m.b;
-            back[buf][w.tg][w.fl * VEC + e] = q;
+            fac[buf][w.tg][w.fl * VEC + e] = m[e].factor();
+            sum[buf][w.tg][w.fl * VEC + e] = m[e].b;
+            back[buf][w.tg][w.fl * VEC + e] = q[e];
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
             const int p = threadIdx.x + k * W::NT;
-            if (p < W::PLACES) {
-                A h = A(0);
-                if (w.scans(p, a.inner)) {
-                    if (a.starts)
-                        h = a.starts[(s * a.outer + w.o) * a.inner + w.i0 + p];
-                    else if (a.h0.p)
-                        h = a.h0.at(w.o, w.i0 + p);
-                }
-#pragma unroll
-                for (int q = 0; q < TG; ++q) {
-                    const A f = fac[buf][q][p], b = sum[buf][q][p];
-                    sum[buf][q][p] = h;
-                    h = apply(f, h, b);
-                }
-            }
+            if (p < W::PLACES) join_groups<false>(fac[buf], sum[buf], p, begin[k]);
             const int r = rev + k * W::NT;
-            if (r < W::PLACES) {
-                A c = carry[k];
-#pragma unroll
-                for (int q = TG - 1; q >= 0; --q) {
-                    const A f = fac[buf][q][r], b = back[buf][q][r];
-                    back[buf][q][r] = c;
-                    c = apply(f, c, b);
-                }
-                carry[k] = c;
-            }
+            if (r < W::PLACES) carry[k] = join_groups<true>(fac[buf], back[buf], r, carry[k]);
         }
         __syncthreads();
-        A before[C][VEC], c_in[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            A h = sum[buf][w.tg][w.fl * VEC + e];
-            c_in[e] = back[buf][w.tg][w.fl * VEC + e];
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                before[c][e] = h;
-                const A gate = A(gs[c].v[e]);
-                h = apply(gate, h, input_of<MIX>(gate, A(xs[c].v[e])));
-            }
-        }
-#pragma unroll
-        for (int c = C - 1; c >= 0; --c) {
-            Pack<T, VEC> ox, og;
+        const int64_t t = s * W::STRETCH + w.tg * C;
+        const int steps = w.writes ? int(std::min<int64_t>(C, a.time - t)) : 0;
+        auto sweep = [&](auto exact) {
+            constexpr bool EXACT = decltype(exact)::value;
+            bool fine = true;
+            A before[C][VEC], c_in[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs[c].v[e]), whole = A(ds[c].v[e]) + c_in[e];
-                A dx, dg;
-                gradients<MIX>(gate, A(xs[c].v[e]), before[c][e], whole, dx, dg);
-                ox.v[e] = T(dx);
-                og.v[e] = T(dg);
-                c_in[e] = back_of(gate, whole);
+                A h = sum[buf][w.tg][w.fl * VEC + e];
+                c_in[e] = back[buf][w.tg][w.fl * VEC + e];
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    before[c][e] = h;
+                    h = step<EXACT, MIX>(A(gs[c][e]), A(xs[c][e]), h);
+                }
+                fine = fine && finite(h);
             }
-            if (t + c < a.time) {
-                if (a.gx.p) store_part<T, VEC>(gx + (t + c) * a.gx.st, ox, w.count);
-                if (a.gg.p) store_part<T, VEC>(gg + (t + c) * a.gg.st, og, w.count);
+            T* to_x = gx + (t + C - 1) * a.gx.st;
+            T* to_g = gg + (t + C - 1) * a.gg.st;
+#pragma unroll
+            for (int c = C - 1; c >= 0; --c, to_x -= a.gx.st, to_g -= a.gg.st) {
+                typename Few<T, VEC>::Elements ox, og;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const A gate = A(gs[c][e]), whole = A(ds[c][e]) + c_in[e];
+                    A dx, dg;
+                    gradients<EXACT, MIX>(gate, A(xs[c][e]), before[c][e], whole, dx, dg);
+                    ox.v[e] = T(dx);
+                    og.v[e] = T(dg);
+                    c_in[e] = back_of<EXACT>(gate, whole);
+                }
+                if (c < steps) {
+                    if (a.gx.p) store_whole<T, VEC>(to_x, ox, a.through);
+                    if (a.gg.p) store_whole<T, VEC>(to_g, og, a.through);
+                }
             }
-        }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) fine = fine && finite(c_in[e]);
+            return fine;
+        };
+        if (!sweep(std::false_type{})) sweep(std::true_type{});
     }
     if (w.segment == 0 && a.gh0.p) {
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
             const int p = rev + k * W::NT;
-            if (w.scans(p, a.inner)) a.gh0.at(w.o, w.i0 + p) = carry[k];
+            if (w.scans(p, a.inner)) a.gh0.at(w.o, w.place(p, a.inner)) = carry[k];
         }
     }
 }
 
 // The map of each segment: a group's steps lie one behind the other here.
-template <typename T, bool MIX, bool BACK, int FL, int TG>
+template <typename T, bool MIX, bool BACK, int FL, int TG, int VEC>
 __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
     using A = wide_t<T>;
-    using W = Tile<T, FL, TG, 1>;
-    constexpr int VEC = W::VEC, U = 8;
+    using W = Tile<T, FL, TG, 1, VEC>;
+    constexpr int U = 8;
     __shared__ A fac[TG][W::PLACES], sum[TG][W::PLACES];
     const W w(a);
     if (!w.live) return;
@@ -416,32 +634,38 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
     const T* d = in.p + w.o * in.so + w.i;
     const bool some = !BACK || in.p;
     Map<A> m[VEC];
+    Few<T, VEC> gs[U], ds[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) ds[u] = Few<T, VEC>::all(T(0));
     for (int64_t n = 0; n < b1 - b0; n += U) {
-        Pack<T, VEC> gs[U], ds[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t t = BACK ? b1 - 1 - n - u : b0 + n + u;
-            const int count = n + u < b1 - b0 ? w.count : 0;
-            gs[u] = load_part<T, VEC>(g + t * a.g.st, count, T(1));
-            ds[u] = load_part<T, VEC>(d + t * in.st, some ? count : 0, T(0));
+            const int64_t k = n + u < b1 - b0 ? n + u : b1 - b0 - 1;
+            const int64_t t = BACK ? b1 - 1 - k : b0 + k;
+            gs[u] = load_whole<T, VEC>(g + t * a.g.st);
+            if (some) ds[u] = load_whole<T, VEC>(d + t * in.st);
+        }
+        if (b1 - b0 - n < U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (n + u >= b1 - b0) {
+                    gs[u] = Few<T, VEC>::all(T(1));
+                    ds[u] = Few<T, VEC>::all(T(0));
+                }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs[u].v[e]), v = A(ds[u].v[e]);
+                const A gate = A(gs[u][e]), v = A(ds[u][e]);
                 if constexpr (BACK) {
-                    m[e].b = back_of(gate, v + m[e].b);
-                    m[e].a *= gate;
-                    m[e].dropped |= gate == A(0);
+                    m[e].b = back_of<true>(gate, v + m[e].b);
+                    m[e].factor_by(gate);
                 } else {
-                    m[e].then(gate, input_of<MIX>(gate, v));
+                    m[e].template then<true, MIX>(gate, v);
                 }
             }
-        // a product of many gates: kept from 0 now and then
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-            if (m[e].a == A(0) && !m[e].dropped) m[e].a = least(m[e].a);
+        }
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -460,7 +684,7 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
             f = kept_product(f, fac[r][p]);
         }
         const int64_t n = a.outer * a.inner;
-        A* to = a.maps + 2 * w.segment * n + w.o * a.inner + w.i0 + p;
+        A* to = a.maps + 2 * w.segment * n + w.o * a.inner + w.place(p, a.inner);
         to[0] = f;
         to[n] = b;
     }
@@ -470,11 +694,10 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
 template <typename T, bool MIX, bool BACK>
 __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
     using A = wide_t<T>;
-    using W = Tile<T, kThreads, 1, 1>;
-    constexpr int VEC = W::VEC;
+    constexpr int VEC = wide_vec<T>();
     // the threads of a workgroup go on to the next outer place where a row has fewer lanes
     const int64_t lanes = (a.inner + VEC - 1) / VEC;
-    const int64_t item = group_index() * kThreads + threadIdx.x;
+    const int64_t item = neighbour_index(a.groups) * kThreads + threadIdx.x;
     if (item >= a.outer * lanes) return;
     int64_t o, lane;
     if (a.outer * lanes < (int64_t(1) << 31)) {
@@ -501,14 +724,13 @@ __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
     };
     if constexpr (!BACK) {
         A h[VEC];
-        Pack<T, VEC> xs = from(a.x, 0, T(0)), gs = from(a.g, 0, T(0));
+        Few<T, VEC> xs = from(a.x, 0, T(0)), gs = from(a.g, 0, T(0));
         states(a.h0, h);
         for (int64_t t = 0; t < a.time; ++t) {
-            Pack<T, VEC> out;
+            typename Few<T, VEC>::Elements out;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs.v[e]);
-                h[e] = apply(gate, h[e], input_of<MIX>(gate, A(xs.v[e])));
+                h[e] = step<true, MIX>(A(gs[e]), A(xs[e]), h[e]);
                 out.v[e] = T(h[e]);
             }
             store_part<T, VEC>(a.y.p + o * a.y.so + t * a.y.st + i, out, count);
@@ -521,7 +743,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
     } else {
         constexpr int MOST = 2;  // kFew
         A before[MOST][VEC], c[VEC];
-        Pack<T, VEC> xs[MOST], gs[MOST], ds[MOST];
+        Few<T, VEC> xs[MOST], gs[MOST], ds[MOST];
 #pragma unroll
         for (int t = 0; t < MOST; ++t)
             if (t < a.time) {
@@ -534,22 +756,21 @@ __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
         if (a.time > 1) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs[0].v[e]);
-                before[1][e] = apply(gate, before[0][e], input_of<MIX>(gate, A(xs[0].v[e])));
+                before[1][e] = step<true, MIX>(A(gs[0][e]), A(xs[0][e]), before[0][e]);
             }
         }
 #pragma unroll
         for (int t = MOST - 1; t >= 0; --t) {
             if (t >= a.time) continue;
-            Pack<T, VEC> ox, og;
+            typename Few<T, VEC>::Elements ox, og;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs[t].v[e]), whole = A(ds[t].v[e]) + c[e];
+                const A gate = A(gs[t][e]), whole = A(ds[t][e]) + c[e];
                 A dx, dg;
-                gradients<MIX>(gate, A(xs[t].v[e]), before[t][e], whole, dx, dg);
+                gradients<true, MIX>(gate, A(xs[t][e]), before[t][e], whole, dx, dg);
                 ox.v[e] = T(dx);
                 og.v[e] = T(dg);
-                c[e] = back_of(gate, whole);
+                c[e] = back_of<true>(gate, whole);
             }
             if (a.gx.p) store_part<T, VEC>(a.gx.p + o * a.gx.so + t * a.gx.st + i, ox, count);
             if (a.gg.p) store_part<T, VEC>(a.gg.p + o * a.gg.so + t * a.gg.st + i, og, count);
@@ -630,7 +851,7 @@ __device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
     return apply(pa, from, pb);
 }
 
-template <typename T, int L>
+template <typename T, int L, bool BACK>
 struct Line {
     static constexpr int VEC = wide_vec<T>();
     static constexpr int STRETCH = L * VEC;
@@ -641,7 +862,9 @@ struct Line {
 
     __device__ __forceinline__ Line(const Args<T>& a) {
         const int64_t rows = a.outer * a.inner;
-        int64_t group = group_index();
+        // (backward 176 us with the workgroups in turn, 171 by neighbours; forward 106 and 121)
+        int64_t group = BACK ? neighbour_index(a.groups) : group_index();
+        live = group < a.groups;
         segment = 0;
         if (a.segments > 1) {  // then groups < 2^31
             segment = fast_div(uint32_t(group), a.tiles);
@@ -649,7 +872,7 @@ struct Line {
         }
         row = group * ROWS + threadIdx.x / L;
         l = threadIdx.x % L;
-        live = group_index() < a.groups && row < rows;
+        live = live && row < rows;
         if (rows < (int64_t(1) << 31)) {
             o = fast_div(uint32_t(row), a.outers);
         } else {
@@ -663,10 +886,24 @@ struct Line {
     }
 };
 
+// The map of a lane's steps.
+template <bool MIX, typename A, typename V>
+__device__ __forceinline__ void line_map(const V& g, const V& x, Map<A>& m) {
+    constexpr int VEC = sizeof(V) / sizeof(g[0]);
+    m = Map<A>();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) m.template then<false, MIX>(A(g[e]), A(x[e]));
+    if (!finite(m.b)) {
+        m = Map<A>();
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m.template then<true, MIX>(A(g[e]), A(x[e]));
+    }
+}
+
 template <typename T, bool MIX, int L>
 __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
     using A = wide_t<T>;
-    using W = Line<T, L>;
+    using W = Line<T, L, false>;
     constexpr int VEC = W::VEC;
     const W w(a);
     const T* x = a.x.p + w.o * a.x.so + w.i * a.x.si;
@@ -676,11 +913,11 @@ __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
     const int64_t t1 = std::min(a.time, t0 + a.per_segment * W::STRETCH);
     int64_t t = t0 + w.l * VEC;
     int count = w.count(t, a.time);
-    Pack<T, VEC> xs = load_part<T, VEC>(x + t, count, T(0)), gs = load_part<T, VEC>(g + t, count, T(1));
+    Few<T, VEC> xs = load_part<T, VEC>(x + t, count, T(0)), gs = load_part<T, VEC>(g + t, count, T(1));
     A carry = w.live ? segment_start<false>(a, w.segment, w.o, w.i) : A(0);
     A h = carry;
     for (int64_t s = t0; s < t1; s += W::STRETCH) {
-        const Pack<T, VEC> xn = xs, gn = gs;
+        const Few<T, VEC> xn = xs, gn = gs;
         const int now = count;
         const int64_t at = t;
         if constexpr (L == 64) {  // the next stretch's loads are under way during this one's scan
@@ -694,21 +931,20 @@ __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
                 a.starts[s / W::STRETCH * (a.outer * a.inner) + w.row] = carry;
         }
         Map<A> m;
-        A in[VEC];
+        line_map<MIX>(gn, xn, m);
+        const A begin = scan_lanes<L, false>(m.factor(), m.b, carry);
+        auto sweep = [&](auto exact) {
+            typename Few<T, VEC>::Elements out;
+            h = begin;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const A gate = A(gn.v[e]);
-            in[e] = input_of<MIX>(gate, A(xn.v[e]));
-            m.then(gate, in[e]);
-        }
-        h = scan_lanes<L, false>(m.factor(), m.b, carry);
-        Pack<T, VEC> out;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            h = apply(A(gn.v[e]), h, in[e]);
-            out.v[e] = T(h);
-        }
-        store_part<T, VEC>(y + at, out, now);
+            for (int e = 0; e < VEC; ++e) {
+                h = step<decltype(exact)::value, MIX>(A(gn[e]), A(xn[e]), h);
+                out.v[e] = T(h);
+            }
+            store_part<T, VEC>(y + at, out, now);
+        };
+        sweep(std::false_type{});
+        if (!finite(h)) sweep(std::true_type{});
     }
     if (w.live && w.segment == a.segments - 1 && w.l == L - 1) a.last.at(w.o, w.i) = h;
 }
@@ -716,7 +952,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
 template <typename T, bool MIX, int L>
 __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
     using A = wide_t<T>;
-    using W = Line<T, L>;
+    using W = Line<T, L, true>;
     constexpr int VEC = W::VEC;
     const W w(a);
     const T* x = a.x.p + w.o * a.x.so + w.i * a.x.si;
@@ -728,7 +964,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
     const int64_t s1 = std::min(s0 + a.per_segment, (a.time + W::STRETCH - 1) / W::STRETCH);
     int64_t t = (s1 - 1) * W::STRETCH + w.l * VEC;
     int count = 0;
-    Pack<T, VEC> xs, gs, ds;
+    Few<T, VEC> xs, gs, ds;
     A start = A(0);
     auto load = [&](int64_t s) {
         count = w.count(t, a.time);
@@ -746,7 +982,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
     A carry = w.live ? segment_start<true>(a, w.segment, w.o, w.i) : A(0);
     A c = carry;
     for (int64_t s = s1 - 1; s >= s0; --s) {
-        const Pack<T, VEC> xn = xs, gn = gs, dn = ds;
+        const Few<T, VEC> xn = xs, gn = gs, dn = ds;
         const int now = count;
         const int64_t at = t;
         A begin = start;
@@ -757,36 +993,42 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
             }
         }
         Map<A> m;
-        A q = A(0), before[VEC];
+        line_map<MIX>(gn, xn, m);
+        A q = A(0);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const A gate = A(gn.v[e]);
-            before[e] = input_of<MIX>(gate, A(xn.v[e]));
-            m.then(gate, before[e]);
+        for (int e = VEC - 1; e >= 0; --e) q = back_of<false>(A(gn[e]), A(dn[e]) + q);
+        if (!finite(q)) {
+            q = A(0);
+#pragma unroll
+            for (int e = VEC - 1; e >= 0; --e) q = back_of<true>(A(gn[e]), A(dn[e]) + q);
         }
-#pragma unroll
-        for (int e = VEC - 1; e >= 0; --e) q = back_of(A(gn.v[e]), A(dn.v[e]) + q);
         const A f = m.factor();
-        A h = scan_lanes<L, false>(f, m.b, begin);
-        c = scan_lanes<L, true>(f, q, carry);
+        const A h0 = scan_lanes<L, false>(f, m.b, begin);
+        const A c0 = scan_lanes<L, true>(f, q, carry);
+        auto sweep = [&](auto exact) {
+            constexpr bool EXACT = decltype(exact)::value;
+            A h = h0, before[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const A in = before[e];
-            before[e] = h;
-            h = apply(A(gn.v[e]), h, in);
-        }
-        Pack<T, VEC> ox, og;
+            for (int e = 0; e < VEC; ++e) {
+                before[e] = h;
+                h = step<EXACT, MIX>(A(gn[e]), A(xn[e]), h);
+            }
+            c = c0;
+            typename Few<T, VEC>::Elements ox, og;
 #pragma unroll
-        for (int e = VEC - 1; e >= 0; --e) {
-            const A gate = A(gn.v[e]), whole = A(dn.v[e]) + c;
-            A dx, dg;
-            gradients<MIX>(gate, A(xn.v[e]), before[e], whole, dx, dg);
-            ox.v[e] = T(dx);
-            og.v[e] = T(dg);
-            c = back_of(gate, whole);
-        }
-        if (a.gx.p) store_part<T, VEC>(gx + at, ox, now);
-        if (a.gg.p) store_part<T, VEC>(gg + at, og, now);
+            for (int e = VEC - 1; e >= 0; --e) {
+                const A gate = A(gn[e]), whole = A(dn[e]) + c;
+                A dx, dg;
+                gradients<EXACT, MIX>(gate, A(xn[e]), before[e], whole, dx, dg);
+                ox.v[e] = T(dx);
+                og.v[e] = T(dg);
+                c = back_of<EXACT>(gate, whole);
+            }
+            if (a.gx.p) store_part<T, VEC>(gx + at, ox, now);
+            if (a.gg.p) store_part<T, VEC>(gg + at, og, now);
+            return finite(h) && finite(c);
+        };
+        if (!sweep(std::false_type{})) sweep(std::true_type{});
     }
     if (w.live && w.segment == 0 && w.l == 0 && a.gh0.p) a.gh0.at(w.o, w.i) = c;
 }
@@ -794,7 +1036,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
 template <typename T, bool MIX, bool BACK>
 __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
     using A = wide_t<T>;
-    using W = Line<T, 64>;
+    using W = Line<T, 64, BACK>;
     constexpr int VEC = W::VEC;
     const W w(a);
     const T* g = a.g.p + w.o * a.g.so + w.i * a.g.si;
@@ -811,24 +1053,19 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
         // (BACK: the last, shorter access first)
         const int64_t t = BACK ? b0 + (b1 - b0 - 1 - n) / VEC * VEC : b0 + n;
         const int count = int(std::min<int64_t>(VEC, b1 - t));
-        const Pack<T, VEC> gs = load_part<T, VEC>(g + t, count, T(1));
-        const Pack<T, VEC> ds = load_part<T, VEC>(d + t, some ? count : 0, T(0));
+        const Few<T, VEC> gs = load_part<T, VEC>(g + t, count, T(1));
+        const Few<T, VEC> ds = load_part<T, VEC>(d + t, some ? count : 0, T(0));
         if constexpr (BACK) {
 #pragma unroll
             for (int e = VEC - 1; e >= 0; --e) {
-                const A gate = A(gs.v[e]);
-                m.b = back_of(gate, A(ds.v[e]) + m.b);
-                m.a *= gate;
-                m.dropped |= gate == A(0);
+                const A gate = A(gs[e]);
+                m.b = back_of<true>(gate, A(ds[e]) + m.b);
+                m.factor_by(gate);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const A gate = A(gs.v[e]);
-                m.then(gate, input_of<MIX>(gate, A(ds.v[e])));
-            }
+            for (int e = 0; e < VEC; ++e) m.template then<true, MIX>(A(gs[e]), A(ds[e]));
         }
-        if (m.a == A(0) && !m.dropped) m.a = least(m.a);
     }
     // the lanes' maps in a row: what the last lane (BACK: the first) makes of the state 0, and of a
     // factor
@@ -854,7 +1091,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
 // ---------------------------------------------------------------- launches
 
 // How a call goes: which kernels, and into how many segments of how many stretches.
-enum Way { kRowsFew, kRowsShort, kRowsLong, kLines4, kLines16, kLines64 };
+enum Way { kRowsFew, kRowsShort, kRowsLong, kRowsNarrow, kLines4, kLines16, kLines64 };
 
 struct Route {
     Way way;
@@ -863,6 +1100,7 @@ struct Route {
     int segments;
     int64_t per_segment;  // stretches
     int64_t units;        // workgroups of one segment
+    int64_t tiles;        // rows: workgroups (kRowsFew: lanes) of an outer place
 };
 
 // Segments where there are fewer workgroups than would fill the chip's 256 CUs: as many as bring
@@ -871,13 +1109,18 @@ void cut(Route& r) {
     int64_t n = 1;
     if (r.units < 256) n = std::min<int64_t>({1024 / r.units, r.stretches / 2, kMaxSegments});
     if (n < 1) n = 1;
-    r.per_segment = ceil_div(r.stretches, n);
+    r.per_segment = (ceil_div(r.stretches, n) + 1) / 2 * 2;  // (a forward may take two at once)
     r.segments = int(ceil_div(r.stretches, r.per_segment));
 }
 
+// Places of a lane of the kernels for inner contiguous.
+int64_t places_of(int dtype) { return dtype == CL_DTYPE_F64 ? 2 : 4; }
+int64_t vec_of(int dtype) { return dtype == CL_DTYPE_F64 ? 2 : dtype == CL_DTYPE_F32 ? 4 : 8; }
+
 // time contiguous: outer * inner lines; else inner contiguous
-Route route_of(int64_t vec, bool lines, int64_t outer, int64_t time, int64_t inner) {
+Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner) {
     Route r{};
+    const int64_t vec = vec_of(dtype), places = places_of(dtype);
     if (lines) {
         const int l = time <= 4 * vec ? 4 : time <= 16 * vec ? 16 : 64;
         r.way = l == 4 ? kLines4 : l == 16 ? kLines16 : kLines64;
@@ -886,13 +1129,14 @@ Route route_of(int64_t vec, bool lines, int64_t outer, int64_t time, int64_t inn
     } else if (time <= kFew) {
         r.way = kRowsFew;
         r.stretch = kFew;
-        r.units = ceil_div(outer * ceil_div(inner, vec), kThreads);
+        r.tiles = ceil_div(inner, vec);
+        r.units = ceil_div(outer * r.tiles, kThreads);
     } else {
-        // 64 lanes side by side and 4 groups of 8 steps, or 8 and 32
-        const bool few = time <= 32;
-        r.way = few ? kRowsShort : kRowsLong;
-        r.stretch = few ? 32 : 256;
-        r.units = outer * ceil_div(inner, (few ? 64 : 8) * vec);
+        // 64 lanes side by side and 4 groups of 8 steps, or 16 and 32 (backward: of 4)
+        r.way = inner < places ? kRowsNarrow : time <= 32 ? kRowsShort : kRowsLong;
+        r.stretch = r.way == kRowsShort ? 32 : r.way == kRowsLong ? 128 : 256;
+        r.tiles = r.way == kRowsNarrow ? 1 : ceil_div(inner, (r.way == kRowsShort ? 64 : 16) * places);
+        r.units = outer * r.tiles;
     }
     r.stretches = ceil_div(time, r.stretch);
     cut(r);
@@ -907,26 +1151,24 @@ int route_args(Args<T>& a, const Route& r, bool lines, void* workspace) {
     if (r.stretches <= 1) a.starts = nullptr;
     a.groups = r.units * r.segments;
     CL_ARG(a.groups < (int64_t(1) << 31), "too many sequences for one call");
-    if (lines) {
-        a.tiles = make_fastdiv(uint32_t(r.units));
-        a.outers = make_fastdiv(uint32_t(std::min<int64_t>(a.inner, INT32_MAX)));
-    } else {
-        const int64_t lanes = ceil_div(a.inner, wide_vec<T>());
-        const int64_t tiles = r.way == kRowsFew ? lanes : ceil_div(lanes, r.way == kRowsShort ? 64 : 8);
-        a.tiles = make_fastdiv(uint32_t(std::min<int64_t>(tiles, INT32_MAX)));
-        a.outers = make_fastdiv(uint32_t(std::min<int64_t>(a.outer, INT32_MAX)));
-    }
+    a.through = double(a.outer) * a.time * a.inner * sizeof(T) >= double(96 << 20);
+    const int64_t most = INT32_MAX;
+    a.tiles = make_fastdiv(uint32_t(std::min(lines ? r.units : r.tiles, most)));
+    a.outers = make_fastdiv(uint32_t(std::min(lines ? a.inner : a.outer, most)));
     return CL_OK;
 }
 
 template <typename T, bool MIX, bool BACK>
 int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
+    constexpr int P = sizeof(T) == 8 ? 2 : 4;
     const dim3 grid = wide_grid(a.groups);
     if (r.segments > 1) {
         if (r.way == kLines64)
             k_lines_maps<T, MIX, BACK><<<grid, kThreads, 0, s>>>(a);
+        else if (r.way == kRowsNarrow)
+            k_rows_maps<T, MIX, BACK, 8, 32, 1><<<grid, kThreads, 0, s>>>(a, int(r.stretch));
         else
-            k_rows_maps<T, MIX, BACK, 8, 32><<<grid, kThreads, 0, s>>>(a, int(r.stretch));
+            k_rows_maps<T, MIX, BACK, 16, 16, P><<<grid, kThreads, 0, s>>>(a, int(r.stretch));
         if (int rc = check_launch("cl_recurrence(maps)")) return rc;
     }
     switch (r.way) {
@@ -935,15 +1177,21 @@ int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
             break;
         case kRowsShort:
             if constexpr (BACK)
-                k_rows_backward<T, MIX, 64, 4, 8><<<grid, kThreads, 0, s>>>(a);
+                k_rows_backward<T, MIX, 64, 4, 8, P><<<grid, kThreads, 0, s>>>(a);
             else
-                k_rows_forward<T, MIX, 64, 4, 8><<<grid, kThreads, 0, s>>>(a);
+                k_rows_forward<T, MIX, 64, 4, 8, P, 1><<<grid, kThreads, 0, s>>>(a);
             break;
         case kRowsLong:
             if constexpr (BACK)
-                k_rows_backward<T, MIX, 8, 32, 8><<<grid, kThreads, 0, s>>>(a);
+                k_rows_backward<T, MIX, 16, 32, 4, P><<<grid, 512, 0, s>>>(a);
             else
-                k_rows_forward<T, MIX, 8, 32, 8><<<grid, kThreads, 0, s>>>(a);
+                k_rows_forward<T, MIX, 16, 32, 8, P, 2><<<grid, 512, 0, s>>>(a);
+            break;
+        case kRowsNarrow:
+            if constexpr (BACK)
+                k_rows_backward<T, MIX, 8, 32, 8, 1><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_rows_forward<T, MIX, 8, 32, 8, 1, 1><<<grid, kThreads, 0, s>>>(a);
             break;
         case kLines4:
             if constexpr (BACK)
@@ -1024,8 +1272,6 @@ int states(States<A>& s, const void* p, const int64_t* strides, const Dims& d, b
     return CL_OK;
 }
 
-int vec_of(int dtype) { return dtype == CL_DTYPE_F64 ? 2 : dtype == CL_DTYPE_F32 ? 4 : 8; }
-
 int sizes(int dtype, int order, int64_t batch, int64_t time, int64_t features, Dims& d, Route& r,
           int64_t& starts, int64_t& bytes) {
     CL_ARG(dtype >= CL_DTYPE_F32 && dtype <= CL_DTYPE_BF16,
@@ -1033,7 +1279,7 @@ int sizes(int dtype, int order, int64_t batch, int64_t time, int64_t features, D
     if (int rc = dims_of(order, batch, time, features, d)) return rc;
     starts = bytes = 0;
     if (batch == 0 || time == 0 || features == 0) return CL_OK;
-    r = route_of(vec_of(dtype), d.lines, d.outer, d.time, d.inner);
+    r = route_of(dtype, d.lines, d.outer, d.time, d.inner);
     const int64_t n = batch * features;
     starts = r.stretches > 1 ? r.stretches * n : 0;
     bytes = r.segments > 1 ? 2 * r.segments * n * (dtype == CL_DTYPE_F64 ? 8 : 4) : 0;
