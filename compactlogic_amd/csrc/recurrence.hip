@@ -150,12 +150,11 @@ __device__ __forceinline__ Few<T, N> load_part(const T* p, int count, T fill) {
     return Few<T, N>::of(r);
 }
 
-// through: past the caches (non-temporal)
-template <typename T, int N>
-__device__ __forceinline__ void store_whole(T* p, const typename Few<T, N>::Elements& r,
-                                            bool through = false) {
+// THROUGH: past the caches (non-temporal)
+template <typename T, int N, bool THROUGH = false>
+__device__ __forceinline__ void store_whole(T* p, const typename Few<T, N>::Elements& r) {
     auto* const to = reinterpret_cast<typename Few<T, N>::Access*>(p);
-    if (through)
+    if constexpr (THROUGH)
         __builtin_nontemporal_store(Few<T, N>::of(r).w, to);
     else
         *to = Few<T, N>::of(r).w;
@@ -202,9 +201,6 @@ struct Args {
     int64_t per_segment;     // stretches
     FastDiv tiles, outers;   // rows: workgroups of an outer place, outer places
     int64_t groups;
-    // Rows: outputs past the 256 MiB cache from 96 MiB on, where what comes next would not find them
-    // in it (134 MB each: forward 94 -> 86 us, backward 135 -> 128; 66 MB: 62 -> 66).
-    bool through;
 };
 
 // The place of this workgroup's work: consecutive workgroups go to the 8 XCDs in turn, each with an L2 of
@@ -271,7 +267,7 @@ struct Tile {
             p += t * from.st;
 #pragma unroll
             for (int c = 0; c < C; ++c, p += from.st) v[c] = load_whole<T, VEC>(p);
-        } else {
+        } else if (t < time) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
                 const int64_t row = t + c < time ? t + c : time - 1;
@@ -280,6 +276,9 @@ struct Tile {
 #pragma unroll
             for (int c = 0; c < C; ++c)
                 if (t + c >= time) v[c] = V::all(fill);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[c] = V::all(fill);
         }
     }
 };
@@ -393,7 +392,7 @@ __device__ __forceinline__ A join_groups(const A (&fac)[TG][PLACES], A (&to)[TG]
 }
 
 // A forward's stretch may be STARTS of the backward's, and leaves a start for each.
-template <typename T, bool MIX, int FL, int TG, int C, int VEC, int STARTS>
+template <typename T, bool MIX, int FL, int TG, int C, int VEC, int STARTS, bool THROUGH = false>
 __global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
     using A = wide_t<T>;
     using W = Tile<T, FL, TG, C, VEC>;
@@ -467,7 +466,7 @@ __global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
                     h[e] = step<decltype(exact)::value, MIX>(A(gs[c][e]), A(xs[c][e]), h[e]);
                     out.v[e] = T(h[e]);
                 }
-                if (c < steps) store_whole<T, VEC>(to, out, a.through);
+                if (c < steps) store_whole<T, VEC, THROUGH>(to, out);
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) fine = fine && finite(h[e]);
@@ -484,7 +483,7 @@ __global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
     }
 }
 
-template <typename T, bool MIX, int FL, int TG, int C, int VEC>
+template <typename T, bool MIX, int FL, int TG, int C, int VEC, bool THROUGH = false>
 __global__ __launch_bounds__(FL * TG) void k_rows_backward(Args<T> a) {
     using A = wide_t<T>;
     using W = Tile<T, FL, TG, C, VEC>;
@@ -597,8 +596,8 @@ __global__ __launch_bounds__(FL * TG) void k_rows_backward(Args<T> a) {
                     c_in[e] = back_of<EXACT>(gate, whole);
                 }
                 if (c < steps) {
-                    if (a.gx.p) store_whole<T, VEC>(to_x, ox, a.through);
-                    if (a.gg.p) store_whole<T, VEC>(to_g, og, a.through);
+                    if (a.gx.p) store_whole<T, VEC, THROUGH>(to_x, ox);
+                    if (a.gg.p) store_whole<T, VEC, THROUGH>(to_g, og);
                 }
             }
 #pragma unroll
@@ -690,8 +689,8 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
     }
 }
 
-// A few steps: a thread walks through them, VEC places side by side.
-template <typename T, bool MIX, bool BACK>
+// A few steps, at most N: a thread walks through them, VEC places side by side.
+template <typename T, bool MIX, bool BACK, int N>
 __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
     using A = wide_t<T>;
     constexpr int VEC = wide_vec<T>();
@@ -719,48 +718,44 @@ __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
         for (int e = 0; e < VEC; ++e)
             if (e < count) s.at(o, i + e) = h[e];
     };
-    auto from = [&](const Seq<const T>& s, int64_t t, T fill) {
-        return load_part<T, VEC>(s.p + o * s.so + t * s.st + i, s.p ? count : 0, fill);
+    auto from = [&](const Seq<const T>& s, Few<T, VEC> (&v)[N]) {
+        const T* p = s.p + o * s.so + i;
+#pragma unroll
+        for (int t = 0; t < N; ++t, p += s.st)
+            if (t < a.time) v[t] = load_part<T, VEC>(p, s.p ? count : 0, T(0));
     };
+    Few<T, VEC> xs[N], gs[N];
+    from(a.x, xs);
+    from(a.g, gs);
+    A h[VEC];
+    states(a.h0, h);
     if constexpr (!BACK) {
-        A h[VEC];
-        Few<T, VEC> xs = from(a.x, 0, T(0)), gs = from(a.g, 0, T(0));
-        states(a.h0, h);
-        for (int64_t t = 0; t < a.time; ++t) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+            if (t >= a.time) break;
             typename Few<T, VEC>::Elements out;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                h[e] = step<true, MIX>(A(gs[e]), A(xs[e]), h[e]);
+                h[e] = step<true, MIX>(A(gs[t][e]), A(xs[t][e]), h[e]);
                 out.v[e] = T(h[e]);
             }
             store_part<T, VEC>(a.y.p + o * a.y.so + t * a.y.st + i, out, count);
-            if (t + 1 < a.time) {
-                xs = from(a.x, t + 1, T(0));
-                gs = from(a.g, t + 1, T(0));
-            }
         }
         put(a.last, h);
     } else {
-        constexpr int MOST = 2;  // kFew
-        A before[MOST][VEC], c[VEC];
-        Few<T, VEC> xs[MOST], gs[MOST], ds[MOST];
-#pragma unroll
-        for (int t = 0; t < MOST; ++t)
-            if (t < a.time) {
-                xs[t] = from(a.x, t, T(0));
-                gs[t] = from(a.g, t, T(0));
-                ds[t] = from(a.gy, t, T(0));
-            }
-        states(a.h0, before[0]);
+        A before[N][VEC], c[VEC];
+        Few<T, VEC> ds[N];
+        from(a.gy, ds);
         states(a.last, c);
-        if (a.time > 1) {
+#pragma unroll
+        for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                before[1][e] = step<true, MIX>(A(gs[0][e]), A(xs[0][e]), before[0][e]);
+                before[t][e] = h[e];
+                if (t + 1 < a.time) h[e] = step<true, MIX>(A(gs[t][e]), A(xs[t][e]), h[e]);
             }
-        }
 #pragma unroll
-        for (int t = MOST - 1; t >= 0; --t) {
+        for (int t = N - 1; t >= 0; --t) {
             if (t >= a.time) continue;
             typename Few<T, VEC>::Elements ox, og;
 #pragma unroll
@@ -778,7 +773,7 @@ __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
         put(a.gh0, c);
     }
 }
-constexpr int64_t kFew = 2;
+constexpr int64_t kFew = 8;
 
 // ---------------------------------------------------------------- time contiguous
 //
@@ -1033,6 +1028,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
     if (w.live && w.segment == 0 && w.l == 0 && a.gh0.p) a.gh0.at(w.o, w.i) = c;
 }
 
+// The map of each segment, stretch by stretch.
 template <typename T, bool MIX, bool BACK>
 __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
     using A = wide_t<T>;
@@ -1043,48 +1039,48 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
     const Seq<const T>& src = BACK ? a.gy : a.x;
     const T* d = src.p + w.o * src.so + w.i * src.si;
     const bool some = !BACK || src.p;
-    const int64_t t0 = w.segment * a.per_segment * W::STRETCH;
-    const int64_t t1 = std::min(a.time, t0 + a.per_segment * W::STRETCH);
-    const int64_t each = (t1 - t0 + 63) / 64;  // a lane's steps, rounded up to whole accesses
-    const int64_t mine = (each + VEC - 1) / VEC * VEC;
-    const int64_t b0 = std::min(t1, t0 + w.l * mine), b1 = w.live ? std::min(t1, b0 + mine) : b0;
-    Map<A> m;
-    for (int64_t n = 0; n < b1 - b0; n += VEC) {
-        // (BACK: the last, shorter access first)
-        const int64_t t = BACK ? b0 + (b1 - b0 - 1 - n) / VEC * VEC : b0 + n;
-        const int count = int(std::min<int64_t>(VEC, b1 - t));
-        const Few<T, VEC> gs = load_part<T, VEC>(g + t, count, T(1));
-        const Few<T, VEC> ds = load_part<T, VEC>(d + t, some ? count : 0, T(0));
+    const int64_t s0 = w.segment * a.per_segment;
+    const int64_t s1 = std::min(s0 + a.per_segment, (a.time + W::STRETCH - 1) / W::STRETCH);
+    Few<T, VEC> gs, ds;
+    auto load = [&](int64_t k) {
+        const int64_t t = (BACK ? s1 - 1 - k : s0 + k) * W::STRETCH + w.l * VEC;
+        const int count = w.count(t, a.time);
+        gs = load_part<T, VEC>(g + t, count, T(1));
+        ds = load_part<T, VEC>(d + t, some ? count : 0, T(0));
+    };
+    load(0);
+    A f = A(1), b = A(0);
+    for (int64_t k = 0; k < s1 - s0; ++k) {
+        const Few<T, VEC> gn = gs, dn = ds;
+        if (k + 1 < s1 - s0) load(k + 1);
+        Map<A> m;
         if constexpr (BACK) {
 #pragma unroll
             for (int e = VEC - 1; e >= 0; --e) {
-                const A gate = A(gs[e]);
-                m.b = back_of<true>(gate, A(ds[e]) + m.b);
-                m.factor_by(gate);
+                m.b = back_of<true>(A(gn[e]), A(dn[e]) + m.b);
+                m.factor_by(A(gn[e]));
             }
         } else {
+            line_map<MIX>(gn, dn, m);
+        }
+        A fac = m.factor(), sum = m.b;
+        scan_step<64, BACK, 1>(fac, sum, w.l);
+        scan_step<64, BACK, 2>(fac, sum, w.l);
+        scan_step<64, BACK, 4>(fac, sum, w.l);
+        scan_step<64, BACK, 8>(fac, sum, w.l);
+        constexpr int ends[4] = {BACK ? 48 : 15, BACK ? 32 : 31, BACK ? 16 : 47, BACK ? 0 : 63};
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) m.template then<true, MIX>(A(gs[e]), A(ds[e]));
+        for (int r = 0; r < 4; ++r) {
+            const A fr = read_lane(fac, ends[r]);
+            b = apply(fr, b, read_lane(sum, ends[r]));
+            f = kept_product(f, fr);
         }
     }
-    // the lanes' maps in a row: what the last lane (BACK: the first) makes of the state 0, and of a
-    // factor
-    A a1 = m.factor(), b1v = m.b;
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-        const A pa = BACK ? __shfl_down(a1, k, 64) : __shfl_up(a1, k, 64);
-        const A pb = BACK ? __shfl_down(b1v, k, 64) : __shfl_up(b1v, k, 64);
-        const bool none = BACK ? w.l + k >= 64 : w.l < k;
-        if (!none) {
-            b1v = apply(a1, pb, b1v);
-            a1 = kept_product(pa, a1);
-        }
-    }
-    if (w.live && w.l == (BACK ? 0 : 63)) {
+    if (w.live && w.l == 0) {
         const int64_t n = a.outer * a.inner;
         A* to = a.maps + 2 * w.segment * n + w.row;
-        to[0] = a1;
-        to[n] = b1v;
+        to[0] = f;
+        to[n] = b;
     }
 }
 
@@ -1132,10 +1128,10 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
         r.tiles = ceil_div(inner, vec);
         r.units = ceil_div(outer * r.tiles, kThreads);
     } else {
-        // 64 lanes side by side and 4 groups of 8 steps, or 16 and 32 (backward: of 4)
+        // 32 lanes side by side and 8 groups of 4 steps, or 16 and 32 (a forward of many steps: of 8)
         r.way = inner < places ? kRowsNarrow : time <= 32 ? kRowsShort : kRowsLong;
         r.stretch = r.way == kRowsShort ? 32 : r.way == kRowsLong ? 128 : 256;
-        r.tiles = r.way == kRowsNarrow ? 1 : ceil_div(inner, (r.way == kRowsShort ? 64 : 16) * places);
+        r.tiles = r.way == kRowsNarrow ? 1 : ceil_div(inner, (r.way == kRowsShort ? 32 : 16) * places);
         r.units = outer * r.tiles;
     }
     r.stretches = ceil_div(time, r.stretch);
@@ -1151,7 +1147,6 @@ int route_args(Args<T>& a, const Route& r, bool lines, void* workspace) {
     if (r.stretches <= 1) a.starts = nullptr;
     a.groups = r.units * r.segments;
     CL_ARG(a.groups < (int64_t(1) << 31), "too many sequences for one call");
-    a.through = double(a.outer) * a.time * a.inner * sizeof(T) >= double(96 << 20);
     const int64_t most = INT32_MAX;
     a.tiles = make_fastdiv(uint32_t(std::min(lines ? r.units : r.tiles, most)));
     a.outers = make_fastdiv(uint32_t(std::min(lines ? a.inner : a.outer, most)));
@@ -1162,6 +1157,9 @@ template <typename T, bool MIX, bool BACK>
 int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
     constexpr int P = sizeof(T) == 8 ? 2 : 4;
     const dim3 grid = wide_grid(a.groups);
+    // Long sequences: outputs past the 256 MiB cache from 96 MiB each on, where what comes next would
+    // not find them in it (134 MB each: forward 94 -> 86 us, backward 135 -> 128; 66 MB: 62 -> 66).
+    const bool through = double(a.outer) * a.time * a.inner * sizeof(T) >= double(96 << 20);
     if (r.segments > 1) {
         if (r.way == kLines64)
             k_lines_maps<T, MIX, BACK><<<grid, kThreads, 0, s>>>(a);
@@ -1173,19 +1171,30 @@ int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
     }
     switch (r.way) {
         case kRowsFew:
-            k_rows_few<T, MIX, BACK><<<grid, kThreads, 0, s>>>(a);
+            if (a.time <= 2)
+                k_rows_few<T, MIX, BACK, 2><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_rows_few<T, MIX, BACK, int(kFew)><<<grid, kThreads, 0, s>>>(a);
             break;
         case kRowsShort:
             if constexpr (BACK)
-                k_rows_backward<T, MIX, 64, 4, 8, P><<<grid, kThreads, 0, s>>>(a);
+                k_rows_backward<T, MIX, 32, 8, 4, P><<<grid, kThreads, 0, s>>>(a);
             else
-                k_rows_forward<T, MIX, 64, 4, 8, P, 1><<<grid, kThreads, 0, s>>>(a);
+                k_rows_forward<T, MIX, 32, 8, 4, P, 1><<<grid, kThreads, 0, s>>>(a);
             break;
         case kRowsLong:
-            if constexpr (BACK)
-                k_rows_backward<T, MIX, 16, 32, 4, P><<<grid, 512, 0, s>>>(a);
-            else
+            if constexpr (BACK) {
+                if (through)
+                    k_rows_backward<T, MIX, 16, 32, 4, P, true><<<grid, 512, 0, s>>>(a);
+                else
+                    k_rows_backward<T, MIX, 16, 32, 4, P><<<grid, 512, 0, s>>>(a);
+            } else if (r.stretches == 1) {
+                k_rows_forward<T, MIX, 16, 32, 4, P, 1><<<grid, 512, 0, s>>>(a);
+            } else if (through) {
+                k_rows_forward<T, MIX, 16, 32, 8, P, 2, true><<<grid, 512, 0, s>>>(a);
+            } else {
                 k_rows_forward<T, MIX, 16, 32, 8, P, 2><<<grid, 512, 0, s>>>(a);
+            }
             break;
         case kRowsNarrow:
             if constexpr (BACK)
