@@ -10,24 +10,28 @@
 // fp64 of exponentials in fp64, of one row of each: next to some 10^5 borders between tokens, fp32 sums
 // would draw a neighbour once in 10^3 draws, as their order goes.
 //
-//   k_small    one workgroup a sequence does it all, where a row is one chunk
-// else, each row cut into chunks of kChunk elements,
-//   k_stats    (m, s) of every chunk of the rows
-//   k_sums     joins them, takes the tests (every workgroup of a sequence the same ones), and the
-//              fp64 sums of its chunk of the two rows
+//   k_small    one workgroup a sequence does it all, for rows of at most kSmall elements
+// else
+//   k_stats    (m, s) of every part of the rows, kPart elements each
+//   k_decide   joins them and takes the tests
+//   k_sums     the fp64 sums of a chunk, kChunk elements, of the two rows
 //   k_weights  the sum of max(p - q, 0) of its chunk
 //   k_pick     the chunk that the number falls into, and the place in it
+// Chunks are short because k_pick takes one by one workgroup, bound by its exponentials (8192 elements
+// of two rows took 11 us).
 #include "row_loss.h"
 #include "storage.h"
 
 namespace cl {
 namespace {
 
-constexpr int kChunk = 8192;
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / 64;
-constexpr int kRun = kChunk / kThreads;  // elements of a thread, one behind the other
+constexpr int kRun = 8;                  // elements of a thread, one behind the other
+constexpr int kThreads = 512;            // k_small, k_decide
+constexpr int kSmall = kThreads * kRun;
+constexpr int kDrawThreads = 256;        // of a chunk
+constexpr int kChunk = kDrawThreads * kRun;
 constexpr int kStatThreads = 256;
+constexpr int kPart = 8192;
 
 template <typename A>
 struct Stat {
@@ -55,8 +59,8 @@ struct Args {
     int64_t* accepted;
     A* lp;
     // workspace, where a row has several chunks
-    int chunks;
-    Stat<A>* stats;                  // [seq][2 drafts + 1][chunk], the target's rows first
+    int parts, chunks;
+    Stat<A>* stats;                  // [seq][2 drafts + 1][part], the target's rows first
     Draw* draws;
     double* sums;                    // [seq][chunk][p, q]
     double* weights;                 // [seq][chunk]
@@ -70,7 +74,7 @@ struct Args {
         return draft ? q + seq * q_seq + i * q_row : p + seq * p_seq + i * p_row;
     }
     __device__ __forceinline__ Stat<A>* stat(int64_t seq, int64_t i, bool draft) const {
-        return stats + (seq * (2 * drafts + 1) + i + (draft ? drafts + 1 : 0)) * chunks;
+        return stats + (seq * (2 * drafts + 1) + i + (draft ? drafts + 1 : 0)) * parts;
     }
     __device__ __forceinline__ bool holds(int64_t token) const { return token >= 0 && token < cols; }
 };
@@ -124,14 +128,14 @@ __device__ __forceinline__ void add(Stat<A>& st, const Stat<A>& more) {
 template <typename T>
 __global__ __launch_bounds__(kStatThreads) void k_stats(Args<T> a) {
     using A = wide_t<T>;
-    constexpr int VEC = wide_vec<T>(), NV = kChunk / kStatThreads / VEC;
+    constexpr int VEC = wide_vec<T>(), NV = kPart / kStatThreads / VEC;
     __shared__ Stat<A> part[kStatThreads / 64];
     const int64_t rows = 2 * a.drafts + 1;
-    int64_t group = group_index();
-    if (group >= a.seqs * rows * a.chunks) return;
-    const int chunk = int(group % a.chunks);
-    group /= a.chunks;
-    const int64_t seq = group / rows, r = group - seq * rows;
+    const int64_t group = group_index();  // below 2^31
+    if (group >= a.seqs * rows * a.parts) return;
+    const uint32_t row = uint32_t(group) / uint32_t(a.parts);
+    const int at_part = int(uint32_t(group) - row * uint32_t(a.parts));
+    const int64_t seq = row / uint32_t(rows), r = row - seq * rows;
     const bool draft = r > a.drafts;
     const int64_t i = draft ? r - a.drafts - 1 : r;
     if (draft && !a.q) return;
@@ -139,14 +143,19 @@ __global__ __launch_bounds__(kStatThreads) void k_stats(Args<T> a) {
     bool ended = false;
     for (int64_t j = 0; j < (draft ? i + 1 : i); ++j) ended |= a.tokens[seq * a.drafts + j] == a.ignore;
     if (ended) return;
-    const int64_t j0 = int64_t(chunk) * kChunk;
+    const int64_t j0 = int64_t(at_part) * kPart;
     const T* x = a.row(seq, i, draft) + j0;
     const int64_t n = a.cols - j0;
     Pack<T, VEC> v[NV];
+    if (n >= kPart) {  // (no branch between the loads: each would be waited for)
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int64_t at = (k * kStatThreads + threadIdx.x) * VEC;
-        v[k] = load_part<T, VEC>(x + at, n - at);
+        for (int k = 0; k < NV; ++k) v[k] = pload<T, VEC>(x + (k * kStatThreads + threadIdx.x) * VEC);
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int64_t at = (k * kStatThreads + threadIdx.x) * VEC;
+            v[k] = load_part<T, VEC>(x + at, n - at);
+        }
     }
     Stat<A> st{-A(__builtin_inf()), A(0)};
 #pragma unroll
@@ -163,7 +172,7 @@ __global__ __launch_bounds__(kStatThreads) void k_stats(Args<T> a) {
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kStatThreads / 64; ++w) add(st, part[w]);
-        a.stat(seq, i, draft)[chunk] = st;
+        a.stat(seq, i, draft)[at_part] = st;
     }
 }
 
@@ -177,8 +186,7 @@ struct Round {
 };
 
 template <int LANES, typename T, typename F>
-__device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANES>& sh, bool write,
-                                       F&& rows) {
+__device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANES>& sh, F&& rows) {
     using A = wide_t<T>;
     constexpr int N = Round<LANES>::N;
     const int g = threadIdx.x / LANES;
@@ -187,6 +195,11 @@ __device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANE
         const int64_t i = i0 + g / 2;
         const int64_t token = i < a.drafts ? a.tokens[seq * a.drafts + i] : a.ignore;
         const bool given = i < a.drafts && token != a.ignore;
+        // by the first wave, in time for the tests
+        const int64_t mine_at = i0 + threadIdx.x;
+        const bool tests = threadIdx.x < N && mine_at < a.drafts;
+        const int64_t mine = tests ? a.tokens[seq * a.drafts + mine_at] : a.ignore;
+        const double u = tests ? a.uniform(seq, mine_at) : 0.0;
         if (draft ? given && a.q : i <= a.drafts) {
             const Stat<A> st = rows(seq, i, draft);
             double pr = 0.0, lp = -__builtin_inf();
@@ -207,17 +220,13 @@ __device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANE
             const int64_t at = i0 + l;
             bool stop = false;
             if (l < N && at <= a.drafts) {
-                const int64_t mine = at < a.drafts ? a.tokens[seq * a.drafts + at] : a.ignore;
                 stop = true;
-                if (at < a.drafts && mine != a.ignore) {
-                    const double q = !a.q ? 1.0 : sh.prob[l][1];
-                    stop = !(a.uniform(seq, at) * q < sh.prob[l][0]);
-                }
+                if (mine != a.ignore) stop = !(u * (a.q ? sh.prob[l][1] : 1.0) < sh.prob[l][0]);
             }
             const uint64_t stops = __ballot(stop);
             const int first = stops ? __builtin_ctzll(stops) : N;
-            if (write && l < first && l < N) {
-                a.out[seq * (a.drafts + 1) + at] = a.tokens[seq * a.drafts + at];
+            if (l < first) {
+                a.out[seq * (a.drafts + 1) + at] = mine;
                 a.lp[seq * (a.drafts + 1) + at] = A(sh.lp[l]);
             }
             if (l == 0) sh.first = first;
@@ -227,13 +236,11 @@ __device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANE
         if (first < N) {
             const int64_t n = i0 + first;
             const bool refused = n < a.drafts && a.tokens[seq * a.drafts + n] != a.ignore;
-            if (write) {
-                for (int64_t k = n + 1 + threadIdx.x; k <= a.drafts; k += kThreads) {
-                    a.out[seq * (a.drafts + 1) + k] = a.ignore;
-                    a.lp[seq * (a.drafts + 1) + k] = A(0);
-                }
-                if (threadIdx.x == 0) a.accepted[seq] = n;
+            for (int64_t k = n + 1 + threadIdx.x; k <= a.drafts; k += kThreads) {
+                a.out[seq * (a.drafts + 1) + k] = a.ignore;
+                a.lp[seq * (a.drafts + 1) + k] = A(0);
             }
+            if (threadIdx.x == 0) a.accepted[seq] = n;
             return {sh.m[first][0], refused && a.q ? sh.m[first][1] : 0.0, n, refused};
         }
         __syncthreads();
@@ -241,18 +248,8 @@ __device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANE
 }
 
 // ---- fp64 sums over a workgroup
-__device__ __forceinline__ double group_total(double v, double* red) {
-    v = wave_total(v);
-    if (lane_id() == 0) red[wave_id()] = v;
-    __syncthreads();
-    double s = red[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) s += red[w];
-    __syncthreads();
-    return s;
-}
-
 // Sum up to and with each thread's v; `total`: of all.
+template <int WAVES>
 __device__ __forceinline__ double group_scan(double v, double* red, double& total) {
     const int l = lane_id();
 #pragma unroll
@@ -265,7 +262,7 @@ __device__ __forceinline__ double group_scan(double v, double* red, double& tota
     double before = 0.0;
     total = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
         if (w == wave_id()) before = total;
         total += red[w];
     }
@@ -273,33 +270,61 @@ __device__ __forceinline__ double group_scan(double v, double* red, double& tota
     return before + v;
 }
 
-// ---- the draw.  A thread's elements of a chunk: `run` of them from `at` on.
-template <typename T>
+// exp of x <= 0 within some 2^-52, without the cases of the library's (30 instructions to 20):
+// 2^n exp(r), n the integer next to x log2 e, exp(r) by its series to r^13 / 13! (|r| < 0.35: what is
+// left out is below 2^-60).
+__device__ __forceinline__ double exp_below(double x) {
+    x = x < -800.0 ? -800.0 : x;  // (0; NaN stays)
+    const double n = __builtin_rint(x * 1.4426950408889634);
+    const double r = fma(n, -1.9082149292705877e-10, fma(n, -0.6931471803691238, x));
+    double s = 1.0 / 6227020800.0;
+    s = fma(s, r, 1.0 / 479001600.0);
+    s = fma(s, r, 1.0 / 39916800.0);
+    s = fma(s, r, 1.0 / 3628800.0);
+    s = fma(s, r, 1.0 / 362880.0);
+    s = fma(s, r, 1.0 / 40320.0);
+    s = fma(s, r, 1.0 / 5040.0);
+    s = fma(s, r, 1.0 / 720.0);
+    s = fma(s, r, 1.0 / 120.0);
+    s = fma(s, r, 1.0 / 24.0);
+    s = fma(s, r, 1.0 / 6.0);
+    s = fma(s, r, 0.5);
+    s = fma(s, r, 1.0);
+    s = fma(s, r, 1.0);
+    return __builtin_ldexp(s, int(n));
+}
+
+// ---- the draw.  A thread's elements of a chunk of NT threads: `run` of them from `at` on.
+template <typename T, int NT>
 struct Place {
     int64_t at;
     int count;
     __device__ __forceinline__ Place(int64_t j0, int64_t cols) {
         constexpr int VEC = wide_vec<T>();
-        const int64_t n = cols - j0 < kChunk ? cols - j0 : kChunk;
-        const int run = int((n + kThreads * VEC - 1) / (kThreads * VEC)) * VEC;
+        const int64_t n = cols - j0 < NT * kRun ? cols - j0 : NT * kRun;
+        const int run = int((n + NT * VEC - 1) / (NT * VEC)) * VEC;
         at = j0 + int64_t(threadIdx.x) * run;
         const int64_t left = j0 + n - at;
         count = left >= run ? run : left > 0 ? int(left) : 0;
     }
 };
 
-// exp(x - m) of the thread's elements in fp64, 0 behind them.
-template <typename T>
-__device__ __forceinline__ void exponentials(const T* row, const Place<T>& w, double m,
-                                             double (&e)[kRun]) {
+// exp(x - m) of the thread's elements in fp64, 0 behind them; returns their sum.
+template <typename T, int NT>
+__device__ __forceinline__ double exponentials(const T* row, const Place<T, NT>& w, double m,
+                                               double (&e)[kRun]) {
     constexpr int VEC = wide_vec<T>();
     Pack<T, VEC> v[kRun / VEC];
 #pragma unroll
     for (int k = 0; k < kRun / VEC; ++k)
         v[k] = load_part<T, VEC>(row + w.at + k * VEC, w.count - k * VEC);
+    double sum = 0.0;
 #pragma unroll
-    for (int k = 0; k < kRun; ++k)
-        e[k] = k < w.count ? exp(double(v[k / VEC].v[k % VEC]) - m) : 0.0;
+    for (int k = 0; k < kRun; ++k) {
+        e[k] = k < w.count ? exp_below(double(v[k / VEC].v[k % VEC]) - m) : 0.0;
+        sum += e[k];
+    }
+    return sum;
 }
 
 template <typename T>
@@ -315,35 +340,36 @@ struct Rows {
     }
 };
 
-// Weights of the thread's elements where a draft was refused: max(p - q, 0).
-template <typename T>
-__device__ __forceinline__ void over(const Rows<T>& r, const Place<T>& w, const Draw& d, double sp,
-                                     double sq, double (&e)[kRun]) {
-    exponentials(r.p, w, d.mp, e);
-    if (r.q) {
-        double f[kRun];
-        exponentials(r.q, w, d.mq, f);
+// Weights where a draft was refused, max(p - q, 0), of the thread's exponentials e and f of the two rows;
+// returns their sum.
+template <typename T, int NT>
+__device__ __forceinline__ double over(const Rows<T>& r, const Place<T, NT>& w, const double (&e)[kRun],
+                                       const double (&f)[kRun], double inv_sp, double inv_sq,
+                                       double (&v)[kRun]) {
+    // equal rows leave nothing: both products are rounded (and both sums taken alike)
+#pragma clang fp contract(off)
+    double sum = 0.0;
 #pragma unroll
-        for (int k = 0; k < kRun; ++k) {
-            const double v = e[k] / sp - f[k] / sq;
-            e[k] = v > 0.0 || v != v ? v : 0.0;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) e[k] = w.at + k == r.token ? 0.0 : e[k] / sp;
+    for (int k = 0; k < kRun; ++k) {
+        double d = e[k] * inv_sp;
+        if (r.q)
+            d -= f[k] * inv_sq;
+        else if (w.at + k == r.token)
+            d = 0.0;
+        v[k] = d > 0.0 || d != d ? d : 0.0;
+        sum += v[k];
     }
+    return sum;
 }
 
 // The place of the first weight up to and with which the sum is above `goal`, `before` counted in; the
 // last weight above 0 if rounding leaves none.  sh: first and last thread; the owner writes `*place`.
-template <typename T>
-__device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T>& w, double upto,
-                                         double before, double goal, int* sh, int64_t* place) {
-    double mine = 0.0;
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) mine += e[k];
+template <typename T, int NT>
+__device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T, NT>& w, double mine,
+                                         double upto, double before, double goal, int* sh,
+                                         int64_t* place) {
     if (threadIdx.x == 0) {
-        sh[0] = kThreads;
+        sh[0] = NT;
         sh[1] = -1;
         *place = -1;
     }
@@ -353,7 +379,7 @@ __device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T>
         atomicMax(&sh[1], int(threadIdx.x));
     }
     __syncthreads();
-    const int owner = sh[0] < kThreads ? sh[0] : sh[1];
+    const int owner = sh[0] < NT ? sh[0] : sh[1];
     if (int(threadIdx.x) == owner) {
         double c = before + (upto - mine);
         int at = -1;
@@ -363,7 +389,7 @@ __device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T>
             c += e[k];
             if (e[k] > 0.0 && !found) {
                 at = k;
-                found = sh[0] < kThreads && c > goal;
+                found = sh[0] < NT && c > goal;
             }
         }
         *place = w.at + at;
@@ -380,20 +406,21 @@ __device__ __forceinline__ void put(const Args<T>& a, int64_t seq, const Draw& d
     a.lp[to] = place >= 0 ? A((double(p[place]) - d.mp) - log(sp)) : A(__builtin_nan(""));
 }
 
-template <typename T>
+template <typename T, int LANES>
 __global__ __launch_bounds__(kThreads) void k_small(Args<T> a) {
     using A = wide_t<T>;
-    constexpr int VEC = wide_vec<T>();
-    __shared__ Round<64> round;
-    __shared__ double red[kWaves];
+    constexpr int VEC = wide_vec<T>(), WAVES = kThreads / 64;
+    __shared__ Round<LANES> round;
+    __shared__ double red[WAVES];
     __shared__ int ends[2];
     __shared__ int64_t place;
     const int64_t seq = group_index();
     if (seq >= a.seqs) return;
-    const Draw d = decide<64>(a, seq, round, true, [&](int64_t s, int64_t i, bool draft) {
+    const double u = a.uniform(seq, a.drafts);
+    const Draw d = decide<LANES>(a, seq, round, [&](int64_t s, int64_t i, bool draft) {
         const T* x = a.row(s, i, draft);
         Stat<A> st{-A(__builtin_inf()), A(0)};
-        for (int64_t j = lane_id() * VEC; j < a.cols; j += 64 * VEC) {
+        for (int64_t j = (threadIdx.x % LANES) * VEC; j < a.cols; j += LANES * VEC) {
             const Pack<T, VEC> v = load_part<T, VEC>(x + j, a.cols - j);
             A m = st.m;
 #pragma unroll
@@ -404,73 +431,66 @@ __global__ __launch_bounds__(kThreads) void k_small(Args<T> a) {
             for (int e = 0; e < VEC; ++e) st.s += exp_diff(A(v.v[e]) - base);
             st.m = m;
         }
-        return join<64>(st);
+        return join<LANES>(st);
     });
     const Rows<T> r(a, seq, d);
-    const Place<T> w(0, a.cols);
-    const double u = a.uniform(seq, a.drafts);
-    double e[kRun], mine = 0.0, total;
-    exponentials(r.p, w, d.mp, e);
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) mine += e[k];
-    const double upto_p = group_scan(mine, red, total);
+    const Place<T, kThreads> w(0, a.cols);
+    double e[kRun], f[kRun] = {}, total;
+    double mine = exponentials(r.p, w, d.mp, e);
+    const double mine_q = r.q ? exponentials(r.q, w, d.mq, f) : 0.0;
+    double upto = group_scan<WAVES>(mine, red, total);
     const double sp = total;
-    double upto = upto_p;
     if (d.refused) {
         double sq = 1.0;
-        if (r.q) {
-            double f[kRun];
-            exponentials(r.q, w, d.mq, f);
-            mine = 0.0;
+        if (r.q) group_scan<WAVES>(mine_q, red, sq);
+        double v[kRun], total_v;
+        const double mine_v = over(r, w, e, f, 1.0 / sp, 1.0 / sq, v);
+        const double upto_v = group_scan<WAVES>(mine_v, red, total_v);
+        if (total_v > 0.0) {  // else nothing is above the draft: the target's own
+            mine = mine_v;
+            upto = upto_v;
+            total = total_v;
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) mine += f[k];
-            sq = group_total(mine, red);
-        }
-        over(r, w, d, sp, sq, e);
-        mine = 0.0;
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) mine += e[k];
-        upto = group_scan(mine, red, total);
-        if (!(total > 0.0)) {  // nothing above the draft: the target's own
-            exponentials(r.p, w, d.mp, e);
-            total = sp;
-            upto = upto_p;
+            for (int k = 0; k < kRun; ++k) e[k] = v[k];
         }
     }
-    place_of(e, w, upto, 0.0, u * total, ends, &place);
+    place_of(e, w, mine, upto, 0.0, u * total, ends, &place);
     if (threadIdx.x == 0) put(a, seq, d, r.p, sp, sp > 0.0 ? place : -1);
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_sums(Args<T> a) {
+__global__ __launch_bounds__(kThreads) void k_decide(Args<T> a) {
     using A = wide_t<T>;
     __shared__ Round<16> round;
-    __shared__ double red[kWaves];
-    const int64_t group = group_index();
-    if (group >= a.seqs * a.chunks) return;
-    const int64_t seq = group / a.chunks;
-    const int chunk = int(group - seq * a.chunks);
-    const Draw d = decide<16>(a, seq, round, chunk == 0, [&](int64_t s, int64_t i, bool draft) {
+    const int64_t seq = group_index();
+    if (seq >= a.seqs) return;
+    const Draw d = decide<16>(a, seq, round, [&](int64_t s, int64_t i, bool draft) {
         const Stat<A>* part = a.stat(s, i, draft);
         Stat<A> st{-A(__builtin_inf()), A(0)};
-        for (int c = threadIdx.x & 15; c < a.chunks; c += 16) add(st, part[c]);
+        for (int c = threadIdx.x & 15; c < a.parts; c += 16) add(st, part[c]);
         return join<16>(st);
     });
-    if (chunk == 0 && threadIdx.x == 0) a.draws[seq] = d;
+    if (threadIdx.x == 0) a.draws[seq] = d;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kDrawThreads) void k_sums(Args<T> a) {
+    constexpr int WAVES = kDrawThreads / 64;
+    __shared__ double red[WAVES];
+    const int64_t group = group_index();  // below 2^31
+    if (group >= a.seqs * a.chunks) return;
+    const int64_t seq = uint32_t(group) / uint32_t(a.chunks);
+    const int64_t chunk = group - seq * a.chunks;
+    const Draw d = a.draws[seq];
     const Rows<T> r(a, seq, d);
-    const Place<T> w(int64_t(chunk) * kChunk, a.cols);
-    double e[kRun], mine = 0.0, total;
-    exponentials(r.p, w, d.mp, e);
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) mine += e[k];
-    group_scan(mine, red, total);   // as k_pick will have it
+    const Place<T, kDrawThreads> w(chunk * kChunk, a.cols);
+    double e[kRun], f[kRun], total;
+    const double mine = exponentials(r.p, w, d.mp, e);
+    const double mine_q = r.q ? exponentials(r.q, w, d.mq, f) : 0.0;
+    group_scan<WAVES>(mine, red, total);  // as k_pick will have it
     if (threadIdx.x == 0) a.sums[2 * group] = total;
     if (r.q) {
-        exponentials(r.q, w, d.mq, e);
-        mine = 0.0;
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) mine += e[k];
-        total = group_total(mine, red);
+        group_scan<WAVES>(mine_q, red, total);
         if (threadIdx.x == 0) a.sums[2 * group + 1] = total;
     }
 }
@@ -483,30 +503,31 @@ __device__ __forceinline__ double chunks_total(const double* sums, int stride, i
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_weights(Args<T> a) {
-    __shared__ double red[kWaves];
+__global__ __launch_bounds__(kDrawThreads) void k_weights(Args<T> a) {
+    constexpr int WAVES = kDrawThreads / 64;
+    __shared__ double red[WAVES];
     const int64_t group = group_index();
     if (group >= a.seqs * a.chunks) return;
-    const int64_t seq = group / a.chunks;
+    const int64_t seq = uint32_t(group) / uint32_t(a.chunks);
     const Draw d = a.draws[seq];
     if (!d.refused) return;
-    const int chunk = int(group - seq * a.chunks);
+    const int64_t chunk = group - seq * a.chunks;
     const Rows<T> r(a, seq, d);
-    const Place<T> w(int64_t(chunk) * kChunk, a.cols);
+    const Place<T, kDrawThreads> w(chunk * kChunk, a.cols);
+    double e[kRun], f[kRun] = {}, v[kRun], total;
+    exponentials(r.p, w, d.mp, e);
+    if (r.q) exponentials(r.q, w, d.mq, f);
     const double* sums = a.sums + 2 * seq * a.chunks;
     const double sp = chunks_total(sums, 2, a.chunks);
     const double sq = r.q ? chunks_total(sums + 1, 2, a.chunks) : 1.0;
-    double e[kRun], mine = 0.0, total;
-    over(r, w, d, sp, sq, e);
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) mine += e[k];
-    group_scan(mine, red, total);
+    group_scan<WAVES>(over(r, w, e, f, 1.0 / sp, 1.0 / sq, v), red, total);
     if (threadIdx.x == 0) a.weights[group] = total;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_pick(Args<T> a) {
-    __shared__ double red[kWaves];
+__global__ __launch_bounds__(kDrawThreads) void k_pick(Args<T> a) {
+    constexpr int WAVES = kDrawThreads / 64;
+    __shared__ double red[WAVES];
     __shared__ int ends[2];
     __shared__ int64_t place;
     const int64_t seq = group_index();
@@ -561,23 +582,26 @@ __global__ __launch_bounds__(kThreads) void k_pick(Args<T> a) {
         if (threadIdx.x == 0) put(a, seq, d, r.p, sp, -1);
         return;
     }
-    const Place<T> w(int64_t(chosen) * kChunk, a.cols);
-    double e[kRun], mine = 0.0;
-    if (own)
-        exponentials(r.p, w, d.mp, e);
-    else
-        over(r, w, d, sp, sq, e);
+    const Place<T, kDrawThreads> w(int64_t(chosen) * kChunk, a.cols);
+    double e[kRun];
+    double mine = exponentials(r.p, w, d.mp, e);
+    if (!own) {
+        double f[kRun] = {}, v[kRun];
+        if (r.q) exponentials(r.q, w, d.mq, f);
+        mine = over(r, w, e, f, 1.0 / sp, 1.0 / sq, v);
 #pragma unroll
-    for (int k = 0; k < kRun; ++k) mine += e[k];
+        for (int k = 0; k < kRun; ++k) e[k] = v[k];
+    }
     double sum;
-    const double upto = group_scan(mine, red, sum);
-    place_of(e, w, upto, before, goal, ends, &place);
+    const double upto = group_scan<WAVES>(mine, red, sum);
+    place_of(e, w, mine, upto, before, goal, ends, &place);
     if (threadIdx.x == 0) put(a, seq, d, r.p, sp, sp > 0.0 ? place : -1);
 }
 
-// Chunks of a row, and the parts of the workspace behind each other on 16 bytes.
+// Parts and chunks of a row, and the arrays of the workspace behind each other on 16 bytes.
 struct Layout {
-    int64_t chunks, stats, draws, sums, weights, total;
+    bool small;
+    int64_t parts, chunks, draws, sums, weights, total;
 };
 
 int layout_of(int dtype, int64_t seqs, int64_t drafts, int64_t cols, Layout& l) {
@@ -585,18 +609,17 @@ int layout_of(int dtype, int64_t seqs, int64_t drafts, int64_t cols, Layout& l) 
            "unsupported dtype code %d (expected F32, F64, F16 or BF16)", dtype);
     CL_ARG(seqs >= 0 && drafts >= 0 && cols >= 1, "bad shape: %lld sequences, %lld drafts, %lld classes",
            (long long)seqs, (long long)drafts, (long long)cols);
+    l.small = cols <= kSmall;
+    l.parts = ceil_div(cols, kPart);
     l.chunks = ceil_div(cols, kChunk);
-    CL_ARG(l.chunks < (int64_t(1) << 24) && drafts < (int64_t(1) << 24) &&
-               seqs < (int64_t(1) << 31) &&
-               double(seqs) * (2.0 * drafts + 1) * l.chunks < double(int64_t(1) << 31),
+    const double most = double(int64_t(1) << 31);
+    CL_ARG(double(seqs) * (2.0 * double(drafts) + 1) * double(l.parts) < most &&
+               double(seqs) * double(l.chunks) < most && double(drafts) < most && double(l.chunks) < most,
            "too many logits for one call");
-    l.stats = 0;
-    if (l.chunks == 1) {
-        l.draws = l.sums = l.weights = l.total = 0;
-        return CL_OK;
-    }
+    l.draws = l.sums = l.weights = l.total = 0;
+    if (l.small) return CL_OK;
     const int64_t wide = dtype == CL_DTYPE_F64 ? 8 : 4;
-    l.draws = ceil_div(2 * wide * seqs * (2 * drafts + 1) * l.chunks, 16) * 16;
+    l.draws = ceil_div(2 * wide * seqs * (2 * drafts + 1) * l.parts, 16) * 16;
     l.sums = l.draws + int64_t(sizeof(Draw)) * seqs;
     l.weights = l.sums + 16 * seqs * l.chunks;
     l.total = l.weights + 8 * seqs * l.chunks;
@@ -657,24 +680,32 @@ extern "C" int cl_verify_drafts(int dtype, const void* logits, int64_t seq_strid
         a.out = tokens;
         a.accepted = accepted;
         a.lp = static_cast<wide_t<T>*>(log_probs);
+        a.parts = int(l.parts);
         a.chunks = int(l.chunks);
-        if (l.chunks == 1) {
-            k_small<T><<<wide_grid(sequences), kThreads, 0, s>>>(a);
+        const dim3 each = wide_grid(sequences);
+        if (l.small) {
+            // rows of up to 32 elements a lane: more positions at once
+            if (cols <= 512)
+                k_small<T, 16><<<each, kThreads, 0, s>>>(a);
+            else
+                k_small<T, 64><<<each, kThreads, 0, s>>>(a);
             return check_launch("cl_verify_drafts");
         }
         char* ws = static_cast<char*>(workspace);
-        a.stats = reinterpret_cast<Stat<wide_t<T>>*>(ws + l.stats);
+        a.stats = reinterpret_cast<Stat<wide_t<T>>*>(ws);
         a.draws = reinterpret_cast<Draw*>(ws + l.draws);
         a.sums = reinterpret_cast<double*>(ws + l.sums);
         a.weights = reinterpret_cast<double*>(ws + l.weights);
         const dim3 grid = wide_grid(sequences * l.chunks);
-        k_stats<T><<<wide_grid(sequences * (2 * drafts + 1) * l.chunks), kStatThreads, 0, s>>>(a);
+        k_stats<T><<<wide_grid(sequences * (2 * drafts + 1) * l.parts), kStatThreads, 0, s>>>(a);
         if (int rc = check_launch("cl_verify_drafts(stats)")) return rc;
-        k_sums<T><<<grid, kThreads, 0, s>>>(a);
+        k_decide<T><<<each, kThreads, 0, s>>>(a);
+        if (int rc = check_launch("cl_verify_drafts(decide)")) return rc;
+        k_sums<T><<<grid, kDrawThreads, 0, s>>>(a);
         if (int rc = check_launch("cl_verify_drafts(sums)")) return rc;
-        k_weights<T><<<grid, kThreads, 0, s>>>(a);
+        k_weights<T><<<grid, kDrawThreads, 0, s>>>(a);
         if (int rc = check_launch("cl_verify_drafts(weights)")) return rc;
-        k_pick<T><<<wide_grid(sequences), kThreads, 0, s>>>(a);
+        k_pick<T><<<each, kDrawThreads, 0, s>>>(a);
         return check_launch("cl_verify_drafts");
     });
 }

@@ -28,8 +28,8 @@ def test_c_arguments_are_checked_before_the_device():
         return lib.cl_verify_drafts_workspace(dtype, s, k, v, ctypes.byref(need))
 
     assert size() == ok and need.value == 0
-    assert size(v=8192) == ok and need.value == 0
-    assert size(v=8193) == ok and need.value >= 2 * 7 * 2 * 8 + 2 * 32 + 2 * 2 * 24
+    assert size(v=4096) == ok and need.value == 0
+    assert size(v=8193) == ok and need.value >= 2 * 7 * 2 * 8 + 2 * 32 + 2 * 5 * 24
     assert size(dtype=4) == bad and size(s=-1) == bad and size(k=-1) == bad and size(v=0) == bad
     assert size(s=1 << 30, v=8193) == bad and b"too many" in lib.cl_last_error()
     assert size(v=1 << 60) == bad and size(k=1 << 60) == bad and size(s=1 << 60) == bad

@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float64, torch.float16, torch.bfloat16]
 # (sequences, drafts, classes): one chunk of a row and its borders, several; more positions than a
 # round of tests takes in either path
-SHAPES = [(1, 0, 1), (3, 0, 10), (5, 1, 2), (256, 4, 10), (7, 3, 63), (4, 2, 1000), (3, 5, 8191), (3, 5, 8192),
+SHAPES = [(1, 0, 1), (3, 0, 10), (5, 1, 2), (256, 4, 10), (7, 3, 63), (4, 2, 1000), (5, 9, 512), (3, 2, 513), (3, 2, 4096),
+          (3, 2, 4097), (3, 5, 8191), (3, 5, 8192),
           (3, 2, 8193), (2, 3, 20011), (1, 7, 131072), (2, 37, 8200), (5, 41, 50)]
 
 
