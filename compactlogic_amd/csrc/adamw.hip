@@ -22,11 +22,14 @@
 // make a step of m / eps.
 #include "storage.h"
 
+#include <algorithm>
+
 namespace cl {
 namespace {
 
 constexpr int kOptThreads = 256;
 constexpr int kTile = 2048;        // elements; whole blocks
+constexpr int kNormTile = 8192;
 constexpr int kTensors = 64;       // of a launch: a lane each
 constexpr int kGroups = 32;
 constexpr int kHeld = 256;         // elements of a block
@@ -83,7 +86,7 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads ts, double* _
                                                              Groups groups,
                                                              double* __restrict__ step,
                                                              double* __restrict__ coefs) {
-    constexpr int VEC = wide_vec<T>(), NV = kTile / kOptThreads / VEC;
+    constexpr int VEC = wide_vec<T>(), NV = kNormTile / kOptThreads / VEC;
     __shared__ double red[kOptThreads / 64];
     if (groups.n > 0 && blockIdx.x == 0 && wave_id() == 0) {
         const double t = step[0] + 1.0;
@@ -106,9 +109,9 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads ts, double* _
     double s = 0.0;
     for (uint32_t tile = blockIdx.x; tile < ts.tiles; tile += gridDim.x) {
         const int k = tensor_of(ts.first, tile);
-        const int64_t i0 = int64_t(tile - ts.first[k]) * kTile, n = ts.numel[k] - i0;
+        const int64_t i0 = int64_t(tile - ts.first[k]) * kNormTile, n = ts.numel[k] - i0;
         const T* g = static_cast<const T*>(ts.grad[k]) + i0;
-        if (n >= kTile) {
+        if (n >= kNormTile) {
             Pack<T, VEC> v[NV];
 #pragma unroll
             for (int j = 0; j < NV; ++j) v[j] = pload<T, VEC>(g + (j * kOptThreads + threadIdx.x) * VEC);
@@ -117,7 +120,16 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads ts, double* _
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) s = fma(double(v[j].v[e]), double(v[j].v[e]), s);
         } else {
-            for (int j = threadIdx.x; j < int(n); j += kOptThreads) s = fma(double(g[j]), double(g[j]), s);
+            const int packs = int(n) / VEC, rest = int(n) - packs * VEC;
+            for (int j = threadIdx.x; j < packs; j += kOptThreads) {
+                const Pack<T, VEC> v = pload<T, VEC>(g + j * VEC);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s = fma(double(v.v[e]), double(v.v[e]), s);
+            }
+            if (int(threadIdx.x) < rest) {
+                const double v = double(g[packs * VEC + threadIdx.x]);
+                s = fma(v, v, s);
+            }
         }
     }
     s = group_total(s, red);
@@ -156,7 +168,7 @@ __device__ __forceinline__ A param_step(A p, A m, A v, const Coefs<A>& c) {
     return fma(p, c.decay, -(c.size * quotient(m, v, c)));
 }
 
-// Every workgroup adds the same sums in the same order.
+// Every workgroup adds the same sums in the same order.  (A NaN scales nothing.)
 template <typename A>
 __device__ __forceinline__ Coefs<A> load_coefs(const double* __restrict__ parts, int nparts,
                                                double max_norm, const double* __restrict__ coefs,
@@ -173,10 +185,16 @@ __device__ __forceinline__ Coefs<A> load_coefs(const double* __restrict__ parts,
     r.eps = A(c[kEps]);
     r.scale = A(1);
     if (nparts > 0) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < nparts; i += kOptThreads) s += parts[i];
-        const double k = max_norm / (sqrt(group_total(s, red)) + 1e-6);
-        r.scale = A(k < 1.0 ? k : 1.0);
+        // by one wave: as much work as some two elements of each thread, and done once instead of by four
+        if (wave_id() == 0) {
+            double s = 0.0;
+#pragma unroll 8
+            for (int i = lane_id(); i < nparts; i += 64) s += parts[i];
+            const double k = max_norm / (sqrt(wave_total(s)) + 1e-6);
+            if (lane_id() == 0) red[0] = k < 1.0 ? k : 1.0;
+        }
+        __syncthreads();
+        r.scale = A(red[0]);
     }
     return r;
 }
@@ -200,21 +218,26 @@ struct Codes {
     uint2 m, v;
 };
 
-// Exponents of the block, from its largest finite magnitude, and the codes of this lane's elements.
-// A code of what is not finite is NaN, whatever the block's other elements are.
 struct Powers {
     int m, v;
 };
 
-// Leaves no m and v that are not finite.
+// 2^k for k in -127..127
+__device__ __forceinline__ float power_of_two(int k) { return __builtin_amdgcn_ldexpf(1.0f, k); }
+
+// Exponents of the block, from its largest finite magnitude, and the codes of this lane's elements.
+// A code of what is not finite is NaN, whatever the block's other elements are.  An infinite m comes
+// with a v that is not finite (the exponential average of finite numbers does not overflow); a NaN
+// is left out of a maximum and is converted to one.
 __device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& power) {
-    uint32_t top_m = 0, top_v = 0;
+    float top = 0.0f;
+    uint32_t top_v = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        top_m = max(top_m, bits_of(m[e]) & kMagnitude);
-        top_v = max(top_v, bits_of(v[e]) & kMagnitude);
+    for (int e = 0; e < 8; e += 2) {
+        top = __builtin_fmaxf(__builtin_fmaxf(top, __builtin_fabsf(m[e])), __builtin_fabsf(m[e + 1]));
+        top_v = max(max(top_v, bits_of(v[e])), bits_of(v[e + 1]));
     }
-    top_m = block_max(top_m);
+    uint32_t top_m = block_max(bits_of(top));
     top_v = block_max(top_v);
     const bool odd = max(top_m, top_v) >= kInfBits;
     uint32_t no_m = 0, no_v = 0;
@@ -241,19 +264,20 @@ __device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& po
     }
     power.m = max(int(top_m >> 23) - 134, -126);
     power.v = max(int(top_v >> 23) - 127, -126);
+    const float to_m = power_of_two(-power.m), to_v = power_of_two(-power.v);
     Codes c;
     uint32_t pm[2], pv[2] = {0, 0};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         float u[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = __builtin_amdgcn_ldexpf(m[4 * h + e], -power.m);
+        for (int e = 0; e < 4; ++e) u[e] = m[4 * h + e] * to_m;
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], 0, false);
         pm[h] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], w, true));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const uint32_t b = bits_of(__builtin_amdgcn_ldexpf(v[4 * h + e], -power.v));
-            const int r = int((b + 0x7FFFFu + ((b >> 20) & 1)) >> 20) - int(kFirstCode);
+            const uint32_t b = bits_of(v[4 * h + e] * to_v);
+            const int r = int(b + (0x7FFFFu - (kFirstCode << 20)) + ((b >> 20) & 1)) >> 20;
             // the middle one of r, 1 and a number that is 0 for v = 0 (r is then below 0) and else not
             // below r, nor 0 where scaling lost v
             const int some = int(b | bits_of(v[4 * h + e]));
@@ -276,21 +300,31 @@ __device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& po
 
 __device__ __forceinline__ void decode(const Codes& c, const Powers& power, float (&m)[8],
                                        float (&v)[8]) {
+    const float of_m = power_of_two(power.m), of_v = power_of_two(power.v);
     const uint32_t wm[2] = {c.m.x, c.m.y}, wv[2] = {c.v.x, c.v.y};
+    uint32_t least = 0xFF, most = 0;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         typedef float pair __attribute__((ext_vector_type(2)));
         const pair lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(wm[h]), false);
         const pair hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(wm[h]), true);
         const float u[4] = {lo.x, lo.y, hi.x, hi.y};
+        uint32_t code[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            m[4 * h + e] = __builtin_amdgcn_ldexpf(u[e], power.m);
-            const uint32_t code = (wv[h] >> (8 * e)) & 0xFFu;
-            // 255 has the bits of 2 * 1.125
-            uint32_t b = code == 0 ? 0u : (code + kFirstCode) << 20;
-            if (code == 0xFFu) b = 0x7FC00000u;
-            v[4 * h + e] = __builtin_amdgcn_ldexpf(float_of(b), power.v);
+            m[4 * h + e] = u[e] * of_m;
+            code[e] = (wv[h] >> (8 * e)) & 0xFFu;
+            v[4 * h + e] = float_of((code[e] << 20) + (kFirstCode << 20)) * of_v;
+        }
+        least = min(min(least, min(code[0], code[1])), min(code[2], code[3]));
+        most = max(max(most, max(code[0], code[1])), max(code[2], code[3]));
+    }
+    if (least == 0 || most == 0xFF) {  // 0 and NaN have no bits of that kind
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t code = (wv[e >> 2] >> (8 * (e & 3))) & 0xFFu;
+            if (code == 0) v[e] = 0.0f;
+            if (code == 0xFF) v[e] = __builtin_nanf("");
         }
     }
 }
@@ -346,30 +380,83 @@ __device__ __forceinline__ void store_eight(T* p, const Eight<T>& r, int count) 
         if (e < count) p[e] = r.v[e];
 }
 
-// Eight elements of a tile per thread, kHeld in 32 lanes; every lane takes part, those past the
-// tensor's end with count <= 0 (and zeros).
+// Eight elements of each half of a tile per thread, kHeld in 32 lanes; every lane takes part, those past
+// the tensor's end with a count of 0 (and zeros).  By halves, because a workgroup's loads are all under
+// way before its first computation.
+constexpr int kHalf = kOptThreads * 8, kHalves = kTile / kHalf;
+
 struct Place {
-    int64_t at;   // of the tensor
+    int64_t at, left;   // first element, and the tensor's from there on
     int64_t block, blocks;
-    int count;
     __device__ __forceinline__ Place(uint32_t tile, int64_t numel) {
         at = int64_t(tile) * kTile + threadIdx.x * 8;
+        left = numel - at;
         block = at / kHeld;
         blocks = (numel + kHeld - 1) / kHeld;
-        const int64_t left = numel - at;
-        count = left >= 8 ? 8 : left > 0 ? int(left) : 0;
     }
+    // WHOLE: the tile lies inside of the tensor.  That is asked once, not at every access: where a whole
+    // access and one by elements meet, the loads before them would be waited for.
+    template <bool WHOLE>
+    __device__ __forceinline__ int count(int h) const {
+        if constexpr (WHOLE) return 8;
+        const int64_t n = left - h * kHalf;
+        return n >= 8 ? 8 : n > 0 ? int(n) : 0;
+    }
+    __device__ __forceinline__ bool whole() const { return left + threadIdx.x * 8 >= kTile; }
 };
 
-__device__ __forceinline__ Powers load_powers(const uint8_t* power, const Place& at) {
-    if (at.count == 0) return {0, 0};
-    return {int(power[at.block]) - 127, int(power[at.blocks + at.block]) - 127};
+template <bool WHOLE>
+__device__ __forceinline__ Powers load_powers(const uint8_t* power, const Place& at, int h) {
+    if (at.count<WHOLE>(h) == 0) return {0, 0};
+    const uint8_t* p = power + at.block + h * (kHalf / kHeld);
+    return {int(p[0]) - 127, int(p[at.blocks]) - 127};
 }
 
-__device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, const Powers& p) {
-    if (at.count > 0 && (threadIdx.x & 31) == 0) {
-        power[at.block] = uint8_t(p.m + 127);
-        power[at.blocks + at.block] = uint8_t(p.v + 127);
+template <bool WHOLE>
+__device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, int h, const Powers& v) {
+    if (at.count<WHOLE>(h) > 0 && (threadIdx.x & 31) == 0) {
+        uint8_t* p = power + at.block + h * (kHalf / kHeld);
+        p[0] = uint8_t(v.m + 127);
+        p[at.blocks] = uint8_t(v.v + 127);
+    }
+}
+
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void step_tile8(const Tensors& ts, int k, const Place& at,
+                                           const double* __restrict__ parts, int nparts,
+                                           double max_norm, const double* __restrict__ coefs,
+                                           double* red) {
+    T* p = static_cast<T*>(ts.param[k]) + at.at;
+    const T* d = static_cast<const T*>(ts.grad[k]) + at.at;
+    uint8_t* pm = static_cast<uint8_t*>(ts.m[k]) + at.at;
+    uint8_t* pv = static_cast<uint8_t*>(ts.v[k]) + at.at;
+    Eight<T> w[kHalves], g[kHalves];
+    Codes held[kHalves];
+    Powers power[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        const int count = at.count<WHOLE>(h);
+        w[h] = load_eight(p + h * kHalf, count);
+        g[h] = load_eight(d + h * kHalf, count);
+        held[h] = {load_codes(pm + h * kHalf, count), load_codes(pv + h * kHalf, count)};
+        power[h] = load_powers<WHOLE>(ts.power[k], at, h);
+    }
+    const Coefs<float> c = load_coefs<float>(parts, nparts, max_norm, coefs, ts.group[k], red);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        const int count = at.count<WHOLE>(h);
+        float m[8], v[8];
+        decode(held[h], power[h], m, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            moments_step(float(g[h].v[e]), m[e], v[e], c);
+            w[h].v[e] = T(param_step(float(w[h].v[e]), m[e], v[e], c));
+        }
+        const Codes next = encode(m, v, power[h]);
+        store_eight(p + h * kHalf, w[h], count);
+        store_codes(pm + h * kHalf, next.m, count);
+        store_codes(pv + h * kHalf, next.v, count);
+        store_powers<WHOLE>(ts.power[k], at, h, power[h]);
     }
 }
 
@@ -382,26 +469,10 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors ts, const double
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
     const Place at(tile - ts.first[k], ts.numel[k]);
-    T* p = static_cast<T*>(ts.param[k]) + at.at;
-    uint8_t* pm = static_cast<uint8_t*>(ts.m[k]) + at.at;
-    uint8_t* pv = static_cast<uint8_t*>(ts.v[k]) + at.at;
-    Eight<T> w = load_eight(p, at.count);
-    const Eight<T> g = load_eight(static_cast<const T*>(ts.grad[k]) + at.at, at.count);
-    const Codes held{load_codes(pm, at.count), load_codes(pv, at.count)};
-    Powers power = load_powers(ts.power[k], at);
-    const Coefs<float> c = load_coefs<float>(parts, nparts, max_norm, coefs, ts.group[k], red);
-    float m[8], v[8];
-    decode(held, power, m, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        moments_step(float(g.v[e]), m[e], v[e], c);
-        w.v[e] = T(param_step(float(w.v[e]), m[e], v[e], c));
-    }
-    const Codes next = encode(m, v, power);
-    store_eight(p, w, at.count);
-    store_codes(pm, next.m, at.count);
-    store_codes(pv, next.v, at.count);
-    store_powers(ts.power[k], at, power);
+    if (at.whole())
+        step_tile8<T, true>(ts, k, at, parts, nparts, max_norm, coefs, red);
+    else
+        step_tile8<T, false>(ts, k, at, parts, nparts, max_norm, coefs, red);
 }
 
 template <typename T>
@@ -457,23 +528,66 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors ts, const double*
 
 // What 8 bits hold, in bf16 (which holds it all), and 8 bits from fp32.  param: exp_avg, grad:
 // exp_avg_sq as they are outside.
+template <bool WHOLE>
+__device__ __forceinline__ void read_tile8(const Tensors& ts, int k, const Place& at) {
+    Codes held[kHalves];
+    Powers power[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        const int64_t i = at.at + h * kHalf;
+        const int count = at.count<WHOLE>(h);
+        held[h] = {load_codes(static_cast<uint8_t*>(ts.m[k]) + i, count),
+                   load_codes(static_cast<uint8_t*>(ts.v[k]) + i, count)};
+        power[h] = load_powers<WHOLE>(ts.power[k], at, h);
+    }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        const int64_t i = at.at + h * kHalf;
+        const int count = at.count<WHOLE>(h);
+        float m[8], v[8];
+        decode(held[h], power[h], m, v);
+        Eight<bf16_t> a, b;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a.v[e] = bf16_t(m[e]);
+            b.v[e] = bf16_t(v[e]);
+        }
+        store_eight(static_cast<bf16_t*>(ts.param[k]) + i, a, count);
+        store_eight(static_cast<bf16_t*>(ts.grad[k]) + i, b, count);
+    }
+}
+
 __global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors ts) {
     const uint32_t tile = uint32_t(group_index());
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
     const Place at(tile - ts.first[k], ts.numel[k]);
-    const Codes held{load_codes(static_cast<uint8_t*>(ts.m[k]) + at.at, at.count),
-                     load_codes(static_cast<uint8_t*>(ts.v[k]) + at.at, at.count)};
-    float m[8], v[8];
-    decode(held, load_powers(ts.power[k], at), m, v);
-    Eight<bf16_t> a, b;
+    if (at.whole())
+        read_tile8<true>(ts, k, at);
+    else
+        read_tile8<false>(ts, k, at);
+}
+
+template <bool WHOLE>
+__device__ __forceinline__ void write_tile8(const Tensors& ts, int k, const Place& at) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        a.v[e] = bf16_t(m[e]);
-        b.v[e] = bf16_t(v[e]);
+    for (int h = 0; h < kHalves; ++h) {
+        const int64_t i = at.at + h * kHalf;
+        const int count = at.count<WHOLE>(h);
+        const Eight<float> a = load_eight(static_cast<const float*>(ts.param[k]) + i, count);
+        const Eight<float> b = load_eight(static_cast<const float*>(ts.grad[k]) + i, count);
+        float m[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m[e] = __builtin_isfinite(a.v[e]) ? a.v[e] : __builtin_nanf("");
+            v[e] = b.v[e] < 0.0f ? __builtin_nanf("") : b.v[e] + 0.0f;  // no -0
+        }
+        Powers power;
+        const Codes c = encode(m, v, power);
+        store_codes(static_cast<uint8_t*>(ts.m[k]) + i, c.m, count);
+        store_codes(static_cast<uint8_t*>(ts.v[k]) + i, c.v, count);
+        store_powers<WHOLE>(ts.power[k], at, h, power);
     }
-    store_eight(static_cast<bf16_t*>(ts.param[k]) + at.at, a, at.count);
-    store_eight(static_cast<bf16_t*>(ts.grad[k]) + at.at, b, at.count);
 }
 
 __global__ __launch_bounds__(kOptThreads) void k_adamw8_write(Tensors ts) {
@@ -481,19 +595,10 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8_write(Tensors ts) {
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
     const Place at(tile - ts.first[k], ts.numel[k]);
-    const Eight<float> a = load_eight(static_cast<const float*>(ts.param[k]) + at.at, at.count);
-    const Eight<float> b = load_eight(static_cast<const float*>(ts.grad[k]) + at.at, at.count);
-    float m[8], v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        m[e] = a.v[e];
-        v[e] = b.v[e] < 0.0f ? __builtin_nanf("") : b.v[e] + 0.0f;  // no -0
-    }
-    Powers power;
-    const Codes c = encode(m, v, power);
-    store_codes(static_cast<uint8_t*>(ts.m[k]) + at.at, c.m, at.count);
-    store_codes(static_cast<uint8_t*>(ts.v[k]) + at.at, c.v, at.count);
-    store_powers(ts.power[k], at, power);
+    if (at.whole())
+        write_tile8<true>(ts, k, at);
+    else
+        write_tile8<false>(ts, k, at);
 }
 
 // ---- tensors into launches
@@ -506,10 +611,6 @@ struct Batch {
         ts.n = 0;
         tiles = 0;
         for (int i = 0; i < kTensors; ++i) ts.first[i] = UINT32_MAX;
-    }
-    // Whether the tensor has a place in this launch.
-    bool fits(int64_t numel) const {
-        return ts.n < kTensors && tiles + ceil_div(numel, kTile) < (int64_t(1) << 31);
     }
     dim3 grid() const { return wide_grid(tiles); }
     void add(const cl_adamw_tensor& t) {
@@ -528,11 +629,12 @@ struct Batch {
     Grads grads() const {
         Grads g;
         g.n = ts.n;
-        g.tiles = uint32_t(tiles);
+        g.tiles = 0;
         for (int i = 0; i < kTensors; ++i) {
-            g.first[i] = ts.first[i];
+            g.first[i] = i < ts.n ? g.tiles : UINT32_MAX;
             g.numel[i] = ts.numel[i];
             g.grad[i] = ts.grad[i];
+            if (i < ts.n) g.tiles += uint32_t(ceil_div(ts.numel[i], kNormTile));
         }
         return g;
     }
@@ -556,7 +658,7 @@ int each_batch(const cl_adamw_tensor* t, int64_t n, Alike alike, F&& f) {
         b.clear();
         for (int64_t i = 0; i < n; ++i) {
             if (t[i].numel == 0 || kind_of(t[i], alike) != kind) continue;
-            if (!b.fits(t[i].numel)) {
+            if (b.ts.n == kTensors) {
                 if (int rc = f(kind, b)) return rc;
                 b.clear();
             }
@@ -584,10 +686,13 @@ int check_tensor(const cl_adamw_tensor& t, int64_t i, int64_t num_groups, bool v
     return CL_OK;
 }
 
-// Sums that a launch of the norm may leave: its share of kNormParts by its tiles, at least one.
-int64_t norm_parts(int64_t tiles, int64_t all) {
-    const int64_t share = tiles * kNormParts / all;
-    return share < 1 ? 1 : share < tiles ? share : tiles;
+// Sums that a launch of the norm leaves: a workgroup for each tile, but no more than its share of
+// kNormParts by its elements' tiles, or kTensors (of many small tensors, one workgroup would have to
+// go through some dozens).
+int64_t norm_parts(int64_t norm_tiles, int64_t tiles, int64_t all) {
+    int64_t share = tiles * kNormParts / all;
+    if (share < kTensors) share = kTensors;
+    return share < norm_tiles ? share : norm_tiles;
 }
 
 }  // namespace
@@ -599,8 +704,10 @@ extern "C" int cl_adamw_workspace(int64_t num_tensors, int64_t* bytes) {
     clear_error();
     CL_ARG(bytes, "null pointer argument");
     CL_ARG(num_tensors >= 0, "negative number of tensors");
-    // coefficients, and the norm's sums: kNormParts, and at most one more for each launch
-    *bytes = 8 * (kGroups * kCoefs + kNormParts + num_tensors);
+    // coefficients, and the norm's sums: kNormParts, and at most kTensors more for each launch, of which
+    // there are those that hold kTensors and one of each type
+    const int64_t launches = std::min<int64_t>(num_tensors, num_tensors / kTensors + 4);
+    *bytes = 8 * (kGroups * kCoefs + kNormParts + kTensors * launches);
     return CL_OK;
 }
 
@@ -630,6 +737,7 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
     for (int64_t i = 0; i < num_tensors; ++i) {
         if (int rc = check_tensor(tensors[i], i, num_groups, false)) return rc;
         all += ceil_div(tensors[i].numel, kTile);
+        CL_ARG(all < (int64_t(1) << 31), "too many elements for one call");
     }
     int64_t need = 0;
     if (int rc = cl_adamw_workspace(num_tensors, &need)) return rc;
@@ -653,8 +761,9 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
     if (gs.n == 0) gs.n = 1;  // the kernel counts the step along with the first group
     if (max_norm > 0 && all > 0) {
         const int rc = each_batch(tensors, num_tensors, Alike::kDtype, [&](int kind, const Batch& b) -> int {
-            const int64_t grid = norm_parts(b.tiles, all);
-            if (int r = begin(kind, b.grads(), unsigned(grid))) return r;
+            const Grads g = b.grads();
+            const int64_t grid = norm_parts(g.tiles, b.tiles, all);
+            if (int r = begin(kind, g, unsigned(grid))) return r;
             nparts += grid;
             return CL_OK;
         });
@@ -683,8 +792,12 @@ int moments(const char* what, bool read, int64_t num_tensors, const cl_adamw_ten
     clear_error();
     CL_ARG(num_tensors >= 0, "negative count");
     CL_ARG(num_tensors == 0 || tensors, "null pointer argument");
-    for (int64_t i = 0; i < num_tensors; ++i)
+    int64_t tiles = 0;
+    for (int64_t i = 0; i < num_tensors; ++i) {
         if (int rc = check_tensor(tensors[i], i, 0, true)) return rc;
+        tiles += ceil_div(tensors[i].numel, kTile);
+        CL_ARG(tiles < (int64_t(1) << 31), "too many elements for one call");
+    }
     hipStream_t s = as_stream(stream);
     return each_batch(tensors, num_tensors, Alike::kAll, [&](int, const Batch& b) -> int {
         if (read)

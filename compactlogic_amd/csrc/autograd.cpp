@@ -784,11 +784,10 @@ bool adamw_step(const py::list& param_groups, const py::dict& states, const Tens
     return true;
 }
 
-// 8-bit moments of each parameter from (write) or to the tensors of `first` and `second`.
-void adamw_moments(const std::vector<Tensor>& params, const py::list& states,
-                   const std::vector<Tensor>& first, const std::vector<Tensor>& second, bool write) {
-    if (params.empty()) return;
-    const c10::DeviceGuard guard(params[0].device());
+// 8-bit moments of the parameters, each with its state, taken in from fp32 tensors (write) or given
+// back into bf16 ones.
+void moments_between(const std::vector<Tensor>& params, const py::list& states,
+                     const std::vector<Tensor>& first, const std::vector<Tensor>& second, bool write) {
     std::vector<cl_adamw_tensor> tensors;
     for (size_t i = 0; i < params.size(); ++i) {
         cl_adamw_tensor t{};
@@ -799,11 +798,30 @@ void adamw_moments(const std::vector<Tensor>& params, const py::list& states,
         t.grad = second[i].data_ptr();
         tensors.push_back(t);
     }
+    const c10::DeviceGuard guard(params[0].device());
     launch(write ? "cl_adamw_moments_write" : "cl_adamw_moments_read", params[0].get_device(),
            [&](void* stream) {
                return (write ? cl_adamw_moments_write : cl_adamw_moments_read)(
                    int64_t(tensors.size()), tensors.data(), stream);
            });
+}
+
+void adamw_hold(const Tensor& param, const py::dict& state, const Tensor& first, const Tensor& second) {
+    py::list states;
+    states.append(state);
+    moments_between({param}, states, {first}, {second}, true);
+}
+
+std::pair<std::vector<Tensor>, std::vector<Tensor>> adamw_held(const std::vector<Tensor>& params,
+                                                               const py::list& states) {
+    std::vector<Tensor> first, second;
+    if (params.empty()) return {first, second};
+    for (const Tensor& p : params) {
+        first.push_back(at::empty(p.sizes(), p.options().dtype(at::kBFloat16)));
+        second.push_back(at::empty(p.sizes(), p.options().dtype(at::kBFloat16)));
+    }
+    moments_between(params, states, first, second, false);
+    return {first, second};
 }
 
 void set_timed(py::object timed) { g_timed.set(std::move(timed)); }
@@ -820,7 +838,8 @@ PYBIND11_MODULE(_autograd, m) {
     m.def("dropout", &dropout, unlocked());
     m.def("dropout_next", &dropout_next, unlocked());
     m.def("adamw_step", &adamw_step);
-    m.def("adamw_moments", &adamw_moments);
+    m.def("adamw_hold", &adamw_hold);
+    m.def("adamw_held", &adamw_held);
     m.def("set_timed", &set_timed);
     m.attr("torch_version") = TORCH_VERSION;
 }

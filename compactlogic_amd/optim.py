@@ -244,10 +244,9 @@ class FusedAdamW(_OneCount):
         elif small:
             _dl._check(p, "parameter")
             self._empty_small(p, st)
-            _native.load().adamw_moments([p], [st], [given["exp_avg"].float()],
-                                         [given["exp_avg_sq"].float()], True)
+            _native.load().adamw_hold(p, st, given["exp_avg"].float(), given["exp_avg_sq"].float())
         else:
-            held = self._read_small([p], [given])
+            held = _native.load().adamw_held([p], [given])
             st.pop("exponents", None)
             st["exp_avg"], st["exp_avg_sq"] = (t[0].float() for t in held)
 
@@ -257,13 +256,6 @@ class FusedAdamW(_OneCount):
                                     device=p.device).view(torch.float8_e4m3fn)
         st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
         st["exponents"] = torch.ones(2 * (-(-p.numel() // 256)), dtype=torch.uint8, device=p.device)
-
-    @staticmethod
-    def _read_small(params, states):
-        first = [torch.empty(p.shape, dtype=torch.bfloat16, device=p.device) for p in params]
-        second = [torch.empty_like(t) for t in first]
-        _native.load().adamw_moments(params, states, first, second, False)
-        return first, second
 
     def _prepare_states(self):
         """Moments for the parameters that have a gradient and none yet, checked for the others."""
@@ -314,16 +306,21 @@ class FusedAdamW(_OneCount):
         """(first, second): lists of the exponential averages of the gradient and of its square of
         `params` (default: every parameter that has them), in float32 (float64) where they are held
         in 32 bits and in bfloat16, which holds all of their values, where in 8."""
-        params = [p for p, _ in self._params() if "exp_avg" in self.state.get(p, {})] \
-            if params is None else list(params)
-        states = [self.state.get(p, {}) for p in params]
-        for st in states:
+        held = [(p, self.state[p]) for p, _ in self._params() if "exp_avg" in self.state.get(p, {})] \
+            if params is None else [(p, self.state.get(p, {})) for p in params]
+        first, second, small = [], [], []
+        for p, st in held:
             if "exp_avg" not in st:
                 raise RuntimeError("a parameter has no moments before its first step")
-        first, second = [st["exp_avg"] for st in states], [st["exp_avg_sq"] for st in states]
-        small = [i for i, st in enumerate(states) if "exponents" in st]
-        if small:
-            held = self._read_small([params[i] for i in small], [states[i] for i in small])
-            for i, m, v in zip(small, *held):
+            small.append("exponents" in st)
+            first.append(st["exp_avg"])
+            second.append(st["exp_avg_sq"])
+        if all(small):
+            return _native.load().adamw_held([p for p, _ in held], [st for _, st in held]) \
+                if small else (first, second)
+        if any(small):
+            at = [i for i, s in enumerate(small) if s]
+            values = _native.load().adamw_held([held[i][0] for i in at], [held[i][1] for i in at])
+            for i, m, v in zip(at, *values):
                 first[i], second[i] = m, v
         return first, second
