@@ -175,8 +175,10 @@ class FusedAdamW(_OneCount):
     lr, betas, eps, weight_decay and state_bits may differ between parameter groups (at most 32);
     ``max_norm`` is one for all, on the norm over all of them (float64 sums in a fixed order: steps
     are bitwise reproducible); None or <= 0 skips the clipping.  The gradients are left as they are:
-    unlike clip_grad_norm_ and FusedAdam, ``p.grad`` is not scaled.  Where it holds infinities or NaN
-    the step follows the formulas (an infinite norm scales finite gradients to 0).
+    unlike clip_grad_norm_ and FusedAdam, ``p.grad`` is not scaled.  An infinite norm scales finite
+    gradients to 0, a norm of NaN scales nothing; what is not finite stays in its own elements.
+    Hyper-parameters are read at every call; a step captured in a graph keeps those of its capture, and
+    the first step of a parameter, which makes its moments, cannot be captured.
 
     State dicts interchange with torch.optim.AdamW's (of float32 moments for parameters of any type)
     and between 32 and 8 bits.  Tensors that are of the type and on the device already are taken as
@@ -257,8 +259,15 @@ class FusedAdamW(_OneCount):
         st["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
         st["exponents"] = torch.ones(2 * (-(-p.numel() // 256)), dtype=torch.uint8, device=p.device)
 
+    @staticmethod
+    def _refuse_in_capture():
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW makes its state in the first step, which a graph would make "
+                               "again at every replay: step once before the capture")
+
     def _prepare_states(self):
         """Moments for the parameters that have a gradient and none yet, checked for the others."""
+        self._refuse_in_capture()
         for p, group in self._params():
             if p.grad is None:
                 continue
@@ -290,6 +299,7 @@ class FusedAdamW(_OneCount):
             if first is None:
                 return loss
             _dl._check(first, "parameter")
+            self._refuse_in_capture()
             self._step_t = torch.full((), self._loaded_step(), dtype=torch.float64,
                                       device=first.device)
             for st in self.state.values():

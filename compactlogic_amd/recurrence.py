@@ -84,6 +84,9 @@ class LogicRecurrence(torch.nn.Module):
         if x.dim() != 3 or x.shape[2] != self.in_dim:
             raise RuntimeError(f"x must be [batch, time, {self.in_dim}], got {tuple(x.shape)}")
         steps = x.shape[:2]
+        if steps.numel() == 0:
+            empty = x.new_zeros((*steps, self.out_dim))
+            return gated_recurrence(empty, empty, state, return_state=return_state)
         rows = to_rows(x.reshape(-1, self.in_dim)).transpose(0, 1)
         gate, data = self.gate(rows), self.data(rows)
         return gated_recurrence(data.unflatten(0, steps), gate.unflatten(0, steps), state,

@@ -294,6 +294,46 @@ def test_graph_replays_like_eager_steps(device, bits):
         assert float(og.state[graphed[0]]["step"]) == 2 + k
 
 
+def test_first_step_is_refused_in_a_capture(device, monkeypatch):
+    (p,) = _params([(10,)], torch.float32, device)
+    opt = cl.FusedAdamW([p])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        opt.step()
+    monkeypatch.undo()
+    opt.step()
+    (q,) = _params([(10,)], torch.float32, device)
+    opt.add_param_group({"params": [q]})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        opt.step()
+    assert float(opt.state[p]["step"]) == 1
+
+
+def test_changed_settings_between_steps(device):
+    """Bits, hyper-parameters and the gradients' types as they are at each call."""
+    p, q = _params([(300,), (40,)], torch.float32, device)
+    opt = cl.FusedAdamW([{"params": [p]}, {"params": [q]}], max_norm=None)
+    opt.step()
+    m = opt.state[p]["exp_avg"].clone()
+    opt.param_groups[0]["state_bits"] = 8
+    opt.param_groups[0]["lr"] = opt.param_groups[0]["weight_decay"] = 0.0
+    before = p.detach().clone()
+    opt.step()
+    assert torch.equal(p, before) and "exponents" in opt.state[p]
+    cm, _, powers = A.hold(m.cpu().numpy(), np.zeros(300))
+    held = A.values(cm, np.zeros(300, np.uint8), powers)[0]
+    want, _ = A.step32(_np(p.grad), held, np.zeros(300), 1.0, (0.9, 0.999))
+    cm, _, powers = A.hold(want, np.zeros(300))
+    np.testing.assert_array_equal(_np(opt.moments([p])[0][0]), A.values(cm, np.zeros(300, np.uint8), powers)[0])
+    first, second = opt.moments()
+    assert first[0].dtype == torch.bfloat16 and first[1].dtype == torch.float32
+    p.grad, p.grad_dtype = None, torch.float64
+    p.grad = torch.ones(300, dtype=torch.float64, device=device)
+    with pytest.raises(RuntimeError, match="dtype"):
+        opt.step()
+
+
 def test_another_stream_and_reproducible(device):
     runs = []
     for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):

@@ -403,3 +403,23 @@ def test_layer_in_eval_is_a_circuit(device):
     assert torch.equal(torch.cat(parts, 1), y)
     m.freeze()
     assert torch.equal(m(x), y)
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (3, 0)])
+def test_layer_without_steps(device, shape):
+    m = cl.LogicRecurrence(20, 16).to(device)
+    state = torch.rand(shape[0], 16, device=device)
+    y, last = m(torch.zeros(*shape, 20, device=device), state, return_state=True)
+    assert y.shape == (*shape, 16) and torch.equal(last, state)
+
+
+def test_layer_in_half(device):
+    """float16 sequences through the layers' half path, against its own outputs walked."""
+    torch.manual_seed(2)
+    m = cl.LogicRecurrence(40, 30).to(device)
+    x = torch.rand(4, 16, 40, device=device).half()
+    y, last = m(x, return_state=True)
+    gate, data = (f(x.reshape(-1, 40)).reshape(4, 16, 30) for f in (m.gate, m.data))
+    h, err = R.forward(_np(data), _np(gate), np.zeros((4, 30)), True)
+    _close(y, h, err, torch.float16)
+    _close(last, h[:, -1], err[:, -1], torch.float16, torch.float32)
