@@ -10,8 +10,8 @@
 //
 // Tensors are cut into tiles, so that a small one costs one workgroup; a launch takes kTensors
 // tensors of one type, their addresses in the kernel's arguments (a captured graph keeps them, and
-// nothing is copied to the device).  A lane holds one tensor's first tile, and the tile's tensor is
-// the number of lanes whose first tile is not behind it.
+// nothing is copied to the device), or kFewTensors in less of them.  A lane holds the first tile of one
+// or two tensors, and the tile's tensor is the number of those that are not behind it.
 //
 // Moments in 8 bits go by blocks of 256 consecutive elements, each with a power of two for m and one
 // for v: codes that have exponents of their own lose nothing by a power of two where a free scale
@@ -30,7 +30,7 @@ namespace {
 constexpr int kOptThreads = 256;
 constexpr int kTile = 2048;        // elements; whole blocks
 constexpr int kNormTile = 8192;
-constexpr int kTensors = 64;       // of a launch: a lane each
+constexpr int kFewTensors = 16, kTensors = 128;  // of a launch
 constexpr int kGroups = 32;
 constexpr int kHeld = 256;         // elements of a block
 constexpr int kNormParts = 512;
@@ -39,25 +39,27 @@ constexpr int kCoefs = 8;
 // A group's coefficients as the first kernel leaves them (fp64).
 enum { kDecay, kSize, kInvRoot, kB1, kRest1, kB2, kRest2, kEps };
 
+template <int N>
 struct Tensors {
     int n;
     uint32_t tiles;
-    uint32_t first[kTensors];  // first tile; those of no tensor: UINT32_MAX
-    int64_t numel[kTensors];
-    void* param[kTensors];
-    void* grad[kTensors];
-    void* m[kTensors];
-    void* v[kTensors];
-    uint8_t* power[kTensors];  // 8 bits: exponents + 127 of the blocks, m's and then v's
-    uint8_t group[kTensors];
+    uint32_t first[N];  // first tile; those of no tensor: UINT32_MAX
+    int64_t numel[N];
+    void* param[N];
+    void* grad[N];
+    void* m[N];
+    void* v[N];
+    uint8_t* power[N];  // 8 bits: exponents + 127 of the blocks, m's and then v's
+    uint8_t group[N];
 };
 
+template <int N>
 struct Grads {
     int n;
     uint32_t tiles;
-    uint32_t first[kTensors];
-    int64_t numel[kTensors];
-    const void* grad[kTensors];
+    uint32_t first[N];
+    int64_t numel[N];
+    const void* grad[N];
 };
 
 struct Groups {
@@ -66,8 +68,13 @@ struct Groups {
 };
 
 // The tensor that a tile lies in, the same in all lanes.
-__device__ __forceinline__ int tensor_of(const uint32_t* first, uint32_t tile) {
-    return int(__builtin_popcountll(__ballot(first[lane_id()] <= tile))) - 1;
+template <int N>
+__device__ __forceinline__ int tensor_of(const uint32_t (&first)[N], uint32_t tile) {
+    static_assert(N <= 64 || N == 128, "tensors of a launch");
+    const int l = lane_id();
+    int n = int(__builtin_popcountll(__ballot(l < N && first[l < N ? l : 0] <= tile)));
+    if constexpr (N == 128) n += int(__builtin_popcountll(__ballot(first[64 + l] <= tile)));
+    return n - 1;
 }
 
 // Sum over the workgroup, the same bits in every thread.
@@ -81,8 +88,8 @@ __device__ __forceinline__ double group_total(double v, double* red) {
     return s;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads ts, double* __restrict__ parts,
+template <typename T, int N>
+__global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads<N> ts, double* __restrict__ parts,
                                                              Groups groups,
                                                              double* __restrict__ step,
                                                              double* __restrict__ coefs) {
@@ -421,8 +428,8 @@ __device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, in
     }
 }
 
-template <typename T, bool WHOLE>
-__device__ __forceinline__ void step_tile8(const Tensors& ts, int k, const Place& at,
+template <typename T, bool WHOLE, int N>
+__device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Place& at,
                                            const double* __restrict__ parts, int nparts,
                                            double max_norm, const double* __restrict__ coefs,
                                            double* red) {
@@ -460,8 +467,8 @@ __device__ __forceinline__ void step_tile8(const Tensors& ts, int k, const Place
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors ts, const double* __restrict__ parts,
+template <typename T, int N>
+__global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors<N> ts, const double* __restrict__ parts,
                                                         int nparts, double max_norm,
                                                         const double* __restrict__ coefs) {
     __shared__ double red[kOptThreads / 64];
@@ -475,8 +482,8 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors ts, const double
         step_tile8<T, false>(ts, k, at, parts, nparts, max_norm, coefs, red);
 }
 
-template <typename T>
-__global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors ts, const double* __restrict__ parts,
+template <typename T, int N>
+__global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors<N> ts, const double* __restrict__ parts,
                                                        int nparts, double max_norm,
                                                        const double* __restrict__ coefs) {
     using A = wide_t<T>;
@@ -528,8 +535,8 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors ts, const double*
 
 // What 8 bits hold, in bf16 (which holds it all), and 8 bits from fp32.  param: exp_avg, grad:
 // exp_avg_sq as they are outside.
-template <bool WHOLE>
-__device__ __forceinline__ void read_tile8(const Tensors& ts, int k, const Place& at) {
+template <bool WHOLE, int N>
+__device__ __forceinline__ void read_tile8(const Tensors<N>& ts, int k, const Place& at) {
     Codes held[kHalves];
     Powers power[kHalves];
 #pragma unroll
@@ -557,7 +564,8 @@ __device__ __forceinline__ void read_tile8(const Tensors& ts, int k, const Place
     }
 }
 
-__global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors ts) {
+template <int N>
+__global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors<N> ts) {
     const uint32_t tile = uint32_t(group_index());
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
@@ -568,8 +576,8 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors ts) {
         read_tile8<false>(ts, k, at);
 }
 
-template <bool WHOLE>
-__device__ __forceinline__ void write_tile8(const Tensors& ts, int k, const Place& at) {
+template <bool WHOLE, int N>
+__device__ __forceinline__ void write_tile8(const Tensors<N>& ts, int k, const Place& at) {
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
         const int64_t i = at.at + h * kHalf;
@@ -590,7 +598,8 @@ __device__ __forceinline__ void write_tile8(const Tensors& ts, int k, const Plac
     }
 }
 
-__global__ __launch_bounds__(kOptThreads) void k_adamw8_write(Tensors ts) {
+template <int N>
+__global__ __launch_bounds__(kOptThreads) void k_adamw8_write(Tensors<N> ts) {
     const uint32_t tile = uint32_t(group_index());
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
@@ -603,42 +612,61 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8_write(Tensors ts) {
 
 // ---- tensors into launches
 struct Batch {
-    Tensors ts{};
+    int n = 0;
     int64_t tiles = 0;
+    const cl_adamw_tensor* t[kTensors];
 
-    Batch() { clear(); }
-    void clear() {
-        ts.n = 0;
-        tiles = 0;
-        for (int i = 0; i < kTensors; ++i) ts.first[i] = UINT32_MAX;
+    void add(const cl_adamw_tensor& tensor) {
+        t[n++] = &tensor;
+        tiles += ceil_div(tensor.numel, kTile);
     }
     dim3 grid() const { return wide_grid(tiles); }
-    void add(const cl_adamw_tensor& t) {
-        const int i = ts.n++;
-        ts.first[i] = uint32_t(tiles);
-        ts.numel[i] = t.numel;
-        ts.param[i] = t.param;
-        ts.grad[i] = t.grad;
-        ts.m[i] = t.exp_avg;
-        ts.v[i] = t.exp_avg_sq;
-        ts.power[i] = t.powers;
-        ts.group[i] = uint8_t(t.group);
-        tiles += ceil_div(t.numel, kTile);
-        ts.tiles = uint32_t(tiles);
+    template <int N>
+    Tensors<N> tensors() const {
+        Tensors<N> ts;
+        ts.n = n;
+        ts.tiles = 0;
+        for (int i = 0; i < N; ++i) {
+            ts.first[i] = i < n ? ts.tiles : UINT32_MAX;
+            if (i >= n) continue;
+            ts.numel[i] = t[i]->numel;
+            ts.param[i] = t[i]->param;
+            ts.grad[i] = t[i]->grad;
+            ts.m[i] = t[i]->exp_avg;
+            ts.v[i] = t[i]->exp_avg_sq;
+            ts.power[i] = t[i]->powers;
+            ts.group[i] = uint8_t(t[i]->group);
+            ts.tiles += uint32_t(ceil_div(t[i]->numel, kTile));
+        }
+        return ts;
     }
-    Grads grads() const {
-        Grads g;
-        g.n = ts.n;
+    template <int N>
+    Grads<N> grads() const {
+        Grads<N> g;
+        g.n = n;
         g.tiles = 0;
-        for (int i = 0; i < kTensors; ++i) {
-            g.first[i] = i < ts.n ? g.tiles : UINT32_MAX;
-            g.numel[i] = ts.numel[i];
-            g.grad[i] = ts.grad[i];
-            if (i < ts.n) g.tiles += uint32_t(ceil_div(ts.numel[i], kNormTile));
+        for (int i = 0; i < N; ++i) {
+            g.first[i] = i < n ? g.tiles : UINT32_MAX;
+            if (i >= n) continue;
+            g.numel[i] = t[i]->numel;
+            g.grad[i] = t[i]->grad;
+            g.tiles += uint32_t(ceil_div(t[i]->numel, kNormTile));
         }
         return g;
     }
 };
+
+// Runs the statement block with N bound to the tensors that a launch for n of them has room for.
+#define CL_ADAMW_ROOM(n, ...)              \
+    do {                                   \
+        if ((n) <= kFewTensors) {          \
+            constexpr int N = kFewTensors; \
+            __VA_ARGS__                    \
+        } else {                           \
+            constexpr int N = kTensors;    \
+            __VA_ARGS__                    \
+        }                                  \
+    } while (0)
 
 // What must be the same within a launch: the type of the gradients; that and the bits of the moments
 // (kinds from 4 on: 8 bits); nothing.
@@ -653,18 +681,17 @@ int kind_of(const cl_adamw_tensor& t, Alike alike) {
 // Calls f(kind, batch) for the launches that the tensors make, kind by kind.
 template <typename F>
 int each_batch(const cl_adamw_tensor* t, int64_t n, Alike alike, F&& f) {
-    Batch b;
     for (int kind = 0; kind < kKinds; ++kind) {
-        b.clear();
+        Batch b;
         for (int64_t i = 0; i < n; ++i) {
             if (t[i].numel == 0 || kind_of(t[i], alike) != kind) continue;
-            if (b.ts.n == kTensors) {
+            if (b.n == kTensors) {
                 if (int rc = f(kind, b)) return rc;
-                b.clear();
+                b = Batch();
             }
             b.add(t[i]);
         }
-        if (b.ts.n)
+        if (b.n)
             if (int rc = f(kind, b)) return rc;
     }
     return CL_OK;
@@ -749,37 +776,40 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
     double* parts = coefs + kGroups * kCoefs;
     int64_t nparts = 0;
     bool begun = false;
-    auto begin = [&](int kind, const Grads& g, unsigned grid) -> int {
+    auto begin = [&](int kind, const Batch& b) -> int {
         Groups now = gs;
         if (begun) now.n = 0;
         begun = true;
-        CL_STORAGE_SWITCH(kind, {
-            k_adamw_begin<scalar_t><<<grid, kOptThreads, 0, s>>>(g, parts + nparts, now, step, coefs);
+        unsigned grid = 1;
+        CL_ADAMW_ROOM(b.n, {
+            const Grads<N> g = b.grads<N>();
+            if (b.n) grid = unsigned(norm_parts(g.tiles, b.tiles, all));
+            CL_STORAGE_SWITCH(kind, {
+                k_adamw_begin<scalar_t, N><<<grid, kOptThreads, 0, s>>>(g, parts + nparts, now, step,
+                                                                       coefs);
+            });
         });
+        if (b.n) nparts += grid;
         return check_launch("cl_adamw_step(begin)");
     };
     if (gs.n == 0) gs.n = 1;  // the kernel counts the step along with the first group
     if (max_norm > 0 && all > 0) {
-        const int rc = each_batch(tensors, num_tensors, Alike::kDtype, [&](int kind, const Batch& b) -> int {
-            const Grads g = b.grads();
-            const int64_t grid = norm_parts(g.tiles, b.tiles, all);
-            if (int r = begin(kind, g, unsigned(grid))) return r;
-            nparts += grid;
-            return CL_OK;
-        });
-        if (rc) return rc;
+        if (int rc = each_batch(tensors, num_tensors, Alike::kDtype, begin)) return rc;
     } else {
-        Grads none{};
-        if (int rc = begin(CL_DTYPE_F32, none, 1)) return rc;
+        if (int rc = begin(CL_DTYPE_F32, Batch())) return rc;
     }
     return each_batch(tensors, num_tensors, Alike::kDtypeAndBits, [&](int kind, const Batch& b) -> int {
-        const dim3 grid = b.grid();
-        CL_STORAGE_SWITCH(kind & 3, {
-            if (kind < 4) {
-                k_adamw<scalar_t><<<grid, kOptThreads, 0, s>>>(b.ts, parts, int(nparts), max_norm, coefs);
-            } else if constexpr (!std::is_same_v<scalar_t, double>) {
-                k_adamw8<scalar_t><<<grid, kOptThreads, 0, s>>>(b.ts, parts, int(nparts), max_norm, coefs);
-            }
+        CL_ADAMW_ROOM(b.n, {
+            const Tensors<N> ts = b.tensors<N>();
+            CL_STORAGE_SWITCH(kind & 3, {
+                if (kind < 4) {
+                    k_adamw<scalar_t, N><<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts),
+                                                                         max_norm, coefs);
+                } else if constexpr (!std::is_same_v<scalar_t, double>) {
+                    k_adamw8<scalar_t, N><<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts),
+                                                                          max_norm, coefs);
+                }
+            });
         });
         return check_launch("cl_adamw_step");
     });
@@ -800,10 +830,13 @@ int moments(const char* what, bool read, int64_t num_tensors, const cl_adamw_ten
     }
     hipStream_t s = as_stream(stream);
     return each_batch(tensors, num_tensors, Alike::kAll, [&](int, const Batch& b) -> int {
-        if (read)
-            k_adamw8_read<<<b.grid(), kOptThreads, 0, s>>>(b.ts);
-        else
-            k_adamw8_write<<<b.grid(), kOptThreads, 0, s>>>(b.ts);
+        CL_ADAMW_ROOM(b.n, {
+            const Tensors<N> ts = b.tensors<N>();
+            if (read)
+                k_adamw8_read<N><<<b.grid(), kOptThreads, 0, s>>>(ts);
+            else
+                k_adamw8_write<N><<<b.grid(), kOptThreads, 0, s>>>(ts);
+        });
         return check_launch(what);
     });
 }

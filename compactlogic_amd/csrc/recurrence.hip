@@ -714,6 +714,13 @@ __global__ __launch_bounds__(kThreads) void k_rows_few(Args<T> a) {
     };
     auto put = [&](const States<A>& s, const A (&h)[VEC]) {
         if (!s.p) return;
+        if (s.si == 1 && count == VEC) {
+            Pack<A, VEC> all;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) all.v[e] = h[e];
+            pstore<A, VEC>(&s.at(o, i), all);
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
             if (e < count) s.at(o, i + e) = h[e];

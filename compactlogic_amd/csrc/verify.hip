@@ -248,16 +248,23 @@ __device__ __forceinline__ Draw decide(const Args<T>& a, int64_t seq, Round<LANE
 }
 
 // ---- fp64 sums over a workgroup
+// Sum up to and with each lane's v: within rows of 16 lanes by shifts (0 comes in from outside), then
+// the rows' sums in turn.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += dpp_move<0x111>(v);  // row_shr:1
+    v += dpp_move<0x112>(v);
+    v += dpp_move<0x114>(v);
+    v += dpp_move<0x118>(v);
+    const double a = read_lane(v, 15), b = a + read_lane(v, 31), c = b + read_lane(v, 47);
+    const int row = lane_id() >> 4;
+    return v + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? b : c);
+}
+
 // Sum up to and with each thread's v; `total`: of all.
 template <int WAVES>
 __device__ __forceinline__ double group_scan(double v, double* red, double& total) {
-    const int l = lane_id();
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-        const double before = __shfl_up(v, k, 64);
-        if (l >= k) v += before;
-    }
-    if (l == 63) red[wave_id()] = v;
+    v = wave_scan(v);
+    if (lane_id() == 63) red[wave_id()] = v;
     __syncthreads();
     double before = 0.0;
     total = 0.0;
@@ -309,7 +316,8 @@ struct Place {
     }
 };
 
-// exp(x - m) of the thread's elements in fp64, 0 behind them; returns their sum.
+// exp(x - m) of the thread's elements in fp64, 0 behind them (whose logits are -inf: asking for each
+// whether it is there, one exponential would wait for the other); returns their sum.
 template <typename T, int NT>
 __device__ __forceinline__ double exponentials(const T* row, const Place<T, NT>& w, double m,
                                                double (&e)[kRun]) {
@@ -321,7 +329,7 @@ __device__ __forceinline__ double exponentials(const T* row, const Place<T, NT>&
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
-        e[k] = k < w.count ? exp_below(double(v[k / VEC].v[k % VEC]) - m) : 0.0;
+        e[k] = exp_below(double(v[k / VEC].v[k % VEC]) - m);
         sum += e[k];
     }
     return sum;
@@ -362,16 +370,20 @@ __device__ __forceinline__ double over(const Rows<T>& r, const Place<T, NT>& w, 
     return sum;
 }
 
-// The place of the first weight up to and with which the sum is above `goal`, `before` counted in; the
-// last weight above 0 if rounding leaves none.  sh: first and last thread; the owner writes `*place`.
+// Draws the first token up to and with which the sum of the weights v is above `goal`, `before` counted
+// in; the last one with a weight above 0 if rounding leaves none.  mine, upto: the thread's sum of v, and
+// that up to and with it; e: its exponentials of the target's row, whose sum is sp.  The thread that
+// holds the token writes it, with its log-probability; where p is no probability, or no weight is above
+// 0, none is drawn.
 template <typename T, int NT>
-__device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T, NT>& w, double mine,
-                                         double upto, double before, double goal, int* sh,
-                                         int64_t* place) {
+__device__ __forceinline__ void draw(const Args<T>& a, int64_t seq, const Draw& d, const T* row,
+                                     const Place<T, NT>& w,
+                                     const double (&v)[kRun], const double (&e)[kRun], double sp,
+                                     double mine, double upto, double before, double goal, int* sh) {
+    using A = wide_t<T>;
     if (threadIdx.x == 0) {
         sh[0] = NT;
         sh[1] = -1;
-        *place = -1;
     }
     __syncthreads();
     if (mine > 0.0) {
@@ -379,31 +391,30 @@ __device__ __forceinline__ void place_of(const double (&e)[kRun], const Place<T,
         atomicMax(&sh[1], int(threadIdx.x));
     }
     __syncthreads();
-    const int owner = sh[0] < NT ? sh[0] : sh[1];
+    const bool hit = sh[0] < NT;
+    const int owner = !(sp > 0.0) ? -1 : hit ? sh[0] : sh[1];
+    const int64_t to = seq * (a.drafts + 1) + d.n;
     if (int(threadIdx.x) == owner) {
-        double c = before + (upto - mine);
-        int at = -1;
+        double c = before + (upto - mine), chosen = 0.0;
+        int at = 0;
         bool found = false;
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            c += e[k];
-            if (e[k] > 0.0 && !found) {
+            c += v[k];
+            if (v[k] > 0.0 && !found) {
                 at = k;
-                found = sh[0] < NT && c > goal;
+                chosen = e[k];
+                found = hit && c > goal;
             }
         }
-        *place = w.at + at;
+        a.out[to] = w.at + at;
+        // (the logit itself where its exponential has lost bits)
+        const double z = chosen > 1e-280 ? log(chosen) : double(row[w.at + at]) - d.mp;
+        a.lp[to] = A(z - log(sp));
+    } else if (owner < 0 && threadIdx.x == 0) {
+        a.out[to] = a.ignore;
+        a.lp[to] = A(__builtin_nan(""));
     }
-    __syncthreads();
-}
-
-template <typename T>
-__device__ __forceinline__ void put(const Args<T>& a, int64_t seq, const Draw& d, const T* p, double sp,
-                                    int64_t place) {
-    using A = wide_t<T>;
-    const int64_t to = seq * (a.drafts + 1) + d.n;
-    a.out[to] = place >= 0 ? place : a.ignore;
-    a.lp[to] = place >= 0 ? A((double(p[place]) - d.mp) - log(sp)) : A(__builtin_nan(""));
 }
 
 template <typename T, int LANES>
@@ -413,7 +424,6 @@ __global__ __launch_bounds__(kThreads) void k_small(Args<T> a) {
     __shared__ Round<LANES> round;
     __shared__ double red[WAVES];
     __shared__ int ends[2];
-    __shared__ int64_t place;
     const int64_t seq = group_index();
     if (seq >= a.seqs) return;
     const double u = a.uniform(seq, a.drafts);
@@ -440,22 +450,24 @@ __global__ __launch_bounds__(kThreads) void k_small(Args<T> a) {
     const double mine_q = r.q ? exponentials(r.q, w, d.mq, f) : 0.0;
     double upto = group_scan<WAVES>(mine, red, total);
     const double sp = total;
+    double v[kRun];
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) v[k] = e[k];
     if (d.refused) {
-        double sq = 1.0;
+        double sq = 1.0, total_v;
         if (r.q) group_scan<WAVES>(mine_q, red, sq);
-        double v[kRun], total_v;
         const double mine_v = over(r, w, e, f, 1.0 / sp, 1.0 / sq, v);
         const double upto_v = group_scan<WAVES>(mine_v, red, total_v);
-        if (total_v > 0.0) {  // else nothing is above the draft: the target's own
+        if (total_v > 0.0) {
             mine = mine_v;
             upto = upto_v;
             total = total_v;
+        } else {  // nothing is above the draft: the target's own
 #pragma unroll
-            for (int k = 0; k < kRun; ++k) e[k] = v[k];
+            for (int k = 0; k < kRun; ++k) v[k] = e[k];
         }
     }
-    place_of(e, w, mine, upto, 0.0, u * total, ends, &place);
-    if (threadIdx.x == 0) put(a, seq, d, r.p, sp, sp > 0.0 ? place : -1);
+    draw(a, seq, d, r.p, w, v, e, sp, mine, upto, 0.0, u * total, ends);
 }
 
 template <typename T>
@@ -529,48 +541,54 @@ __global__ __launch_bounds__(kDrawThreads) void k_pick(Args<T> a) {
     constexpr int WAVES = kDrawThreads / 64;
     __shared__ double red[WAVES];
     __shared__ int ends[2];
-    __shared__ int64_t place;
     const int64_t seq = group_index();
     if (seq >= a.seqs) return;
-    const Draw d = a.draws[seq];
-    const Rows<T> r(a, seq, d);
+    // a lane's chunks are read before anything is known of them (weights of a sequence that refused no
+    // token were not written, and are not used)
     const double* sums = a.sums + 2 * seq * a.chunks;
-    const double sp = chunks_total(sums, 2, a.chunks);
-    const double sq = r.q ? chunks_total(sums + 1, 2, a.chunks) : 1.0;
-    const double* parts = a.weights + seq * a.chunks;
-    int stride = 1;
-    double total = d.refused ? chunks_total(parts, 1, a.chunks) : 0.0;
-    const bool own = !(total > 0.0);  // the target's own: no draft was refused, or nothing is above it
-    if (own) {
-        parts = sums;
-        stride = 2;
-        total = sp;
+    const double* weights = a.weights + seq * a.chunks;
+    const Draw d = a.draws[seq];
+    const double u = a.uniform(seq, a.drafts);
+    const int l = lane_id();
+    double first_p = 0.0, first_q = 0.0, first_w = 0.0;
+    if (l < a.chunks) {
+        first_p = sums[2 * l];
+        first_q = sums[2 * l + 1];
+        first_w = weights[l];
     }
-    // the chunk, as place_of finds a place in it; every wave alike
-    const double goal = a.uniform(seq, a.drafts) * total;
+    const Rows<T> r(a, seq, d);
+    double sp = first_p, sq = r.q ? first_q : 0.0, total = d.refused ? first_w : 0.0;
+    for (int c = l + 64; c < a.chunks; c += 64) {
+        sp += sums[2 * int64_t(c)];
+        if (r.q) sq += sums[2 * int64_t(c) + 1];
+        if (d.refused) total += weights[c];
+    }
+    sp = wave_total(sp);
+    sq = r.q ? wave_total(sq) : 1.0;
+    total = wave_total(total);
+    const bool own = !(total > 0.0);  // the target's own: no draft was refused, or nothing is above it
+    if (own) total = sp;
+    // the chunk, as draw finds a place in it; every wave alike
+    const double goal = u * total;
     int chosen = -1, last = -1;
     double before = 0.0, at_last = 0.0, carry = 0.0;
     for (int c0 = 0; c0 < a.chunks && chosen < 0; c0 += 64) {
-        const int c = c0 + lane_id();
-        const double mine = c < a.chunks ? parts[int64_t(c) * stride] : 0.0;
-        double v = mine;
-#pragma unroll
-        for (int k = 1; k < 64; k *= 2) {
-            const double prior = __shfl_up(v, k, 64);
-            if (lane_id() >= k) v += prior;
-        }
+        const int c = c0 + l;
+        double mine = own ? first_p : first_w;
+        if (c0 > 0) mine = c >= a.chunks ? 0.0 : own ? sums[2 * int64_t(c)] : weights[c];
+        const double v = wave_scan(mine);
         const uint64_t some = __ballot(mine > 0.0);
         const uint64_t hit = __ballot(mine > 0.0 && carry + v > goal);
         const double start = __shfl_up(v, 1, 64);
-        const double prior = carry + (lane_id() == 0 ? 0.0 : start);
+        const double prior = carry + (l == 0 ? 0.0 : start);
         if (hit) {
-            const int l = __builtin_ctzll(hit);
-            chosen = c0 + l;
-            before = read_lane(prior, l);
+            const int h = __builtin_ctzll(hit);
+            chosen = c0 + h;
+            before = read_lane(prior, h);
         } else if (some) {
-            const int l = 63 - __builtin_clzll(some);
-            last = c0 + l;
-            at_last = read_lane(prior, l);
+            const int h = 63 - __builtin_clzll(some);
+            last = c0 + h;
+            at_last = read_lane(prior, h);
         }
         carry += read_lane(v, 63);
     }
@@ -578,24 +596,19 @@ __global__ __launch_bounds__(kDrawThreads) void k_pick(Args<T> a) {
         chosen = last;
         before = at_last;
     }
-    if (chosen < 0) {  // no weight anywhere, or NaN
-        if (threadIdx.x == 0) put(a, seq, d, r.p, sp, -1);
-        return;
-    }
-    const Place<T, kDrawThreads> w(int64_t(chosen) * kChunk, a.cols);
-    double e[kRun];
+    // (where no chunk has a weight, or NaN, the first one finds the same)
+    const Place<T, kDrawThreads> w(int64_t(chosen < 0 ? 0 : chosen) * kChunk, a.cols);
+    // (one copy of the code for either kind of weights: a workgroup alone waits for its instructions too)
+    double e[kRun], f[kRun] = {}, v[kRun], sum;
     double mine = exponentials(r.p, w, d.mp, e);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) v[k] = e[k];
     if (!own) {
-        double f[kRun] = {}, v[kRun];
         if (r.q) exponentials(r.q, w, d.mq, f);
         mine = over(r, w, e, f, 1.0 / sp, 1.0 / sq, v);
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) e[k] = v[k];
     }
-    double sum;
     const double upto = group_scan<WAVES>(mine, red, sum);
-    place_of(e, w, mine, upto, before, goal, ends, &place);
-    if (threadIdx.x == 0) put(a, seq, d, r.p, sp, sp > 0.0 ? place : -1);
+    draw(a, seq, d, r.p, w, v, e, sp, mine, upto, before, goal, ends);
 }
 
 // Parts and chunks of a row, and the arrays of the workspace behind each other on 16 bytes.

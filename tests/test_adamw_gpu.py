@@ -174,6 +174,35 @@ def test_many_tensors_of_every_type(device):
         np.testing.assert_allclose(_np(p), _np(q) * c, rtol=1e-5, atol=0)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_hundreds_of_tensors_captured(device, bits):
+    """Several launches of one type, whose addresses a graph keeps; and one launch more or less."""
+    for count in (16, 17, 128, 129, 300):
+        shapes = [((7 * i) % 613 + 1,) for i in range(count)]
+        ps, qs = (_params(shapes, torch.float32, device, seed=count) for _ in range(2))
+        op, oq = (cl.FusedAdamW(x, max_norm=0.2, state_bits=bits) for x in (ps, qs))
+        op.step()
+        oq.step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            oq.step()
+        for _ in range(3):
+            for p, q in zip(ps, qs):
+                p.grad.mul_(-0.9)
+                q.grad.copy_(p.grad)
+            op.step()
+            graph.replay()
+            torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+        scale = A.scale_of([_np(p.grad) for p in ps], 0.2)
+        before, (m, v) = [_np(p) for p in ps], ([_np(t) for t in ts] for ts in op.moments())
+        op.step()
+        for i, p in enumerate(ps):
+            (want, err), _, _ = A.step(before[i], _np(p.grad), m[i], v[i], 5, scale, 1e-3, (0.9, 0.999), 1e-8, 0.01)
+            _check(_np(p), want, err, torch.float32)
+
+
 def test_gradients_lie_anywhere_and_may_be_missing(device):
     p, q = _params([(64, 33), (50,)], torch.float32, device)
     g = p.grad.clone()

@@ -114,6 +114,13 @@ def test_ends_of_the_random_numbers(device, vocab):
         _check(cl.verify_drafts(logits, tokens, draft, uniforms), logits, tokens, draft, uniforms)
         wide = uniforms.double()
         _check(cl.verify_drafts(logits, tokens, draft, wide), logits, tokens, draft, wide)
+    # the likeliest token 740 above the others: probabilities below the smallest normal fp64 number
+    far = torch.full((40, 4, vocab), -740.0, device=device)
+    far[:, :, vocab // 2] = 0.0
+    none = torch.full((40, 3), -100, dtype=torch.int64, device=device)
+    uniforms = torch.zeros((40, 4), device=device)
+    want = _check(cl.verify_drafts(far, none, None, uniforms), far, none, None, uniforms)
+    assert (want[0][:, 0] == 0).all()
     # a draft that is the target: every token accepted below 1, and nothing above it to draw from at 1
     uniforms = torch.full((40, 4), below, device=device)
     tokens = draft.argmax(2)
