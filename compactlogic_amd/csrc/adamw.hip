@@ -350,10 +350,14 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t* p, int count) {
     return make_uint2(w[0], w[1]);
 }
 
+template <bool THROUGH>
 __device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int count) {
     if (count >= 8) {
         typedef uint32_t words __attribute__((ext_vector_type(2), aligned(1)));
-        *reinterpret_cast<words*>(p) = words{c.x, c.y};
+        if constexpr (THROUGH)
+            __builtin_nontemporal_store(words{c.x, c.y}, reinterpret_cast<words*>(p));
+        else
+            *reinterpret_cast<words*>(p) = words{c.x, c.y};
         return;
     }
     const uint32_t w[2] = {c.x, c.y};
@@ -376,10 +380,10 @@ __device__ __forceinline__ Eight<T> load_eight(const T* p, int count) {
     return r;
 }
 
-template <typename T>
+template <bool THROUGH, typename T>
 __device__ __forceinline__ void store_eight(T* p, const Eight<T>& r, int count) {
     if (count >= 8) {
-        pstore<T, 8>(p, __builtin_bit_cast(Pack<T, 8>, r));
+        pstore<T, 8, THROUGH>(p, __builtin_bit_cast(Pack<T, 8>, r));
         return;
     }
 #pragma unroll
@@ -428,7 +432,7 @@ __device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, in
     }
 }
 
-template <typename T, bool WHOLE, int N>
+template <typename T, bool WHOLE, bool THROUGH, int N>
 __device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Place& at,
                                            const double* __restrict__ parts, int nparts,
                                            double max_norm, const double* __restrict__ coefs,
@@ -460,14 +464,14 @@ __device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Pl
             w[h].v[e] = T(param_step(float(w[h].v[e]), m[e], v[e], c));
         }
         const Codes next = encode(m, v, power[h]);
-        store_eight(p + h * kHalf, w[h], count);
-        store_codes(pm + h * kHalf, next.m, count);
-        store_codes(pv + h * kHalf, next.v, count);
+        store_eight<THROUGH>(p + h * kHalf, w[h], count);
+        store_codes<THROUGH>(pm + h * kHalf, next.m, count);
+        store_codes<THROUGH>(pv + h * kHalf, next.v, count);
         store_powers<WHOLE>(ts.power[k], at, h, power[h]);
     }
 }
 
-template <typename T, int N>
+template <typename T, int N, bool THROUGH>
 __global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors<N> ts, const double* __restrict__ parts,
                                                         int nparts, double max_norm,
                                                         const double* __restrict__ coefs) {
@@ -477,9 +481,9 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors<N> ts, const dou
     const int k = tensor_of(ts.first, tile);
     const Place at(tile - ts.first[k], ts.numel[k]);
     if (at.whole())
-        step_tile8<T, true>(ts, k, at, parts, nparts, max_norm, coefs, red);
+        step_tile8<T, true, THROUGH>(ts, k, at, parts, nparts, max_norm, coefs, red);
     else
-        step_tile8<T, false>(ts, k, at, parts, nparts, max_norm, coefs, red);
+        step_tile8<T, false, THROUGH>(ts, k, at, parts, nparts, max_norm, coefs, red);
 }
 
 template <typename T, int N>
@@ -535,7 +539,7 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors<N> ts, const doub
 
 // What 8 bits hold, in bf16 (which holds it all), and 8 bits from fp32.  param: exp_avg, grad:
 // exp_avg_sq as they are outside.
-template <bool WHOLE, int N>
+template <bool WHOLE, bool THROUGH, int N>
 __device__ __forceinline__ void read_tile8(const Tensors<N>& ts, int k, const Place& at) {
     Codes held[kHalves];
     Powers power[kHalves];
@@ -559,21 +563,21 @@ __device__ __forceinline__ void read_tile8(const Tensors<N>& ts, int k, const Pl
             a.v[e] = bf16_t(m[e]);
             b.v[e] = bf16_t(v[e]);
         }
-        store_eight(static_cast<bf16_t*>(ts.param[k]) + i, a, count);
-        store_eight(static_cast<bf16_t*>(ts.grad[k]) + i, b, count);
+        store_eight<THROUGH>(static_cast<bf16_t*>(ts.param[k]) + i, a, count);
+        store_eight<THROUGH>(static_cast<bf16_t*>(ts.grad[k]) + i, b, count);
     }
 }
 
-template <int N>
+template <int N, bool THROUGH>
 __global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors<N> ts) {
     const uint32_t tile = uint32_t(group_index());
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
     const Place at(tile - ts.first[k], ts.numel[k]);
     if (at.whole())
-        read_tile8<true>(ts, k, at);
+        read_tile8<true, THROUGH>(ts, k, at);
     else
-        read_tile8<false>(ts, k, at);
+        read_tile8<false, THROUGH>(ts, k, at);
 }
 
 template <bool WHOLE, int N>
@@ -592,8 +596,8 @@ __device__ __forceinline__ void write_tile8(const Tensors<N>& ts, int k, const P
         }
         Powers power;
         const Codes c = encode(m, v, power);
-        store_codes(static_cast<uint8_t*>(ts.m[k]) + i, c.m, count);
-        store_codes(static_cast<uint8_t*>(ts.v[k]) + i, c.v, count);
+        store_codes<false>(static_cast<uint8_t*>(ts.m[k]) + i, c.m, count);
+        store_codes<false>(static_cast<uint8_t*>(ts.v[k]) + i, c.v, count);
         store_powers<WHOLE>(ts.power[k], at, h, power);
     }
 }
@@ -672,6 +676,12 @@ struct Batch {
 // (kinds from 4 on: 8 bits); nothing.
 enum class Alike { kDtype, kDtypeAndBits, kAll };
 constexpr int kKinds = 8;
+
+// From so many bytes on what a call with moments in 8 bits writes goes past the 256 MiB cache, where it
+// would push out what the next one reads (37.8 M bf16 elements, each step followed by giving the moments
+// back: 80 -> 65 us, the norm 20 -> 15, the moments 39 -> 35).  Steps alone, of more than the cache holds,
+// take the same time either way, and so do those with moments in 32 bits.
+constexpr double kThrough = 96 << 20;
 
 int kind_of(const cl_adamw_tensor& t, Alike alike) {
     if (alike == Alike::kAll) return 0;
@@ -761,8 +771,11 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
         gs.decay[i] = g.weight_decay;
     }
     int64_t all = 0;
+    double written = 0;
     for (int64_t i = 0; i < num_tensors; ++i) {
         if (int rc = check_tensor(tensors[i], i, num_groups, false)) return rc;
+        const int size = tensors[i].dtype == CL_DTYPE_F32 ? 4 : 2;
+        if (tensors[i].bits == 8) written += double(tensors[i].numel) * (size + 2);
         all += ceil_div(tensors[i].numel, kTile);
         CL_ARG(all < (int64_t(1) << 31), "too many elements for one call");
     }
@@ -771,6 +784,7 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
     CL_ARG(workspace && workspace_bytes >= need, "workspace of %lld bytes needed (cl_adamw_workspace)",
            (long long)need);
     CL_ARG(aligned(workspace, 8), "workspace must be aligned to 8 bytes");
+    const bool through = written >= kThrough;
     hipStream_t s = as_stream(stream);
     double* coefs = static_cast<double*>(workspace);
     double* parts = coefs + kGroups * kCoefs;
@@ -806,8 +820,8 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
                     k_adamw<scalar_t, N><<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts),
                                                                          max_norm, coefs);
                 } else if constexpr (!std::is_same_v<scalar_t, double>) {
-                    k_adamw8<scalar_t, N><<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts),
-                                                                          max_norm, coefs);
+                    (through ? k_adamw8<scalar_t, N, true> : k_adamw8<scalar_t, N, false>)
+                        <<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts), max_norm, coefs);
                 }
             });
         });
@@ -828,12 +842,14 @@ int moments(const char* what, bool read, int64_t num_tensors, const cl_adamw_ten
         tiles += ceil_div(tensors[i].numel, kTile);
         CL_ARG(tiles < (int64_t(1) << 31), "too many elements for one call");
     }
+    const bool through = double(tiles) * kTile * 4 >= kThrough;
     hipStream_t s = as_stream(stream);
     return each_batch(tensors, num_tensors, Alike::kAll, [&](int, const Batch& b) -> int {
         CL_ADAMW_ROOM(b.n, {
             const Tensors<N> ts = b.tensors<N>();
             if (read)
-                k_adamw8_read<N><<<b.grid(), kOptThreads, 0, s>>>(ts);
+                (through ? k_adamw8_read<N, true> : k_adamw8_read<N, false>)
+                    <<<b.grid(), kOptThreads, 0, s>>>(ts);
             else
                 k_adamw8_write<N><<<b.grid(), kOptThreads, 0, s>>>(ts);
         });
