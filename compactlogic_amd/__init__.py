@@ -5,9 +5,10 @@ LogicLayer, ConvLayer, GroupSum and the autograd bridges LogicLayerCudaFunction 
 ConvLayerCudaFunction, plus the packed-bit inference API (PackBitsTensor), and the logic-tree
 conv blocks of the third-party ConvLogic package (ConvLogicLayer, TreeLogicLayer,
 PoolLogicLayer).  Beside the reference's modules: losses for training by reward or preference
-(policy.py), dropout between logic layers (dropout_layer.py), a fused optimizer step (optim.py).
-All numerics run in libcompactlogic_hip.so, built in-tree (with the C++ autograd Functions of the
-losses and of dropout, csrc/autograd.cpp) by ``python -m compactlogic_amd.build``.
+(policy.py), dropout between logic layers (dropout_layer.py), recurrences over sequences
+(recurrence.py), the verification of drafted actions (drafts.py), fused optimizer steps (optim.py).
+All numerics run in libcompactlogic_hip.so, built in-tree (with the C++ side of the calls of all of
+these but FusedAdam, csrc/autograd.cpp) by ``python -m compactlogic_amd.build``.
 """
 from . import checkpoint, circuit, convlogic_hip, difflogic_hip
 from .dropout_layer import Dropout, dropout

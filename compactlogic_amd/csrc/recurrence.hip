@@ -204,8 +204,9 @@ struct Args {
 };
 
 // The place of this workgroup's work: consecutive workgroups go to the 8 XCDs in turn, each with an L2 of
-// its own, so each XCD gets a run of neighbours.  Two tiles that share lines of memory (64 bytes of a
-// row each) otherwise fetch every line twice.
+// its own, so each XCD gets a run of neighbours.  Tiles that share lines of memory otherwise fetch them
+// twice (8 x 4096 x 2048 bf16 in tiles of 64 bytes: forward 126 -> 106 us; 65521 x 251 fp32, whose rows
+// are off every line: 56 -> 35).
 __device__ __forceinline__ int64_t neighbour_index(int64_t groups) {
     const uint32_t b = uint32_t(group_index()), n = uint32_t(groups);
     if (b >= n) return b;
@@ -216,7 +217,10 @@ __device__ __forceinline__ int64_t neighbour_index(int64_t groups) {
 // ---------------------------------------------------------------- inner contiguous
 //
 // FL lanes side by side, of VEC places, TG groups of C steps each one after the other: a stretch is
-// TG * C steps.  The groups' maps go through LDS; one thread per inner place scans them.  While a
+// TG * C steps.  Long sequences take 16 lanes (128 bytes of 16-bit elements; 64 bytes were slower, 128
+// and 106 us became 99 and 88) and 32 groups of 8 steps, or of 4 in the backward, whose 8 spill: 8 x
+// 4096 x 2048 bf16 84 us forward (4.8 TB/s) and 128 backward (5.2), VALU 22 and 31 % busy; what is
+// missing to 6.2 is the latency of a stretch with one workgroup a CU.  The groups' maps go through LDS; one thread per inner place scans them.  While a
 // stretch is worked on, the loads of the next one are under way.
 //
 // Every access is a whole one: the last lane of a row starts VEC places before its end, beside (and
@@ -786,7 +790,8 @@ constexpr int64_t kFew = 8;
 //
 // L lanes of 16 bytes of one sequence one after the other: a stretch is L * VEC steps, scanned across
 // the lanes; 64 lanes for long sequences, which go through their stretches one by one, 16 or 4 where
-// one stretch of those is enough.
+// one stretch of those is enough.  Bound by memory: 64 x 64 x 12000 fp32 105 us forward (5.6 TB/s) and
+// 167 backward (5.9), VALU 60 % busy.
 
 // The value k lanes before (after: BACK) in the 16 lanes of a DPP row, `none` where there is none.
 template <bool BACK, int K, typename A>

@@ -18,7 +18,8 @@
 //   k_weights  the sum of max(p - q, 0) of its chunk
 //   k_pick     the chunk that the number falls into, and the place in it
 // Chunks are short because k_pick takes one by one workgroup, bound by its exponentials (8192 elements
-// of two rows took 11 us).
+// of two rows took 11 us).  256 sequences of 4 drafts of 10: 9 us, latency.  64 of 5 of 50021 bf16:
+// statistics 16 us (4.4 TB/s), sums, weights and place 9 to 10 each (the exponentials), tests 4.5.
 #include "row_loss.h"
 #include "storage.h"
 

@@ -12,6 +12,9 @@ them, and the Adam update of every parameter.  The step count is a device tensor
 captured in a HIP graph replays with correct bias corrections.  Sums have a fixed order: the
 update is bitwise reproducible.
 
+`FusedAdamW` is the same with decoupled weight decay over tensors of any type, and with moments in 8
+bits (cl_adamw_step); the reference has no counterpart of it.
+
 Differences from torch.optim.Adam: every parameter of the optimizer shares one step count,
 which advances on every call (torch advances a parameter's count only when it has a
 gradient); amsgrad and maximize are not supported, weight decay by `FusedAdamW` alone.  State dicts interchange
