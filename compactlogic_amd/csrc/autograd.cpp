@@ -5,8 +5,8 @@
 // A small call's kernels take 6 to 15 us.  As Functions in Python such calls took 76 to 97 us, here
 // 45 to 62: autograd runs a backward on a thread of its own, and an interpreter on either side of
 // that hand-over costs 30 us more (torch's own negation, forward and backward, takes 45).
-// Arguments are checked in policy.py, dropout_layer.py, recurrence.py and
-// drafts.py; nothing here is a public interface.
+// Most arguments are checked in policy.py, dropout_layer.py and drafts.py; nothing here is a public
+// interface.
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
@@ -601,9 +601,49 @@ struct Recurrence : Function<Recurrence> {
 
 // ---- what Python calls, with the arguments checked
 
+// (Its arguments are checked here: for one step of a sequence the checks in Python took 1.5 of 7 us.)
+std::string said(const Tensor& t) {
+    std::string s = "[";
+    for (const int64_t n : t.sizes()) s += (s.size() > 1 ? ", " : "") + std::to_string(n);
+    return s + "] " + c10::toString(t.scalar_type());
+}
+
 std::pair<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& gate,
-                                           const c10::optional<Tensor>& state, int64_t form) {
+                                           const c10::optional<Tensor>& given, int64_t form) {
+    const auto require = [](bool good, auto&& text) {
+        if (!good) throw std::runtime_error(text());
+    };
+    require(x.is_cuda() && gate.device() == x.device(),
+            [] { return std::string("x and gate must be on the same HIP device"); });
+    const at::ScalarType type = x.scalar_type();
+    require(type == at::kFloat || type == at::kDouble || type == at::kHalf || type == at::kBFloat16, [&] {
+        return std::string("unsupported floating dtype ") + c10::toString(type) +
+               "; the kernels take float16, bfloat16, float32 and float64";
+    });
+    require(x.dim() == 3 && gate.sizes() == x.sizes() && gate.scalar_type() == type, [&] {
+        return "x and gate must be [batch, time, features] of one shape and dtype, got " + said(x) +
+               " and " + said(gate);
+    });
+    require(x.layout() == at::kStrided && gate.layout() == at::kStrided,
+            [] { return std::string("x and gate must be dense"); });
     const c10::DeviceGuard guard(x.device());
+    const at::ScalarType wide = type == at::kDouble ? at::kDouble : at::kFloat;
+    c10::optional<Tensor> state = given;
+    if (given) {
+        const Tensor& h = *given;
+        require(h.device() == x.device() && h.dim() == 2 && h.size(0) == x.size(0) &&
+                    h.size(1) == x.size(2) && at::isFloatingType(h.scalar_type()) &&
+                    h.layout() == at::kStrided,
+                [&] {
+                    return "state must be a floating-point tensor of shape [" +
+                           std::to_string(x.size(0)) + ", " + std::to_string(x.size(2)) +
+                           "] on x's device, got " + said(h);
+                });
+        if (h.scalar_type() != wide) state = h.to(wide);
+    }
+    if (x.size(1) == 0)
+        return {x.clone(),
+                state ? state->clone() : at::zeros({x.size(0), x.size(2)}, x.options().dtype(wide))};
     const Tensor h0 = state.value_or(Tensor());
     if (at::GradMode::is_enabled() &&
         (x.requires_grad() || gate.requires_grad() || (h0.defined() && h0.requires_grad()))) {
@@ -833,7 +873,8 @@ PYBIND11_MODULE(_autograd, m) {
     m.def("selected_log_probs", &selected_log_probs, unlocked());
     m.def("policy_loss", &policy_loss, unlocked());
     m.def("preference_loss", &preference_loss, unlocked());
-    m.def("gated_recurrence", &gated_recurrence, unlocked());
+    m.def("gated_recurrence", &gated_recurrence, unlocked(), py::arg("x"), py::arg("gate"),
+          py::arg("state"), py::arg("form"));
     m.def("verify_drafts", &verify_drafts, unlocked());
     m.def("dropout", &dropout, unlocked());
     m.def("dropout_next", &dropout_next, unlocked());

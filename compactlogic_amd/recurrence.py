@@ -11,7 +11,6 @@ from __future__ import annotations
 import torch
 
 from . import _native
-from . import difflogic_hip as _dl
 from .layers import LogicLayer, PackBitsTensor, to_rows
 
 _FORMS = {"mix": 0, "add": 1}
@@ -32,32 +31,10 @@ def gated_recurrence(x, gate, state=None, form: str = "mix", return_state: bool 
     A gate of exactly 0 drops what came before, and one of exactly 1 leaves x unread in "mix": a
     sequence may begin anew inside of a row, or end before it, whatever the other steps hold, NaN
     included (the gate's own gradient is the formula's there)."""
-    if not isinstance(x, torch.Tensor) or not isinstance(gate, torch.Tensor):
-        raise TypeError("x and gate must be tensors")
-    if not x.is_cuda or gate.device != x.device:
-        raise RuntimeError("x and gate must be on the same HIP device")
-    _dl.storage_dtype_code(x)
-    if x.dim() != 3 or gate.shape != x.shape or gate.dtype != x.dtype:
-        raise RuntimeError(f"x and gate must be [batch, time, features] of one shape and dtype, got "
-                           f"{tuple(x.shape)} {x.dtype} and {tuple(gate.shape)} {gate.dtype}")
     code = _FORMS.get(form)
     if code is None:
         raise ValueError(f"form must be one of {sorted(_FORMS)}, got {form!r}")
-    if state is not None:
-        if not isinstance(state, torch.Tensor):
-            raise TypeError("state must be a tensor")
-        if state.device != x.device or state.shape != (x.shape[0], x.shape[2]) \
-                or not state.is_floating_point():
-            raise RuntimeError(f"state must be a floating-point tensor of shape "
-                               f"{(x.shape[0], x.shape[2])} on {x.device}")
-        wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-        if state.dtype != wide:
-            state = state.to(wide)
-    if x.shape[1] == 0:
-        wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-        last = x.new_zeros((x.shape[0], x.shape[2]), dtype=wide) if state is None else state.clone()
-        return (x.clone(), last) if return_state else x.clone()
-    y, last = _native.load().gated_recurrence(x, gate, state, code)
+    y, last = _native.load().gated_recurrence(x, gate, state, code)   # (the tensors are checked there)
     return (y, last) if return_state else y
 
 

@@ -44,7 +44,7 @@ def test_c_arguments_are_checked_before_the_device():
         return lib.cl_recurrence_sizes(dtype, order, batch, time, features, ctypes.byref(a), ctypes.byref(b))
 
     assert size() == ok and (a.value, b.value) == (0, 0)
-    assert size(time=1000) == ok and a.value == 4 * 8 and b.value > 0     # 4 stretches of 256 steps
+    assert size(time=1000) == ok and a.value == 8 * 8 and b.value > 0     # 8 stretches of 128 steps
     assert size(order=9) == bad and size(dtype=7) == bad and size(batch=-1) == bad
     assert size(order=3) == bad and b"one step" in lib.cl_last_error()
     assert size(order=3, time=1) == ok

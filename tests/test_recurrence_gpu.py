@@ -423,3 +423,22 @@ def test_layer_in_half(device):
     h, err = R.forward(_np(data), _np(gate), np.zeros((4, 30)), True)
     _close(y, h, err, torch.float16)
     _close(last, h[:, -1], err[:, -1], torch.float16, torch.float32)
+
+
+def test_gates_outside_of_the_unit_interval(device):
+    """Negative and growing gates are as good as any."""
+    gen = torch.Generator().manual_seed(3)
+    for shape in ((2, 70, 9), (3, 5, 40), (1, 300, 3)):
+        x, g = (torch.randn(shape, generator=gen).to(device) for _ in range(2))
+        g = (g * 0.4).clamp(-1.3, 1.3)
+        for layout in ("features", "time_features"):
+            for form in ("mix", "add"):
+                a, b = (_lay(t, layout).requires_grad_() for t in (x, g))
+                y = cl.gated_recurrence(a, b, form=form)
+                zero = np.zeros((shape[0], shape[2]))
+                h, err = R.forward(_np(x), _np(g), zero, form == "mix")
+                _close(y, h, err, torch.float32)
+                gx, gg = torch.autograd.grad(y, (a, b), torch.ones_like(y))
+                (wx, ex), (wg, eg), _ = R.backward(_np(x), _np(g), zero, np.ones(shape), zero, form == "mix")
+                _close(gx, wx, ex, torch.float32)
+                _close(gg, wg, eg, torch.float32)
