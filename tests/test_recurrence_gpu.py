@@ -442,3 +442,20 @@ def test_gates_outside_of_the_unit_interval(device):
                 (wx, ex), (wg, eg), _ = R.backward(_np(x), _np(g), zero, np.ones(shape), zero, form == "mix")
                 _close(gx, wx, ex, torch.float32)
                 _close(gg, wg, eg, torch.float32)
+
+
+@pytest.mark.parametrize("layout", ["features", "time_features"])
+def test_saved_tensors_may_move(device, layout):
+    """Hooks on saved tensors may hand them back with other strides; x and gate may be one tensor."""
+    x, g, gy, h0, gl = _inputs((3, 300, 17), torch.float32, device, 11)
+    a, b = (_lay(t, layout).requires_grad_() for t in (x, g))
+    y = cl.gated_recurrence(a, b, h0)
+    want = torch.autograd.grad(y, (a, b), gy)
+    for pack in (lambda t: t.cpu(), lambda t: t.contiguous().clone()):
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(device)):
+            y = cl.gated_recurrence(a, b, h0)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (a, b), gy), want))
+    one = cl.gated_recurrence(b, b, h0)
+    (got,) = torch.autograd.grad(one, b, gy)
+    (wx, ex), (wg, eg), _ = R.backward(_np(g), _np(g), _np(h0), _np(gy), 0 * _np(gl), True)
+    _close(got, wx + wg, ex + eg + np.abs(wx) + np.abs(wg), torch.float32)
