@@ -1140,10 +1140,27 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
         r.tiles = ceil_div(inner, vec);
         r.units = ceil_div(outer * r.tiles, kThreads);
     } else {
-        // 32 lanes side by side and 8 groups of 4 steps, or 16 and 32 (a forward of many steps: of 8)
-        r.way = inner < places ? kRowsNarrow : time <= 32 ? kRowsShort : kRowsLong;
-        r.stretch = r.way == kRowsShort ? 32 : r.way == kRowsLong ? 128 : 256;
-        r.tiles = r.way == kRowsNarrow ? 1 : ceil_div(inner, (r.way == kRowsShort ? 32 : 16) * places);
+        // 32 lanes side by side and 8 groups of 4 steps, whose workgroups are small and fill the chip
+        // without a long time, or 16 and 32 (a forward: of 8), whose stretches are fewer.  Measured,
+        // the first against the second, forward / backward in us:
+        //   256 x 33 x 1000 fp16   16 / 42   32 / 78      256 x 96 x 1000 fp32   48 / 102   76 / 121
+        //   64 x 64 x 12000 fp32  112 / 193 192 / 295     256 x 256 x 1000 fp16  87 / 152   92 / 188
+        //   64 x 1000 x 1024 fp32 153 / 260 150 / 252     16 x 4000 x 2048 fp16 256 / 270  178 / 270
+        // (The first is never cut into segments: up to 96 steps it has no two pairs of stretches.)
+        const int64_t broad = ceil_div(inner, 32 * places);
+        if (inner < places) {
+            r.way = kRowsNarrow;
+            r.tiles = 1;
+            r.stretch = 256;
+        } else if (time <= 96 || (time <= 512 && outer * broad >= 512)) {
+            r.way = kRowsShort;
+            r.tiles = broad;
+            r.stretch = 32;
+        } else {
+            r.way = kRowsLong;
+            r.tiles = ceil_div(inner, 16 * places);
+            r.stretch = 128;
+        }
         r.units = outer * r.tiles;
     }
     r.stretches = ceil_div(time, r.stretch);

@@ -96,6 +96,15 @@ def test_matches_a_walk(device, dtype, form, layout):
             assert y.is_contiguous()
 
 
+# up to three stretches of 32, one more step; many workgroups with up to 16 of them, one more step
+@pytest.mark.parametrize("shape", [(3, 65, 130), (3, 96, 5), (3, 97, 5), (512, 100, 6), (171, 512, 300),
+                                   (512, 513, 5)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_stretches_of_either_length(device, dtype, shape):
+    for layout in ("features", "padded"):
+        _run_and_check(shape, dtype, device, layout, "mix" if shape[0] > 3 else "add", 3)
+
+
 @pytest.mark.parametrize("shape", [(300, 1, 1), (1, 1, 300), (300, 40, 1), (1, 40, 300)])
 def test_dimensions_of_one(device, shape):
     for layout in LAYOUTS:
