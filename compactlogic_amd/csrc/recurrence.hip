@@ -789,7 +789,7 @@ constexpr int64_t kFew = 8;
 // ---------------------------------------------------------------- time contiguous
 //
 // L lanes of 16 bytes of one sequence one after the other: a stretch is L * VEC steps, scanned across
-// the lanes; 64 lanes for long sequences, which go through their stretches one by one, 16 or 4 where
+// the lanes; 64 lanes for long sequences, which go through their stretches one by one, 4 to 32 where
 // one stretch of those is enough.  Bound by memory: 64 x 64 x 12000 fp32 105 us forward (5.6 TB/s) and
 // 167 backward (5.9), VALU 60 % busy.
 
@@ -832,10 +832,8 @@ __device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
     const int l = lane_id() & (L - 1);
     scan_step<L, BACK, 1>(a, b, l);
     scan_step<L, BACK, 2>(a, b, l);
-    if constexpr (L >= 16) {
-        scan_step<L, BACK, 4>(a, b, l);
-        scan_step<L, BACK, 8>(a, b, l);
-    }
+    if constexpr (L >= 8) scan_step<L, BACK, 4>(a, b, l);
+    if constexpr (L >= 16) scan_step<L, BACK, 8>(a, b, l);
     A pa = beside<BACK, 1>(a, A(1)), pb = beside<BACK, 1>(b, A(0));
     if constexpr (L < 16) {
         if (BACK ? l + 1 >= L : l < 1) {
@@ -844,6 +842,14 @@ __device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
         }
     }
     A from = carry;
+    if constexpr (L == 32) {  // the state after the row of 16 before, in the lane's own half of the wave
+        constexpr int end = BACK ? 16 : 15;
+        const bool high = lane_id() >= 32;
+        const A la = read_lane(a, end), lb = read_lane(b, end);
+        const A ha = read_lane(a, end + 32), hb = read_lane(b, end + 32);
+        const A h = apply(high ? ha : la, carry, high ? hb : lb);
+        if (BACK ? l < 16 : l >= 16) from = h;
+    }
     if constexpr (L == 64) {
         constexpr int ends[4] = {BACK ? 48 : 15, BACK ? 32 : 31, BACK ? 16 : 47, BACK ? 0 : 63};
         const int row = BACK ? 3 - (l >> 4) : l >> 4;
@@ -1099,7 +1105,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
 // ---------------------------------------------------------------- launches
 
 // How a call goes: which kernels, and into how many segments of how many stretches.
-enum Way { kRowsFew, kRowsShort, kRowsLong, kRowsNarrow, kLines4, kLines16, kLines64 };
+enum Way { kRowsFew, kRowsShort, kRowsLong, kRowsNarrow, kLines4, kLines8, kLines16, kLines32, kLines64 };
 
 struct Route {
     Way way;
@@ -1130,8 +1136,9 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
     Route r{};
     const int64_t vec = vec_of(dtype), places = places_of(dtype);
     if (lines) {
-        const int l = time <= 4 * vec ? 4 : time <= 16 * vec ? 16 : 64;
-        r.way = l == 4 ? kLines4 : l == 16 ? kLines16 : kLines64;
+        int way = kLines4, l = 4;  // lanes of a sequence: as few as hold it
+        while (l < 64 && l * vec < time) l *= 2, ++way;
+        r.way = Way(way);
         r.stretch = l * vec;
         r.units = ceil_div(outer * inner, kThreads / l);
     } else if (time <= kFew) {
@@ -1237,11 +1244,23 @@ int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
             else
                 k_lines_forward<T, MIX, 4><<<grid, kThreads, 0, s>>>(a);
             break;
+        case kLines8:
+            if constexpr (BACK)
+                k_lines_backward<T, MIX, 8><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_lines_forward<T, MIX, 8><<<grid, kThreads, 0, s>>>(a);
+            break;
         case kLines16:
             if constexpr (BACK)
                 k_lines_backward<T, MIX, 16><<<grid, kThreads, 0, s>>>(a);
             else
                 k_lines_forward<T, MIX, 16><<<grid, kThreads, 0, s>>>(a);
+            break;
+        case kLines32:
+            if constexpr (BACK)
+                k_lines_backward<T, MIX, 32><<<grid, kThreads, 0, s>>>(a);
+            else
+                k_lines_forward<T, MIX, 32><<<grid, kThreads, 0, s>>>(a);
             break;
         case kLines64:
             if constexpr (BACK)
