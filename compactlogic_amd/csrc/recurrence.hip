@@ -789,8 +789,8 @@ constexpr int64_t kFew = 8;
 // ---------------------------------------------------------------- time contiguous
 //
 // L lanes of 16 bytes of one sequence one after the other: a stretch is L * VEC steps, scanned across
-// the lanes; 64 lanes for long sequences, which go through their stretches one by one, 4 to 32 where
-// one stretch of those is enough.  Bound by memory: 64 x 64 x 12000 fp32 105 us forward (5.6 TB/s) and
+// the lanes; 64 lanes for long sequences (32 for some), which go through their stretches one by one,
+// 4 to 32 where one stretch of those is enough.  Bound by memory: 64 x 64 x 12000 fp32 105 us forward (5.6 TB/s) and
 // 167 backward (5.9), VALU 60 % busy.
 
 // The value k lanes before (after: BACK) in the 16 lanes of a DPP row, `none` where there is none.
@@ -826,7 +826,7 @@ __device__ __forceinline__ void scan_step(A& a, A& b, int l) {
 }
 
 // From the lanes' maps and the state `carry` that the stretch starts with (BACK: from its end), the
-// state that each lane starts with; carry becomes the one after the stretch where L is 64.
+// state that each lane starts with; carry becomes the one after the stretch where L is 32 or 64.
 template <int L, bool BACK, typename A>
 __device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
     const int l = lane_id() & (L - 1);
@@ -843,12 +843,16 @@ __device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
     }
     A from = carry;
     if constexpr (L == 32) {  // the state after the row of 16 before, in the lane's own half of the wave
-        constexpr int end = BACK ? 16 : 15;
+        constexpr int ends[2] = {BACK ? 16 : 15, BACK ? 0 : 31};
         const bool high = lane_id() >= 32;
-        const A la = read_lane(a, end), lb = read_lane(b, end);
-        const A ha = read_lane(a, end + 32), hb = read_lane(b, end + 32);
-        const A h = apply(high ? ha : la, carry, high ? hb : lb);
+        auto after = [&](A h, int end) {
+            const A la = read_lane(a, end), lb = read_lane(b, end);
+            const A ha = read_lane(a, end + 32), hb = read_lane(b, end + 32);
+            return apply(high ? ha : la, h, high ? hb : lb);
+        };
+        const A h = after(carry, ends[0]);
         if (BACK ? l < 16 : l >= 16) from = h;
+        carry = after(h, ends[1]);
     }
     if constexpr (L == 64) {
         constexpr int ends[4] = {BACK ? 48 : 15, BACK ? 32 : 31, BACK ? 16 : 47, BACK ? 0 : 63};
@@ -913,7 +917,8 @@ __device__ __forceinline__ void line_map(const V& g, const V& x, Map<A>& m) {
     }
 }
 
-template <typename T, bool MIX, int L>
+// MORE: more than one stretch
+template <typename T, bool MIX, int L, bool MORE = L == 64>
 __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
     using A = wide_t<T>;
     using W = Line<T, L, false>;
@@ -933,7 +938,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
         const Few<T, VEC> xn = xs, gn = gs;
         const int now = count;
         const int64_t at = t;
-        if constexpr (L == 64) {  // the next stretch's loads are under way during this one's scan
+        if constexpr (MORE) {  // the next stretch's loads are under way during this one's scan
             if (s + W::STRETCH < t1) {
                 t += W::STRETCH;
                 count = w.count(t, a.time);
@@ -962,7 +967,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
     if (w.live && w.segment == a.segments - 1 && w.l == L - 1) a.last.at(w.o, w.i) = h;
 }
 
-template <typename T, bool MIX, int L>
+template <typename T, bool MIX, int L, bool MORE = L == 64>
 __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
     using A = wide_t<T>;
     using W = Line<T, L, true>;
@@ -985,7 +990,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
         gs = load_part<T, VEC>(g + t, count, T(1));
         ds = load_part<T, VEC>(gy + t, a.gy.p ? count : 0, T(0));
         if (w.live) {
-            if (L == 64 && a.starts)
+            if (MORE && a.starts)
                 start = a.starts[s * (a.outer * a.inner) + w.row];
             else if (a.h0.p)
                 start = a.h0.at(w.o, w.i);
@@ -999,7 +1004,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
         const int now = count;
         const int64_t at = t;
         A begin = start;
-        if constexpr (L == 64) {
+        if constexpr (MORE) {
             if (s > s0) {
                 t -= W::STRETCH;
                 load(s - 1);
@@ -1136,8 +1141,18 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
     Route r{};
     const int64_t vec = vec_of(dtype), places = places_of(dtype);
     if (lines) {
-        int way = kLines4, l = 4;  // lanes of a sequence: as few as hold it
-        while (l < 64 && l * vec < time) l *= 2, ++way;
+        // As few lanes a sequence as hold it; where 32 do not, 32 with two stretches, of 16-bit values
+        // three, or 64.  With 64 one stretch has no next one whose loads cover its scan, and many lanes
+        // have no steps: 64 x T x 12000, 32 lanes against 64, forward / backward in us:
+        //   fp32 T 129  310 / 444  411 / 516      bf16 T 300  352 / 658  516 / 918
+        //   fp32 T 200  346 / 588  411 / 524      bf16 T 500  456 / 775  557 / 1009
+        //   fp32 T 300  500 / 991  602 / 838      bf16 T 600  564 / 934  700 / 1172
+        //   fp32 T 500  933 / 1656 787 / 1427     bf16 T 1000 x 2000  159 / 286  147 / 246
+        // Few sequences take 64, and one stretch rather than two.
+        int way = kLines4, l = 4;
+        while (l < 32 && l * vec < time) l *= 2, ++way;
+        const bool many = outer * inner >= 256 * (kThreads / 32);
+        if (l * vec < time && !(many && time <= (vec == 8 ? 3 : 2) * 32 * vec)) l = 64, ++way;
         r.way = Way(way);
         r.stretch = l * vec;
         r.units = ceil_div(outer * inner, kThreads / l);
@@ -1256,11 +1271,18 @@ int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
             else
                 k_lines_forward<T, MIX, 16><<<grid, kThreads, 0, s>>>(a);
             break;
-        case kLines32:
-            if constexpr (BACK)
-                k_lines_backward<T, MIX, 32><<<grid, kThreads, 0, s>>>(a);
-            else
-                k_lines_forward<T, MIX, 32><<<grid, kThreads, 0, s>>>(a);
+        case kLines32:  // (one stretch by the other kernel, 64 x 200 x 12000 bf16: backward 427, 349 us)
+            if constexpr (BACK) {
+                if (r.stretches > 1)
+                    k_lines_backward<T, MIX, 32, true><<<grid, kThreads, 0, s>>>(a);
+                else
+                    k_lines_backward<T, MIX, 32><<<grid, kThreads, 0, s>>>(a);
+            } else {
+                if (r.stretches > 1)
+                    k_lines_forward<T, MIX, 32, true><<<grid, kThreads, 0, s>>>(a);
+                else
+                    k_lines_forward<T, MIX, 32><<<grid, kThreads, 0, s>>>(a);
+            }
             break;
         case kLines64:
             if constexpr (BACK)

@@ -105,6 +105,15 @@ def test_stretches_of_either_length(device, dtype, shape):
         _run_and_check(shape, dtype, device, layout, "mix" if shape[0] > 3 else "add", 3)
 
 
+# many sequences: one stretch of 32 lanes, two and three, then 64
+@pytest.mark.parametrize("shape", [(41, 65, 50), (2, 128, 1024), (41, 129, 50), (3, 257, 700), (41, 500, 50),
+                                   (41, 513, 50), (3, 769, 700)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lanes_of_either_count(device, dtype, shape):
+    for layout in ("time_batch", "padded time"):
+        _run_and_check(shape, dtype, device, layout, "add" if shape[0] > 3 else "mix", 4)
+
+
 @pytest.mark.parametrize("shape", [(300, 1, 1), (1, 1, 300), (300, 40, 1), (1, 40, 300)])
 def test_dimensions_of_one(device, shape):
     for layout in LAYOUTS:
