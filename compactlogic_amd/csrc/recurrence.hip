@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
 // ---------------------------------------------------------------- launches
 
 // How a call goes: which kernels, and into how many segments of how many stretches.
-enum Way { kRowsFew, kRowsShort, kRowsLong, kRowsNarrow, kLines4, kLines8, kLines16, kLines32, kLines64 };
+enum Way { kRowsFew, kRowsHalf, kRowsShort, kRowsLong, kRowsNarrow, kLines4, kLines8, kLines16, kLines32, kLines64 };
 
 struct Route {
     Way way;
@@ -1162,22 +1162,27 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
         r.tiles = ceil_div(inner, vec);
         r.units = ceil_div(outer * r.tiles, kThreads);
     } else {
-        // 32 lanes side by side and 8 groups of 4 steps, whose workgroups are small and fill the chip
+        // 32 lanes side by side and 8 groups (4) of 4 steps, whose workgroups are small and fill the chip
         // without a long time, or 16 and 32 (a forward: of 8), whose stretches are fewer.  Measured,
         // the first against the second, forward / backward in us:
-        //   256 x 33 x 1000 fp16   16 / 42   32 / 78      256 x 96 x 1000 fp32   48 / 102   76 / 121
-        //   64 x 64 x 12000 fp32  112 / 193 192 / 295     256 x 256 x 1000 fp16  87 / 152   92 / 188
+        //   256 x 64 x 1000 fp16   19 / 32   32 / 77      256 x 96 x 1000 fp32   48 / 102   76 / 121
+        //   64 x 64 x 12000 fp32  112 / 193 192 / 295     256 x 256 x 1000 fp16  71 / 152   92 / 188
         //   64 x 1000 x 1024 fp32 153 / 260 150 / 252     16 x 4000 x 2048 fp16 256 / 270  178 / 270
-        // (The first is never cut into segments: up to 96 steps it has no two pairs of stretches.)
+        // (The first is never cut into segments: up to 96 steps or with 512 workgroups.)
         const int64_t broad = ceil_div(inner, 32 * places);
         if (inner < places) {
             r.way = kRowsNarrow;
             r.tiles = 1;
             r.stretch = 256;
         } else if (time <= 96 || (time <= 512 && outer * broad >= 512)) {
-            r.way = kRowsShort;
+            // Stretches of 16, by 4 groups, where they leave fewer groups without steps: one instead of 32
+            // for 512 x 16 x 4000 fp16 58 / 170 -> 34 / 70, two for 512 x 24 x 4000 fp16 82 / 187 ->
+            // 63 / 144, three for 256 x 48 x 1000 fp32 27 / 56 -> 24 / 40 (four 66 -> 69 backward; where
+            // there is no other workgroup to hide it, each further one costs 2 us).
+            const bool half = time <= 16 || (time <= 48 && outer * broad >= 512);
+            r.way = half ? kRowsHalf : kRowsShort;
             r.tiles = broad;
-            r.stretch = 32;
+            r.stretch = half ? 16 : 32;
         } else {
             r.way = kRowsLong;
             r.tiles = ceil_div(inner, 16 * places);
@@ -1227,9 +1232,17 @@ int launch_recurrence(const Args<T>& a, const Route& r, hipStream_t s) {
             else
                 k_rows_few<T, MIX, BACK, int(kFew)><<<grid, kThreads, 0, s>>>(a);
             break;
-        case kRowsShort:
+        case kRowsHalf:
+            if constexpr (BACK)
+                k_rows_backward<T, MIX, 32, 4, 4, P><<<grid, 128, 0, s>>>(a);
+            else
+                k_rows_forward<T, MIX, 32, 4, 4, P, 1><<<grid, 128, 0, s>>>(a);
+            break;
+        case kRowsShort:  // (the forward past the cache: 256 x 256 x 1000 fp16 89 -> 71 us; no gain in the backward)
             if constexpr (BACK)
                 k_rows_backward<T, MIX, 32, 8, 4, P><<<grid, kThreads, 0, s>>>(a);
+            else if (through)
+                k_rows_forward<T, MIX, 32, 8, 4, P, 1, true><<<grid, kThreads, 0, s>>>(a);
             else
                 k_rows_forward<T, MIX, 32, 8, 4, P, 1><<<grid, kThreads, 0, s>>>(a);
             break;

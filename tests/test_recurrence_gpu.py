@@ -96,9 +96,10 @@ def test_matches_a_walk(device, dtype, form, layout):
             assert y.is_contiguous()
 
 
-# up to three stretches of 32, one more step; many workgroups with up to 16 of them, one more step
-@pytest.mark.parametrize("shape", [(3, 65, 130), (3, 96, 5), (3, 97, 5), (512, 100, 6), (171, 512, 300),
-                                   (512, 513, 5)])
+# one stretch of 16, up to three of 32, one more step; many workgroups with up to 16 of them, one more step
+@pytest.mark.parametrize("shape", [(2, 9, 4), (3, 16, 131), (70, 13, 300), (2, 17, 9), (3, 65, 130), (3, 96, 5),
+                                   (3, 97, 5), (512, 17, 6), (513, 48, 5), (512, 49, 6), (512, 100, 6),
+                                   (171, 512, 300), (512, 513, 5)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_stretches_of_either_length(device, dtype, shape):
     for layout in ("features", "padded"):
