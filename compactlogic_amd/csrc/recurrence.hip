@@ -13,6 +13,11 @@
 // A gate of exactly 0 drops what came before and one of exactly 1 leaves x unread, NaN and infinities
 // too: a * h is not formed where a is 0, and a product of gates that are not 0 is kept from becoming 0.
 //
+// Gates may be of any magnitude.  A product of gates that passes the range says nothing about a state of
+// 0, or a small one, that it is applied to: where a thread's product does (or, in a scan, is above
+// kGrowth, so that sixteen of them may), the threads' steps are walked one after the other instead, and
+// the maps of segments have factors with an exponent of their own.
+//
 // Where there are too few sequences for the chip, time is cut into segments: a first pass finds the
 // map of each (reading everything once more), and every segment starts from the maps before it.
 //
@@ -52,6 +57,13 @@ __device__ __forceinline__ double least_magnitude(double a, double b) {
     return __builtin_fmin(a, __builtin_fabs(b));
 }
 
+__device__ __forceinline__ float greatest_magnitude(float a, float b) {
+    return __builtin_fmaxf(a, __builtin_fabsf(b));
+}
+__device__ __forceinline__ double greatest_magnitude(double a, double b) {
+    return __builtin_fmax(a, __builtin_fabs(b));
+}
+
 // One step.  The rules of the ends of the gate differ from plain arithmetic only where something is
 // not finite, and what is not finite stays so (0 * inf and 0 * NaN are NaN): a walk is taken in plain
 // arithmetic, and again by the rules (EXACT) if its last value is not finite.  That saves three of some
@@ -86,6 +98,95 @@ __device__ __forceinline__ bool finite(A v) {
     return __builtin_isfinite(v);
 }
 
+// A product of gates, m 2^e: it neither leaves the range nor becomes 0.  |m| <= 1, and e is kept to where
+// sums of it and a type's exponents fit 32 bits.
+__device__ __forceinline__ float mantissa(float v) { return __builtin_amdgcn_frexp_mantf(v); }
+__device__ __forceinline__ double mantissa(double v) { return __builtin_amdgcn_frexp_mant(v); }
+__device__ __forceinline__ int exponent(float v) { return __builtin_amdgcn_frexp_expf(v); }
+__device__ __forceinline__ int exponent(double v) { return __builtin_amdgcn_frexp_exp(v); }
+__device__ __forceinline__ float scaled(float m, int e) { return __builtin_amdgcn_ldexpf(m, e); }
+__device__ __forceinline__ double scaled(double m, int e) { return __builtin_amdgcn_ldexp(m, e); }
+
+constexpr float kSmall = 1.0f / 32768.0f;  // eight of them are a normal number
+
+template <typename A>
+struct Product {
+    A m = A(1);
+    int e = 0;
+    // (at most 126 of them before the next `even`)
+    __device__ __forceinline__ void by(A m2, int e2) {
+        m = m == A(0) || m2 == A(0) ? A(0) : m * m2;
+        e += e2;
+    }
+    __device__ __forceinline__ void by(A gate) { by(mantissa(gate), exponent(gate)); }
+    __device__ __forceinline__ void even() {
+        constexpr int most = 1 << 24;
+        const int k = e + exponent(m);
+        e = k < -most ? -most : k > most ? most : k;
+        m = mantissa(m);
+    }
+    // An exponent of 0 where the product is a normal number (or 0, infinite, NaN).
+    __device__ __forceinline__ void plain() {
+        constexpr int most = sizeof(A) == 4 ? 127 : 1023;
+        even();
+        if (m == A(0) || !__builtin_isfinite(m) || (e > 1 - most && e <= most)) {
+            m = scaled(m, e);
+            e = 0;
+        }
+    }
+    // m 2^e h + b: only the result may leave the range
+    __device__ __forceinline__ A applied(A h, A b) const {
+        const A r = scaled(mantissa(h) * m, exponent(h) + e) + b;
+        return m == A(0) ? b : r;
+    }
+};
+
+// Each product of f by the gates of N <= 8 steps at its place, at once where they are neither small nor
+// infinite, nor NaN.
+template <int N, int VEC, typename A, typename V>
+__device__ __forceinline__ void by_steps(Product<A> (&f)[VEC], const V (&gs)[N]) {
+    static_assert(N <= 8);
+    A p[VEC], lowest = A(1), rest = A(0);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        p[e] = A(1);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            p[e] *= A(gs[k][e]);
+            lowest = least_magnitude(lowest, A(gs[k][e]));
+        }
+        rest = fma(p[e], A(0), rest);
+    }
+    if (lowest >= A(kSmall) && rest == A(0)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e].by(p[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+#pragma unroll
+            for (int k = 0; k < N; ++k) f[e].by(A(gs[k][e]));
+    }
+}
+
+// The first `count` of the maps (f, b) applied to h in turn: in one instruction each where no factor has
+// an exponent, in five else.
+template <int N, typename A>
+__device__ __forceinline__ A all_applied(const Product<A> (&f)[N], const A (&b)[N], int count, A h) {
+    int e = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) e |= f[k].e;
+    if (e == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < count) h = apply(f[k].m, h, b[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < count) h = f[k].applied(h, b[k]);
+    }
+    return h;
+}
+
 // The map of consecutive steps.
 template <typename A>
 struct Map {
@@ -103,7 +204,18 @@ struct Map {
     __device__ __forceinline__ A factor() const {
         return lowest == A(0) ? A(0) : a == A(0) ? least(a) : a;
     }
+    // Of a factor that has not left the range a product on the way may have, below it, if one of the
+    // gates was small.  (As whole numbers, so that 0 is none of them in the same comparison.)
+    using Bits = std::conditional_t<sizeof(A) == 4, uint32_t, uint64_t>;
+    __device__ __forceinline__ Bits lowest_bits() const { return __builtin_bit_cast(Bits, lowest) - 1; }
+    static __device__ __forceinline__ bool small(Bits lowest) {
+        return lowest < __builtin_bit_cast(Bits, A(kSmall)) - 1;
+    }
 };
+
+// From where on a lane's factor is not multiplied with its neighbours': sixteen of this one are 2^64, and
+// what a product below the smallest number leaves of a state, by as much, is below 2^-80 of it.
+constexpr float kGrowth = 16.0f;
 
 // N elements of an access of 8 or 16 bytes at any address that is a multiple of the element size.  They
 // stay as they were loaded until they are used: unpacked where the loads of a partial access and of a
@@ -196,6 +308,7 @@ struct Args {
     States<A> gh0;
     A* starts;               // states at the stretches' starts [stretch, outer, inner]; may be null
     A* maps;                 // [segment][a, b][outer, inner]; null: one segment
+    int* exps;               // of a, [segment][outer, inner]
     int64_t outer, time, inner;
     int segments;
     int64_t per_segment;     // stretches
@@ -312,20 +425,20 @@ __device__ __forceinline__ wide_t<T> segment_start(const Args<T>& a, int64_t seg
     if (!a.maps) return h;
     const int64_t n = a.outer * a.inner;
     const A* m = a.maps + o * a.inner + i;
+    const int* exps = a.exps + o * a.inner + i;
     constexpr int U = 16;  // loads under way at once: one by one, 63 maps took 40 us
     const int count = int(BACK ? a.segments - 1 - segment : segment);
     for (int k0 = 0; k0 < count; k0 += U) {
-        A f[U], b[U];
+        Product<A> f[U];
+        A b[U];
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int j = k0 + k < count ? k0 + k : count - 1;
             const int64_t s = BACK ? a.segments - 1 - j : j;
-            f[k] = m[2 * s * n];
+            f[k] = {m[2 * s * n], exps[s * n]};
             b[k] = m[(2 * s + 1) * n];
         }
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (k0 + k < count) h = apply(f[k], h, b[k]);
+        h = all_applied(f, b, count - k0, h);
     }
     return h;
 }
@@ -395,12 +508,62 @@ __device__ __forceinline__ A join_groups(const A (&fac)[TG][PLACES], A (&to)[TG]
     return h;
 }
 
+// Whether a thread's steps have to be walked, where factors f of its maps have left the range, or have
+// come back to it: by gates of a magnitude above 2.
+template <typename A, typename V, int C, int VEC>
+__device__ __forceinline__ bool any_walked(const Map<A> (&m)[VEC], const A (&f)[VEC], const V (&gs)[C]) {
+    auto low = m[0].lowest_bits();
+    A top = A(0);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const auto bits = m[e].lowest_bits();
+        low = bits < low ? bits : low;
+        top = greatest_magnitude(top, f[e]);
+    }
+    if (!Map<A>::small(low) && !__builtin_isinf(top)) return false;
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        odd = odd || __builtin_isinf(f[e]);
+#pragma unroll
+        for (int c = 0; c < C; ++c) odd = odd || A(gs[c][e]) > A(2) || A(gs[c][e]) < A(-2);
+    }
+    return odd;
+}
+
+// What a group's steps make of the states h at its places, and `starts` gets what they were.
+template <bool MIX, typename A, typename V, int C, int VEC>
+__device__ __forceinline__ void walk_group(const V (&gs)[C], const V (&xs)[C], A* h, A* starts) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        A v = h[e];
+        starts[e] = v;
+#pragma unroll
+        for (int c = 0; c < C; ++c) v = step<true, MIX>(A(gs[c][e]), A(xs[c][e]), v);
+        h[e] = v;
+    }
+}
+
+// And of the gradients behind it.
+template <typename A, typename V, int C, int VEC>
+__device__ __forceinline__ void walk_group_back(const V (&gs)[C], const V (&ds)[C], A* q, A* ends) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        A v = q[e];
+        ends[e] = v;
+#pragma unroll
+        for (int c = C - 1; c >= 0; --c) v = back_of<true>(A(gs[c][e]), A(ds[c][e]) + v);
+        q[e] = v;
+    }
+}
+
 // A forward's stretch may be STARTS of the backward's, and leaves a start for each.
 template <typename T, bool MIX, int FL, int TG, int C, int VEC, int STARTS, bool THROUGH = false>
-__global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
+__global__ __launch_bounds__(FL * TG, sizeof(T) == 2 && FL == 32 ? 4 : 1) void k_rows_forward(Args<T> a) {
     using A = wide_t<T>;
     using W = Tile<T, FL, TG, C, VEC>;
     __shared__ A fac[2][TG][W::PLACES], sum[2][TG][W::PLACES];
+    __shared__ int walks[2][W::NT / 64];  // a wave's steps of the stretch have to be
     const W w(a);
     if (!w.live) return;
     const int64_t s0 = w.segment * a.per_segment / STARTS;
@@ -433,17 +596,52 @@ __global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
         maps_of<MIX>(gs, xs, m);
         keep_packed(gs);
         keep_packed(xs);
+        A f[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            fac[buf][w.tg][w.fl * VEC + e] = m[e].factor();
+            f[e] = m[e].factor();
+            fac[buf][w.tg][w.fl * VEC + e] = f[e];
             sum[buf][w.tg][w.fl * VEC + e] = m[e].b;
         }
+        const bool walked = __any(any_walked(m, f, gs));
+        if (lane_id() == 0) walks[buf][wave_id()] = walked;
+        keep_packed(gs);
         __syncthreads();
+        int walk = 0;
+#pragma unroll
+        for (int i = 0; i < W::NT / 64; ++i) walk |= walks[buf][i];
+        walk = __builtin_amdgcn_readfirstlane(walk);
+        A begin[W::PER];
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
             const int p = threadIdx.x + k * W::NT;
-            if (p >= W::PLACES) continue;
-            carry[k] = join_groups<false>(fac[buf], sum[buf], p, carry[k]);
+            begin[k] = carry[k];
+            if (p < W::PLACES) carry[k] = join_groups<false>(fac[buf], sum[buf], p, carry[k]);
+        }
+        if (walk) {
+            __syncthreads();
+            A* const now = fac[buf][0];
+#pragma unroll
+            for (int k = 0; k < W::PER; ++k) {
+                const int p = threadIdx.x + k * W::NT;
+                if (p < W::PLACES) now[p] = begin[k];
+            }
+            for (int q = 0; q < TG; ++q) {
+                __syncthreads();
+                if (w.tg == q)
+                    walk_group<MIX, A, Few<T, VEC>, C, VEC>(gs, xs, now + w.fl * VEC,
+                                                            &sum[buf][q][w.fl * VEC]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < W::PER; ++k) {
+                const int p = threadIdx.x + k * W::NT;
+                if (p < W::PLACES) carry[k] = now[p];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < W::PER; ++k) {
+            const int p = threadIdx.x + k * W::NT;
             if (a.starts && w.scans(p, a.inner)) {
                 const int64_t i = w.place(p, a.inner);
 #pragma unroll
@@ -488,10 +686,11 @@ __global__ __launch_bounds__(FL * TG) void k_rows_forward(Args<T> a) {
 }
 
 template <typename T, bool MIX, int FL, int TG, int C, int VEC, bool THROUGH = false>
-__global__ __launch_bounds__(FL * TG) void k_rows_backward(Args<T> a) {
+__global__ __launch_bounds__(FL * TG, 2) void k_rows_backward(Args<T> a) {
     using A = wide_t<T>;
     using W = Tile<T, FL, TG, C, VEC>;
     __shared__ A fac[2][TG][W::PLACES], sum[2][TG][W::PLACES], back[2][TG][W::PLACES];
+    __shared__ int walks[2][W::NT / 64];  // as in the forward
     const W w(a);
     if (!w.live) return;
     const int64_t s0 = w.segment * a.per_segment;
@@ -553,21 +752,57 @@ __global__ __launch_bounds__(FL * TG) void k_rows_backward(Args<T> a) {
         backs_of(gs, ds, q);
         keep_packed(gs);
         keep_packed(ds);
+        A f[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-            fac[buf][w.tg][w.fl * VEC + e] = m[e].factor();
+            f[e] = m[e].factor();
+            fac[buf][w.tg][w.fl * VEC + e] = f[e];
             sum[buf][w.tg][w.fl * VEC + e] = m[e].b;
             back[buf][w.tg][w.fl * VEC + e] = q[e];
         }
+        const bool walked = __any(any_walked(m, f, gs));
+        if (lane_id() == 0) walks[buf][wave_id()] = walked;
+        keep_packed(gs);
         __syncthreads();
+        int walk = 0;
+#pragma unroll
+        for (int i = 0; i < W::NT / 64; ++i) walk |= walks[buf][i];
+        walk = __builtin_amdgcn_readfirstlane(walk);
+        A behind[W::PER];
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
             const int p = threadIdx.x + k * W::NT;
             if (p < W::PLACES) join_groups<false>(fac[buf], sum[buf], p, begin[k]);
             const int r = rev + k * W::NT;
+            behind[k] = carry[k];
             if (r < W::PLACES) carry[k] = join_groups<true>(fac[buf], back[buf], r, carry[k]);
         }
         __syncthreads();
+        if (walk) {
+            A* const now = fac[buf][0];
+            A* const later = fac[buf][1];
+#pragma unroll
+            for (int k = 0; k < W::PER; ++k) {
+                const int p = threadIdx.x + k * W::NT, r = rev + k * W::NT;
+                if (p < W::PLACES) now[p] = begin[k];
+                if (r < W::PLACES) later[r] = behind[k];
+            }
+            for (int q = 0; q < TG; ++q) {
+                __syncthreads();
+                if (w.tg == q)
+                    walk_group<MIX, A, Few<T, VEC>, C, VEC>(gs, xs, now + w.fl * VEC,
+                                                            &sum[buf][q][w.fl * VEC]);
+                if (w.tg == TG - 1 - q)
+                    walk_group_back<A, Few<T, VEC>, C, VEC>(gs, ds, later + w.fl * VEC,
+                                                            &back[buf][w.tg][w.fl * VEC]);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < W::PER; ++k) {
+                const int r = rev + k * W::NT;
+                if (r < W::PLACES) carry[k] = later[r];
+            }
+        }
         const int64_t t = s * W::STRETCH + w.tg * C;
         const int steps = w.writes ? int(std::min<int64_t>(C, a.time - t)) : 0;
         auto sweep = [&](auto exact) {
@@ -626,6 +861,7 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
     using W = Tile<T, FL, TG, 1, VEC>;
     constexpr int U = 8;
     __shared__ A fac[TG][W::PLACES], sum[TG][W::PLACES];
+    __shared__ int exp[TG][W::PLACES];
     const W w(a);
     if (!w.live) return;
     const int64_t t0 = w.segment * a.per_segment * stretch;
@@ -636,7 +872,8 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
     const Seq<const T>& in = BACK ? a.gy : a.x;
     const T* d = in.p + w.o * in.so + w.i;
     const bool some = !BACK || in.p;
-    Map<A> m[VEC];
+    A h[VEC] = {};
+    Product<A> f[VEC];
     Few<T, VEC> gs[U], ds[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) ds[u] = Few<T, VEC>::all(T(0));
@@ -661,35 +898,54 @@ __global__ __launch_bounds__(FL * TG) void k_rows_maps(Args<T> a, int stretch) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const A gate = A(gs[u][e]), v = A(ds[u][e]);
-                if constexpr (BACK) {
-                    m[e].b = back_of<true>(gate, v + m[e].b);
-                    m[e].factor_by(gate);
-                } else {
-                    m[e].template then<true, MIX>(gate, v);
-                }
+                if constexpr (BACK)
+                    h[e] = back_of<true>(gate, v + h[e]);
+                else
+                    h[e] = step<true, MIX>(gate, v, h[e]);
             }
+        }
+        by_steps(f, gs);
+        if ((n & 63) == 0) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e].even();
         }
     }
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        fac[w.tg][w.fl * VEC + e] = m[e].factor();
-        sum[w.tg][w.fl * VEC + e] = m[e].b;
+        f[e].plain();
+        fac[w.tg][w.fl * VEC + e] = f[e].m;
+        exp[w.tg][w.fl * VEC + e] = f[e].e;
+        sum[w.tg][w.fl * VEC + e] = h[e];
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < W::PER; ++k) {
         const int p = threadIdx.x + k * W::NT;
         if (!w.scans(p, a.inner)) continue;
-        A f = A(1), b = A(0);
-        for (int q = 0; q < TG; ++q) {
-            const int r = BACK ? TG - 1 - q : q;
-            b = apply(fac[r][p], b, sum[r][p]);
-            f = kept_product(f, fac[r][p]);
+        Product<A> all;
+        A b = A(0);
+        constexpr int N = 8;
+#pragma unroll
+        for (int q0 = 0; q0 < TG; q0 += N) {
+            Product<A> f[N];
+            A h[N];
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const int r = BACK ? TG - 1 - q0 - q : q0 + q;
+                f[q] = {fac[r][p], exp[r][p]};
+                h[q] = sum[r][p];
+            }
+            b = all_applied(f, h, N, b);
+#pragma unroll
+            for (int q = 0; q < N; ++q) all.by(mantissa(f[q].m), exponent(f[q].m) + f[q].e);
+            all.even();
         }
-        const int64_t n = a.outer * a.inner;
-        A* to = a.maps + 2 * w.segment * n + w.o * a.inner + w.place(p, a.inner);
-        to[0] = f;
+        all.plain();
+        const int64_t n = a.outer * a.inner, at = w.o * a.inner + w.place(p, a.inner);
+        A* to = a.maps + 2 * w.segment * n + at;
+        to[0] = all.m;
         to[n] = b;
+        a.exps[w.segment * n + at] = all.e;
     }
 }
 
@@ -868,6 +1124,61 @@ __device__ __forceinline__ A scan_lanes(A a, A b, A& carry) {
     return apply(pa, from, pb);
 }
 
+// The same where maps are not joined (MIX as in step; in: x, or the gradients of the outputs): from the
+// state, or the gradient, that the stretch starts with the lanes walk their steps one after the other.
+template <int L, bool MIX, bool BACK, typename A, typename V>
+__device__ __forceinline__ A walk_lanes(const V& g, const V& in, A& carry) {
+    constexpr int VEC = sizeof(V) / sizeof(g[0]);
+    const int l = lane_id() & (L - 1);
+    A h = carry, from = h;
+#pragma unroll 1
+    for (int k = 0; k < L; ++k) {
+        const int q = BACK ? L - 1 - k : k;
+        if (l == q) from = h;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if constexpr (BACK)
+                h = back_of<true>(A(g[VEC - 1 - e]), A(in[VEC - 1 - e]) + h);
+            else
+                h = step<true, MIX>(A(g[e]), A(in[e]), h);
+        }
+        h = __shfl(h, q, L);
+    }
+    carry = h;
+    return from;
+}
+
+// Whether the factor f of any lane's map is none, or none to be multiplied with others; the same in all
+// lanes.
+template <typename A, typename V>
+__device__ __forceinline__ bool lanes_walked(const Map<A>& m, A f, const V& g) {
+    constexpr int VEC = sizeof(V) / sizeof(g[0]);
+    bool odd = greatest_magnitude(A(0), f) > A(kGrowth);
+    if (Map<A>::small(m.lowest_bits())) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) odd = odd || A(g[e]) > A(2) || A(g[e]) < A(-2);
+    }
+    return __any(odd);
+}
+
+// A product by a lane's gates, as by_steps has it.
+template <typename A, typename V>
+__device__ __forceinline__ void by_gates(Product<A>& f, const V& g) {
+    constexpr int VEC = sizeof(V) / sizeof(g[0]);
+    A p = A(1), lowest = A(1);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        p *= A(g[e]);
+        lowest = least_magnitude(lowest, A(g[e]));
+    }
+    if (lowest >= A(kSmall) && finite(p)) {
+        f.by(p);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f.by(A(g[e]));
+    }
+}
+
 template <typename T, int L, bool BACK>
 struct Line {
     static constexpr int VEC = wide_vec<T>();
@@ -950,7 +1261,9 @@ __global__ __launch_bounds__(kThreads) void k_lines_forward(Args<T> a) {
         }
         Map<A> m;
         line_map<MIX>(gn, xn, m);
-        const A begin = scan_lanes<L, false>(m.factor(), m.b, carry);
+        const A f = m.factor();
+        const A begin = lanes_walked(m, f, gn) ? walk_lanes<L, MIX, false>(gn, xn, carry)
+                                            : scan_lanes<L, false>(f, m.b, carry);
         auto sweep = [&](auto exact) {
             typename Few<T, VEC>::Elements out;
             h = begin;
@@ -1021,8 +1334,9 @@ __global__ __launch_bounds__(kThreads) void k_lines_backward(Args<T> a) {
             for (int e = VEC - 1; e >= 0; --e) q = back_of<true>(A(gn[e]), A(dn[e]) + q);
         }
         const A f = m.factor();
-        const A h0 = scan_lanes<L, false>(f, m.b, begin);
-        const A c0 = scan_lanes<L, true>(f, q, carry);
+        const bool walk = lanes_walked(m, f, gn);
+        const A h0 = walk ? walk_lanes<L, MIX, false>(gn, xn, begin) : scan_lanes<L, false>(f, m.b, begin);
+        const A c0 = walk ? walk_lanes<L, MIX, true>(gn, dn, carry) : scan_lanes<L, true>(f, q, carry);
         auto sweep = [&](auto exact) {
             constexpr bool EXACT = decltype(exact)::value;
             A h = h0, before[VEC];
@@ -1072,7 +1386,8 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
         ds = load_part<T, VEC>(d + t, some ? count : 0, T(0));
     };
     load(0);
-    A f = A(1), b = A(0);
+    Product<A> f;
+    A b = A(0);
     for (int64_t k = 0; k < s1 - s0; ++k) {
         const Few<T, VEC> gn = gs, dn = ds;
         if (k + 1 < s1 - s0) load(k + 1);
@@ -1087,23 +1402,37 @@ __global__ __launch_bounds__(kThreads) void k_lines_maps(Args<T> a) {
             line_map<MIX>(gn, dn, m);
         }
         A fac = m.factor(), sum = m.b;
-        scan_step<64, BACK, 1>(fac, sum, w.l);
-        scan_step<64, BACK, 2>(fac, sum, w.l);
-        scan_step<64, BACK, 4>(fac, sum, w.l);
-        scan_step<64, BACK, 8>(fac, sum, w.l);
-        constexpr int ends[4] = {BACK ? 48 : 15, BACK ? 32 : 31, BACK ? 16 : 47, BACK ? 0 : 63};
+        if (lanes_walked(m, fac, gn)) {
+            walk_lanes<64, MIX, BACK>(gn, dn, b);
+        } else {
+            scan_step<64, BACK, 1>(fac, sum, w.l);
+            scan_step<64, BACK, 2>(fac, sum, w.l);
+            scan_step<64, BACK, 4>(fac, sum, w.l);
+            scan_step<64, BACK, 8>(fac, sum, w.l);
+            constexpr int ends[4] = {BACK ? 48 : 15, BACK ? 32 : 31, BACK ? 16 : 47, BACK ? 0 : 63};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const A fr = read_lane(fac, ends[r]);
-            b = apply(fr, b, read_lane(sum, ends[r]));
-            f = kept_product(f, fr);
+            for (int r = 0; r < 4; ++r)
+                b = apply(read_lane(fac, ends[r]), b, read_lane(sum, ends[r]));
         }
+        by_gates(f, gn);  // the lane's own steps of every stretch
+        f.even();
     }
+    // over the lanes: rows of 16, as wave_total goes, then the rows
+    f.by(dpp_move<0xB1>(f.m), dpp_move<0xB1>(f.e));
+    f.by(dpp_move<0x4E>(f.m), dpp_move<0x4E>(f.e));
+    f.by(dpp_move<0x124>(f.m), dpp_move<0x124>(f.e));
+    f.by(dpp_move<0x128>(f.m), dpp_move<0x128>(f.e));
+    const Product<A> one = f;
+    f = Product<A>();
+#pragma unroll
+    for (int r = 0; r < 64; r += 16) f.by(read_lane(one.m, r), read_lane(one.e, r));
+    f.plain();
     if (w.live && w.l == 0) {
         const int64_t n = a.outer * a.inner;
         A* to = a.maps + 2 * w.segment * n + w.row;
-        to[0] = f;
+        to[0] = f.m;
         to[n] = b;
+        a.exps[w.segment * n + w.row] = f.e;
     }
 }
 
@@ -1200,6 +1529,7 @@ int route_args(Args<T>& a, const Route& r, bool lines, void* workspace) {
     a.segments = r.segments;
     a.per_segment = r.per_segment;
     a.maps = r.segments > 1 ? static_cast<wide_t<T>*>(workspace) : nullptr;
+    a.exps = a.maps ? reinterpret_cast<int*>(a.maps + 2 * r.segments * a.outer * a.inner) : nullptr;
     if (r.stretches <= 1) a.starts = nullptr;
     a.groups = r.units * r.segments;
     CL_ARG(a.groups < (int64_t(1) << 31), "too many sequences for one call");
@@ -1374,7 +1704,7 @@ int sizes(int dtype, int order, int64_t batch, int64_t time, int64_t features, D
     r = route_of(dtype, d.lines, d.outer, d.time, d.inner);
     const int64_t n = batch * features;
     starts = r.stretches > 1 ? r.stretches * n : 0;
-    bytes = r.segments > 1 ? 2 * r.segments * n * (dtype == CL_DTYPE_F64 ? 8 : 4) : 0;
+    bytes = r.segments > 1 ? r.segments * n * (2 * (dtype == CL_DTYPE_F64 ? 8 : 4) + 4) : 0;
     return CL_OK;
 }
 

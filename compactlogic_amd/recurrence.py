@@ -30,7 +30,10 @@ def gated_recurrence(x, gate, state=None, form: str = "mix", return_state: bool 
 
     A gate of exactly 0 drops what came before, and one of exactly 1 leaves x unread in "mix": a
     sequence may begin anew inside of a row, or end before it, whatever the other steps hold, NaN
-    included (the gate's own gradient is the formula's there)."""
+    included (the gate's own gradient is the formula's there).  Gates may be of any magnitude, also where
+    a run of them multiplies past the largest number over states that are 0 or small.  Stretches of time
+    with such runs are walked, which takes longer (where times are contiguous, from gates on whose
+    product over 4 float32 or 8 16-bit steps is above 16)."""
     code = _FORMS.get(form)
     if code is None:
         raise ValueError(f"form must be one of {sorted(_FORMS)}, got {form!r}")

@@ -574,6 +574,9 @@ int cl_adam_clip_step(int dtype, int64_t num_tensors, void* const* params, void*
  * grad_last,  grad_x_t = (1 - g_t) G_t or G_t,  grad_gate_t = G_t (h_(t-1) - x_t) or G_t h_(t-1),
  * grad_state = c before the first step.  A gate of exactly 0 drops what came before (and what comes
  * back from behind), one of exactly 1 leaves x unread in the outputs of MIX, NaN and infinities too.
+ * Gates may be of any magnitude: a product of theirs that leaves the range of numbers does no harm to
+ * states and gradients that stay in it.  (What a long run of growing steps adds up from a state of 0 has
+ * to stay in it too, which differs only where its terms cancel.)
  *
  * x, gate, y and their gradients: dtype (F32, F64, F16, BF16), [batch, time, features] by strides
  * (elements: batch, time, features); state, last and theirs: fp32 (fp64 for F64), [batch, features]

@@ -478,3 +478,145 @@ def test_saved_tensors_may_move(device, layout):
     (got,) = torch.autograd.grad(one, b, gy)
     (wx, ex), (wg, eg), _ = R.backward(_np(g), _np(g), _np(h0), _np(gy), 0 * _np(gl), True)
     _close(got, wx + wg, ex + eg + np.abs(wx) + np.abs(wg), torch.float32)
+
+
+# A run of steps whose gates multiply past the type's largest number, in every kernel: few steps, one
+# stretch and several of either length, narrow rows, segments; 4 to 64 lanes, two stretches, segments.
+GROWING = [("features", (2, 8, 12)), ("features", (3, 16, 40)), ("features", (2, 90, 40)),
+           ("features", (2, 128, 70)), ("features", (2, 300, 9)), ("features", (512, 100, 6)),
+           ("features", (2, 300, 3)), ("features", (1, 3000, 12)), ("features", (1, 3000, 2)),
+           ("time_batch", (3, 15, 5)), ("time_features", (3, 31, 7)), ("time_batch", (3, 63, 7)),
+           ("time_features", (40, 127, 52)), ("time_batch", (40, 250, 52)), ("time_features", (40, 255, 52)),
+           ("time_batch", (3, 500, 4)), ("time_features", (2, 3000, 3))]
+
+
+def _near(got, want, units, dtype, out=None):
+    """_close, and no NaN (which no comparison of magnitudes finds)."""
+    assert np.isfinite(want).all() and torch.isfinite(got).all()
+    _close(got, want, units, dtype, out)
+
+
+def _growth(time, dtype, share):
+    """A gate whose product over `share` of the time passes the range of the arithmetic; at most what
+    the type holds."""
+    bits = 1030 if dtype == torch.float64 else 130
+    most = {torch.float16: 15.0, torch.float64: 300.0}.get(dtype, 100.0)
+    return float(2.0 ** min(most, np.ceil(32 * bits / (share * time)) / 32))
+
+
+@pytest.mark.parametrize("form", ["mix", "add"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_growing_gates_over_nothing(device, dtype, form):
+    """Steps of nothing, however large their gates' product: no state, no inputs up to the last three
+    steps, no gradients behind the first three."""
+    for layout, shape in GROWING:
+        print(layout, shape, flush=True)
+        b, s, f = shape
+        gate = torch.tensor(_growth(s, dtype, 0.9), dtype=torch.float64).to(dtype)
+        x, _, gy, _, gl = _inputs(shape, dtype, device, 12)
+        x[:, :-3] = 0
+        gy[:, 3:] = 0
+        gl.zero_()
+        x, gy = (t * 2.0**-10 for t in (x, gy))       # three steps of up to 2^100 each stay in the range
+        if float(gate) > 2.0**40:
+            x, gy = (t * float(gate)**-1 for t in (x, gy))
+        g = torch.full_like(x, float(gate))
+        nx, ng, ngy = (_np(t) for t in (x, g, gy))
+        none = np.zeros((b, f))
+        x, g, gy = (_lay(t, layout) for t in (x, g, gy))
+        x.requires_grad_(), g.requires_grad_()
+        y, last = cl.gated_recurrence(x, g, form=form, return_state=True)
+        h, eh = R.forward(nx, ng, none, form == "mix")
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        if dtype != torch.float16 or np.abs(h).max() < 6e4:
+            _near(y, h, eh, dtype)
+        _near(last, h[:, -1], eh[:, -1], dtype, wide)
+        gx, gg = torch.autograd.grad(y, (x, g), gy)
+        (wx, ex), (wg, eg), _ = R.backward(nx, ng, none, ngy, none, form == "mix")
+        if dtype != torch.float16 or np.abs(wx).max() < 6e4:
+            _near(gx, wx, ex, dtype)
+        if dtype != torch.float16 or np.abs(wg).max() < 6e4:
+            _near(gg, wg, eg, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+def test_growing_gates_from_a_small_state(device, dtype):
+    """A state next to the smallest numbers grows to a large one, and so does a gradient."""
+    low, growth = (-1000.0, 1900.0) if dtype == torch.float64 else (-110.0, 200.0)
+    for layout, shape in GROWING:
+        print(layout, shape, flush=True)
+        b, s, f = shape
+        gate = float(torch.tensor(2.0 ** (growth / s), dtype=torch.float64).to(dtype))
+        if not np.log2(gate) * s + low < (1000 if dtype == torch.float64 else 120):
+            continue                                  # (a type of few bits rounds the gate up)
+        x, _, gy, h0, gl = _inputs(shape, dtype, device, 13)
+        x, gy, h0, gl = (torch.zeros_like(x), torch.zeros_like(gy), h0 * 2.0**low, gl * 2.0**low)
+        g = torch.full_like(x, gate)
+        nx, ng, ngy, nh, ngl = (_np(t) for t in (x, g, gy, h0, gl))
+        x, g, gy = (_lay(t, layout) for t in (x, g, gy))
+        x.requires_grad_(), h0.requires_grad_()
+        y, last = cl.gated_recurrence(x, g, h0, form="add", return_state=True)
+        h, eh = R.forward(nx, ng, nh, False)
+        wide = torch.float64 if dtype == torch.float64 else torch.float32
+        _near(y, h, eh, dtype)
+        _near(last, h[:, -1], eh[:, -1], dtype, wide)
+        gx, gs = torch.autograd.grad((y, last), (x, h0), (gy, gl))
+        (wx, ex), _, (ws, es) = R.backward(nx, ng, nh, ngy, ngl, False)
+        _near(gx, wx, ex, dtype)
+        _near(gs, ws, es, dtype, wide)
+
+
+def test_gates_that_shrink_and_grow(device):
+    """Products below the smallest number that grow again, within a thread's steps and beyond them: what
+    is left of a large state is what a walk leaves."""
+    for layout, shape in GROWING:
+        b, s, f = shape
+        if s < 8:
+            continue
+        print(layout, shape, flush=True)
+        _, _, _, h0, gl = _inputs(shape, torch.float32, device, 14)
+        h0, gl = (t.sign() * 2.0**100 for t in (h0, gl))
+        x = torch.zeros(shape, device=device)
+        g = torch.ones_like(x)
+        g[:, 1:3] = 2.0**-80
+        g[:, 3:5] = 2.0**80                           # 2^100, 2^20, 2^-60, 2^20, 2^100
+        nx, ng, nh, ngl = (_np(t) for t in (x, g, h0, gl))
+        x, g = (_lay(t, layout) for t in (x, g))
+        x.requires_grad_()
+        y, last = cl.gated_recurrence(x, g, h0, form="add", return_state=True)
+        h, _ = R.forward(nx, ng, nh, False)
+        assert np.array_equal(_np(y), h) and np.array_equal(_np(last), h[:, -1])
+        (gx,) = torch.autograd.grad(last, x, gl)
+        with np.errstate(over="ignore"):              # (2^100 times 2^80 is infinite, and stays so)
+            c, want = ngl.astype(np.float32), np.empty_like(ng, np.float32)
+            for t in range(s - 1, -1, -1):
+                want[:, t], c = c, ng[:, t].astype(np.float32) * c
+        assert np.array_equal(_np(gx), want)
+
+
+def test_growth_past_the_range(device):
+    """What leaves the range is infinite, and a gate of 0 begins anew."""
+    for layout, shape in GROWING:
+        if shape[1] < 15:
+            continue
+        print(layout, shape, flush=True)
+        s = shape[1]
+        cut = s - s // 4
+        x = torch.ones(shape, device=device)
+        g = torch.full_like(x, 2.0 ** min(100.0, np.ceil(300 / cut * 8) / 8))
+        g[:, cut] = 0.0
+        g[:, cut + 1:] = 0.5
+        y = cl.gated_recurrence(_lay(x, layout), _lay(g, layout), form="add")
+        assert torch.isinf(y[:, cut - 1]).all() and (y[:, cut - 1] > 0).all()
+        k = torch.arange(s - cut, device=device, dtype=torch.float64)
+        want = (2 - 0.5**k)[None, :, None].expand(shape[0], s - cut, shape[2])
+        _near(y[:, cut:], _np(want), 64 * np.ones(want.shape), torch.float32)
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_results_are_finite(device, layout):
+    """NaN passes a comparison of magnitudes: none where inputs are finite."""
+    for i, shape in enumerate(SHAPES):
+        for dtype in (torch.float32, torch.bfloat16):
+            for t in _run_and_check(shape, dtype, device, layout, "mix", i)[1:]:
+                assert all(torch.isfinite(v).all() for v in (t if isinstance(t, tuple) else (t,)))
