@@ -645,8 +645,12 @@ std::pair<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& gate,
         return {x.clone(),
                 state ? state->clone() : at::zeros({x.size(0), x.size(2)}, x.options().dtype(wide))};
     const Tensor h0 = state.value_or(Tensor());
-    if (at::GradMode::is_enabled() &&
-        (x.requires_grad() || gate.requires_grad() || (h0.defined() && h0.requires_grad()))) {
+    // (a tensor with a tangent, which torch refuses there, need not require a gradient)
+    const auto traced = [](const Tensor& t) {
+        return t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) ||
+                               t._fw_grad(0).defined());
+    };
+    if (traced(x) || traced(gate) || traced(h0)) {
         variable_list r = Recurrence::apply(x, gate, state, form);
         return {r[0], r[1]};
     }

@@ -26,7 +26,8 @@ def gated_recurrence(x, gate, state=None, form: str = "mix", return_state: bool 
     x and gate: float32, float64, float16 or bfloat16.  Features or times may lie contiguous (a
     LogicLayer's output for batch * time samples has its times so, and the result lies alike); other
     layouts are copied.  States and arithmetic are float32 (float64), each result is rounded once.
-    Differentiable once by x, gate and state, through the outputs and the last state.
+    Differentiable once by x, gate and state, through the outputs and the last state; not in forward
+    mode, whose tangents are refused.
 
     A gate of exactly 0 drops what came before, and one of exactly 1 leaves x unread in "mix": a
     sequence may begin anew inside of a row, or end before it, whatever the other steps hold, NaN

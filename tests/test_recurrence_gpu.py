@@ -620,3 +620,16 @@ def test_results_are_finite(device, layout):
         for dtype in (torch.float32, torch.bfloat16):
             for t in _run_and_check(shape, dtype, device, layout, "mix", i)[1:]:
                 assert all(torch.isfinite(v).all() for v in (t if isinstance(t, tuple) else (t,)))
+
+
+def test_forward_mode_is_refused(device):
+    """Tangents are not dropped without a word, whichever argument has them."""
+    import torch.autograd.forward_ad as fw
+    x, g, _, h0, _ = _inputs((2, 6, 5), torch.float32, device, 15)
+    for k in range(3):
+        args = [x, g, h0]
+        with fw.dual_level():
+            args[k] = fw.make_dual(args[k], torch.ones_like(args[k]))
+            for on in (True, False):
+                with torch.set_grad_enabled(on), pytest.raises(RuntimeError, match="jvp"):
+                    cl.gated_recurrence(*args)
