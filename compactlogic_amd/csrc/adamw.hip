@@ -149,8 +149,9 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads<N> ts, double
 
 // ---- the update of one element.  m and v are rounded product by product, so that an 8-bit code does
 // not depend on what a compiler fuses; the quotient, which only p takes, by the hardware's square
-// root and reciprocal, each within a unit in the last place (fp32; a v below 2^-126 counts as 0
-// there).  The IEEE forms take some 20 instructions more of about 60.
+// root and reciprocal, each within a unit in the last place (fp32).  The IEEE forms take some 20
+// instructions more of about 60.  Both take a number below 2^-126 for 0, which would make a step of
+// m / 0 where eps is 0 or that small too: for a v below it, both sides of the division times 2^32.
 template <typename A>
 struct Coefs {
     A scale;  // of the gradient
@@ -158,8 +159,11 @@ struct Coefs {
 };
 
 __device__ __forceinline__ float quotient(float m, float v, const Coefs<float>& c) {
-    const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v), c.inv_root, c.eps);
-    return m * __builtin_amdgcn_rcpf(d);
+    const bool low = v < 0x1p-126f;
+    const float root = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v);
+    const float up = low ? 0x1p32f : 1.0f;
+    const float d = __builtin_fmaf(root, c.inv_root, c.eps * up);
+    return m * up * __builtin_amdgcn_rcpf(d);
 }
 __device__ __forceinline__ double quotient(double m, double v, const Coefs<double>& c) {
     return m / (sqrt(v) * c.inv_root + c.eps);

@@ -434,3 +434,36 @@ def test_trains_a_network(device):
         opt.step()
     assert all(torch.isfinite(p).all() and not torch.equal(p, q)
                for p, q in zip(model.parameters(), ref))
+
+
+@pytest.mark.parametrize("numel", [3, 2048, 5000])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_roots_of_the_smallest_moments(device, bits, numel):
+    """An exp_avg_sq below the smallest normal number has a root, also where eps is 0 or next to it."""
+    for eps in (0.0, 1e-21):
+        (p,) = _params([(numel,)], torch.float32, device)
+        # the square of a gradient, times 1 - beta2, from 2^-148 to 2^-120
+        e = torch.arange(numel, device=device) % 57
+        p.grad = torch.exp2(-72.5 + e / 4) * torch.where(e % 2 == 0, 1.0, -1.0)
+        opt = cl.FusedAdamW([p], lr=0.01, betas=(0.9, 0.5), eps=eps, weight_decay=0.0, max_norm=None,
+                            state_bits=bits)
+        for t in range(1, 4):
+            before, g = _np(p), _np(p.grad)
+            st = opt.state[p]
+            if t == 1:
+                m = v = np.zeros(numel)
+            elif bits == 32:
+                m, v = _np(st["exp_avg"]), _np(st["exp_avg_sq"])
+            else:                                     # (bfloat16 ends at 2^-133)
+                m, v = A.values(*(x.cpu().numpy() for x in (st["exp_avg"].view(torch.uint8), st["exp_avg_sq"],
+                                                            st["exponents"])))
+            opt.step()
+            assert torch.isfinite(p).all()
+            # (m and v in float32, where these numbers have few bits, are the formula's own)
+            m, v = (a.astype(np.float64) for a in A.step32(g, m, v, 1.0, (0.9, 0.5)))
+            assert v.min() > 0 and v.min() < 2.0**-126
+            d = np.sqrt(v) / np.sqrt(1 - 0.5**t) + eps
+            move = 0.01 / (1 - 0.9**t) * m / d
+            # constants, root, reciprocal and products as in the oracle's step, and p's own rounding
+            err = 14 * A.U * np.abs(move) + 3 * A.U * np.abs(before)
+            _check(_np(p), before - move, err, torch.float32)
