@@ -545,7 +545,7 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors<N> ts, const doub
     }
 }
 
-// What 8 bits hold, in bf16 (which holds it all), and 8 bits from fp32.  param: exp_avg, grad:
+// What 8 bits hold, in bf16 (which holds it all from 2^-130 on), and 8 bits from fp32.  param: exp_avg, grad:
 // exp_avg_sq as they are outside.
 template <bool WHOLE, bool THROUGH, int N>
 __device__ __forceinline__ void read_tile8(const Tensors<N>& ts, int k, const Place& at) {

@@ -318,7 +318,7 @@ class FusedAdamW(_OneCount):
     def moments(self, params=None):
         """(first, second): lists of the exponential averages of the gradient and of its square of
         `params` (default: every parameter that has them), in float32 (float64) where they are held
-        in 32 bits and in bfloat16, which holds all of their values, where in 8."""
+        in 32 bits, and in bfloat16, which holds all of their values from 2^-130 on, where in 8."""
         held = [(p, self.state[p]) for p, _ in self._params() if "exp_avg" in self.state.get(p, {})] \
             if params is None else [(p, self.state.get(p, {})) for p in params]
         first, second, small = [], [], []

@@ -636,8 +636,8 @@ int cl_recurrence_backward(int dtype, int order, int form, const void* x, const 
  * group: its hyper-parameters; at most 32 groups a call.  workspace: cl_adamw_workspace bytes, on
  * 8 bytes.  Sums have a fixed order: bitwise reproducible.
  *
- * cl_adamw_moments_read gives back what 8 bits hold, in bf16 (exactly), exp_avg to param and
- * exp_avg_sq to grad; cl_adamw_moments_write takes fp32 elements from param and grad into 8 bits
+ * cl_adamw_moments_read gives back what 8 bits hold, in bf16 (exactly from 2^-130 on; below it, bf16 has
+ * fewer bits, and none below 2^-134), exp_avg to param and exp_avg_sq to grad; cl_adamw_moments_write takes fp32 elements from param and grad into 8 bits
  * (an exp_avg_sq below 0 becomes NaN).  Both go by the tensors' other fields, dtype and group unread.
  * ----------------------------------------------------------------------------------------- */
 typedef struct {

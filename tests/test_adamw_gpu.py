@@ -467,3 +467,20 @@ def test_roots_of_the_smallest_moments(device, bits, numel):
             # constants, root, reciprocal and products as in the oracle's step, and p's own rounding
             err = 14 * A.U * np.abs(move) + 3 * A.U * np.abs(before)
             _check(_np(p), before - move, err, torch.float32)
+
+
+def test_smallest_moments_are_given_back(device):
+    """bfloat16 holds what 8 bits do from 2^-130 on, and rounds what is smaller."""
+    (p,) = _params([(600,)], torch.float32, device)
+    p.grad = torch.exp2(-75 + torch.arange(600, device=device) % 40 / 4.0)
+    opt = cl.FusedAdamW([p], betas=(0.9, 0.5), max_norm=None, state_bits=8)
+    opt.step()
+    st = opt.state[p]
+    held = A.values(*(x.cpu().numpy() for x in (st["exp_avg"].view(torch.uint8), st["exp_avg_sq"], st["exponents"])))
+    low = 0
+    for got, want in zip(opt.moments(), held):
+        got, keep = _np(got[0]), np.abs(want) >= 2.0**-130
+        low += int(np.sum(~keep & (want != 0)))
+        np.testing.assert_array_equal(got[keep], want[keep])
+        assert np.all(np.abs(got - want)[~keep] <= 2.0**-134)
+    assert low > 100
