@@ -484,3 +484,17 @@ def test_smallest_moments_are_given_back(device):
         np.testing.assert_array_equal(got[keep], want[keep])
         assert np.all(np.abs(got - want)[~keep] <= 2.0**-134)
     assert low > 100
+
+
+def test_a_norm_of_nan_scales_nothing(device):
+    """NaN stays in its own element; the others step as they would without the clipping."""
+    for bits in (32, 8):
+        (p,) = _params([(5000,)], torch.float32, device)
+        p.grad[17] = float("nan")
+        q = copy.deepcopy(p)
+        q.grad = p.grad.clone()
+        cl.FusedAdamW([p], max_norm=0.5, state_bits=bits).step()
+        cl.FusedAdamW([q], max_norm=None, state_bits=bits).step()
+        assert torch.isnan(p[17]) and int(torch.isnan(p).sum()) == 1
+        keep = torch.arange(5000, device=device) != 17
+        assert torch.equal(p[keep], q[keep])
