@@ -184,7 +184,8 @@ class FusedAdamW(_OneCount):
     the first step of a parameter, which makes its moments, cannot be captured.
 
     State dicts interchange with torch.optim.AdamW's (of float32 moments for parameters of any type)
-    and between 32 and 8 bits.  Tensors that are of the type and on the device already are taken as
+    and between 32 and 8 bits, and FusedAdam's are taken, with the weight_decay that the groups have.
+    Tensors that are of the type and on the device already are taken as
     they are, without a copy."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -215,10 +216,14 @@ class FusedAdamW(_OneCount):
     def load_state_dict(self, state_dict):
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
             raise RuntimeError("FusedAdamW has no amsgrad and no maximize")
-        bits = [g["state_bits"] for g in self.param_groups]
+        if any(k not in g for g in state_dict["param_groups"] for k in ("lr", "betas", "eps")):
+            raise RuntimeError("the state dict's groups have no lr, betas and eps: it is not one of Adam's")
+        before = [dict(g) for g in self.param_groups]
         super().load_state_dict(state_dict)
-        for group, n in zip(self.param_groups, bits):   # how moments are held stays as it was
-            group["state_bits"] = n
+        for group, old in zip(self.param_groups, before):
+            group["state_bits"] = old["state_bits"]     # how moments are held stays as it was
+            for key, value in old.items():              # (FusedAdam has no weight_decay)
+                group.setdefault(key, value)
         # torch has cast the moments to the parameters' types: take them as they were given
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         with torch.no_grad():

@@ -44,6 +44,21 @@ def test_state_dicts_of_other_algorithms_are_refused():
         cl.FusedAdamW([p]).load_state_dict(other.state_dict())
 
 
+def test_groups_without_a_decay_keep_theirs():
+    """FusedAdam's groups have none; those of other algorithms lack more."""
+    p, q = torch.nn.Parameter(torch.zeros(4)), torch.nn.Parameter(torch.zeros(3))
+    other = cl.FusedAdam([{"params": [p]}, {"params": [q]}], lr=0.25, betas=(0.5, 0.75), eps=1e-4)
+    opt = cl.FusedAdamW([{"params": [p], "weight_decay": 0.5}, {"params": [q], "state_bits": 8}], weight_decay=0.125)
+    opt.load_state_dict(other.state_dict())
+    for group, decay, bits in zip(opt.param_groups, (0.5, 0.125), (32, 8)):
+        assert set(group) >= {"params", "lr", "betas", "eps", "weight_decay", "state_bits"}
+        assert (group["lr"], tuple(group["betas"]), group["eps"]) == (0.25, (0.5, 0.75), 1e-4)
+        assert group["weight_decay"] == decay and group["state_bits"] == bits
+    assert opt.param_groups[0]["params"][0] is p
+    with pytest.raises(RuntimeError, match="betas"):
+        opt.load_state_dict(torch.optim.SGD([{"params": [p]}, {"params": [q]}], lr=0.1).state_dict())
+
+
 def test_copies_keep_their_settings():
     p = torch.nn.Parameter(torch.zeros(4))
     opt = cl.FusedAdamW([p], max_norm=3.0, state_bits=8)

@@ -498,3 +498,20 @@ def test_a_norm_of_nan_scales_nothing(device):
         assert torch.isnan(p[17]) and int(torch.isnan(p).sum()) == 1
         keep = torch.arange(5000, device=device) != 17
         assert torch.equal(p[keep], q[keep])
+
+
+def test_resumes_from_fused_adam(device):
+    """Its state dict, which has no weight_decay: the moments, the count and the settings go on."""
+    ps = _params([(300, 7), (513,)], torch.float32, device, seed=6)
+    adam = cl.FusedAdam(ps, lr=0.02, betas=(0.8, 0.95), eps=1e-6, max_norm=None)
+    adam.step()
+    adam.step()
+    held = [tuple(_np(adam.state[p][k]) for k in ("exp_avg", "exp_avg_sq")) for p in ps]
+    opt = cl.FusedAdamW(ps, max_norm=None, weight_decay=0.3)
+    opt.load_state_dict(copy.deepcopy(adam.state_dict()))
+    before = [_np(p) for p in ps]
+    opt.step()
+    for p, b, (m, v) in zip(ps, before, held):
+        (want, err), _, _ = A.step(b, _np(p.grad), m, v, 3, 1.0, 0.02, (0.8, 0.95), 1e-6, 0.3)
+        _check(_np(p), want, err, torch.float32)
+        assert float(opt.state[p]["step"]) == 3
