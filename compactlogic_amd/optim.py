@@ -97,6 +97,12 @@ class FusedAdam(_OneCount):
         self._step_t = None     # shared device step count
         self._workspace = None
 
+    def load_state_dict(self, state_dict):
+        if any("exponents" in st for st in state_dict["state"].values()):
+            raise RuntimeError("FusedAdam holds no moments in 8 bits; load them into a FusedAdamW with "
+                               "state_bits=32, and its state dict here")
+        super().load_state_dict(state_dict)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

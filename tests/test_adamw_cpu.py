@@ -59,6 +59,19 @@ def test_groups_without_a_decay_keep_theirs():
         opt.load_state_dict(torch.optim.SGD([{"params": [p]}, {"params": [q]}], lr=0.1).state_dict())
 
 
+def test_fused_adam_refuses_moments_in_8_bits():
+    """Their codes would be taken for values."""
+    p = torch.nn.Parameter(torch.zeros(4))
+    held = cl.FusedAdamW([p], state_bits=8).state_dict()
+    held["state"] = {0: {"exp_avg": torch.zeros(4, dtype=torch.uint8).view(torch.float8_e4m3fn),
+                         "exp_avg_sq": torch.full((4,), 200, dtype=torch.uint8),
+                         "exponents": torch.ones(2, dtype=torch.uint8), "step": torch.tensor(1.0)}}
+    opt = cl.FusedAdam([p])
+    with pytest.raises(RuntimeError, match="8 bits"):
+        opt.load_state_dict(held)
+    assert not opt.state
+
+
 def test_copies_keep_their_settings():
     p = torch.nn.Parameter(torch.zeros(4))
     opt = cl.FusedAdamW([p], max_norm=3.0, state_bits=8)
