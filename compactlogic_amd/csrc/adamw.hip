@@ -399,10 +399,9 @@ __device__ __forceinline__ void store_eight(T* p, const Eight<T>& r, int count) 
         if (e < count) p[e] = r.v[e];
 }
 
-// Eight elements of each half of a tile per thread, kHeld in 32 lanes; every lane takes part, those past
-// the tensor's end with a count of 0 (and zeros).  By halves, because a workgroup's loads are all under
-// way before its first computation.
-constexpr int kHalf = kOptThreads * 8, kHalves = kTile / kHalf;
+// Eight elements of a tile per thread, kHeld in 32 lanes; every lane takes part, those past the tensor's end
+// with a count of 0 (and zeros).
+static_assert(kTile == kOptThreads * 8);
 
 struct Place {
     int64_t at, left;   // first element, and the tensor's from there on
@@ -416,25 +415,21 @@ struct Place {
     // WHOLE: the tile lies inside of the tensor.  That is asked once, not at every access: where a whole
     // access and one by elements meet, the loads before them would be waited for.
     template <bool WHOLE>
-    __device__ __forceinline__ int count(int h) const {
-        if constexpr (WHOLE) return 8;
-        const int64_t n = left - h * kHalf;
-        return n >= 8 ? 8 : n > 0 ? int(n) : 0;
+    __device__ __forceinline__ int count() const {
+        return WHOLE || left >= 8 ? 8 : left > 0 ? int(left) : 0;
     }
     __device__ __forceinline__ bool whole() const { return left + threadIdx.x * 8 >= kTile; }
 };
 
-template <bool WHOLE>
-__device__ __forceinline__ Powers load_powers(const uint8_t* power, const Place& at, int h) {
-    if (at.count<WHOLE>(h) == 0) return {0, 0};
-    const uint8_t* p = power + at.block + h * (kHalf / kHeld);
+__device__ __forceinline__ Powers load_powers(const uint8_t* power, const Place& at, int count) {
+    if (count == 0) return {0, 0};
+    const uint8_t* p = power + at.block;
     return {int(p[0]) - 127, int(p[at.blocks]) - 127};
 }
 
-template <bool WHOLE>
-__device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, int h, const Powers& v) {
-    if (at.count<WHOLE>(h) > 0 && (threadIdx.x & 31) == 0) {
-        uint8_t* p = power + at.block + h * (kHalf / kHeld);
+__device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, int count, const Powers& v) {
+    if (count > 0 && (threadIdx.x & 31) == 0) {
+        uint8_t* p = power + at.block;
         p[0] = uint8_t(v.m + 127);
         p[at.blocks] = uint8_t(v.v + 127);
     }
@@ -449,34 +444,24 @@ __device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Pl
     const T* d = static_cast<const T*>(ts.grad[k]) + at.at;
     uint8_t* pm = static_cast<uint8_t*>(ts.m[k]) + at.at;
     uint8_t* pv = static_cast<uint8_t*>(ts.v[k]) + at.at;
-    Eight<T> w[kHalves], g[kHalves];
-    Codes held[kHalves];
-    Powers power[kHalves];
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        const int count = at.count<WHOLE>(h);
-        w[h] = load_eight(p + h * kHalf, count);
-        g[h] = load_eight(d + h * kHalf, count);
-        held[h] = {load_codes(pm + h * kHalf, count), load_codes(pv + h * kHalf, count)};
-        power[h] = load_powers<WHOLE>(ts.power[k], at, h);
-    }
+    const int count = at.count<WHOLE>();
+    Eight<T> w = load_eight(p, count);
+    const Eight<T> g = load_eight(d, count);
+    const Codes held{load_codes(pm, count), load_codes(pv, count)};
+    Powers power = load_powers(ts.power[k], at, count);
     const Coefs<float> c = load_coefs<float>(parts, nparts, max_norm, coefs, ts.group[k], red);
+    float m[8], v[8];
+    decode(held, power, m, v);
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        const int count = at.count<WHOLE>(h);
-        float m[8], v[8];
-        decode(held[h], power[h], m, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            moments_step(float(g[h].v[e]), m[e], v[e], c);
-            w[h].v[e] = T(param_step(float(w[h].v[e]), m[e], v[e], c));
-        }
-        const Codes next = encode(m, v, power[h]);
-        store_eight<THROUGH>(p + h * kHalf, w[h], count);
-        store_codes<THROUGH>(pm + h * kHalf, next.m, count);
-        store_codes<THROUGH>(pv + h * kHalf, next.v, count);
-        store_powers<WHOLE>(ts.power[k], at, h, power[h]);
+    for (int e = 0; e < 8; ++e) {
+        moments_step(float(g.v[e]), m[e], v[e], c);
+        w.v[e] = T(param_step(float(w.v[e]), m[e], v[e], c));
     }
+    const Codes next = encode(m, v, power);
+    store_eight<THROUGH>(p, w, count);
+    store_codes<THROUGH>(pm, next.m, count);
+    store_codes<THROUGH>(pv, next.v, count);
+    store_powers(ts.power[k], at, count, power);
 }
 
 template <typename T, int N, bool THROUGH>
@@ -549,31 +534,20 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw(Tensors<N> ts, const doub
 // exp_avg_sq as they are outside.
 template <bool WHOLE, bool THROUGH, int N>
 __device__ __forceinline__ void read_tile8(const Tensors<N>& ts, int k, const Place& at) {
-    Codes held[kHalves];
-    Powers power[kHalves];
+    const int count = at.count<WHOLE>();
+    const Codes held{load_codes(static_cast<uint8_t*>(ts.m[k]) + at.at, count),
+                     load_codes(static_cast<uint8_t*>(ts.v[k]) + at.at, count)};
+    const Powers power = load_powers(ts.power[k], at, count);
+    float m[8], v[8];
+    decode(held, power, m, v);
+    Eight<bf16_t> a, b;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        const int64_t i = at.at + h * kHalf;
-        const int count = at.count<WHOLE>(h);
-        held[h] = {load_codes(static_cast<uint8_t*>(ts.m[k]) + i, count),
-                   load_codes(static_cast<uint8_t*>(ts.v[k]) + i, count)};
-        power[h] = load_powers<WHOLE>(ts.power[k], at, h);
+    for (int e = 0; e < 8; ++e) {
+        a.v[e] = bf16_t(m[e]);
+        b.v[e] = bf16_t(v[e]);
     }
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        const int64_t i = at.at + h * kHalf;
-        const int count = at.count<WHOLE>(h);
-        float m[8], v[8];
-        decode(held[h], power[h], m, v);
-        Eight<bf16_t> a, b;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            a.v[e] = bf16_t(m[e]);
-            b.v[e] = bf16_t(v[e]);
-        }
-        store_eight<THROUGH>(static_cast<bf16_t*>(ts.param[k]) + i, a, count);
-        store_eight<THROUGH>(static_cast<bf16_t*>(ts.grad[k]) + i, b, count);
-    }
+    store_eight<THROUGH>(static_cast<bf16_t*>(ts.param[k]) + at.at, a, count);
+    store_eight<THROUGH>(static_cast<bf16_t*>(ts.grad[k]) + at.at, b, count);
 }
 
 template <int N, bool THROUGH>
@@ -590,24 +564,20 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8_read(Tensors<N> ts) {
 
 template <bool WHOLE, int N>
 __device__ __forceinline__ void write_tile8(const Tensors<N>& ts, int k, const Place& at) {
+    const int count = at.count<WHOLE>();
+    const Eight<float> a = load_eight(static_cast<const float*>(ts.param[k]) + at.at, count);
+    const Eight<float> b = load_eight(static_cast<const float*>(ts.grad[k]) + at.at, count);
+    float m[8], v[8];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        const int64_t i = at.at + h * kHalf;
-        const int count = at.count<WHOLE>(h);
-        const Eight<float> a = load_eight(static_cast<const float*>(ts.param[k]) + i, count);
-        const Eight<float> b = load_eight(static_cast<const float*>(ts.grad[k]) + i, count);
-        float m[8], v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m[e] = __builtin_isfinite(a.v[e]) ? a.v[e] : __builtin_nanf("");
-            v[e] = b.v[e] < 0.0f ? __builtin_nanf("") : b.v[e] + 0.0f;  // no -0
-        }
-        Powers power;
-        const Codes c = encode(m, v, power);
-        store_codes<false>(static_cast<uint8_t*>(ts.m[k]) + i, c.m, count);
-        store_codes<false>(static_cast<uint8_t*>(ts.v[k]) + i, c.v, count);
-        store_powers<WHOLE>(ts.power[k], at, h, power);
+    for (int e = 0; e < 8; ++e) {
+        m[e] = __builtin_isfinite(a.v[e]) ? a.v[e] : __builtin_nanf("");
+        v[e] = b.v[e] < 0.0f ? __builtin_nanf("") : b.v[e] + 0.0f;  // no -0
     }
+    Powers power;
+    const Codes c = encode(m, v, power);
+    store_codes<false>(static_cast<uint8_t*>(ts.m[k]) + at.at, c.m, count);
+    store_codes<false>(static_cast<uint8_t*>(ts.v[k]) + at.at, c.v, count);
+    store_powers(ts.power[k], at, count, power);
 }
 
 template <int N>
