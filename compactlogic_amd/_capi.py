@@ -193,7 +193,7 @@ class AdamWTensor(ctypes.Structure):
     """cl_adamw_tensor"""
     _fields_ = [("param", _p), ("grad", _p), ("exp_avg", _p), ("exp_avg_sq", _p), ("powers", _p),
                 ("numel", _i64), ("dtype", _i32), ("bits", _i32), ("group", _i32),
-                ("reserved", _i32)]
+                ("rounding", _i32)]
 
 
 class AdamWGroup(ctypes.Structure):

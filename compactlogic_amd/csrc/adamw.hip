@@ -21,6 +21,16 @@
 // is held as 0: the root of v divides, and an element whose v were lost under its neighbours' would
 // make a step of m / eps.
 //
+// An average that moves by less than half a step of its codes stays where it is when it is rounded to the
+// nearest, which is (1 - b2) |g^2 - v| < v / 18 falling (codes are up to 1/9 apart) and v / 16 rising:
+// with a b2 of 0.9 v stays within 2.25 times of where it belongs, above 17/18 it need not fall at all.
+// Rounded at random, up with the probability of its distance from the code below, it is
+// right on average (b2 = 0.999, gradients of one size: after 3000 steps the mean v is 0.02 of the true one
+// by the nearest and 1.00 at random, steps 4.8 and 1.00 times theirs).  The random numbers are a hash of
+// the step count, the tile and the element, by the finalizer of MurmurHash3 (Appleby), one word for the
+// 16 bits of m and of v each: 200 M bf16 391 us instead of 356 (with the norm 577, 468), 100 M fp32 287
+// as by the nearest.
+//
 // Bound by memory: 100 M fp32 elements 530 us without the norm (5.3 TB/s), 200 M bf16 with moments in 8
 // bits 356 (5.6; some 46 vector instructions an element, 59 % of what the VALU can do in that time); the
 // norm's pass 15 to 20 us per 76 MB.  Small tensors are the host's: two launches of 3.5 us each.
@@ -40,8 +50,16 @@ constexpr int kHeld = 256;         // elements of a block
 constexpr int kNormParts = 512;
 constexpr int kCoefs = 8;
 
-// A group's coefficients as the first kernel leaves them (fp64).
+// A group's coefficients as the first kernel leaves them (fp64), and behind those of all groups the step's
+// key to its random numbers.
 enum { kDecay, kSize, kInvRoot, kB1, kRest1, kB2, kRest2, kEps };
+constexpr int kCoefSpace = kGroups * kCoefs + 1;
+
+template <typename D>
+__device__ __forceinline__ auto random_key(D* coefs) {
+    using Word = std::conditional_t<std::is_const_v<D>, const uint32_t, uint32_t>;
+    return reinterpret_cast<Word*>(coefs + kGroups * kCoefs);
+}
 
 template <int N>
 struct Tensors {
@@ -54,6 +72,7 @@ struct Tensors {
     void* m[N];
     void* v[N];
     uint8_t* power[N];  // 8 bits: exponents + 127 of the blocks, m's and then v's
+    uint32_t number[N]; // of the tensor's first tile among all of the call
     uint8_t group[N];
 };
 
@@ -65,6 +84,13 @@ struct Grads {
     int64_t numel[N];
     const void* grad[N];
 };
+
+// x mixed: every bit of the result hangs on every bit of x.
+__device__ __forceinline__ uint32_t mixed(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x85EBCA6Bu;
+    x = (x ^ (x >> 13)) * 0xC2B2AE35u;
+    return x ^ (x >> 16);
+}
 
 struct Groups {
     int n;
@@ -114,7 +140,11 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw_begin(Grads<N> ts, double
             c[kRest2] = 1.0 - b2;
             c[kEps] = groups.eps[i];
         }
-        if (i == 0) step[0] = t;
+        if (i == 0) {
+            step[0] = t;
+            const uint64_t count = uint64_t(t);
+            *random_key(coefs) = mixed(uint32_t(count) ^ mixed(uint32_t(count >> 32) + 0x9E3779B9u));
+        }
     }
     if (ts.n == 0) return;
     double s = 0.0;
@@ -244,7 +274,13 @@ __device__ __forceinline__ float power_of_two(int k) { return __builtin_amdgcn_l
 // A code of what is not finite is NaN, whatever the block's other elements are.  An infinite m comes
 // with a v that is not finite (the exponential average of finite numbers does not overflow); a NaN
 // is left out of a maximum and is converted to one.
-__device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& power) {
+//
+// RANDOM: by the random words of elements `place` on under `key`, the lower half for m and the upper for v.
+// e4m3 has the same step below 2^-6, its smallest normal number, as above it: 2^-6 more, and the bits of
+// any number hold its code and 20 bits behind it.
+template <bool RANDOM>
+__device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& power, uint32_t key = 0,
+                                        uint32_t place = 0) {
     float top = 0.0f;
     uint32_t top_v = 0;
 #pragma unroll
@@ -287,12 +323,23 @@ __device__ __forceinline__ Codes encode(float (&m)[8], float (&v)[8], Powers& po
         float u[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) u[e] = m[4 * h + e] * to_m;
+        uint32_t word[4];
+        if constexpr (RANDOM) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                word[e] = mixed(key + (place + uint32_t(4 * h + e)) * 0x9E3779B9u);
+                const float size = __builtin_fabsf(u[e]), more = size < 0x1p-6f ? 0x1p-6f : 0.0f;
+                const uint32_t up = ((word[e] & 0xFFFFu) << 4) + 8;
+                u[e] = __builtin_copysignf(float_of((bits_of(size + more) + up) & 0xFFF00000u) - more, u[e]);
+            }
+        }
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], 0, false);
         pm[h] = uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], w, true));
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t b = bits_of(v[4 * h + e] * to_v);
-            const int r = int(b + (0x7FFFFu - (kFirstCode << 20)) + ((b >> 20) & 1)) >> 20;
+            const uint32_t up = RANDOM ? ((word[e] >> 16) << 4) + 8 : 0x7FFFFu + ((b >> 20) & 1);
+            const int r = int(b + up - (kFirstCode << 20)) >> 20;
             // the middle one of r, 1 and a number that is 0 for v = 0 (r is then below 0) and else not
             // below r, nor 0 where scaling lost v
             const int some = int(b | bits_of(v[4 * h + e]));
@@ -435,11 +482,11 @@ __device__ __forceinline__ void store_powers(uint8_t* power, const Place& at, in
     }
 }
 
-template <typename T, bool WHOLE, bool THROUGH, int N>
+template <typename T, bool WHOLE, bool THROUGH, bool RANDOM, int N>
 __device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Place& at,
                                            const double* __restrict__ parts, int nparts,
                                            double max_norm, const double* __restrict__ coefs,
-                                           double* red) {
+                                           double* red, uint32_t tile) {
     T* p = static_cast<T*>(ts.param[k]) + at.at;
     const T* d = static_cast<const T*>(ts.grad[k]) + at.at;
     uint8_t* pm = static_cast<uint8_t*>(ts.m[k]) + at.at;
@@ -449,6 +496,8 @@ __device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Pl
     const Eight<T> g = load_eight(d, count);
     const Codes held{load_codes(pm, count), load_codes(pv, count)};
     Powers power = load_powers(ts.power[k], at, count);
+    uint32_t key = 0;
+    if constexpr (RANDOM) key = mixed(ts.number[k] + tile + *random_key(coefs));
     const Coefs<float> c = load_coefs<float>(parts, nparts, max_norm, coefs, ts.group[k], red);
     float m[8], v[8];
     decode(held, power, m, v);
@@ -457,14 +506,14 @@ __device__ __forceinline__ void step_tile8(const Tensors<N>& ts, int k, const Pl
         moments_step(float(g.v[e]), m[e], v[e], c);
         w.v[e] = T(param_step(float(w.v[e]), m[e], v[e], c));
     }
-    const Codes next = encode(m, v, power);
+    const Codes next = encode<RANDOM>(m, v, power, key, threadIdx.x * 8);
     store_eight<THROUGH>(p, w, count);
     store_codes<THROUGH>(pm, next.m, count);
     store_codes<THROUGH>(pv, next.v, count);
     store_powers(ts.power[k], at, count, power);
 }
 
-template <typename T, int N, bool THROUGH>
+template <typename T, int N, bool THROUGH, bool RANDOM>
 __global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors<N> ts, const double* __restrict__ parts,
                                                         int nparts, double max_norm,
                                                         const double* __restrict__ coefs) {
@@ -472,11 +521,12 @@ __global__ __launch_bounds__(kOptThreads) void k_adamw8(Tensors<N> ts, const dou
     const uint32_t tile = uint32_t(group_index());
     if (tile >= ts.tiles) return;
     const int k = tensor_of(ts.first, tile);
-    const Place at(tile - ts.first[k], ts.numel[k]);
+    const uint32_t own = tile - ts.first[k];
+    const Place at(own, ts.numel[k]);
     if (at.whole())
-        step_tile8<T, true, THROUGH>(ts, k, at, parts, nparts, max_norm, coefs, red);
+        step_tile8<T, true, THROUGH, RANDOM>(ts, k, at, parts, nparts, max_norm, coefs, red, own);
     else
-        step_tile8<T, false, THROUGH>(ts, k, at, parts, nparts, max_norm, coefs, red);
+        step_tile8<T, false, THROUGH, RANDOM>(ts, k, at, parts, nparts, max_norm, coefs, red, own);
 }
 
 template <typename T, int N>
@@ -574,7 +624,7 @@ __device__ __forceinline__ void write_tile8(const Tensors<N>& ts, int k, const P
         v[e] = b.v[e] < 0.0f ? __builtin_nanf("") : b.v[e] + 0.0f;  // no -0
     }
     Powers power;
-    const Codes c = encode(m, v, power);
+    const Codes c = encode<false>(m, v, power);
     store_codes<false>(static_cast<uint8_t*>(ts.m[k]) + at.at, c.m, count);
     store_codes<false>(static_cast<uint8_t*>(ts.v[k]) + at.at, c.v, count);
     store_powers(ts.power[k], at, count, power);
@@ -597,8 +647,10 @@ struct Batch {
     int n = 0;
     int64_t tiles = 0;
     const cl_adamw_tensor* t[kTensors];
+    uint32_t number[kTensors];
 
-    void add(const cl_adamw_tensor& tensor) {
+    void add(const cl_adamw_tensor& tensor, int64_t first) {
+        number[n] = uint32_t(first);
         t[n++] = &tensor;
         tiles += ceil_div(tensor.numel, kTile);
     }
@@ -617,6 +669,7 @@ struct Batch {
             ts.m[i] = t[i]->exp_avg;
             ts.v[i] = t[i]->exp_avg_sq;
             ts.power[i] = t[i]->powers;
+            ts.number[i] = number[i];
             ts.group[i] = uint8_t(t[i]->group);
             ts.tiles += uint32_t(ceil_div(t[i]->numel, kTile));
         }
@@ -650,10 +703,10 @@ struct Batch {
         }                                  \
     } while (0)
 
-// What must be the same within a launch: the type of the gradients; that and the bits of the moments
-// (kinds from 4 on: 8 bits); nothing.
+// What must be the same within a launch: the type of the gradients; that, the bits of the moments (kinds
+// from 4 on: 8 bits) and how they are rounded (from 8 on: at random); nothing.
 enum class Alike { kDtype, kDtypeAndBits, kAll };
-constexpr int kKinds = 8;
+constexpr int kKinds = 12;
 
 // From so many bytes on what a call with moments in 8 bits writes goes past the 256 MiB cache, where it
 // would push out what the next one reads (37.8 M bf16 elements, each step followed by giving the moments
@@ -663,7 +716,8 @@ constexpr double kThrough = 96 << 20;
 
 int kind_of(const cl_adamw_tensor& t, Alike alike) {
     if (alike == Alike::kAll) return 0;
-    return t.dtype + (alike == Alike::kDtypeAndBits && t.bits == 8 ? 4 : 0);
+    if (alike == Alike::kDtype || t.bits != 8) return t.dtype;
+    return t.dtype + (t.rounding == CL_ADAMW_AT_RANDOM ? 8 : 4);
 }
 
 // Calls f(kind, batch) for the launches that the tensors make, kind by kind.
@@ -671,13 +725,15 @@ template <typename F>
 int each_batch(const cl_adamw_tensor* t, int64_t n, Alike alike, F&& f) {
     for (int kind = 0; kind < kKinds; ++kind) {
         Batch b;
-        for (int64_t i = 0; i < n; ++i) {
+        int64_t first = 0, next = 0;  // tiles of the tensors before this one, and with it
+        for (int64_t i = 0; i < n; ++i, first = next) {
+            next = first + ceil_div(t[i].numel, kTile);
             if (t[i].numel == 0 || kind_of(t[i], alike) != kind) continue;
             if (b.n == kTensors) {
                 if (int rc = f(kind, b)) return rc;
                 b = Batch();
             }
-            b.add(t[i]);
+            b.add(t[i], first);
         }
         if (b.n)
             if (int rc = f(kind, b)) return rc;
@@ -698,6 +754,8 @@ int check_tensor(const cl_adamw_tensor& t, int64_t i, int64_t num_groups, bool v
            "unsupported dtype code %d (expected F32, F64, F16 or BF16)", int(t.dtype));
     CL_ARG(t.bits == 32 || t.dtype != CL_DTYPE_F64, "fp64 parameters have no moments in 8 bits");
     CL_ARG(t.group >= 0 && t.group < num_groups, "no group %d", int(t.group));
+    CL_ARG(t.rounding == CL_ADAMW_NEAREST || t.rounding == CL_ADAMW_AT_RANDOM, "unknown rounding %d",
+           int(t.rounding));
     return CL_OK;
 }
 
@@ -722,7 +780,7 @@ extern "C" int cl_adamw_workspace(int64_t num_tensors, int64_t* bytes) {
     // coefficients, and the norm's sums: kNormParts, and at most kTensors more for each launch, of which
     // there are those that hold kTensors and one of each type
     const int64_t launches = std::min<int64_t>(num_tensors, num_tensors / kTensors + 4);
-    *bytes = 8 * (kGroups * kCoefs + kNormParts + kTensors * launches);
+    *bytes = 8 * (kCoefSpace + kNormParts + kTensors * launches);
     return CL_OK;
 }
 
@@ -765,7 +823,7 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
     const bool through = written >= kThrough;
     hipStream_t s = as_stream(stream);
     double* coefs = static_cast<double*>(workspace);
-    double* parts = coefs + kGroups * kCoefs;
+    double* parts = coefs + kCoefSpace;
     int64_t nparts = 0;
     bool begun = false;
     auto begin = [&](int kind, const Batch& b) -> int {
@@ -798,7 +856,8 @@ extern "C" int cl_adamw_step(int64_t num_tensors, const cl_adamw_tensor* tensors
                     k_adamw<scalar_t, N><<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts),
                                                                          max_norm, coefs);
                 } else if constexpr (!std::is_same_v<scalar_t, double>) {
-                    (through ? k_adamw8<scalar_t, N, true> : k_adamw8<scalar_t, N, false>)
+                    (kind < 8 ? through ? k_adamw8<scalar_t, N, true, false> : k_adamw8<scalar_t, N, false, false>
+                     : through ? k_adamw8<scalar_t, N, true, true> : k_adamw8<scalar_t, N, false, true>)
                         <<<b.grid(), kOptThreads, 0, s>>>(ts, parts, int(nparts), max_norm, coefs);
                 }
             });

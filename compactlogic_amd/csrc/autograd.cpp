@@ -770,6 +770,15 @@ bool moments_of(const Tensor& p, PyObject* state, int bits, cl_adamw_tensor& out
     return true;
 }
 
+// (A group from an older pickle has none.)
+int rounding_of(py::handle name) {
+    if (name.is_none()) return CL_ADAMW_NEAREST;
+    const auto text = py::cast<std::string>(name);
+    if (text == "nearest") return CL_ADAMW_NEAREST;
+    if (text != "random") refuse("rounds moments to the \"nearest\" or at \"random\", not by \"" + text + "\"");
+    return CL_ADAMW_AT_RANDOM;
+}
+
 // False, with nothing done, where a parameter with a gradient has no moments yet.
 bool adamw_step(const py::list& param_groups, const py::dict& states, const Tensor& step,
                 double max_norm) {
@@ -782,6 +791,7 @@ bool adamw_step(const py::list& param_groups, const py::dict& states, const Tens
     for (const py::handle group : param_groups) {
         const auto betas = py::cast<py::sequence>(item_of(group.ptr(), "betas"));
         const int bits = py::cast<int>(item_of(group.ptr(), "state_bits"));
+        const int rounding = rounding_of(item_of(group.ptr(), "rounding"));
         const int64_t first = int64_t(tensors.size());
         for (const py::handle item : py::cast<py::list>(item_of(group.ptr(), "params"))) {
             const Tensor& p = THPVariable_Unpack(item.ptr());
@@ -805,6 +815,7 @@ bool adamw_step(const py::list& param_groups, const py::dict& states, const Tens
             }
             t.dtype = code_of(p);
             t.group = int(groups.size());
+            t.rounding = rounding;
             tensors.push_back(t);
             stepped.push_back(p.unsafeGetTensorImpl());
         }

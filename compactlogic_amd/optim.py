@@ -25,6 +25,7 @@ loaded steps (which must agree), so the bias corrections continue where they sto
 from __future__ import annotations
 
 import ctypes
+import warnings
 
 import torch
 
@@ -181,7 +182,15 @@ class FusedAdamW(_OneCount):
     ``exp_avg_sq`` uint8 codes and the blocks' ``exponents``; `moments` gives their values.  The
     update itself takes the new moments before they are rounded to 8 bits.
 
-    lr, betas, eps, weight_decay and state_bits may differ between parameter groups (at most 32);
+    rounding="random" rounds them up or down so that they are right on average, by a hash of the step
+    count, the parameter's place among those that have a gradient, and the element: a run gives the same
+    bits again.  rounding="nearest" is for betas up to 0.9 alone, and warns above: a step that changes a
+    moment by less than half of its codes' distance (1/32 to 1/16 of it) does not change it at all.  With a
+    beta of 0.9 a moment then stays within 2.25 times of where it belongs.  With
+    beta2 = 0.999 exp_avg_sq then stays where the first steps took it: 0.02 of what it should be after 3000
+    steps of constant gradients, or a hundred times too much once gradients shrink tenfold.
+
+    lr, betas, eps, weight_decay, state_bits and rounding may differ between parameter groups (at most 32);
     ``max_norm`` is one for all, on the norm over all of them (float64 sums in a fixed order: steps
     are bitwise reproducible); None or <= 0 skips the clipping.  The gradients are left as they are:
     unlike clip_grad_norm_ and FusedAdam, ``p.grad`` is not scaled.  An infinite norm scales finite
@@ -195,9 +204,10 @@ class FusedAdamW(_OneCount):
     they are, without a copy."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 0.01, max_norm: float | None = 10.0, state_bits: int = 32):
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
-                                      weight_decay=weight_decay, state_bits=state_bits))
+                 weight_decay: float = 0.01, max_norm: float | None = 10.0, state_bits: int = 32,
+                 rounding: str = "nearest"):
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay,
+                                      state_bits=state_bits, rounding=rounding))
         self.max_norm = max_norm
 
     def __getstate__(self):
@@ -217,7 +227,13 @@ class FusedAdamW(_OneCount):
                              f"eps={g['eps']} weight_decay={g['weight_decay']}")
         if g["state_bits"] not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {g['state_bits']}")
+        if g["rounding"] not in ("nearest", "random"):
+            raise ValueError(f"rounding must be 'nearest' or 'random', got {g['rounding']!r}")
         super().add_param_group(param_group)
+        if g["state_bits"] == 8 and g["rounding"] == "nearest" and max(b1, b2) > 0.9:
+            warnings.warn("FusedAdamW: 8-bit moments rounded to the nearest stay where they are under "
+                          f"betas above 0.9, got {tuple(g['betas'])}: pass rounding=\"random\"",
+                          stacklevel=4)
 
     def load_state_dict(self, state_dict):
         if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
@@ -228,6 +244,7 @@ class FusedAdamW(_OneCount):
         super().load_state_dict(state_dict)
         for group, old in zip(self.param_groups, before):
             group["state_bits"] = old["state_bits"]     # how moments are held stays as it was
+            group["rounding"] = old["rounding"]
             for key, value in old.items():              # (FusedAdam has no weight_decay)
                 group.setdefault(key, value)
         # torch has cast the moments to the parameters' types: take them as they were given

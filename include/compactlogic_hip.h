@@ -632,14 +632,23 @@ int cl_recurrence_backward(int dtype, int order, int form, const void* x, const 
  * in e4m3 (OCP), the block's largest in [128, 256) times its power of two; exp_avg_sq as code c = 0
  * for 0, 255 for NaN, else the fp32 number of bits (c + 770) << 20, the block's largest in [1, 2)
  * times its power of two; exponents are at least -126, what is above 0 is at least code 1, what is
- * not finite is NaN and does not count for its block.  Codes are rounded to nearest, ties to even.
+ * not finite is NaN and does not count for its block.  Codes are rounded as rounding says:
+ *   CL_ADAMW_NEAREST    to nearest, ties to even.  A change of less than half a code's step (1/32 to 1/16)
+ *                       is lost at every step: moments stay where they are unless betas are small (0.9)
+ *   CL_ADAMW_AT_RANDOM  up with the probability of the distance to the code below, so that moments are
+ *                       right on average, by 16 bits each of a hash of t, the tensors before this one in
+ *                       the call (their tiles of 2048 elements) and the element's place
  * group: its hyper-parameters; at most 32 groups a call.  workspace: cl_adamw_workspace bytes, on
  * 8 bytes.  Sums have a fixed order: bitwise reproducible.
  *
  * cl_adamw_moments_read gives back what 8 bits hold, in bf16 (exactly from 2^-130 on; below it, bf16 has
  * fewer bits, and none below 2^-134), exp_avg to param and exp_avg_sq to grad; cl_adamw_moments_write takes fp32 elements from param and grad into 8 bits
- * (an exp_avg_sq below 0 becomes NaN).  Both go by the tensors' other fields, dtype and group unread.
+ * to the nearest (an exp_avg_sq below 0 becomes NaN).  Both go by the tensors' other fields; dtype, group
+ * and rounding are not read.
  * ----------------------------------------------------------------------------------------- */
+#define CL_ADAMW_NEAREST 0
+#define CL_ADAMW_AT_RANDOM 1
+
 typedef struct {
     void* param;
     void* grad;
@@ -650,7 +659,7 @@ typedef struct {
     int32_t dtype;
     int32_t bits;
     int32_t group;
-    int32_t reserved;
+    int32_t rounding;
 } cl_adamw_tensor;
 
 typedef struct {

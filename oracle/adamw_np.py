@@ -75,18 +75,56 @@ def _e5m3():
     return np.concatenate([[0.0], (1 + (c & 7) / 8) * 2.0**((c >> 3) - 127.0)])
 
 
-def hold(m, v):
-    """(codes of m, codes of v, exponents + 127) as 8 bits hold them."""
+def _mixed(x):
+    """The finalizer of MurmurHash3 (Appleby) of 32-bit numbers."""
+    x = np.asarray(x, np.uint32)
+    with np.errstate(over="ignore"):
+        x = (x ^ (x >> np.uint32(16))) * np.uint32(0x85EBCA6B)
+        x = (x ^ (x >> np.uint32(13))) * np.uint32(0xC2B2AE35)
+    return x ^ (x >> np.uint32(16))
+
+
+def words(t, n, first_tile=0):
+    """The random words of step number t for the n elements of a tensor whose first tile of 2048 elements
+    is number first_tile of the call."""
+    key = _mixed(np.uint32(int(t) & 0xFFFFFFFF) ^ _mixed(np.uint32((int(t) >> 32) + 0x9E3779B9)))
+    i = np.arange(n, dtype=np.uint64)
+    tile, at = (i // 2048 + first_tile).astype(np.uint32), (i % 2048).astype(np.uint32)
+    with np.errstate(over="ignore"):
+        return _mixed(_mixed(tile + key) + at * np.uint32(0x9E3779B9))
+
+
+def _at_random(u, values, fraction):
+    """The place of u in the sorted values, of its two neighbours the upper one where the fraction of the
+    way that is left to it is at most `fraction`."""
+    lo = np.clip(np.searchsorted(values, u, side="right") - 1, 0, len(values) - 2)
+    way = (u - values[lo]) / (values[lo + 1] - values[lo])
+    # the kernel's 20 bits of it
+    return lo + (np.floor(way * 2.0**20) / 2.0**20 + fraction >= 1)
+
+
+def hold(m, v, random=None):
+    """(codes of m, codes of v, exponents + 127) as 8 bits hold them: the nearest, or by random words of
+    32 bits for each element, m by the lower half and v by the upper."""
     n = np.asarray(m).size
+    if random is not None:
+        random = np.concatenate([random, np.zeros(-n % 256, np.uint32)]).reshape(-1, 256)
+        rm, rv = (((r & np.uint32(0xFFFF)) * 16.0 + 8) / 2.0**20 for r in (random, random >> np.uint32(16)))
+        # (below 2^-6, the type's smallest normal number, the kernel's sum with it is rounded to float32)
+        small = lambda u: np.where(u < 2.0**-6, (u + 2.0**-6).astype(np.float32).astype(np.float64) - 2.0**-6, u)
+        place_m = lambda u: _at_random(small(u), _e4m3(), rm)
+        place_v = lambda u: _at_random(u, _e5m3(), rv)
+    else:
+        place_m, place_v = (lambda u: _nearest(u, _e4m3())), (lambda u: _nearest(u, _e5m3()))
     bm, bv = _blocks(m), _blocks(v)
     km, kv = _exponents(bm, 7), _exponents(bv, 0)
     with np.errstate(invalid="ignore"):
         um, uv = bm * 2.0**-km, bv * 2.0**-kv
-        cm = _nearest(np.abs(np.where(np.isfinite(um), um, 0)), _e4m3())
+        cm = place_m(np.abs(np.where(np.isfinite(um), um, 0)))
         cm = np.where(np.signbit(um), cm | 0x80, cm)
         cm = np.where(np.isfinite(bm), cm, cm | 0x7F)
         fv = np.where(np.isfinite(uv), uv, 0)
-        cv = np.where(fv > 0, np.maximum(_nearest(fv, _e5m3()), 1), 0)
+        cv = np.where(fv > 0, np.maximum(place_v(fv), 1), 0)
         cv = np.where(np.isfinite(bv), cv, 255)
     powers = np.concatenate([km[:, 0], kv[:, 0]]) + 127
     return cm.reshape(-1)[:n].astype(np.uint8), cv.reshape(-1)[:n].astype(np.uint8), \

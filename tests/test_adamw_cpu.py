@@ -2,6 +2,7 @@
 import copy
 import ctypes
 import pickle
+import warnings
 
 import numpy as np
 import pytest
@@ -72,6 +73,113 @@ def test_fused_adam_refuses_moments_in_8_bits():
     assert not opt.state
 
 
+def test_rounding_is_checked_and_warned_of():
+    p = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match="rounding"):
+        cl.FusedAdamW([p], rounding="up")
+    for betas, bits, rounding, warned in (((0.9, 0.999), 8, "nearest", True), ((0.95, 0.9), 8, "nearest", True),
+                                          ((0.9, 0.9), 8, "nearest", False), ((0.9, 0.999), 8, "random", False),
+                                          ((0.9, 0.999), 32, "nearest", False)):
+        with warnings.catch_warnings(record=True) as seen:
+            warnings.simplefilter("always")
+            opt = cl.FusedAdamW([torch.nn.Parameter(torch.zeros(1))], betas=betas, state_bits=bits, rounding=rounding)
+        assert [("betas above 0.9" in str(w.message)) for w in seen] == [True] * warned
+        assert opt.param_groups[0]["rounding"] == rounding
+    other = cl.FusedAdamW([p], state_bits=8, rounding="random")
+    other.load_state_dict(cl.FusedAdamW([p], lr=0.5).state_dict())
+    assert other.param_groups[0]["rounding"] == "random" and other.param_groups[0]["lr"] == 0.5
+
+
+def _run_held(betas, gradient, steps, n, at_random):
+    """Moments held in 8 bits over `steps`, the same in float64, and the sizes of the last updates."""
+    m = v = np.zeros(n)
+    fm, fv = np.zeros(n), np.zeros(n)
+    for t in range(1, steps + 1):
+        g = gradient(t)
+        m1, v1 = A.step32(g, m, v, 1.0, betas)
+        fm, fv = betas[0] * fm + (1 - betas[0]) * g, betas[1] * fv + (1 - betas[1]) * g.astype(np.float64)**2
+        m, v = A.values(*A.hold(m1, v1, A.words(t, n) if at_random else None))
+    sizes = [np.mean(np.abs(a) / (np.sqrt(b) + 1e-12)) for a, b in ((m1, v1), (fm, fv))]
+    return m, v, fm, fv, sizes[0] / sizes[1]
+
+
+def _trajectories():
+    r = np.random.default_rng(3)
+    n = 2048
+    flat = (np.where(r.random(n) < 0.5, -1, 1) * r.uniform(0.5, 2, n)).astype(np.float32)
+    noise = r.standard_normal((64, n)).astype(np.float32)
+    at = lambda t: np.roll(noise[t % 64], t)
+    return n, {"flat": ((0.9, 0.999), lambda t: flat, 2500), "noise": ((0.9, 0.999), at, 2500),
+               "shrinks": ((0.9, 0.98), lambda t: at(t) * np.float32(1 if t < 400 else 0.1), 1200)}
+
+
+@pytest.mark.parametrize("name", ["flat", "noise", "shrinks"])
+def test_rounded_at_random_moments_follow(name):
+    """Thousands of steps.  A held value's rounding has mean 0 and a variance of at most (what the step
+    changes) x (the codes' distance, 1/8 of v): for v at most (1 - b2)(g^2 + v) v / 8, which sums up with
+    weights b2^2k to v^2 / 8 at most (E g^2 = v), for |m| at most m E|g| / 8 + m^2 / 8 likewise, below a
+    fourth of the mean g^2.  A mean over 2048 elements is within 6 deviations, 6 sqrt(1/4 / 2048) = 0.07.
+    The root's mean is off by 3/8 of v's relative variance more, 0.05."""
+    n, runs = _trajectories()
+    betas, gradient, steps = runs[name]
+    m, v, fm, fv, sizes = _run_held(betas, gradient, steps, n, True)
+    assert abs(v.mean() / fv.mean() - 1) < 0.07
+    scale = np.sqrt(fv.mean())
+    assert abs(np.mean((m - fm) * np.sign(fm)) / scale) < 0.07
+    assert abs(sizes - 1) < 0.12
+
+
+def test_rounded_to_the_nearest_moments_stay():
+    """What the warning is about: exp_avg_sq next to its first steps' values, or those before gradients
+    shrank.  With betas of 0.9 it follows: it moves where (1 - b2) |g^2 - v| is above v / 16 (rising, codes
+    up to 1/8 apart) or v / 18 (falling, 1/9), which leaves g^2 / 1.625 to g^2 / (1 - 10/18)."""
+    n, runs = _trajectories()
+    betas, gradient, steps = runs["flat"]
+    _, v, _, fv, sizes = _run_held(betas, gradient, steps, n, False)
+    assert v.mean() < 0.1 * fv.mean() and sizes > 3
+    betas, gradient, steps = runs["shrinks"]
+    _, v, _, fv, sizes = _run_held(betas, gradient, steps, n, False)
+    assert v.mean() > 50 * fv.mean() and sizes < 0.2
+    for name in ("flat", "shrinks"):
+        _, gradient, steps = runs[name]
+        _, v, _, fv, _ = _run_held((0.9, 0.9), gradient, steps, n, False)
+        assert 1 / 1.625 < v.mean() / fv.mean() < 2.25
+
+
+def test_random_words_and_codes():
+    """Uniform words, and codes that are one of a value's two neighbours, up as often as their distance
+    says, itself where it is one; NaN, 0 and the smallest as by the nearest."""
+    w = A.words(7, 1 << 16, 3)
+    halves = np.concatenate([w & 0xFFFF, w >> np.uint32(16)]) / 65536.0
+    assert abs(halves.mean() - 0.5) < 6 * np.sqrt(1 / 12 / len(halves))
+    assert abs(np.corrcoef(w & 0xFFFF, w >> np.uint32(16))[0, 1]) < 6 / np.sqrt(len(w))
+    assert not np.array_equal(w, A.words(8, 1 << 16, 3)) and np.array_equal(w[2048:], A.words(7, (1 << 16) - 2048, 4))
+    n = 1 << 14
+    m, v = np.full(n, 1.03, np.float32), np.full(n, 1.03, np.float32)
+    m[::256] = v[::256] = 1.0                # (a code itself: 128 and 1 with their blocks' powers)
+    got_m, got_v = A.values(*A.hold(m, v, A.words(1, n)))
+    for got in (got_m, got_v):
+        assert np.all(got[::256] == 1.0)
+        rest = np.delete(got, np.arange(0, n, 256))
+        assert set(np.unique(rest)) == {1.0, 1.125}
+        p = 0.03 / 0.125
+        assert abs(np.mean(rest == 1.125) - p) < 6 * np.sqrt(p * (1 - p) / len(rest))
+    small = np.full(512, 2.0**-12, np.float32)      # held as 2^-5 and 1/8 of it apart
+    small[0] = 1.0
+    small[1:256] += np.float32(2.0**-18)
+    cm, _, powers = A.hold(small, small, A.words(2, 512))
+    got = A.values(cm, np.zeros(512, np.uint8), powers)[0]
+    assert set(np.unique(got[1:256])) == {2.0**-12, 2.0**-12 + 2.0**-15} and np.all(got[256:] == 2.0**-12)
+    small[1:256] = np.float32(2.0**-15 + 2.0**-18)  # below the normal codes of m, where they are 2^-16 apart
+    cm, _, powers = A.hold(small, small, A.words(2, 512))
+    got = A.values(cm, np.zeros(512, np.uint8), powers)[0]
+    assert set(np.unique(got[1:256])) == {2.0**-15, 2.0**-15 + 2.0**-16}
+    odd = np.zeros(256, np.float32)
+    odd[:4] = np.nan, 0.0, 1e-30, 1.0
+    cm, cv, _ = A.hold(odd, odd, A.words(3, 256))
+    assert (cm[0] & 127, cv[0], cm[1], cv[1], cv[2]) == (127, 255, 0, 0, 1)
+
+
 def test_copies_keep_their_settings():
     p = torch.nn.Parameter(torch.zeros(4))
     opt = cl.FusedAdamW([p], max_norm=3.0, state_bits=8)
@@ -108,6 +216,14 @@ def test_c_arguments_are_checked_before_the_device():
         assert getattr(lib, name)(1, ctypes.addressof(t), None) == bad   # 32 bits
         assert getattr(lib, name)(-1, None, None) == bad and getattr(lib, name)(1, None, None) == bad
         assert getattr(lib, name)(0, None, None) == _capi.CL_OK
+
+
+def test_unknown_rounding_is_refused_by_the_library():
+    lib = _capi.load()
+    t = _capi.AdamWTensor(16, 16, 16, 16, 16, 10, 0, 8, 0, 2)
+    g = _capi.AdamWGroup(1e-3, 0.9, 0.999, 1e-8, 0.0)
+    assert lib.cl_adamw_step(1, ctypes.addressof(t), 1, ctypes.addressof(g), 0.0, 8, 8, 1 << 20, None) \
+        == _capi.CL_ERR_INVALID_ARGUMENT and b"rounding" in lib.cl_last_error()
 
 
 def test_oracle_holds_its_own_values():

@@ -515,3 +515,111 @@ def test_resumes_from_fused_adam(device):
         (want, err), _, _ = A.step(b, _np(p.grad), m, v, 3, 1.0, 0.02, (0.8, 0.95), 1e-6, 0.3)
         _check(_np(p), want, err, torch.float32)
         assert float(opt.state[p]["step"]) == 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_rounding_at_random(device, dtype):
+    """Codes as the random words of the step, the tensors before and the element have them; parameters as
+    with the moments before they are rounded."""
+    params = _params(SHAPES, dtype, device, seed=3, offset=1)
+    with torch.no_grad():
+        params[8].grad[300:600] *= 1e-6
+        params[9].grad[:20] = 0
+    wide, small = params[:3], params[3:]
+    betas, lr, eps, decay = (0.9, 0.999), 0.01, 1e-8, 0.1
+    opt = cl.FusedAdamW([{"params": wide}, {"params": small, "state_bits": 8}], lr=lr, betas=betas, eps=eps,
+                        weight_decay=decay, max_norm=0.5, rounding="random")
+    tiles = [-(-p.numel() // 2048) for p in params]
+    held = [(np.zeros(p.shape), np.zeros(p.shape)) for p in small]
+    for t in range(1, 5):
+        scale = A.scale_of([_np(p.grad) for p in params], 0.5)
+        before = [_np(p) for p in small]
+        opt.step()
+        for i, p in enumerate(small):
+            g, (m, v) = _np(p.grad), held[i]
+            (wp, ep), _, _ = A.step(before[i], g, m, v, t, scale, lr, betas, eps, decay)
+            _check(_np(p), wp, ep, dtype)
+            words = A.words(t, p.numel(), sum(tiles[:3 + i]))
+            codes = A.hold(*A.step32(g, m, v, scale, betas), words)
+            st = opt.state[p]
+            for name, want in zip(("exp_avg", "exp_avg_sq", "exponents"), codes):
+                np.testing.assert_array_equal(st[name].view(torch.uint8).cpu().numpy().reshape(-1), want)
+            m, v = A.values(*codes)
+            held[i] = m.reshape(p.shape), v.reshape(p.shape)
+        for p in params:
+            p.grad = (p.grad * (-0.7 if t % 2 else 3.0)).to(dtype)
+
+
+def test_extremes_rounded_at_random(device):
+    p = torch.nn.Parameter(torch.zeros(1024, device=device))
+    r = np.random.default_rng(1)
+    g = r.standard_normal(1024).astype(np.float32)
+    g[5], g[9], g[300] = np.inf, np.nan, -np.inf
+    g[512:768] = 2.0**-149
+    g[768:] = 1e19
+    g[800], g[801] = 1e-19, 0
+    p.grad = torch.tensor(g, device=device)
+    opt = cl.FusedAdamW([p], betas=(0.9, 0.99), max_norm=None, state_bits=8, rounding="random")
+    opt.step()
+    with np.errstate(over="ignore", invalid="ignore"):
+        cm, cv, powers = A.hold(*A.step32(g, np.zeros(1024), np.zeros(1024), 1.0, (0.9, 0.99)), A.words(1, 1024))
+    st = opt.state[p]
+    got = st["exp_avg"].view(torch.uint8).cpu().numpy()
+    nan = np.array([5, 9, 300])
+    assert np.all((got[nan] & 0x7F) == 0x7F)
+    keep = np.setdiff1d(np.arange(1024), nan)
+    np.testing.assert_array_equal(got[keep], cm[keep])
+    np.testing.assert_array_equal(st["exp_avg_sq"].cpu().numpy(), cv)
+    np.testing.assert_array_equal(st["exponents"].cpu().numpy(), powers)
+
+
+def test_random_rounding_in_a_graph(device):
+    """Each replay draws its own step's numbers, those of an eager step."""
+    eager, graphed = (_params([(5000,), (33, 9)], torch.bfloat16, device) for _ in range(2))
+    oe, og = (cl.FusedAdamW(ps, lr=0.01, max_norm=0.3, state_bits=8, rounding="random") for ps in (eager, graphed))
+    oe.step()
+    og.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        og.step()
+    drawn = []
+    for _ in range(4):
+        oe.step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(eager, graphed):
+            assert torch.equal(p, q)
+        for x, y in zip(oe.moments(), og.moments()):
+            assert all(torch.equal(s, t) for s, t in zip(x, y))
+        drawn.append(og.state[graphed[0]]["exp_avg_sq"].clone())
+    assert not any(torch.equal(a, b) for a, b in zip(drawn, drawn[1:]))
+
+
+@pytest.mark.parametrize("name", ["flat", "shrinks"])
+def test_thousands_of_steps_in_8_bits(device, name):
+    """Moments and updates next to those of float64.  A held value's relative variance is at most 1/4 (what
+    a step changes, times 1/8 of v between codes, summed up), so a mean over 65536 elements is within 6
+    deviations, 6 sqrt(1/4 / 65536) = 0.012 (m relative to the root of v); the root's mean is off by 3/8 of
+    the variance more."""
+    n = 65536
+    gen = torch.Generator().manual_seed(8)
+    beta2, steps = (0.999, 2500) if name == "flat" else (0.98, 1200)
+    sign = torch.randn(n, generator=gen).sign()
+    flat = (sign * (0.5 + 1.5 * torch.rand(n, generator=gen))).to(device)
+    noise = torch.randn(16, n, generator=gen).to(device)
+    p = torch.nn.Parameter(torch.zeros(n, device=device))
+    opt = cl.FusedAdamW([p], lr=1.0, betas=(0.9, beta2), eps=1e-12, weight_decay=0.0, max_norm=None,
+                        state_bits=8, rounding="random")
+    fm = fv = torch.zeros(n, dtype=torch.float64, device=device)
+    for t in range(1, steps + 1):
+        p.grad = flat if name == "flat" else noise[t % 16] * (1.0 if t < 400 else 0.1)
+        fm, fv = 0.9 * fm + 0.1 * p.grad.double(), beta2 * fv + (1 - beta2) * p.grad.double()**2
+        if t == steps:
+            p.data.zero_()
+        opt.step()
+    m, v = (x[0].double() for x in opt.moments())
+    assert abs(float(v.mean() / fv.mean()) - 1) < 0.012
+    assert abs(float(((m - fm) * fm.sign()).mean() / fv.mean().sqrt())) < 0.012
+    want = fm / (1 - 0.9**steps) / (fv / (1 - beta2**steps)).sqrt()
+    assert abs(float(p.abs().mean().double() / want.abs().mean()) - 1) < 0.012 + 3 / 8 / 4
