@@ -141,25 +141,39 @@ struct Product {
     }
 };
 
+// |v| as a whole number, less one: 0 is above all others, and not among the small ones.
+__device__ __forceinline__ uint32_t size_bits(float v) {
+    return __builtin_bit_cast(uint32_t, __builtin_fabsf(v)) - 1;
+}
+__device__ __forceinline__ uint64_t size_bits(double v) {
+    return __builtin_bit_cast(uint64_t, __builtin_fabs(v)) - 1;
+}
+
 // Each product of f by the gates of N <= 8 steps at its place, at once where they are neither small nor
 // infinite, nor NaN.
 template <int N, int VEC, typename A, typename V>
 __device__ __forceinline__ void by_steps(Product<A> (&f)[VEC], const V (&gs)[N]) {
     static_assert(N <= 8);
-    A p[VEC], lowest = A(1), rest = A(0);
+    A p[VEC], rest = A(0);
+    auto low = size_bits(A(0));
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
+        A lowest = A(1);
         p[e] = A(1);
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             p[e] *= A(gs[k][e]);
             lowest = least_magnitude(lowest, A(gs[k][e]));
         }
-        rest = fma(p[e], A(0), rest);
+        low = std::min(low, size_bits(lowest));
+        rest = fma(p[e], A(0), fma(f[e].m, A(0), rest));
     }
-    if (lowest >= A(kSmall) && rest == A(0)) {
+    if (low >= size_bits(A(kSmall)) && rest == A(0)) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e].by(p[e]);
+        for (int e = 0; e < VEC; ++e) {
+            f[e].m *= mantissa(p[e]);
+            f[e].e += exponent(p[e]);
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
@@ -205,12 +219,8 @@ struct Map {
         return lowest == A(0) ? A(0) : a == A(0) ? least(a) : a;
     }
     // Of a factor that has not left the range a product on the way may have, below it, if one of the
-    // gates was small.  (As whole numbers, so that 0 is none of them in the same comparison.)
-    using Bits = std::conditional_t<sizeof(A) == 4, uint32_t, uint64_t>;
-    __device__ __forceinline__ Bits lowest_bits() const { return __builtin_bit_cast(Bits, lowest) - 1; }
-    static __device__ __forceinline__ bool small(Bits lowest) {
-        return lowest < __builtin_bit_cast(Bits, A(kSmall)) - 1;
-    }
+    // gates was small.
+    __device__ __forceinline__ bool small() const { return size_bits(lowest) < size_bits(A(kSmall)); }
 };
 
 // From where on a lane's factor is not multiplied with its neighbours': sixteen of this one are 2^64, and
@@ -512,15 +522,14 @@ __device__ __forceinline__ A join_groups(const A (&fac)[TG][PLACES], A (&to)[TG]
 // come back to it: by gates of a magnitude above 2.
 template <typename A, typename V, int C, int VEC>
 __device__ __forceinline__ bool any_walked(const Map<A> (&m)[VEC], const A (&f)[VEC], const V (&gs)[C]) {
-    auto low = m[0].lowest_bits();
+    auto low = size_bits(A(0));
     A top = A(0);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-        const auto bits = m[e].lowest_bits();
-        low = bits < low ? bits : low;
+        low = std::min(low, size_bits(m[e].lowest));
         top = greatest_magnitude(top, f[e]);
     }
-    if (!Map<A>::small(low) && !__builtin_isinf(top)) return false;
+    if (low >= size_bits(A(kSmall)) && !__builtin_isinf(top)) return false;
     bool odd = false;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -607,10 +616,6 @@ __global__ __launch_bounds__(FL * TG, sizeof(T) == 2 && FL == 32 ? 4 : 1) void k
         if (lane_id() == 0) walks[buf][wave_id()] = walked;
         keep_packed(gs);
         __syncthreads();
-        int walk = 0;
-#pragma unroll
-        for (int i = 0; i < W::NT / 64; ++i) walk |= walks[buf][i];
-        walk = __builtin_amdgcn_readfirstlane(walk);
         A begin[W::PER];
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
@@ -618,6 +623,10 @@ __global__ __launch_bounds__(FL * TG, sizeof(T) == 2 && FL == 32 ? 4 : 1) void k
             begin[k] = carry[k];
             if (p < W::PLACES) carry[k] = join_groups<false>(fac[buf], sum[buf], p, carry[k]);
         }
+        int walk = 0;
+#pragma unroll
+        for (int i = 0; i < W::NT / 64; ++i) walk |= walks[buf][i];
+        walk = __builtin_amdgcn_readfirstlane(walk);
         if (walk) {
             __syncthreads();
             A* const now = fac[buf][0];
@@ -764,10 +773,6 @@ __global__ __launch_bounds__(FL * TG, 2) void k_rows_backward(Args<T> a) {
         if (lane_id() == 0) walks[buf][wave_id()] = walked;
         keep_packed(gs);
         __syncthreads();
-        int walk = 0;
-#pragma unroll
-        for (int i = 0; i < W::NT / 64; ++i) walk |= walks[buf][i];
-        walk = __builtin_amdgcn_readfirstlane(walk);
         A behind[W::PER];
 #pragma unroll
         for (int k = 0; k < W::PER; ++k) {
@@ -777,6 +782,10 @@ __global__ __launch_bounds__(FL * TG, 2) void k_rows_backward(Args<T> a) {
             behind[k] = carry[k];
             if (r < W::PLACES) carry[k] = join_groups<true>(fac[buf], back[buf], r, carry[k]);
         }
+        int walk = 0;
+#pragma unroll
+        for (int i = 0; i < W::NT / 64; ++i) walk |= walks[buf][i];
+        walk = __builtin_amdgcn_readfirstlane(walk);
         __syncthreads();
         if (walk) {
             A* const now = fac[buf][0];
@@ -1154,7 +1163,7 @@ template <typename A, typename V>
 __device__ __forceinline__ bool lanes_walked(const Map<A>& m, A f, const V& g) {
     constexpr int VEC = sizeof(V) / sizeof(g[0]);
     bool odd = greatest_magnitude(A(0), f) > A(kGrowth);
-    if (Map<A>::small(m.lowest_bits())) {
+    if (m.small()) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) odd = odd || A(g[e]) > A(2) || A(g[e]) < A(-2);
     }
