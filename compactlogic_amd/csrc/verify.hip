@@ -6,9 +6,10 @@
 // p_i, by the last number r: the first j whose sum of weights up to j is above r times their sum.  What
 // comes out is distributed as the target's own tokens are, whatever the draft was.
 //
-// The tests take a maximum and a sum in fp32 over each row, as the losses do.  The draw takes a sum in
-// fp64 of exponentials in fp64, of one row of each: next to some 10^5 borders between tokens, fp32 sums
-// would draw a neighbour once in 10^3 draws, as their order goes.
+// The tests take a maximum and a sum in fp32 (fp64 for fp64) over each row, as the losses do: a number
+// within some 10^-7 of its border is tested as the order of the sums goes.  The draw takes a sum in fp64 of
+// exponentials in fp64, of one row of each: next to some 10^5 borders between tokens, fp32 sums would draw
+// a neighbour once in 10^3 draws.
 //
 //   k_small    one workgroup a sequence does it all, for rows of at most kSmall elements
 // else
@@ -17,9 +18,11 @@
 //   k_sums     the fp64 sums of a chunk, kChunk elements, of the two rows
 //   k_weights  the sum of max(p - q, 0) of its chunk
 //   k_pick     the chunk that the number falls into, and the place in it
-// Chunks are short because k_pick takes one by one workgroup, bound by its exponentials (8192 elements
-// of two rows took 11 us).  256 sequences of 4 drafts of 10: 9 us, latency.  64 of 5 of 50021 bf16:
-// statistics 16 us (4.4 TB/s), sums, weights and place 9 to 10 each (the exponentials), tests 4.5.
+// Chunks are short because k_pick takes one by one workgroup (8192 elements of two rows took 11 us).  256
+// sequences of 4 drafts of 10: 9 us, latency.  64 of 5 of 50021 bf16: statistics 16 us (4.4 TB/s), sums,
+// weights and place 9 to 10 each, tests 4.5.  These four are latency too, of launches that wait for one
+// another and of each one's loads, scans and exponentials in a row: VALU 28 % busy in sums and weights, 2 %
+// in the tests and the place.
 #include "row_loss.h"
 #include "storage.h"
 
@@ -279,8 +282,9 @@ __device__ __forceinline__ double group_scan(double v, double* red, double& tota
 }
 
 // exp of x <= 0 within some 2^-52, without the cases of the library's (30 instructions to 20):
-// 2^n exp(r), n the integer next to x log2 e, exp(r) by its series to r^13 / 13! (|r| < 0.35: what is
-// left out is below 2^-60).
+// 2^n exp(r), n the integer next to x log2 e, ln 2 in two parts as fdlibm's exp has them (after Cody and
+// Waite: the first one times n is exact), exp(r) by its series to r^13 / 13!.  |r| < 0.35: what is left out,
+// r^14 / 14! and on, is below 2^-57, and of exp(r) >= 0.7 below 2^-56; the last roundings are the rest.
 __device__ __forceinline__ double exp_below(double x) {
     x = x < -800.0 ? -800.0 : x;  // (0; NaN stays)
     const double n = __builtin_rint(x * 1.4426950408889634);

@@ -31,7 +31,8 @@ def verify_drafts(logits, draft_tokens, draft_logits, uniforms, ignore_index: in
     tokens, the drawn one and ignore_index behind it; how many were accepted; the target's
     log-probabilities of the tokens, 0 behind them (float32; float64 for float64 logits).  Where the
     target's logits hold NaN or +inf, or nothing but -inf, no token is drawn: ignore_index, with a
-    log-probability of NaN.  Not differentiable.  The draw's sums are float64."""
+    log-probability of NaN.  Not differentiable.  The draw's sums are float64; the tests' are float32
+    (float64 for float64 logits), so that a number within some 1e-7 of its border may go either way."""
     for t, name in ((logits, "logits"), (draft_tokens, "draft_tokens"), (uniforms, "uniforms")):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")

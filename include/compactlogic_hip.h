@@ -775,7 +775,8 @@ int cl_group_sum_chosen_backward(int dtype, const void* scores, int64_t batch, i
  * tokens [sequences, drafts + 1]: these, then ignore_index; accepted [sequences]: how many were;
  * log_probs [sequences, drafts + 1] (fp32, fp64 for F64): the target's, then 0.  Where p is no
  * probability (NaN, infinite logits, none above -infinity) no token is drawn: ignore_index and NaN.
- * The draw's sums are in fp64.  workspace: cl_verify_drafts_workspace bytes, on 16 bytes. */
+ * The draw's sums are in fp64, the tests' in fp32 (fp64 for F64).  workspace: cl_verify_drafts_workspace
+ * bytes, on 16 bytes. */
 int cl_verify_drafts_workspace(int dtype, int64_t sequences, int64_t drafts, int64_t cols,
                                int64_t* bytes);
 int cl_verify_drafts(int dtype, const void* logits, int64_t seq_stride, int64_t row_stride,
