@@ -32,8 +32,7 @@
 // as by the nearest.
 //
 // Bound by memory: 100 M fp32 elements 530 us without the norm (5.3 TB/s), 200 M bf16 with moments in 8
-// bits 356 (5.6; some 46 vector instructions an element, 59 % of what the VALU can do in that time); the
-// norm's pass 15 to 20 us per 76 MB.  Small tensors are the host's: two launches of 3.5 us each.
+// bits 356 (5.6; with 77 % of what the VALU can do in that time); the norm's pass 15 to 20 us per 76 MB.  Small tensors are the host's: two launches of 3.5 us each.
 #include "storage.h"
 
 #include <algorithm>

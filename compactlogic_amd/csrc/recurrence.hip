@@ -342,7 +342,7 @@ __device__ __forceinline__ int64_t neighbour_index(int64_t groups) {
 // FL lanes side by side, of VEC places, TG groups of C steps each one after the other: a stretch is
 // TG * C steps.  Long sequences take 16 lanes (128 bytes of 16-bit elements; 64 bytes were slower, 128
 // and 106 us became 99 and 88) and 32 groups of 8 steps, or of 4 in the backward, whose 8 spill: 8 x
-// 4096 x 2048 bf16 84 us forward (4.8 TB/s) and 128 backward (5.2), VALU 22 and 31 % busy; what is
+// 4096 x 2048 bf16 88 us forward (4.6 TB/s) and 130 backward (5.2), VALU 22 and 32 % busy; what is
 // missing to 6.2 is the latency of a stretch with one workgroup a CU.  The groups' maps go through LDS; one thread per inner place scans them.  While a
 // stretch is worked on, the loads of the next one are under way.
 //
@@ -1055,8 +1055,9 @@ constexpr int64_t kFew = 8;
 //
 // L lanes of 16 bytes of one sequence one after the other: a stretch is L * VEC steps, scanned across
 // the lanes; 64 lanes for long sequences (32 for some), which go through their stretches one by one,
-// 4 to 32 where one stretch of those is enough.  Bound by memory: 64 x 64 x 12000 fp32 105 us forward (5.6 TB/s) and
-// 167 backward (5.9), VALU 60 % busy.
+// 4 to 32 where one stretch of those is enough.  Bound by memory: 64 x 64 x 12000 fp32 109 us forward (5.4 TB/s) and
+// 170 backward (5.8), VALU 69 and 66 % busy; 64 x 129 x 12000 bf16, half of whose lanes have no steps, 241
+// and 388, VALU 99 and 93 %.
 
 // The value k lanes before (after: BACK) in the 16 lanes of a DPP row, `none` where there is none.
 template <bool BACK, int K, typename A>
@@ -1482,10 +1483,10 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
         // As few lanes a sequence as hold it; where 32 do not, 32 with two stretches, of 16-bit values
         // three, or 64.  With 64 one stretch has no next one whose loads cover its scan, and many lanes
         // have no steps: 64 x T x 12000, 32 lanes against 64, forward / backward in us:
-        //   fp32 T 129  310 / 444  411 / 516      bf16 T 300  352 / 658  516 / 918
-        //   fp32 T 200  346 / 588  411 / 524      bf16 T 500  456 / 775  557 / 1009
-        //   fp32 T 300  500 / 991  602 / 838      bf16 T 600  564 / 934  700 / 1172
-        //   fp32 T 500  933 / 1656 787 / 1427     bf16 T 1000 x 2000  159 / 286  147 / 246
+        //   fp32 T 129  271 / 429  367 / 522      bf16 T 300  360 / 686  461 / 940
+        //   fp32 T 200  323 / 575  380 / 566      bf16 T 500  468 / 794  499 / 1030
+        //   fp32 T 300  516 / 976  565 / 872      bf16 T 600  570 / 945  659 / 1220
+        //   fp32 T 500  985 / 1640 793 / 1411     bf16 T 1000 x 2000  164 / 286  140 / 246
         // Few sequences take 64, and one stretch rather than two.
         int way = kLines4, l = 4;
         while (l < 32 && l * vec < time) l *= 2, ++way;
@@ -1503,9 +1504,9 @@ Route route_of(int dtype, bool lines, int64_t outer, int64_t time, int64_t inner
         // 32 lanes side by side and 8 groups (4) of 4 steps, whose workgroups are small and fill the chip
         // without a long time, or 16 and 32 (a forward: of 8), whose stretches are fewer.  Measured,
         // the first against the second, forward / backward in us:
-        //   256 x 64 x 1000 fp16   19 / 32   32 / 77      256 x 96 x 1000 fp32   48 / 102   76 / 121
-        //   64 x 64 x 12000 fp32  112 / 193 192 / 295     256 x 256 x 1000 fp16  71 / 152   92 / 188
-        //   64 x 1000 x 1024 fp32 153 / 260 150 / 252     16 x 4000 x 2048 fp16 256 / 270  178 / 270
+        //   256 x 64 x 1000 fp16   20 / 34   32 / 75      256 x 96 x 1000 fp32   48 / 102   59 / 115
+        //   64 x 64 x 12000 fp32  109 / 193 126 / 282     256 x 256 x 1000 fp16  73 / 155   95 / 196
+        //   64 x 1000 x 1024 fp32 148 / 260 152 / 260     16 x 4000 x 2048 fp16 183 / 270  165 / 275
         // (The first is never cut into segments: up to 96 steps or with 512 workgroups.)
         const int64_t broad = ceil_div(inner, 32 * places);
         if (inner < places) {
