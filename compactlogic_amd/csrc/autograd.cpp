@@ -770,9 +770,7 @@ bool moments_of(const Tensor& p, PyObject* state, int bits, cl_adamw_tensor& out
     return true;
 }
 
-// (A group from an older pickle has none.)
 int rounding_of(py::handle name) {
-    if (name.is_none()) return CL_ADAMW_NEAREST;
     const auto text = py::cast<std::string>(name);
     if (text == "nearest") return CL_ADAMW_NEAREST;
     if (text != "random") refuse("rounds moments to the \"nearest\" or at \"random\", not by \"" + text + "\"");

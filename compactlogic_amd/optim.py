@@ -213,6 +213,12 @@ class FusedAdamW(_OneCount):
     def __getstate__(self):
         return {**super().__getstate__(), "max_norm": self.max_norm}
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:         # (pickled before there was a choice)
+            group.setdefault("rounding", "nearest")
+        self.defaults.setdefault("rounding", "nearest")
+
     def add_param_group(self, param_group):
         params = param_group["params"]
         if not isinstance(params, torch.Tensor):

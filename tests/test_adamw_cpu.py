@@ -187,6 +187,17 @@ def test_copies_keep_their_settings():
         assert other.max_norm == 3.0 and other.param_groups[0]["state_bits"] == 8
 
 
+def test_pickles_without_a_rounding_go_on():
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = cl.FusedAdamW([p])
+    del opt.param_groups[0]["rounding"], opt.defaults["rounding"]
+    old = pickle.loads(pickle.dumps(opt))
+    assert old.param_groups[0]["rounding"] == "nearest"
+    old.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2))]})
+    old.load_state_dict(old.state_dict())
+    assert [g["rounding"] for g in old.param_groups] == ["nearest"] * 2
+
+
 def test_c_arguments_are_checked_before_the_device():
     lib = _capi.load()
     bad = _capi.CL_ERR_INVALID_ARGUMENT
