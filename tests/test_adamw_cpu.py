@@ -235,6 +235,7 @@ def test_unknown_rounding_is_refused_by_the_library():
     g = _capi.AdamWGroup(1e-3, 0.9, 0.999, 1e-8, 0.0)
     assert lib.cl_adamw_step(1, ctypes.addressof(t), 1, ctypes.addressof(g), 0.0, 8, 8, 1 << 20, None) \
         == _capi.CL_ERR_INVALID_ARGUMENT and b"rounding" in lib.cl_last_error()
+    assert lib.cl_adamw_moments_read(0, None, None) == _capi.CL_OK and lib.cl_last_error() == b""
 
 
 def test_oracle_holds_its_own_values():
